@@ -56,6 +56,10 @@ extern "C" {
 #define IRIS_ERR_PAGE_ID 0x40          /* page id outside [0, num_pages)     (IndexError) */
 #define IRIS_ERR_PIPELINE_TIMEOUT 0x80 /* a bounded wait gave up             (RuntimeError) */
 
+/* ---- 16-bit element types of the entry points that take either ---------- */
+#define IRIS_DTYPE_FP16 0
+#define IRIS_DTYPE_BF16 1
+
 /* Library version (major*10000 + minor*100 + patch). */
 IRIS_API int iris_b200_version(void);
 
@@ -174,9 +178,69 @@ IRIS_API int iris_b200_rope_fp16_paged_append(const void* key, const void* value
                                               int64_t max_position, int64_t num_pages, int32_t page_size,
                                               int32_t* error_word, void* stream);
 
+/* Most position axes of iris_b200_mrope_int4_paged_append. */
+#define IRIS_MROPE_MAX_AXES 4
+
+/*
+ * Rotary positions with several axes + group-32 symmetric INT4 quantisation +
+ * paged append (the write path of models whose tokens have a position per
+ * axis: time, height, width), and in the same launch the rotated queries and,
+ * if wanted, the rotated keys.  No counterpart in the reference.
+ *
+ *   key, value [num_tokens, num_kv_heads, head_dim], query [num_tokens,
+ *   num_q_heads, head_dim] (NULL with num_q_heads 0), of `dtype`; heads and
+ *   dims contiguous, tokens *_stride elements apart (a multiple of 8)
+ *   positions  int32, axis a's num_tokens positions at positions +
+ *              a * positions_stride
+ *   sections   host array of num_axes counts that add up to rotary_dim / 2:
+ *              the frequencies each axis turns, in runs, or dealt out in turn
+ *              with `interleaved` (axis 0, 1, .., passing over an axis that
+ *              has its count)
+ *   cos_cache, sin_cache [max_position, rotary_dim / 2] of `dtype`
+ *   query_out  [num_tokens, num_q_heads, head_dim], key_out [num_tokens,
+ *              num_kv_heads, head_dim] or NULL: contiguous, of `dtype`
+ * Dims i and i + rotary_dim / 2 turn together, dims from rotary_dim on pass
+ * through.  Rotation in fp32, not rounded before the quantisation; scale =
+ * fp16(min(max(amax / 7, 2^-14), 65504)), q = clamp(rint(y / scale), -7, 7);
+ * a group holding an infinity or NaN keeps that as its scale.
+ * head_dim % 64 == 0 and <= 512, rotary_dim % 16 == 0.
+ *
+ * A token whose slot is negative is padding: nothing of it is read but its
+ * slot, and its rows of query_out / key_out are zeros.  The batch is validated
+ * in this call (slot range, every axis's position range, duplicate slots); a
+ * batch that fails, or that finds such a bit pending in *error_word, writes
+ * nothing at all.  Batches of more than IRIS_APPEND_INLINE_CHECK_TOKENS
+ * tokens need a workspace of iris_b200_append_check_workspace_bytes.
+ */
+IRIS_API int iris_b200_mrope_int4_paged_append(
+    const void* key, int64_t key_stride, const void* value, int64_t value_stride, const void* query,
+    int64_t query_stride, const int32_t* positions, int64_t positions_stride, const int32_t* sections,
+    int32_t num_axes, int32_t interleaved, const int32_t* slot_mapping, const void* cos_cache, const void* sin_cache,
+    void* k_data, void* v_data, void* k_scale, void* v_scale, void* query_out, void* key_out, int64_t num_tokens,
+    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim, int64_t max_position,
+    int64_t num_pages, int32_t page_size, int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* error_word,
+    void* stream);
+
 /* ======================================================================
  * READ PATH
  * ====================================================================== */
+
+/*
+ * The cache read back: sequence b's tokens from first_token[b] (NULL: 0) on,
+ * cu_seqlens[b + 1] - cu_seqlens[b] of them, dequantised (nibble * scale, one
+ * rounding to `dtype`) into rows cu_seqlens[b] .. of key / value [num_tokens,
+ * num_kv_heads, head_dim].  cu_seqlens [batch + 1] int32 rises from 0; rows
+ * from cu_seqlens[batch] on are zeros.  A token without a page (table too
+ * narrow, bad page id) gives zeros and its bit.  Any page_size; head_dim a
+ * multiple of 32 up to 512; key / value 16-byte aligned.  No counterpart in
+ * the reference.
+ */
+IRIS_API int iris_b200_int4_paged_gather(const void* k_data, const void* v_data, const void* k_scale,
+                                         const void* v_scale, const int32_t* block_table, int64_t block_table_stride,
+                                         const int32_t* cu_seqlens, const int32_t* first_token, void* key,
+                                         void* value, int64_t num_tokens, int32_t batch, int32_t num_kv_heads,
+                                         int32_t head_dim, int64_t num_pages, int32_t page_size,
+                                         int32_t max_pages_per_seq, int32_t dtype, int32_t* error_word, void* stream);
 
 /* Output forms of the decode. */
 #define IRIS_DECODE_OUT_FP16 0 /* output [B, Hq, D] fp16 = softmax(QK^T) V (reference form) */
@@ -300,6 +364,80 @@ IRIS_API int iris_b200_merge_lse_partials(const float* parts_o, const float* par
  */
 IRIS_API int iris_b200_merge_lse_packed(const float* parts, int32_t num_parts, int64_t rows, int32_t head_dim,
                                         void* output, void* stream);
+
+/* ======================================================================
+ * SPARSE READ PATH: page bounds, page selection, attention over the selection
+ * ====================================================================== */
+
+/*
+ * Bounds of the stored keys, per physical page and KV head: for every dim the
+ * lowest and the highest key over the page's tokens inside the sequence, as
+ * 8-bit codes of one step, rounded outwards.  No counterpart in the reference.
+ *
+ *   bounds      [num_pages, num_kv_heads, 2, head_dim] int8 (lowest, highest)
+ *   bounds_step [num_pages, num_kv_heads] fp32: max |key| / 127
+ *   values      NULL, or [num_pages, num_kv_heads, 2, head_dim] fp16: what the
+ *               codes stand for, rounded to fp16
+ * Sequence b's pages from the one of token first_token[b] (NULL: 0) to its
+ * last are computed anew from the cache; others keep their bounds.  A page
+ * with a scale that is not finite gets step = inf, codes -127 and 127.
+ * Sequences that share a page have to share its length inside the page.
+ * page_size 16, head_dim 64 or 128; a length of 0 is allowed.
+ */
+IRIS_API int iris_b200_int4_page_bounds(const void* k_data, const void* k_scale, const int32_t* block_table,
+                                        int64_t block_table_stride, const int32_t* seq_lens,
+                                        const int32_t* first_token, void* bounds, float* bounds_step, void* values,
+                                        int32_t batch, int32_t num_kv_heads, int32_t head_dim, int64_t num_pages,
+                                        int32_t page_size, int32_t max_pages_per_seq, int32_t* error_word,
+                                        void* stream);
+
+/* Bytes of device workspace iris_b200_page_select needs. */
+IRIS_API size_t iris_b200_page_select_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t max_pages_per_seq);
+
+/*
+ * Per sequence and KV head, the max_pages pages that score highest, in rising
+ * order: page_list [batch, num_kv_heads, max_pages] int32 (logical pages, -1
+ * behind the last) and page_count [batch, num_kv_heads].  The first sink_pages
+ * and the last recent_pages are always among them (their sum <= max_pages);
+ * ties go to the lowest page; a sequence of at most max_pages pages keeps all.
+ * Score of a page: the maximum over the KV head's query heads of
+ *   ((sum_d max(c_d lo_d, c_d hi_d)) * step) * unit     (fp32 products)
+ * with the bounds' codes lo, hi and step, and the query head's codes
+ * c = clamp(rint(q / unit), -127, 127), unit = max |q| / 127 (a query head that
+ * is zero or not finite: c = 0, unit = 0).  A page whose step is not finite
+ * scores +inf.  No counterpart in the reference.
+ *   query [batch, num_q_heads, head_dim] of `dtype`; num_q_heads / num_kv_heads
+ *   <= 16; page_size 16, head_dim 64 or 128; workspace 16-byte aligned.
+ */
+IRIS_API int iris_b200_page_select(const void* query, const void* bounds, const float* bounds_step,
+                                   const int32_t* block_table, int64_t block_table_stride, const int32_t* seq_lens,
+                                   int32_t* page_list, int32_t* page_count, int32_t batch, int32_t num_q_heads,
+                                   int32_t num_kv_heads, int32_t head_dim, int64_t num_pages, int32_t page_size,
+                                   int32_t max_pages_per_seq, int32_t max_pages, int32_t sink_pages,
+                                   int32_t recent_pages, int32_t dtype, void* workspace, size_t workspace_bytes,
+                                   int32_t* error_word, void* stream);
+
+/*
+ * INT4 paged decode attention over listed pages: query head i of KV head h
+ * attends to the tokens of the first page_count[b, h] logical pages of
+ * page_list[b, h, :max_pages] that lie inside the sequence.  Entries that are
+ * negative or past the sequence's end count for nothing; a page listed twice
+ * counts twice.  No tokens: output 0, lse -inf.  No counterpart in the
+ * reference.
+ *   query, output [batch, num_q_heads, head_dim] of `dtype`; out_lse [batch,
+ *   num_q_heads] fp32 or NULL: log2-sum-exp2 of the scaled logits, as in
+ *   IRIS_DECODE_OUT_LSE.  Limits as iris_b200_int4_paged_decode; seq_lens may
+ *   be 0.
+ */
+IRIS_API int iris_b200_int4_sparse_paged_decode(const void* query, const void* k_data, const void* v_data,
+                                                const void* k_scale, const void* v_scale, const int32_t* block_table,
+                                                int64_t block_table_stride, const int32_t* seq_lens,
+                                                const int32_t* page_list, const int32_t* page_count, void* output,
+                                                float* out_lse, int32_t batch, int32_t num_q_heads,
+                                                int32_t num_kv_heads, int32_t head_dim, int64_t num_pages,
+                                                int32_t page_size, int32_t max_pages_per_seq, int32_t max_pages,
+                                                float softmax_scale, int32_t dtype, int32_t* error_word,
+                                                void* stream);
 
 /* ======================================================================
  * SPLIT-CONTEXT MERGE OVER NVLINK PEER MEMORY

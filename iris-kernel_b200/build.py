@@ -19,7 +19,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 OUT = os.path.join(HERE, "iris_kernel", "libiris_b200.so")
-SOURCES = ["append.cu", "decode.cu", "decode_noalloc.cu", "exchange.cu"]
+SOURCES = ["append.cu", "mrope_append.cu", "gather.cu", "decode.cu", "decode_noalloc.cu", "page_index.cu",
+           "sparse_decode.cu", "exchange.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,0 +1,31 @@
+// The two 16-bit element types of keys, values and queries, behind one
+// interface: pairs packed in a 32-bit word, converted to and from fp32.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace iris {
+
+struct Fp16Elem {
+  IRIS_DEV static float2 unpack(uint32_t w) { return __half22float2(u32_as_h2(w)); }
+  IRIS_DEV static uint32_t pack(float lo, float hi) { return h2_as_u32(__floats2half2_rn(lo, hi)); }
+};
+
+struct Bf16Elem {
+  IRIS_DEV static float2 unpack(uint32_t w) {  // a bf16 is the upper half of its fp32
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  IRIS_DEV static uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+};
+
+// Signed nibble i (0..7) of a packed word.
+IRIS_DEV int nibble(uint32_t w, int i) { return static_cast<int>(w << (28 - 4 * i)) >> 28; }
+
+inline bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+}  // namespace iris

@@ -1,0 +1,155 @@
+// Reading the INT4 paged cache back: the keys and values of every sequence's
+// tokens, dequantised (value = nibble * group scale, one rounding to the
+// output type), as dense rows one sequence after another.
+//
+// A copy: per token and head 1.125 D bytes in and 4 D bytes out.  The heads of
+// a token are contiguous in the cache and in the output, so a token is one
+// row of R = Hkv D dims.  A CTA takes a tile of consecutive output rows, looks
+// each row's sequence and page up once (one thread a row, binary search in
+// the offsets), and then passes over the tile's 8-dim vectors: four packed
+// bytes in, one 16-byte store out, consecutive lanes on consecutive vectors.
+#include "elem.cuh"
+
+namespace iris {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTile = 16;  // output rows per CTA
+
+struct GatherParams {
+  const uint8_t* k_data;
+  const uint8_t* v_data;
+  const __half* k_scale;
+  const __half* v_scale;
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* cu_seqlens;
+  const int32_t* first_token;  // NULL: every sequence from its token 0
+  void* key;
+  void* value;
+  int64_t num_tokens;
+  int64_t num_pages;
+  int32_t batch;
+  int32_t max_pages;
+  int32_t vecs;  // 8-dim vectors per token: Hkv D / 8
+  int32_t page_size;
+  int32_t* err;
+};
+
+// Cache row (page * page_size + offset) of output row n, -1 if it has none.
+IRIS_DEV int64_t row_of(const GatherParams& p, int64_t n) {
+  int lo = 0, hi = p.batch;  // the last sequence whose offset is <= n
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (static_cast<int64_t>(__ldg(p.cu_seqlens + mid)) <= n) lo = mid;
+    else hi = mid;
+  }
+  const int64_t start = __ldg(p.cu_seqlens + lo), end = __ldg(p.cu_seqlens + lo + 1);
+  const int64_t from = p.first_token != nullptr ? __ldg(p.first_token + lo) : 0;
+  const int64_t total = __ldg(p.cu_seqlens + p.batch);
+  if (n >= total) return -1;                                // past the last sequence: zeros
+  if (n < start || n >= end || end > total || from < 0) {  // offsets that do not rise from 0
+    set_error(p.err, IRIS_ERR_SEQ_LEN);
+    return -1;
+  }
+  const int64_t at = from + n - start, col = at / p.page_size;
+  if (col >= p.max_pages) {
+    set_error(p.err, IRIS_ERR_BLOCK_TABLE);
+    return -1;
+  }
+  const int64_t page = __ldg(p.block_table + lo * p.table_stride + col);
+  if (page < 0 || page >= p.num_pages) {
+    set_error(p.err, IRIS_ERR_PAGE_ID);
+    return -1;
+  }
+  return page * p.page_size + at % p.page_size;
+}
+
+template <typename E>
+IRIS_DEV uint4 dequant8(uint32_t w, __half scale) {
+  const float s = __half2float(scale);
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(static_cast<float>(nibble(w, i)), s);
+  return make_uint4(E::pack(x[0], x[1]), E::pack(x[2], x[3]), E::pack(x[4], x[5]), E::pack(x[6], x[7]));
+}
+
+template <typename E>
+__global__ void __launch_bounds__(kThreads) gather_kernel(const GatherParams p) {
+  __shared__ int64_t s_row[kTile];
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kTile;
+  const int rows = static_cast<int>(p.num_tokens - n0 < kTile ? p.num_tokens - n0 : kTile);
+  if (threadIdx.x < rows) s_row[threadIdx.x] = row_of(p, n0 + threadIdx.x);
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * p.vecs; i += kThreads) {
+    const int r = i / p.vecs, v = i - r * p.vecs;
+    const int64_t src = s_row[r], dst = (n0 + r) * p.vecs + v;
+    uint4 k = make_uint4(0, 0, 0, 0), w = k;
+    if (src >= 0) {
+      const int64_t at = src * p.vecs + v;
+      k = dequant8<E>(__ldg(reinterpret_cast<const uint32_t*>(p.k_data) + at), p.k_scale[at >> 2]);
+      w = dequant8<E>(__ldg(reinterpret_cast<const uint32_t*>(p.v_data) + at), p.v_scale[at >> 2]);
+    }
+    static_cast<uint4*>(p.key)[dst] = k;
+    static_cast<uint4*>(p.value)[dst] = w;
+  }
+}
+
+}  // namespace
+}  // namespace iris
+
+using namespace iris;
+
+extern "C" int iris_b200_int4_paged_gather(const void* k_data, const void* v_data, const void* k_scale,
+                                           const void* v_scale, const int32_t* block_table, int64_t block_table_stride,
+                                           const int32_t* cu_seqlens, const int32_t* first_token, void* key,
+                                           void* value, int64_t num_tokens, int32_t batch, int32_t num_kv_heads,
+                                           int32_t head_dim, int64_t num_pages, int32_t page_size,
+                                           int32_t max_pages_per_seq, int32_t dtype, int32_t* error_word,
+                                           void* stream) {
+  if (num_tokens < 0 || batch < 0 || num_kv_heads <= 0 || page_size <= 0 || num_pages < 0 || max_pages_per_seq < 0)
+    return IRIS_EINVAL;
+  if (dtype != IRIS_DTYPE_FP16 && dtype != IRIS_DTYPE_BF16) return IRIS_EINVAL;
+  if (head_dim <= 0 || head_dim % 32 != 0 || head_dim > 512) return IRIS_EUNSUPPORTED;
+  if (num_tokens == 0) return IRIS_OK;
+  if (batch == 0) return IRIS_EINVAL;
+  if (static_cast<int64_t>(num_kv_heads) * head_dim > (1 << 24)) return IRIS_EUNSUPPORTED;
+  if (num_tokens > (static_cast<int64_t>(kTile) << 30)) return IRIS_EUNSUPPORTED;
+  const void* ptrs[] = {k_data, v_data, k_scale, v_scale, block_table, cu_seqlens, key, value};
+  for (const void* q : ptrs)
+    if (q == nullptr) return IRIS_EINVAL;
+  if (!aligned_to(key, 16) || !aligned_to(value, 16) || !aligned_to(k_data, 4) || !aligned_to(v_data, 4) ||
+      !aligned_to(k_scale, 2) || !aligned_to(v_scale, 2))
+    return IRIS_EALIGN;
+  GatherParams p = {};
+  p.k_data = static_cast<const uint8_t*>(k_data);
+  p.v_data = static_cast<const uint8_t*>(v_data);
+  p.k_scale = static_cast<const __half*>(k_scale);
+  p.v_scale = static_cast<const __half*>(v_scale);
+  p.block_table = block_table;
+  p.table_stride = block_table_stride;
+  p.cu_seqlens = cu_seqlens;
+  p.first_token = first_token;
+  p.key = key;
+  p.value = value;
+  p.num_tokens = num_tokens;
+  p.num_pages = num_pages;
+  p.batch = batch;
+  p.max_pages = max_pages_per_seq;
+  p.vecs = num_kv_heads * (head_dim / 8);
+  p.page_size = page_size;
+  p.err = error_word;
+  clear_stale_cuda_error();
+  const unsigned blocks = static_cast<unsigned>((num_tokens + kTile - 1) / kTile);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == IRIS_DTYPE_FP16)
+    gather_kernel<Fp16Elem><<<blocks, kThreads, 0, s>>>(p);
+  else
+    gather_kernel<Bf16Elem><<<blocks, kThreads, 0, s>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) {
+    record_cuda_error(e, "gather_kernel launch");
+    return IRIS_ECUDA;
+  }
+  return IRIS_OK;
+}

@@ -27,6 +27,10 @@ ERR_PIPELINE_TIMEOUT = 0x80
 DECODE_OUT_FP16 = 0
 DECODE_OUT_LSE = 1
 
+DTYPE_FP16 = 0
+DTYPE_BF16 = 1
+MROPE_MAX_AXES = 4  # IRIS_MROPE_MAX_AXES
+
 DECODE_NOALLOC_SCRATCH_BYTES = 32 << 20  # IRIS_DECODE_NOALLOC_SCRATCH_BYTES
 APPEND_INLINE_CHECK_TOKENS = 128  # IRIS_APPEND_INLINE_CHECK_TOKENS
 
@@ -66,6 +70,28 @@ SIGNATURES = {
         ctypes.c_int,
         [_c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32,
          _c_i32, _c_f, _c_p, _c_sz, _c_p, _c_p]),
+    "iris_b200_mrope_int4_paged_append": (
+        ctypes.c_int,
+        [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i32, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_p,
+         _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i64, _c_i32, _c_i32, _c_p, _c_sz,
+         _c_p, _c_p]),
+    "iris_b200_int4_paged_gather": (
+        ctypes.c_int,
+        [_c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32,
+         _c_i32, _c_i32, _c_p, _c_p]),
+    "iris_b200_int4_page_bounds": (
+        ctypes.c_int,
+        [_c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, _c_i32, _c_p,
+         _c_p]),
+    "iris_b200_page_select_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i32]),
+    "iris_b200_page_select": (
+        ctypes.c_int,
+        [_c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, _c_i32,
+         _c_i32, _c_i32, _c_i32, _c_i32, _c_p, _c_sz, _c_p, _c_p]),
+    "iris_b200_int4_sparse_paged_decode": (
+        ctypes.c_int,
+        [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i32,
+         _c_i64, _c_i32, _c_i32, _c_i32, _c_f, _c_i32, _c_p, _c_p]),
     "iris_b200_xchg_buffer_bytes": (_c_sz, [_c_i64, _c_i32]),
     "iris_b200_xchg_alloc": (ctypes.c_int, [_c_sz, ctypes.POINTER(_c_p)]),
     "iris_b200_xchg_free": (ctypes.c_int, [_c_p]),

@@ -117,6 +117,69 @@ def require_sm100(device: torch.device) -> None:
         raise RuntimeError(f"iris_kernel is built for sm_100a (B200); device capability is {cap}")
 
 
+# element type codes of the entry points that take FP16 or BF16
+DTYPES = {torch.float16: _lib.DTYPE_FP16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def dtype_code(name: str, dtype: torch.dtype) -> int:
+    code = DTYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"{name} must use FP16(torch.float16) or BF16(torch.bfloat16)")
+    return code
+
+
+def require_device(name: str, t: torch.Tensor) -> torch.device:
+    """The tensor's device, which has to be a B200."""
+    if not cuda_available():
+        raise RuntimeError("Iris fused kernels require CUDA")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    device = t.device
+    require_sm100(device)
+    return device
+
+
+def check_tensor(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> None:
+    """Shape, type, device and contiguity of one argument."""
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must use {dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def check_block_table(block_table: torch.Tensor, batch: int, device: torch.device) -> None:
+    if block_table.ndim != 2 or block_table.shape[0] != batch:
+        raise ValueError("block_table must have shape [B, max_pages_per_sequence]")
+    if block_table.dtype != torch.int32:
+        raise TypeError("block_table must use torch.int32")
+    if block_table.device != device:
+        raise ValueError(f"block_table must be on {device}")
+    if batch > 0 and block_table.shape[1] == 0:
+        raise ValueError("block_table must have at least one column")
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        raise ValueError("block_table rows must be contiguous")
+
+
+def launch(fn, what: str, device: torch.device, word: torch.Tensor, *args) -> None:
+    """One C call on ``device`` with the error word and its current stream
+    as the last two arguments, and the validation mode applied."""
+    cur = torch.cuda.current_device()
+    other = device.index is not None and device.index != cur
+    if other:
+        torch.cuda.set_device(device.index)
+    try:
+        _lib.check_status(fn(*args, word.data_ptr(), stream_ptr(device)), what)
+    finally:
+        if other:
+            torch.cuda.set_device(cur)
+    if validation_mode() == "sync":
+        raise_for_bits(read_and_clear(word))
+
+
 _scratch: dict = {}
 
 

@@ -5,8 +5,15 @@ Hunter2030ZeRo/Iris-Kernel (src/iris_kernel/fused_kv.py:600-780): same
 signature, tensor layouts and exception types.  The work runs in the sm_100a
 kernel ``iris_b200_rope_int4_paged_append`` (csrc/append.cu) and is
 bit-exact with the reference's eager path (torch_eager_kv.py:110-337).
+
+``fused_mrope_int4_paged_append`` (rotary positions with several axes, queries
+rotated in the same launch) and ``fused_int4_paged_gather`` (the cache read
+back as dense keys and values) have no counterpart in the reference.
 """
 from __future__ import annotations
+
+import ctypes
+import functools
 
 import torch
 
@@ -297,3 +304,225 @@ def fused_rope_fp16_append(
             "iris_b200_rope_fp16_paged_append")
         if _runtime.validation_mode() == "sync":
             _runtime.raise_for_bits(_runtime.read_and_clear(word))
+
+
+@functools.lru_cache(maxsize=256)
+def _sections_array(sections: tuple, rotary_dim: int):
+    """The axes' frequency counts as a C array, checked."""
+    if not 1 <= len(sections) <= _lib.MROPE_MAX_AXES:
+        raise ValueError(f"sections must name 1 to {_lib.MROPE_MAX_AXES} axes")
+    if any(n < 0 for n in sections) or sum(sections) != rotary_dim // 2:
+        raise ValueError(f"sections must be non-negative and add up to rotary_dim // 2 = {rotary_dim // 2}")
+    return (ctypes.c_int32 * len(sections))(*sections)
+
+
+def _token_rows(name, t, shape, dtype, device):
+    """Checks ``[T, H, D]`` rows whose tokens may be apart (a slice of a fused
+    projection) and returns the elements between them."""
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must use {dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+    tokens, heads, dim = shape
+    if tokens == 0:
+        return 0
+    stride = t.stride()
+    if stride[2] != 1 or (heads > 1 and stride[1] != dim) or (tokens > 1 and stride[0] % 8 != 0):
+        raise ValueError(f"{name} must have contiguous heads and dims, and a token stride that is a multiple of 8")
+    if t.data_ptr() % 16 != 0:
+        raise ValueError(f"{name} must start on a 16-byte boundary")
+    return stride[0] if tokens > 1 else 0
+
+
+def fused_mrope_int4_paged_append(
+    key: torch.Tensor,
+    value: torch.Tensor,
+    positions: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    cos_cache: torch.Tensor,
+    sin_cache: torch.Tensor,
+    k_data: torch.Tensor,
+    v_data: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    query: torch.Tensor | None = None,
+    *,
+    sections: tuple,
+    rotary_dim: int,
+    interleaved: bool = False,
+    group_size: int = 32,
+    page_size: int,
+    query_out: torch.Tensor | None = None,
+    key_out: torch.Tensor | None = None,
+) -> torch.Tensor | None:
+    """Rotary positions with several axes, group-32 INT4 quantisation and paged
+    append of ``key / value [T, Hkv, D]`` (FP16 or BF16), in place; returns
+    ``query [T, Hq, D]`` rotated (in ``query_out`` if given), or None.
+
+    ``positions [A, T]`` int32 holds a position per axis; ``sections`` says how
+    many of the ``rotary_dim // 2`` frequencies each axis turns: the first
+    ``sections[0]`` frequencies by axis 0, and so on, or with ``interleaved``
+    dealt out in turn (axis 0, 1, .., 0, 1, .., an axis that has its count
+    being passed over).  ``cos_cache / sin_cache [max_position, rotary_dim //
+    2]`` have the keys' type.  Dims ``i`` and ``i + rotary_dim // 2`` turn
+    together; dims from ``rotary_dim`` on pass through.  Unlike
+    :func:`fused_rope_int4_paged_append`, which rounds to FP16 after every
+    operation as the reference does, the rotation is in FP32 and is not rounded
+    before the quantisation.
+
+    ``key_out [T, Hkv, D]`` receives the rotated keys, as a prefill's own
+    attention needs them.  ``key``, ``value`` and ``query`` may be slices of a
+    fused projection: tokens apart, heads and dims contiguous.  Tokens with
+    ``slot_mapping < 0`` are padding: not stored, their rotated rows zero.  A
+    batch with a bad slot or position writes nothing."""
+    device = _runtime.require_device("key", key)
+    if key.ndim != 3 or value.shape != key.shape:
+        raise ValueError("key and value must have shape [T, Hkv, D]")
+    dtype = key.dtype
+    code = _runtime.dtype_code("key", dtype)
+    num_tokens, num_kv_heads, head_dim = key.shape
+    if head_dim % 64 != 0 or not 64 <= head_dim <= 512:
+        raise NotImplementedError("fused append requires head_dim divisible by 64, up to 512")
+    if group_size != 32:
+        raise NotImplementedError("fused append supports group_size=32")
+    if rotary_dim % 16 != 0 or not 16 <= rotary_dim <= head_dim:
+        raise NotImplementedError("fused append requires rotary_dim divisible by 16, up to head_dim")
+    if num_kv_heads == 0:
+        raise ValueError("key and value must have at least one head")
+    if page_size <= 0:
+        raise ValueError("page_size must be positive")
+    counts = _sections_array(tuple(sections), rotary_dim)
+    axes = len(counts)
+    key_stride = _token_rows("key", key, (num_tokens, num_kv_heads, head_dim), dtype, device)
+    value_stride = _token_rows("value", value, (num_tokens, num_kv_heads, head_dim), dtype, device)
+    if tuple(positions.shape) != (axes, num_tokens):
+        raise ValueError(f"positions must have shape [{axes}, T]")
+    if positions.dtype != torch.int32:
+        raise TypeError("positions must use torch.int32")
+    if positions.device != device:
+        raise ValueError(f"positions must be on {device}")
+    if num_tokens > 1 and positions.stride(1) != 1:
+        raise ValueError("positions of one axis must be contiguous")
+    check = _runtime.check_tensor
+    check("slot_mapping", slot_mapping, (num_tokens,), torch.int32, device)
+    if cos_cache.ndim != 2:
+        raise ValueError("cos_cache must have shape [max_position, rotary_dim // 2]")
+    table = (cos_cache.shape[0], rotary_dim // 2)
+    check("cos_cache", cos_cache, table, dtype, device)
+    check("sin_cache", sin_cache, table, dtype, device)
+    if k_data.ndim != 4:
+        raise ValueError("k_data/v_data must be rank-4 tensors")
+    num_pages = k_data.shape[0]
+    data, scale = (num_pages, page_size, num_kv_heads, head_dim // 2), (num_pages, page_size, num_kv_heads,
+                                                                        head_dim // 32)
+    check("k_data", k_data, data, torch.uint8, device)
+    check("v_data", v_data, data, torch.uint8, device)
+    check("k_scale", k_scale, scale, torch.float16, device)
+    check("v_scale", v_scale, scale, torch.float16, device)
+    num_q_heads = query_stride = 0
+    if query is not None:
+        if query.ndim != 3 or query.shape[1] == 0:
+            raise ValueError("query must have shape [T, Hq, D]")
+        num_q_heads = query.shape[1]
+        query_stride = _token_rows("query", query, (num_tokens, num_q_heads, head_dim), dtype, device)
+        if query_out is None:
+            query_out = torch.empty((num_tokens, num_q_heads, head_dim), dtype=dtype, device=device)
+        else:
+            check("query_out", query_out, (num_tokens, num_q_heads, head_dim), dtype, device)
+    elif query_out is not None:
+        raise ValueError("query_out needs a query")
+    if key_out is not None:
+        check("key_out", key_out, (num_tokens, num_kv_heads, head_dim), dtype, device)
+    if num_tokens == 0:
+        return query_out
+    word = _runtime.error_word(device)
+    ws_ptr, ws_bytes = None, 0
+    if num_tokens > _lib.APPEND_INLINE_CHECK_TOKENS:  # smaller batches are checked without a workspace
+        need = _runtime.workspace_bytes(_lib.lib.iris_b200_append_check_workspace_bytes, num_pages, page_size)
+        ws = _runtime.scratch(device, _runtime.stream_ptr(device), "append_check", max(need, 4))
+        ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
+    _runtime.launch(
+        _lib.lib.iris_b200_mrope_int4_paged_append, "iris_b200_mrope_int4_paged_append", device, word,
+        key.data_ptr(), key_stride, value.data_ptr(), value_stride, None if query is None else query.data_ptr(),
+        query_stride, positions.data_ptr(), positions.stride(0), counts, axes, int(bool(interleaved)),
+        slot_mapping.data_ptr(), cos_cache.data_ptr(), sin_cache.data_ptr(), k_data.data_ptr(), v_data.data_ptr(),
+        k_scale.data_ptr(), v_scale.data_ptr(), None if query_out is None else query_out.data_ptr(),
+        None if key_out is None else key_out.data_ptr(), num_tokens, num_q_heads, num_kv_heads, head_dim, rotary_dim,
+        cos_cache.shape[0], num_pages, page_size, code, ws_ptr, ws_bytes)
+    return query_out
+
+
+def fused_int4_paged_gather(
+    k_data: torch.Tensor,
+    v_data: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    key: torch.Tensor | None = None,
+    value: torch.Tensor | None = None,
+    *,
+    num_tokens: int,
+    first_token: torch.Tensor | None = None,
+    dtype: torch.dtype = torch.float16,
+    page_size: int = 16,
+    group_size: int = 32,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cache read back: ``(key, value) [num_tokens, Hkv, D]`` of ``dtype``
+    (FP16 or BF16), as attention reads them.
+
+    Sequence ``b`` fills rows ``cu_seqlens[b] .. cu_seqlens[b + 1]`` (int32
+    ``[B + 1]``, rising from 0) with its tokens from ``first_token[b]`` on
+    (int32 ``[B]``; None: from its first).  ``num_tokens`` is the host's count
+    of rows, ``cu_seqlens[-1]``; rows past that are zeros.  For another chunk
+    of prefill over a cached context, or to move a cache to another format."""
+    device = _runtime.require_device("k_data", k_data)
+    if group_size != 32:
+        raise NotImplementedError("gather supports group_size=32")
+    if k_data.ndim != 4:
+        raise ValueError("k_data/v_data must be rank-4 tensors")
+    num_pages, cache_page_size, num_kv_heads, packed_dim = k_data.shape
+    head_dim = 2 * packed_dim
+    if cache_page_size != page_size or page_size <= 0 or num_kv_heads == 0:
+        raise ValueError("packed cache shape does not match page_size")
+    if head_dim % 32 != 0 or not 32 <= head_dim <= 512:
+        raise NotImplementedError("gather requires head_dim divisible by 32, up to 512")
+    check = _runtime.check_tensor
+    check("k_data", k_data, tuple(k_data.shape), torch.uint8, device)
+    check("v_data", v_data, tuple(k_data.shape), torch.uint8, device)
+    scale = (num_pages, page_size, num_kv_heads, head_dim // 32)
+    check("k_scale", k_scale, scale, torch.float16, device)
+    check("v_scale", v_scale, scale, torch.float16, device)
+    batch = block_table.shape[0]
+    _runtime.check_block_table(block_table, batch, device)
+    check("cu_seqlens", cu_seqlens, (batch + 1,), torch.int32, device)
+    if first_token is not None:
+        check("first_token", first_token, (batch,), torch.int32, device)
+    if num_tokens < 0:
+        raise ValueError("num_tokens must not be negative")
+    shape = (num_tokens, num_kv_heads, head_dim)
+    code = _runtime.dtype_code("dtype", dtype if key is None else key.dtype)
+    if key is None:
+        key = torch.empty(shape, dtype=dtype, device=device)
+    else:
+        dtype = key.dtype
+        check("key", key, shape, dtype, device)
+    if value is None:
+        value = torch.empty(shape, dtype=dtype, device=device)
+    else:
+        check("value", value, shape, dtype, device)
+    if num_tokens == 0:
+        return key, value
+    if batch == 0:
+        raise ValueError("num_tokens must be 0 without sequences")
+    if num_pages == 0:
+        raise IndexError("block_table contains an invalid physical page id")
+    _runtime.launch(
+        _lib.lib.iris_b200_int4_paged_gather, "iris_b200_int4_paged_gather", device, _runtime.error_word(device),
+        k_data.data_ptr(), v_data.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
+        block_table.stride(0), cu_seqlens.data_ptr(), None if first_token is None else first_token.data_ptr(),
+        key.data_ptr(), value.data_ptr(), num_tokens, batch, num_kv_heads, head_dim, num_pages, page_size,
+        block_table.shape[1], code)
+    return key, value
