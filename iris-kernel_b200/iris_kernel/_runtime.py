@@ -141,41 +141,56 @@ def require_device(name: str, t: torch.Tensor) -> torch.device:
 
 def check_tensor(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> None:
     """Shape, type, device and contiguity of one argument."""
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must have shape {shape}")
+    if t.shape == shape and t.dtype is dtype and t.device == device and t.is_contiguous():
+        return
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must use {dtype}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+    raise ValueError(f"{name} must be contiguous")
 
 
-def check_block_table(block_table: torch.Tensor, batch: int, device: torch.device) -> None:
-    if block_table.ndim != 2 or block_table.shape[0] != batch:
+def check_block_table(block_table: torch.Tensor, batch: int, device: torch.device) -> tuple[int, int]:
+    """Its columns and the elements between its rows (rows may be apart)."""
+    shape = block_table.shape
+    if len(shape) != 2 or shape[0] != batch:
         raise ValueError("block_table must have shape [B, max_pages_per_sequence]")
-    if block_table.dtype != torch.int32:
+    if block_table.dtype is not torch.int32:
         raise TypeError("block_table must use torch.int32")
     if block_table.device != device:
         raise ValueError(f"block_table must be on {device}")
-    if batch > 0 and block_table.shape[1] == 0:
+    width = shape[1]
+    if batch > 0 and width == 0:
         raise ValueError("block_table must have at least one column")
-    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+    stride = block_table.stride()
+    if width > 1 and stride[1] != 1:
         raise ValueError("block_table rows must be contiguous")
+    return width, stride[0]
 
 
-def launch(fn, what: str, device: torch.device, word: torch.Tensor, *args) -> None:
-    """One C call on ``device`` with the error word and its current stream
-    as the last two arguments, and the validation mode applied."""
-    cur = torch.cuda.current_device()
-    other = device.index is not None and device.index != cur
-    if other:
-        torch.cuda.set_device(device.index)
-    try:
-        _lib.check_status(fn(*args, word.data_ptr(), stream_ptr(device)), what)
-    finally:
-        if other:
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def launch(fn, what: str, device: torch.device, *args) -> None:
+    """One C call on ``device``, the error word and its current stream as the
+    last two arguments, with the validation mode applied."""
+    idx = device.index
+    word = _words.get(idx)
+    if word is None:
+        word = error_word(device)
+    cur = _current_device()
+    if cur == idx:
+        status = fn(*args, word.data_ptr(), stream_ptr(device))
+    else:
+        torch.cuda.set_device(idx)
+        try:
+            status = fn(*args, word.data_ptr(), stream_ptr(device))
+        finally:
             torch.cuda.set_device(cur)
+    if status:
+        _lib.check_status(status, what)
     if validation_mode() == "sync":
         raise_for_bits(read_and_clear(word))
 

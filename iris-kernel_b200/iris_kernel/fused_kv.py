@@ -318,22 +318,23 @@ def _sections_array(sections: tuple, rotary_dim: int):
 
 def _token_rows(name, t, shape, dtype, device):
     """Checks ``[T, H, D]`` rows whose tokens may be apart (a slice of a fused
-    projection) and returns the elements between them."""
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must have shape {shape}")
-    if t.dtype != dtype:
+    projection); returns their address and the elements between them."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}")
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must use {dtype}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}")
     tokens, heads, dim = shape
     if tokens == 0:
-        return 0
-    stride = t.stride()
-    if stride[2] != 1 or (heads > 1 and stride[1] != dim) or (tokens > 1 and stride[0] % 8 != 0):
+        return 0, 0
+    apart, head, one = t.stride()
+    if one != 1 or (heads > 1 and head != dim) or (tokens > 1 and apart % 8 != 0):
         raise ValueError(f"{name} must have contiguous heads and dims, and a token stride that is a multiple of 8")
-    if t.data_ptr() % 16 != 0:
+    ptr = t.data_ptr()
+    if ptr % 16 != 0:
         raise ValueError(f"{name} must start on a 16-byte boundary")
-    return stride[0] if tokens > 1 else 0
+    return ptr, apart if tokens > 1 else 0
 
 
 def fused_mrope_int4_paged_append(
@@ -395,9 +396,10 @@ def fused_mrope_int4_paged_append(
         raise ValueError("page_size must be positive")
     counts = _sections_array(tuple(sections), rotary_dim)
     axes = len(counts)
-    key_stride = _token_rows("key", key, (num_tokens, num_kv_heads, head_dim), dtype, device)
-    value_stride = _token_rows("value", value, (num_tokens, num_kv_heads, head_dim), dtype, device)
-    if tuple(positions.shape) != (axes, num_tokens):
+    shape = key.shape
+    key_ptr, key_stride = _token_rows("key", key, shape, dtype, device)
+    value_ptr, value_stride = _token_rows("value", value, shape, dtype, device)
+    if positions.shape != (axes, num_tokens):
         raise ValueError(f"positions must have shape [{axes}, T]")
     if positions.dtype != torch.int32:
         raise TypeError("positions must use torch.int32")
@@ -421,32 +423,31 @@ def fused_mrope_int4_paged_append(
     check("v_data", v_data, data, torch.uint8, device)
     check("k_scale", k_scale, scale, torch.float16, device)
     check("v_scale", v_scale, scale, torch.float16, device)
-    num_q_heads = query_stride = 0
+    query_ptr, num_q_heads, query_stride = None, 0, 0
     if query is not None:
         if query.ndim != 3 or query.shape[1] == 0:
             raise ValueError("query must have shape [T, Hq, D]")
         num_q_heads = query.shape[1]
-        query_stride = _token_rows("query", query, (num_tokens, num_q_heads, head_dim), dtype, device)
+        q_shape = (num_tokens, num_q_heads, head_dim)
+        query_ptr, query_stride = _token_rows("query", query, q_shape, dtype, device)
         if query_out is None:
-            query_out = torch.empty((num_tokens, num_q_heads, head_dim), dtype=dtype, device=device)
+            query_out = query.new_empty(q_shape)
         else:
-            check("query_out", query_out, (num_tokens, num_q_heads, head_dim), dtype, device)
+            check("query_out", query_out, q_shape, dtype, device)
     elif query_out is not None:
         raise ValueError("query_out needs a query")
     if key_out is not None:
-        check("key_out", key_out, (num_tokens, num_kv_heads, head_dim), dtype, device)
+        check("key_out", key_out, shape, dtype, device)
     if num_tokens == 0:
         return query_out
-    word = _runtime.error_word(device)
     ws_ptr, ws_bytes = None, 0
     if num_tokens > _lib.APPEND_INLINE_CHECK_TOKENS:  # smaller batches are checked without a workspace
         need = _runtime.workspace_bytes(_lib.lib.iris_b200_append_check_workspace_bytes, num_pages, page_size)
         ws = _runtime.scratch(device, _runtime.stream_ptr(device), "append_check", max(need, 4))
         ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
     _runtime.launch(
-        _lib.lib.iris_b200_mrope_int4_paged_append, "iris_b200_mrope_int4_paged_append", device, word,
-        key.data_ptr(), key_stride, value.data_ptr(), value_stride, None if query is None else query.data_ptr(),
-        query_stride, positions.data_ptr(), positions.stride(0), counts, axes, int(bool(interleaved)),
+        _lib.lib.iris_b200_mrope_int4_paged_append, "iris_b200_mrope_int4_paged_append", device,
+        key_ptr, key_stride, value_ptr, value_stride, query_ptr, query_stride, positions.data_ptr(), positions.stride(0), counts, axes, int(bool(interleaved)),
         slot_mapping.data_ptr(), cos_cache.data_ptr(), sin_cache.data_ptr(), k_data.data_ptr(), v_data.data_ptr(),
         k_scale.data_ptr(), v_scale.data_ptr(), None if query_out is None else query_out.data_ptr(),
         None if key_out is None else key_out.data_ptr(), num_tokens, num_q_heads, num_kv_heads, head_dim, rotary_dim,
@@ -490,13 +491,14 @@ def fused_int4_paged_gather(
     if head_dim % 32 != 0 or not 32 <= head_dim <= 512:
         raise NotImplementedError("gather requires head_dim divisible by 32, up to 512")
     check = _runtime.check_tensor
-    check("k_data", k_data, tuple(k_data.shape), torch.uint8, device)
-    check("v_data", v_data, tuple(k_data.shape), torch.uint8, device)
+    data = k_data.shape
+    check("k_data", k_data, data, torch.uint8, device)
+    check("v_data", v_data, data, torch.uint8, device)
     scale = (num_pages, page_size, num_kv_heads, head_dim // 32)
     check("k_scale", k_scale, scale, torch.float16, device)
     check("v_scale", v_scale, scale, torch.float16, device)
     batch = block_table.shape[0]
-    _runtime.check_block_table(block_table, batch, device)
+    width, table_stride = _runtime.check_block_table(block_table, batch, device)
     check("cu_seqlens", cu_seqlens, (batch + 1,), torch.int32, device)
     if first_token is not None:
         check("first_token", first_token, (batch,), torch.int32, device)
@@ -504,7 +506,9 @@ def fused_int4_paged_gather(
         raise ValueError("num_tokens must not be negative")
     shape = (num_tokens, num_kv_heads, head_dim)
     code = _runtime.dtype_code("dtype", dtype if key is None else key.dtype)
-    if key is None:
+    if key is None and value is None:
+        key, value = torch.empty((2, *shape), dtype=dtype, device=device).unbind()
+    elif key is None:
         key = torch.empty(shape, dtype=dtype, device=device)
     else:
         dtype = key.dtype
@@ -520,9 +524,9 @@ def fused_int4_paged_gather(
     if num_pages == 0:
         raise IndexError("block_table contains an invalid physical page id")
     _runtime.launch(
-        _lib.lib.iris_b200_int4_paged_gather, "iris_b200_int4_paged_gather", device, _runtime.error_word(device),
+        _lib.lib.iris_b200_int4_paged_gather, "iris_b200_int4_paged_gather", device,
         k_data.data_ptr(), v_data.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
-        block_table.stride(0), cu_seqlens.data_ptr(), None if first_token is None else first_token.data_ptr(),
+        table_stride, cu_seqlens.data_ptr(), None if first_token is None else first_token.data_ptr(),
         key.data_ptr(), value.data_ptr(), num_tokens, batch, num_kv_heads, head_dim, num_pages, page_size,
-        block_table.shape[1], code)
+        width, code)
     return key, value

@@ -86,7 +86,7 @@ def fused_int4_page_bounds(
     if values is not None:
         check("values", values, (num_pages, num_kv_heads, 2, head_dim), torch.float16, device)
     batch = block_table.shape[0]
-    _runtime.check_block_table(block_table, batch, device)
+    width, table_stride = _runtime.check_block_table(block_table, batch, device)
     check("seq_lens", seq_lens, (batch,), torch.int32, device)
     if first_token is not None:
         check("first_token", first_token, (batch,), torch.int32, device)
@@ -95,11 +95,11 @@ def fused_int4_page_bounds(
     if num_pages == 0:
         raise IndexError("block_table contains an invalid physical page id")
     _runtime.launch(
-        _lib.lib.iris_b200_int4_page_bounds, "iris_b200_int4_page_bounds", device, _runtime.error_word(device),
-        k_data.data_ptr(), k_scale.data_ptr(), block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(),
+        _lib.lib.iris_b200_int4_page_bounds, "iris_b200_int4_page_bounds", device,
+        k_data.data_ptr(), k_scale.data_ptr(), block_table.data_ptr(), table_stride, seq_lens.data_ptr(),
         None if first_token is None else first_token.data_ptr(), bounds.data_ptr(), bounds_step.data_ptr(),
         None if values is None else values.data_ptr(), batch, num_kv_heads, head_dim, num_pages, page_size,
-        block_table.shape[1])
+        width)
 
 
 def fused_page_select(
@@ -139,9 +139,9 @@ def fused_page_select(
     if max_pages <= 0 or sink_pages < 0 or recent_pages < 0 or sink_pages + recent_pages > max_pages:
         raise ValueError("max_pages must be positive and hold sink_pages and recent_pages")
     check = _runtime.check_tensor
-    check("bounds", bounds, tuple(bounds.shape), torch.int8, device)
+    check("bounds", bounds, bounds.shape, torch.int8, device)
     check("bounds_step", bounds_step, (num_pages, num_kv_heads), torch.float32, device)
-    _runtime.check_block_table(block_table, batch, device)
+    width, table_stride = _runtime.check_block_table(block_table, batch, device)
     check("seq_lens", seq_lens, (batch,), torch.int32, device)
     if page_list is None:
         page_list = torch.empty((batch, num_kv_heads, max_pages), dtype=torch.int32, device=device)
@@ -155,12 +155,11 @@ def fused_page_select(
         return page_list, page_count
     if num_pages == 0:
         raise IndexError("block_table contains an invalid physical page id")
-    width = block_table.shape[1]
     need = _runtime.workspace_bytes(_lib.lib.iris_b200_page_select_workspace_bytes, batch, num_kv_heads, width)
     ws = _runtime.scratch(device, _runtime.stream_ptr(device), "page_select", need)
     _runtime.launch(
-        _lib.lib.iris_b200_page_select, "iris_b200_page_select", device, _runtime.error_word(device),
-        query.data_ptr(), bounds.data_ptr(), bounds_step.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+        _lib.lib.iris_b200_page_select, "iris_b200_page_select", device,
+        query.data_ptr(), bounds.data_ptr(), bounds_step.data_ptr(), block_table.data_ptr(), table_stride,
         seq_lens.data_ptr(), page_list.data_ptr(), page_count.data_ptr(), batch, num_q_heads, num_kv_heads, head_dim,
         num_pages, page_size, width, max_pages, sink_pages, recent_pages, code, ws.data_ptr(), ws.numel())
     return page_list, page_count
@@ -212,7 +211,7 @@ def fused_int4_sparse_paged_decode_attention(
     check("v_data", v_data, data, torch.uint8, device)
     check("k_scale", k_scale, scale, torch.float16, device)
     check("v_scale", v_scale, scale, torch.float16, device)
-    _runtime.check_block_table(block_table, batch, device)
+    width, table_stride = _runtime.check_block_table(block_table, batch, device)
     check("seq_lens", seq_lens, (batch,), torch.int32, device)
     if page_list.ndim != 3 or page_list.shape[2] == 0:
         raise ValueError("page_list must have shape [B, Hkv, max_pages], max_pages >= 1")
@@ -230,9 +229,9 @@ def fused_int4_sparse_paged_decode_attention(
         factor = head_dim ** -0.5 if softmax_scale is None or softmax_scale == 0.0 else float(softmax_scale)
         _runtime.launch(
             _lib.lib.iris_b200_int4_sparse_paged_decode, "iris_b200_int4_sparse_paged_decode", device,
-            _runtime.error_word(device), query.data_ptr(), k_data.data_ptr(), v_data.data_ptr(), k_scale.data_ptr(),
-            v_scale.data_ptr(), block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(),
+            query.data_ptr(), k_data.data_ptr(), v_data.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), block_table.data_ptr(), table_stride, seq_lens.data_ptr(),
             page_list.data_ptr(), page_count.data_ptr(), output.data_ptr(), None if lse is None else lse.data_ptr(),
-            batch, num_q_heads, num_kv_heads, head_dim, num_pages, page_size, block_table.shape[1], max_pages, factor,
+            batch, num_q_heads, num_kv_heads, head_dim, num_pages, page_size, width, max_pages, factor,
             code)
     return (output, lse) if return_lse else output
