@@ -417,6 +417,10 @@ IRIS_API int iris_b200_page_select(const void* query, const void* bounds, const 
                                    int32_t recent_pages, int32_t dtype, void* workspace, size_t workspace_bytes,
                                    int32_t* error_word, void* stream);
 
+/* Bytes of device workspace iris_b200_int4_sparse_paged_decode needs on a device. */
+IRIS_API size_t iris_b200_sparse_decode_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                                        int32_t head_dim, int32_t max_pages, int32_t device);
+
 /*
  * INT4 paged decode attention over listed pages: query head i of KV head h
  * attends to the tokens of the first page_count[b, h] logical pages of
@@ -427,7 +431,9 @@ IRIS_API int iris_b200_page_select(const void* query, const void* bounds, const 
  *   query, output [batch, num_q_heads, head_dim] of `dtype`; out_lse [batch,
  *   num_q_heads] fp32 or NULL: log2-sum-exp2 of the scaled logits, as in
  *   IRIS_DECODE_OUT_LSE.  Limits as iris_b200_int4_paged_decode; seq_lens may
- *   be 0.
+ *   be 0; batch * num_kv_heads * max_pages below 2^31.  query, k_data, v_data
+ *   and workspace 16-byte aligned, the scales and output 8-byte.  The
+ *   workspace's contents do not matter and belong to one call at a time.
  */
 IRIS_API int iris_b200_int4_sparse_paged_decode(const void* query, const void* k_data, const void* v_data,
                                                 const void* k_scale, const void* v_scale, const int32_t* block_table,
@@ -436,8 +442,8 @@ IRIS_API int iris_b200_int4_sparse_paged_decode(const void* query, const void* k
                                                 float* out_lse, int32_t batch, int32_t num_q_heads,
                                                 int32_t num_kv_heads, int32_t head_dim, int64_t num_pages,
                                                 int32_t page_size, int32_t max_pages_per_seq, int32_t max_pages,
-                                                float softmax_scale, int32_t dtype, int32_t* error_word,
-                                                void* stream);
+                                                float softmax_scale, int32_t dtype, void* workspace,
+                                                size_t workspace_bytes, int32_t* error_word, void* stream);
 
 /* ======================================================================
  * SPLIT-CONTEXT MERGE OVER NVLINK PEER MEMORY

@@ -9,20 +9,39 @@
 //
 // Layout.  The head's share of a page is 16 rows of D/2 packed bytes and D/16
 // scale bytes, for K and V: small strided pieces, so each warp copies its own
-// pages with 16-byte asynchronous copies into a ring of its own (no barrier
-// between warps) and keeps its own running softmax.  Products run on the
-// tensor cores with fp32 accumulation:
-//   S = Q K^T  rows = query heads, columns = tokens; K as the exact integers
-//              in the query's 16-bit type, one accumulator per 32-dim group,
-//              the group scale applied in fp32;
-//   O = P V    rows = query heads, columns = dims; V as the exact integers in
-//              bf16; p * scale is split into two bf16 terms (16 bits, and
-//              fp32's range).  With G <= 8 the second term fills the product's
-//              idle rows 8 .. 15 at no cost; otherwise it takes a second
-//              product.
-// The warps' partial results meet in shared memory, over a cluster of up to 8
-// CTAs where few rows have to fill the GPU, and each CTA writes its share of
-// the outputs.
+// pages with asynchronous copies into a ring of its own (no barrier between
+// warps) and keeps its own running softmax.  The copies ask L2 for 64 bytes at
+// a time: a token's other heads lie next to its own, and were fetched with it.
+//
+// Products run on the tensor cores with fp16 operands and fp32 accumulation:
+//   S = Q K^T      rows = query heads, columns = tokens, one accumulator per
+//                  32-dim group, the group scale applied in fp32.  A nibble n
+//                  enters as the subnormal fp16 (n + 8) 2^-24, one logic
+//                  operation for two; the accumulator starts at -8 sum(q)
+//                  2^-24.  Each query head is scaled by a power of two to a
+//                  largest value in [1, 2) and put back in the logits' scale:
+//                  exact but for elements 2^-14 below its largest.
+//   O^T = V^T P^T  rows = dims, columns = query heads; V as exact integers; a
+//                  weight p is two fp16 terms, p * scale again two: the rounded
+//                  product and, by fused multiply-adds, what it left off (22
+//                  bits, no step finer than 2^-24; scales are at least 2^-14).
+//                  S's accumulator registers are the fragment of P^T as they
+//                  are.
+// A 16-byte chunk of a page's row is one group: ldmatrix hands each lane the
+// eight dims of a token that its place in K's fragment needs, and its
+// transposing form four dims of two tokens, as V's fragment needs them.
+// Work.  A step takes two pages (their products and exponentials are
+// independent; maxima, votes and rescalings are shared).  All steps of all rows
+// (sequence x KV head), one after another, are cut into equal runs, one a warp,
+// by the lists' real lengths: every warp finishes at the same time whatever the
+// batch looks like, and waits for no other.  A row inside one run is written at
+// once; the parts of the others go to the workspace as (o, m, l), and a second
+// kernel joins them in the order of the list.
+#include <map>
+#include <mutex>
+#include <type_traits>
+#include <utility>
+
 #include "elem.cuh"
 
 namespace iris {
@@ -30,7 +49,8 @@ namespace {
 
 constexpr int kPage = 16;
 constexpr int kWarps = 4;
-constexpr int kStages = 4;
+constexpr int kStages = 3;  // steps in flight and in use, per warp
+constexpr int kSlots = 2 * kStages;
 
 struct SparseParams {
   const void* query;
@@ -49,16 +69,22 @@ struct SparseParams {
   int32_t max_pages;
   int32_t kv_heads, group;
   int32_t keep;
+  int32_t rows;       // B * Hkv
+  int32_t min_steps;  // shortest run of a warp
+  int32_t vector_counts;  // counts is 16-byte aligned
+  float* part_o;      // [2 * warps][group][D]
+  float* part_ml;     // [2 * warps][group][2]
+  int32_t* row_start;  // [rows + 1]: number of the row's first step; last, the length of a run
   float scale_log2;
   int32_t* err;
 };
 
 IRIS_DEV void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  asm volatile("cp.async.cg.shared.global.L2::64B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 template <int N>
 IRIS_DEV void cp_async_small(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+  asm volatile("cp.async.ca.shared.global.L2::64B [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
 }
 IRIS_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -66,65 +92,108 @@ IRIS_DEV void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-IRIS_DEV void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-IRIS_DEV void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// D = A B + C for m16n8k16.  (Not volatile: a function of its operands, and the
+// compiler may interleave independent ones.)
+IRIS_DEV void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// The signed nibbles in bits 0-3 and 16-19 of w as two bf16: 0x4300 | n ^ 8 is
-// 128 + (n + 8) (one lop3, as for fp16 in common.cuh), minus 136 exactly.
-IRIS_DEV uint32_t nibbles_bf16(uint32_t w) {
-  const uint32_t biased = lop3<kLutMagic>(w, 0x000f000fu, 0x43084308u);
-  const __nv_bfloat162 v =
-      __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&biased), __floats2bfloat162_rn(136.0f, 136.0f));
-  return *reinterpret_cast<const uint32_t*>(&v);
+// Four 8 x 8 matrices of 16-bit elements (rows of 16 bytes); lane L gives row
+// L % 8 of matrix L / 8.  (With a memory clobber: the copies' waits order them.)
+IRIS_DEV void load_matrices(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+IRIS_DEV void load_matrices_transposed(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
 }
 
-// Eight nibbles of a word as four pairs (0,4) (1,5) (2,6) (3,7) of the type.
-IRIS_DEV void pairs(const Fp16Elem&, uint32_t w, uint32_t (&o)[4]) {
-  o[0] = int4_lo_exact(w);
-  o[1] = int4_hi_exact(w);
-  o[2] = int4_lo_exact(w >> 8);
-  o[3] = int4_hi_exact(w >> 8);
+// Signed nibbles n of w as (n + 8) in place: (w ^ 8) & 15.  Read as fp16, the
+// nibbles in bits 0-3 are (n + 8) 2^-24 and those in bits 4-7 (n + 8) 2^-20.
+constexpr int kLutOffset = 0x48;  // (a ^ c) & b
+IRIS_DEV uint32_t offset_lo(uint32_t w) { return lop3<kLutOffset>(w, 0x000f000fu, 0x00080008u); }
+IRIS_DEV uint32_t offset_hi(uint32_t w) { return lop3<kLutOffset>(w, 0x00f000f0u, 0x00800080u); }
+
+// Steps of a row.
+IRIS_DEV int steps_of(const SparseParams& p, int row) {
+  return (min(max(__ldg(p.counts + row), 0), p.keep) + 1) >> 1;
 }
-IRIS_DEV void pairs(const Bf16Elem&, uint32_t w, uint32_t (&o)[4]) {
+
+// Number of all steps, and the row (with the number of its first step) that
+// holds step `at` if there is one.  The whole warp calls it.
+struct Place {
+  int total, row, start;
+};
+IRIS_DEV int warp_scan(int x) {  // inclusive
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) o[j] = nibbles_bf16(w >> (4 * j));
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
 }
-IRIS_DEV void mma_qk(const Fp16Elem&, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  mma_f16(d, a, b0, b1);
+// run_of(total) gives this warp's first step
+template <typename F>
+IRIS_DEV Place locate(const SparseParams& p, F&& run_of) {
+  const int lane = threadIdx.x & 31;
+  const int per = (p.rows + 127) / 128 * 4;  // consecutive rows a lane, in fours
+  const auto clamped = [&](int c) { return (min(max(c, 0), p.keep) + 1) >> 1; };
+  int sum = 0;
+  for (int i = 0; i < per; i += 16) {  // up to four loads in flight
+    int4 c[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = lane * per + i + 4 * j;
+      c[j] = make_int4(0, 0, 0, 0);
+      if (i + 4 * j < per && r < p.rows) {
+        if (p.vector_counts && r + 3 < p.rows) {
+          c[j] = __ldg(reinterpret_cast<const int4*>(p.counts + r));
+        } else {
+          c[j].x = __ldg(p.counts + r);
+          if (r + 1 < p.rows) c[j].y = __ldg(p.counts + r + 1);
+          if (r + 2 < p.rows) c[j].z = __ldg(p.counts + r + 2);
+          if (r + 3 < p.rows) c[j].w = __ldg(p.counts + r + 3);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum += clamped(c[j].x) + clamped(c[j].y) + clamped(c[j].z) + clamped(c[j].w);
+  }
+  const int upto = warp_scan(sum);
+  Place out;
+  out.total = __shfl_sync(0xffffffffu, upto, 31);
+  out.row = -1;
+  out.start = 0;
+  const int at = run_of(out.total);
+  if (at >= out.total) return out;
+  const int who = __ffs(__ballot_sync(0xffffffffu, upto > at)) - 1;
+  int base = __shfl_sync(0xffffffffu, upto - sum, who);
+  for (int i = 0; i < per; i += 32) {  // the rows of that lane, 32 at a time
+    const int r = who * per + i + lane;
+    const int n = i + lane < per && r < p.rows ? steps_of(p, r) : 0;
+    const int end = base + warp_scan(n);
+    const unsigned past = __ballot_sync(0xffffffffu, end > at);
+    if (past != 0) {
+      const int l = __ffs(past) - 1;
+      out.row = who * per + i + l;
+      out.start = __shfl_sync(0xffffffffu, end - n, l);
+      return out;
+    }
+    base = __shfl_sync(0xffffffffu, end, 31);
+  }
+  return out;  // not reached: the lane's rows hold the step
 }
-IRIS_DEV void mma_qk(const Bf16Elem&, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  mma_bf16(d, a, b0, b1);
-}
-
-IRIS_DEV uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
-  uint32_t out;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
-  return out;
-}
-IRIS_DEV float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-IRIS_DEV void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-IRIS_DEV uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
+IRIS_DEV int run_length(const SparseParams& p, int total, int warps) {
+  return max(p.min_steps, (total + warps - 1) / warps);
 }
 
 template <int D>
@@ -132,10 +201,14 @@ struct SparseCfg {
   static constexpr int kGroups = D / 32;
   static constexpr int kData = kPage * D / 2;        // bytes of a page's head, K or V
   static constexpr int kScale = kPage * kGroups * 2;  // bytes of its scales
-  static constexpr int kStage = 2 * (kData + kScale);
-  static constexpr int kRing = kStages * kStage;  // per warp
+  static constexpr int kStage = 2 * (kData + kScale);  // one page's slot
+  static constexpr int kRing = kSlots * kStage;  // per warp
   static constexpr int kChunks = D / 32;          // 16-byte chunks per row
 };
+
+// Shared memory of a warp: its ring, its row's query fragments, its slots' info.
+template <int D, bool kWide>
+constexpr int kWarpBytes = SparseCfg<D>::kRing + (kWide ? 2 : 1) * SparseCfg<D>::kGroups * 512 + 64;
 
 // Byte offset of 16-byte chunk c of row r: rows 0, 2, 4, .. would start at the
 // same banks, so the chunks of a row are turned by a function of the row.
@@ -145,334 +218,576 @@ IRIS_DEV int chunk_at(int r, int c) {
   else return r * 32 + ((c ^ ((r >> 2) & 1)) << 4);
 }
 
-// Output records: per warp and query head, fp32 [D + 2]: o, m, l.
+// A page's slot of the ring as the warp's lanes see it: its row, and how many
+// tokens from its first one lie inside the sequence (0 or less: none, or no
+// such page).
+struct SlotInfo {
+  int32_t row, left;
+};
+
 template <typename E, int D, bool kWide>
-__global__ void __launch_bounds__(32 * kWarps) sparse_decode_kernel(const SparseParams p, int splits) {
+__global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse_decode_kernel(const SparseParams p) {
   using C = SparseCfg<D>;
-  constexpr int kHeads = kWide ? 16 : 8;
   constexpr int G4 = C::kGroups;
+  constexpr int kH = kWide ? 2 : 1;  // query heads a lane has logits of: g, g + 8
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int row = blockIdx.x / splits;  // sequence * Hkv + head
-  const int split = splits > 1 ? static_cast<int>(cluster_rank()) : 0;
-  const int b = row / p.kv_heads, h = row - b * p.kv_heads;
-  const int len = __ldg(p.seq_lens + b);
-  if (len < 0 && h == 0 && split == 0 && threadIdx.x == 0) set_error(p.err, IRIS_ERR_SEQ_LEN);
-  const int count = min(max(__ldg(p.counts + row), 0), p.keep);
-  const int workers = splits * kWarps, me = split * kWarps + warp;
-  const int mine = count > me ? (count - me + workers - 1) / workers : 0;  // pages me, me + workers, ..
-  const int32_t* list = p.lists + static_cast<int64_t>(row) * p.keep;
+  const int me = blockIdx.x * kWarps + warp, warps = gridDim.x * kWarps;
+  grid_dependents_launch();
+  const Place first = locate(p, [&](int total) {
+    return min(static_cast<int64_t>(me) * run_length(p, total, warps), static_cast<int64_t>(total));
+  });
+  const int length = run_length(p, first.total, warps);
+  if (me == 0 && lane == 0) p.row_start[p.rows] = length;
+  if (first.row < 0) return;  // (nothing below waits for another warp)
+  const int begin = me * length, end = min(begin + length, first.total);  // below 2^30 + the run
 
-  const uint32_t ring = smem_u32(smem) + warp * C::kRing;
-  int32_t* stage_col = reinterpret_cast<int32_t*>(smem + kWarps * C::kRing) + warp * kStages;
-  int32_t my_col = -1;   // this lane's page of the current 32: logical
-  int64_t my_page = -1;  // and physical, -1 where there is none
-  const auto look_up = [&](int at) {
-    my_col = -1;
+  uint8_t* ring = smem + warp * (kWarpBytes<D, kWide>);
+  uint4* s_query = reinterpret_cast<uint4*>(ring + C::kRing);  // [half][group][lane]
+  SlotInfo* info = reinterpret_cast<SlotInfo*>(ring + C::kRing + kH * G4 * 512);
+  const uint32_t ring_addr = smem_u32(ring);
+
+  // ---- copies: pages of 16 steps are looked up at a time, a page a lane ----
+  int32_t my_page = -1;
+  SlotInfo my_info = {0, 0};
+  int my_head = 0;
+  int seek_row = first.row, seek_start = first.start;  // the row of the next step to look up, or an earlier one
+  const auto look_up = [&](int step) {
+    const int u = min(step + (lane >> 1), end - 1);
+    int row = seek_row, start = seek_start, n = steps_of(p, row);
+    while (u >= start + n) {
+      start += n;
+      n = steps_of(p, ++row);
+    }
+    seek_row = __shfl_sync(0xffffffffu, row, 31);
+    seek_start = __shfl_sync(0xffffffffu, start, 31);
+    const int entry = 2 * (u - start) + (lane & 1);
+    const int b = row / p.kv_heads;
+    const int len = __ldg(p.seq_lens + b);
     my_page = -1;
-    if (at >= mine) return;
-    const int col = __ldg(list + me + static_cast<int64_t>(at) * workers);
+    my_info = {row, 0};
+    my_head = row - b * p.kv_heads;
+    if (entry >= min(__ldg(p.counts + row), p.keep)) return;
+    const int col = __ldg(p.lists + static_cast<int64_t>(row) * p.keep + entry);
     if (col < 0 || static_cast<int64_t>(col) * kPage >= len) return;
     if (col >= p.max_pages) {
       set_error(p.err, IRIS_ERR_BLOCK_TABLE);
       return;
     }
-    const int64_t page = __ldg(p.block_table + b * p.table_stride + col);
+    const int32_t page = __ldg(p.block_table + b * p.table_stride + col);
     if (page < 0 || page >= p.num_pages) {
       set_error(p.err, IRIS_ERR_PAGE_ID);
       return;
     }
-    my_col = col;
     my_page = page;
+    my_info.left = len - col * kPage;
   };
-  // starts the copies of the warp's page i, or of nothing where there is none
-  const auto fetch = [&](int i) {
-    if (i < mine) {
-      if ((i & 31) == 0) look_up(i + lane);
-      const int64_t page = __shfl_sync(0xffffffffu, my_page, i & 31);
-      const int32_t col = __shfl_sync(0xffffffffu, my_col, i & 31);
-      if (lane == 0) stage_col[i % kStages] = col;
-      if (page >= 0) {
-        const uint32_t st = ring + (i % kStages) * C::kStage;
-        const int64_t row0 = page * kPage * p.kv_heads + h;
-        const uint8_t* kd = p.k_data + row0 * (D / 2);
-        const uint8_t* vd = p.v_data + row0 * (D / 2);
-        const int64_t step = static_cast<int64_t>(p.kv_heads) * (D / 2);
+  // this lane's chunks of any page: row lane / kChunks (and 8 below it for D = 128), and one row's scales
+  const int r0 = lane / C::kChunks, c0 = lane % C::kChunks;
+  const uint32_t row_bytes = static_cast<uint32_t>(p.kv_heads) * (D / 2);
+  const uint32_t data_off = r0 * row_bytes + 16 * c0;
+  const uint8_t* k_src = p.k_data + data_off;
+  const uint8_t* v_src = p.v_data + data_off;
+  const uint8_t* s_src = reinterpret_cast<const uint8_t*>(lane < 16 ? p.k_scale : p.v_scale) +
+                         static_cast<uint32_t>(lane & 15) * p.kv_heads * (2 * G4);
+  const uint32_t dst0 = chunk_at<D>(r0, c0);
+  const uint32_t s_dst = 2 * C::kData + (lane >> 4) * C::kScale + (lane & 15) * 2 * G4;
+  // starts the copies of a step's two pages, as far as there are any
+  const auto fetch = [&](int step) {
+    if (step < end) {
+      const int at = (step - begin) & 15;
+      if (at == 0) look_up(step);
+      const int slot = 2 * ((step - begin) % kStages);
+      if ((lane >> 1) == at) info[slot + (lane & 1)] = my_info;
 #pragma unroll
-        for (int j = lane; j < kPage * C::kChunks; j += 32) {
-          const int r = j / C::kChunks, c = j % C::kChunks;
-          const int at = chunk_at<D>(r, c);
-          cp_async16(st + at, kd + r * step + 16 * c);
-          cp_async16(st + C::kData + at, vd + r * step + 16 * c);
+      for (int pg = 0; pg < 2; ++pg) {
+        const int32_t page = __shfl_sync(0xffffffffu, my_page, 2 * at + pg);
+        const int32_t head = __shfl_sync(0xffffffffu, my_head, 2 * at + pg);
+        if (page >= 0) {
+          const uint32_t st = ring_addr + (slot + pg) * C::kStage;
+          const uint64_t off = static_cast<uint64_t>(static_cast<uint32_t>(page)) * (kPage * row_bytes) + head * (D / 2);
+          cp_async16(st + dst0, k_src + off);
+          cp_async16(st + C::kData + dst0, v_src + off);
+          if constexpr (D == 128) {
+            cp_async16(st + dst0 + C::kData / 2, k_src + off + 8 * row_bytes);
+            cp_async16(st + C::kData + dst0 + C::kData / 2, v_src + off + 8 * row_bytes);
+          }
+          cp_async_small<2 * G4>(st + s_dst, s_src + (off >> 3));
         }
-        const int r = lane & 15;
-        const __half* sc = (lane < 16 ? p.k_scale : p.v_scale) + (row0 + static_cast<int64_t>(r) * p.kv_heads) * G4;
-        cp_async_small<2 * G4>(st + 2 * C::kData + (lane >> 4) * C::kScale + r * 2 * G4, sc);
       }
     }
     cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch(i);
+  for (int i = 0; i < kStages - 1; ++i) fetch(begin + i);
 
-  // query fragments, in the pair order of the unpacked nibbles
-  uint32_t qa[G4][2][4];
+  // ---- state of the row at hand ----
+  constexpr int kTiles = D / 16;  // of 16 dims; a lane has two dims of each for heads 2 t, 2 t + 1 (+ 8)
+  float o[kH][kTiles][4];
+  float m[kH], l[kH], q_sum[kH][G4], head_scale[kH];
+  int cur = -1, cur_start = first.start;
+
+  // Query fragments.  Of this lane's eight dims of a group, the first product
+  // takes 0, 4, 2, 6 (nibbles in bits 0-3 of a half word), the second 1, 5, 3, 7
+  // (bits 4-7, 16 times as large) times 1/16.
+  const auto start_row = [&](int row) {
+    __syncwarp();  // the last row's fragments have been read
 #pragma unroll
-  for (int k = 0; k < G4; ++k) {
+    for (int half = 0; half < kH; ++half) {
+      m[half] = -INFINITY;
+      l[half] = 0.0f;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      uint4 w = make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < kTiles; ++j) o[half][j][0] = o[half][j][1] = o[half][j][2] = o[half][j][3] = 0.0f;
       const int hq = g + 8 * half;
-      if ((half == 0 || kWide) && hq < p.group)
-        w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.query) +
-                                                 (static_cast<int64_t>(row) * p.group + hq) * D + 32 * k + 8 * t));
-      // words hold dims (0,1) (2,3) (4,5) (6,7) of this lane's eight
-      qa[k][0][half] = prmt(w.x, w.z, 0x5410);      // dims 0, 4
-      qa[k][0][half + 2] = prmt(w.x, w.z, 0x7632);  // dims 1, 5
-      qa[k][1][half] = prmt(w.y, w.w, 0x5410);      // dims 2, 6
-      qa[k][1][half + 2] = prmt(w.y, w.w, 0x7632);  // dims 3, 7
+      uint4 w[G4];
+      float top = 0.0f;
+#pragma unroll
+      for (int k = 0; k < G4; ++k) {
+        w[k] = hq < p.group ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.query) +
+                                                                   (static_cast<int64_t>(row) * p.group + hq) * D +
+                                                                   32 * k + 8 * t))
+                            : make_uint4(0, 0, 0, 0);
+        const uint32_t v[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = E::unpack(v[j]);
+          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+      const float down = __uint_as_float((254u - e) << 23);  // 2^-(e - 127)
+      head_scale[half] = (p.scale_log2 * 16777216.0f) * __uint_as_float(e << 23);
+#pragma unroll
+      for (int k = 0; k < G4; ++k) {
+        const uint32_t v[4] = {w[k].x, w[k].y, w[k].z, w[k].w};  // dims (0,1) (2,3) (4,5) (6,7)
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = E::unpack(v[j]);
+          f[2 * j] = x.x * down;
+          f[2 * j + 1] = x.y * (down * 0.0625f);
+        }
+        const uint32_t a[4] = {Fp16Elem::pack(f[0], f[4]), Fp16Elem::pack(f[2], f[6]), Fp16Elem::pack(f[1], f[5]),
+                               Fp16Elem::pack(f[3], f[7])};
+        s_query[(half * G4 + k) * 32 + lane] = make_uint4(a[0], a[1], a[2], a[3]);
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = Fp16Elem::unpack(a[j]);
+          sum += (j < 2 ? 1.0f : 16.0f) * (x.x + x.y);
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        q_sum[half][k] = sum * -4.76837158203125e-07f;  // -8 2^-24
+      }
     }
-  }
-
-  constexpr int kTiles = D / 8;
-  float o[kTiles][4];
+    // (each lane reads back only what it wrote)
+  };
+  // the row's outputs, or this warp's part of them
+  const auto finish_row = [&]() {
+    const int after = cur_start + steps_of(p, cur);
+    const bool starts = cur_start >= begin, whole = starts && after <= end;
+    const int64_t part = 2 * static_cast<int64_t>(me) + (starts ? 1 : 0);  // the run's first row may have begun earlier
+    if (starts && lane == 0) p.row_start[cur] = cur_start;
 #pragma unroll
-  for (int j = 0; j < kTiles; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-  constexpr int kH = kWide ? 2 : 1;  // query heads a lane: g, g + 8
-  float m[kH], l[kH];
+    for (int hh = 0; hh < kH; ++hh) {
+      l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
+      l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
+      const int hq = g + 8 * hh;
+      const float inv = l[hh] == 0.0f ? 0.0f : __fdiv_rn(1.0f, l[hh]);
+      if (t == 0 && hq < p.group) {
+        if (!whole)
+          *reinterpret_cast<float2*>(p.part_ml + (part * p.group + hq) * 2) = make_float2(m[hh], l[hh]);
+        else if (p.lse != nullptr)
+          p.lse[static_cast<int64_t>(cur) * p.group + hq] = l[hh] == 0.0f ? -INFINITY : m[hh] + log2f(l[hh]);
+      }
 #pragma unroll
-  for (int a = 0; a < kH; ++a) {
-    m[a] = -INFINITY;
-    l[a] = 0.0f;
-  }
-  const uint32_t v_sel = g < 4 ? 0x5410u : 0x7632u;
+      for (int e = 0; e < 2; ++e) {  // columns 2 t and 2 t + 1: the heads of lanes 8 t and 8 t + 4
+        const int head = 2 * t + e + 8 * hh;
+        const float f = __shfl_sync(0xffffffffu, inv, 8 * t + 4 * e);
+        if (head < p.group) {
+#pragma unroll
+          for (int k = 0; k < G4; ++k) {  // this lane's four dims of the group are adjacent
+            const float4 v = make_float4(o[hh][2 * k][e], o[hh][2 * k][2 + e], o[hh][2 * k + 1][e], o[hh][2 * k + 1][2 + e]);
+            const int d = 32 * k + 4 * g;
+            if (whole)
+              *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.output) +
+                                        (static_cast<int64_t>(cur) * p.group + head) * D + d) =
+                  make_uint2(E::pack(v.x * f, v.y * f), E::pack(v.z * f, v.w * f));
+            else
+              *reinterpret_cast<float4*>(p.part_o + (part * p.group + head) * D + d) = v;
+          }
+        }
+      }
+    }
+  };
 
-  for (int i = 0; i < mine; ++i) {
-    __syncwarp();  // every lane is done with the stage that is filled next
-    fetch(i + kStages - 1);
+  // this lane's row of the four 8 x 16-byte matrices (tokens 0-7 and 8-15) x (groups 0 and 1)
+  const uint32_t mat = chunk_at<D>((lane & 7) + (lane & 8), (lane >> 4) & 1);
+  // words of the scales of this lane's token pairs (2 t, 2 t + 1) and (2 t + 8, 2 t + 9), adjacent in
+  // memory: token 2 t's groups two a word, then the next token's
+  const auto scale_words = [&](const uint8_t* at, uint32_t (&w)[2][G4]) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      if constexpr (G4 == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(at + (2 * t + 8 * n) * 8);
+        w[n][0] = v.x, w[n][1] = v.y, w[n][2] = v.z, w[n][3] = v.w;
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(at + (2 * t + 8 * n) * 4);
+        w[n][0] = v.x, w[n][1] = v.y;
+      }
+    }
+  };
+  // group k's scales of the two tokens
+  const auto scale_pair = [&](const uint32_t (&w)[G4], int k) {
+    const float2 a = __half22float2(u32_as_h2(w[k / 2])), c = __half22float2(u32_as_h2(w[(G4 + k) / 2]));
+    return k % 2 == 0 ? make_float2(a.x, c.x) : make_float2(a.y, c.y);
+  };
+
+  for (int step = begin; step < end; ++step) {
+    __syncwarp();  // every lane is done with the slots that are filled next
+    fetch(step + kStages - 1);
     cp_async_wait<kStages - 1>();
     __syncwarp();
-    const int col = stage_col[i % kStages];
-    if (col < 0) continue;
-    const uint32_t st = ring + (i % kStages) * C::kStage;
+    const int slot = 2 * ((step - begin) % kStages);
+    const SlotInfo i0 = info[slot], i1 = info[slot + 1];
+    if (i0.row != cur) {
+      if (cur >= 0) {
+        finish_row();
+        cur_start = step;  // (rows without steps lie between, if any)
+      }
+      cur = i0.row;
+      start_row(cur);
+    }
+    const int left[2] = {i0.left, i1.left};
+    if (max(left[0], left[1]) <= 0) continue;
+    const uint8_t* st = ring + slot * C::kStage;
+    const uint32_t st_addr = ring_addr + slot * C::kStage;
 
-    // scales of this lane's tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-    float ks[4][G4], vs[4][G4];
+    // S = Q K^T, one accumulator per group, scaled in fp32 (2^-24 and the query's power of two left out)
+    float2 x[kH][2][2];  // [head][page][token pair]
+    {
+      uint32_t ks[2][2][G4];
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const int tok = 2 * t + (a & 1) + 8 * (a >> 1);
-      const uint32_t at = st + 2 * C::kData + tok * 2 * G4;
+      for (int pg = 0; pg < 2; ++pg) scale_words(st + pg * C::kStage + 2 * C::kData, ks[pg]);
 #pragma unroll
-      for (int k = 0; k < G4; k += 2) {
-        const float2 x = __half22float2(u32_as_h2(lds32(at + 2 * k)));
-        const float2 y = __half22float2(u32_as_h2(lds32(at + C::kScale + 2 * k)));
-        ks[a][k] = x.x, ks[a][k + 1] = x.y;
-        vs[a][k] = y.x, vs[a][k + 1] = y.y;
+      for (int k0 = 0; k0 < G4; k0 += 2) {
+        uint32_t kw[2][4];  // [page][group k0, tokens 0-7 | 8-15, group k0 + 1, ..]
+#pragma unroll
+        for (int pg = 0; pg < 2; ++pg) load_matrices(kw[pg], st_addr + pg * C::kStage + (mat ^ (16 * k0)));
+#pragma unroll
+        for (int k = k0; k < k0 + 2; ++k) {
+          const uint4 q0 = s_query[k * 32 + lane], q1 = kWide ? s_query[(G4 + k) * 32 + lane] : make_uint4(0, 0, 0, 0);
+          const uint32_t a0[4] = {q0.x, q1.x, q0.y, q1.y}, a1[4] = {q0.z, q1.z, q0.w, q1.w};
+          const float init[4] = {q_sum[0][k], q_sum[0][k], kWide ? q_sum[kH - 1][k] : 0.0f,
+                                 kWide ? q_sum[kH - 1][k] : 0.0f};
+#pragma unroll
+          for (int pg = 0; pg < 2; ++pg) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const uint32_t w = kw[pg][2 * (k - k0) + n], v = w >> 8;
+              float acc[4];
+              mma_f16(acc, a0, offset_lo(w), offset_lo(v), init);
+              mma_f16(acc, a1, offset_hi(w), offset_hi(v), acc);
+              const float2 sc = scale_pair(ks[pg][n], k);
+#pragma unroll
+              for (int hh = 0; hh < kH; ++hh) {
+                const float2 a = make_float2(acc[2 * hh], acc[2 * hh + 1]);
+                x[hh][pg][n] = k == 0 ? __fmul2_rn(a, sc) : __ffma2_rn(a, sc, x[hh][pg][n]);
+              }
+            }
+          }
+        }
       }
     }
+    uint32_t vs[2][2][G4];
+#pragma unroll
+    for (int pg = 0; pg < 2; ++pg) scale_words(st + pg * C::kStage + 2 * C::kData + C::kScale, vs[pg]);
 
-    // S = Q K^T, one accumulator per group, scaled in fp32
-    float x[kH][4];  // [head][token]
+    // tokens past the sequence's end count for nothing, whatever their bytes hold
+    if (min(left[0], left[1]) < kPage) {
 #pragma unroll
-    for (int a = 0; a < kH; ++a) x[a][0] = x[a][1] = x[a][2] = x[a][3] = 0.0f;
+      for (int pg = 0; pg < 2; ++pg) {
 #pragma unroll
-    for (int k = 0; k < G4; ++k) {
+        for (int n = 0; n < 2; ++n) {
+          const bool out0 = 2 * t + 8 * n >= left[pg], out1 = 2 * t + 8 * n + 1 >= left[pg];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        uint32_t kw[4];
-        pairs(E{}, lds32(st + chunk_at<D>(8 * n + g, k) + 4 * t), kw);
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        mma_qk(E{}, acc, qa[k][0], kw[0], kw[1]);
-        mma_qk(E{}, acc, qa[k][1], kw[2], kw[3]);
-        x[0][2 * n] = fmaf(acc[0], ks[2 * n][k], x[0][2 * n]);
-        x[0][2 * n + 1] = fmaf(acc[1], ks[2 * n + 1][k], x[0][2 * n + 1]);
-        if constexpr (kWide) {
-          x[kH - 1][2 * n] = fmaf(acc[2], ks[2 * n][k], x[kH - 1][2 * n]);
-          x[kH - 1][2 * n + 1] = fmaf(acc[3], ks[2 * n + 1][k], x[kH - 1][2 * n + 1]);
+          for (int hh = 0; hh < kH; ++hh) {
+            if (out0) x[hh][pg][n].x = -INFINITY;
+            if (out1) x[hh][pg][n].y = -INFINITY;
+          }
+#pragma unroll
+          for (int k = 0; k < G4 / 2; ++k) {
+            if (out0) vs[pg][n][k] = 0u;
+            if (out1) vs[pg][n][k + G4 / 2] = 0u;
+          }
         }
       }
     }
 
-    // running softmax; tokens past the sequence's end count for nothing, whatever their bytes hold
-    const int left = len - col * kPage;  // > 0
-    if (left < kPage) {
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        if (2 * t + (a & 1) + 8 * (a >> 1) >= left) {
-#pragma unroll
-          for (int hh = 0; hh < kH; ++hh) x[hh][a] = -INFINITY;
-#pragma unroll
-          for (int k = 0; k < G4; ++k) vs[a][k] = 0.0f;
-        }
-      }
-    }
+    // running softmax
     float alpha[kH];
     bool moved = false;
 #pragma unroll
     for (int hh = 0; hh < kH; ++hh) {
-#pragma unroll
-      for (int a = 0; a < 4; ++a) x[hh][a] *= p.scale_log2;
-      float top = fmaxf(fmaxf(x[hh][0], x[hh][1]), fmaxf(x[hh][2], x[hh][3]));
+      float top = fmaxf(fmaxf(fmaxf(x[hh][0][0].x, x[hh][0][0].y), fmaxf(x[hh][0][1].x, x[hh][0][1].y)),
+                        fmaxf(fmaxf(x[hh][1][0].x, x[hh][1][0].y), fmaxf(x[hh][1][1].x, x[hh][1][1].y)));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      top = fmaxf(top, m[hh]);
+      top = fmaxf(top * head_scale[hh], m[hh]);
       const float base = top == -INFINITY ? 0.0f : top;
       alpha[hh] = ex2(m[hh] - base);
       moved |= top != m[hh];
       m[hh] = top;
-      float sum = 0.0f;
+      const float2 base2 = make_float2(-base, -base), scale2 = make_float2(head_scale[hh], head_scale[hh]);
+      float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        x[hh][a] = ex2(x[hh][a] - base);
-        sum += x[hh][a];
+      for (int pg = 0; pg < 2; ++pg) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float2 y = __ffma2_rn(x[hh][pg][n], scale2, base2);
+          x[hh][pg][n] = make_float2(ex2(y.x), ex2(y.y));
+          sum = __fadd2_rn(sum, x[hh][pg][n]);
+        }
       }
-      l[hh] = fmaf(l[hh], alpha[hh], sum);
+      l[hh] = fmaf(l[hh], alpha[hh], sum.x + sum.y);
     }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-      for (int j = 0; j < kTiles; ++j) {
-        o[j][0] *= alpha[0];
-        o[j][1] *= alpha[0];
-        o[j][2] *= alpha[kH - 1];
-        o[j][3] *= alpha[kH - 1];
+      for (int hh = 0; hh < kH; ++hh) {  // columns 2 t and 2 t + 1 are the heads of lanes 8 t and 8 t + 4
+        const float2 f = make_float2(__shfl_sync(0xffffffffu, alpha[hh], 8 * t),
+                                     __shfl_sync(0xffffffffu, alpha[hh], 8 * t + 4));
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const float2 v = __fmul2_rn(make_float2(o[hh][j][e], o[hh][j][e + 1]), f);
+            o[hh][j][e] = v.x;
+            o[hh][j][e + 1] = v.y;
+          }
+        }
       }
     }
 
-    // O += P V
+    // O^T += V^T P^T
 #pragma unroll
-    for (int k = 0; k < G4; ++k) {
-      uint32_t hi[4], lo[4];  // A registers: (head g | g + 8) x (tokens 2 t, 2 t + 1 | 2 t + 8, 2 t + 9)
+    for (int pg = 0; pg < 2; ++pg) {
+      __half2 ph[kH][2], pl[kH][2];  // weights of the token pairs: rounded, and the rest
 #pragma unroll
       for (int hh = 0; hh < kH; ++hh) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const float u = x[hh][2 * n] * vs[2 * n][k], v = x[hh][2 * n + 1] * vs[2 * n + 1][k];
-          const uint32_t w = Bf16Elem::pack(u, v);
-          const float2 r = Bf16Elem::unpack(w);
-          hi[2 * n + hh] = w;
-          lo[2 * n + hh] = Bf16Elem::pack(u - r.x, v - r.y);
+          ph[hh][n] = __floats2half2_rn(x[hh][pg][n].x, x[hh][pg][n].y);
+          const float2 r = __half22float2(ph[hh][n]);
+          pl[hh][n] = __floats2half2_rn(x[hh][pg][n].x - r.x, x[hh][pg][n].y - r.y);
         }
       }
-      if constexpr (!kWide) {  // the second terms are rows 8 .. 15
-        hi[1] = lo[0];
-        hi[3] = lo[2];
-      }
-      uint32_t w[4];
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
-        w[a] = lds32(st + C::kData + chunk_at<D>(2 * t + (a & 1) + 8 * (a >> 1), k) + 4 * (g & 3));
-      const uint32_t v0 = prmt(w[0], w[1], v_sel), v1 = prmt(w[2], w[3], v_sel);
+      for (int k0 = 0; k0 < G4; k0 += 2) {
+        uint32_t vw[4];  // group k0: tokens (2 t, 2 t + 1), (2 t + 8, 2 t + 9), group k0 + 1: ..
+        load_matrices_transposed(vw, st_addr + pg * C::kStage + C::kData + (mat ^ (16 * k0)));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t b0 = nibbles_bf16(v0 >> (4 * j)), b1 = nibbles_bf16(v1 >> (4 * j));
-        mma_bf16(o[4 * k + j], hi, b0, b1);
-        if constexpr (kWide) mma_bf16(o[4 * k + j], lo, b0, b1);
+        for (int k = k0; k < k0 + 2; ++k) {
+          uint32_t hi[kH][2], lo[kH][2];  // P^T: head g (and g + 8), token pairs
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            // the group's scales of the pair
+            const __half2 sc = u32_as_h2(prmt(vs[pg][n][k / 2], vs[pg][n][(G4 + k) / 2], k % 2 == 0 ? 0x5410 : 0x7632));
+#pragma unroll
+            for (int hh = 0; hh < kH; ++hh) {
+              const __half2 a = __hmul2_rn(ph[hh][n], sc);
+              const __half2 c = __hfma2(pl[hh][n], sc, __hfma2(ph[hh][n], sc, __hneg2(a)));
+              hi[hh][n] = h2_as_u32(a);
+              lo[hh][n] = h2_as_u32(c);
+            }
+          }
+          const uint32_t v0 = vw[2 * (k - k0)], v1 = vw[2 * (k - k0) + 1];
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) {  // rows g and g + 8 of the tile: dims 4 g + 2 jj and 4 g + 2 jj + 1
+            const uint32_t a[4] = {int4_lo_exact(v0 >> (8 * jj)), int4_hi_exact(v0 >> (8 * jj)),
+                                   int4_lo_exact(v1 >> (8 * jj)), int4_hi_exact(v1 >> (8 * jj))};
+#pragma unroll
+            for (int hh = 0; hh < kH; ++hh) {
+              float(&acc)[4] = o[hh][2 * k + jj];
+              mma_f16(acc, a, hi[hh][0], hi[hh][1], acc);
+              mma_f16(acc, a, lo[hh][0], lo[hh][1], acc);
+            }
+          }
+        }
       }
     }
   }
 
-  // ---- join the warps' partial results ----
-  cp_async_wait<0>();
-  __syncthreads();  // the rings are free: [warp][head][D] outputs, then [warp][head] (m, l)
-  float* part_o = reinterpret_cast<float*>(smem);
-  float* part_ml = part_o + kWarps * kHeads * D;
+  finish_row();
+}
+
+// Joins the parts of the rows that no single warp had, one warp per query head;
+// rows without a step are written here too.
+template <typename E, int D>
+__global__ void __launch_bounds__(128) sparse_join_kernel(const SparseParams p) {
+  constexpr int kPer = D / 32;   // dims a lane
+  constexpr int kAhead = 8;      // parts loaded at a time
+  using Vec = std::conditional_t<kPer == 4, float4, float2>;
+  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5);
+  const int n = steps_of(p, row);
+  if (head == 0 && lane == 0 && __ldg(p.seq_lens + row / p.kv_heads) < 0) set_error(p.err, IRIS_ERR_SEQ_LEN);
+  grid_dependency_wait();
+  if (head >= p.group) return;
+  const int64_t out = static_cast<int64_t>(row) * p.group + head;
+  float acc[kPer];
 #pragma unroll
-  for (int hh = 0; hh < kH; ++hh) {
-    l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
-    l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
-    const int head = warp * kHeads + g + 8 * hh;
+  for (int j = 0; j < kPer; ++j) acc[j] = 0.0f;
+  float top = -INFINITY, sum = 0.0f;
+  if (n > 0) {
+    const int start = __ldcg(p.row_start + row), length = __ldcg(p.row_start + p.rows);
+    const int first = start / length, parts = (start + n - 1) / length - first + 1;
+    if (parts == 1) return;  // its warp wrote the outputs
+    const auto part_at = [&](int i) {
+      return (2 * static_cast<int64_t>(first + i) + (i == 0 ? 1 : 0)) * p.group + head;
+    };
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      float2 ml = make_float2(-INFINITY, 0.0f);
+      if (i0 + lane < parts) ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + part_at(i0 + lane));
+      const int here = min(32, parts - i0);
+      float w = 0.0f;
+      for (int i = 0; i < here; i += kAhead) {
+        Vec v[kAhead];
 #pragma unroll
-    for (int k = 0; k < G4; ++k) {
+        for (int j = 0; j < kAhead; ++j)
+          if (i + j < here)
+            v[j] = __ldcg(reinterpret_cast<const Vec*>(p.part_o + part_at(i0 + i + j) * D) + lane);
+        if (i == 0) {  // the weights of these up to 32 parts, while the first parts are on their way
+          float m = ml.x;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {  // column 2 t + e of the tiles: dims 32 k + at .. at + 3
-        const int n = 2 * t + e;
-        float4 v;
-        float* f = reinterpret_cast<float*>(&v);
+          for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+          m = fmaxf(m, top);
+          const float base = m == -INFINITY ? 0.0f : m, old = ex2(top - base);
+          top = m;
+          w = ex2(ml.x - base);
+          sum = fmaf(sum, old, w * ml.y);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = kWide ? o[4 * k + j][2 * hh + e] : o[4 * k + j][e] + o[4 * k + j][2 + e];
-        *reinterpret_cast<float4*>(part_o + head * D + 32 * k + 8 * (n & 3) + 4 * (n >> 2)) = v;
+          for (int j = 0; j < kPer; ++j) acc[j] *= old;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const float f = __shfl_sync(0xffffffffu, w, i + j);
+          if (i + j < here) {
+            const float* x = reinterpret_cast<const float*>(&v[j]);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) acc[e] = fmaf(f, x[e], acc[e]);
+          }
+        }
       }
     }
-    if (t == 0) {
-      part_ml[2 * head] = m[hh];
-      part_ml[2 * head + 1] = l[hh];
-    }
-  }
-  if (splits > 1) cluster_barrier();
-  else __syncthreads();
-  float* weight = reinterpret_cast<float*>(smem + kWarps * (C::kRing + kStages * 4));  // [head][record]
-  const uint32_t o_addr = smem_u32(part_o), ml_addr = smem_u32(part_ml);
-  const int records = splits * kWarps;  // at most 32
-  for (int head = warp; head < p.group; head += kWarps) {
-    float mr = -INFINITY, lr = 0.0f;
-    if (lane < records) {
-      const uint32_t at = map_to_rank(ml_addr, lane / kWarps) + 8 * ((lane % kWarps) * kHeads + head);
-      mr = ld_cluster(at);
-      lr = ld_cluster(at + 4);
-    }
-    float top = mr;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    const float w = ex2(mr - (top == -INFINITY ? 0.0f : top));
-    float sum = w * lr;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    weight[head * 32 + lane] = sum == 0.0f ? 0.0f : __fdiv_rn(w, sum);
-    if (lane == 0 && split == 0 && p.lse != nullptr)
-      p.lse[static_cast<int64_t>(row) * p.group + head] = sum == 0.0f ? -INFINITY : top + log2f(sum);
   }
-  __syncthreads();
-  uint32_t* out = static_cast<uint32_t*>(p.output) + static_cast<int64_t>(row) * p.group * (D / 2);
-  for (int i = split * 32 * kWarps + threadIdx.x; i < p.group * (D / 2); i += splits * 32 * kWarps) {
-    const int head = i / (D / 2), d = i % (D / 2) * 2;
-    float a = 0.0f, c = 0.0f;
-    for (int r = 0; r < records; ++r) {
-      const float w = weight[head * 32 + r];
-      const uint32_t at = map_to_rank(o_addr, r / kWarps) + 4 * (((r % kWarps) * kHeads + head) * D + d);
-      a = fmaf(w, ld_cluster(at), a);
-      c = fmaf(w, ld_cluster(at + 4), c);
-    }
-    out[i] = E::pack(a, c);
-  }
-  if (splits > 1) cluster_barrier();  // nobody leaves while its memory is read
+  const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+  uint32_t* dst = static_cast<uint32_t*>(p.output) + out * (D / 2) + lane * (kPer / 2);
+#pragma unroll
+  for (int j = 0; j < kPer / 2; ++j) dst[j] = E::pack(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+  if (lane == 0 && p.lse != nullptr) p.lse[out] = sum == 0.0f ? -INFINITY : top + log2f(sum);
 }
 
-template <typename E, int D, bool kWide>
-cudaError_t launch(const SparseParams& p, int64_t rows, int splits, cudaStream_t s) {
-  const int bytes = kWarps * (SparseCfg<D>::kRing + kStages * 4) + 16 * 32 * 4;
-  const auto fn = sparse_decode_kernel<E, D, kWide>;
-  if (bytes > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+// Warps that one launch of the kernel keeps on the current GPU (asked once per kernel and GPU).
+cudaError_t resident_warps(const void* fn, int bytes, int* out) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, int> known;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  const auto key = std::make_pair(fn, device);
+  auto it = known.find(key);
+  if (it == known.end()) {
+    int sms = 0, per_sm = 0;
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, 32 * kWarps, bytes);
     if (e != cudaSuccess) return e;
+    it = known.emplace(key, sms * (per_sm > 0 ? per_sm : 1) * kWarps).first;
   }
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows * splits));
-  cfg.blockDim = dim3(32 * kWarps);
-  cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = splits > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, fn, p, splits);
+  *out = it->second;
+  return cudaSuccess;
 }
 
-template <typename E>
-cudaError_t launch_any(const SparseParams& p, int head_dim, int64_t rows, int splits, cudaStream_t s) {
-  const bool wide = p.group > 8;
-  if (head_dim == 128)
-    return wide ? launch<E, 128, true>(p, rows, splits, s) : launch<E, 128, false>(p, rows, splits, s);
-  return wide ? launch<E, 64, true>(p, rows, splits, s) : launch<E, 64, false>(p, rows, splits, s);
+struct Kernel {
+  const void* fn;
+  const void* join;
+  int bytes;  // of shared memory
+};
+template <typename E, int D, bool kWide>
+Kernel kernel() {
+  return {reinterpret_cast<const void*>(sparse_decode_kernel<E, D, kWide>),
+          reinterpret_cast<const void*>(sparse_join_kernel<E, D>), kWarps * kWarpBytes<D, kWide>};
 }
+Kernel kernel_for(int dtype, int head_dim, bool wide) {
+  if (dtype == IRIS_DTYPE_FP16) {
+    if (head_dim == 128) return wide ? kernel<Fp16Elem, 128, true>() : kernel<Fp16Elem, 128, false>();
+    return wide ? kernel<Fp16Elem, 64, true>() : kernel<Fp16Elem, 64, false>();
+  }
+  if (head_dim == 128) return wide ? kernel<Bf16Elem, 128, true>() : kernel<Bf16Elem, 128, false>();
+  return wide ? kernel<Bf16Elem, 64, true>() : kernel<Bf16Elem, 64, false>();
+}
+
+struct SparseGrid {
+  int ctas;
+  size_t part_o, part_ml, bytes;  // offsets of the workspace's parts after row_start, and its size
+};
+cudaError_t grid_for(const Kernel& k, int64_t rows, int group, int head_dim, int64_t max_pages, int min_steps,
+                     SparseGrid* out) {
+  int resident = 0;
+  const cudaError_t e = resident_warps(k.fn, k.bytes, &resident);
+  if (e != cudaSuccess) return e;
+  const int64_t runs = (rows * ((max_pages + 1) / 2) + min_steps - 1) / min_steps;  // at most
+  const int64_t warps = runs < resident ? runs : resident;
+  out->ctas = static_cast<int>((warps + kWarps - 1) / kWarps);
+  const size_t parts = 2 * static_cast<size_t>(out->ctas) * kWarps * group;
+  out->part_o = (static_cast<size_t>(rows + 1) * 4 + 255) / 256 * 256;
+  out->part_ml = out->part_o + parts * head_dim * 4;
+  out->bytes = out->part_ml + parts * 8;
+  return cudaSuccess;
+}
+
+// Shortest run of a warp, in steps.
+constexpr int kMinSteps = 2;
 
 }  // namespace
 }  // namespace iris
 
 using namespace iris;
+
+static bool sparse_shape_ok(int32_t batch, int32_t hq, int32_t hkv, int32_t head_dim, int32_t max_pages) {
+  return batch > 0 && hq > 0 && hkv > 0 && max_pages > 0 && hq % hkv == 0 && hq / hkv <= 16 &&
+         (head_dim == 64 || head_dim == 128) && hkv <= (1 << 20) &&
+         static_cast<int64_t>(batch) * hkv * ((static_cast<int64_t>(max_pages) + 1) / 2) < (1ll << 30);
+}
+
+extern "C" size_t iris_b200_sparse_decode_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                                          int32_t head_dim, int32_t max_pages, int32_t device) {
+  if (!sparse_shape_ok(batch, num_q_heads, num_kv_heads, head_dim, max_pages)) return 0;
+  int before = 0;
+  if (cudaGetDevice(&before) != cudaSuccess) return 0;
+  if (before != device && cudaSetDevice(device) != cudaSuccess) return 0;
+  const int group = num_q_heads / num_kv_heads;
+  size_t bytes = 0;
+  for (const int dtype : {IRIS_DTYPE_FP16, IRIS_DTYPE_BF16}) {
+    SparseGrid grid;
+    if (grid_for(kernel_for(dtype, head_dim, group > 8), static_cast<int64_t>(batch) * num_kv_heads, group, head_dim,
+                 max_pages, kMinSteps, &grid) != cudaSuccess) {
+      bytes = 0;
+      break;
+    }
+    if (grid.bytes > bytes) bytes = grid.bytes;
+  }
+  if (before != device) cudaSetDevice(before);
+  return bytes;
+}
 
 extern "C" int iris_b200_int4_sparse_paged_decode(const void* query, const void* k_data, const void* v_data,
                                                   const void* k_scale, const void* v_scale, const int32_t* block_table,
@@ -481,24 +796,33 @@ extern "C" int iris_b200_int4_sparse_paged_decode(const void* query, const void*
                                                   float* out_lse, int32_t batch, int32_t num_q_heads,
                                                   int32_t num_kv_heads, int32_t head_dim, int64_t num_pages,
                                                   int32_t page_size, int32_t max_pages_per_seq, int32_t max_pages,
-                                                  float softmax_scale, int32_t dtype, int32_t* error_word,
-                                                  void* stream) {
+                                                  float softmax_scale, int32_t dtype, void* workspace,
+                                                  size_t workspace_bytes, int32_t* error_word, void* stream) {
   if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_pages < 0 || max_pages_per_seq < 0 || max_pages <= 0)
     return IRIS_EINVAL;
   if (num_q_heads % num_kv_heads != 0 || !(softmax_scale > 0.0f)) return IRIS_EINVAL;
   if (dtype != IRIS_DTYPE_FP16 && dtype != IRIS_DTYPE_BF16) return IRIS_EINVAL;
-  const int group = num_q_heads / num_kv_heads;
-  if (page_size != kPage || (head_dim != 64 && head_dim != 128) || group > 16) return IRIS_EUNSUPPORTED;
-  const int64_t rows = static_cast<int64_t>(batch) * num_kv_heads;
-  if (rows == 0) return IRIS_OK;
+  if (batch == 0) return IRIS_OK;
+  if (page_size != kPage || !sparse_shape_ok(batch, num_q_heads, num_kv_heads, head_dim, max_pages))
+    return IRIS_EUNSUPPORTED;
   if (num_pages == 0) return IRIS_EINVAL;
-  if (rows > (1 << 27)) return IRIS_EUNSUPPORTED;
   const void* ptrs[] = {query, k_data, v_data, k_scale, v_scale, block_table, seq_lens, page_list, page_count, output};
   for (const void* q : ptrs)
     if (q == nullptr) return IRIS_EINVAL;
   if (!aligned_to(query, 16) || !aligned_to(k_data, 16) || !aligned_to(v_data, 16) || !aligned_to(k_scale, 8) ||
-      !aligned_to(v_scale, 8) || !aligned_to(output, 4) || !aligned_to(out_lse, 4))
+      !aligned_to(v_scale, 8) || !aligned_to(output, 8) || !aligned_to(out_lse, 4) || !aligned_to(workspace, 16))
     return IRIS_EALIGN;
+  const int group = num_q_heads / num_kv_heads;
+  const int64_t rows = static_cast<int64_t>(batch) * num_kv_heads;
+  const Kernel k = kernel_for(dtype, head_dim, group > 8);
+  clear_stale_cuda_error();
+  SparseGrid grid;
+  cudaError_t e = grid_for(k, rows, group, head_dim, max_pages, kMinSteps, &grid);
+  if (e != cudaSuccess) {
+    record_cuda_error(e, "sparse_decode_kernel occupancy");
+    return IRIS_ECUDA;
+  }
+  if (workspace == nullptr || workspace_bytes < grid.bytes) return IRIS_EWORKSPACE;
   SparseParams p = {};
   p.query = query;
   p.k_data = static_cast<const uint8_t*>(k_data);
@@ -517,14 +841,33 @@ extern "C" int iris_b200_int4_sparse_paged_decode(const void* query, const void*
   p.kv_heads = num_kv_heads;
   p.group = group;
   p.keep = max_pages;
+  p.rows = static_cast<int32_t>(rows);
+  p.min_steps = kMinSteps;
+  p.vector_counts = aligned_to(page_count, 16) ? 1 : 0;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.row_start = reinterpret_cast<int32_t*>(ws);
+  p.part_o = reinterpret_cast<float*>(ws + grid.part_o);
+  p.part_ml = reinterpret_cast<float*>(ws + grid.part_ml);
   p.scale_log2 = static_cast<float>(static_cast<double>(softmax_scale) * 1.4426950408889634);
   p.err = error_word;
-  int splits = 1;
-  while (splits < 8 && rows * splits < 444 && max_pages > splits * kWarps) splits *= 2;
-  clear_stale_cuda_error();
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == IRIS_DTYPE_FP16 ? launch_any<Fp16Elem>(p, head_dim, rows, splits, s)
-                                                 : launch_any<Bf16Elem>(p, head_dim, rows, splits, s);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid.ctas));
+  cfg.blockDim = dim3(32 * kWarps);
+  cfg.dynamicSmemBytes = static_cast<size_t>(k.bytes);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  void* args[] = {&p};
+  e = cudaLaunchKernelExC(&cfg, k.fn, args);
+  if (e == cudaSuccess) {  // starts while the runs finish
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(rows), static_cast<unsigned>((group + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelExC(&cfg, k.join, args);
+  }
   if (e != cudaSuccess) {
     record_cuda_error(e, "sparse_decode_kernel launch");
     return IRIS_ECUDA;

@@ -91,7 +91,8 @@ SIGNATURES = {
     "iris_b200_int4_sparse_paged_decode": (
         ctypes.c_int,
         [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i32,
-         _c_i64, _c_i32, _c_i32, _c_i32, _c_f, _c_i32, _c_p, _c_p]),
+         _c_i64, _c_i32, _c_i32, _c_i32, _c_f, _c_i32, _c_p, _c_sz, _c_p, _c_p]),
+    "iris_b200_sparse_decode_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
     "iris_b200_xchg_buffer_bytes": (_c_sz, [_c_i64, _c_i32]),
     "iris_b200_xchg_alloc": (ctypes.c_int, [_c_sz, ctypes.POINTER(_c_p)]),
     "iris_b200_xchg_free": (ctypes.c_int, [_c_p]),

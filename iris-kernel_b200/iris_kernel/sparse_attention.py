@@ -226,6 +226,9 @@ def fused_int4_sparse_paged_decode_attention(
     if batch > 0:
         if num_pages == 0:
             raise IndexError("block_table contains an invalid physical page id")
+        need = _runtime.workspace_bytes(_lib.lib.iris_b200_sparse_decode_workspace_bytes, batch, num_q_heads,
+                                        num_kv_heads, head_dim, max_pages, device.index)
+        ws = _runtime.scratch(device, _runtime.stream_ptr(device), "sparse_decode", need)
         factor = head_dim ** -0.5 if softmax_scale is None or softmax_scale == 0.0 else float(softmax_scale)
         _runtime.launch(
             _lib.lib.iris_b200_int4_sparse_paged_decode, "iris_b200_int4_sparse_paged_decode", device,
@@ -233,5 +236,5 @@ def fused_int4_sparse_paged_decode_attention(
             v_scale.data_ptr(), block_table.data_ptr(), table_stride, seq_lens.data_ptr(),
             page_list.data_ptr(), page_count.data_ptr(), output.data_ptr(), None if lse is None else lse.data_ptr(),
             batch, num_q_heads, num_kv_heads, head_dim, num_pages, page_size, width, max_pages, factor,
-            code)
+            code, ws.data_ptr(), ws.numel())
     return (output, lse) if return_lse else output

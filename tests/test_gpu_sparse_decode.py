@@ -3,7 +3,7 @@ the attention over selected pages against 64 bits.
 
 Tolerance of the attention, per output: half a unit in the last place of the
 output's type (2^-11 or 2^-8 of the value), and 2^-14 of the largest value in
-the page list: p * scale is held in two bf16 terms (2^-18), and a logit of up to
+the page list: p * scale is held in two 16-bit terms (2^-18 or better), and a logit of up to
 128 products, summed in fp32 with at most 2^-22 of the running sum lost an
 addition and sums below 16, is off by less than 2^-15, which moves p and the
 normaliser by 2^-15.5 each.  The lse, a logit plus a logarithm, by 2^-14."""
