@@ -51,12 +51,28 @@ IRIS_DEV float quotient(float a, float b, float r) {
   return fmaf(fmaf(-t, b, a), r, t);
 }
 
-IRIS_DEV uint32_t pack_s8(const int (&v)[4]) {
-  return (v[0] & 0xff) | (v[1] & 0xff) << 8 | (v[2] & 0xff) << 16 | static_cast<uint32_t>(v[3]) << 24;
+IRIS_DEV float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+IRIS_DEV float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// The lowest bytes of four words.
+IRIS_DEV uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return prmt(prmt(a, b, 0x0040), prmt(c, d, 0x0040), 0x5410);
 }
 
 // One CTA per page (looping), one thread per 8-dim vector of one head; the
-// D / 8 threads of a head are adjacent lanes.
+// D / 8 threads of a head are adjacent lanes.  All of the thread's 16 words and
+// 16 scales are asked for before the first is used.  Two nibbles become fp16
+// with two operations, fp32 with one each, two products take one (exact), and
+// two tokens one three-way minimum and maximum: it is these that bound the
+// kernel, not the bytes.
 template <int D>
 __global__ void __launch_bounds__(256) bounds_kernel(const BoundsParams p) {
   constexpr int V = D / 8;
@@ -79,71 +95,90 @@ __global__ void __launch_bounds__(256) bounds_kernel(const BoundsParams p) {
       if (threadIdx.x == 0) set_error(p.err, IRIS_ERR_PAGE_ID);
       continue;
     }
-    const int tokens = min(kPage, len - col * kPage);
+    const int final_token = min(kPage, len - col * kPage) - 1;
     // whole warps go round together: lanes past the last vector repeat it and store nothing
     for (int i0 = threadIdx.x & ~31; i0 < vecs; i0 += blockDim.x) {
       const int i = min(i0 + static_cast<int>(threadIdx.x & 31), vecs - 1);
       const bool mine = i0 + static_cast<int>(threadIdx.x & 31) < vecs;
       const uint32_t* src = reinterpret_cast<const uint32_t*>(p.k_data) + page * kPage * vecs + i;
-      const __half* scl = p.k_scale + page * kPage * (vecs >> 2) + (i >> 2);
+      const unsigned short* scl =
+          reinterpret_cast<const unsigned short*>(p.k_scale) + page * kPage * (vecs >> 2) + (i >> 2);
       uint32_t w[kPage];
-      float s[kPage];
+      unsigned short sh[kPage];
 #pragma unroll
-      for (int t = 0; t < kPage; ++t) {
-        w[t] = t < tokens ? __ldg(src + static_cast<int64_t>(t) * vecs) : 0u;
-        s[t] = t < tokens ? __half2float(__ldg(scl + static_cast<int64_t>(t) * (vecs >> 2))) : 0.0f;
+      for (int t = 0; t < kPage; ++t) {  // tokens past the last one repeat it
+        const int tok = min(t, final_token);
+        w[t] = __ldg(src + tok * vecs);
+        sh[t] = __ldg(scl + tok * (vecs >> 2));
       }
-      float lo[8], hi[8];
-      bool bad = false;
+      float lo[8], hi[8], bad = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         lo[j] = INFINITY;
         hi[j] = -INFINITY;
       }
 #pragma unroll
-      for (int t = 0; t < kPage; ++t) {
-        if (t < tokens) {
-          bad |= !(fabsf(s[t]) <= 65504.0f);
+      for (int t = 0; t < kPage; t += 2) {
+        float x[2][8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float x = static_cast<float>(nibble(w[t], j)) * s[t];  // exact
-            lo[j] = fminf(lo[j], x);
-            hi[j] = fmaxf(hi[j], x);
+        for (int e = 0; e < 2; ++e) {
+          const float s = __half2float(__ushort_as_half(sh[t + e]));
+          const float2 s2 = make_float2(s, s);
+          bad = fmaf(s, 0.0f, bad);  // NaN from a scale that is not finite
+          const uint32_t v = w[t + e], u = v >> 8;
+          const uint32_t n[4] = {int4_lo_exact(v), int4_hi_exact(v), int4_lo_exact(u), int4_hi_exact(u)};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {  // dims j and j + 4
+            const float2 y = __fmul2_rn(__half22float2(u32_as_h2(n[j])), s2);
+            x[e][j] = y.x;
+            x[e][j + 4] = y.y;
           }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          lo[j] = min3(lo[j], x[0][j], x[1][j]);
+          hi[j] = max3(hi[j], x[0][j], x[1][j]);
         }
       }
       float m = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = fmaxf(m, fmaxf(fabsf(lo[j]), fabsf(hi[j])));
-      if (bad) m = INFINITY;
+      for (int j = 0; j < 8; ++j) m = max3(m, -lo[j], hi[j]);
+      if (bad != bad) m = INFINITY;
 #pragma unroll
       for (int o = 1; o < V; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       const bool finite = m <= 3.0e38f;
       const float step = finite ? __fdiv_rn(m, 127.0f) : INFINITY;
-      int cl[8], ch[8];
-      const float r = finite && step > 0.0f ? __frcp_rn(step) : 0.0f;
+      const float unit = finite && step > 0.0f ? step : 1.0f;  // (a head of zeros: lo = hi = 0)
+      const float r = __frcp_rn(unit);
+      const float kMagic = 12582912.0f;  // 1.5 2^23: a sum's low byte is the rounded value's
+      float zl[8], zh[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        cl[j] = finite ? (step > 0.0f ? max(-127, __float2int_rd(quotient(lo[j], step, r))) : 0) : -127;
-        ch[j] = finite ? (step > 0.0f ? min(127, __float2int_ru(quotient(hi[j], step, r))) : 0) : 127;
-        cl[j] = min(127, cl[j]);
-        ch[j] = max(-127, ch[j]);
+        const float a = finite ? quotient(lo[j], unit, r) : -127.0f, c = finite ? quotient(hi[j], unit, r) : 127.0f;
+        zl[j] = __fadd_rd(fminf(fmaxf(a, -127.0f), 127.0f), kMagic);
+        zh[j] = __fadd_ru(fminf(fmaxf(c, -127.0f), 127.0f), kMagic);
       }
       if (mine) {
         const int h = i / V, v = i - h * V;
         const int64_t head = page * p.kv_heads + h;
-        const int l0[4] = {cl[0], cl[1], cl[2], cl[3]}, l1[4] = {cl[4], cl[5], cl[6], cl[7]};
-        const int h0[4] = {ch[0], ch[1], ch[2], ch[3]}, h1[4] = {ch[4], ch[5], ch[6], ch[7]};
+        uint32_t cl[2], ch[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          cl[j] = low_bytes(__float_as_uint(zl[4 * j]), __float_as_uint(zl[4 * j + 1]), __float_as_uint(zl[4 * j + 2]),
+                            __float_as_uint(zl[4 * j + 3]));
+          ch[j] = low_bytes(__float_as_uint(zh[4 * j]), __float_as_uint(zh[4 * j + 1]), __float_as_uint(zh[4 * j + 2]),
+                            __float_as_uint(zh[4 * j + 3]));
+        }
         uint2* out = reinterpret_cast<uint2*>(p.bounds + head * 2 * D) + v;
-        out[0] = make_uint2(pack_s8(l0), pack_s8(l1));
-        out[V] = make_uint2(pack_s8(h0), pack_s8(h1));
+        out[0] = make_uint2(cl[0], cl[1]);
+        out[V] = make_uint2(ch[0], ch[1]);
         if (v == 0) p.step[head] = step;
         if (p.values != nullptr) {
           uint32_t a[4], c[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            a[j] = Fp16Elem::pack(cl[2 * j] * step, cl[2 * j + 1] * step);
-            c[j] = Fp16Elem::pack(ch[2 * j] * step, ch[2 * j + 1] * step);
+            a[j] = Fp16Elem::pack((zl[2 * j] - kMagic) * step, (zl[2 * j + 1] - kMagic) * step);
+            c[j] = Fp16Elem::pack((zh[2 * j] - kMagic) * step, (zh[2 * j + 1] - kMagic) * step);
           }
           uint4* val = reinterpret_cast<uint4*>(p.values + head * 2 * D) + v;
           val[0] = make_uint4(a[0], a[1], a[2], a[3]);
@@ -201,6 +236,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps) score_kernel(const ScorePara
   constexpr int kRow = 2 * D + 16;
   constexpr int kSpans = 2 * D / 64;
   constexpr int kRows = kWide ? 16 : 8;
+  grid_dependents_launch();  // the selection may come up meanwhile
   const int b = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int len = __ldg(p.seq_lens + b);
@@ -211,53 +247,116 @@ __global__ void __launch_bounds__(32 * kScoreWarps) score_kernel(const ScorePara
   const int n = static_cast<int>(all < p.max_pages ? all : p.max_pages);
   const int oct0 = blockIdx.x * p.octets;
   if (n <= p.max_keep || oct0 * 8 >= n) return;  // every page is kept, or none of these exist
-  uint8_t* codes = smem;
-  float* units = reinterpret_cast<float*>(smem + p.kv_heads * kRows * kRow);  // [Hkv][kRows]
-
-  // quantise the query heads, one warp a head at a time
-  for (int i = warp; i < p.kv_heads * kRows; i += kScoreWarps) {
-    const int h = i / kRows, g = i - h * kRows;
-    constexpr int W = D / 64;  // words a lane
-    uint32_t q[W];
-    float m = 0.0f;
-    bool nan = false;
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-      q[k] = g < p.group ? __ldg(static_cast<const uint32_t*>(p.query) +
-                                 (static_cast<int64_t>(b) * p.kv_heads * p.group + h * p.group + g) * (D / 2) + lane * W + k)
-                         : 0u;
-      const float2 f = E::unpack(q[k]);
-      m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
-      nan |= f.x != f.x || f.y != f.y;
-    }
-    if (nan) m = INFINITY;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    // a head that is not finite scores every page alike
-    const float unit = m <= 3.402823466e38f ? __fdiv_rn(m, 127.0f) : 0.0f;
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-      const float2 f = E::unpack(q[k]);
-      const int x = unit > 0.0f ? max(-127, min(127, __float2int_rn(__fdiv_rn(f.x, unit)))) : 0;
-      const int y = unit > 0.0f ? max(-127, min(127, __float2int_rn(__fdiv_rn(f.y, unit)))) : 0;
-      uint8_t* at = codes + i * kRow + 2 * (lane * W + k);
-      *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>((min(x, 0) & 0xff) | (min(y, 0) & 0xff) << 8);
-      *reinterpret_cast<uint16_t*>(at + D) = static_cast<uint16_t>(max(x, 0) | max(y, 0) << 8);
-    }
-    if (lane == 0) units[i] = unit;
-  }
-  __syncthreads();
-
   const int g = lane >> 2, t = lane & 3;
   const int octs = min(p.octets, (n + 7) / 8 - oct0);
   // units of work: (head, octet), a contiguous run of them for each warp
   const int total = p.kv_heads * octs;
   const int lo = total * warp / kScoreWarps, hi = total * (warp + 1) / kScoreWarps;
-  int head = -1;
+  // Loads run one unit ahead of the products and page numbers two, so that
+  // what a warp waits for is always already asked for.
+  const int32_t* table = p.block_table + b * p.table_stride + oct0 * 8 + g;
+  const int cols = n - oct0 * 8 - g;  // this lane's pages, one an octet
+  const auto page_of = [&](int oct) -> int32_t { return oct * 8 < cols ? __ldg(table + oct * 8) : 0; };
+  int h1 = lo / octs, oct1 = lo - h1 * octs;  // the unit whose bounds are loaded next
+  const auto advance = [&](int& h, int& oct) {
+    if (++oct == octs) {
+      oct = 0;
+      ++h;
+    }
+  };
+  int32_t page1 = lo < hi ? page_of(oct1) : 0, page2 = 0;  // its pages, and those of the one after it
+  uint4 next[kSpans];
+  float next_step = 0.0f;
+  const int8_t* bounds = p.bounds + 16 * t;
+  const auto load_unit = [&](int i) {
+    if (i < hi) {
+      if (page1 < 0 || page1 >= p.num_pages) {
+        set_error(p.err, IRIS_ERR_PAGE_ID);
+        page1 = 0;
+      }
+      const int64_t row = static_cast<int64_t>(page1) * p.kv_heads + h1;
+      const uint4* src = reinterpret_cast<const uint4*>(bounds + row * 2 * D);
+#pragma unroll
+      for (int k = 0; k < kSpans; ++k) next[k] = __ldg(src + 4 * k);
+      next_step = __ldg(p.step + row);
+      advance(h1, oct1);
+      page1 = page2;
+      if (i + 2 < hi) {
+        int h2 = h1, oct2 = oct1;
+        advance(h2, oct2);
+        page2 = page_of(oct2);
+      }
+    }
+  };
+  if (lo + 1 < hi) {
+    int h2 = h1, oct2 = oct1;
+    advance(h2, oct2);
+    page2 = page_of(oct2);
+  }
+
+  // Quantise the query heads, four rows of a warp at a time.
+  uint8_t* codes = smem;
+  float* units = reinterpret_cast<float*>(smem + p.kv_heads * kRows * kRow);  // [Hkv][kRows]
+  constexpr int W = D / 64;  // words a lane
+  constexpr int kAtOnce = 4;
+  bool loaded = false;
+  for (int i0 = warp; i0 < p.kv_heads * kRows; i0 += kAtOnce * kScoreWarps) {
+    uint32_t q[kAtOnce][W];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int i = i0 + j * kScoreWarps, h = i / kRows, gg = i % kRows;
+      const bool there = i < p.kv_heads * kRows && gg < p.group;
+#pragma unroll
+      for (int k = 0; k < W; ++k)
+        q[j][k] = there ? __ldg(static_cast<const uint32_t*>(p.query) +
+                                ((static_cast<int64_t>(b) * p.kv_heads + h) * p.group + gg) * (D / 2) + lane * W + k)
+                        : 0u;
+    }
+    if (!loaded) load_unit(lo);  // on its way while the heads are quantised
+    loaded = true;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int i = i0 + j * kScoreWarps;
+      float m = 0.0f;
+      bool nan = false;
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const float2 f = E::unpack(q[j][k]);
+        m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
+        nan |= f.x != f.x || f.y != f.y;
+      }
+      if (nan) m = INFINITY;
+      // magnitudes order as their bit patterns
+      m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+      // a head that is not finite scores every page alike
+      const float unit = m <= 3.402823466e38f ? __fdiv_rn(m, 127.0f) : 0.0f;
+      if (i < p.kv_heads * kRows) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+          const float2 f = E::unpack(q[j][k]);
+          const int x = unit > 0.0f ? max(-127, min(127, __float2int_rn(__fdiv_rn(f.x, unit)))) : 0;
+          const int y = unit > 0.0f ? max(-127, min(127, __float2int_rn(__fdiv_rn(f.y, unit)))) : 0;
+          uint8_t* at = codes + i * kRow + 2 * (lane * W + k);
+          *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>((min(x, 0) & 0xff) | (min(y, 0) & 0xff) << 8);
+          *reinterpret_cast<uint16_t*>(at + D) = static_cast<uint16_t>(max(x, 0) | max(y, 0) << 8);
+        }
+        if (lane == 0) units[i] = unit;
+      }
+    }
+  }
+  if (!loaded) load_unit(lo);  // (a warp without a row)
+  __syncthreads();
+
+  int head = -1, h = lo / octs, oct = lo - h * octs;
   uint32_t a[kSpans][kWide ? 8 : 4];
   float u0 = 0.0f, u1 = 0.0f;
+  uint32_t* out = p.keys + (static_cast<int64_t>(b) * p.kv_heads + h) * p.key_stride + oct0 * 8 + 2 * t;
   for (int i = lo; i < hi; ++i) {
-    const int h = i / octs, oct = oct0 + i - h * octs;
+    uint4 w[kSpans];
+#pragma unroll
+    for (int k = 0; k < kSpans; ++k) w[k] = next[k];
+    const float step = next_step;
+    load_unit(i + 1);
     if (h != head) {
       head = h;
       const uint8_t* row = codes + (h * kRows + g) * kRow + 16 * t;
@@ -273,17 +372,6 @@ __global__ void __launch_bounds__(32 * kScoreWarps) score_kernel(const ScorePara
       u0 = units[h * kRows + g];
       u1 = kWide ? units[h * kRows + g + 8] : 0.0f;
     }
-    const int col = oct * 8 + g;
-    int64_t page = col < n ? __ldg(p.block_table + b * p.table_stride + col) : 0;
-    if (page < 0 || page >= p.num_pages) {
-      set_error(p.err, IRIS_ERR_PAGE_ID);
-      page = 0;
-    }
-    const uint4* src = reinterpret_cast<const uint4*>(p.bounds + (page * p.kv_heads + h) * 2 * D) + t;
-    uint4 w[kSpans];
-#pragma unroll
-    for (int k = 0; k < kSpans; ++k) w[k] = __ldg(src + 4 * k);
-    const float step = __ldg(p.step + page * p.kv_heads + h);
     int acc[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int k = 0; k < kSpans; ++k) {
@@ -310,8 +398,12 @@ __global__ void __launch_bounds__(32 * kScoreWarps) score_kernel(const ScorePara
       // a page whose keys are not all finite comes before every other
       const uint32_t k0 = s0 <= 3.402823466e38f ? ordered(m0) : ordered(INFINITY);
       const uint32_t k1 = s1 <= 3.402823466e38f ? ordered(m1) : ordered(INFINITY);
-      uint32_t* out = p.keys + (static_cast<int64_t>(b) * p.kv_heads + h) * p.key_stride + oct * 8 + 2 * t;
-      *reinterpret_cast<uint2*>(out) = make_uint2(k0, k1);
+      *reinterpret_cast<uint2*>(out + oct * 8) = make_uint2(k0, k1);
+    }
+    if (++oct == octs) {
+      oct = 0;
+      ++h;
+      out += p.key_stride;
     }
   }
 }
@@ -325,112 +417,194 @@ struct SelectParams {
   int32_t* counts;  // [B, Hkv]
   int32_t max_pages;
   int32_t kv_heads;
+  int32_t rows;
   int32_t keep, sink, recent;
 };
 
-// Sum of v over the CTA, in every thread.  `slot` alternates between calls so
-// that one barrier a call is enough.
-template <int kThreads>
-IRIS_DEV int block_sum(int v, int* part, int slot) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  if ((threadIdx.x & 31) == 0) part[slot * 32 + (threadIdx.x >> 5)] = v;
-  __syncthreads();
-  const int lane = threadIdx.x & 31;
-  return __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? part[slot * 32 + lane] : 0);
+// What one row needs, before its keys are looked at.
+struct SelectRow {
+  int n, keep;  // pages there are, and pages to list
+  int32_t* out;
+  const uint32_t* keys;
+};
+IRIS_DEV SelectRow select_row(const SelectParams& p, int row) {
+  const int len = __ldg(p.seq_lens + row / p.kv_heads);
+  const int64_t all = len > 0 ? (static_cast<int64_t>(len) + kPage - 1) / kPage : 0;
+  SelectRow r;
+  r.n = static_cast<int>(all < p.max_pages ? all : p.max_pages);
+  r.keep = min(p.keep, r.n);
+  r.out = p.lists + static_cast<int64_t>(row) * p.keep;
+  r.keys = p.keys + static_cast<int64_t>(row) * p.key_stride;
+  return r;
+}
+// The key by which page i is chosen: kept ends above every score, 0 (below every key) past the end.
+IRIS_DEV uint32_t select_key(const SelectParams& p, const SelectRow& r, int i, uint32_t stored) {
+  return i >= r.n ? 0u : i < p.sink || i >= r.n - p.recent ? 0xffffffffu : stored;
 }
 
-// One CTA per (sequence, KV head).  The highest `keep` keys: the largest
-// threshold that at least `keep` keys reach, found bit by bit from the top
-// (32 counts over the CTA, keys in registers for KPT > 0, read again each
-// time otherwise), then one pass that writes the keys above it and the first
-// of those equal to it.
-template <int kThreads, int KPT>
-__global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) {
-  __shared__ int s_part[64];
-  __shared__ int s_scan[32];
-  const int row = blockIdx.x, b = row / p.kv_heads;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int len = __ldg(p.seq_lens + b);
-  const int64_t all = len > 0 ? (static_cast<int64_t>(len) + kPage - 1) / kPage : 0;
-  const int n = static_cast<int>(all < p.max_pages ? all : p.max_pages);
-  int32_t* out = p.lists + static_cast<int64_t>(row) * p.keep;
-  const int keep = min(p.keep, n);
-  if (tid == 0) p.counts[row] = keep;
-  for (int i = keep + tid; i < p.keep; i += kThreads) out[i] = -1;
-  if (n <= p.keep) {
-    for (int i = tid; i < n; i += kThreads) out[i] = i;
+// The highest `keep` keys are those above a threshold, the largest one that at
+// least `keep` keys reach, and the first of those equal to it.  The threshold
+// is found from its highest bit down by counting.
+
+// One warp per row of up to 32 KPT pages, all keys in registers, KPT
+// consecutive ones a lane: a count is a sum over the warp, no barrier.
+template <int KPT>
+__global__ void __launch_bounds__(128) select_warp_kernel(const SelectParams p) {
+  const int lane = threadIdx.x & 31, row = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  const SelectRow r = select_row(p, row);
+  if (lane == 0) p.counts[row] = r.keep;
+  for (int i = r.keep + lane; i < p.keep; i += 32) r.out[i] = -1;
+  if (r.n <= p.keep) {
+    for (int i = lane; i < r.n; i += 32) r.out[i] = i;
+    grid_dependency_wait();  // (nothing here runs ahead of the kernels before)
     return;
   }
-  const uint32_t* keys = p.keys + static_cast<int64_t>(row) * p.key_stride;
-  const auto key_at = [&](int i) -> uint32_t {  // 0 past the end: below every key
-    if (i >= n) return 0u;
-    return i < p.sink || i >= n - p.recent ? 0xffffffffu : __ldg(keys + i);
-  };
+  grid_dependency_wait();  // the scores are there
+  uint32_t k[KPT];
+#pragma unroll
+  for (int j = 0; j < KPT; j += 4) {
+    const int i = lane * KPT + j;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (i < r.n) v = __ldcg(reinterpret_cast<const uint4*>(r.keys + i));  // (the row's stride is a multiple of 8)
+    k[j] = select_key(p, r, i, v.x);
+    k[j + 1] = select_key(p, r, i + 1, v.y);
+    k[j + 2] = select_key(p, r, i + 2, v.z);
+    k[j + 3] = select_key(p, r, i + 3, v.w);
+  }
+  uint32_t thr = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t cand = thr | 1u << bit;
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) c += k[j] >= cand;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c >= r.keep) thr = cand;
+    if (c == r.keep) break;  // exactly the wanted ones reach it
+  }
+  int above = 0, equal = 0;
+#pragma unroll
+  for (int j = 0; j < KPT; ++j) {
+    above += k[j] > thr;
+    equal += k[j] == thr;
+  }
+  const int need = r.keep - __reduce_add_sync(0xffffffffu, above);
+  int a = above, e = equal;  // inclusive sums over the lanes
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, e, o);
+    if (lane >= o) a += x, e += y;
+  }
+  int eq = e - equal, at = a - above + min(eq, need);
+#pragma unroll
+  for (int j = 0; j < KPT; ++j) {
+    bool take = k[j] > thr;
+    if (k[j] == thr) take = eq++ < need;
+    if (take) r.out[at++] = lane * KPT + j;
+  }
+}
+
+// Sums over the CTA, in every thread.  `slot` alternates between calls so that
+// one barrier a call is enough.
+template <int kThreads>
+IRIS_DEV int block_sum(int v, int (*part)[32], int slot) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) part[slot][threadIdx.x >> 5] = v;
+  __syncthreads();
+  return __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? part[slot][lane] : 0);
+}
+
+// One CTA per longer row: KPT consecutive keys a thread in registers, or for
+// KPT = 0 read again for every count.  Two bits of the threshold at a time,
+// which halves the barriers.
+template <int kThreads, int KPT>
+__global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) {
+  __shared__ int s_part[6][32];
+  __shared__ int s_scan[2][32];
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const SelectRow r = select_row(p, row);
+  if (tid == 0) p.counts[row] = r.keep;
+  for (int i = r.keep + tid; i < p.keep; i += kThreads) r.out[i] = -1;
+  if (r.n <= p.keep) {
+    for (int i = tid; i < r.n; i += kThreads) r.out[i] = i;
+    grid_dependency_wait();  // (nothing here runs ahead of the kernels before)
+    return;
+  }
+  grid_dependency_wait();  // the scores are there
+  const auto key_at = [&](int i) { return select_key(p, r, i, i < r.n ? __ldcg(r.keys + i) : 0u); };
   constexpr int kRegs = KPT > 0 ? KPT : 1;
   uint32_t k[kRegs];
   if constexpr (KPT > 0) {
 #pragma unroll
-    for (int j = 0; j < KPT; ++j) k[j] = key_at(tid * KPT + j);
-  }
-  const auto count = [&](uint32_t at_least) {
-    int c = 0;
-    if constexpr (KPT > 0) {
-#pragma unroll
-      for (int j = 0; j < KPT; ++j) c += k[j] >= at_least;
-    } else {
-      for (int i = tid; i < n; i += kThreads) c += key_at(i) >= at_least;
+    for (int j = 0; j < KPT; j += 4) {
+      const int i = tid * KPT + j;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (i < r.n) v = __ldcg(reinterpret_cast<const uint4*>(r.keys + i));
+      k[j] = select_key(p, r, i, v.x);
+      k[j + 1] = select_key(p, r, i + 1, v.y);
+      k[j + 2] = select_key(p, r, i + 2, v.z);
+      k[j + 3] = select_key(p, r, i + 3, v.w);
     }
-    return c;
-  };
-  uint32_t thr = 0;
-  int slot = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t cand = thr | 1u << bit;
-    const int c = block_sum<kThreads>(count(cand), s_part, slot);
-    slot ^= 1;
-    if (c >= keep) thr = cand;
-    if (c == keep) break;  // exactly the wanted ones reach it
   }
-  // keys above the threshold, and how many of those equal to it come along
   const auto each = [&](auto&& f) {
     if constexpr (KPT > 0) {
 #pragma unroll
       for (int j = 0; j < KPT; ++j) f(tid * KPT + j, k[j]);
     } else {
-      const int per = (n + kThreads - 1) / kThreads;  // consecutive keys a thread
+      const int per = (r.n + kThreads - 1) / kThreads;  // consecutive keys a thread
       for (int j = 0; j < per; ++j) f(tid * per + j, key_at(tid * per + j));
     }
   };
+  uint32_t thr = 0;
+  int slot = 0;
+  for (int bit = 30; bit >= 0; bit -= 2) {
+    const uint32_t c1 = thr | 1u << bit, c2 = thr | 2u << bit, c3 = thr | 3u << bit;
+    int n1 = 0, n2 = 0, n3 = 0;
+    if constexpr (KPT > 0) {
+      each([&](int, uint32_t x) { n1 += x >= c1, n2 += x >= c2, n3 += x >= c3; });
+    } else {  // in any order
+      for (int i = tid; i < r.n; i += kThreads) {
+        const uint32_t x = key_at(i);
+        n1 += x >= c1, n2 += x >= c2, n3 += x >= c3;
+      }
+    }
+    n1 = __reduce_add_sync(0xffffffffu, n1);
+    n2 = __reduce_add_sync(0xffffffffu, n2);
+    n3 = __reduce_add_sync(0xffffffffu, n3);
+    if (lane == 0) s_part[slot][warp] = n1, s_part[slot + 1][warp] = n2, s_part[slot + 2][warp] = n3;
+    __syncthreads();
+    const bool in = lane < kThreads / 32;
+    n1 = __reduce_add_sync(0xffffffffu, in ? s_part[slot][lane] : 0);
+    n2 = __reduce_add_sync(0xffffffffu, in ? s_part[slot + 1][lane] : 0);
+    n3 = __reduce_add_sync(0xffffffffu, in ? s_part[slot + 2][lane] : 0);
+    slot = 3 - slot;
+    const int got = n3 >= r.keep ? n3 : n2 >= r.keep ? n2 : n1 >= r.keep ? n1 : 0;
+    thr = n3 >= r.keep ? c3 : n2 >= r.keep ? c2 : n1 >= r.keep ? c1 : thr;
+    if (got == r.keep) break;  // exactly the wanted ones reach it
+  }
   int above = 0, equal = 0;
   each([&](int, uint32_t x) {
     above += x > thr;
     equal += x == thr;
   });
-  const int total_above = block_sum<kThreads>(above, s_part, slot);
-  slot ^= 1;
-  const int need = keep - total_above;
-  // exclusive scans over the threads: of `above`, then of `equal`
-  int pre[2];
+  const int need = r.keep - block_sum<kThreads>(above, s_part + slot, 0);
+  int a = above, e = equal;  // inclusive sums over the lanes, then over the warps
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    const int own = which == 0 ? above : equal;
-    int x = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    __syncthreads();  // the previous round's readers are done
-    if (lane == 31) s_scan[warp] = x;
-    __syncthreads();
-    const int w = lane < kThreads / 32 && lane < warp ? s_scan[lane] : 0;
-    pre[which] = x - own + __reduce_add_sync(0xffffffffu, w);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, e, o);
+    if (lane >= o) a += x, e += y;
   }
-  int at = pre[0] + min(pre[1], need), eq = pre[1];
+  if (lane == 31) s_scan[0][warp] = a, s_scan[1][warp] = e;
+  __syncthreads();
+  const bool before = lane < warp;  // warp < 32
+  a += __reduce_add_sync(0xffffffffu, before ? s_scan[0][lane] : 0);
+  e += __reduce_add_sync(0xffffffffu, before ? s_scan[1][lane] : 0);
+  int eq = e - equal, at = a - above + min(eq, need);
   each([&](int i, uint32_t x) {
     bool take = x > thr;
     if (x == thr) take = eq++ < need;
-    if (take) out[at++] = i;
+    if (take) r.out[at++] = i;
   });
 }
 
@@ -449,17 +623,29 @@ cudaError_t launch_score(const ScoreParams& p, int head_dim, dim3 grid, cudaStre
   return cudaGetLastError();
 }
 
-cudaError_t launch_select(const SelectParams& p, int64_t rows, cudaStream_t s) {
-  const unsigned blocks = static_cast<unsigned>(rows);
-  if (p.max_pages <= 2048)
-    select_kernel<256, 8><<<blocks, 256, 0, s>>>(p);
-  else if (p.max_pages <= 8192)
-    select_kernel<1024, 8><<<blocks, 1024, 0, s>>>(p);
-  else if (p.max_pages <= 32768)
-    select_kernel<1024, 32><<<blocks, 1024, 0, s>>>(p);
-  else
-    select_kernel<1024, 0><<<blocks, 1024, 0, s>>>(p);
-  return cudaGetLastError();
+template <typename F>
+cudaError_t launch_after_scores(F* fn, unsigned blocks, unsigned threads, const SelectParams& p, cudaStream_t s) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fn, p);
+}
+
+cudaError_t launch_select(const SelectParams& p, cudaStream_t s) {
+  const unsigned rows = static_cast<unsigned>(p.rows), fours = (rows + 3) / 4;
+  if (p.max_pages <= 256) return launch_after_scores(select_warp_kernel<8>, fours, 128, p, s);
+  if (p.max_pages <= 512) return launch_after_scores(select_kernel<64, 8>, rows, 64, p, s);
+  if (p.max_pages <= 1024) return launch_after_scores(select_kernel<128, 8>, rows, 128, p, s);
+  if (p.max_pages <= 2048) return launch_after_scores(select_kernel<256, 8>, rows, 256, p, s);
+  if (p.max_pages <= 8192) return launch_after_scores(select_kernel<1024, 8>, rows, 1024, p, s);
+  if (p.max_pages <= 32768) return launch_after_scores(select_kernel<1024, 32>, rows, 1024, p, s);
+  return launch_after_scores(select_kernel<1024, 0>, rows, 1024, p, s);
 }
 
 int sm_count() {
@@ -552,7 +738,7 @@ extern "C" int iris_b200_page_select(const void* query, const void* bounds, cons
   if (num_kv_heads * (group > 8 ? 16 : 8) * (2 * head_dim + 20) > 200 * 1024) return IRIS_EUNSUPPORTED;
   if (batch == 0) return IRIS_OK;
   if (num_pages == 0) return IRIS_EINVAL;
-  if (batch > 65535 || max_pages_per_seq > (1 << 27)) return IRIS_EUNSUPPORTED;
+  if (batch > 65535 || num_kv_heads > 16384 || max_pages_per_seq > (1 << 27)) return IRIS_EUNSUPPORTED;
   const void* ptrs[] = {query, bounds, bounds_step, block_table, seq_lens, page_list, page_count};
   for (const void* q : ptrs)
     if (q == nullptr) return IRIS_EINVAL;
@@ -579,7 +765,7 @@ extern "C" int iris_b200_page_select(const void* query, const void* bounds, cons
   p.err = error_word;
   const int octets = static_cast<int>(key_stride_of(max_pages_per_seq) / 8);
   // the score kernel also reports bad lengths, so it runs even where every page is kept
-  const int want = (2 * sm_count() + batch - 1) / batch;
+  const int want = 3 * sm_count() / batch > 1 ? 3 * sm_count() / batch : 1;  // CTAs a sequence: three an SM in all
   p.octets = octets > 0 ? (octets + want - 1) / want : 1;
   const dim3 grid(octets > 0 ? static_cast<unsigned>((octets + p.octets - 1) / p.octets) : 1u,
                   static_cast<unsigned>(batch));
@@ -594,10 +780,11 @@ extern "C" int iris_b200_page_select(const void* query, const void* bounds, cons
     q.counts = page_count;
     q.max_pages = max_pages_per_seq;
     q.kv_heads = num_kv_heads;
+    q.rows = batch * num_kv_heads;
     q.keep = max_pages;
     q.sink = sink_pages;
     q.recent = recent_pages;
-    e = launch_select(q, static_cast<int64_t>(batch) * num_kv_heads, s);
+    e = launch_select(q, s);
   }
   if (e != cudaSuccess) {
     record_cuda_error(e, "page selection launch");
