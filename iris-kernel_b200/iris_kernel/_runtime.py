@@ -25,7 +25,7 @@ import threading
 
 import torch
 
-from . import _lib
+from . import _lib, _ops
 
 _MODES = ("sync", "deferred")
 _state = threading.local()
@@ -117,82 +117,23 @@ def require_sm100(device: torch.device) -> None:
         raise RuntimeError(f"iris_kernel is built for sm_100a (B200); device capability is {cap}")
 
 
-# element type codes of the entry points that take FP16 or BF16
-DTYPES = {torch.float16: _lib.DTYPE_FP16, torch.bfloat16: _lib.DTYPE_BF16}
-
-
-def dtype_code(name: str, dtype: torch.dtype) -> int:
-    code = DTYPES.get(dtype)
-    if code is None:
-        raise TypeError(f"{name} must use FP16(torch.float16) or BF16(torch.bfloat16)")
-    return code
-
-
-def require_device(name: str, t: torch.Tensor) -> torch.device:
-    """The tensor's device, which has to be a B200."""
-    if not cuda_available():
-        raise RuntimeError("Iris fused kernels require CUDA")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
-    device = t.device
+def _prepare(index: int) -> int:
+    """For the bindings: the address of a GPU's error word, once it is known
+    that the GPU can run the kernels."""
+    device = torch.device("cuda", index)
     require_sm100(device)
-    return device
+    return error_word(device).data_ptr()
 
 
-def check_tensor(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device) -> None:
-    """Shape, type, device and contiguity of one argument."""
-    if t.shape == shape and t.dtype is dtype and t.device == device and t.is_contiguous():
-        return
-    if t.shape != shape:
-        raise ValueError(f"{name} must have shape {tuple(shape)}")
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must use {dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}")
-    raise ValueError(f"{name} must be contiguous")
+_ops.set_up(_prepare)
 
 
-def check_block_table(block_table: torch.Tensor, batch: int, device: torch.device) -> tuple[int, int]:
-    """Its columns and the elements between its rows (rows may be apart)."""
-    shape = block_table.shape
-    if len(shape) != 2 or shape[0] != batch:
-        raise ValueError("block_table must have shape [B, max_pages_per_sequence]")
-    if block_table.dtype is not torch.int32:
-        raise TypeError("block_table must use torch.int32")
-    if block_table.device != device:
-        raise ValueError(f"block_table must be on {device}")
-    width = shape[1]
-    if batch > 0 and width == 0:
-        raise ValueError("block_table must have at least one column")
-    stride = block_table.stride()
-    if width > 1 and stride[1] != 1:
-        raise ValueError("block_table rows must be contiguous")
-    return width, stride[0]
-
-
-_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-
-
-def launch(fn, what: str, device: torch.device, *args) -> None:
-    """One C call on ``device``, the error word and its current stream as the
-    last two arguments, with the validation mode applied."""
-    idx = device.index
-    word = _words.get(idx)
-    if word is None:
-        word = error_word(device)
-    cur = _current_device()
-    if cur == idx:
-        status = fn(*args, word.data_ptr(), stream_ptr(device))
-    else:
-        torch.cuda.set_device(idx)
-        try:
-            status = fn(*args, word.data_ptr(), stream_ptr(device))
-        finally:
-            torch.cuda.set_device(cur)
-    if status:
-        _lib.check_status(status, what)
+def finish(t: torch.Tensor) -> None:
+    """Applies the validation mode after a call of the bindings on the device of ``t``."""
     if validation_mode() == "sync":
-        raise_for_bits(read_and_clear(word))
+        word = _words.get(t.get_device())
+        if word is not None:
+            raise_for_bits(read_and_clear(word))
 
 
 _scratch: dict = {}

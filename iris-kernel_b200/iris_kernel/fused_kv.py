@@ -12,12 +12,9 @@ back as dense keys and values) have no counterpart in the reference.
 """
 from __future__ import annotations
 
-import ctypes
-import functools
-
 import torch
 
-from . import _lib, _runtime
+from . import _lib, _ops, _runtime
 
 
 def _check_append_args(key, value, positions, slot_mapping, cos_cache, sin_cache, k_data, v_data, k_scale, v_scale,
@@ -306,37 +303,6 @@ def fused_rope_fp16_append(
             _runtime.raise_for_bits(_runtime.read_and_clear(word))
 
 
-@functools.lru_cache(maxsize=256)
-def _sections_array(sections: tuple, rotary_dim: int):
-    """The axes' frequency counts as a C array, checked."""
-    if not 1 <= len(sections) <= _lib.MROPE_MAX_AXES:
-        raise ValueError(f"sections must name 1 to {_lib.MROPE_MAX_AXES} axes")
-    if any(n < 0 for n in sections) or sum(sections) != rotary_dim // 2:
-        raise ValueError(f"sections must be non-negative and add up to rotary_dim // 2 = {rotary_dim // 2}")
-    return (ctypes.c_int32 * len(sections))(*sections)
-
-
-def _token_rows(name, t, shape, dtype, device):
-    """Checks ``[T, H, D]`` rows whose tokens may be apart (a slice of a fused
-    projection); returns their address and the elements between them."""
-    if t.shape != shape:
-        raise ValueError(f"{name} must have shape {tuple(shape)}")
-    if t.dtype is not dtype:
-        raise TypeError(f"{name} must use {dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}")
-    tokens, heads, dim = shape
-    if tokens == 0:
-        return 0, 0
-    apart, head, one = t.stride()
-    if one != 1 or (heads > 1 and head != dim) or (tokens > 1 and apart % 8 != 0):
-        raise ValueError(f"{name} must have contiguous heads and dims, and a token stride that is a multiple of 8")
-    ptr = t.data_ptr()
-    if ptr % 16 != 0:
-        raise ValueError(f"{name} must start on a 16-byte boundary")
-    return ptr, apart if tokens > 1 else 0
-
-
 def fused_mrope_int4_paged_append(
     key: torch.Tensor,
     value: torch.Tensor,
@@ -378,81 +344,11 @@ def fused_mrope_int4_paged_append(
     fused projection: tokens apart, heads and dims contiguous.  Tokens with
     ``slot_mapping < 0`` are padding: not stored, their rotated rows zero.  A
     batch with a bad slot or position writes nothing."""
-    device = _runtime.require_device("key", key)
-    if key.ndim != 3 or value.shape != key.shape:
-        raise ValueError("key and value must have shape [T, Hkv, D]")
-    dtype = key.dtype
-    code = _runtime.dtype_code("key", dtype)
-    num_tokens, num_kv_heads, head_dim = key.shape
-    if head_dim % 64 != 0 or not 64 <= head_dim <= 512:
-        raise NotImplementedError("fused append requires head_dim divisible by 64, up to 512")
-    if group_size != 32:
-        raise NotImplementedError("fused append supports group_size=32")
-    if rotary_dim % 16 != 0 or not 16 <= rotary_dim <= head_dim:
-        raise NotImplementedError("fused append requires rotary_dim divisible by 16, up to head_dim")
-    if num_kv_heads == 0:
-        raise ValueError("key and value must have at least one head")
-    if page_size <= 0:
-        raise ValueError("page_size must be positive")
-    counts = _sections_array(tuple(sections), rotary_dim)
-    axes = len(counts)
-    shape = key.shape
-    key_ptr, key_stride = _token_rows("key", key, shape, dtype, device)
-    value_ptr, value_stride = _token_rows("value", value, shape, dtype, device)
-    if positions.shape != (axes, num_tokens):
-        raise ValueError(f"positions must have shape [{axes}, T]")
-    if positions.dtype != torch.int32:
-        raise TypeError("positions must use torch.int32")
-    if positions.device != device:
-        raise ValueError(f"positions must be on {device}")
-    if num_tokens > 1 and positions.stride(1) != 1:
-        raise ValueError("positions of one axis must be contiguous")
-    check = _runtime.check_tensor
-    check("slot_mapping", slot_mapping, (num_tokens,), torch.int32, device)
-    if cos_cache.ndim != 2:
-        raise ValueError("cos_cache must have shape [max_position, rotary_dim // 2]")
-    table = (cos_cache.shape[0], rotary_dim // 2)
-    check("cos_cache", cos_cache, table, dtype, device)
-    check("sin_cache", sin_cache, table, dtype, device)
-    if k_data.ndim != 4:
-        raise ValueError("k_data/v_data must be rank-4 tensors")
-    num_pages = k_data.shape[0]
-    data, scale = (num_pages, page_size, num_kv_heads, head_dim // 2), (num_pages, page_size, num_kv_heads,
-                                                                        head_dim // 32)
-    check("k_data", k_data, data, torch.uint8, device)
-    check("v_data", v_data, data, torch.uint8, device)
-    check("k_scale", k_scale, scale, torch.float16, device)
-    check("v_scale", v_scale, scale, torch.float16, device)
-    query_ptr, num_q_heads, query_stride = None, 0, 0
-    if query is not None:
-        if query.ndim != 3 or query.shape[1] == 0:
-            raise ValueError("query must have shape [T, Hq, D]")
-        num_q_heads = query.shape[1]
-        q_shape = (num_tokens, num_q_heads, head_dim)
-        query_ptr, query_stride = _token_rows("query", query, q_shape, dtype, device)
-        if query_out is None:
-            query_out = query.new_empty(q_shape)
-        else:
-            check("query_out", query_out, q_shape, dtype, device)
-    elif query_out is not None:
-        raise ValueError("query_out needs a query")
-    if key_out is not None:
-        check("key_out", key_out, shape, dtype, device)
-    if num_tokens == 0:
-        return query_out
-    ws_ptr, ws_bytes = None, 0
-    if num_tokens > _lib.APPEND_INLINE_CHECK_TOKENS:  # smaller batches are checked without a workspace
-        need = _runtime.workspace_bytes(_lib.lib.iris_b200_append_check_workspace_bytes, num_pages, page_size)
-        ws = _runtime.scratch(device, _runtime.stream_ptr(device), "append_check", max(need, 4))
-        ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
-    _runtime.launch(
-        _lib.lib.iris_b200_mrope_int4_paged_append, "iris_b200_mrope_int4_paged_append", device,
-        key_ptr, key_stride, value_ptr, value_stride, query_ptr, query_stride, positions.data_ptr(), positions.stride(0), counts, axes, int(bool(interleaved)),
-        slot_mapping.data_ptr(), cos_cache.data_ptr(), sin_cache.data_ptr(), k_data.data_ptr(), v_data.data_ptr(),
-        k_scale.data_ptr(), v_scale.data_ptr(), None if query_out is None else query_out.data_ptr(),
-        None if key_out is None else key_out.data_ptr(), num_tokens, num_q_heads, num_kv_heads, head_dim, rotary_dim,
-        cos_cache.shape[0], num_pages, page_size, code, ws_ptr, ws_bytes)
-    return query_out
+    rotated = _ops.mrope_append(key, value, positions, slot_mapping, cos_cache, sin_cache, k_data, v_data, k_scale,
+                                v_scale, query, sections, rotary_dim, interleaved, group_size, page_size, query_out,
+                                key_out)
+    _runtime.finish(key)
+    return rotated
 
 
 def fused_int4_paged_gather(
@@ -479,54 +375,8 @@ def fused_int4_paged_gather(
     (int32 ``[B]``; None: from its first).  ``num_tokens`` is the host's count
     of rows, ``cu_seqlens[-1]``; rows past that are zeros.  For another chunk
     of prefill over a cached context, or to move a cache to another format."""
-    device = _runtime.require_device("k_data", k_data)
-    if group_size != 32:
-        raise NotImplementedError("gather supports group_size=32")
-    if k_data.ndim != 4:
-        raise ValueError("k_data/v_data must be rank-4 tensors")
-    num_pages, cache_page_size, num_kv_heads, packed_dim = k_data.shape
-    head_dim = 2 * packed_dim
-    if cache_page_size != page_size or page_size <= 0 or num_kv_heads == 0:
-        raise ValueError("packed cache shape does not match page_size")
-    if head_dim % 32 != 0 or not 32 <= head_dim <= 512:
-        raise NotImplementedError("gather requires head_dim divisible by 32, up to 512")
-    check = _runtime.check_tensor
-    data = k_data.shape
-    check("k_data", k_data, data, torch.uint8, device)
-    check("v_data", v_data, data, torch.uint8, device)
-    scale = (num_pages, page_size, num_kv_heads, head_dim // 32)
-    check("k_scale", k_scale, scale, torch.float16, device)
-    check("v_scale", v_scale, scale, torch.float16, device)
-    batch = block_table.shape[0]
-    width, table_stride = _runtime.check_block_table(block_table, batch, device)
-    check("cu_seqlens", cu_seqlens, (batch + 1,), torch.int32, device)
-    if first_token is not None:
-        check("first_token", first_token, (batch,), torch.int32, device)
-    if num_tokens < 0:
-        raise ValueError("num_tokens must not be negative")
-    shape = (num_tokens, num_kv_heads, head_dim)
-    code = _runtime.dtype_code("dtype", dtype if key is None else key.dtype)
-    if key is None and value is None:
-        key, value = torch.empty((2, *shape), dtype=dtype, device=device).unbind()
-    elif key is None:
-        key = torch.empty(shape, dtype=dtype, device=device)
-    else:
-        dtype = key.dtype
-        check("key", key, shape, dtype, device)
-    if value is None:
-        value = torch.empty(shape, dtype=dtype, device=device)
-    else:
-        check("value", value, shape, dtype, device)
-    if num_tokens == 0:
-        return key, value
-    if batch == 0:
-        raise ValueError("num_tokens must be 0 without sequences")
-    if num_pages == 0:
-        raise IndexError("block_table contains an invalid physical page id")
-    _runtime.launch(
-        _lib.lib.iris_b200_int4_paged_gather, "iris_b200_int4_paged_gather", device,
-        k_data.data_ptr(), v_data.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
-        table_stride, cu_seqlens.data_ptr(), None if first_token is None else first_token.data_ptr(),
-        key.data_ptr(), value.data_ptr(), num_tokens, batch, num_kv_heads, head_dim, num_pages, page_size,
-        width, code)
-    return key, value
+    bf16 = True if dtype is torch.bfloat16 else False if dtype is torch.float16 else None
+    out = _ops.gather(k_data, v_data, k_scale, v_scale, block_table, cu_seqlens, key, value, num_tokens, first_token,
+                      bf16, page_size, group_size)
+    _runtime.finish(k_data)
+    return out
