@@ -4,10 +4,10 @@
 //
 // A copy: per token and head 1.125 D bytes in and 4 D bytes out.  The heads of
 // a token are contiguous in the cache and in the output, so a token is one
-// row of R = Hkv D dims.  A CTA takes a tile of consecutive output rows, looks
-// each row's sequence and page up once (one thread a row, binary search in
-// the offsets), and then passes over the tile's 8-dim vectors: four packed
-// bytes in, one 16-byte store out, consecutive lanes on consecutive vectors.
+// row of R = Hkv D dims.  A CTA takes a tile of consecutive output rows; one
+// warp finds the first row's sequence and, a lane a row, the rows' places in
+// the cache; then all pass over the tile's 8-dim vectors: four packed bytes
+// in, one 16-byte store out, consecutive lanes on consecutive vectors.
 #include "elem.cuh"
 
 namespace iris {
@@ -36,18 +36,33 @@ struct GatherParams {
   int32_t* err;
 };
 
-// Cache row (page * page_size + offset) of output row n, -1 if it has none.
-IRIS_DEV int64_t row_of(const GatherParams& p, int64_t n) {
-  int lo = 0, hi = p.batch;  // the last sequence whose offset is <= n
+// The last sequence whose offset is <= n.  The whole warp calls it: 32 offsets
+// are tried at a time, so that a thousand sequences take two loads in a row.
+IRIS_DEV int sequence_of(const GatherParams& p, int64_t n) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = p.batch;
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (static_cast<int64_t>(__ldg(p.cu_seqlens + mid)) <= n) lo = mid;
-    else hi = mid;
+    const int step = (hi - lo + 31) >> 5, at = lo + lane * step;
+    const bool below = at < hi && static_cast<int64_t>(__ldg(p.cu_seqlens + at)) <= n;
+    const unsigned mask = __ballot_sync(0xffffffffu, below);
+    const int k = mask != 0 ? 31 - __clz(mask) : 0;
+    lo += k * step;
+    hi = min(hi, lo + step);
   }
-  const int64_t start = __ldg(p.cu_seqlens + lo), end = __ldg(p.cu_seqlens + lo + 1);
-  const int64_t from = p.first_token != nullptr ? __ldg(p.first_token + lo) : 0;
+  return lo;
+}
+
+// Cache row (page * page_size + offset) of output row n, -1 if it has none;
+// `seq`: the sequence of a row at or before it.
+IRIS_DEV int64_t row_of(const GatherParams& p, int64_t n, int seq) {
   const int64_t total = __ldg(p.cu_seqlens + p.batch);
-  if (n >= total) return -1;                                // past the last sequence: zeros
+  if (n >= total) return -1;  // past the last sequence: zeros
+  int64_t start = __ldg(p.cu_seqlens + seq), end = __ldg(p.cu_seqlens + seq + 1);
+  while (n >= end && seq + 1 < p.batch) {
+    start = end;
+    end = __ldg(p.cu_seqlens + ++seq + 1);
+  }
+  const int64_t from = p.first_token != nullptr ? __ldg(p.first_token + seq) : 0;
   if (n < start || n >= end || end > total || from < 0) {  // offsets that do not rise from 0
     set_error(p.err, IRIS_ERR_SEQ_LEN);
     return -1;
@@ -57,7 +72,7 @@ IRIS_DEV int64_t row_of(const GatherParams& p, int64_t n) {
     set_error(p.err, IRIS_ERR_BLOCK_TABLE);
     return -1;
   }
-  const int64_t page = __ldg(p.block_table + lo * p.table_stride + col);
+  const int64_t page = __ldg(p.block_table + seq * p.table_stride + col);
   if (page < 0 || page >= p.num_pages) {
     set_error(p.err, IRIS_ERR_PAGE_ID);
     return -1;
@@ -79,7 +94,10 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const GatherParams p) 
   __shared__ int64_t s_row[kTile];
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kTile;
   const int rows = static_cast<int>(p.num_tokens - n0 < kTile ? p.num_tokens - n0 : kTile);
-  if (threadIdx.x < rows) s_row[threadIdx.x] = row_of(p, n0 + threadIdx.x);
+  if (threadIdx.x < 32) {
+    const int seq = sequence_of(p, n0);
+    if (threadIdx.x < rows) s_row[threadIdx.x] = row_of(p, n0 + threadIdx.x, seq);
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < rows * p.vecs; i += kThreads) {
     const int r = i / p.vecs, v = i - r * p.vecs;

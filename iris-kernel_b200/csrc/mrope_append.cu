@@ -14,11 +14,12 @@
 // that reading it back gives NaN.
 //
 // The work is a copy with arithmetic on the way: per token 2 Hkv D (and Hq D)
-// 16-bit values in, 1.125 Hkv D bytes (and Hq D values) out.  One CTA takes
-// one token, a thread one 8-dim vector of the row: the rotary rows of the
-// token are read, and their axes blended, once per thread and used for all
-// the rows (keys, values, queries) that the thread passes over.  A group is
-// four adjacent lanes; its absmax takes two shuffles.
+// 16-bit values in, 1.125 Hkv D bytes (and Hq D values) out.  A token takes
+// row_lanes x D / 8 threads, a thread one 8-dim vector of every row_lanes-th
+// head: the token's rotary rows are read, and their axes blended, once per
+// thread and used for all its keys and queries.  A group is four adjacent
+// lanes; its absmax takes two shuffles.  What bounds it is instructions, then
+// bytes: arithmetic goes two values at a time.
 #include "append_common.cuh"
 #include "elem.cuh"
 
@@ -50,6 +51,7 @@ struct MropeParams {
   int64_t num_slots;
   int32_t axes;
   int32_t kv_heads, q_heads;
+  int32_t row_lanes;    // threads of a token that share a vector
   int32_t vecs;         // 8-dim vectors per row
   int32_t rotary_vecs;  // of them rotated
   int32_t* err;
@@ -83,6 +85,31 @@ __global__ void __launch_bounds__(kThreads) mrope_check_kernel(const MropeParams
   if (bits) set_error(p.err, bits);
 }
 
+// The same for batches of up to kPairwiseTokens tokens without a bitmap, and
+// so without clearing one first: every slot is held against all the others, by
+// eight lanes a token.
+constexpr int64_t kPairwiseTokens = 2048;
+__global__ void __launch_bounds__(kThreads) mrope_check_pairs_kernel(const MropeParams p) {
+  __shared__ __align__(16) int32_t s_slot[kPairwiseTokens];
+  grid_dependents_launch();
+  const int T = static_cast<int>(p.num_tokens), T4 = (T + 3) & ~3;
+  for (int i = threadIdx.x; i < T4; i += kThreads) s_slot[i] = i < T ? __ldg(p.slots + i) : -1;
+  const int i = (blockIdx.x * kThreads + threadIdx.x) >> 3, part = threadIdx.x & 7;
+  const int32_t slot = i < T ? __ldg(p.slots + i) : -1;
+  int32_t bits = 0;
+  if (slot >= 0 && part == 0) bits = token_bits(p, slot, i);
+  __syncthreads();
+  if (slot < 0) return;
+  int hits = 0;
+  for (int j = 4 * part; j < T4; j += 32) {
+    const int4 v = *reinterpret_cast<const int4*>(s_slot + j);
+    hits += (v.x == slot) + (v.y == slot) + (v.z == slot) + (v.w == slot);
+  }
+  const unsigned mates = 0xFFu << (threadIdx.x & 24);  // the token's lanes, which all came here
+  if (__reduce_add_sync(mates, hits) > 1) bits |= IRIS_ERR_DUP_SLOT;
+  if (part == 0 && bits) set_error(p.err, bits);
+}
+
 // The same for at most kInlineCheckTokens tokens, by every CTA of the append.
 IRIS_DEV bool check_small_batch(const MropeParams& p) {
   __shared__ __align__(16) int32_t s_slot[kInlineCheckTokens];
@@ -111,7 +138,7 @@ IRIS_DEV bool check_small_batch(const MropeParams& p) {
 // cos / sin of eight frequencies, each from the row of its own axis.  `code`
 // holds the eight axes, two bits each; one load if they are all the same.
 template <typename E>
-IRIS_DEV void blend_rows(const MropeParams& p, int64_t tok, int fv, float (&c)[8], float (&s)[8]) {
+IRIS_DEV void blend_rows(const MropeParams& p, int64_t tok, int fv, float2 (&c)[4], float2 (&s)[4]) {
   const uint32_t code = (p.axis_map[fv >> 1] >> (16 * (fv & 1))) & 0xffffu;
   const int64_t width = static_cast<int64_t>(p.rotary_vecs) * 4;  // R / 2
   uint32_t cw[4] = {0, 0, 0, 0}, sw[4] = {0, 0, 0, 0};
@@ -133,23 +160,28 @@ IRIS_DEV void blend_rows(const MropeParams& p, int64_t tok, int fv, float (&c)[8
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float2 a = E::unpack(cw[j]), b = E::unpack(sw[j]);
-    c[2 * j] = a.x;
-    c[2 * j + 1] = a.y;
-    s[2 * j] = b.x;
-    s[2 * j + 1] = b.y;
+    c[j] = E::unpack(cw[j]);
+    s[j] = E::unpack(sw[j]);
   }
 }
 
 template <typename E>
-IRIS_DEV void unpack8(const uint4& w, float (&x)[8]) {
-  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 f = E::unpack(v[j]);
-    x[2 * j] = f.x;
-    x[2 * j + 1] = f.y;
-  }
+IRIS_DEV void unpack8(const uint4& w, float2 (&x)[4]) {
+  x[0] = E::unpack(w.x);
+  x[1] = E::unpack(w.y);
+  x[2] = E::unpack(w.z);
+  x[3] = E::unpack(w.w);
+}
+template <typename E>
+IRIS_DEV uint4 pack8(const float2 (&x)[4]) {
+  return make_uint4(E::pack(x[0].x, x[0].y), E::pack(x[1].x, x[1].y), E::pack(x[2].x, x[2].y), E::pack(x[3].x, x[3].y));
+}
+
+// max(|a|, |b|, |c|), NaN if one of them is.
+IRIS_DEV float absmax3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  return d;
 }
 
 // Eight fp32 values of a group of four lanes -> fp16 group scale and this
@@ -157,119 +189,207 @@ IRIS_DEV void unpack8(const uint4& w, float (&x)[8]) {
 // is the correctly rounded reciprocal, t = x r is off by at most 1.5 ulp, and
 // one residual step (Markstein 1990) leaves an error of 2^-23 ulp before the
 // last rounding, while a quotient of a 24-bit by an 11-bit number that is no
-// rounding midpoint stays 2^-12 ulp away from one.
-IRIS_DEV uint32_t quant8(const float (&x)[8], uint32_t quad, __half& scale16) {
-  float m = 0.0f;
-  bool nan = false;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    m = fmaxf(m, fabsf(x[j]));  // skips NaN
-    nan |= x[j] != x[j];
-  }
-  if (nan) m = __int_as_float(0x7fffffff);  // as an integer above every magnitude
-  // magnitudes order as their bit patterns, NaN on top
-  uint32_t b = __float_as_uint(m);
-  b = max(b, __shfl_xor_sync(quad, b, 1));
-  b = max(b, __shfl_xor_sync(quad, b, 2));
-  m = __uint_as_float(b);
+// rounding midpoint stays 2^-12 ulp away from one.  amax / 7 takes two such
+// steps, its first quotient then being faithful whatever amax is.
+IRIS_DEV uint32_t quant8(const float2 (&x)[4], uint32_t quad, __half& scale16) {
+  float m = absmax3(x[0].x, x[0].y, x[1].x);
+  m = absmax3(m, x[1].y, x[2].x);
+  m = absmax3(m, x[2].y, x[3].x);
+  m = absmax3(m, x[3].y, __shfl_xor_sync(quad, absmax3(m, x[3].y, 0.0f), 1));
+  m = absmax3(m, 0.0f, __shfl_xor_sync(quad, m, 2));
   if (!(m <= 3.402823466e38f)) {  // an infinity or NaN in the group
     scale16 = __float2half_rn(m);
     return 0u;
   }
-  const float s = fminf(fmaxf(__fdiv_rn(m, 7.0f), 6.103515625e-05f), 65504.0f);
-  scale16 = __float2half_rn(s);
+  const float r7 = 0.142857149f;  // fp32(1 / 7)
+  float s = m * r7;
+  s = fmaf(fmaf(-s, 7.0f, m), r7, s);
+  s = fmaf(fmaf(-s, 7.0f, m), r7, s);
+  scale16 = __float2half_rn(fminf(fmaxf(s, 6.103515625e-05f), 65504.0f));
   const float sc = __half2float(scale16), r = __frcp_rn(sc);
+  const float2 r2 = make_float2(r, r), ns2 = make_float2(-sc, -sc);
+  float2 q[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 t = __fmul2_rn(x[j], r2);
+    q[j] = __ffma2_rn(__ffma2_rn(t, ns2, x[j]), r2, t);
+  }
+  if (s > 65504.0f) {  // only then can a quotient pass 7 by more than a rounding
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      q[j].x = fminf(fmaxf(q[j].x, -7.0f), 7.0f);
+      q[j].y = fminf(fmaxf(q[j].y, -7.0f), 7.0f);
+    }
+  }
+  const float2 magic = make_float2(8388624.0f, 8388624.0f);  // 2^23 + 16: rounds half to even, low four bits the nibble
   uint32_t z[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float t = __fmul_rn(x[j], r);
-    const float q = fmaf(fmaf(-t, sc, x[j]), r, t);
-    // 2^23 + 16: rounds half to even, low four bits are the nibble
-    z[j] = __float_as_uint(__fadd_rn(fminf(fmaxf(q, -7.0f), 7.0f), 8388624.0f));
+  for (int j = 0; j < 4; ++j) {
+    const float2 v = __fadd2_rn(q[j], magic);
+    z[2 * j] = __float_as_uint(v.x);
+    z[2 * j + 1] = __float_as_uint(v.y);
   }
   const uint32_t ev = __byte_perm(__byte_perm(z[0], z[2], 0x0040), __byte_perm(z[4], z[6], 0x0040), 0x5410);
   const uint32_t od = __byte_perm(__byte_perm(z[1], z[3], 0x0040), __byte_perm(z[5], z[7], 0x0040), 0x5410);
   return (ev & 0x0F0F0F0Fu) | ((od << 4) & 0xF0F0F0F0u);
 }
 
-template <typename E>
-IRIS_DEV uint4 pack8(const float (&x)[8]) {
-  return make_uint4(E::pack(x[0], x[1]), E::pack(x[2], x[3]), E::pack(x[4], x[5]), E::pack(x[6], x[7]));
-}
-
-// gridDim = (tokens, row splits).  kSmall: at most kInlineCheckTokens tokens,
-// validated here; otherwise the check kernel before this launch did it.
+// kSmall: at most kInlineCheckTokens tokens, one a CTA, validated here;
+// otherwise the check kernel before this launch did it.  The first keys (with
+// few tokens the first values and queries too) are asked for before anything
+// else is looked at: they depend on neither the slot nor the positions.  With
+// many tokens more warps on an SM do more than more loads a thread: 64
+// registers a thread took 78 us at 8192 tokens of 32 + 2 x 8 heads, 85
+// registers 85 us, 128 102 us (each with the 15 us of its check and read back).
 template <typename E, bool kSmall>
-__global__ void __launch_bounds__(kThreads) mrope_append_kernel(const MropeParams p) {
-  const int v = threadIdx.x % p.vecs;  // vector within the row
-  const int per_pass = blockDim.x / p.vecs;
-  const int64_t tok = blockIdx.x;
-  const int rows = 2 * p.kv_heads + p.q_heads;
-  const int32_t slot = __ldg(p.slots + tok);
-  bool rejected = false;
-  if constexpr (kSmall) rejected = check_small_batch(p);
-  // A token with a bad slot or position: never touch memory outside the cache
-  // or the tables.  (The check has recorded its bits.)
-  const bool live = slot >= 0 && token_bits(p, slot, tok) == 0;
+__global__ void __launch_bounds__(kThreads, kSmall ? 2 : 4) mrope_append_kernel(const MropeParams p) {
+  constexpr int kBatch = 2;  // heads whose vectors a thread has on the way, of each kind
+  const int per_token = p.row_lanes * p.vecs;
+  const int here = threadIdx.x / per_token, in_token = threadIdx.x - here * per_token;
+  const int row = in_token / p.vecs, v = in_token - row * p.vecs;  // first head, and vector within the head
+  const int64_t tok = static_cast<int64_t>(blockIdx.x) * (blockDim.x / per_token) + here;
+  const bool there = tok < p.num_tokens;  // (the last CTA's threads past the end go along with the checks)
+  const int64_t at = there ? tok : 0;
   const int half = p.rotary_vecs / 2;  // vectors of the rotary half
-  const bool turns = live && v < p.rotary_vecs;
-  const bool low = v < half;
-  const int fv = low ? v : v - half;
-  float c[8], s[8];
-  if (turns) blend_rows<E>(p, tok, fv, c, s);
-  const uint32_t quad = 0xFu << (threadIdx.x & 28);
-  if constexpr (!kSmall) grid_dependency_wait();
-  if (rejected || (p.err != nullptr && (*reinterpret_cast<volatile int32_t*>(p.err) & kRejectBits) != 0)) return;
-  const int64_t D = 8ll * p.vecs;
-  for (int r = threadIdx.x / p.vecs + per_pass * blockIdx.y; r < rows; r += per_pass * gridDim.y) {
-    const bool is_v = r >= p.kv_heads && r < 2 * p.kv_heads, is_q = r >= 2 * p.kv_heads;
-    const int h = is_q ? r - 2 * p.kv_heads : is_v ? r - p.kv_heads : r;
-    const char* base = static_cast<const char*>(is_q ? p.query : is_v ? p.value : p.key);
-    const int64_t stride = is_q ? p.query_stride : is_v ? p.value_stride : p.key_stride;
-    char* out = static_cast<char*>(is_q ? p.query_out : is_v ? nullptr : p.key_out);
-    if (out != nullptr) out += ((tok * (is_q ? p.q_heads : p.kv_heads) + h) * D + 8 * v) * 2;
-    if (!live) {  // padding: its rotated rows are zeros
-      if (out != nullptr) *reinterpret_cast<uint4*>(out) = make_uint4(0, 0, 0, 0);
-      continue;
-    }
-    const char* row = base + (tok * stride + h * D) * 2;
-    float x[8];
-    unpack8<E>(ldg_nc_v4(row + 16 * v), x);
-    if (!is_v && turns) {
-      float o[8];
-      unpack8<E>(ldg_nc_v4(row + 16 * (low ? v + half : v - half)), o);
+  const bool rotary = v < p.rotary_vecs, low = v < half;
+  const int64_t D2 = 16ll * p.vecs;                      // bytes of a head
+  const int64_t mate = (low ? half : -half) * 16ll;      // bytes to the vector that turns with this one
+  const int64_t stride = D2 * p.row_lanes;               // bytes to this thread's next head
+  const char* key = static_cast<const char*>(p.key) + at * p.key_stride * 2 + row * D2 + 16 * v;
+  const char* value = static_cast<const char*>(p.value) + at * p.value_stride * 2 + row * D2 + 16 * v;
+  const char* query = static_cast<const char*>(p.query) + at * p.query_stride * 2 + row * D2 + 16 * v;
+  // vectors of heads h, h + row_lanes, .. of a tensor, and for a turning one their mates
+  const auto load = [&](const char* src, int h, int heads, bool turning, uint4 (&x)[kBatch], uint4 (&o)[kBatch]) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float t = __fmul_rn(o[j], s[j]), u = __fmul_rn(x[j], c[j]);  // both exact
-        x[j] = low ? __fsub_rn(u, t) : __fadd_rn(u, t);
+    for (int j = 0; j < kBatch; ++j) {
+      if (h + j * p.row_lanes < heads) {
+        x[j] = ldg_nc_v4(src + j * stride);
+        if (turning) o[j] = ldg_nc_v4(src + j * stride + mate);
       }
     }
-    if (out != nullptr) *reinterpret_cast<uint4*>(out) = pack8<E>(x);
-    if (!is_q) {
-      __half scale;
-      const uint32_t word = quant8(x, quad, scale);
-      const int64_t cache_row = static_cast<int64_t>(slot) * p.kv_heads + h;
-      *reinterpret_cast<uint32_t*>((is_v ? p.v_data : p.k_data) + cache_row * (D / 2) + 4 * v) = word;
-      if ((v & 3) == 0) (is_v ? p.v_scale : p.k_scale)[cache_row * (D / 32) + (v >> 2)] = scale;
+  };
+  uint4 kx[kBatch], ko[kBatch];
+  load(key, row, p.kv_heads, rotary, kx, ko);
+  uint4 vx[kBatch], none[kBatch], qx[kBatch], qo[kBatch];
+  if constexpr (kSmall) {
+    load(value, row, p.kv_heads, false, vx, none);
+    load(query, row, p.q_heads, rotary, qx, qo);
+  }
+  const int32_t slot = there ? __ldg(p.slots + tok) : -1;
+  // A token with a bad slot or position: never touch memory outside the cache
+  // or the tables.  (The check records its bits.)
+  const bool live = slot >= 0 && token_bits(p, slot, at) == 0;
+  float2 c[4], s[4];
+  if (live && rotary) {
+    blend_rows<E>(p, tok, low ? v : v - half, c, s);
+    if (low) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = make_float2(-s[j].x, -s[j].y);
     }
+  }
+  bool rejected = false;
+  if constexpr (kSmall) rejected = check_small_batch(p);
+  else grid_dependency_wait();
+  if (rejected || (p.err != nullptr && (*reinterpret_cast<volatile int32_t*>(p.err) & kRejectBits) != 0)) return;
+  if (!there) return;
+  const uint32_t quad = 0xFu << (threadIdx.x & 28);
+
+  // x cos + mate (-+ sin): both products are exact, one rounding in all
+  const auto turn = [&](const uint4& xw, const uint4& ow, float2 (&x)[4]) {
+    unpack8<E>(xw, x);
+    if (rotary) {
+      float2 o[4];
+      unpack8<E>(ow, o);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = __ffma2_rn(x[j], c[j], __fmul2_rn(o[j], s[j]));
+    }
+  };
+  const int64_t cache_row = static_cast<int64_t>(slot) * p.kv_heads;
+  const auto store = [&](const float2 (&x)[4], int h, uint8_t* data, __half* scales) {
+    __half scale;
+    const uint32_t word = quant8(x, quad, scale);
+    reinterpret_cast<uint32_t*>(data)[(cache_row + h) * p.vecs + v] = word;
+    if ((v & 3) == 0) scales[(cache_row + h) * (p.vecs >> 2) + (v >> 2)] = scale;
+  };
+
+  char* out = p.key_out != nullptr ? static_cast<char*>(p.key_out) + (at * p.kv_heads + row) * D2 + 16 * v : nullptr;
+  for (int h = row; h < p.kv_heads; h += kBatch * p.row_lanes) {
+    if (h != row) load(key, h, p.kv_heads, rotary, kx, ko);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int hh = h + j * p.row_lanes;
+      if (hh < p.kv_heads) {
+        if (live) {
+          float2 x[4];
+          turn(kx[j], ko[j], x);
+          if (out != nullptr) *reinterpret_cast<uint4*>(out + j * stride) = pack8<E>(x);
+          store(x, hh, p.k_data, p.k_scale);
+        } else if (out != nullptr) {  // padding: its rotated rows are zeros
+          *reinterpret_cast<uint4*>(out + j * stride) = make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+    key += kBatch * stride;
+    if (out != nullptr) out += kBatch * stride;
+  }
+  if (live) {
+    for (int h = row; h < p.kv_heads; h += kBatch * p.row_lanes) {
+      if (!kSmall || h != row) load(value, h, p.kv_heads, false, vx, none);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int hh = h + j * p.row_lanes;
+        if (hh < p.kv_heads) {
+          float2 x[4];
+          unpack8<E>(vx[j], x);
+          store(x, hh, p.v_data, p.v_scale);
+        }
+      }
+      value += kBatch * stride;
+    }
+  }
+  out = static_cast<char*>(p.query_out) + (at * p.q_heads + row) * D2 + 16 * v;
+  for (int h = row; h < p.q_heads; h += kBatch * p.row_lanes) {
+    if (!kSmall || h != row) load(query, h, p.q_heads, rotary, qx, qo);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (h + j * p.row_lanes < p.q_heads) {
+        float2 x[4];
+        uint4 word = make_uint4(0, 0, 0, 0);
+        if (live) {
+          turn(qx[j], qo[j], x);
+          word = pack8<E>(x);
+        }
+        *reinterpret_cast<uint4*>(out + j * stride) = word;
+      }
+    }
+    query += kBatch * stride;
+    out += kBatch * stride;
   }
 }
 
 template <typename E>
-cudaError_t launch_mrope(const MropeParams& p, uint32_t* bitmap, size_t bitmap_bytes, cudaStream_t stream) {
-  const int threads = kThreads / p.vecs * p.vecs;
-  const int rows = 2 * p.kv_heads + p.q_heads, per_pass = threads / p.vecs;
-  const int passes = (rows + per_pass - 1) / per_pass;
+cudaError_t launch_mrope(MropeParams& p, uint32_t* bitmap, size_t bitmap_bytes, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.stream = stream;
-  cfg.blockDim = dim3(threads);
-  if (p.num_tokens <= kInlineCheckTokens) {
-    cfg.gridDim = dim3(static_cast<unsigned>(p.num_tokens), static_cast<unsigned>(passes));
+  if (p.num_tokens <= kInlineCheckTokens) {  // few tokens: as many threads on each as fit
+    p.row_lanes = kThreads / p.vecs;
+    cfg.blockDim = dim3(p.row_lanes * p.vecs);
+    cfg.gridDim = dim3(static_cast<unsigned>(p.num_tokens));
     return cudaLaunchKernelEx(&cfg, mrope_append_kernel<E, true>, p);
   }
-  cudaError_t e = bitmap_bytes > 0 ? cudaMemsetAsync(bitmap, 0, bitmap_bytes, stream) : cudaSuccess;
-  if (e != cudaSuccess) return e;
-  mrope_check_kernel<<<static_cast<unsigned>((p.num_tokens + kThreads - 1) / kThreads), kThreads, 0, stream>>>(p, bitmap);
+  // many: few threads a token, so that each blended row serves many heads
+  p.row_lanes = 4;
+  const int tokens = kThreads / (4 * p.vecs);  // a CTA
+  cfg.blockDim = dim3(tokens * 4 * p.vecs);
+  cfg.gridDim = dim3(static_cast<unsigned>((p.num_tokens + tokens - 1) / tokens));
+  cudaError_t e = cudaSuccess;
+  if (p.num_tokens <= kPairwiseTokens) {
+    mrope_check_pairs_kernel<<<static_cast<unsigned>((8 * p.num_tokens + kThreads - 1) / kThreads), kThreads, 0, stream>>>(p);
+  } else {
+    if (bitmap_bytes > 0) e = cudaMemsetAsync(bitmap, 0, bitmap_bytes, stream);
+    if (e != cudaSuccess) return e;
+    mrope_check_kernel<<<static_cast<unsigned>((p.num_tokens + kThreads - 1) / kThreads), kThreads, 0, stream>>>(p, bitmap);
+  }
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];  // starts while the check kernel finishes
@@ -277,7 +397,6 @@ cudaError_t launch_mrope(const MropeParams& p, uint32_t* bitmap, size_t bitmap_b
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(p.num_tokens), 1);
   return cudaLaunchKernelEx(&cfg, mrope_append_kernel<E, false>, p);
 }
 
