@@ -67,14 +67,20 @@ IRIS_DEV uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return prmt(prmt(a, b, 0x0040), prmt(c, d, 0x0040), 0x5410);
 }
 
-// One CTA per page (looping), one thread per 8-dim vector of one head; the
-// D / 8 threads of a head are adjacent lanes.  All of the thread's 16 words and
-// 16 scales are asked for before the first is used.  Two nibbles become fp16
-// with two operations, fp32 with one each, two products take one (exact), and
-// two tokens one three-way minimum and maximum: it is these that bound the
-// kernel, not the bytes.
+// A product of two fp16 in fp32: exact, one operation.
+IRIS_DEV float product(__half a, __half b) {
+  float d;
+  asm("fma.rn.f32.f16 %0, %1, %2, %3;" : "=f"(d) : "h"(__half_as_ushort(a)), "h"(__half_as_ushort(b)), "f"(0.0f));
+  return d;
+}
+
+// One CTA per page (looping), one thread per 8 dims of one head; the D / 8
+// threads of a head are adjacent lanes.  All of the thread's 16 words and 16
+// scales are asked for before the first is used.  Two nibbles become
+// fp16 with two operations, a product takes one, and two tokens one three-way
+// minimum and maximum: it is these that bound the kernel, not the bytes.
 template <int D>
-__global__ void __launch_bounds__(256) bounds_kernel(const BoundsParams p) {
+__global__ void __launch_bounds__(256, 3) bounds_kernel(const BoundsParams p) {
   constexpr int V = D / 8;
   const int b = blockIdx.y;
   const int len = __ldg(p.seq_lens + b);
@@ -119,19 +125,18 @@ __global__ void __launch_bounds__(256) bounds_kernel(const BoundsParams p) {
       }
 #pragma unroll
       for (int t = 0; t < kPage; t += 2) {
+        bad = fmaf(__half2float(__ushort_as_half(sh[t])), 0.0f, bad);  // NaN from a scale that is not finite
+        bad = fmaf(__half2float(__ushort_as_half(sh[t + 1])), 0.0f, bad);
         float x[2][8];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float s = __half2float(__ushort_as_half(sh[t + e]));
-          const float2 s2 = make_float2(s, s);
-          bad = fmaf(s, 0.0f, bad);  // NaN from a scale that is not finite
           const uint32_t v = w[t + e], u = v >> 8;
           const uint32_t n[4] = {int4_lo_exact(v), int4_hi_exact(v), int4_lo_exact(u), int4_hi_exact(u)};
+          const __half s = __ushort_as_half(sh[t + e]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {  // dims j and j + 4
-            const float2 y = __fmul2_rn(__half22float2(u32_as_h2(n[j])), s2);
-            x[e][j] = y.x;
-            x[e][j + 4] = y.y;
+            x[e][j] = product(__low2half(u32_as_h2(n[j])), s);
+            x[e][j + 4] = product(__high2half(u32_as_h2(n[j])), s);
           }
         }
 #pragma unroll
@@ -151,38 +156,40 @@ __global__ void __launch_bounds__(256) bounds_kernel(const BoundsParams p) {
       const float unit = finite && step > 0.0f ? step : 1.0f;  // (a head of zeros: lo = hi = 0)
       const float r = __frcp_rn(unit);
       const float kMagic = 12582912.0f;  // 1.5 2^23: a sum's low byte is the rounded value's
-      float zl[8], zh[8];
+      if (!finite) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) lo[j] = -127.0f, hi[j] = 127.0f;
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float a = finite ? quotient(lo[j], unit, r) : -127.0f, c = finite ? quotient(hi[j], unit, r) : 127.0f;
-        zl[j] = __fadd_rd(fminf(fmaxf(a, -127.0f), 127.0f), kMagic);
-        zh[j] = __fadd_ru(fminf(fmaxf(c, -127.0f), 127.0f), kMagic);
+        // (a quotient passes 127 by less than a step: the rounded-outward one is held to it)
+        lo[j] = fmaxf(__fadd_rd(quotient(lo[j], unit, r), kMagic), kMagic - 127.0f);
+        hi[j] = fminf(__fadd_ru(quotient(hi[j], unit, r), kMagic), kMagic + 127.0f);
       }
       if (mine) {
         const int h = i / V, v = i - h * V;
         const int64_t head = page * p.kv_heads + h;
-        uint32_t cl[2], ch[2];
+        const auto bytes = [&](const float (&z)[8]) {
+          uint32_t c[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          cl[j] = low_bytes(__float_as_uint(zl[4 * j]), __float_as_uint(zl[4 * j + 1]), __float_as_uint(zl[4 * j + 2]),
-                            __float_as_uint(zl[4 * j + 3]));
-          ch[j] = low_bytes(__float_as_uint(zh[4 * j]), __float_as_uint(zh[4 * j + 1]), __float_as_uint(zh[4 * j + 2]),
-                            __float_as_uint(zh[4 * j + 3]));
-        }
+          for (int j = 0; j < 2; ++j)
+            c[j] = low_bytes(__float_as_uint(z[4 * j]), __float_as_uint(z[4 * j + 1]), __float_as_uint(z[4 * j + 2]),
+                             __float_as_uint(z[4 * j + 3]));
+          return make_uint2(c[0], c[1]);
+        };
         uint2* out = reinterpret_cast<uint2*>(p.bounds + head * 2 * D) + v;
-        out[0] = make_uint2(cl[0], cl[1]);
-        out[V] = make_uint2(ch[0], ch[1]);
+        out[0] = bytes(lo);
+        out[V] = bytes(hi);
         if (v == 0) p.step[head] = step;
         if (p.values != nullptr) {
-          uint32_t a[4], c[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            a[j] = Fp16Elem::pack((zl[2 * j] - kMagic) * step, (zl[2 * j + 1] - kMagic) * step);
-            c[j] = Fp16Elem::pack((zh[2 * j] - kMagic) * step, (zh[2 * j + 1] - kMagic) * step);
-          }
+          const auto value = [&](const float (&z)[8], int j) {
+            const float2 c = __fadd2_rn(make_float2(z[2 * j], z[2 * j + 1]), make_float2(-kMagic, -kMagic));
+            const float2 x = __fmul2_rn(c, make_float2(step, step));
+            return Fp16Elem::pack(x.x, x.y);
+          };
           uint4* val = reinterpret_cast<uint4*>(p.values + head * 2 * D) + v;
-          val[0] = make_uint4(a[0], a[1], a[2], a[3]);
-          val[V] = make_uint4(c[0], c[1], c[2], c[3]);
+          val[0] = make_uint4(value(lo, 0), value(lo, 1), value(lo, 2), value(lo, 3));
+          val[V] = make_uint4(value(hi, 0), value(hi, 1), value(hi, 2), value(hi, 3));
         }
       }
     }
@@ -208,6 +215,7 @@ struct ScoreParams {
 };
 
 constexpr int kScoreWarps = 8;
+constexpr int kScoreStages = 3;  // units of a warp in flight and in use
 
 // Four adjacent k-steps of m16n8k32 share one 16-byte load a lane: lane t of
 // a quad holds bytes 16 t .. 16 t + 15 of a 64-byte span, words 0 and 1 of
@@ -228,14 +236,28 @@ IRIS_DEV uint32_t ordered(float f) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// kWide: more than 8 query heads a KV head (rows 8 .. 15 of the product).
+// A ring slot: each lane's four 16-byte pieces, then its page's step.
+template <int D>
+constexpr int kSlotBytes = 2 * D / 64 * 512 + 128;
+
+IRIS_DEV void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+IRIS_DEV void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// One CTA a run of octets (8 pages each) of one sequence; its warps share the
+// (KV head, octet) units.  A unit's bounds are a product of 16 rows (query
+// heads) x 8 columns (pages); two units ahead of it are on their way to shared
+// memory.  kWide: more than 8 query heads a KV head (rows 8 .. 15).
 template <typename E, int D, bool kWide>
-__global__ void __launch_bounds__(32 * kScoreWarps) score_kernel(const ScoreParams p) {
-  // codes of the query heads: [head][min(c, 0) : D][max(c, 0) : D], rows padded by 16 bytes
+__global__ void __launch_bounds__(32 * kScoreWarps, 3) score_kernel(const ScoreParams p) {
+  // codes of the query heads: [Hq][min(c, 0) : D][max(c, 0) : D], rows padded by 16 bytes; their units;
+  // the warps' rings
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr int kRow = 2 * D + 16;
   constexpr int kSpans = 2 * D / 64;
-  constexpr int kRows = kWide ? 16 : 8;
   grid_dependents_launch();  // the selection may come up meanwhile
   const int b = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -252,8 +274,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps) score_kernel(const ScorePara
   // units of work: (head, octet), a contiguous run of them for each warp
   const int total = p.kv_heads * octs;
   const int lo = total * warp / kScoreWarps, hi = total * (warp + 1) / kScoreWarps;
-  // Loads run one unit ahead of the products and page numbers two, so that
-  // what a warp waits for is always already asked for.
+  // Page numbers are asked for a unit before the copies that need them.
   const int32_t* table = p.block_table + b * p.table_stride + oct0 * 8 + g;
   const int cols = n - oct0 * 8 - g;  // this lane's pages, one an octet
   const auto page_of = [&](int oct) -> int32_t { return oct * 8 < cols ? __ldg(table + oct * 8) : 0; };
@@ -265,8 +286,11 @@ __global__ void __launch_bounds__(32 * kScoreWarps) score_kernel(const ScorePara
     }
   };
   int32_t page1 = lo < hi ? page_of(oct1) : 0, page2 = 0;  // its pages, and those of the one after it
-  uint4 next[kSpans];
-  float next_step = 0.0f;
+  const int heads = p.kv_heads * p.group;
+  uint8_t* codes = smem;
+  float* units = reinterpret_cast<float*>(smem + heads * kRow);  // [Hq]
+  // A lane copies and reads back its own 16 bytes of each span, so that a slot needs no barrier.
+  uint8_t* ring = smem + (heads * (kRow + 4) + 15) / 16 * 16 + warp * kScoreStages * kSlotBytes<D> + 16 * lane;
   const int8_t* bounds = p.bounds + 16 * t;
   const auto load_unit = [&](int i) {
     if (i < hi) {
@@ -275,10 +299,11 @@ __global__ void __launch_bounds__(32 * kScoreWarps) score_kernel(const ScorePara
         page1 = 0;
       }
       const int64_t row = static_cast<int64_t>(page1) * p.kv_heads + h1;
-      const uint4* src = reinterpret_cast<const uint4*>(bounds + row * 2 * D);
+      const int8_t* src = bounds + row * 2 * D;
+      const uint32_t dst = smem_u32(ring + (i - lo) % kScoreStages * kSlotBytes<D>);
 #pragma unroll
-      for (int k = 0; k < kSpans; ++k) next[k] = __ldg(src + 4 * k);
-      next_step = __ldg(p.step + row);
+      for (int k = 0; k < kSpans; ++k) copy16(dst + 512 * k, src + 64 * k);
+      copy4(dst + 512 * kSpans - 12 * lane, p.step + row);
       advance(h1, oct1);
       page1 = page2;
       if (i + 2 < hi) {
@@ -287,6 +312,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps) score_kernel(const ScorePara
         page2 = page_of(oct2);
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   if (lo + 1 < hi) {
     int h2 = h1, oct2 = oct1;
@@ -294,26 +320,24 @@ __global__ void __launch_bounds__(32 * kScoreWarps) score_kernel(const ScorePara
     page2 = page_of(oct2);
   }
 
-  // Quantise the query heads, four rows of a warp at a time.
-  uint8_t* codes = smem;
-  float* units = reinterpret_cast<float*>(smem + p.kv_heads * kRows * kRow);  // [Hkv][kRows]
+  // the first units' bounds, on their way while the heads are quantised
+#pragma unroll
+  for (int j = 0; j < kScoreStages - 1; ++j) load_unit(lo + j);
+
+  // Quantise the query heads, four of a warp at a time.
   constexpr int W = D / 64;  // words a lane
   constexpr int kAtOnce = 4;
-  bool loaded = false;
-  for (int i0 = warp; i0 < p.kv_heads * kRows; i0 += kAtOnce * kScoreWarps) {
+  for (int i0 = warp; i0 < heads; i0 += kAtOnce * kScoreWarps) {
     uint32_t q[kAtOnce][W];
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
-      const int i = i0 + j * kScoreWarps, h = i / kRows, gg = i % kRows;
-      const bool there = i < p.kv_heads * kRows && gg < p.group;
+      const int i = i0 + j * kScoreWarps;
 #pragma unroll
       for (int k = 0; k < W; ++k)
-        q[j][k] = there ? __ldg(static_cast<const uint32_t*>(p.query) +
-                                ((static_cast<int64_t>(b) * p.kv_heads + h) * p.group + gg) * (D / 2) + lane * W + k)
-                        : 0u;
+        q[j][k] = i < heads ? __ldg(static_cast<const uint32_t*>(p.query) +
+                                    (static_cast<int64_t>(b) * heads + i) * (D / 2) + lane * W + k)
+                            : 0u;
     }
-    if (!loaded) load_unit(lo);  // on its way while the heads are quantised
-    loaded = true;
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
       const int i = i0 + j * kScoreWarps;
@@ -330,21 +354,28 @@ __global__ void __launch_bounds__(32 * kScoreWarps) score_kernel(const ScorePara
       m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
       // a head that is not finite scores every page alike
       const float unit = m <= 3.402823466e38f ? __fdiv_rn(m, 127.0f) : 0.0f;
-      if (i < p.kv_heads * kRows) {
+      if (i < heads) {
+        const bool plain = unit >= 1.0e-30f;  // its reciprocal is an ordinary number
+        const float r = plain ? __frcp_rn(unit) : 0.0f;
+        const auto code = [&](float x) {  // as a float, rounded half to even
+          const float t = plain ? quotient(x, unit, r) : unit > 0.0f ? __fdiv_rn(x, unit) : 0.0f;
+          return __fadd_rn(__fadd_rn(fminf(fmaxf(t, -127.0f), 127.0f), 12582912.0f), -12582912.0f);
+        };
+        const auto byte = [](float c) { return __float_as_uint(c + 12582912.0f); };
 #pragma unroll
         for (int k = 0; k < W; ++k) {
           const float2 f = E::unpack(q[j][k]);
-          const int x = unit > 0.0f ? max(-127, min(127, __float2int_rn(__fdiv_rn(f.x, unit)))) : 0;
-          const int y = unit > 0.0f ? max(-127, min(127, __float2int_rn(__fdiv_rn(f.y, unit)))) : 0;
+          const float x = unit > 0.0f ? code(f.x) : 0.0f, y = unit > 0.0f ? code(f.y) : 0.0f;
           uint8_t* at = codes + i * kRow + 2 * (lane * W + k);
-          *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>((min(x, 0) & 0xff) | (min(y, 0) & 0xff) << 8);
-          *reinterpret_cast<uint16_t*>(at + D) = static_cast<uint16_t>(max(x, 0) | max(y, 0) << 8);
+          *reinterpret_cast<uint16_t*>(at) =
+              static_cast<uint16_t>(prmt(byte(fminf(x, 0.0f)), byte(fminf(y, 0.0f)), 0x0040));
+          *reinterpret_cast<uint16_t*>(at + D) =
+              static_cast<uint16_t>(prmt(byte(fmaxf(x, 0.0f)), byte(fmaxf(y, 0.0f)), 0x0040));
         }
         if (lane == 0) units[i] = unit;
       }
     }
   }
-  if (!loaded) load_unit(lo);  // (a warp without a row)
   __syncthreads();
 
   int head = -1, h = lo / octs, oct = lo - h * octs;
@@ -352,27 +383,32 @@ __global__ void __launch_bounds__(32 * kScoreWarps) score_kernel(const ScorePara
   float u0 = 0.0f, u1 = 0.0f;
   uint32_t* out = p.keys + (static_cast<int64_t>(b) * p.kv_heads + h) * p.key_stride + oct0 * 8 + 2 * t;
   for (int i = lo; i < hi; ++i) {
+    load_unit(i + kScoreStages - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kScoreStages - 1) : "memory");
+    const uint8_t* slot = ring + (i - lo) % kScoreStages * kSlotBytes<D>;
     uint4 w[kSpans];
 #pragma unroll
-    for (int k = 0; k < kSpans; ++k) w[k] = next[k];
-    const float step = next_step;
-    load_unit(i + 1);
+    for (int k = 0; k < kSpans; ++k) w[k] = *reinterpret_cast<const uint4*>(slot + 512 * k);
+    const float step = *reinterpret_cast<const float*>(slot + 512 * kSpans - 12 * lane);
     if (h != head) {
       head = h;
-      const uint8_t* row = codes + (h * kRows + g) * kRow + 16 * t;
+      const uint8_t* row = codes + (h * p.group + g) * kRow + 16 * t;
+      const bool one = g < p.group, two = kWide && g + 8 < p.group;
 #pragma unroll
       for (int k = 0; k < kSpans; ++k) {
-        const uint4 x = *reinterpret_cast<const uint4*>(row + 64 * k);
+        const uint4 x = one ? *reinterpret_cast<const uint4*>(row + 64 * k) : make_uint4(0, 0, 0, 0);
         a[k][0] = x.x, a[k][1] = x.y, a[k][2] = x.z, a[k][3] = x.w;
         if constexpr (kWide) {
-          const uint4 y = *reinterpret_cast<const uint4*>(row + 8 * kRow + 64 * k);
+          const uint4 y = two ? *reinterpret_cast<const uint4*>(row + 8 * kRow + 64 * k) : make_uint4(0, 0, 0, 0);
           a[k][4] = y.x, a[k][5] = y.y, a[k][6] = y.z, a[k][7] = y.w;
         }
       }
-      u0 = units[h * kRows + g];
-      u1 = kWide ? units[h * kRows + g + 8] : 0.0f;
+      u0 = one ? units[h * p.group + g] : 0.0f;
+      u1 = two ? units[h * p.group + g + 8] : 0.0f;
     }
-    int acc[4] = {0, 0, 0, 0};
+    // sums start at the bits of 1.5 2^23, so that their own are a float's: below 2^22, they come out exact
+    constexpr int kStart = 0x4B400000;
+    int acc[4] = {kStart, kStart, kStart, kStart};
 #pragma unroll
     for (int k = 0; k < kSpans; ++k) {
       mma_s8(acc, a[k][0], kWide ? a[k][4] : 0u, a[k][1], kWide ? a[k][5] : 0u, w[k].x, w[k].y);
@@ -380,26 +416,25 @@ __global__ void __launch_bounds__(32 * kScoreWarps) score_kernel(const ScorePara
     }
     // acc: head g (and g + 8), pages 2 t and 2 t + 1 of the octet
     const float s0 = __shfl_sync(0xffffffffu, step, 8 * t), s1 = __shfl_sync(0xffffffffu, step, 8 * t + 4);
+    const auto score = [](int sum, float step, float unit) {
+      return __fmul_rn(__fmul_rn(__int_as_float(sum) - 12582912.0f, step), unit);
+    };
     float m0 = -INFINITY, m1 = -INFINITY;
     if (g < p.group) {
-      m0 = __fmul_rn(__fmul_rn(static_cast<float>(acc[0]), s0), u0);
-      m1 = __fmul_rn(__fmul_rn(static_cast<float>(acc[1]), s1), u0);
+      m0 = score(acc[0], s0, u0);
+      m1 = score(acc[1], s1, u0);
     }
     if (kWide && g + 8 < p.group) {
-      m0 = fmaxf(m0, __fmul_rn(__fmul_rn(static_cast<float>(acc[2]), s0), u1));
-      m1 = fmaxf(m1, __fmul_rn(__fmul_rn(static_cast<float>(acc[3]), s1), u1));
+      m0 = fmaxf(m0, score(acc[2], s0, u1));
+      m1 = fmaxf(m1, score(acc[3], s1, u1));
     }
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
-      m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-      m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-    }
-    if (g == 0) {
-      // a page whose keys are not all finite comes before every other
-      const uint32_t k0 = s0 <= 3.402823466e38f ? ordered(m0) : ordered(INFINITY);
-      const uint32_t k1 = s1 <= 3.402823466e38f ? ordered(m1) : ordered(INFINITY);
-      *reinterpret_cast<uint2*>(out + oct * 8) = make_uint2(k0, k1);
-    }
+    // the maximum over the heads; the first exchange leaves page 2 t to the lanes of even g, 2 t + 1 to the others
+    const bool odd = g & 1;
+    float m = fmaxf(odd ? m1 : m0, __shfl_xor_sync(0xffffffffu, odd ? m0 : m1, 4));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+    // a page whose keys are not all finite comes before every other
+    if (g < 2) out[oct * 8 + g] = (odd ? s1 : s0) <= 3.402823466e38f ? ordered(m) : ordered(INFINITY);
     if (++oct == octs) {
       oct = 0;
       ++h;
@@ -441,10 +476,21 @@ IRIS_DEV SelectRow select_row(const SelectParams& p, int row) {
 IRIS_DEV uint32_t select_key(const SelectParams& p, const SelectRow& r, int i, uint32_t stored) {
   return i >= r.n ? 0u : i < p.sink || i >= r.n - p.recent ? 0xffffffffu : stored;
 }
+IRIS_DEV bool scored(uint32_t key) { return key != 0u && key != 0xffffffffu; }
 
 // The highest `keep` keys are those above a threshold, the largest one that at
 // least `keep` keys reach, and the first of those equal to it.  The threshold
-// is found from its highest bit down by counting.
+// is found bit by bit by counting, from the highest bit in which the scored
+// keys differ at all; a count that hits `keep` ends the search.
+struct Search {
+  uint32_t thr;
+  int bit;  // the next one to decide; -1: none
+};
+IRIS_DEV Search search_from(uint32_t lowest, uint32_t highest) {
+  const uint32_t differ = lowest ^ highest;
+  const int top = differ != 0 ? 31 - __clz(differ) : -1;
+  return {top < 0 ? highest : (highest >> top >> 1) << 1 << top, top};
+}
 
 // One warp per row of up to 32 KPT pages, all keys in registers, KPT
 // consecutive ones a lane: a count is a sum over the warp, no barrier.
@@ -461,7 +507,7 @@ __global__ void __launch_bounds__(128) select_warp_kernel(const SelectParams p) 
     return;
   }
   grid_dependency_wait();  // the scores are there
-  uint32_t k[KPT];
+  uint32_t k[KPT], lowest = 0xffffffffu, highest = 0u;
 #pragma unroll
   for (int j = 0; j < KPT; j += 4) {
     const int i = lane * KPT + j;
@@ -472,21 +518,27 @@ __global__ void __launch_bounds__(128) select_warp_kernel(const SelectParams p) 
     k[j + 2] = select_key(p, r, i + 2, v.z);
     k[j + 3] = select_key(p, r, i + 3, v.w);
   }
-  uint32_t thr = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t cand = thr | 1u << bit;
-    int c = 0;
 #pragma unroll
-    for (int j = 0; j < KPT; ++j) c += k[j] >= cand;
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (c >= r.keep) thr = cand;
-    if (c == r.keep) break;  // exactly the wanted ones reach it
+  for (int j = 0; j < KPT; ++j) {
+    if (scored(k[j])) lowest = min(lowest, k[j]), highest = max(highest, k[j]);
+  }
+  lowest = __reduce_min_sync(0xffffffffu, lowest);
+  highest = __reduce_max_sync(0xffffffffu, highest);
+  Search f = search_from(lowest, highest);
+  for (; f.bit >= 0; --f.bit) {
+    const uint32_t cand = f.thr | 1u << f.bit;
+    int c[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) c[j & 3] += k[j] >= cand;
+    const int all = __reduce_add_sync(0xffffffffu, (c[0] + c[1]) + (c[2] + c[3]));
+    if (all >= r.keep) f.thr = cand;
+    if (all == r.keep) break;  // exactly the wanted ones reach it
   }
   int above = 0, equal = 0;
 #pragma unroll
   for (int j = 0; j < KPT; ++j) {
-    above += k[j] > thr;
-    equal += k[j] == thr;
+    above += k[j] > f.thr;
+    equal += k[j] == f.thr;
   }
   const int need = r.keep - __reduce_add_sync(0xffffffffu, above);
   int a = above, e = equal;  // inclusive sums over the lanes
@@ -498,8 +550,8 @@ __global__ void __launch_bounds__(128) select_warp_kernel(const SelectParams p) 
   int eq = e - equal, at = a - above + min(eq, need);
 #pragma unroll
   for (int j = 0; j < KPT; ++j) {
-    bool take = k[j] > thr;
-    if (k[j] == thr) take = eq++ < need;
+    bool take = k[j] > f.thr;
+    if (k[j] == f.thr) take = eq++ < need;
     if (take) r.out[at++] = lane * KPT + j;
   }
 }
@@ -522,6 +574,7 @@ template <int kThreads, int KPT>
 __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) {
   __shared__ int s_part[6][32];
   __shared__ int s_scan[2][32];
+  __shared__ uint32_t s_range[2][32];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const SelectRow r = select_row(p, row);
   if (tid == 0) p.counts[row] = r.keep;
@@ -556,10 +609,26 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
       for (int j = 0; j < per; ++j) f(tid * per + j, key_at(tid * per + j));
     }
   };
-  uint32_t thr = 0;
+  uint32_t lowest = 0xffffffffu, highest = 0u;
+  const auto widen = [&](uint32_t x) {
+    if (scored(x)) lowest = min(lowest, x), highest = max(highest, x);
+  };
+  if constexpr (KPT > 0) {
+    each([&](int, uint32_t x) { widen(x); });
+  } else {
+    for (int i = tid; i < r.n; i += kThreads) widen(key_at(i));
+  }
+  lowest = __reduce_min_sync(0xffffffffu, lowest);
+  highest = __reduce_max_sync(0xffffffffu, highest);
+  if (lane == 0) s_range[0][warp] = lowest, s_range[1][warp] = highest;
+  __syncthreads();
+  lowest = __reduce_min_sync(0xffffffffu, lane < kThreads / 32 ? s_range[0][lane] : 0xffffffffu);
+  highest = __reduce_max_sync(0xffffffffu, lane < kThreads / 32 ? s_range[1][lane] : 0u);
+  const Search from = search_from(lowest, highest);
+  uint32_t thr = from.thr;
   int slot = 0;
-  for (int bit = 30; bit >= 0; bit -= 2) {
-    const uint32_t c1 = thr | 1u << bit, c2 = thr | 2u << bit, c3 = thr | 3u << bit;
+  for (int bit = from.bit - 1; bit >= -1; bit -= 2) {  // bits bit + 1 and bit (at -1, of bit 0 alone)
+    const uint32_t c2 = thr | 1u << (bit + 1), c1 = bit >= 0 ? thr | 1u << bit : c2, c3 = bit >= 0 ? c2 | 1u << bit : c2;
     int n1 = 0, n2 = 0, n3 = 0;
     if constexpr (KPT > 0) {
       each([&](int, uint32_t x) { n1 += x >= c1, n2 += x >= c2, n3 += x >= c3; });
@@ -579,8 +648,8 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
     n2 = __reduce_add_sync(0xffffffffu, in ? s_part[slot + 1][lane] : 0);
     n3 = __reduce_add_sync(0xffffffffu, in ? s_part[slot + 2][lane] : 0);
     slot = 3 - slot;
-    const int got = n3 >= r.keep ? n3 : n2 >= r.keep ? n2 : n1 >= r.keep ? n1 : 0;
     thr = n3 >= r.keep ? c3 : n2 >= r.keep ? c2 : n1 >= r.keep ? c1 : thr;
+    const int got = n3 >= r.keep ? n3 : n2 >= r.keep ? n2 : n1 >= r.keep ? n1 : 0;
     if (got == r.keep) break;  // exactly the wanted ones reach it
   }
   int above = 0, equal = 0;
@@ -608,17 +677,20 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
   });
 }
 
+// Shared memory of the score kernel.
+int64_t score_bytes(int64_t q_heads, int head_dim) {
+  return (q_heads * (2 * head_dim + 20) + 15) / 16 * 16 +
+         kScoreWarps * kScoreStages * (head_dim == 128 ? kSlotBytes<128> : kSlotBytes<64>);
+}
+
 template <typename E>
 cudaError_t launch_score(const ScoreParams& p, int head_dim, dim3 grid, cudaStream_t s) {
   const bool wide = p.group > 8;
-  const int rows = p.kv_heads * (wide ? 16 : 8);
-  const int bytes = rows * (2 * head_dim + 16) + rows * 4;
+  const int bytes = static_cast<int>(score_bytes(p.kv_heads * p.group, head_dim));
   const auto fn = head_dim == 128 ? (wide ? score_kernel<E, 128, true> : score_kernel<E, 128, false>)
                                   : (wide ? score_kernel<E, 64, true> : score_kernel<E, 64, false>);
-  if (bytes > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return e;
-  }
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
   fn<<<grid, 32 * kScoreWarps, bytes, s>>>(p);
   return cudaGetLastError();
 }
@@ -677,7 +749,7 @@ extern "C" int iris_b200_int4_page_bounds(const void* k_data, const void* k_scal
   const void* ptrs[] = {k_data, k_scale, block_table, seq_lens, bounds, bounds_step};
   for (const void* q : ptrs)
     if (q == nullptr) return IRIS_EINVAL;
-  if (!aligned_to(k_data, 4) || !aligned_to(k_scale, 2) || !aligned_to(bounds, 16) || !aligned_to(bounds_step, 4) ||
+  if (!aligned_to(k_data, 8) || !aligned_to(k_scale, 2) || !aligned_to(bounds, 16) || !aligned_to(bounds_step, 4) ||
       !aligned_to(values, 16))
     return IRIS_EALIGN;
   BoundsParams p = {};
@@ -735,7 +807,7 @@ extern "C" int iris_b200_page_select(const void* query, const void* bounds, cons
   if (dtype != IRIS_DTYPE_FP16 && dtype != IRIS_DTYPE_BF16) return IRIS_EINVAL;
   const int group = num_q_heads / num_kv_heads;
   if (page_size != kPage || (head_dim != 64 && head_dim != 128) || group > 16) return IRIS_EUNSUPPORTED;
-  if (num_kv_heads * (group > 8 ? 16 : 8) * (2 * head_dim + 20) > 200 * 1024) return IRIS_EUNSUPPORTED;
+  if (score_bytes(num_q_heads, head_dim) > 227 * 1024) return IRIS_EUNSUPPORTED;  // 630 query heads of 128 dims
   if (batch == 0) return IRIS_OK;
   if (num_pages == 0) return IRIS_EINVAL;
   if (batch > 65535 || num_kv_heads > 16384 || max_pages_per_seq > (1 << 27)) return IRIS_EUNSUPPORTED;
