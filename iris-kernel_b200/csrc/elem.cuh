@@ -26,6 +26,26 @@ struct Bf16Elem {
 // Signed nibble i (0..7) of a packed word.
 IRIS_DEV int nibble(uint32_t w, int i) { return static_cast<int>(w << (28 - 4 * i)) >> 28; }
 
+// Launches a kernel that may come up while the kernel before it in the stream
+// drains (a programmatic dependent launch).  The kernel calls
+// grid_dependency_wait() before it reads or writes anything; a kernel that
+// itself lets a second one come up early does so after that wait, so that the
+// second one, too, finds what came before both.
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*fn)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fn, static_cast<A&&>(args)...);
+}
+
 inline bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 }  // namespace iris

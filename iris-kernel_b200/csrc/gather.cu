@@ -92,6 +92,7 @@ IRIS_DEV uint4 dequant8(uint32_t w, __half scale) {
 template <typename E>
 __global__ void __launch_bounds__(kThreads) gather_kernel(const GatherParams p) {
   __shared__ int64_t s_row[kTile];
+  grid_dependency_wait();
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kTile;
   const int rows = static_cast<int>(p.num_tokens - n0 < kTile ? p.num_tokens - n0 : kTile);
   if (threadIdx.x < 32) {
@@ -160,11 +161,8 @@ extern "C" int iris_b200_int4_paged_gather(const void* k_data, const void* v_dat
   clear_stale_cuda_error();
   const unsigned blocks = static_cast<unsigned>((num_tokens + kTile - 1) / kTile);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == IRIS_DTYPE_FP16)
-    gather_kernel<Fp16Elem><<<blocks, kThreads, 0, s>>>(p);
-  else
-    gather_kernel<Bf16Elem><<<blocks, kThreads, 0, s>>>(p);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = dtype == IRIS_DTYPE_FP16 ? launch_early(gather_kernel<Fp16Elem>, blocks, kThreads, 0, s, p)
+                                                 : launch_early(gather_kernel<Bf16Elem>, blocks, kThreads, 0, s, p);
   if (e != cudaSuccess) {
     record_cuda_error(e, "gather_kernel launch");
     return IRIS_ECUDA;

@@ -72,7 +72,8 @@ IRIS_DEV int32_t token_bits(const MropeParams& p, int32_t slot, int64_t tok) {
 // Validation of a large batch before the append: ranges, and one bit per slot
 // for duplicates.  The append's launch overlaps it.
 __global__ void __launch_bounds__(kThreads) mrope_check_kernel(const MropeParams p, uint32_t* __restrict__ bitmap) {
-  grid_dependents_launch();
+  grid_dependency_wait();
+  grid_dependents_launch();  // the append may come up meanwhile
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (i >= p.num_tokens) return;
   const int32_t slot = __ldg(p.slots + i);
@@ -91,7 +92,8 @@ __global__ void __launch_bounds__(kThreads) mrope_check_kernel(const MropeParams
 constexpr int64_t kPairwiseTokens = 2048;
 __global__ void __launch_bounds__(kThreads) mrope_check_pairs_kernel(const MropeParams p) {
   __shared__ __align__(16) int32_t s_slot[kPairwiseTokens];
-  grid_dependents_launch();
+  grid_dependency_wait();
+  grid_dependents_launch();  // the append may come up meanwhile
   const int T = static_cast<int>(p.num_tokens), T4 = (T + 3) & ~3;
   for (int i = threadIdx.x; i < T4; i += kThreads) s_slot[i] = i < T ? __ldg(p.slots + i) : -1;
   const int i = (blockIdx.x * kThreads + threadIdx.x) >> 3, part = threadIdx.x & 7;
@@ -243,6 +245,7 @@ IRIS_DEV uint32_t quant8(const float2 (&x)[4], uint32_t quad, __half& scale16) {
 // registers 85 us, 128 102 us (each with the 15 us of its check and read back).
 template <typename E, bool kSmall>
 __global__ void __launch_bounds__(kThreads, kSmall ? 2 : 4) mrope_append_kernel(const MropeParams p) {
+  if constexpr (kSmall) grid_dependency_wait();
   constexpr int kBatch = 2;  // heads whose vectors a thread has on the way, of each kind
   const int per_token = p.row_lanes * p.vecs;
   const int here = threadIdx.x / per_token, in_token = threadIdx.x - here * per_token;
@@ -369,35 +372,28 @@ __global__ void __launch_bounds__(kThreads, kSmall ? 2 : 4) mrope_append_kernel(
 
 template <typename E>
 cudaError_t launch_mrope(MropeParams& p, uint32_t* bitmap, size_t bitmap_bytes, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.stream = stream;
   if (p.num_tokens <= kInlineCheckTokens) {  // few tokens: as many threads on each as fit
     p.row_lanes = kThreads / p.vecs;
-    cfg.blockDim = dim3(p.row_lanes * p.vecs);
-    cfg.gridDim = dim3(static_cast<unsigned>(p.num_tokens));
-    return cudaLaunchKernelEx(&cfg, mrope_append_kernel<E, true>, p);
+    return launch_early(mrope_append_kernel<E, true>, static_cast<unsigned>(p.num_tokens), p.row_lanes * p.vecs, 0,
+                        stream, p);
   }
   // many: few threads a token, so that each blended row serves many heads
   p.row_lanes = 4;
   const int tokens = kThreads / (4 * p.vecs);  // a CTA
-  cfg.blockDim = dim3(tokens * 4 * p.vecs);
-  cfg.gridDim = dim3(static_cast<unsigned>((p.num_tokens + tokens - 1) / tokens));
   cudaError_t e = cudaSuccess;
   if (p.num_tokens <= kPairwiseTokens) {
-    mrope_check_pairs_kernel<<<static_cast<unsigned>((8 * p.num_tokens + kThreads - 1) / kThreads), kThreads, 0, stream>>>(p);
+    e = launch_early(mrope_check_pairs_kernel, static_cast<unsigned>((8 * p.num_tokens + kThreads - 1) / kThreads),
+                     kThreads, 0, stream, p);
   } else {
     if (bitmap_bytes > 0) e = cudaMemsetAsync(bitmap, 0, bitmap_bytes, stream);
-    if (e != cudaSuccess) return e;
-    mrope_check_kernel<<<static_cast<unsigned>((p.num_tokens + kThreads - 1) / kThreads), kThreads, 0, stream>>>(p, bitmap);
+    if (e == cudaSuccess)
+      e = launch_early(mrope_check_kernel, static_cast<unsigned>((p.num_tokens + kThreads - 1) / kThreads), kThreads, 0,
+                       stream, p, bitmap);
   }
-  e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  cudaLaunchAttribute attr[1];  // starts while the check kernel finishes
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, mrope_append_kernel<E, false>, p);
+  // comes up while the check finishes
+  return launch_early(mrope_append_kernel<E, false>, static_cast<unsigned>((p.num_tokens + tokens - 1) / tokens),
+                      tokens * 4 * p.vecs, 0, stream, p);
 }
 
 }  // namespace

@@ -82,6 +82,7 @@ IRIS_DEV float product(__half a, __half b) {
 template <int D>
 __global__ void __launch_bounds__(256, 3) bounds_kernel(const BoundsParams p) {
   constexpr int V = D / 8;
+  grid_dependency_wait();
   const int b = blockIdx.y;
   const int len = __ldg(p.seq_lens + b);
   if (len <= 0) {
@@ -258,6 +259,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 3) score_kernel(const ScoreP
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr int kRow = 2 * D + 16;
   constexpr int kSpans = 2 * D / 64;
+  grid_dependency_wait();
   grid_dependents_launch();  // the selection may come up meanwhile
   const int b = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -691,33 +693,18 @@ cudaError_t launch_score(const ScoreParams& p, int head_dim, dim3 grid, cudaStre
                                   : (wide ? score_kernel<E, 64, true> : score_kernel<E, 64, false>);
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
-  fn<<<grid, 32 * kScoreWarps, bytes, s>>>(p);
-  return cudaGetLastError();
-}
-
-template <typename F>
-cudaError_t launch_after_scores(F* fn, unsigned blocks, unsigned threads, const SelectParams& p, cudaStream_t s) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(threads);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fn, p);
+  return launch_early(fn, grid, dim3(32 * kScoreWarps), static_cast<size_t>(bytes), s, p);
 }
 
 cudaError_t launch_select(const SelectParams& p, cudaStream_t s) {
   const unsigned rows = static_cast<unsigned>(p.rows), fours = (rows + 3) / 4;
-  if (p.max_pages <= 256) return launch_after_scores(select_warp_kernel<8>, fours, 128, p, s);
-  if (p.max_pages <= 512) return launch_after_scores(select_kernel<64, 8>, rows, 64, p, s);
-  if (p.max_pages <= 1024) return launch_after_scores(select_kernel<128, 8>, rows, 128, p, s);
-  if (p.max_pages <= 2048) return launch_after_scores(select_kernel<256, 8>, rows, 256, p, s);
-  if (p.max_pages <= 8192) return launch_after_scores(select_kernel<1024, 8>, rows, 1024, p, s);
-  if (p.max_pages <= 32768) return launch_after_scores(select_kernel<1024, 32>, rows, 1024, p, s);
-  return launch_after_scores(select_kernel<1024, 0>, rows, 1024, p, s);
+  if (p.max_pages <= 256) return launch_early(select_warp_kernel<8>, fours, 128, 0, s, p);
+  if (p.max_pages <= 512) return launch_early(select_kernel<64, 8>, rows, 64, 0, s, p);
+  if (p.max_pages <= 1024) return launch_early(select_kernel<128, 8>, rows, 128, 0, s, p);
+  if (p.max_pages <= 2048) return launch_early(select_kernel<256, 8>, rows, 256, 0, s, p);
+  if (p.max_pages <= 8192) return launch_early(select_kernel<1024, 8>, rows, 1024, 0, s, p);
+  if (p.max_pages <= 32768) return launch_early(select_kernel<1024, 32>, rows, 1024, 0, s, p);
+  return launch_early(select_kernel<1024, 0>, rows, 1024, 0, s, p);
 }
 
 int sm_count() {
@@ -774,11 +761,8 @@ extern "C" int iris_b200_int4_page_bounds(const void* k_data, const void* k_scal
   if (x < 1) x = 1;
   const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(batch));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128)
-    bounds_kernel<128><<<grid, threads, 0, s>>>(p);
-  else
-    bounds_kernel<64><<<grid, threads, 0, s>>>(p);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_early(head_dim == 128 ? bounds_kernel<128> : bounds_kernel<64>, grid,
+                                     dim3(static_cast<unsigned>(threads)), 0, s, p);
   if (e != cudaSuccess) {
     record_cuda_error(e, "bounds_kernel launch");
     return IRIS_ECUDA;

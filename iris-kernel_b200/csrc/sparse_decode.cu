@@ -17,8 +17,8 @@
 //   S = Q K^T      rows = query heads, columns = tokens, one accumulator per
 //                  32-dim group, the group scale applied in fp32.  A nibble n
 //                  enters as the subnormal fp16 (n + 8) 2^-24, one logic
-//                  operation for two; the accumulator starts at -8 sum(q)
-//                  2^-24.  Each query head is scaled by a power of two to a
+//                  operation for two; -8 sum(q) 2^-24 is added to the
+//                  group's sum.  Each query head is scaled by a power of two to a
 //                  largest value in [1, 2) and put back in the logits' scale:
 //                  exact but for elements 2^-14 below its largest.
 //   O^T = V^T P^T  rows = dims, columns = query heads; V as exact integers; a
@@ -71,6 +71,7 @@ struct SparseParams {
   int32_t keep;
   int32_t rows;       // B * Hkv
   int32_t min_steps;  // shortest run of a warp
+  int32_t warps;
   int32_t vector_counts;  // counts is 16-byte aligned
   float* part_o;      // [2 * warps][group][D]
   float* part_ml;     // [2 * warps][group][2]
@@ -99,6 +100,13 @@ IRIS_DEV void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32
       "{%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
+IRIS_DEV void mma_f16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // Four 8 x 8 matrices of 16-bit elements (rows of 16 bytes); lane L gives row
@@ -148,10 +156,10 @@ IRIS_DEV Place locate(const SparseParams& p, F&& run_of) {
   const int per = (p.rows + 127) / 128 * 4;  // consecutive rows a lane, in fours
   const auto clamped = [&](int c) { return (min(max(c, 0), p.keep) + 1) >> 1; };
   int sum = 0;
-  for (int i = 0; i < per; i += 16) {  // up to four loads in flight
-    int4 c[4];
+  for (int i = 0; i < per; i += 64) {  // up to sixteen loads in flight
+    int4 c[16];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 16; ++j) {
       const int r = lane * per + i + 4 * j;
       c[j] = make_int4(0, 0, 0, 0);
       if (i + 4 * j < per && r < p.rows) {
@@ -166,7 +174,7 @@ IRIS_DEV Place locate(const SparseParams& p, F&& run_of) {
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum += clamped(c[j].x) + clamped(c[j].y) + clamped(c[j].z) + clamped(c[j].w);
+    for (int j = 0; j < 16; ++j) sum += clamped(c[j].x) + clamped(c[j].y) + clamped(c[j].z) + clamped(c[j].w);
   }
   const int upto = warp_scan(sum);
   Place out;
@@ -226,19 +234,20 @@ struct SlotInfo {
 };
 
 template <typename E, int D, bool kWide>
-__global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse_decode_kernel(const SparseParams p) {
+__global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse_decode_kernel(SparseParams p) {
   using C = SparseCfg<D>;
   constexpr int G4 = C::kGroups;
   constexpr int kH = kWide ? 2 : 1;  // query heads a lane has logits of: g, g + 8
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int me = blockIdx.x * kWarps + warp, warps = gridDim.x * kWarps;
-  grid_dependents_launch();
+  const int me = blockIdx.x * kWarps + warp;
+  grid_dependency_wait();
+  grid_dependents_launch();  // the joining kernel may come up meanwhile
   const Place first = locate(p, [&](int total) {
-    return min(static_cast<int64_t>(me) * run_length(p, total, warps), static_cast<int64_t>(total));
+    return min(static_cast<int64_t>(me) * run_length(p, total, p.warps), static_cast<int64_t>(total));
   });
-  const int length = run_length(p, first.total, warps);
+  const int length = run_length(p, first.total, p.warps);
   if (me == 0 && lane == 0) p.row_start[p.rows] = length;
   if (first.row < 0) return;  // (nothing below waits for another warp)
   const int begin = me * length, end = min(begin + length, first.total);  // below 2^30 + the run
@@ -249,9 +258,9 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
   const uint32_t ring_addr = smem_u32(ring);
 
   // ---- copies: pages of 16 steps are looked up at a time, a page a lane ----
-  int32_t my_page = -1;
+  int64_t my_off = -1;  // bytes from k_data to the head's share of the page; -1: nothing there
   SlotInfo my_info = {0, 0};
-  int my_head = 0;
+  const uint32_t row_bytes = static_cast<uint32_t>(p.kv_heads) * (D / 2);
   int seek_row = first.row, seek_start = first.start;  // the row of the next step to look up, or an earlier one
   const auto look_up = [&](int step) {
     const int u = min(step + (lane >> 1), end - 1);
@@ -265,9 +274,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
     const int entry = 2 * (u - start) + (lane & 1);
     const int b = row / p.kv_heads;
     const int len = __ldg(p.seq_lens + b);
-    my_page = -1;
+    my_off = -1;
     my_info = {row, 0};
-    my_head = row - b * p.kv_heads;
     if (entry >= min(__ldg(p.counts + row), p.keep)) return;
     const int col = __ldg(p.lists + static_cast<int64_t>(row) * p.keep + entry);
     if (col < 0 || static_cast<int64_t>(col) * kPage >= len) return;
@@ -280,12 +288,11 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
       set_error(p.err, IRIS_ERR_PAGE_ID);
       return;
     }
-    my_page = page;
+    my_off = static_cast<int64_t>(page) * (kPage * static_cast<int64_t>(row_bytes)) + (row - b * p.kv_heads) * (D / 2);
     my_info.left = len - col * kPage;
   };
   // this lane's chunks of any page: row lane / kChunks (and 8 below it for D = 128), and one row's scales
   const int r0 = lane / C::kChunks, c0 = lane % C::kChunks;
-  const uint32_t row_bytes = static_cast<uint32_t>(p.kv_heads) * (D / 2);
   const uint32_t data_off = r0 * row_bytes + 16 * c0;
   const uint8_t* k_src = p.k_data + data_off;
   const uint8_t* v_src = p.v_data + data_off;
@@ -293,34 +300,36 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
                          static_cast<uint32_t>(lane & 15) * p.kv_heads * (2 * G4);
   const uint32_t dst0 = chunk_at<D>(r0, c0);
   const uint32_t s_dst = 2 * C::kData + (lane >> 4) * C::kScale + (lane & 15) * 2 * G4;
-  // starts the copies of a step's two pages, as far as there are any
-  const auto fetch = [&](int step) {
-    if (step < end) {
-      const int at = (step - begin) & 15;
-      if (at == 0) look_up(step);
-      const int slot = 2 * ((step - begin) % kStages);
-      if ((lane >> 1) == at) info[slot + (lane & 1)] = my_info;
+  const uint8_t* k_low = k_src + 8 * row_bytes;
+  const uint8_t* v_low = v_src + 8 * row_bytes;
+  // starts the copies of the next step's two pages, as far as there are any
+  int ahead = 0, fill = 0;  // steps asked for, and the slot pair of the next one
+  const auto fetch = [&]() {
+    if (begin + ahead < end) {
+      const int at = ahead & 15;
+      if (at == 0) look_up(begin + ahead);
+      if ((lane >> 1) == at) info[2 * fill + (lane & 1)] = my_info;
 #pragma unroll
       for (int pg = 0; pg < 2; ++pg) {
-        const int32_t page = __shfl_sync(0xffffffffu, my_page, 2 * at + pg);
-        const int32_t head = __shfl_sync(0xffffffffu, my_head, 2 * at + pg);
-        if (page >= 0) {
-          const uint32_t st = ring_addr + (slot + pg) * C::kStage;
-          const uint64_t off = static_cast<uint64_t>(static_cast<uint32_t>(page)) * (kPage * row_bytes) + head * (D / 2);
+        const int64_t off = __shfl_sync(0xffffffffu, my_off, 2 * at + pg);
+        if (off >= 0) {
+          const uint32_t st = ring_addr + (2 * fill + pg) * C::kStage;
           cp_async16(st + dst0, k_src + off);
           cp_async16(st + C::kData + dst0, v_src + off);
           if constexpr (D == 128) {
-            cp_async16(st + dst0 + C::kData / 2, k_src + off + 8 * row_bytes);
-            cp_async16(st + C::kData + dst0 + C::kData / 2, v_src + off + 8 * row_bytes);
+            cp_async16(st + dst0 + C::kData / 2, k_low + off);
+            cp_async16(st + C::kData + dst0 + C::kData / 2, v_low + off);
           }
           cp_async_small<2 * G4>(st + s_dst, s_src + (off >> 3));
         }
       }
     }
     cp_async_commit();
+    ++ahead;
+    fill = fill + 1 == kStages ? 0 : fill + 1;
   };
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch(begin + i);
+  for (int i = 0; i < kStages - 1; ++i) fetch();
 
   // ---- state of the row at hand ----
   constexpr int kTiles = D / 16;  // of 16 dims; a lane has two dims of each for heads 2 t, 2 t + 1 (+ 8)
@@ -447,12 +456,13 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
     return k % 2 == 0 ? make_float2(a.x, c.x) : make_float2(a.y, c.y);
   };
 
+  int slot = -2;
   for (int step = begin; step < end; ++step) {
     __syncwarp();  // every lane is done with the slots that are filled next
-    fetch(step + kStages - 1);
+    fetch();
     cp_async_wait<kStages - 1>();
     __syncwarp();
-    const int slot = 2 * ((step - begin) % kStages);
+    slot = slot + 2 == kSlots ? 0 : slot + 2;
     const SlotInfo i0 = info[slot], i1 = info[slot + 1];
     if (i0.row != cur) {
       if (cur >= 0) {
@@ -482,20 +492,19 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
         for (int k = k0; k < k0 + 2; ++k) {
           const uint4 q0 = s_query[k * 32 + lane], q1 = kWide ? s_query[(G4 + k) * 32 + lane] : make_uint4(0, 0, 0, 0);
           const uint32_t a0[4] = {q0.x, q1.x, q0.y, q1.y}, a1[4] = {q0.z, q1.z, q0.w, q1.w};
-          const float init[4] = {q_sum[0][k], q_sum[0][k], kWide ? q_sum[kH - 1][k] : 0.0f,
-                                 kWide ? q_sum[kH - 1][k] : 0.0f};
 #pragma unroll
           for (int pg = 0; pg < 2; ++pg) {
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
               const uint32_t w = kw[pg][2 * (k - k0) + n], v = w >> 8;
               float acc[4];
-              mma_f16(acc, a0, offset_lo(w), offset_lo(v), init);
+              mma_f16_zero(acc, a0, offset_lo(w), offset_lo(v));
               mma_f16(acc, a1, offset_hi(w), offset_hi(v), acc);
               const float2 sc = scale_pair(ks[pg][n], k);
 #pragma unroll
               for (int hh = 0; hh < kH; ++hh) {
-                const float2 a = make_float2(acc[2 * hh], acc[2 * hh + 1]);
+                const float2 a = __fadd2_rn(make_float2(acc[2 * hh], acc[2 * hh + 1]),
+                                            make_float2(q_sum[hh][k], q_sum[hh][k]));
                 x[hh][pg][n] = k == 0 ? __fmul2_rn(a, sc) : __ffma2_rn(a, sc, x[hh][pg][n]);
               }
             }
@@ -627,13 +636,27 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
 // Joins the parts of the rows that no single warp had, one warp per query head;
 // rows without a step are written here too.
 template <typename E, int D>
-__global__ void __launch_bounds__(128) sparse_join_kernel(const SparseParams p) {
+__global__ void __launch_bounds__(128) sparse_join_kernel(SparseParams p) {
   constexpr int kPer = D / 32;   // dims a lane
   constexpr int kAhead = 8;      // parts loaded at a time
   using Vec = std::conditional_t<kPer == 4, float4, float2>;
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5);
   const int n = steps_of(p, row);
+  // The row's first step and the length of a run: with few rows from the counts, while the runs finish; otherwise
+  // from what they wrote down.
+  const bool few = p.rows <= 256;
+  int start = 0, length = 1;
+  if (few) {
+    int before = 0, all = 0;
+    for (int r = lane; r < p.rows; r += 32) {
+      const int x = steps_of(p, r);
+      all += x;
+      before += r < row ? x : 0;
+    }
+    start = __reduce_add_sync(0xffffffffu, before);
+    length = run_length(p, __reduce_add_sync(0xffffffffu, all), p.warps);
+  }
   if (head == 0 && lane == 0 && __ldg(p.seq_lens + row / p.kv_heads) < 0) set_error(p.err, IRIS_ERR_SEQ_LEN);
   grid_dependency_wait();
   if (head >= p.group) return;
@@ -643,7 +666,10 @@ __global__ void __launch_bounds__(128) sparse_join_kernel(const SparseParams p) 
   for (int j = 0; j < kPer; ++j) acc[j] = 0.0f;
   float top = -INFINITY, sum = 0.0f;
   if (n > 0) {
-    const int start = __ldcg(p.row_start + row), length = __ldcg(p.row_start + p.rows);
+    if (!few) {
+      start = __ldcg(p.row_start + row);
+      length = __ldcg(p.row_start + p.rows);
+    }
     const int first = start / length, parts = (start + n - 1) / length - first + 1;
     if (parts == 1) return;  // its warp wrote the outputs
     const auto part_at = [&](int i) {
@@ -716,15 +742,15 @@ cudaError_t resident_warps(const void* fn, int bytes, int* out) {
   return cudaSuccess;
 }
 
+using KernelFn = void (*)(SparseParams);
 struct Kernel {
-  const void* fn;
-  const void* join;
+  KernelFn fn;
+  KernelFn join;
   int bytes;  // of shared memory
 };
 template <typename E, int D, bool kWide>
 Kernel kernel() {
-  return {reinterpret_cast<const void*>(sparse_decode_kernel<E, D, kWide>),
-          reinterpret_cast<const void*>(sparse_join_kernel<E, D>), kWarps * kWarpBytes<D, kWide>};
+  return {sparse_decode_kernel<E, D, kWide>, sparse_join_kernel<E, D>, kWarps * kWarpBytes<D, kWide>};
 }
 Kernel kernel_for(int dtype, int head_dim, bool wide) {
   if (dtype == IRIS_DTYPE_FP16) {
@@ -742,7 +768,7 @@ struct SparseGrid {
 cudaError_t grid_for(const Kernel& k, int64_t rows, int group, int head_dim, int64_t max_pages, int min_steps,
                      SparseGrid* out) {
   int resident = 0;
-  const cudaError_t e = resident_warps(k.fn, k.bytes, &resident);
+  const cudaError_t e = resident_warps(reinterpret_cast<const void*>(k.fn), k.bytes, &resident);
   if (e != cudaSuccess) return e;
   const int64_t runs = (rows * ((max_pages + 1) / 2) + min_steps - 1) / min_steps;  // at most
   const int64_t warps = runs < resident ? runs : resident;
@@ -843,6 +869,7 @@ extern "C" int iris_b200_int4_sparse_paged_decode(const void* query, const void*
   p.keep = max_pages;
   p.rows = static_cast<int32_t>(rows);
   p.min_steps = kMinSteps;
+  p.warps = grid.ctas * kWarps;
   p.vector_counts = aligned_to(page_count, 16) ? 1 : 0;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.row_start = reinterpret_cast<int32_t*>(ws);
@@ -850,24 +877,10 @@ extern "C" int iris_b200_int4_sparse_paged_decode(const void* query, const void*
   p.part_ml = reinterpret_cast<float*>(ws + grid.part_ml);
   p.scale_log2 = static_cast<float>(static_cast<double>(softmax_scale) * 1.4426950408889634);
   p.err = error_word;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid.ctas));
-  cfg.blockDim = dim3(32 * kWarps);
-  cfg.dynamicSmemBytes = static_cast<size_t>(k.bytes);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  void* args[] = {&p};
-  e = cudaLaunchKernelExC(&cfg, k.fn, args);
-  if (e == cudaSuccess) {  // starts while the runs finish
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(rows), static_cast<unsigned>((group + 3) / 4));
-    cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = 0;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelExC(&cfg, k.join, args);
-  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  e = launch_early(k.fn, static_cast<unsigned>(grid.ctas), 32 * kWarps, static_cast<size_t>(k.bytes), s, p);
+  if (e == cudaSuccess)
+    e = launch_early(k.join, dim3(static_cast<unsigned>(rows), static_cast<unsigned>((group + 3) / 4)), 128, 0, s, p);
   if (e != cudaSuccess) {
     record_cuda_error(e, "sparse_decode_kernel launch");
     return IRIS_ECUDA;
