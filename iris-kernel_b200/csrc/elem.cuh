@@ -32,18 +32,27 @@ IRIS_DEV int nibble(uint32_t w, int i) { return static_cast<int>(w << (28 - 4 * 
 // itself lets a second one come up early does so after that wait, so that the
 // second one, too, finds what came before both.
 template <typename... P, typename... A>
-cudaError_t launch_early(void (*fn)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
-  cudaLaunchAttribute attr[1];
+cudaError_t launch_early_clusters(void (*fn)(P...), dim3 grid, dim3 block, unsigned cluster, size_t smem,
+                                  cudaStream_t stream, A&&... args) {
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, fn, static_cast<A&&>(args)...);
+}
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*fn)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
+  return launch_early_clusters(fn, grid, block, 1, smem, stream, static_cast<A&&>(args)...);
 }
 
 inline bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }

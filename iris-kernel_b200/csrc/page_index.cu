@@ -210,7 +210,8 @@ struct ScoreParams {
   int64_t num_pages;
   int32_t max_pages;
   int32_t kv_heads, group;
-  int32_t octets;  // 8-page groups per CTA
+  int32_t octets;        // 8-page groups per CTA
+  int32_t cta_heads;     // KV heads per CTA
   int32_t max_keep;
   int32_t* err;
 };
@@ -248,8 +249,8 @@ IRIS_DEV void copy4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// One CTA a run of octets (8 pages each) of one sequence; its warps share the
-// (KV head, octet) units.  A unit's bounds are a product of 16 rows (query
+// One CTA a run of octets (8 pages each) of one sequence and some of its KV
+// heads; its warps share the (KV head, octet) units.  A unit's bounds are a product of 16 rows (query
 // heads) x 8 columns (pages); two units ahead of it are on their way to shared
 // memory.  kWide: more than 8 query heads a KV head (rows 8 .. 15).
 template <typename E, int D, bool kWide>
@@ -264,7 +265,8 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 3) score_kernel(const ScoreP
   const int b = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int len = __ldg(p.seq_lens + b);
-  const bool first = blockIdx.x == 0 && threadIdx.x == 0;
+  const int head0 = blockIdx.z * p.cta_heads;  // this CTA's first KV head
+  const bool first = blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0;
   if (len < 0 && first) set_error(p.err, IRIS_ERR_SEQ_LEN);
   const int64_t all = len > 0 ? (static_cast<int64_t>(len) + kPage - 1) / kPage : 0;
   if (all > p.max_pages && first) set_error(p.err, IRIS_ERR_BLOCK_TABLE);
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 3) score_kernel(const ScoreP
   const int g = lane >> 2, t = lane & 3;
   const int octs = min(p.octets, (n + 7) / 8 - oct0);
   // units of work: (head, octet), a contiguous run of them for each warp
-  const int total = p.kv_heads * octs;
+  const int total = p.cta_heads * octs;
   const int lo = total * warp / kScoreWarps, hi = total * (warp + 1) / kScoreWarps;
   // Page numbers are asked for a unit before the copies that need them.
   const int32_t* table = p.block_table + b * p.table_stride + oct0 * 8 + g;
@@ -288,7 +290,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 3) score_kernel(const ScoreP
     }
   };
   int32_t page1 = lo < hi ? page_of(oct1) : 0, page2 = 0;  // its pages, and those of the one after it
-  const int heads = p.kv_heads * p.group;
+  const int heads = p.cta_heads * p.group;
   uint8_t* codes = smem;
   float* units = reinterpret_cast<float*>(smem + heads * kRow);  // [Hq]
   // A lane copies and reads back its own 16 bytes of each span, so that a slot needs no barrier.
@@ -300,7 +302,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 3) score_kernel(const ScoreP
         set_error(p.err, IRIS_ERR_PAGE_ID);
         page1 = 0;
       }
-      const int64_t row = static_cast<int64_t>(page1) * p.kv_heads + h1;
+      const int64_t row = static_cast<int64_t>(page1) * p.kv_heads + head0 + h1;
       const int8_t* src = bounds + row * 2 * D;
       const uint32_t dst = smem_u32(ring + (i - lo) % kScoreStages * kSlotBytes<D>);
 #pragma unroll
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 3) score_kernel(const ScoreP
 #pragma unroll
       for (int k = 0; k < W; ++k)
         q[j][k] = i < heads ? __ldg(static_cast<const uint32_t*>(p.query) +
-                                    (static_cast<int64_t>(b) * heads + i) * (D / 2) + lane * W + k)
+                                    ((static_cast<int64_t>(b) * p.kv_heads + head0) * p.group + i) * (D / 2) + lane * W + k)
                             : 0u;
     }
 #pragma unroll
@@ -383,7 +385,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 3) score_kernel(const ScoreP
   int head = -1, h = lo / octs, oct = lo - h * octs;
   uint32_t a[kSpans][kWide ? 8 : 4];
   float u0 = 0.0f, u1 = 0.0f;
-  uint32_t* out = p.keys + (static_cast<int64_t>(b) * p.kv_heads + h) * p.key_stride + oct0 * 8 + 2 * t;
+  uint32_t* out = p.keys + (static_cast<int64_t>(b) * p.kv_heads + head0 + h) * p.key_stride + oct0 * 8 + 2 * t;
   for (int i = lo; i < hi; ++i) {
     load_unit(i + kScoreStages - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(kScoreStages - 1) : "memory");
@@ -558,33 +560,70 @@ __global__ void __launch_bounds__(128) select_warp_kernel(const SelectParams p) 
   }
 }
 
-// Sums over the CTA, in every thread.  `slot` alternates between calls so that
-// one barrier a call is enough.
-template <int kThreads>
-IRIS_DEV int block_sum(int v, int (*part)[32], int slot) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  const int lane = threadIdx.x & 31;
-  if (lane == 0) part[slot][threadIdx.x >> 5] = v;
-  __syncthreads();
-  return __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? part[slot][lane] : 0);
-}
+// What the warps of a row tell one another: an array entry a warp, in the
+// shared memory of each of the row's CTAs.  put() leaves a warp's value there,
+// meet() waits for all warps' (every CTA of a cluster comes to it), and then
+// any warp sums the entries, or those of the warps before it.
+template <int kThreads, int kCtas>
+struct Board {
+  static constexpr int kPerCta = kThreads / 32, kEntries = kCtas * kPerCta;
+  IRIS_DEV static int rank() {
+    if constexpr (kCtas == 1) return 0;
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return static_cast<int>(r);
+  }
+  IRIS_DEV static int entry() { return rank() * kPerCta + (threadIdx.x >> 5); }
+  IRIS_DEV static void put(uint32_t* board, uint32_t v) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (kCtas == 1) {
+      if (lane == 0) board[entry()] = v;
+    } else if (lane < kCtas) {
+      uint32_t to;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(board + entry())), "r"(lane));
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(v) : "memory");
+    }
+  }
+  IRIS_DEV static void meet() {
+    if constexpr (kCtas == 1) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  }
+  // sum of the first `n` entries, in every lane
+  IRIS_DEV static int sum(const uint32_t* board, int n = kEntries) {
+    uint32_t v = 0;
+    for (int i = threadIdx.x & 31; i < n; i += 32) v += board[i];
+    return static_cast<int>(__reduce_add_sync(0xffffffffu, v));
+  }
+  IRIS_DEV static uint32_t lowest(const uint32_t* board) {
+    uint32_t v = 0xffffffffu;
+    for (int i = threadIdx.x & 31; i < kEntries; i += 32) v = min(v, board[i]);
+    return __reduce_min_sync(0xffffffffu, v);
+  }
+  IRIS_DEV static uint32_t highest(const uint32_t* board) {
+    uint32_t v = 0;
+    for (int i = threadIdx.x & 31; i < kEntries; i += 32) v = max(v, board[i]);
+    return __reduce_max_sync(0xffffffffu, v);
+  }
+};
 
-// One CTA per longer row: KPT consecutive keys a thread in registers, or for
-// KPT = 0 read again for every count.  Two bits of the threshold at a time,
-// which halves the barriers.
-template <int kThreads, int KPT>
+// kCtas CTAs (a cluster) per longer row: KPT consecutive keys a thread in
+// registers, or for KPT = 0 read again for every count.  Two bits of the
+// threshold at a time, which halves the barriers.  Counting is what takes the
+// time, so that a row of one long sequence goes over several SMs.
+template <int kThreads, int KPT, int kCtas>
 __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) {
-  __shared__ int s_part[6][32];
-  __shared__ int s_scan[2][32];
-  __shared__ uint32_t s_range[2][32];
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  using B = Board<kThreads, kCtas>;
+  __shared__ uint32_t s_part[6][B::kEntries];
+  __shared__ uint32_t s_more[4][B::kEntries];
+  constexpr int kAll = kThreads * kCtas;
+  const int row = blockIdx.x / kCtas, tid = B::rank() * kThreads + threadIdx.x, lane = threadIdx.x & 31;
   const SelectRow r = select_row(p, row);
   if (tid == 0) p.counts[row] = r.keep;
-  for (int i = r.keep + tid; i < p.keep; i += kThreads) r.out[i] = -1;
+  for (int i = r.keep + tid; i < p.keep; i += kAll) r.out[i] = -1;
   if (r.n <= p.keep) {
-    for (int i = tid; i < r.n; i += kThreads) r.out[i] = i;
+    for (int i = tid; i < r.n; i += kAll) r.out[i] = i;
     grid_dependency_wait();  // (nothing here runs ahead of the kernels before)
-    return;
+    return;                  // (nor does any CTA of the row go on)
   }
   grid_dependency_wait();  // the scores are there
   const auto key_at = [&](int i) { return select_key(p, r, i, i < r.n ? __ldcg(r.keys + i) : 0u); };
@@ -607,7 +646,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
 #pragma unroll
       for (int j = 0; j < KPT; ++j) f(tid * KPT + j, k[j]);
     } else {
-      const int per = (r.n + kThreads - 1) / kThreads;  // consecutive keys a thread
+      const int per = (r.n + kAll - 1) / kAll;  // consecutive keys a thread
       for (int j = 0; j < per; ++j) f(tid * per + j, key_at(tid * per + j));
     }
   };
@@ -618,37 +657,35 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
   if constexpr (KPT > 0) {
     each([&](int, uint32_t x) { widen(x); });
   } else {
-    for (int i = tid; i < r.n; i += kThreads) widen(key_at(i));
+    for (int i = tid; i < r.n; i += kAll) widen(key_at(i));
   }
   lowest = __reduce_min_sync(0xffffffffu, lowest);
   highest = __reduce_max_sync(0xffffffffu, highest);
-  if (lane == 0) s_range[0][warp] = lowest, s_range[1][warp] = highest;
-  __syncthreads();
-  lowest = __reduce_min_sync(0xffffffffu, lane < kThreads / 32 ? s_range[0][lane] : 0xffffffffu);
-  highest = __reduce_max_sync(0xffffffffu, lane < kThreads / 32 ? s_range[1][lane] : 0u);
-  const Search from = search_from(lowest, highest);
+  if constexpr (kCtas > 1) B::meet();  // the other CTAs' memory is there to write to
+  B::put(s_more[0], lowest);
+  B::put(s_more[1], highest);
+  B::meet();
+  const Search from = search_from(B::lowest(s_more[0]), B::highest(s_more[1]));
   uint32_t thr = from.thr;
-  int slot = 0;
+  int slot = 0;  // alternates, so that one meeting a round is enough
   for (int bit = from.bit - 1; bit >= -1; bit -= 2) {  // bits bit + 1 and bit (at -1, of bit 0 alone)
     const uint32_t c2 = thr | 1u << (bit + 1), c1 = bit >= 0 ? thr | 1u << bit : c2, c3 = bit >= 0 ? c2 | 1u << bit : c2;
     int n1 = 0, n2 = 0, n3 = 0;
     if constexpr (KPT > 0) {
       each([&](int, uint32_t x) { n1 += x >= c1, n2 += x >= c2, n3 += x >= c3; });
     } else {  // in any order
-      for (int i = tid; i < r.n; i += kThreads) {
+      for (int i = tid; i < r.n; i += kAll) {
         const uint32_t x = key_at(i);
         n1 += x >= c1, n2 += x >= c2, n3 += x >= c3;
       }
     }
-    n1 = __reduce_add_sync(0xffffffffu, n1);
-    n2 = __reduce_add_sync(0xffffffffu, n2);
-    n3 = __reduce_add_sync(0xffffffffu, n3);
-    if (lane == 0) s_part[slot][warp] = n1, s_part[slot + 1][warp] = n2, s_part[slot + 2][warp] = n3;
-    __syncthreads();
-    const bool in = lane < kThreads / 32;
-    n1 = __reduce_add_sync(0xffffffffu, in ? s_part[slot][lane] : 0);
-    n2 = __reduce_add_sync(0xffffffffu, in ? s_part[slot + 1][lane] : 0);
-    n3 = __reduce_add_sync(0xffffffffu, in ? s_part[slot + 2][lane] : 0);
+    B::put(s_part[slot], __reduce_add_sync(0xffffffffu, n1));
+    B::put(s_part[slot + 1], __reduce_add_sync(0xffffffffu, n2));
+    B::put(s_part[slot + 2], __reduce_add_sync(0xffffffffu, n3));
+    B::meet();
+    n1 = B::sum(s_part[slot]);
+    n2 = B::sum(s_part[slot + 1]);
+    n3 = B::sum(s_part[slot + 2]);
     slot = 3 - slot;
     thr = n3 >= r.keep ? c3 : n2 >= r.keep ? c2 : n1 >= r.keep ? c1 : thr;
     const int got = n3 >= r.keep ? n3 : n2 >= r.keep ? n2 : n1 >= r.keep ? n1 : 0;
@@ -659,18 +696,18 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
     above += x > thr;
     equal += x == thr;
   });
-  const int need = r.keep - block_sum<kThreads>(above, s_part + slot, 0);
-  int a = above, e = equal;  // inclusive sums over the lanes, then over the warps
+  int a = above, e = equal;  // inclusive sums over the lanes, then over the warps before
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, e, o);
     if (lane >= o) a += x, e += y;
   }
-  if (lane == 31) s_scan[0][warp] = a, s_scan[1][warp] = e;
-  __syncthreads();
-  const bool before = lane < warp;  // warp < 32
-  a += __reduce_add_sync(0xffffffffu, before ? s_scan[0][lane] : 0);
-  e += __reduce_add_sync(0xffffffffu, before ? s_scan[1][lane] : 0);
+  B::put(s_more[2], __shfl_sync(0xffffffffu, a, 31));
+  B::put(s_more[3], __shfl_sync(0xffffffffu, e, 31));
+  B::meet();  // the last one: nothing is written to another CTA's memory after it
+  const int need = r.keep - B::sum(s_more[2]);
+  a += B::sum(s_more[2], B::entry());
+  e += B::sum(s_more[3], B::entry());
   int eq = e - equal, at = a - above + min(eq, need);
   each([&](int i, uint32_t x) {
     bool take = x > thr;
@@ -688,7 +725,7 @@ int64_t score_bytes(int64_t q_heads, int head_dim) {
 template <typename E>
 cudaError_t launch_score(const ScoreParams& p, int head_dim, dim3 grid, cudaStream_t s) {
   const bool wide = p.group > 8;
-  const int bytes = static_cast<int>(score_bytes(p.kv_heads * p.group, head_dim));
+  const int bytes = static_cast<int>(score_bytes(p.cta_heads * p.group, head_dim));
   const auto fn = head_dim == 128 ? (wide ? score_kernel<E, 128, true> : score_kernel<E, 128, false>)
                                   : (wide ? score_kernel<E, 64, true> : score_kernel<E, 64, false>);
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -699,12 +736,12 @@ cudaError_t launch_score(const ScoreParams& p, int head_dim, dim3 grid, cudaStre
 cudaError_t launch_select(const SelectParams& p, cudaStream_t s) {
   const unsigned rows = static_cast<unsigned>(p.rows), fours = (rows + 3) / 4;
   if (p.max_pages <= 256) return launch_early(select_warp_kernel<8>, fours, 128, 0, s, p);
-  if (p.max_pages <= 512) return launch_early(select_kernel<64, 8>, rows, 64, 0, s, p);
-  if (p.max_pages <= 1024) return launch_early(select_kernel<128, 8>, rows, 128, 0, s, p);
-  if (p.max_pages <= 2048) return launch_early(select_kernel<256, 8>, rows, 256, 0, s, p);
-  if (p.max_pages <= 8192) return launch_early(select_kernel<1024, 8>, rows, 1024, 0, s, p);
-  if (p.max_pages <= 32768) return launch_early(select_kernel<1024, 32>, rows, 1024, 0, s, p);
-  return launch_early(select_kernel<1024, 0>, rows, 1024, 0, s, p);
+  if (p.max_pages <= 512) return launch_early(select_kernel<64, 8, 1>, rows, 64, 0, s, p);
+  if (p.max_pages <= 1024) return launch_early(select_kernel<128, 8, 1>, rows, 128, 0, s, p);
+  if (p.max_pages <= 2048) return launch_early(select_kernel<256, 8, 1>, rows, 256, 0, s, p);
+  if (p.max_pages <= 8192) return launch_early_clusters(select_kernel<256, 8, 4>, 4 * rows, 256, 4, 0, s, p);
+  if (p.max_pages <= 32768) return launch_early_clusters(select_kernel<512, 8, 8>, 8 * rows, 512, 8, 0, s, p);
+  return launch_early(select_kernel<1024, 0, 1>, rows, 1024, 0, s, p);
 }
 
 int sm_count() {
@@ -821,10 +858,17 @@ extern "C" int iris_b200_page_select(const void* query, const void* bounds, cons
   p.err = error_word;
   const int octets = static_cast<int>(key_stride_of(max_pages_per_seq) / 8);
   // the score kernel also reports bad lengths, so it runs even where every page is kept
-  const int want = 3 * sm_count() / batch > 1 ? 3 * sm_count() / batch : 1;  // CTAs a sequence: three an SM in all
+  // Three CTAs an SM in all, as many a sequence as there are sequences for.  A CTA quantises the queries of its heads
+  // before it starts, so the heads are shared out first, as long as three CTAs a share of the heads are left for the
+  // pages (one sequence of 8192 pages, 64 heads: 17.9 -> 16.1 us with the selection).
+  int want = 3 * sm_count() / batch > 1 ? 3 * sm_count() / batch : 1;
+  int shares = 1;
+  while (num_kv_heads % (2 * shares) == 0 && want / (2 * shares) >= 3) shares *= 2;
+  want /= shares;
+  p.cta_heads = num_kv_heads / shares;
   p.octets = octets > 0 ? (octets + want - 1) / want : 1;
   const dim3 grid(octets > 0 ? static_cast<unsigned>((octets + p.octets - 1) / p.octets) : 1u,
-                  static_cast<unsigned>(batch));
+                  static_cast<unsigned>(batch), static_cast<unsigned>(shares));
   cudaError_t e = dtype == IRIS_DTYPE_FP16 ? launch_score<Fp16Elem>(p, head_dim, grid, s)
                                            : launch_score<Bf16Elem>(p, head_dim, grid, s);
   if (e == cudaSuccess) {
