@@ -24,6 +24,7 @@ namespace iris {
 namespace {
 
 constexpr int kPage = 16;
+constexpr int kBoundsCtas = 4;  // CTAs an SM of the bounds kernel: one wave (5 to 8: 1 us more for a step, no less for all)
 
 // ------------------------------------------------------------------ bounds
 struct BoundsParams {
@@ -74,17 +75,20 @@ IRIS_DEV float product(__half a, __half b) {
   return d;
 }
 
-// One CTA per page (looping), one thread per 8 dims of one head; the D / 8
-// threads of a head are adjacent lanes.  All of the thread's 16 words and 16
-// scales are asked for before the first is used.  Two nibbles become
-// fp16 with two operations, a product takes one, and two tokens one three-way
+// A CTA takes every gridDim.x-th of a sequence's pages, one thread per 8 dims
+// of one head; the D / 8 threads of a head are adjacent lanes.  The 16 words
+// and 16 scales of a thread's next page are asked for before the present one
+// is worked on, so that one wave of CTAs does: more would only come and go
+// where a decode step has one new page a sequence.  Two nibbles become fp16
+// with two operations, a product takes one, and two tokens one three-way
 // minimum and maximum: it is these that bound the kernel, not the bytes.
 template <int D>
-__global__ void __launch_bounds__(256, 3) bounds_kernel(const BoundsParams p) {
+__global__ void __launch_bounds__(256, 2) bounds_kernel(const BoundsParams p) {
   constexpr int V = D / 8;
   grid_dependency_wait();
   const int b = blockIdx.y;
   const int len = __ldg(p.seq_lens + b);
+  const int from = p.first_token != nullptr ? max(0, __ldg(p.first_token + b)) / kPage : 0;
   if (len <= 0) {
     if (len < 0 && blockIdx.x == 0 && threadIdx.x == 0) set_error(p.err, IRIS_ERR_SEQ_LEN);
     return;
@@ -94,30 +98,52 @@ __global__ void __launch_bounds__(256, 3) bounds_kernel(const BoundsParams p) {
     if (blockIdx.x == 0 && threadIdx.x == 0) set_error(p.err, IRIS_ERR_BLOCK_TABLE);
     last = p.max_pages - 1;
   }
-  const int from = p.first_token != nullptr ? max(0, __ldg(p.first_token + b)) / kPage : 0;
   const int vecs = p.kv_heads * V;
-  for (int col = from + blockIdx.x; col <= last; col += gridDim.x) {
-    const int64_t page = __ldg(p.block_table + b * p.table_stride + col);
-    if (page < 0 || page >= p.num_pages) {
-      if (threadIdx.x == 0) set_error(p.err, IRIS_ERR_PAGE_ID);
-      continue;
-    }
-    const int final_token = min(kPage, len - col * kPage) - 1;
-    // whole warps go round together: lanes past the last vector repeat it and store nothing
-    for (int i0 = threadIdx.x & ~31; i0 < vecs; i0 += blockDim.x) {
-      const int i = min(i0 + static_cast<int>(threadIdx.x & 31), vecs - 1);
-      const bool mine = i0 + static_cast<int>(threadIdx.x & 31) < vecs;
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.k_data) + page * kPage * vecs + i;
-      const unsigned short* scl =
-          reinterpret_cast<const unsigned short*>(p.k_scale) + page * kPage * (vecs >> 2) + (i >> 2);
-      uint32_t w[kPage];
-      unsigned short sh[kPage];
+  const int32_t* table = p.block_table + b * p.table_stride;
+  const int step0 = static_cast<int>(blockDim.x), stride = static_cast<int>(gridDim.x);
+  // Whole warps go round together, over the pages and over the vectors where a page has more than the CTA threads:
+  // lanes past the last vector repeat it and store nothing.
+  const int lane = threadIdx.x & 31;
+  int next_col = from + static_cast<int>(blockIdx.x), next_i0 = static_cast<int>(threadIdx.x) - lane;
+  const auto page_at = [&](int col) -> int32_t { return col <= last ? __ldg(table + col) : -1; };
+  int32_t next_page = page_at(next_col), page_after = page_at(next_col + stride);
+  uint32_t w[kPage];
+  unsigned short sh[kPage];
+  const auto load = [&]() {  // what next_col and next_i0 say
+    if (next_col > last || next_page < 0 || next_page >= p.num_pages || next_i0 >= vecs) return;
+    const int i = min(next_i0 + lane, vecs - 1);
+    const int final_token = min(kPage, len - next_col * kPage) - 1;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(p.k_data) + static_cast<int64_t>(next_page) * kPage * vecs + i;
+    const unsigned short* scl = reinterpret_cast<const unsigned short*>(p.k_scale) +
+                                static_cast<int64_t>(next_page) * kPage * (vecs >> 2) + (i >> 2);
 #pragma unroll
-      for (int t = 0; t < kPage; ++t) {  // tokens past the last one repeat it
-        const int tok = min(t, final_token);
-        w[t] = __ldg(src + tok * vecs);
-        sh[t] = __ldg(scl + tok * (vecs >> 2));
-      }
+    for (int t = 0; t < kPage; ++t) {  // tokens past the last one repeat it
+      const int tok = min(t, final_token);
+      w[t] = __ldg(src + tok * vecs);
+      sh[t] = __ldg(scl + tok * (vecs >> 2));
+    }
+  };
+  load();
+  while (next_col <= last) {
+    const int i0 = next_i0;
+    const int64_t page = next_page;
+    const bool known = page >= 0 && page < p.num_pages, here = known && i0 < vecs;
+    if (!known && threadIdx.x == 0) set_error(p.err, IRIS_ERR_PAGE_ID);
+    uint32_t cw[kPage];
+    unsigned short cs[kPage];
+#pragma unroll
+    for (int t = 0; t < kPage; ++t) cw[t] = w[t], cs[t] = sh[t];
+    next_i0 += step0;
+    if (next_i0 >= vecs || !known) {
+      next_i0 = static_cast<int>(threadIdx.x) - lane;
+      next_col += stride;
+      next_page = page_after;
+      page_after = page_at(next_col + stride);
+    }
+    load();
+    if (here) {
+      const int i = min(i0 + lane, vecs - 1);
+      const bool mine = i0 + lane < vecs;
       float lo[8], hi[8], bad = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -126,14 +152,14 @@ __global__ void __launch_bounds__(256, 3) bounds_kernel(const BoundsParams p) {
       }
 #pragma unroll
       for (int t = 0; t < kPage; t += 2) {
-        bad = fmaf(__half2float(__ushort_as_half(sh[t])), 0.0f, bad);  // NaN from a scale that is not finite
-        bad = fmaf(__half2float(__ushort_as_half(sh[t + 1])), 0.0f, bad);
+        bad = fmaf(__half2float(__ushort_as_half(cs[t])), 0.0f, bad);  // NaN from a scale that is not finite
+        bad = fmaf(__half2float(__ushort_as_half(cs[t + 1])), 0.0f, bad);
         float x[2][8];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t v = w[t + e], u = v >> 8;
+          const uint32_t v = cw[t + e], u = v >> 8;
           const uint32_t n[4] = {int4_lo_exact(v), int4_hi_exact(v), int4_lo_exact(u), int4_hi_exact(u)};
-          const __half s = __ushort_as_half(sh[t + e]);
+          const __half s = __ushort_as_half(cs[t + e]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {  // dims j and j + 4
             x[e][j] = product(__low2half(u32_as_h2(n[j])), s);
@@ -793,10 +819,7 @@ extern "C" int iris_b200_int4_page_bounds(const void* k_data, const void* k_scal
   clear_stale_cuda_error();
   const int vecs = num_kv_heads * (head_dim / 8);
   const int threads = vecs >= 256 ? 256 : (vecs + 31) / 32 * 32;
-  // CTAs: 16 an SM for whole sequences; 6 where only the pages from a token on are new, which a decode step's are one
-  // or two of (64 sequences of 257 pages: one page each 4.8 us with 6, 6.4 us with 16; all pages of 16 sequences of
-  // 8191 tokens 47.0 us with 6, 39.5 us with 16).
-  const int64_t want = (static_cast<int64_t>(sm_count()) * (first_token != nullptr ? 6 : 16) + batch - 1) / batch;
+  const int64_t want = (static_cast<int64_t>(sm_count()) * kBoundsCtas + batch - 1) / batch;
   int64_t x = want < max_pages_per_seq ? want : max_pages_per_seq;
   if (x < 1) x = 1;
   const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(batch));
