@@ -194,6 +194,18 @@ Rows token_rows(const char* name, const Tensor& t, at::IntArrayRef shape, at::Sc
   return {ptr(t), shape[0] > 1 ? t.stride(0) : 0};
 }
 
+// A kernel that reads vectors of `in` after it has written others of `out`
+// cannot have both in one place.
+void check_apart(const char* name, const Tensor& out, const char* of, const Tensor& in) {
+  if (out.numel() == 0 || in.numel() == 0) return;
+  int64_t last = 0;
+  for (int64_t d = 0; d < in.dim(); ++d) last += (in.size(d) - 1) * in.stride(d);
+  const char* a = static_cast<const char*>(out.const_data_ptr());
+  const char* b = static_cast<const char*>(in.const_data_ptr());
+  if (a < b + (last + 1) * in.element_size() && b < a + out.numel() * out.element_size())
+    refuse(PyExc_ValueError, std::string(name) + " must not overlap " + of);
+}
+
 // (key, value, positions, slot_mapping, cos, sin, k_data, v_data, k_scale, v_scale, query, sections, rotary_dim,
 //  interleaved, group_size, page_size, query_out, key_out) -> rotated query or None
 PyObject* mrope_append(PyObject* const* a) {
@@ -264,12 +276,20 @@ PyObject* mrope_append(PyObject* const* a) {
       rotated = empty(shape, type, device);
     } else {
       check("query_out", *query_out, shape, type, device);
+      check_apart("query_out", *query_out, "query", *query);
+      check_apart("query_out", *query_out, "key", key);
+      check_apart("query_out", *query_out, "value", value);
       rotated = *query_out;
     }
   } else {
     require(query_out == nullptr, PyExc_ValueError, "query_out needs a query");
   }
-  if (key_out != nullptr) check("key_out", *key_out, key.sizes(), type, device);
+  if (key_out != nullptr) {
+    check("key_out", *key_out, key.sizes(), type, device);
+    check_apart("key_out", *key_out, "key", key);
+    check_apart("key_out", *key_out, "value", value);
+    if (query != nullptr) check_apart("key_out", *key_out, "query", *query);
+  }
   require(heads <= INT32_MAX && q_heads <= INT32_MAX, PyExc_ValueError, "too many heads");
   if (tokens > 0) {
     Tensor ws;

@@ -101,14 +101,14 @@ __global__ void __launch_bounds__(kThreads) mrope_check_pairs_kernel(const Mrope
   int32_t bits = 0;
   if (slot >= 0 && part == 0) bits = token_bits(p, slot, i);
   __syncthreads();
-  if (slot < 0) return;
+  if (slot < 0) return;  // all eight lanes of the token
   int hits = 0;
   for (int j = 4 * part; j < T4; j += 32) {
     const int4 v = *reinterpret_cast<const int4*>(s_slot + j);
     hits += (v.x == slot) + (v.y == slot) + (v.z == slot) + (v.w == slot);
   }
   const unsigned mates = 0xFFu << (threadIdx.x & 24);  // the token's lanes, which all came here
-  if (__reduce_add_sync(mates, hits) > 1) bits |= IRIS_ERR_DUP_SLOT;
+  if (__reduce_add_sync(mates, hits) > 1 && static_cast<int64_t>(slot) < p.num_slots) bits |= IRIS_ERR_DUP_SLOT;
   if (part == 0 && bits) set_error(p.err, bits);
 }
 
@@ -125,7 +125,7 @@ IRIS_DEV bool check_small_batch(const MropeParams& p) {
   __syncthreads();
   for (int i = threadIdx.x; i < T; i += blockDim.x) {
     const int32_t s = s_slot[i];
-    if (s < 0) continue;
+    if (s < 0 || static_cast<int64_t>(s) >= p.num_slots) continue;
     int hits = 0;
     for (int j = 0; j < T4; j += 4) {
       const int4 v = *reinterpret_cast<const int4*>(s_slot + j);

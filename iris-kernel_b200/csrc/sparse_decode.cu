@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
   const auto look_up = [&](int step) {
     const int u = min(step + (lane >> 1), end - 1);
     int row = seek_row, start = seek_start, n = steps_of(p, row);
-    while (u >= start + n) {
+    while (u >= start + n && row + 1 < p.rows) {
       start += n;
       n = steps_of(p, ++row);
     }

@@ -197,6 +197,42 @@ def test_a_bad_batch_writes_nothing(T, what, error):
     _check(_case(13, T=T, pages=15))  # the next batch is written
 
 
+@pytest.mark.parametrize("T", [20, 200, 2100])
+def test_slots_past_the_cache_are_an_index_error_even_twice(T):
+    c = _case(30, T=T, pages=140, pad=0.0)
+    c["slots"][3] = c["slots"][T - 1] = 140 * 16
+    with pytest.raises(IndexError):
+        _run(c)
+
+
+@pytest.mark.parametrize("T", [2048, 2049, 5000])
+def test_large_batches(T):
+    """Both forms of the duplicate check, and a duplicate far away."""
+    c = _case(31, T=T, hq=2, hkv=1, dim=64, sections=(16, 8, 8), pages=330)
+    _check(c)
+    c = _case(32, T=T, hq=1, hkv=1, dim=64, sections=(16, 8, 8), pages=330, pad=0.0)
+    before = [x.clone() for x in c["cache"]]
+    c["slots"][T - 1] = c["slots"][7].clone()
+    with pytest.raises(ValueError):
+        _run(c)
+    for x, y in zip(before, c["cache"]):
+        assert torch.equal(x, y)
+
+
+def test_positions_shared_by_the_axes_and_a_single_head():
+    """One row of positions expanded over the axes, as text tokens have them,
+    is the rotation with one axis."""
+    c = _case(33, T=12, hq=2, hkv=1, pad=0.0)
+    one = {**c, "positions": c["positions"][:1], "sections": (64,), "cache": [x.clone() for x in c["cache"]]}
+    c["positions"] = c["positions"][:1].expand(3, -1)
+    q, k = _run(c)
+    q1, k1 = _run(one)
+    _same_bits(q, q1.cpu())
+    _same_bits(k, k1.cpu())
+    for x, y in zip(c["cache"], one["cache"]):
+        _same_bits(x, y.cpu())
+
+
 def test_on_a_side_stream():
     c = _case(14, T=150, pages=12)
     want = _expect(c)
@@ -235,6 +271,8 @@ def test_refusals():
     flat = torch.zeros(c["key"].numel() + 1, dtype=torch.float16, device="cuda")
     call(ValueError, key=flat[1:].view(c["key"].shape))  # not on a 16-byte boundary
     call(ValueError, key=c["key"].cpu())
+    with pytest.raises(ValueError):
+        _run(c, key_out=False, query_out=c["query"])  # a rotation in place would read what it has overwritten
     with pytest.raises(NotImplementedError):
         _run(c, group_size=64)
     with pytest.raises(ValueError):
