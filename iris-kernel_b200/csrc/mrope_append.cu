@@ -18,8 +18,10 @@
 // row_lanes x D / 8 threads, a thread one 8-dim vector of every row_lanes-th
 // head: the token's rotary rows are read, and their axes blended, once per
 // thread and used for all its keys and queries.  A group is four adjacent
-// lanes; its absmax takes two shuffles.  What bounds it is instructions, then
-// bytes: arithmetic goes two values at a time.
+// lanes; its absmax takes two shuffles.  Arithmetic goes two values at a time.
+// 8192 tokens of 32 + 2 x 8 heads of 128 dims, three axes dealt out in turn,
+// rotated keys wanted: 69 us with the check and the read back of the cache;
+// the append itself 53 us, 3.7 TB/s, waiting for its loads.
 #include "append_common.cuh"
 #include "elem.cuh"
 

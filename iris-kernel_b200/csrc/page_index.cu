@@ -17,7 +17,13 @@
 // Selection.  Per sequence and KV head the max_pages highest scores, the
 // first sink_pages and last recent_pages before all others, ties to the
 // lowest page; written in rising order.
-
+//
+// Measured (B200, 8 KV heads of 128 dims).  Bounds of 16 sequences of up to
+// 8191 tokens: 36.3 us, 3.1 TB/s, the integer and minimum pipe at two thirds;
+// of one new page in each of 64 sequences 3.1 us.  Scores and selection over
+// 64 sequences of up to 16384 tokens: 33.8 us, 3.6 TB/s, the scores 3/4 of it,
+// waiting for bounds; one sequence of 131072 tokens 16.3 us, two launches and
+// their chains of dependent loads.
 #include "elem.cuh"
 
 namespace iris {

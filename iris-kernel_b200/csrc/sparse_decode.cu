@@ -11,7 +11,9 @@
 // scale bytes, for K and V: small strided pieces, so each warp copies its own
 // pages with asynchronous copies into a ring of its own (no barrier between
 // warps) and keeps its own running softmax.  The copies ask L2 for 64 bytes at
-// a time: a token's other heads lie next to its own, and were fetched with it.
+// a time: a token's other heads lie next to its own, and without that were
+// fetched with it (the copies alone, 64 sequences x 128 pages, 8 KV heads of
+// 128 dims: 49.2 -> 40.8 us).
 //
 // Products run on the tensor cores with fp16 operands and fp32 accumulation:
 //   S = Q K^T      rows = query heads, columns = tokens, one accumulator per
@@ -30,6 +32,7 @@
 // A 16-byte chunk of a page's row is one group: ldmatrix hands each lane the
 // eight dims of a token that its place in K's fragment needs, and its
 // transposing form four dims of two tokens, as V's fragment needs them.
+//
 // Work.  A step takes two pages (their products and exponentials are
 // independent; maxima, votes and rescalings are shared).  All steps of all rows
 // (sequence x KV head), one after another, are cut into equal runs, one a warp,
@@ -37,6 +40,13 @@
 // batch looks like, and waits for no other.  A row inside one run is written at
 // once; the parts of the others go to the workspace as (o, m, l), and a second
 // kernel joins them in the order of the list.
+//
+// Measured (B200): 64 sequences x 128 pages of 8192 tokens, 32 + 8 heads of 128
+// dims: 62.7 us, 2.4 TB/s of the bytes it needs (DRAM moves 1.5 times those:
+// other heads' scales share a sector).  Bound by instructions: about 440 a page
+// and warp at half an instruction a cycle, three CTAs of 168 registers an SM
+// (four CTAs spill: 73 us); with the pages in L2 it takes 54.  One sequence,
+// 128 pages: 11.6 us, a chain of launches and dependent loads.
 #include <map>
 #include <mutex>
 #include <type_traits>
@@ -780,7 +790,8 @@ cudaError_t grid_for(const Kernel& k, int64_t rows, int group, int head_dim, int
   return cudaSuccess;
 }
 
-// Shortest run of a warp, in steps.
+// Shortest run of a warp, in steps (one sequence of 128 pages, 8 KV heads: 11.1 us with 2; 13.1, 12.3 and 12.1 with 1,
+// 3 and 4: shorter runs leave more parts to join, longer ones fewer warps).
 constexpr int kMinSteps = 2;
 
 }  // namespace
