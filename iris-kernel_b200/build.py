@@ -71,7 +71,7 @@ def _bindings_command() -> list:
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE,
             *[x for d in include for x in ("-isystem", d)], os.path.join(CSRC, "bindings.cpp"),
             "-o", BINDINGS + ".tmp", "-L", os.path.dirname(OUT), "-l:libiris_b200.so", "-L", os.path.join(root, "lib"),
-            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

@@ -9,11 +9,13 @@
 namespace iris {
 
 struct Fp16Elem {
+  static constexpr bool kFp16 = true;
   IRIS_DEV static float2 unpack(uint32_t w) { return __half22float2(u32_as_h2(w)); }
   IRIS_DEV static uint32_t pack(float lo, float hi) { return h2_as_u32(__floats2half2_rn(lo, hi)); }
 };
 
 struct Bf16Elem {
+  static constexpr bool kFp16 = false;
   IRIS_DEV static float2 unpack(uint32_t w) {  // a bf16 is the upper half of its fp32
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }

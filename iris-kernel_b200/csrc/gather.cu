@@ -8,14 +8,15 @@
 // warp finds the first row's sequence and, a lane a row, the rows' places in
 // the cache; then all pass over the tile's 8-dim vectors: four packed bytes
 // in, one 16-byte store out, consecutive lanes on consecutive vectors.  8 x 8192
-// tokens of 8 heads of 128 dims: 59.5 us, 5.2 TB/s (81 % of a plain copy).
+// tokens of 8 heads of 128 dims: 58.2 us, 5.3 TB/s (82 % of a plain copy), DRAM
+// bound; 517 tokens of 8 heads of 64 dims: 2.4 us, launch and dependent loads.
 #include "elem.cuh"
 
 namespace iris {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 16;  // output rows per CTA
+constexpr int kTile = 16;  // most output rows per CTA
 
 struct GatherParams {
   const uint8_t* k_data;
@@ -34,6 +35,7 @@ struct GatherParams {
   int32_t max_pages;
   int32_t vecs;  // 8-dim vectors per token: Hkv D / 8
   int32_t page_size;
+  int32_t tile;  // output rows per CTA
   int32_t* err;
 };
 
@@ -81,37 +83,79 @@ IRIS_DEV int64_t row_of(const GatherParams& p, int64_t n, int seq) {
   return page * p.page_size + at % p.page_size;
 }
 
+// Eight nibbles times their scale, rounded once to the output type.  A pair's
+// nibbles become 1024 + u and 1024 + 16 u in fp16 (u = nibble + 8, by setting
+// the exponent over them), one fused step makes them exact whole numbers.
+// FP16: their product with the scale is that type's own; BF16: it is exact in
+// fp32 (14 bits) and rounded from there.
 template <typename E>
 IRIS_DEV uint4 dequant8(uint32_t w, __half scale) {
-  const float s = __half2float(scale);
-  float x[8];
+  w ^= 0x88888888u;
+  const uint32_t lo = __byte_perm(w, 0u, 0x1010), hi = __byte_perm(w, 0u, 0x3232);
+  const uint32_t u[4] = {lo, lo >> 8, hi, hi >> 8};
+  uint32_t x[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(static_cast<float>(nibble(w, i)), s);
-  return make_uint4(E::pack(x[0], x[1]), E::pack(x[2], x[3]), E::pack(x[4], x[5]), E::pack(x[6], x[7]));
+  for (int i = 0; i < 4; ++i) {
+    const __half2 q = __hfma2(u32_as_h2((u[i] & 0x00F0000Fu) | 0x64006400u), u32_as_h2(0x2C003C00u) /* 1/16, 1 */,
+                              u32_as_h2(0xD480E408u) /* -72, -1032 */);
+    if constexpr (E::kFp16) {
+      x[i] = h2_as_u32(__hmul2(q, __half2half2(scale)));
+    } else {
+      const float2 f = __half22float2(q);
+      const float s = __half2float(scale);
+      x[i] = E::pack(__fmul_rn(f.x, s), __fmul_rn(f.y, s));
+    }
+  }
+  return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
 template <typename E>
 __global__ void __launch_bounds__(kThreads) gather_kernel(const GatherParams p) {
+  // Vectors of each tensor that a thread has on the way at a time: 1, 2, 4 and 8 of them take 58.5, 58.1, 64.1 and
+  // 75.3 us at 8 x 8192 tokens (more registers, fewer warps), 3.4, 3.3, 3.4 and 3.6 at 517.
+  constexpr int kAhead = 2;
   __shared__ int64_t s_row[kTile];
   grid_dependency_wait();
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kTile;
-  const int rows = static_cast<int>(p.num_tokens - n0 < kTile ? p.num_tokens - n0 : kTile);
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * p.tile;
+  const int rows = static_cast<int>(p.num_tokens - n0 < p.tile ? p.num_tokens - n0 : p.tile);
   if (threadIdx.x < 32) {
     const int seq = sequence_of(p, n0);
     if (threadIdx.x < rows) s_row[threadIdx.x] = row_of(p, n0 + threadIdx.x, seq);
   }
+  const int down = kThreads / p.vecs, along = kThreads - down * p.vecs;  // from a thread's vector to its next one
+  int r = threadIdx.x / p.vecs, v = threadIdx.x - r * p.vecs;
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * p.vecs; i += kThreads) {
-    const int r = i / p.vecs, v = i - r * p.vecs;
-    const int64_t src = s_row[r], dst = (n0 + r) * p.vecs + v;
-    uint4 k = make_uint4(0, 0, 0, 0), w = k;
-    if (src >= 0) {
-      const int64_t at = src * p.vecs + v;
-      k = dequant8<E>(__ldg(reinterpret_cast<const uint32_t*>(p.k_data) + at), p.k_scale[at >> 2]);
-      w = dequant8<E>(__ldg(reinterpret_cast<const uint32_t*>(p.v_data) + at), p.v_scale[at >> 2]);
+  while (r < rows) {
+    uint32_t kw[kAhead], vw[kAhead];
+    __half ks[kAhead], vs[kAhead];
+    int64_t dst[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      dst[j] = r < rows ? (n0 + r) * p.vecs + v : -1;
+      kw[j] = vw[j] = 0u;
+      ks[j] = vs[j] = __ushort_as_half(0);
+      const int64_t src = r < rows ? s_row[r] : -1;
+      if (src >= 0) {
+        const int64_t at = src * p.vecs + v;
+        kw[j] = __ldg(reinterpret_cast<const uint32_t*>(p.k_data) + at);
+        vw[j] = __ldg(reinterpret_cast<const uint32_t*>(p.v_data) + at);
+        ks[j] = __ldg(p.k_scale + (at >> 2));
+        vs[j] = __ldg(p.v_scale + (at >> 2));
+      }
+      r += down;
+      v += along;
+      if (v >= p.vecs) {
+        v -= p.vecs;
+        ++r;
+      }
     }
-    static_cast<uint4*>(p.key)[dst] = k;
-    static_cast<uint4*>(p.value)[dst] = w;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (dst[j] >= 0) {
+        static_cast<uint4*>(p.key)[dst[j]] = dequant8<E>(kw[j], ks[j]);
+        static_cast<uint4*>(p.value)[dst[j]] = dequant8<E>(vw[j], vs[j]);
+      }
+    }
   }
 }
 
@@ -134,7 +178,7 @@ extern "C" int iris_b200_int4_paged_gather(const void* k_data, const void* v_dat
   if (num_tokens == 0) return IRIS_OK;
   if (batch == 0) return IRIS_EINVAL;
   if (static_cast<int64_t>(num_kv_heads) * head_dim > (1 << 24)) return IRIS_EUNSUPPORTED;
-  if (num_tokens > (static_cast<int64_t>(kTile) << 30)) return IRIS_EUNSUPPORTED;
+  if (num_tokens > (1ll << 30)) return IRIS_EUNSUPPORTED;
   const void* ptrs[] = {k_data, v_data, k_scale, v_scale, block_table, cu_seqlens, key, value};
   for (const void* q : ptrs)
     if (q == nullptr) return IRIS_EINVAL;
@@ -159,8 +203,17 @@ extern "C" int iris_b200_int4_paged_gather(const void* k_data, const void* v_dat
   p.vecs = num_kv_heads * (head_dim / 8);
   p.page_size = page_size;
   p.err = error_word;
+  // Rows per CTA: one vector a thread at least; then more, as long as 1024 CTAs
+  // are left to fill the machine.  With 1, 2, 4, 8 and 16 rows of 1024 dims an
+  // append of 64 tokens and its read back take 7.2, 7.4, 8.0, 9.2 and 11.5 us, of
+  // 8192 tokens 65.4, 59.7, 57.7, 56.5 and 57.8; reading 65536 tokens takes 114,
+  // 80, 63, 58.6 and 58.1.
+  p.tile = 1;
+  while (p.tile < kTile && (p.tile * p.vecs < kThreads ||
+                            (2 * p.tile * p.vecs <= 8 * kThreads && num_tokens >= 1024 * 2ll * p.tile)))
+    p.tile *= 2;
   clear_stale_cuda_error();
-  const unsigned blocks = static_cast<unsigned>((num_tokens + kTile - 1) / kTile);
+  const unsigned blocks = static_cast<unsigned>((num_tokens + p.tile - 1) / p.tile);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = dtype == IRIS_DTYPE_FP16 ? launch_early(gather_kernel<Fp16Elem>, blocks, kThreads, 0, s, p)
                                                  : launch_early(gather_kernel<Bf16Elem>, blocks, kThreads, 0, s, p);

@@ -16,12 +16,15 @@
 // The work is a copy with arithmetic on the way: per token 2 Hkv D (and Hq D)
 // 16-bit values in, 1.125 Hkv D bytes (and Hq D values) out.  A token takes
 // row_lanes x D / 8 threads, a thread one 8-dim vector of every row_lanes-th
-// head: the token's rotary rows are read, and their axes blended, once per
-// thread and used for all its keys and queries.  A group is four adjacent
-// lanes; its absmax takes two shuffles.  Arithmetic goes two values at a time.
+// head (in large batches of whole turning groups two vectors, the ones that
+// turn together, by half as many threads): the token's rotary rows are read,
+// and their axes blended, once per thread and used for all its keys and
+// queries.  A group is four adjacent lanes; its absmax takes two shuffles.
+// Arithmetic goes two values at a time.
 // 8192 tokens of 32 + 2 x 8 heads of 128 dims, three axes dealt out in turn,
-// rotated keys wanted: 69 us with the check and the read back of the cache;
-// the append itself 53 us, 3.7 TB/s, waiting for its loads.
+// rotated keys wanted: 57 us with the check and the read back of the cache,
+// bound by the latency of its loads and by issue; 64 tokens of them 7.4 us with
+// the read back, chains of dependent loads.
 #include "append_common.cuh"
 #include "elem.cuh"
 
@@ -60,15 +63,21 @@ struct MropeParams {
   uint32_t axis_map[kMaxFreqs / 16];  // two bits per frequency
 };
 
-// Error bits of one token's slot and positions.
+// Error bits of one token's slot and positions; a token without a slot has
+// none.  (All its positions are asked for at once, whatever the slot is.)
 IRIS_DEV int32_t token_bits(const MropeParams& p, int32_t slot, int64_t tok) {
+  int32_t pos[kMaxAxes];
+#pragma unroll
+  for (int a = 0; a < kMaxAxes; ++a) pos[a] = a < p.axes ? __ldg(p.positions + a * p.positions_stride + tok) : 0;
   int32_t bits = static_cast<int64_t>(slot) >= p.num_slots ? IRIS_ERR_SLOT_RANGE : 0;
-  for (int a = 0; a < p.axes; ++a) {
-    const int32_t pos = __ldg(p.positions + a * p.positions_stride + tok);
-    if (pos < 0) bits |= IRIS_ERR_POS_NEGATIVE;
-    else if (static_cast<int64_t>(pos) >= p.max_position) bits |= IRIS_ERR_POS_RANGE;
+#pragma unroll
+  for (int a = 0; a < kMaxAxes; ++a) {
+    if (a < p.axes) {
+      if (pos[a] < 0) bits |= IRIS_ERR_POS_NEGATIVE;
+      else if (static_cast<int64_t>(pos[a]) >= p.max_position) bits |= IRIS_ERR_POS_RANGE;
+    }
   }
-  return bits;
+  return slot >= 0 ? bits : 0;
 }
 
 // Validation of a large batch before the append: ranges, and one bit per slot
@@ -79,8 +88,8 @@ __global__ void __launch_bounds__(kThreads) mrope_check_kernel(const MropeParams
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (i >= p.num_tokens) return;
   const int32_t slot = __ldg(p.slots + i);
-  if (slot < 0) return;
   int32_t bits = token_bits(p, slot, i);
+  if (slot < 0) return;
   if (!(bits & IRIS_ERR_SLOT_RANGE)) {
     const uint32_t bit = 1u << (slot & 31);
     if (atomicOr(bitmap + (slot >> 5), bit) & bit) bits |= IRIS_ERR_DUP_SLOT;
@@ -121,7 +130,7 @@ IRIS_DEV bool check_small_batch(const MropeParams& p) {
   int32_t bits = 0;
   for (int i = threadIdx.x; i < T4; i += blockDim.x) {
     const int32_t s = i < T ? __ldg(p.slots + i) : -1;
-    if (s >= 0) bits |= token_bits(p, s, i);
+    if (i < T) bits |= token_bits(p, s, i);
     s_slot[i] = s;
   }
   __syncthreads();
@@ -242,25 +251,29 @@ IRIS_DEV uint32_t quant8(const float2 (&x)[4], uint32_t quad, __half& scale16) {
 // otherwise the check kernel before this launch did it.  The first keys (with
 // few tokens the first values and queries too) are asked for before anything
 // else is looked at: they depend on neither the slot nor the positions.  With
-// many tokens more warps on an SM do more than more loads a thread: 64
-// registers a thread took 78 us at 8192 tokens of 32 + 2 x 8 heads, 85
-// registers 85 us, 128 102 us (each with the 15 us of its check and read back,
-// before the prefetch).
-template <typename E, bool kSmall>
+// few tokens the check comes next, whose loads do not wait for one another, so
+// that a thread's own slot and positions are then at hand (64 tokens: 9.0 ->
+// 7.9 us).  With many tokens more warps on an SM do more than more loads a
+// thread: with 64 registers a thread 8192 tokens take 62.3 us, with 85 68.4
+// and with 48 73.5.
+template <typename E, bool kSmall, bool kPaired>
 __global__ void __launch_bounds__(kThreads, kSmall ? 2 : 4) mrope_append_kernel(const MropeParams p) {
   if constexpr (kSmall) grid_dependency_wait();
-  constexpr int kBatch = 2;  // heads whose vectors a thread has on the way, of each kind
-  const int per_token = p.row_lanes * p.vecs;
+  constexpr int kBatch = kPaired ? 1 : 2;  // heads whose vectors a thread has on the way, of each kind
+  const int units = kPaired ? p.vecs / 2 : p.vecs;
+  const int per_token = p.row_lanes * units;
   const int here = threadIdx.x / per_token, in_token = threadIdx.x - here * per_token;
-  const int row = in_token / p.vecs, v = in_token - row * p.vecs;  // first head, and vector within the head
+  const int row = in_token / units, unit = in_token - row * units;  // first head, and place within the head
   const int64_t tok = static_cast<int64_t>(blockIdx.x) * (blockDim.x / per_token) + here;
   const bool there = tok < p.num_tokens;  // (the last CTA's threads past the end go along with the checks)
   const int64_t at = there ? tok : 0;
   const int half = p.rotary_vecs / 2;  // vectors of the rotary half
-  const bool rotary = v < p.rotary_vecs, low = v < half;
-  const int64_t D2 = 16ll * p.vecs;                      // bytes of a head
-  const int64_t mate = (low ? half : -half) * 16ll;      // bytes to the vector that turns with this one
-  const int64_t stride = D2 * p.row_lanes;               // bytes to this thread's next head
+  // this thread's vector v and, `mate` vectors on, the one that turns with it (of the dims that do not turn, their other half's)
+  const bool rotary = unit < (kPaired ? half : p.rotary_vecs), low = kPaired || unit < half;
+  const int v = kPaired && !rotary ? unit + half : unit;
+  const int mate = kPaired && !rotary ? (p.vecs - p.rotary_vecs) / 2 : low ? half : -half;
+  const int64_t D2 = 16ll * p.vecs;         // bytes of a head
+  const int64_t stride = D2 * p.row_lanes;  // bytes to this thread's next head
   const char* key = static_cast<const char*>(p.key) + at * p.key_stride * 2 + row * D2 + 16 * v;
   const char* value = static_cast<const char*>(p.value) + at * p.value_stride * 2 + row * D2 + 16 * v;
   const char* query = static_cast<const char*>(p.query) + at * p.query_stride * 2 + row * D2 + 16 * v;
@@ -272,27 +285,33 @@ __global__ void __launch_bounds__(kThreads, kSmall ? 2 : 4) mrope_append_kernel(
         prefetch_l2_bulk(static_cast<const char*>(p.query) + at * p.query_stride * 2, static_cast<uint32_t>(D2 * p.q_heads));
     }
   }
-  // vectors of heads h, h + row_lanes, .. of a tensor, and for a turning one their mates
-  const auto load = [&](const char* src, int h, int heads, bool turning, uint4 (&x)[kBatch], uint4 (&o)[kBatch]) {
+  // vectors of heads h, h + row_lanes, .. of a tensor, and if wanted their mates
+  const auto load = [&](const char* src, int h, int heads, bool mates, uint4 (&x)[kBatch], uint4 (&o)[kBatch]) {
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       if (h + j * p.row_lanes < heads) {
         x[j] = ldg_nc_v4(src + j * stride);
-        if (turning) o[j] = ldg_nc_v4(src + j * stride + mate);
+        if (kPaired || mates) o[j] = ldg_nc_v4(src + j * stride + 16 * mate);
       }
     }
   };
   uint4 kx[kBatch], ko[kBatch];
   load(key, row, p.kv_heads, rotary, kx, ko);
-  uint4 vx[kBatch], none[kBatch], qx[kBatch], qo[kBatch];
+  uint4 vx[kBatch], vo[kBatch], qx[kBatch], qo[kBatch];
   if constexpr (kSmall) {
-    load(value, row, p.kv_heads, false, vx, none);
+    load(value, row, p.kv_heads, false, vx, vo);
     load(query, row, p.q_heads, rotary, qx, qo);
+  }
+  bool rejected = false;
+  int32_t pending = 0;
+  if constexpr (kSmall) {  // before the token's own slot: that and its positions then come from L1
+    if (p.err != nullptr) pending = *reinterpret_cast<volatile int32_t*>(p.err);
+    rejected = check_small_batch(p);
   }
   const int32_t slot = there ? __ldg(p.slots + tok) : -1;
   // A token with a bad slot or position: never touch memory outside the cache
   // or the tables.  (The check records its bits.)
-  const bool live = slot >= 0 && token_bits(p, slot, at) == 0;
+  const bool live = token_bits(p, slot, at) == 0 && slot >= 0;
   float2 c[4], s[4];
   if (live && rotary) {
     blend_rows<E>(p, tok, low ? v : v - half, c, s);
@@ -301,29 +320,33 @@ __global__ void __launch_bounds__(kThreads, kSmall ? 2 : 4) mrope_append_kernel(
       for (int j = 0; j < 4; ++j) s[j] = make_float2(-s[j].x, -s[j].y);
     }
   }
-  bool rejected = false;
-  if constexpr (kSmall) rejected = check_small_batch(p);
-  else grid_dependency_wait();
-  if (rejected || (p.err != nullptr && (*reinterpret_cast<volatile int32_t*>(p.err) & kRejectBits) != 0)) return;
+  if constexpr (!kSmall) {
+    grid_dependency_wait();
+    if (p.err != nullptr) pending = *reinterpret_cast<volatile int32_t*>(p.err);
+  }
+  if (rejected || (pending & kRejectBits) != 0) return;
   if (!there) return;
   const uint32_t quad = 0xFu << (threadIdx.x & 28);
 
-  // x cos + mate (-+ sin): both products are exact, one rounding in all
-  const auto turn = [&](const uint4& xw, const uint4& ow, float2 (&x)[4]) {
+  // x cos + mate (-+ sin): both products are exact, one rounding in all.  Paired: the mate's, too.
+  const auto turn = [&](const uint4& xw, const uint4& ow, float2 (&x)[4], float2 (&o)[4]) {
     unpack8<E>(xw, x);
+    if (kPaired || rotary) unpack8<E>(ow, o);
     if (rotary) {
-      float2 o[4];
-      unpack8<E>(ow, o);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = __ffma2_rn(x[j], c[j], __fmul2_rn(o[j], s[j]));
+      for (int j = 0; j < 4; ++j) {
+        const float2 xs = __fmul2_rn(x[j], s[j]);
+        x[j] = __ffma2_rn(x[j], c[j], __fmul2_rn(o[j], s[j]));
+        if constexpr (kPaired) o[j] = __ffma2_rn(o[j], c[j], make_float2(-xs.x, -xs.y));
+      }
     }
   };
   const int64_t cache_row = static_cast<int64_t>(slot) * p.kv_heads;
-  const auto store = [&](const float2 (&x)[4], int h, uint8_t* data, __half* scales) {
+  const auto store = [&](const float2 (&x)[4], int64_t vec, uint8_t* data, __half* scales) {
     __half scale;
     const uint32_t word = quant8(x, quad, scale);
-    reinterpret_cast<uint32_t*>(data)[(cache_row + h) * p.vecs + v] = word;
-    if ((v & 3) == 0) scales[(cache_row + h) * (p.vecs >> 2) + (v >> 2)] = scale;
+    reinterpret_cast<uint32_t*>(data)[vec] = word;
+    if ((unit & 3) == 0) scales[vec >> 2] = scale;
   };
 
   char* out = p.key_out != nullptr ? static_cast<char*>(p.key_out) + (at * p.kv_heads + row) * D2 + 16 * v : nullptr;
@@ -333,13 +356,20 @@ __global__ void __launch_bounds__(kThreads, kSmall ? 2 : 4) mrope_append_kernel(
     for (int j = 0; j < kBatch; ++j) {
       const int hh = h + j * p.row_lanes;
       if (hh < p.kv_heads) {
+        uint4* to = reinterpret_cast<uint4*>(out + j * stride);
         if (live) {
-          float2 x[4];
-          turn(kx[j], ko[j], x);
-          if (out != nullptr) *reinterpret_cast<uint4*>(out + j * stride) = pack8<E>(x);
-          store(x, hh, p.k_data, p.k_scale);
+          float2 x[4], o[4];
+          turn(kx[j], ko[j], x, o);
+          const int64_t vec = (cache_row + hh) * p.vecs + v;
+          if (out != nullptr) *to = pack8<E>(x);
+          store(x, vec, p.k_data, p.k_scale);
+          if constexpr (kPaired) {
+            if (out != nullptr) to[mate] = pack8<E>(o);
+            store(o, vec + mate, p.k_data, p.k_scale);
+          }
         } else if (out != nullptr) {  // padding: its rotated rows are zeros
-          *reinterpret_cast<uint4*>(out + j * stride) = make_uint4(0, 0, 0, 0);
+          *to = make_uint4(0, 0, 0, 0);
+          if constexpr (kPaired) to[mate] = make_uint4(0, 0, 0, 0);
         }
       }
     }
@@ -348,14 +378,19 @@ __global__ void __launch_bounds__(kThreads, kSmall ? 2 : 4) mrope_append_kernel(
   }
   if (live) {
     for (int h = row; h < p.kv_heads; h += kBatch * p.row_lanes) {
-      if (!kSmall || h != row) load(value, h, p.kv_heads, false, vx, none);
+      if (!kSmall || h != row) load(value, h, p.kv_heads, false, vx, vo);
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const int hh = h + j * p.row_lanes;
         if (hh < p.kv_heads) {
           float2 x[4];
+          const int64_t vec = (cache_row + hh) * p.vecs + v;
           unpack8<E>(vx[j], x);
-          store(x, hh, p.v_data, p.v_scale);
+          store(x, vec, p.v_data, p.v_scale);
+          if constexpr (kPaired) {
+            unpack8<E>(vo[j], x);
+            store(x, vec + mate, p.v_data, p.v_scale);
+          }
         }
       }
       value += kBatch * stride;
@@ -367,13 +402,16 @@ __global__ void __launch_bounds__(kThreads, kSmall ? 2 : 4) mrope_append_kernel(
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       if (h + j * p.row_lanes < p.q_heads) {
-        float2 x[4];
-        uint4 word = make_uint4(0, 0, 0, 0);
+        float2 x[4], o[4];
+        uint4 word = make_uint4(0, 0, 0, 0), other = word;
         if (live) {
-          turn(qx[j], qo[j], x);
+          turn(qx[j], qo[j], x, o);
           word = pack8<E>(x);
+          if constexpr (kPaired) other = pack8<E>(o);
         }
-        *reinterpret_cast<uint4*>(out + j * stride) = word;
+        uint4* to = reinterpret_cast<uint4*>(out + j * stride);
+        *to = word;
+        if constexpr (kPaired) to[mate] = other;
       }
     }
     query += kBatch * stride;
@@ -381,16 +419,26 @@ __global__ void __launch_bounds__(kThreads, kSmall ? 2 : 4) mrope_append_kernel(
   }
 }
 
+// Threads of a token of a large batch that share a vector.  More of them read
+// and blend the token's rotary rows more often, fewer walk longer over its
+// heads: 8192 tokens as above take 68.4, 66.1, 62.3 and 74.9 us with 2, 4, 8
+// and 16, 1021 tokens of 3 x 16 heads 26.7, 20.5, 16.4 and 17.5.
+constexpr int kRowLanes = 8;
+
 template <typename E>
 cudaError_t launch_mrope(MropeParams& p, uint32_t* bitmap, size_t bitmap_bytes, cudaStream_t stream) {
   if (p.num_tokens <= kInlineCheckTokens) {  // few tokens: as many threads on each as fit
     p.row_lanes = kThreads / p.vecs;
-    return launch_early(mrope_append_kernel<E, true>, static_cast<unsigned>(p.num_tokens), p.row_lanes * p.vecs, 0,
+    return launch_early(mrope_append_kernel<E, true, false>, static_cast<unsigned>(p.num_tokens), p.row_lanes * p.vecs, 0,
                         stream, p);
   }
-  // many: few threads a token, so that each blended row serves many heads
-  p.row_lanes = 4;
-  const int tokens = kThreads / (4 * p.vecs);  // a CTA
+  // Vectors in pairs where whole groups turn with whole groups (8192 tokens: 69 -> 62 us); with few tokens the
+  // longer work of a thread costs more than its loads (64 tokens: 14.4 -> 15.0 us).
+  const bool paired = p.rotary_vecs % 8 == 0;
+  const int units = paired ? p.vecs / 2 : p.vecs;
+  p.row_lanes = kThreads / units < kRowLanes ? kThreads / units : kRowLanes;
+  const int threads = kThreads / (p.row_lanes * units) * (p.row_lanes * units);
+  const int64_t tokens = threads / (p.row_lanes * units);  // a CTA
   cudaError_t e = cudaSuccess;
   if (p.num_tokens <= kPairwiseTokens) {
     e = launch_early(mrope_check_pairs_kernel, static_cast<unsigned>((8 * p.num_tokens + kThreads - 1) / kThreads),
@@ -403,8 +451,8 @@ cudaError_t launch_mrope(MropeParams& p, uint32_t* bitmap, size_t bitmap_bytes, 
   }
   if (e != cudaSuccess) return e;
   // comes up while the check finishes
-  return launch_early(mrope_append_kernel<E, false>, static_cast<unsigned>((p.num_tokens + tokens - 1) / tokens),
-                      tokens * 4 * p.vecs, 0, stream, p);
+  return launch_early(paired ? mrope_append_kernel<E, false, true> : mrope_append_kernel<E, false, false>,
+                      static_cast<unsigned>((p.num_tokens + tokens - 1) / tokens), threads, 0, stream, p);
 }
 
 }  // namespace
