@@ -21,9 +21,9 @@
 // Measured (B200, 8 KV heads of 128 dims).  Bounds of 16 sequences of up to
 // 8191 tokens: 36.3 us, 3.1 TB/s, the integer and minimum pipe at two thirds;
 // of one new page in each of 64 sequences 3.1 us.  Scores and selection over
-// 64 sequences of up to 16384 tokens: 33.8 us, 3.6 TB/s, the scores 3/4 of it,
-// waiting for bounds; one sequence of 131072 tokens 16.3 us, two launches and
-// their chains of dependent loads.
+// 64 sequences of up to 16384 tokens: 32.9 us, 3.7 TB/s; the scores take 26 of
+// them, 23 at 5.4 TB/s behind a start of 3.5.  One sequence of 131072 tokens
+// 10.8 us, two launches and their chains of dependent loads.
 #include "elem.cuh"
 
 namespace iris {
@@ -242,20 +242,20 @@ struct ScoreParams {
   int64_t num_pages;
   int32_t max_pages;
   int32_t kv_heads, group;
-  int32_t octets;        // 8-page groups per CTA
-  int32_t cta_heads;     // KV heads per CTA
+  int32_t cta_heads;  // KV heads per CTA
   int32_t max_keep;
   int32_t* err;
 };
 
 constexpr int kScoreWarps = 8;
-constexpr int kScoreStages = 3;  // units of a warp in flight and in use
+constexpr int kScoreStages = 2;  // units of a warp in flight and in use
 
-// Four adjacent k-steps of m16n8k32 share one 16-byte load a lane: lane t of
-// a quad holds bytes 16 t .. 16 t + 15 of a 64-byte span, words 0 and 1 of
-// which are one product's two B registers and words 2 and 3 the next one's.
-// The query's codes are read with the same assignment, so the sum runs over
-// the span in another order than in memory, which whole numbers do not mind.
+// Two adjacent k-steps of m16n8k32 share one 16-byte load a lane: lane t of
+// a quad holds bytes 16 t .. 16 t + 15 of a 64-byte span of its page, words 0
+// and 1 of which are one product's two A registers of that page and words 2
+// and 3 the next one's.  The query's codes are read with the same assignment,
+// so the sum runs over the span in another order than in memory, which whole
+// numbers do not mind.
 IRIS_DEV void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -270,9 +270,9 @@ IRIS_DEV uint32_t ordered(float f) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// A ring slot: each lane's four 16-byte pieces, then its page's step.
+// A ring slot: each lane's 16-byte pieces of its two pages, then their steps.
 template <int D>
-constexpr int kSlotBytes = 2 * D / 64 * 512 + 128;
+constexpr int kSlotBytes = 2 * (2 * D / 64 * 512 + 128);
 
 IRIS_DEV void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -281,10 +281,10 @@ IRIS_DEV void copy4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// One CTA a run of octets (8 pages each) of one sequence and some of its KV
-// heads; its warps share the (KV head, octet) units.  A unit's bounds are a product of 16 rows (query
-// heads) x 8 columns (pages); two units ahead of it are on their way to shared
-// memory.  kWide: more than 8 query heads a KV head (rows 8 .. 15).
+// One CTA a part of one sequence's pages and some of its KV heads; its warps
+// share the units, (KV head, 16 pages).  A unit's bounds are a product of 16
+// rows (pages) x 8 columns (query heads; kWide, more than 8 a KV head: two of
+// them); the unit after it is on its way to shared memory.
 template <typename E, int D, bool kWide>
 __global__ void __launch_bounds__(32 * kScoreWarps, 3) score_kernel(const ScoreParams p) {
   // codes of the query heads: [Hq][min(c, 0) : D][max(c, 0) : D], rows padded by 16 bytes; their units;
@@ -296,75 +296,14 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 3) score_kernel(const ScoreP
   grid_dependents_launch();  // the selection may come up meanwhile
   const int b = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int len = __ldg(p.seq_lens + b);
   const int head0 = blockIdx.z * p.cta_heads;  // this CTA's first KV head
-  const bool first = blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0;
-  if (len < 0 && first) set_error(p.err, IRIS_ERR_SEQ_LEN);
-  const int64_t all = len > 0 ? (static_cast<int64_t>(len) + kPage - 1) / kPage : 0;
-  if (all > p.max_pages && first) set_error(p.err, IRIS_ERR_BLOCK_TABLE);
-  const int n = static_cast<int>(all < p.max_pages ? all : p.max_pages);
-  const int oct0 = blockIdx.x * p.octets;
-  if (n <= p.max_keep || oct0 * 8 >= n) return;  // every page is kept, or none of these exist
-  const int g = lane >> 2, t = lane & 3;
-  const int octs = min(p.octets, (n + 7) / 8 - oct0);
-  // units of work: (head, octet), a contiguous run of them for each warp
-  const int total = p.cta_heads * octs;
-  const int lo = total * warp / kScoreWarps, hi = total * (warp + 1) / kScoreWarps;
-  // Page numbers are asked for a unit before the copies that need them.
-  const int32_t* table = p.block_table + b * p.table_stride + oct0 * 8 + g;
-  const int cols = n - oct0 * 8 - g;  // this lane's pages, one an octet
-  const auto page_of = [&](int oct) -> int32_t { return oct * 8 < cols ? __ldg(table + oct * 8) : 0; };
-  int h1 = lo / octs, oct1 = lo - h1 * octs;  // the unit whose bounds are loaded next
-  const auto advance = [&](int& h, int& oct) {
-    if (++oct == octs) {
-      oct = 0;
-      ++h;
-    }
-  };
-  int32_t page1 = lo < hi ? page_of(oct1) : 0, page2 = 0;  // its pages, and those of the one after it
+  const int len = __ldg(p.seq_lens + b);
+  // the warp's first query heads (heads warp, warp + 8, ..) are asked for together with the length
   const int heads = p.cta_heads * p.group;
-  uint8_t* codes = smem;
-  float* units = reinterpret_cast<float*>(smem + heads * kRow);  // [Hq]
-  // A lane copies and reads back its own 16 bytes of each span, so that a slot needs no barrier.
-  uint8_t* ring = smem + (heads * (kRow + 4) + 15) / 16 * 16 + warp * kScoreStages * kSlotBytes<D> + 16 * lane;
-  const int8_t* bounds = p.bounds + 16 * t;
-  const auto load_unit = [&](int i) {
-    if (i < hi) {
-      if (page1 < 0 || page1 >= p.num_pages) {
-        set_error(p.err, IRIS_ERR_PAGE_ID);
-        page1 = 0;
-      }
-      const int64_t row = static_cast<int64_t>(page1) * p.kv_heads + head0 + h1;
-      const int8_t* src = bounds + row * 2 * D;
-      const uint32_t dst = smem_u32(ring + (i - lo) % kScoreStages * kSlotBytes<D>);
-#pragma unroll
-      for (int k = 0; k < kSpans; ++k) copy16(dst + 512 * k, src + 64 * k);
-      copy4(dst + 512 * kSpans - 12 * lane, p.step + row);
-      advance(h1, oct1);
-      page1 = page2;
-      if (i + 2 < hi) {
-        int h2 = h1, oct2 = oct1;
-        advance(h2, oct2);
-        page2 = page_of(oct2);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  if (lo + 1 < hi) {
-    int h2 = h1, oct2 = oct1;
-    advance(h2, oct2);
-    page2 = page_of(oct2);
-  }
-
-  // the first units' bounds, on their way while the heads are quantised
-#pragma unroll
-  for (int j = 0; j < kScoreStages - 1; ++j) load_unit(lo + j);
-
-  // Quantise the query heads, four of a warp at a time.
   constexpr int W = D / 64;  // words a lane
   constexpr int kAtOnce = 4;
-  for (int i0 = warp; i0 < heads; i0 += kAtOnce * kScoreWarps) {
-    uint32_t q[kAtOnce][W];
+  uint32_t q[kAtOnce][W];
+  const auto load_queries = [&](int i0) {
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
       const int i = i0 + j * kScoreWarps;
@@ -374,6 +313,86 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 3) score_kernel(const ScoreP
                                     ((static_cast<int64_t>(b) * p.kv_heads + head0) * p.group + i) * (D / 2) + lane * W + k)
                             : 0u;
     }
+  };
+  load_queries(warp);
+  const bool first = blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0;
+  if (len < 0 && first) set_error(p.err, IRIS_ERR_SEQ_LEN);
+  const int64_t all = len > 0 ? (static_cast<int64_t>(len) + kPage - 1) / kPage : 0;
+  if (all > p.max_pages && first) set_error(p.err, IRIS_ERR_BLOCK_TABLE);
+  const int n = static_cast<int>(all < p.max_pages ? all : p.max_pages);
+  const int sixteens = (n + 15) / 16, share = (sixteens + gridDim.x - 1) / gridDim.x, unit0 = blockIdx.x * share;
+  if (n <= p.max_keep || unit0 >= sixteens) return;  // every page is kept, or none of these exist
+  const int g = lane >> 2, t = lane & 3;
+  const int count = min(share, sixteens - unit0);  // a head
+  const int total = p.cta_heads * count;           // a contiguous run of them for each warp
+  const int lo = total * warp / kScoreWarps, hi = total * (warp + 1) / kScoreWarps;
+  // Page numbers are asked for a unit before the copies that need them.
+  const int page0 = unit0 * 16 + g;  // this lane's first page; its others: 8 after it, and 16 a unit on
+  const int32_t* table = p.block_table + b * p.table_stride + page0;
+  const auto page_of = [&](int u, int half) -> int32_t {
+    return page0 + 16 * u + 8 * half < n ? __ldg(table + 16 * u + 8 * half) : 0;
+  };
+  int h1 = lo / count, u1 = lo - h1 * count;  // the unit whose bounds are loaded next
+  const auto advance = [&](int& h, int& u) {
+    if (++u == count) {
+      u = 0;
+      ++h;
+    }
+  };
+  int h = h1, u = u1;
+  int32_t page[2] = {0, 0}, after[2] = {0, 0};  // its pages, and those of the unit after it
+  if (lo < hi) {
+    page[0] = page_of(u1, 0);
+    page[1] = page_of(u1, 1);
+  }
+  uint8_t* codes = smem;
+  float* units = reinterpret_cast<float*>(smem + heads * kRow);  // [Hq]
+  // A lane copies and reads back its own 16 bytes of each span, so that a slot needs no barrier.
+  uint8_t* ring = smem + (heads * (kRow + 4) + 15) / 16 * 16 + warp * kScoreStages * kSlotBytes<D> + 16 * lane;
+  const int8_t* bounds = p.bounds + 16 * t;
+  const uint32_t page_bytes = static_cast<uint32_t>(p.kv_heads) * (2 * D);  // (at most 2^14 heads)
+  int fill = 0;  // the slot of the unit that is loaded next
+  const auto load_unit = [&](int i) {
+    if (i < hi) {
+      const int head = head0 + h1;
+      const uint32_t dst = smem_u32(ring + fill * kSlotBytes<D>);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (page[half] < 0 || page[half] >= p.num_pages) {
+          set_error(p.err, IRIS_ERR_PAGE_ID);
+          page[half] = 0;
+        }
+        const int8_t* src = bounds + static_cast<int64_t>(page[half]) * page_bytes + head * (2 * D);
+#pragma unroll
+        for (int k = 0; k < kSpans; ++k) copy16(dst + 512 * (2 * k + half), src + 64 * k);
+        copy4(dst + 1024 * kSpans + 128 * half - 12 * lane, p.step + static_cast<int64_t>(page[half]) * p.kv_heads + head);
+        page[half] = after[half];
+      }
+      advance(h1, u1);
+      if (i + 2 < hi) {
+        int h2 = h1, u2 = u1;
+        advance(h2, u2);
+        after[0] = page_of(u2, 0);
+        after[1] = page_of(u2, 1);
+      }
+      fill = fill + 1 == kScoreStages ? 0 : fill + 1;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (lo + 1 < hi) {
+    int h2 = h1, u2 = u1;
+    advance(h2, u2);
+    after[0] = page_of(u2, 0);
+    after[1] = page_of(u2, 1);
+  }
+
+  // the first units' bounds, on their way while the heads are quantised
+#pragma unroll
+  for (int j = 0; j < kScoreStages - 1; ++j) load_unit(lo + j);
+
+  // Quantise the query heads, four of a warp at a time.
+  for (int i0 = warp; i0 < heads; i0 += kAtOnce * kScoreWarps) {
+    if (i0 != warp) load_queries(i0);
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
       const int i = i0 + j * kScoreWarps;
@@ -414,68 +433,64 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 3) score_kernel(const ScoreP
   }
   __syncthreads();
 
-  int head = -1, h = lo / octs, oct = lo - h * octs;
-  uint32_t a[kSpans][kWide ? 8 : 4];
-  float u0 = 0.0f, u1 = 0.0f;
-  uint32_t* out = p.keys + (static_cast<int64_t>(b) * p.kv_heads + head0 + h) * p.key_stride + oct0 * 8 + 2 * t;
-  for (int i = lo; i < hi; ++i) {
+  int head = -1, use = 0;
+  uint4 code[kWide ? 2 : 1][kSpans];  // codes of query head g (and g + 8): the product's column
+  float unit[kWide ? 4 : 2];       // of query heads 2 t, 2 t + 1 (and 8 after them): the results' columns
+  uint32_t* out = p.keys + (static_cast<int64_t>(b) * p.kv_heads + head0) * p.key_stride + unit0 * 16;
+  for (int i = lo; i < hi; ++i, advance(h, u)) {
     load_unit(i + kScoreStages - 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(kScoreStages - 1) : "memory");
-    const uint8_t* slot = ring + (i - lo) % kScoreStages * kSlotBytes<D>;
-    uint4 w[kSpans];
-#pragma unroll
-    for (int k = 0; k < kSpans; ++k) w[k] = *reinterpret_cast<const uint4*>(slot + 512 * k);
-    const float step = *reinterpret_cast<const float*>(slot + 512 * kSpans - 12 * lane);
     if (h != head) {
       head = h;
-      const uint8_t* row = codes + (h * p.group + g) * kRow + 16 * t;
-      const bool one = g < p.group, two = kWide && g + 8 < p.group;
 #pragma unroll
-      for (int k = 0; k < kSpans; ++k) {
-        const uint4 x = one ? *reinterpret_cast<const uint4*>(row + 64 * k) : make_uint4(0, 0, 0, 0);
-        a[k][0] = x.x, a[k][1] = x.y, a[k][2] = x.z, a[k][3] = x.w;
-        if constexpr (kWide) {
-          const uint4 y = two ? *reinterpret_cast<const uint4*>(row + 8 * kRow + 64 * k) : make_uint4(0, 0, 0, 0);
-          a[k][4] = y.x, a[k][5] = y.y, a[k][6] = y.z, a[k][7] = y.w;
-        }
+      for (int w = 0; w < (kWide ? 2 : 1); ++w) {
+        const int hq = g + 8 * w, cols = 2 * t + 8 * w;
+#pragma unroll
+        for (int k = 0; k < kSpans; ++k)
+          code[w][k] = hq < p.group ? *reinterpret_cast<const uint4*>(codes + (h * p.group + hq) * kRow + 16 * t + 64 * k)
+                                 : make_uint4(0, 0, 0, 0);
+        unit[2 * w] = cols < p.group ? units[h * p.group + cols] : 0.0f;
+        unit[2 * w + 1] = cols + 1 < p.group ? units[h * p.group + cols + 1] : 0.0f;
       }
-      u0 = one ? units[h * p.group + g] : 0.0f;
-      u1 = two ? units[h * p.group + g + 8] : 0.0f;
     }
+    asm volatile("cp.async.wait_group %0;" ::"n"(kScoreStages - 1) : "memory");
+    const uint8_t* slot = ring + use * kSlotBytes<D>;
+    use = use + 1 == kScoreStages ? 0 : use + 1;
     // sums start at the bits of 1.5 2^23, so that their own are a float's: below 2^22, they come out exact
     constexpr int kStart = 0x4B400000;
-    int acc[4] = {kStart, kStart, kStart, kStart};
+    int acc[kWide ? 2 : 1][4];
+#pragma unroll
+    for (int w = 0; w < (kWide ? 2 : 1); ++w) acc[w][0] = acc[w][1] = acc[w][2] = acc[w][3] = kStart;
 #pragma unroll
     for (int k = 0; k < kSpans; ++k) {
-      mma_s8(acc, a[k][0], kWide ? a[k][4] : 0u, a[k][1], kWide ? a[k][5] : 0u, w[k].x, w[k].y);
-      mma_s8(acc, a[k][2], kWide ? a[k][6] : 0u, a[k][3], kWide ? a[k][7] : 0u, w[k].z, w[k].w);
+      const uint4 x = *reinterpret_cast<const uint4*>(slot + 1024 * k), y = *reinterpret_cast<const uint4*>(slot + 1024 * k + 512);
+#pragma unroll
+      for (int w = 0; w < (kWide ? 2 : 1); ++w) {
+        mma_s8(acc[w], x.x, y.x, x.y, y.y, code[w][k].x, code[w][k].y);
+        mma_s8(acc[w], x.z, y.z, x.w, y.w, code[w][k].z, code[w][k].w);
+      }
     }
-    // acc: head g (and g + 8), pages 2 t and 2 t + 1 of the octet
-    const float s0 = __shfl_sync(0xffffffffu, step, 8 * t), s1 = __shfl_sync(0xffffffffu, step, 8 * t + 4);
+    // the maxima over the heads of pages g and g + 8
+    const float s0 = *reinterpret_cast<const float*>(slot + 1024 * kSpans - 12 * lane);
+    const float s1 = *reinterpret_cast<const float*>(slot + 1024 * kSpans + 128 - 12 * lane);
     const auto score = [](int sum, float step, float unit) {
       return __fmul_rn(__fmul_rn(__int_as_float(sum) - 12582912.0f, step), unit);
     };
     float m0 = -INFINITY, m1 = -INFINITY;
-    if (g < p.group) {
-      m0 = score(acc[0], s0, u0);
-      m1 = score(acc[1], s1, u0);
+#pragma unroll
+    for (int c = 0; c < (kWide ? 4 : 2); ++c) {
+      if (2 * t + (c & 1) + 8 * (c >> 1) < p.group) {
+        m0 = fmaxf(m0, score(acc[c >> 1][c & 1], s0, unit[c]));
+        m1 = fmaxf(m1, score(acc[c >> 1][2 + (c & 1)], s1, unit[c]));
+      }
     }
-    if (kWide && g + 8 < p.group) {
-      m0 = fmaxf(m0, score(acc[2], s0, u1));
-      m1 = fmaxf(m1, score(acc[3], s1, u1));
-    }
-    // the maximum over the heads; the first exchange leaves page 2 t to the lanes of even g, 2 t + 1 to the others
-    const bool odd = g & 1;
-    float m = fmaxf(odd ? m1 : m0, __shfl_xor_sync(0xffffffffu, odd ? m0 : m1, 4));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+    // the first exchange leaves page g to the lanes of even t, g + 8 to the others
+    const bool odd = t & 1;
+    float m = fmaxf(odd ? m1 : m0, __shfl_xor_sync(0xffffffffu, odd ? m0 : m1, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
     // a page whose keys are not all finite comes before every other
-    if (g < 2) out[oct * 8 + g] = (odd ? s1 : s0) <= 3.402823466e38f ? ordered(m) : ordered(INFINITY);
-    if (++oct == octs) {
-      oct = 0;
-      ++h;
-      out += p.key_stride;
-    }
+    if (t < 2 && page0 + 16 * u + 8 * t < n)
+      out[h * p.key_stride + 16 * u + 8 * t + g] =
+          (odd ? s1 : s0) <= 3.402823466e38f ? ordered(m) : ordered(INFINITY);
   }
 }
 
@@ -515,9 +530,9 @@ IRIS_DEV uint32_t select_key(const SelectParams& p, const SelectRow& r, int i, u
 IRIS_DEV bool scored(uint32_t key) { return key != 0u && key != 0xffffffffu; }
 
 // The highest `keep` keys are those above a threshold, the largest one that at
-// least `keep` keys reach, and the first of those equal to it.  The threshold
-// is found bit by bit by counting, from the highest bit in which the scored
-// keys differ at all; a count that hits `keep` ends the search.
+// least `keep` keys reach, and the first of those equal to it.  A warp with a
+// short row finds it bit by bit by counting, from the highest bit in which the
+// scored keys differ at all; a count that hits `keep` ends the search.
 struct Search {
   uint32_t thr;
   int bit;  // the next one to decide; -1: none
@@ -592,6 +607,12 @@ __global__ void __launch_bounds__(128) select_warp_kernel(const SelectParams p) 
   }
 }
 
+// The bin in which the wanted number of keys is reached, the keys in the bins
+// before it and in it.
+struct Bin {
+  int index, before, count;
+};
+
 // What the warps of a row tell one another: an array entry a warp, in the
 // shared memory of each of the row's CTAs.  put() leaves a warp's value there,
 // meet() waits for all warps' (every CTA of a cluster comes to it), and then
@@ -626,6 +647,60 @@ struct Board {
     for (int i = threadIdx.x & 31; i < n; i += 32) v += board[i];
     return static_cast<int>(__reduce_add_sync(0xffffffffu, v));
   }
+  // the first of 256 bins, over all CTAs' counts, up to which there are at least `need` keys; for a whole warp
+  IRIS_DEV static Bin find(const uint32_t* bins, int need) {
+    const int lane = threadIdx.x & 31;
+    uint32_t c[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < kCtas; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {
+        const uint32_t* at = bins + 8 * lane + j;
+        uint4 v;
+        if constexpr (kCtas == 1) {
+          v = *reinterpret_cast<const uint4*>(at);
+        } else {
+          uint32_t from;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(smem_u32(at)), "r"(i));
+          asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                       : "r"(from)
+                       : "memory");
+        }
+        c[j] += v.x;
+        c[j + 1] += v.y;
+        c[j + 2] += v.z;
+        c[j + 3] += v.w;
+      }
+    }
+    int sum = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += static_cast<int>(c[j]);
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const int who = __ffs(__ballot_sync(0xffffffffu, upto >= need)) - 1;
+    Bin b = {8 * lane, upto - sum, 0};
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (!found) {
+        b.count = static_cast<int>(c[j]);
+        found = b.before + b.count >= need;
+        if (!found) {
+          b.before += b.count;
+          ++b.index;
+        }
+      }
+    }
+    b.index = __shfl_sync(0xffffffffu, b.index, who);
+    b.before = __shfl_sync(0xffffffffu, b.before, who);
+    b.count = __shfl_sync(0xffffffffu, b.count, who);
+    return b;
+  }
   IRIS_DEV static uint32_t lowest(const uint32_t* board) {
     uint32_t v = 0xffffffffu;
     for (int i = threadIdx.x & 31; i < kEntries; i += 32) v = min(v, board[i]);
@@ -639,14 +714,17 @@ struct Board {
 };
 
 // kCtas CTAs (a cluster) per longer row: KPT consecutive keys a thread in
-// registers, or for KPT = 0 read again for every count.  Two bits of the
-// threshold at a time, which halves the barriers.  Counting is what takes the
-// time, so that a row of one long sequence goes over several SMs.
+// registers, or for KPT = 0 read again for every count.  The threshold is
+// found with histograms over the range that it still can lie in: two or three
+// rounds of one barrier, where two bits at a time took about eight (8 rows of
+// 8192 pages, with the scores: 13.7 -> 10.8 us).  A row of one long sequence
+// goes over several SMs.
 template <int kThreads, int KPT, int kCtas>
 __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) {
   using B = Board<kThreads, kCtas>;
-  __shared__ uint32_t s_part[6][B::kEntries];
   __shared__ uint32_t s_more[4][B::kEntries];
+  __shared__ __align__(16) uint32_t s_bins[4][256];
+  __shared__ Bin s_found;
   constexpr int kAll = kThreads * kCtas;
   const int row = blockIdx.x / kCtas, tid = B::rank() * kThreads + threadIdx.x, lane = threadIdx.x & 31;
   const SelectRow r = select_row(p, row);
@@ -657,6 +735,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
     grid_dependency_wait();  // (nothing here runs ahead of the kernels before)
     return;                  // (nor does any CTA of the row go on)
   }
+  for (int i = threadIdx.x; i < 256; i += kThreads) reinterpret_cast<uint4*>(s_bins)[i] = make_uint4(0, 0, 0, 0);
   grid_dependency_wait();  // the scores are there
   const auto key_at = [&](int i) { return select_key(p, r, i, i < r.n ? __ldcg(r.keys + i) : 0u); };
   constexpr int kRegs = KPT > 0 ? KPT : 1;
@@ -697,31 +776,41 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
   B::put(s_more[0], lowest);
   B::put(s_more[1], highest);
   B::meet();
-  const Search from = search_from(B::lowest(s_more[0]), B::highest(s_more[1]));
-  uint32_t thr = from.thr;
-  int slot = 0;  // alternates, so that one meeting a round is enough
-  for (int bit = from.bit - 1; bit >= -1; bit -= 2) {  // bits bit + 1 and bit (at -1, of bit 0 alone)
-    const uint32_t c2 = thr | 1u << (bit + 1), c1 = bit >= 0 ? thr | 1u << bit : c2, c3 = bit >= 0 ? c2 | 1u << bit : c2;
-    int n1 = 0, n2 = 0, n3 = 0;
+  uint32_t low = B::lowest(s_more[0]), high = B::highest(s_more[1]);
+  // The scored keys that are wanted lie in [low, high], and the last of them is to be found: 256 bins over the range,
+  // counted from the top, until one bin's keys are all wanted, or all the same.  (At most four rounds: 32 bits.)
+  int need = r.keep - p.sink - p.recent;  // (n > keep: the two ends do not meet)
+  uint32_t thr = high;                    // keys above it are taken, and the first `need` equal ones
+  for (int round = 0; need > 0; ++round) {
+    const uint32_t range = high - low;
+    const int shift = max(24 - __clz(range), 0);
+    uint32_t* bins = s_bins[round];
+    const auto count = [&](uint32_t x) {
+      if (x - low <= range) atomicAdd(bins + ((high - x) >> shift), 1u);
+    };
     if constexpr (KPT > 0) {
-      each([&](int, uint32_t x) { n1 += x >= c1, n2 += x >= c2, n3 += x >= c3; });
+      each([&](int, uint32_t x) { count(x); });
     } else {  // in any order
-      for (int i = tid; i < r.n; i += kAll) {
-        const uint32_t x = key_at(i);
-        n1 += x >= c1, n2 += x >= c2, n3 += x >= c3;
-      }
+      for (int i = tid; i < r.n; i += kAll) count(key_at(i));
     }
-    B::put(s_part[slot], __reduce_add_sync(0xffffffffu, n1));
-    B::put(s_part[slot + 1], __reduce_add_sync(0xffffffffu, n2));
-    B::put(s_part[slot + 2], __reduce_add_sync(0xffffffffu, n3));
     B::meet();
-    n1 = B::sum(s_part[slot]);
-    n2 = B::sum(s_part[slot + 1]);
-    n3 = B::sum(s_part[slot + 2]);
-    slot = 3 - slot;
-    thr = n3 >= r.keep ? c3 : n2 >= r.keep ? c2 : n1 >= r.keep ? c1 : thr;
-    const int got = n3 >= r.keep ? n3 : n2 >= r.keep ? n2 : n1 >= r.keep ? n1 : 0;
-    if (got == r.keep) break;  // exactly the wanted ones reach it
+    Bin bin;
+    if (kCtas == 1 || threadIdx.x < 32) bin = B::find(bins, need);
+    if constexpr (kCtas > 1) {
+      if (threadIdx.x == 0) s_found = bin;
+      __syncthreads();
+      bin = s_found;  // (next written behind another meeting)
+    }
+    need -= bin.before;
+    high -= static_cast<uint32_t>(bin.index) << shift;
+    low = max(low, high - ((1u << shift) - 1u));
+    if (bin.count == need) {  // exactly the wanted ones
+      thr = low - 1u;
+      need = 0;
+    } else if (shift == 0) {
+      thr = low;
+      break;
+    }
   }
   int above = 0, equal = 0;
   each([&](int, uint32_t x) {
@@ -737,7 +826,6 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
   B::put(s_more[2], __shfl_sync(0xffffffffu, a, 31));
   B::put(s_more[3], __shfl_sync(0xffffffffu, e, 31));
   B::meet();  // the last one: nothing is written to another CTA's memory after it
-  const int need = r.keep - B::sum(s_more[2]);
   a += B::sum(s_more[2], B::entry());
   e += B::sum(s_more[3], B::entry());
   int eq = e - equal, at = a - above + min(eq, need);
@@ -888,18 +976,18 @@ extern "C" int iris_b200_page_select(const void* query, const void* bounds, cons
   p.group = group;
   p.max_keep = max_pages;
   p.err = error_word;
-  const int octets = static_cast<int>(key_stride_of(max_pages_per_seq) / 8);
   // the score kernel also reports bad lengths, so it runs even where every page is kept
-  // Three CTAs an SM in all, as many a sequence as there are sequences for.  A CTA quantises the queries of its heads
-  // before it starts, so the heads are shared out first, as long as three CTAs a share of the heads are left for the
-  // pages (one sequence of 8192 pages, 64 heads: 17.9 -> 16.1 us with the selection).
-  int want = 3 * sm_count() / batch > 1 ? 3 * sm_count() / batch : 1;
+  // Two CTAs an SM in all, as many a sequence as there are sequences for (three: 36.7 instead of 33.0 us at 64 sequences,
+  // 15.9 instead of 14.0 at one, both with the selection: what a CTA does before its first unit then costs more than
+  // its loads hide).  A CTA quantises the queries of its heads before it starts, so the heads are shared out first, as
+  // long as three CTAs a share of the heads are left for the pages (one sequence of 8192 pages, 64 heads: 17.9 -> 16.1).
+  int want = 2 * sm_count() / batch > 1 ? 2 * sm_count() / batch : 1;
   int shares = 1;
   while (num_kv_heads % (2 * shares) == 0 && want / (2 * shares) >= 3) shares *= 2;
   want /= shares;
   p.cta_heads = num_kv_heads / shares;
-  p.octets = octets > 0 ? (octets + want - 1) / want : 1;
-  const dim3 grid(octets > 0 ? static_cast<unsigned>((octets + p.octets - 1) / p.octets) : 1u,
+  const int sixteens = (max_pages_per_seq + 15) / 16;
+  const dim3 grid(static_cast<unsigned>(want < sixteens ? want : sixteens > 0 ? sixteens : 1),
                   static_cast<unsigned>(batch), static_cast<unsigned>(shares));
   cudaError_t e = dtype == IRIS_DTYPE_FP16 ? launch_score<Fp16Elem>(p, head_dim, grid, s)
                                            : launch_score<Bf16Elem>(p, head_dim, grid, s);
