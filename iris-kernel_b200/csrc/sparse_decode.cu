@@ -225,8 +225,8 @@ struct SparseCfg {
 };
 
 // Shared memory of a warp: its ring, its row's query fragments, its slots' info.
-template <int D, bool kWide>
-constexpr int kWarpBytes = SparseCfg<D>::kRing + (kWide ? 2 : 1) * SparseCfg<D>::kGroups * 512 + 64;
+template <int D, int kHeads>
+constexpr int kWarpBytes = SparseCfg<D>::kRing + (kHeads > 8 ? 2 : 1) * SparseCfg<D>::kGroups * 512 + 64;
 
 // Byte offset of 16-byte chunk c of row r: rows 0, 2, 4, .. would start at the
 // same banks, so the chunks of a row are turned by a function of the row.
@@ -243,10 +243,14 @@ struct SlotInfo {
   int32_t row, left;
 };
 
-template <typename E, int D, bool kWide>
-__global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse_decode_kernel(SparseParams p) {
+// kHeads: 4, 8 or 16, what the group fits in.  With up to four query heads
+// the columns 4 to 7 are theirs again: rows 4 to 7 of S repeat rows 0 to 3, and
+// the second terms of the scaled weights take the place of a second product.
+template <typename E, int D, int kHeads>
+__global__ void __launch_bounds__(32 * kWarps, kHeads > 8 || D == 128 ? 3 : 5) sparse_decode_kernel(SparseParams p) {
   using C = SparseCfg<D>;
   constexpr int G4 = C::kGroups;
+  constexpr bool kWide = kHeads > 8, kTwice = kHeads == 4;
   constexpr int kH = kWide ? 2 : 1;  // query heads a lane has logits of: g, g + 8
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -262,7 +266,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
   if (first.row < 0) return;  // (nothing below waits for another warp)
   const int begin = me * length, end = min(begin + length, first.total);  // below 2^30 + the run
 
-  uint8_t* ring = smem + warp * (kWarpBytes<D, kWide>);
+  uint8_t* ring = smem + warp * (kWarpBytes<D, kHeads>);
   uint4* s_query = reinterpret_cast<uint4*>(ring + C::kRing);  // [half][group][lane]
   SlotInfo* info = reinterpret_cast<SlotInfo*>(ring + C::kRing + kH * G4 * 512);
   const uint32_t ring_addr = smem_u32(ring);
@@ -358,7 +362,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
       l[half] = 0.0f;
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) o[half][j][0] = o[half][j][1] = o[half][j][2] = o[half][j][3] = 0.0f;
-      const int hq = g + 8 * half;
+      const int hq = kTwice ? g & 3 : g + 8 * half;
       uint4 w[G4];
       float top = 0.0f;
 #pragma unroll
@@ -422,6 +426,13 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
           *reinterpret_cast<float2*>(p.part_ml + (part * p.group + hq) * 2) = make_float2(m[hh], l[hh]);
         else if (p.lse != nullptr)
           p.lse[static_cast<int64_t>(cur) * p.group + hq] = l[hh] == 0.0f ? -INFINITY : m[hh] + log2f(l[hh]);
+      }
+      if constexpr (kTwice) {  // the two terms' sums
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[hh][j][e] += __shfl_xor_sync(0xffffffffu, o[hh][j][e], 2);
+        }
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {  // columns 2 t and 2 t + 1: the heads of lanes 8 t and 8 t + 4
@@ -594,7 +605,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
     // O^T += V^T P^T
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) {
-      __half2 ph[kH][2], pl[kH][2];  // weights of the token pairs: rounded, and the rest
+      // weights of the token pairs: rounded, and the rest; kTwice: neither -ph nor the rest where the first term is wanted
+      __half2 ph[kH][2], pl[kH][2], minus[kH][2];
 #pragma unroll
       for (int hh = 0; hh < kH; ++hh) {
 #pragma unroll
@@ -602,6 +614,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
           ph[hh][n] = __floats2half2_rn(x[hh][pg][n].x, x[hh][pg][n].y);
           const float2 r = __half22float2(ph[hh][n]);
           pl[hh][n] = __floats2half2_rn(x[hh][pg][n].x - r.x, x[hh][pg][n].y - r.y);
+          minus[hh][n] = __hneg2(ph[hh][n]);
+          if (kTwice && g < 4) pl[hh][n] = minus[hh][n] = __float2half2_rn(0.0f);
         }
       }
 #pragma unroll
@@ -617,9 +631,9 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
             const __half2 sc = u32_as_h2(prmt(vs[pg][n][k / 2], vs[pg][n][(G4 + k) / 2], k % 2 == 0 ? 0x5410 : 0x7632));
 #pragma unroll
             for (int hh = 0; hh < kH; ++hh) {
-              const __half2 a = __hmul2_rn(ph[hh][n], sc);
-              const __half2 c = __hfma2(pl[hh][n], sc, __hfma2(ph[hh][n], sc, __hneg2(a)));
-              hi[hh][n] = h2_as_u32(a);
+              const __half2 a = __hmul2_rn(kTwice ? minus[hh][n] : ph[hh][n], sc);
+              const __half2 c = __hfma2(pl[hh][n], sc, __hfma2(ph[hh][n], sc, kTwice ? a : __hneg2(a)));
+              hi[hh][n] = h2_as_u32(kTwice ? c : a);
               lo[hh][n] = h2_as_u32(c);
             }
           }
@@ -632,7 +646,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWide || D == 128 ? 3 : 5) sparse
             for (int hh = 0; hh < kH; ++hh) {
               float(&acc)[4] = o[hh][2 * k + jj];
               mma_f16(acc, a, hi[hh][0], hi[hh][1], acc);
-              mma_f16(acc, a, lo[hh][0], lo[hh][1], acc);
+              if constexpr (!kTwice) mma_f16(acc, a, lo[hh][0], lo[hh][1], acc);
             }
           }
         }
@@ -758,17 +772,17 @@ struct Kernel {
   KernelFn join;
   int bytes;  // of shared memory
 };
-template <typename E, int D, bool kWide>
+template <typename E, int D, int kHeads>
 Kernel kernel() {
-  return {sparse_decode_kernel<E, D, kWide>, sparse_join_kernel<E, D>, kWarps * kWarpBytes<D, kWide>};
+  return {sparse_decode_kernel<E, D, kHeads>, sparse_join_kernel<E, D>, kWarps * kWarpBytes<D, kHeads>};
 }
-Kernel kernel_for(int dtype, int head_dim, bool wide) {
-  if (dtype == IRIS_DTYPE_FP16) {
-    if (head_dim == 128) return wide ? kernel<Fp16Elem, 128, true>() : kernel<Fp16Elem, 128, false>();
-    return wide ? kernel<Fp16Elem, 64, true>() : kernel<Fp16Elem, 64, false>();
-  }
-  if (head_dim == 128) return wide ? kernel<Bf16Elem, 128, true>() : kernel<Bf16Elem, 128, false>();
-  return wide ? kernel<Bf16Elem, 64, true>() : kernel<Bf16Elem, 64, false>();
+template <typename E>
+Kernel kernel_of(int head_dim, int group) {
+  if (head_dim == 128) return group > 8 ? kernel<E, 128, 16>() : group > 4 ? kernel<E, 128, 8>() : kernel<E, 128, 4>();
+  return group > 8 ? kernel<E, 64, 16>() : group > 4 ? kernel<E, 64, 8>() : kernel<E, 64, 4>();
+}
+Kernel kernel_for(int dtype, int head_dim, int group) {
+  return dtype == IRIS_DTYPE_FP16 ? kernel_of<Fp16Elem>(head_dim, group) : kernel_of<Bf16Elem>(head_dim, group);
 }
 
 struct SparseGrid {
@@ -815,7 +829,7 @@ extern "C" size_t iris_b200_sparse_decode_workspace_bytes(int32_t batch, int32_t
   size_t bytes = 0;
   for (const int dtype : {IRIS_DTYPE_FP16, IRIS_DTYPE_BF16}) {
     SparseGrid grid;
-    if (grid_for(kernel_for(dtype, head_dim, group > 8), static_cast<int64_t>(batch) * num_kv_heads, group, head_dim,
+    if (grid_for(kernel_for(dtype, head_dim, group), static_cast<int64_t>(batch) * num_kv_heads, group, head_dim,
                  max_pages, kMinSteps, &grid) != cudaSuccess) {
       bytes = 0;
       break;
@@ -851,7 +865,7 @@ extern "C" int iris_b200_int4_sparse_paged_decode(const void* query, const void*
     return IRIS_EALIGN;
   const int group = num_q_heads / num_kv_heads;
   const int64_t rows = static_cast<int64_t>(batch) * num_kv_heads;
-  const Kernel k = kernel_for(dtype, head_dim, group > 8);
+  const Kernel k = kernel_for(dtype, head_dim, group);
   clear_stale_cuda_error();
   SparseGrid grid;
   cudaError_t e = grid_for(k, rows, group, head_dim, max_pages, kMinSteps, &grid);
