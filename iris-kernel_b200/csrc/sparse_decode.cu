@@ -16,7 +16,7 @@
 // 128 dims: 49.2 -> 40.8 us).
 //
 // Products run on the tensor cores with fp16 operands and fp32 accumulation:
-//   S = Q K^T      rows = query heads, columns = tokens, one accumulator per
+//   S^T = K Q^T    rows = tokens, columns = query heads, one accumulator per
 //                  32-dim group, the group scale applied in fp32.  A nibble n
 //                  enters as the subnormal fp16 (n + 8) 2^-24, one logic
 //                  operation for two; -8 sum(q) 2^-24 is added to the
@@ -27,8 +27,10 @@
 //                  weight p is two fp16 terms, p * scale again two: the rounded
 //                  product and, by fused multiply-adds, what it left off (22
 //                  bits, no step finer than 2^-24; scales are at least 2^-14).
-//                  S's accumulator registers are the fragment of P^T as they
-//                  are.
+//                  S^T's accumulators become the fragment of P^T by a transposing
+//                  move of 8 x 8 matrices, which costs less than S = Q K^T, whose
+//                  accumulators are that fragment, and whose products are twice
+//                  as many with up to eight heads.
 // A 16-byte chunk of a page's row is one group: ldmatrix hands each lane the
 // eight dims of a token that its place in K's fragment needs, and its
 // transposing form four dims of two tokens, as V's fragment needs them.
@@ -42,11 +44,12 @@
 // kernel joins them in the order of the list.
 //
 // Measured (B200): 64 sequences x 128 pages of 8192 tokens, 32 + 8 heads of 128
-// dims: 62.7 us, 2.4 TB/s of the bytes it needs (DRAM moves 1.5 times those:
-// other heads' scales share a sector).  Bound by instructions: about 440 a page
-// and warp at half an instruction a cycle, three CTAs of 168 registers an SM
-// (four CTAs spill: 73 us); with the pages in L2 it takes 54.  One sequence,
-// 128 pages: 11.6 us, a chain of launches and dependent loads.
+// dims: 56.2 us, 2.7 TB/s of the bytes it needs (DRAM moves 1.5 times those:
+// other heads' scales share a sector).  Bound by instructions, about 400 a page
+// and warp at half an instruction a cycle, three CTAs of 158 registers an SM.
+// 96 x 45 pages, 16 heads of 64 dims: 51.4 us; DRAM moves 200 MB, 2.5 times what
+// is needed.  One sequence, 128 pages: 11.6 us, a chain of launches and
+// dependent loads.
 #include <map>
 #include <mutex>
 #include <type_traits>
@@ -132,6 +135,13 @@ IRIS_DEV void load_matrices_transposed(uint32_t (&r)[4], uint32_t addr) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
+}
+
+// An 8 x 8 matrix of 16-bit elements, two adjacent ones of row lane / 4 a lane, transposed.
+IRIS_DEV uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 // Signed nibbles n of w as (n + 8) in place: (w ^ 8) & 15.  Read as fp16, the
@@ -244,14 +254,17 @@ struct SlotInfo {
 };
 
 // kHeads: 4, 8 or 16, what the group fits in.  With up to four query heads
-// the columns 4 to 7 are theirs again: rows 4 to 7 of S repeat rows 0 to 3, and
-// the second terms of the scaled weights take the place of a second product.
+// the columns 4 to 7 are theirs again, and the second terms of the scaled
+// weights take the place of a second product (64 x 128 pages: 62.3 -> 59.0 us).
+// CTAs an SM, by registers: 16 heads of 128 dims 2 (82.7 us; 3 spill: 107), of
+// 64 dims 3 (54.7; 2 or 4: 56.1); fewer heads of 128 dims 3 (4 spill), of 64
+// dims 5 (96 x 45 pages 51.4; 4: 52.1, 6: 53.9).
 template <typename E, int D, int kHeads>
-__global__ void __launch_bounds__(32 * kWarps, kHeads > 8 || D == 128 ? 3 : 5) sparse_decode_kernel(SparseParams p) {
+__global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) : (kHeads > 8 ? 3 : 5)) sparse_decode_kernel(SparseParams p) {
   using C = SparseCfg<D>;
   constexpr int G4 = C::kGroups;
   constexpr bool kWide = kHeads > 8, kTwice = kHeads == 4;
-  constexpr int kH = kWide ? 2 : 1;  // query heads a lane has logits of: g, g + 8
+  constexpr int kH = kWide ? 2 : 1;  // eights of query heads; a lane has logits of heads 2 t and 2 t + 1 of each
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -348,7 +361,7 @@ __global__ void __launch_bounds__(32 * kWarps, kHeads > 8 || D == 128 ? 3 : 5) s
   // ---- state of the row at hand ----
   constexpr int kTiles = D / 16;  // of 16 dims; a lane has two dims of each for heads 2 t, 2 t + 1 (+ 8)
   float o[kH][kTiles][4];
-  float m[kH], l[kH], q_sum[kH][G4], head_scale[kH];
+  float2 m[kH], minus_base[kH], l[kH], q_sum[kH][G4], head_scale[kH];  // (l: of this lane's tokens)
   int cur = -1, cur_start = first.start;
 
   // Query fragments.  Of this lane's eight dims of a group, the first product
@@ -358,8 +371,8 @@ __global__ void __launch_bounds__(32 * kWarps, kHeads > 8 || D == 128 ? 3 : 5) s
     __syncwarp();  // the last row's fragments have been read
 #pragma unroll
     for (int half = 0; half < kH; ++half) {
-      m[half] = -INFINITY;
-      l[half] = 0.0f;
+      m[half] = make_float2(-INFINITY, -INFINITY);
+      minus_base[half] = l[half] = make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) o[half][j][0] = o[half][j][1] = o[half][j][2] = o[half][j][3] = 0.0f;
       const int hq = kTwice ? g & 3 : g + 8 * half;
@@ -382,7 +395,10 @@ __global__ void __launch_bounds__(32 * kWarps, kHeads > 8 || D == 128 ? 3 : 5) s
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
       const float down = __uint_as_float((254u - e) << 23);  // 2^-(e - 127)
-      head_scale[half] = (p.scale_log2 * 16777216.0f) * __uint_as_float(e << 23);
+      const auto of_columns = [&](float x) {  // head g's -> heads 2 t and 2 t + 1's
+        return make_float2(__shfl_sync(0xffffffffu, x, 8 * t), __shfl_sync(0xffffffffu, x, 8 * t + 4));
+      };
+      head_scale[half] = of_columns((p.scale_log2 * 16777216.0f) * __uint_as_float(e << 23));
 #pragma unroll
       for (int k = 0; k < G4; ++k) {
         const uint32_t v[4] = {w[k].x, w[k].y, w[k].z, w[k].w};  // dims (0,1) (2,3) (4,5) (6,7)
@@ -404,7 +420,7 @@ __global__ void __launch_bounds__(32 * kWarps, kHeads > 8 || D == 128 ? 3 : 5) s
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        q_sum[half][k] = sum * -4.76837158203125e-07f;  // -8 2^-24
+        q_sum[half][k] = of_columns(sum * -4.76837158203125e-07f);  // -8 2^-24
       }
     }
     // (each lane reads back only what it wrote)
@@ -417,15 +433,23 @@ __global__ void __launch_bounds__(32 * kWarps, kHeads > 8 || D == 128 ? 3 : 5) s
     if (starts && lane == 0) p.row_start[cur] = cur_start;
 #pragma unroll
     for (int hh = 0; hh < kH; ++hh) {
-      l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
-      l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
-      const int hq = g + 8 * hh;
-      const float inv = l[hh] == 0.0f ? 0.0f : __fdiv_rn(1.0f, l[hh]);
-      if (t == 0 && hq < p.group) {
-        if (!whole)
-          *reinterpret_cast<float2*>(p.part_ml + (part * p.group + hq) * 2) = make_float2(m[hh], l[hh]);
-        else if (p.lse != nullptr)
-          p.lse[static_cast<int64_t>(cur) * p.group + hq] = l[hh] == 0.0f ? -INFINITY : m[hh] + log2f(l[hh]);
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        l[hh].x += __shfl_xor_sync(0xffffffffu, l[hh].x, d);
+        l[hh].y += __shfl_xor_sync(0xffffffffu, l[hh].y, d);
+      }
+      const float lv[2] = {l[hh].x, l[hh].y}, mv[2] = {m[hh].x, m[hh].y};
+      float inv[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int hq = 2 * t + e + 8 * hh;
+        inv[e] = lv[e] == 0.0f ? 0.0f : __fdiv_rn(1.0f, lv[e]);
+        if (g == 0 && hq < p.group) {
+          if (!whole)
+            *reinterpret_cast<float2*>(p.part_ml + (part * p.group + hq) * 2) = make_float2(mv[e], lv[e]);
+          else if (p.lse != nullptr)
+            p.lse[static_cast<int64_t>(cur) * p.group + hq] = lv[e] == 0.0f ? -INFINITY : mv[e] + log2f(lv[e]);
+        }
       }
       if constexpr (kTwice) {  // the two terms' sums
 #pragma unroll
@@ -435,9 +459,9 @@ __global__ void __launch_bounds__(32 * kWarps, kHeads > 8 || D == 128 ? 3 : 5) s
         }
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {  // columns 2 t and 2 t + 1: the heads of lanes 8 t and 8 t + 4
+      for (int e = 0; e < 2; ++e) {
         const int head = 2 * t + e + 8 * hh;
-        const float f = __shfl_sync(0xffffffffu, inv, 8 * t + 4 * e);
+        const float f = inv[e];
         if (head < p.group) {
 #pragma unroll
           for (int k = 0; k < G4; ++k) {  // this lane's four dims of the group are adjacent
@@ -471,12 +495,7 @@ __global__ void __launch_bounds__(32 * kWarps, kHeads > 8 || D == 128 ? 3 : 5) s
       }
     }
   };
-  // group k's scales of the two tokens
-  const auto scale_pair = [&](const uint32_t (&w)[G4], int k) {
-    const float2 a = __half22float2(u32_as_h2(w[k / 2])), c = __half22float2(u32_as_h2(w[(G4 + k) / 2]));
-    return k % 2 == 0 ? make_float2(a.x, c.x) : make_float2(a.y, c.y);
-  };
-
+  const uint32_t second_term = g < 4 ? 0u : 0xffffffffu;  // kTwice
   int slot = -2;
   for (int step = begin; step < end; ++step) {
     __syncwarp();  // every lane is done with the slots that are filled next
@@ -498,35 +517,54 @@ __global__ void __launch_bounds__(32 * kWarps, kHeads > 8 || D == 128 ? 3 : 5) s
     const uint8_t* st = ring + slot * C::kStage;
     const uint32_t st_addr = ring_addr + slot * C::kStage;
 
-    // S = Q K^T, one accumulator per group, scaled in fp32 (2^-24 and the query's power of two left out)
-    float2 x[kH][2][2];  // [head][page][token pair]
+    // S^T = K Q^T, one accumulator per group, scaled in fp32 (2^-24 and the query's power of two left out)
+    float2 x[kH][2][2];  // [eight][page][token g | g + 8]: heads 2 t and 2 t + 1
     {
-      uint32_t ks[2][2][G4];
+      uint32_t ks[2][2][G4 / 2];  // [page][token][groups, two a word]
 #pragma unroll
-      for (int pg = 0; pg < 2; ++pg) scale_words(st + pg * C::kStage + 2 * C::kData, ks[pg]);
+      for (int pg = 0; pg < 2; ++pg) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint8_t* at = st + pg * C::kStage + 2 * C::kData + (g + 8 * r) * (2 * G4);
+          if constexpr (G4 == 4) {
+            const uint2 v = *reinterpret_cast<const uint2*>(at);
+            ks[pg][r][0] = v.x, ks[pg][r][1] = v.y;
+          } else {
+            ks[pg][r][0] = *reinterpret_cast<const uint32_t*>(at);
+          }
+        }
+      }
 #pragma unroll
       for (int k0 = 0; k0 < G4; k0 += 2) {
         uint32_t kw[2][4];  // [page][group k0, tokens 0-7 | 8-15, group k0 + 1, ..]
+        float2 sc[2][2];    // [page][token]: of groups k0 and k0 + 1
 #pragma unroll
-        for (int pg = 0; pg < 2; ++pg) load_matrices(kw[pg], st_addr + pg * C::kStage + (mat ^ (16 * k0)));
+        for (int pg = 0; pg < 2; ++pg) {
+          load_matrices(kw[pg], st_addr + pg * C::kStage + (mat ^ (16 * k0)));
+#pragma unroll
+          for (int r = 0; r < 2; ++r) sc[pg][r] = __half22float2(u32_as_h2(ks[pg][r][k0 / 2]));
+        }
 #pragma unroll
         for (int k = k0; k < k0 + 2; ++k) {
-          const uint4 q0 = s_query[k * 32 + lane], q1 = kWide ? s_query[(G4 + k) * 32 + lane] : make_uint4(0, 0, 0, 0);
-          const uint32_t a0[4] = {q0.x, q1.x, q0.y, q1.y}, a1[4] = {q0.z, q1.z, q0.w, q1.w};
+          uint4 q[kH];
+#pragma unroll
+          for (int hh = 0; hh < kH; ++hh) q[hh] = s_query[(hh * G4 + k) * 32 + lane];
 #pragma unroll
           for (int pg = 0; pg < 2; ++pg) {
+            const uint32_t w0 = kw[pg][2 * (k - k0)], w1 = kw[pg][2 * (k - k0) + 1], v0 = w0 >> 8, v1 = w1 >> 8;
+            const uint32_t a0[4] = {offset_lo(w0), offset_lo(w1), offset_lo(v0), offset_lo(v1)};
+            const uint32_t a1[4] = {offset_hi(w0), offset_hi(w1), offset_hi(v0), offset_hi(v1)};
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              const uint32_t w = kw[pg][2 * (k - k0) + n], v = w >> 8;
+            for (int hh = 0; hh < kH; ++hh) {
               float acc[4];
-              mma_f16_zero(acc, a0, offset_lo(w), offset_lo(v));
-              mma_f16(acc, a1, offset_hi(w), offset_hi(v), acc);
-              const float2 sc = scale_pair(ks[pg][n], k);
+              mma_f16_zero(acc, a0, q[hh].x, q[hh].y);
+              mma_f16(acc, a1, q[hh].z, q[hh].w, acc);
 #pragma unroll
-              for (int hh = 0; hh < kH; ++hh) {
-                const float2 a = __fadd2_rn(make_float2(acc[2 * hh], acc[2 * hh + 1]),
-                                            make_float2(q_sum[hh][k], q_sum[hh][k]));
-                x[hh][pg][n] = k == 0 ? __fmul2_rn(a, sc) : __ffma2_rn(a, sc, x[hh][pg][n]);
+              for (int r = 0; r < 2; ++r) {
+                const float scale = k == k0 ? sc[pg][r].x : sc[pg][r].y;
+                const float2 a = __fadd2_rn(make_float2(acc[2 * r], acc[2 * r + 1]), q_sum[hh][k]);
+                const float2 scale2 = make_float2(scale, scale);
+                x[hh][pg][r] = k == 0 ? __fmul2_rn(a, scale2) : __ffma2_rn(a, scale2, x[hh][pg][r]);
               }
             }
           }
@@ -546,8 +584,7 @@ __global__ void __launch_bounds__(32 * kWarps, kHeads > 8 || D == 128 ? 3 : 5) s
           const bool out0 = 2 * t + 8 * n >= left[pg], out1 = 2 * t + 8 * n + 1 >= left[pg];
 #pragma unroll
           for (int hh = 0; hh < kH; ++hh) {
-            if (out0) x[hh][pg][n].x = -INFINITY;
-            if (out1) x[hh][pg][n].y = -INFINITY;
+            if (g + 8 * n >= left[pg]) x[hh][pg][n] = make_float2(-INFINITY, -INFINITY);
           }
 #pragma unroll
           for (int k = 0; k < G4 / 2; ++k) {
@@ -558,38 +595,29 @@ __global__ void __launch_bounds__(32 * kWarps, kHeads > 8 || D == 128 ? 3 : 5) s
       }
     }
 
-    // running softmax
-    float alpha[kH];
-    bool moved = false;
+    // running softmax; the maxima are looked at across the tokens only when one rises
+    bool rises = false;
+    float2 top[kH];
 #pragma unroll
     for (int hh = 0; hh < kH; ++hh) {
-      float top = fmaxf(fmaxf(fmaxf(x[hh][0][0].x, x[hh][0][0].y), fmaxf(x[hh][0][1].x, x[hh][0][1].y)),
-                        fmaxf(fmaxf(x[hh][1][0].x, x[hh][1][0].y), fmaxf(x[hh][1][1].x, x[hh][1][1].y)));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      top = fmaxf(top * head_scale[hh], m[hh]);
-      const float base = top == -INFINITY ? 0.0f : top;
-      alpha[hh] = ex2(m[hh] - base);
-      moved |= top != m[hh];
-      m[hh] = top;
-      const float2 base2 = make_float2(-base, -base), scale2 = make_float2(head_scale[hh], head_scale[hh]);
-      float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-      for (int pg = 0; pg < 2; ++pg) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float2 y = __ffma2_rn(x[hh][pg][n], scale2, base2);
-          x[hh][pg][n] = make_float2(ex2(y.x), ex2(y.y));
-          sum = __fadd2_rn(sum, x[hh][pg][n]);
-        }
-      }
-      l[hh] = fmaf(l[hh], alpha[hh], sum.x + sum.y);
+      top[hh].x = fmaxf(fmaxf(x[hh][0][0].x, x[hh][0][1].x), fmaxf(x[hh][1][0].x, x[hh][1][1].x)) * head_scale[hh].x;
+      top[hh].y = fmaxf(fmaxf(x[hh][0][0].y, x[hh][0][1].y), fmaxf(x[hh][1][0].y, x[hh][1][1].y)) * head_scale[hh].y;
+      rises |= top[hh].x > m[hh].x || top[hh].y > m[hh].y;
     }
-    if (__any_sync(0xffffffffu, moved)) {
+    if (__any_sync(0xffffffffu, rises)) {
 #pragma unroll
-      for (int hh = 0; hh < kH; ++hh) {  // columns 2 t and 2 t + 1 are the heads of lanes 8 t and 8 t + 4
-        const float2 f = make_float2(__shfl_sync(0xffffffffu, alpha[hh], 8 * t),
-                                     __shfl_sync(0xffffffffu, alpha[hh], 8 * t + 4));
+      for (int hh = 0; hh < kH; ++hh) {
+        float2 to = top[hh];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          to.x = fmaxf(to.x, __shfl_xor_sync(0xffffffffu, to.x, d));
+          to.y = fmaxf(to.y, __shfl_xor_sync(0xffffffffu, to.y, d));
+        }
+        to = make_float2(fmaxf(to.x, m[hh].x), fmaxf(to.y, m[hh].y));
+        minus_base[hh] = make_float2(to.x == -INFINITY ? 0.0f : -to.x, to.y == -INFINITY ? 0.0f : -to.y);
+        const float2 f = make_float2(ex2(m[hh].x + minus_base[hh].x), ex2(m[hh].y + minus_base[hh].y));
+        m[hh] = to;
+        l[hh] = __fmul2_rn(l[hh], f);
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
@@ -601,21 +629,36 @@ __global__ void __launch_bounds__(32 * kWarps, kHeads > 8 || D == 128 ? 3 : 5) s
         }
       }
     }
+#pragma unroll
+    for (int hh = 0; hh < kH; ++hh) {
+#pragma unroll
+      for (int pg = 0; pg < 2; ++pg) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float2 y = __ffma2_rn(x[hh][pg][n], head_scale[hh], minus_base[hh]);
+          x[hh][pg][n] = make_float2(ex2(y.x), ex2(y.y));
+          l[hh] = __fadd2_rn(l[hh], x[hh][pg][n]);
+        }
+      }
+    }
 
     // O^T += V^T P^T
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) {
-      // weights of the token pairs: rounded, and the rest; kTwice: neither -ph nor the rest where the first term is wanted
+      // Weights, rounded and the rest, turned round to head g and the token pairs (2 t, 2 t + 1), (2 t + 8, 2 t + 9);
+      // kTwice: neither -ph nor the rest where the first term is wanted.
       __half2 ph[kH][2], pl[kH][2], minus[kH][2];
 #pragma unroll
       for (int hh = 0; hh < kH; ++hh) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          ph[hh][n] = __floats2half2_rn(x[hh][pg][n].x, x[hh][pg][n].y);
-          const float2 r = __half22float2(ph[hh][n]);
-          pl[hh][n] = __floats2half2_rn(x[hh][pg][n].x - r.x, x[hh][pg][n].y - r.y);
-          minus[hh][n] = __hneg2(ph[hh][n]);
-          if (kTwice && g < 4) pl[hh][n] = minus[hh][n] = __float2half2_rn(0.0f);
+          const __half2 h = __floats2half2_rn(x[hh][pg][n].x, x[hh][pg][n].y);
+          const float2 r = __half22float2(h);
+          const uint32_t hi_bits = transposed(h2_as_u32(h));
+          const uint32_t lo_bits = transposed(h2_as_u32(__floats2half2_rn(x[hh][pg][n].x - r.x, x[hh][pg][n].y - r.y)));
+          ph[hh][n] = u32_as_h2(hi_bits);
+          pl[hh][n] = u32_as_h2(kTwice ? lo_bits & second_term : lo_bits);
+          minus[hh][n] = u32_as_h2((hi_bits ^ 0x80008000u) & second_term);
         }
       }
 #pragma unroll
