@@ -24,6 +24,10 @@
 // 64 sequences of up to 16384 tokens: 32.9 us, 3.7 TB/s; the scores take 26 of
 // them, 23 at 5.4 TB/s behind a start of 3.5.  One sequence of 131072 tokens
 // 10.8 us, two launches and their chains of dependent loads.
+#include <mutex>
+#include <set>
+#include <utility>
+
 #include "elem.cuh"
 
 namespace iris {
@@ -836,10 +840,27 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
   });
 }
 
+constexpr int kMaxShared = 227 * 1024;
+
 // Shared memory of the score kernel.
 int64_t score_bytes(int64_t q_heads, int head_dim) {
   return (q_heads * (2 * head_dim + 20) + 15) / 16 * 16 +
          kScoreWarps * kScoreStages * (head_dim == 128 ? kSlotBytes<128> : kSlotBytes<64>);
+}
+
+// All the shared memory that a CTA can have, asked for once per kernel and GPU.
+cudaError_t allow_shared_memory(const void* fn) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  const auto key = std::make_pair(fn, device);
+  if (done.count(key) != 0) return cudaSuccess;
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared);
+  if (e == cudaSuccess) done.insert(key);
+  return e;
 }
 
 template <typename E>
@@ -848,7 +869,7 @@ cudaError_t launch_score(const ScoreParams& p, int head_dim, dim3 grid, cudaStre
   const int bytes = static_cast<int>(score_bytes(p.cta_heads * p.group, head_dim));
   const auto fn = head_dim == 128 ? (wide ? score_kernel<E, 128, true> : score_kernel<E, 128, false>)
                                   : (wide ? score_kernel<E, 64, true> : score_kernel<E, 64, false>);
-  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  const cudaError_t e = allow_shared_memory(reinterpret_cast<const void*>(fn));
   if (e != cudaSuccess) return e;
   return launch_early(fn, grid, dim3(32 * kScoreWarps), static_cast<size_t>(bytes), s, p);
 }
@@ -948,7 +969,7 @@ extern "C" int iris_b200_page_select(const void* query, const void* bounds, cons
   if (dtype != IRIS_DTYPE_FP16 && dtype != IRIS_DTYPE_BF16) return IRIS_EINVAL;
   const int group = num_q_heads / num_kv_heads;
   if (page_size != kPage || (head_dim != 64 && head_dim != 128) || group > 16) return IRIS_EUNSUPPORTED;
-  if (score_bytes(num_q_heads, head_dim) > 227 * 1024) return IRIS_EUNSUPPORTED;  // 630 query heads of 128 dims
+  if (score_bytes(num_q_heads, head_dim) > kMaxShared) return IRIS_EUNSUPPORTED;  // 589 query heads of 128 dims
   if (batch == 0) return IRIS_OK;
   if (num_pages == 0) return IRIS_EINVAL;
   if (batch > 65535 || num_kv_heads > 16384 || max_pages_per_seq > (1 << 27)) return IRIS_EUNSUPPORTED;
