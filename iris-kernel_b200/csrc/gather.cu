@@ -7,9 +7,11 @@
 // row of R = Hkv D dims.  A CTA takes a tile of consecutive output rows; one
 // warp finds the first row's sequence and, a lane a row, the rows' places in
 // the cache; then all pass over the tile's 8-dim vectors: four packed bytes
-// in, one 16-byte store out, consecutive lanes on consecutive vectors.  8 x 8192
-// tokens of 8 heads of 128 dims: 58.2 us, 5.3 TB/s (82 % of a plain copy), DRAM
-// bound; 517 tokens of 8 heads of 64 dims: 2.4 us, launch and dependent loads.
+// in, one 16-byte store out (or eight and 32), consecutive lanes on consecutive
+// vectors.  8 x 8192 tokens of 8 heads of 128 dims: 53.2 us, 5.8 TB/s (90 % of a
+// plain copy), DRAM bound; 517 tokens of 8 heads of 64 dims: 2.4 us, launch and dependent loads.
+#include <type_traits>
+
 #include "elem.cuh"
 
 namespace iris {
@@ -109,11 +111,18 @@ IRIS_DEV uint4 dequant8(uint32_t w, __half scale) {
   return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
-template <typename E>
+// 32 bytes, 32-byte aligned.
+IRIS_DEV void store32(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z),
+               "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
+// kWide: 16 dims a thread and one 32-byte store, where everything is aligned to
+// that: 65536 tokens of 8 heads of 128 dims 58.2 -> 53.2 us.  (A second vector
+// of each tensor on the way takes 52.7, but 8192 tokens then 2 us more.)
+template <typename E, bool kWide>
 __global__ void __launch_bounds__(kThreads) gather_kernel(const GatherParams p) {
-  // Vectors of each tensor that a thread has on the way at a time: 1, 2, 4 and 8 of them take 58.5, 58.1, 64.1 and
-  // 75.3 us at 8 x 8192 tokens (more registers, fewer warps), 3.4, 3.3, 3.4 and 3.6 at 517.
-  constexpr int kAhead = 2;
   __shared__ int64_t s_row[kTile];
   grid_dependency_wait();
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * p.tile;
@@ -122,39 +131,35 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const GatherParams p) 
     const int seq = sequence_of(p, n0);
     if (threadIdx.x < rows) s_row[threadIdx.x] = row_of(p, n0 + threadIdx.x, seq);
   }
-  const int down = kThreads / p.vecs, along = kThreads - down * p.vecs;  // from a thread's vector to its next one
-  int r = threadIdx.x / p.vecs, v = threadIdx.x - r * p.vecs;
+  constexpr int kVecs = kWide ? 2 : 1;
+  const int units = p.vecs / kVecs;
+  const int down = kThreads / units, along = kThreads - down * units;  // from a thread's unit to its next one
+  int r = threadIdx.x / units, v = threadIdx.x - r * units;
   __syncthreads();
+  using Word = std::conditional_t<kWide, uint2, uint32_t>;
   while (r < rows) {
-    uint32_t kw[kAhead], vw[kAhead];
-    __half ks[kAhead], vs[kAhead];
-    int64_t dst[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      dst[j] = r < rows ? (n0 + r) * p.vecs + v : -1;
-      kw[j] = vw[j] = 0u;
-      ks[j] = vs[j] = __ushort_as_half(0);
-      const int64_t src = r < rows ? s_row[r] : -1;
-      if (src >= 0) {
-        const int64_t at = src * p.vecs + v;
-        kw[j] = __ldg(reinterpret_cast<const uint32_t*>(p.k_data) + at);
-        vw[j] = __ldg(reinterpret_cast<const uint32_t*>(p.v_data) + at);
-        ks[j] = __ldg(p.k_scale + (at >> 2));
-        vs[j] = __ldg(p.v_scale + (at >> 2));
-      }
-      r += down;
-      v += along;
-      if (v >= p.vecs) {
-        v -= p.vecs;
-        ++r;
-      }
+    Word kw = {}, vw = {};
+    __half ks = __ushort_as_half(0), vs = ks;
+    const int64_t src = s_row[r], dst = (n0 + r) * units + v;
+    if (src >= 0) {
+      const int64_t at = src * units + v, scale = at * kVecs >> 2;
+      kw = __ldg(reinterpret_cast<const Word*>(p.k_data) + at);
+      vw = __ldg(reinterpret_cast<const Word*>(p.v_data) + at);
+      ks = __ldg(p.k_scale + scale);
+      vs = __ldg(p.v_scale + scale);
     }
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      if (dst[j] >= 0) {
-        static_cast<uint4*>(p.key)[dst[j]] = dequant8<E>(kw[j], ks[j]);
-        static_cast<uint4*>(p.value)[dst[j]] = dequant8<E>(vw[j], vs[j]);
-      }
+    if constexpr (kWide) {
+      store32(static_cast<char*>(p.key) + 32 * dst, dequant8<E>(kw.x, ks), dequant8<E>(kw.y, ks));
+      store32(static_cast<char*>(p.value) + 32 * dst, dequant8<E>(vw.x, vs), dequant8<E>(vw.y, vs));
+    } else {
+      static_cast<uint4*>(p.key)[dst] = dequant8<E>(kw, ks);
+      static_cast<uint4*>(p.value)[dst] = dequant8<E>(vw, vs);
+    }
+    r += down;
+    v += along;
+    if (v >= units) {
+      v -= units;
+      ++r;
     }
   }
 }
@@ -215,8 +220,10 @@ extern "C" int iris_b200_int4_paged_gather(const void* k_data, const void* v_dat
   clear_stale_cuda_error();
   const unsigned blocks = static_cast<unsigned>((num_tokens + p.tile - 1) / p.tile);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == IRIS_DTYPE_FP16 ? launch_early(gather_kernel<Fp16Elem>, blocks, kThreads, 0, s, p)
-                                                 : launch_early(gather_kernel<Bf16Elem>, blocks, kThreads, 0, s, p);
+  const bool wide = aligned_to(key, 32) && aligned_to(value, 32) && aligned_to(k_data, 8) && aligned_to(v_data, 8);
+  const auto fn = dtype == IRIS_DTYPE_FP16 ? (wide ? gather_kernel<Fp16Elem, true> : gather_kernel<Fp16Elem, false>)
+                                           : (wide ? gather_kernel<Bf16Elem, true> : gather_kernel<Bf16Elem, false>);
+  const cudaError_t e = launch_early(fn, blocks, kThreads, 0, s, p);
   if (e != cudaSuccess) {
     record_cuda_error(e, "gather_kernel launch");
     return IRIS_ECUDA;

@@ -333,6 +333,47 @@ def test_gather_matches_the_cache(hkv, dim, page, lens, first, dtype):
     _same_bits(k[:int(cu[-1])], want[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("offset", [0, 8, 16])
+def test_gather_into_rows_at_any_16_bytes(offset, dtype):
+    """Outputs that start 0, 16 or 32 bytes into their memory: the narrow and the wide stores."""
+    from iris_kernel.fused_kv import fused_int4_paged_gather
+
+    rng = np.random.default_rng(7 + offset)
+    lens, hkv, dim = [45, 0, 18], 3, 96
+    bt, pages = _table(rng, lens, 16)
+    cache = R.random_cache(rng, pages + 1, hkv, dim)
+    cache = [np.ascontiguousarray(x[:pages]) for x in cache]
+    cu = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    dev = [torch.from_numpy(x).cuda() for x in (*cache, bt, cu)]
+    want = _gather_expect(cache, bt, lens, [0, 0, 0], dtype, 16)
+    n = int(cu[-1]) * hkv * dim
+    room = torch.full((2, n + 64), 5.0, dtype=dtype, device="cuda")
+    key, value = (room[i, 32 * i + offset:32 * i + offset + n].view(-1, hkv, dim) for i in range(2))
+    fused_int4_paged_gather(*dev[:4], dev[4], dev[5], key, value, num_tokens=int(cu[-1]))
+    _same_bits(key, want[0])
+    _same_bits(value, want[1])
+    for i in range(2):  # and nothing around them
+        assert bool((room[i, :32 * i + offset] == 5).all()) and bool((room[i, 32 * i + offset + n:] == 5).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gather_of_extreme_scales(dtype):
+    """Every nibble with the smallest, the largest and the non-finite scales."""
+    from iris_kernel.fused_kv import fused_int4_paged_gather
+
+    values = np.array([0.0, 2.0 ** -24, 2.0 ** -14, 3.0 / 7, 9375.0, 65504.0, np.inf, np.nan, -0.5], np.float16)
+    n = len(values)
+    data = np.broadcast_to(R.pack(np.tile(np.arange(-8, 8, dtype=np.int8), 2)), (1, n, 1, 16)).copy()
+    scale = values.reshape(1, n, 1, 1).copy()
+    dev = [torch.from_numpy(x).cuda() for x in (data, data, scale, scale, np.zeros((1, 1), np.int32),
+                                                 np.array([0, n], np.int32))]
+    with np.errstate(invalid="ignore", over="ignore"):
+        want = _gather_expect((data, data, scale, scale), np.zeros((1, 1), np.int32), [n], [0], dtype, n)
+    for got, w in zip(fused_int4_paged_gather(*dev, num_tokens=n, dtype=dtype, page_size=n), want):
+        _same_bits(got, w)
+
+
 def test_gather_errors_and_refusals():
     from iris_kernel.fused_kv import fused_int4_paged_gather
 
