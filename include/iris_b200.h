@@ -181,6 +181,10 @@ IRIS_API int iris_b200_rope_fp16_paged_append(const void* key, const void* value
 /* Most position axes of iris_b200_mrope_int4_paged_append. */
 #define IRIS_MROPE_MAX_AXES 4
 
+/* Bytes of device workspace iris_b200_mrope_int4_paged_append needs (0 for
+ * batches of up to 2048 tokens). */
+IRIS_API size_t iris_b200_mrope_append_workspace_bytes(int64_t num_tokens, int64_t num_pages, int32_t page_size);
+
 /*
  * Rotary positions with several axes + group-32 symmetric INT4 quantisation +
  * paged append (the write path of models whose tokens have a position per
@@ -205,12 +209,12 @@ IRIS_API int iris_b200_rope_fp16_paged_append(const void* key, const void* value
  * a group holding an infinity or NaN keeps that as its scale.
  * head_dim % 64 == 0 and <= 512, rotary_dim % 16 == 0.
  *
- * A token whose slot is negative is padding: nothing of it is read but its
+ * A token whose slot is negative is padding: nothing of it counts but its
  * slot, and its rows of query_out / key_out are zeros.  The batch is validated
  * in this call (slot range, every axis's position range, duplicate slots); a
  * batch that fails, or that finds such a bit pending in *error_word, writes
- * nothing at all.  Batches of more than IRIS_APPEND_INLINE_CHECK_TOKENS
- * tokens need a workspace of iris_b200_append_check_workspace_bytes.
+ * nothing at all.  Larger batches need a workspace for that, see
+ * iris_b200_mrope_append_workspace_bytes.
  */
 IRIS_API int iris_b200_mrope_int4_paged_append(
     const void* key, int64_t key_stride, const void* value, int64_t value_stride, const void* query,

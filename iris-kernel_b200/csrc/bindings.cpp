@@ -294,11 +294,9 @@ PyObject* mrope_append(PyObject* const* a) {
   require(heads <= INT32_MAX && q_heads <= INT32_MAX, PyExc_ValueError, "too many heads");
   if (tokens > 0) {
     Tensor ws;
-    size_t bytes = 0;
-    if (tokens > IRIS_APPEND_INLINE_CHECK_TOKENS) {  // smaller batches are checked without a workspace
-      bytes = iris_b200_append_check_workspace_bytes(cache.num_pages, static_cast<int32_t>(page_size));
-      ws = workspace(bytes > 0 ? bytes : 4, device);
-    }
+    const size_t bytes =
+        iris_b200_mrope_append_workspace_bytes(tokens, cache.num_pages, static_cast<int32_t>(page_size));
+    if (bytes > 0) ws = workspace(bytes, device);
     const int interleaved = PyObject_IsTrue(a[13]);
     if (interleaved < 0) throw Raised{};
     launch("iris_b200_mrope_int4_paged_append", device, [&](int32_t* word, void* stream) {

@@ -70,6 +70,7 @@ SIGNATURES = {
         ctypes.c_int,
         [_c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32,
          _c_i32, _c_f, _c_p, _c_sz, _c_p, _c_p]),
+    "iris_b200_mrope_append_workspace_bytes": (_c_sz, [_c_i64, _c_i64, _c_i32]),
     "iris_b200_mrope_int4_paged_append": (
         ctypes.c_int,
         [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i32, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_p,

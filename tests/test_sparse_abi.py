@@ -44,6 +44,16 @@ def test_append_of_no_tokens_is_done_at_once():
     assert _append(num_tokens=0, key=None, value=None, slots=None) == 0
 
 
+def test_append_workspace():
+    """None for batches that are validated without a bitmap, a bit a slot for the others."""
+    need = lib.iris_b200_mrope_append_workspace_bytes
+    for tokens in (0, 1, 128, 129, 2048):
+        assert need(tokens, 1 << 20, 16) == 0
+    for tokens in (2049, 1 << 20):
+        assert need(tokens, 1000, 16) == 1000 * 16 // 8
+    assert need(4096, 0, 16) == 0
+
+
 def _gather(**kw):
     a = dict(k_data=P, v_data=P, k_scale=P, v_scale=P, block_table=P, stride=4, cu=P, first=None, key=P, value=P,
              num_tokens=8, batch=2, hkv=8, head_dim=128, num_pages=4, page_size=16, max_pages_per_seq=4,
