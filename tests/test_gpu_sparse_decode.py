@@ -182,6 +182,21 @@ def test_long_tables_with_many_equal_scores(width):
     _check_select(width, 2, 2, 64, [16 * width - 3], 300, width=width, pages=4000)
 
 
+@pytest.mark.parametrize("pages", [200, 500, 1000, 2000, 8000, 33000])
+def test_scores_of_all_sizes_and_scores_that_differ_in_their_last_bits(pages):
+    """Each key layout: half of the scores lie within 40 units in the last
+    place, the others are spread over 2^120, and the budget ends among the
+    former."""
+    def change(query, bounds, step, bt):
+        rng = np.random.default_rng(pages)
+        bounds[:] = bounds[0]
+        near = rng.permutation(len(step))[:len(step) // 2]
+        step[:] = np.exp2(rng.uniform(-60, 60, step.shape)).astype(np.float32)
+        step[near] = (1 + rng.integers(0, 40, (len(near), step.shape[1])) * 2.0 ** -23).astype(np.float32)
+
+    _check_select(pages, 2, 2, 64, [16 * pages - 5], pages // 4 + 7 * (pages // 16), change=change)
+
+
 def test_all_scores_equal_or_zero():
     _check_select(1, 4, 2, 64, [1600], 9, spread=0)  # every bound 0
 
