@@ -29,6 +29,7 @@
 #include <utility>
 
 #include "elem.cuh"
+#include "key_range.h"
 
 namespace iris {
 namespace {
@@ -727,7 +728,7 @@ template <int kThreads, int KPT, int kCtas>
 __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) {
   using B = Board<kThreads, kCtas>;
   __shared__ uint32_t s_more[4][B::kEntries];
-  __shared__ __align__(16) uint32_t s_bins[4][256];
+  __shared__ __align__(16) uint32_t s_bins[kRangeRounds][256];
   __shared__ Bin s_found;
   constexpr int kAll = kThreads * kCtas;
   const int row = blockIdx.x / kCtas, tid = B::rank() * kThreads + threadIdx.x, lane = threadIdx.x & 31;
@@ -739,7 +740,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
     grid_dependency_wait();  // (nothing here runs ahead of the kernels before)
     return;                  // (nor does any CTA of the row go on)
   }
-  for (int i = threadIdx.x; i < 256; i += kThreads) reinterpret_cast<uint4*>(s_bins)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < kRangeRounds * 64; i += kThreads) reinterpret_cast<uint4*>(s_bins)[i] = make_uint4(0, 0, 0, 0);
   grid_dependency_wait();  // the scores are there
   const auto key_at = [&](int i) { return select_key(p, r, i, i < r.n ? __ldcg(r.keys + i) : 0u); };
   constexpr int kRegs = KPT > 0 ? KPT : 1;
@@ -780,17 +781,16 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
   B::put(s_more[0], lowest);
   B::put(s_more[1], highest);
   B::meet();
-  uint32_t low = B::lowest(s_more[0]), high = B::highest(s_more[1]);
-  // The scored keys that are wanted lie in [low, high], and the last of them is to be found: 256 bins over the range,
-  // counted from the top, until one bin's keys are all wanted, or all the same.  (At most four rounds: 32 bits.)
+  KeyRange range = {B::lowest(s_more[0]), B::highest(s_more[1])};
+  // The scored keys that are wanted lie in the range, and the last of them is to be found: 256 bins over the range,
+  // counted from the top, until one bin's keys are all wanted, or all the same.
   int need = r.keep - p.sink - p.recent;  // (n > keep: the two ends do not meet)
-  uint32_t thr = high;                    // keys above it are taken, and the first `need` equal ones
-  for (int round = 0; need > 0; ++round) {
-    const uint32_t range = high - low;
-    const int shift = max(24 - __clz(range), 0);
+  uint32_t thr = range.high;              // keys above it are taken, and the first `need` equal ones
+  for (int round = 0; need > 0 && round < kRangeRounds; ++round) {
+    const int shift = max(24 - __clz(range.high - range.low), 0);
     uint32_t* bins = s_bins[round];
     const auto count = [&](uint32_t x) {
-      if (x - low <= range) atomicAdd(bins + ((high - x) >> shift), 1u);
+      if (range.holds(x)) atomicAdd(bins + range.bin(x, shift), 1u);
     };
     if constexpr (KPT > 0) {
       each([&](int, uint32_t x) { count(x); });
@@ -806,13 +806,12 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectParams p) 
       bin = s_found;  // (next written behind another meeting)
     }
     need -= bin.before;
-    high -= static_cast<uint32_t>(bin.index) << shift;
-    low = max(low, high - ((1u << shift) - 1u));
+    range.narrow(static_cast<uint32_t>(bin.index), shift);
     if (bin.count == need) {  // exactly the wanted ones
-      thr = low - 1u;
+      thr = range.low - 1u;
       need = 0;
     } else if (shift == 0) {
-      thr = low;
+      thr = range.low;
       break;
     }
   }

@@ -197,6 +197,31 @@ def test_scores_of_all_sizes_and_scores_that_differ_in_their_last_bits(pages):
     _check_select(pages, 2, 2, 64, [16 * pages - 5], pages // 4 + 7 * (pages // 16), change=change)
 
 
+@pytest.mark.parametrize("pages", [200, 500, 1000, 2000, 8000, 20000, 33000])
+@pytest.mark.parametrize("top", ["ordinary", "infinite"])
+def test_scores_that_overflow(pages, top):
+    """Each key layout: most scores are minus infinity (a finite step times a
+    negative sum), some lie just above it, a few are ordinary or plus infinity;
+    the budget ends among each of them, and where one kind ends."""
+    n, few = pages, 3 + pages // 100
+    near = pages // 10
+
+    def change(query, bounds, step, bt):
+        rng = np.random.default_rng(pages)
+        query[:] = query.abs().clamp(min=0.5)
+        kind = rng.permutation(n)
+        low, high = bt[0, kind[few + near:]], bt[0, kind[:few]]
+        bounds[:] = -100  # of a positive query: a negative sum
+        step[:] = (4e32 * (1 - rng.random(step.shape) / 64)).astype(np.float32)  # sums below 8.2e5: finite
+        step[low] = 3e38
+        bounds[high] = 100
+        step[high] = np.inf if top == "infinite" else 0.25
+
+    for keep in (2 + few // 2, 2 + few, 2 + few + near // 2, few + near, 2 + few + near, few + near + (n - few - near) // 2,
+                 n - 1):
+        _check_select(pages, 2, 2, 64, [16 * n - 5], keep, change=change)
+
+
 def test_all_scores_equal_or_zero():
     _check_select(1, 4, 2, 64, [1600], 9, spread=0)  # every bound 0
 
