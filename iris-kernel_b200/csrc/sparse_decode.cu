@@ -150,6 +150,11 @@ constexpr int kLutOffset = 0x48;  // (a ^ c) & b
 IRIS_DEV uint32_t offset_lo(uint32_t w) { return lop3<kLutOffset>(w, 0x000f000fu, 0x00080008u); }
 IRIS_DEV uint32_t offset_hi(uint32_t w) { return lop3<kLutOffset>(w, 0x00f000f0u, 0x00800080u); }
 
+// NaN in place of an infinite scale: the key is NaN (its nibbles are zeros), but
+// the offset's share of a sum may leave a rounding that is not zero, and an
+// infinite logit, if negative, would pass for a weight of zero.
+IRIS_DEV __half2 finite_or_nan(__half2 s) { return __hfma2(s, __half2half2(__ushort_as_half(0)), s); }
+
 // Steps of a row.
 IRIS_DEV int steps_of(const SparseParams& p, int row) {
   return (min(max(__ldg(p.counts + row), 0), p.keep) + 1) >> 1;
@@ -542,7 +547,7 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
         for (int pg = 0; pg < 2; ++pg) {
           load_matrices(kw[pg], st_addr + pg * C::kStage + (mat ^ (16 * k0)));
 #pragma unroll
-          for (int r = 0; r < 2; ++r) sc[pg][r] = __half22float2(u32_as_h2(ks[pg][r][k0 / 2]));
+          for (int r = 0; r < 2; ++r) sc[pg][r] = __half22float2(finite_or_nan(u32_as_h2(ks[pg][r][k0 / 2])));
         }
 #pragma unroll
         for (int k = k0; k < k0 + 2; ++k) {

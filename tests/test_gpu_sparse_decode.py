@@ -486,3 +486,25 @@ def test_attention_errors_and_refusals():
     _attend(good)
     none = _attend([good[0][:0], *good[1:5], good[5][:0], good[6][:0], good[7][:0], good[8][:0]])
     assert none[0].shape == (0, 4, 64) and none[1].shape == (0, 4)
+
+
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_key_group_that_is_not_finite_always_shows(dim, bad):
+    """Its nibbles are zeros, as the append leaves them: the key is NaN, and so
+    is every output of its head, whatever the query; other heads do not change."""
+    lens = [200 + i for i in range(24)]
+    c = _case(24, 8, 2, dim, lens, 14)
+    rng = np.random.default_rng(24)
+    total = [-(-n // 16) for n in lens]
+    for b in range(24):
+        c["lists"][b] = -1
+        c["lists"][b, :, :total[b]] = np.arange(total[b])
+        c["counts"][b] = total[b]
+        page, tok, k = c["bt"][b, rng.integers(0, total[b] - 1)], rng.integers(0, 16), rng.integers(0, dim // 32)
+        c["cache"][2][page, tok, 1, k] = bad
+        c["cache"][0][page, tok, 1, 16 * k:16 * k + 16] = 0
+    args = [c["query"].cuda(), *_dev(*c["cache"], c["bt"], c["lens"], c["lists"], c["counts"])]
+    out, lse = _attend(args)
+    assert torch.isnan(out[:, 4:]).all() and torch.isnan(lse[:, 4:]).all()
+    assert torch.isfinite(out[:, :4]).all() and torch.isfinite(lse[:, :4]).all()
