@@ -21,8 +21,10 @@
 //                  enters as the subnormal fp16 (n + 8) 2^-24, one logic
 //                  operation for two; -8 sum(q) 2^-24 is added to the
 //                  group's sum.  Each query head is scaled by a power of two to a
-//                  largest value in [1, 2) and put back in the logits' scale:
-//                  exact but for elements 2^-14 below its largest.
+//                  largest value in [2^15, 2^16) and put back in the logits' scale:
+//                  odd dims enter times 1/16, so an element keeps all its bits
+//                  down to 2^-25 of the head's largest, and a step of 2^-35
+//                  of it below that.
 //   O^T = V^T P^T  rows = dims, columns = query heads; V as exact integers; a
 //                  weight p is two fp16 terms, p * scale again two: the rounded
 //                  product and, by fused multiply-adds, what it left off (22
@@ -398,12 +400,12 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-      const float down = __uint_as_float((254u - e) << 23);  // 2^-(e - 127)
+      const uint32_t e = min(max(__float_as_uint(top) >> 23, 15u), 254u);
+      const float down = __uint_as_float((269u - e) << 23);  // 2^(15 - (e - 127))
       const auto of_columns = [&](float x) {  // head g's -> heads 2 t and 2 t + 1's
         return make_float2(__shfl_sync(0xffffffffu, x, 8 * t), __shfl_sync(0xffffffffu, x, 8 * t + 4));
       };
-      head_scale[half] = of_columns((p.scale_log2 * 16777216.0f) * __uint_as_float(e << 23));
+      head_scale[half] = of_columns((p.scale_log2 * 512.0f) * __uint_as_float(e << 23));  // 2^24 / 2^15
 #pragma unroll
       for (int k = 0; k < G4; ++k) {
         const uint32_t v[4] = {w[k].x, w[k].y, w[k].z, w[k].w};  // dims (0,1) (2,3) (4,5) (6,7)

@@ -508,3 +508,39 @@ def test_a_key_group_that_is_not_finite_always_shows(dim, bad):
     out, lse = _attend(args)
     assert torch.isnan(out[:, 4:]).all() and torch.isnan(lse[:, 4:]).all()
     assert torch.isfinite(out[:, :4]).all() and torch.isfinite(lse[:, :4]).all()
+
+
+def _close(c, scale=None):
+    """The attention against 64 bits, every output on its own: half a unit in
+    the last place (FP16: or 2^-25) and 2^-14 of the sum of the magnitudes that
+    are added up for it (the errors of p and the normaliser, as above)."""
+    args = [c["query"].cuda(), *_dev(*c["cache"], c["bt"], c["lens"], c["lists"], c["counts"])]
+    out, lse = _attend(args, softmax_scale=scale)
+    rest = (c["bt"], c["lens"], c["lists"], c["counts"], scale)
+    kd, vd, ks, vs = c["cache"]
+    want, want_lse = R.attend_ref(R.f32(c["query"]), kd, vd, ks, vs, *rest)
+    magnitude, _ = R.attend_ref(R.f32(c["query"]), kd, R.pack(np.abs(R.unpack(vd))), ks, vs, *rest)
+    half = c["query"].dtype == torch.float16
+    rounding = np.maximum(2.0 ** -11 * np.abs(want), 2.0 ** -25) if half else 2.0 ** -8 * np.abs(want)
+    got, got_lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= rounding + 2.0 ** -14 * magnitude).all()
+    assert (np.abs(got_lse - want_lse) <= 2.0 ** -14).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_small_elements_of_a_query_with_a_large_one(dim, dtype):
+    """The largest element meets zero keys; the logits are the odd dims', 2^-14
+    (BF16: 2^-18) of it, in the other groups."""
+    c = _case(22, 4, 2, dim, [700], 20, dtype)
+    small = 2.0 ** (-4 if dtype == torch.float16 else -8)
+    rng = np.random.default_rng(22)
+    query = np.zeros((1, 4, dim), np.float32)
+    query[..., 33::2] = small * rng.uniform(1, 2, query[..., 33::2].shape) * rng.choice([-1, 1], query[..., 33::2].shape)
+    query[..., 0] = 1024
+    c["query"] = R.to_type(query, dtype)
+    keys = R.unpack(c["cache"][0])
+    keys[..., :32] = 0
+    c["cache"][0] = R.pack(keys)
+    _close(c, 1.5 / (small * 3 * 0.28 * 1.5 * (dim // 2 - 16) ** 0.5))
