@@ -582,6 +582,17 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) scale_words(st + pg * C::kStage + 2 * C::kData + C::kScale, vs[pg]);
 
+    // The logits, rounded to fp32 before a maximum is taken from them: a fused multiply-add would leave the largest
+    // token that maximum's own rounding, which passes an exponential's range for logits from 2^30 on.
+#pragma unroll
+    for (int hh = 0; hh < kH; ++hh) {
+#pragma unroll
+      for (int pg = 0; pg < 2; ++pg) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) x[hh][pg][n] = __fmul2_rn(x[hh][pg][n], head_scale[hh]);
+      }
+    }
+
     // tokens past the sequence's end count for nothing, whatever their bytes hold
     if (min(left[0], left[1]) < kPage) {
 #pragma unroll
@@ -607,8 +618,8 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
     float2 top[kH];
 #pragma unroll
     for (int hh = 0; hh < kH; ++hh) {
-      top[hh].x = fmaxf(fmaxf(x[hh][0][0].x, x[hh][0][1].x), fmaxf(x[hh][1][0].x, x[hh][1][1].x)) * head_scale[hh].x;
-      top[hh].y = fmaxf(fmaxf(x[hh][0][0].y, x[hh][0][1].y), fmaxf(x[hh][1][0].y, x[hh][1][1].y)) * head_scale[hh].y;
+      top[hh].x = fmaxf(fmaxf(x[hh][0][0].x, x[hh][0][1].x), fmaxf(x[hh][1][0].x, x[hh][1][1].x));
+      top[hh].y = fmaxf(fmaxf(x[hh][0][0].y, x[hh][0][1].y), fmaxf(x[hh][1][0].y, x[hh][1][1].y));
       rises |= top[hh].x > m[hh].x || top[hh].y > m[hh].y;
     }
     if (__any_sync(0xffffffffu, rises)) {
@@ -642,7 +653,7 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
       for (int pg = 0; pg < 2; ++pg) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          const float2 y = __ffma2_rn(x[hh][pg][n], head_scale[hh], minus_base[hh]);
+          const float2 y = __fadd2_rn(x[hh][pg][n], minus_base[hh]);
           x[hh][pg][n] = make_float2(ex2(y.x), ex2(y.y));
           l[hh] = __fadd2_rn(l[hh], x[hh][pg][n]);
         }

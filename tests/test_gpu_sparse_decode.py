@@ -544,3 +544,18 @@ def test_small_elements_of_a_query_with_a_large_one(dim, dtype):
     keys[..., :32] = 0
     c["cache"][0] = R.pack(keys)
     _close(c, 1.5 / (small * 3 * 0.28 * 1.5 * (dim // 2 - 16) ** 0.5))
+
+
+@pytest.mark.parametrize("exponent", [-130, -120, 100, 108, 116])
+def test_queries_near_the_ends_of_bf16(exponent):
+    """Logits too small to tell the tokens apart give their mean; logits far
+    beyond an exponential's range give the one largest's value."""
+    c = _case(23, 6, 2, 128, [300, 40], 19, torch.bfloat16)
+    c["query"] = (c["query"].double() * 2.0 ** exponent).to(torch.bfloat16)
+    args = [c["query"].cuda(), *_dev(*c["cache"], c["bt"], c["lens"], c["lists"], c["counts"])]
+    out, lse = _attend(args)
+    want, want_lse = R.attend_ref(c["query"].double().numpy(), *c["cache"], np.maximum(c["bt"], 0), c["lens"],
+                                  c["lists"], c["counts"])
+    got = out.double().cpu().numpy()
+    assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -14 * 7 * float(c["cache"][3].max())).all()
+    assert (np.abs(lse.double().cpu().numpy() - want_lse) <= 2.0 ** -14 + 2.0 ** -18 * np.abs(want_lse)).all()
