@@ -28,7 +28,14 @@
 //   O^T = V^T P^T  rows = dims, columns = query heads; V as exact integers; a
 //                  weight p is two fp16 terms, p * scale again two: the rounded
 //                  product and, by fused multiply-adds, what it left off (22
-//                  bits, no step finer than 2^-24; scales are at least 2^-14).
+//                  bits).  FP16 ends at 2^-24, and so would a small weight of
+//                  a small scale: weights are taken up to 2^14, which leaves
+//                  a term a step of 2^-38 of the largest weight, 2^-24 of it
+//                  times the smallest scale.  A row in which a scale of 2 or more
+//                  is seen takes them up to 2^7, and each group's scales times a
+//                  power of two of its own that brings the group's largest one
+//                  so far to [2^7, 2^8), 2^7 at most; its sums are divided by
+//                  it when the row is done.
 //                  S^T's accumulators become the fragment of P^T by a transposing
 //                  move of 8 x 8 matrices, which costs less than S = Q K^T, whose
 //                  accumulators are that fragment, and whose products are twice
@@ -156,6 +163,18 @@ IRIS_DEV uint32_t offset_hi(uint32_t w) { return lop3<kLutOffset>(w, 0x00f000f0u
 // the offset's share of a sum may leave a rounding that is not zero, and an
 // infinite logit, if negative, would pass for a weight of zero.
 IRIS_DEV __half2 finite_or_nan(__half2 s) { return __hfma2(s, __half2half2(__ushort_as_half(0)), s); }
+
+// The largest logit of a row, rounded up, has weight 2^14; with scaled values 2^7.
+constexpr float kWeightExponent = 14.0f, kScaledExponent = 7.0f;
+// The largest value scales a pair of groups has been made ready for, their bits
+// below the exponent set.  Below 2 there is nothing to do; beyond, the factors
+// for exponent fields e are 2^(22 - e), 2^7 to 2^-8.
+constexpr uint32_t kPlainCap = 0x3fff3fffu;
+IRIS_DEV __half2 factors_of(uint32_t cap) { return u32_as_h2(0x94009400u - (cap & 0x7c007c00u)); }
+// 127 + the exponent of one's factor
+IRIS_DEV uint32_t factor_of(uint32_t cap, int half, bool scaled) {
+  return scaled ? 149u - ((cap >> (10 + 16 * half)) & 31u) : 127u;
+}
 
 // Steps of a row.
 IRIS_DEV int steps_of(const SparseParams& p, int row) {
@@ -369,6 +388,8 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
   constexpr int kTiles = D / 16;  // of 16 dims; a lane has two dims of each for heads 2 t, 2 t + 1 (+ 8)
   float o[kH][kTiles][4];
   float2 m[kH], minus_base[kH], l[kH], q_sum[kH][G4], head_scale[kH];  // (l: of this lane's tokens)
+  uint32_t v_cap[G4 / 2];  // of two groups each
+  bool scaled = false;     // (the same in every lane)
   int cur = -1, cur_start = first.start;
 
   // Query fragments.  Of this lane's eight dims of a group, the first product
@@ -376,6 +397,9 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
   // (bits 4-7, 16 times as large) times 1/16.
   const auto start_row = [&](int row) {
     __syncwarp();  // the last row's fragments have been read
+#pragma unroll
+    for (int k = 0; k < G4 / 2; ++k) v_cap[k] = kPlainCap;
+    scaled = false;
 #pragma unroll
     for (int half = 0; half < kH; ++half) {
       m[half] = make_float2(-INFINITY, -INFINITY);
@@ -445,7 +469,7 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
         l[hh].x += __shfl_xor_sync(0xffffffffu, l[hh].x, d);
         l[hh].y += __shfl_xor_sync(0xffffffffu, l[hh].y, d);
       }
-      const float lv[2] = {l[hh].x, l[hh].y}, mv[2] = {m[hh].x, m[hh].y};
+      const float lv[2] = {l[hh].x, l[hh].y}, minus[2] = {minus_base[hh].x, minus_base[hh].y};
       float inv[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -453,9 +477,10 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
         inv[e] = lv[e] == 0.0f ? 0.0f : __fdiv_rn(1.0f, lv[e]);
         if (g == 0 && hq < p.group) {
           if (!whole)
-            *reinterpret_cast<float2*>(p.part_ml + (part * p.group + hq) * 2) = make_float2(mv[e], lv[e]);
+            *reinterpret_cast<float2*>(p.part_ml + (part * p.group + hq) * 2) =
+                make_float2(lv[e] == 0.0f ? -INFINITY : -minus[e], lv[e]);
           else if (p.lse != nullptr)
-            p.lse[static_cast<int64_t>(cur) * p.group + hq] = lv[e] == 0.0f ? -INFINITY : mv[e] + log2f(lv[e]);
+            p.lse[static_cast<int64_t>(cur) * p.group + hq] = lv[e] == 0.0f ? -INFINITY : log2f(lv[e]) - minus[e];
         }
       }
       if constexpr (kTwice) {  // the two terms' sums
@@ -472,7 +497,9 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
         if (head < p.group) {
 #pragma unroll
           for (int k = 0; k < G4; ++k) {  // this lane's four dims of the group are adjacent
-            const float4 v = make_float4(o[hh][2 * k][e], o[hh][2 * k][2 + e], o[hh][2 * k + 1][e], o[hh][2 * k + 1][2 + e]);
+            const float down = __uint_as_float((254u - factor_of(v_cap[k >> 1], k & 1, scaled)) << 23);  // 1 / the group's factor
+            const float4 v = make_float4(o[hh][2 * k][e] * down, o[hh][2 * k][2 + e] * down, o[hh][2 * k + 1][e] * down,
+                                         o[hh][2 * k + 1][2 + e] * down);
             const int d = 32 * k + 4 * g;
             if (whole)
               *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.output) +
@@ -581,6 +608,13 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
     uint32_t vs[2][2][G4];
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) scale_words(st + pg * C::kStage + 2 * C::kData + C::kScale, vs[pg]);
+    // and, to see the largest of them, a lane two groups of one token of a page (of each, or of its half of the lanes)
+    constexpr int kLook = D == 128 ? 2 : 1;
+    uint32_t look[kLook];
+#pragma unroll
+    for (int i = 0; i < kLook; ++i)
+      look[i] = *reinterpret_cast<const uint32_t*>(st + (D == 128 ? i : lane >> 4) * C::kStage + 2 * C::kData + C::kScale +
+                                                   4 * (D == 128 ? lane : lane & 15));
 
     // The logits, rounded to fp32 before a maximum is taken from them: a fused multiply-add would leave the largest
     // token that maximum's own rounding, which passes an exponential's range for logits from 2^30 on.
@@ -595,6 +629,10 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
 
     // tokens past the sequence's end count for nothing, whatever their bytes hold
     if (min(left[0], left[1]) < kPage) {
+#pragma unroll
+      for (int i = 0; i < kLook; ++i) {
+        if ((D == 128 ? lane >> 1 : lane & 15) >= (D == 128 ? left[i] : lane < 16 ? left[0] : left[1])) look[i] = 0u;
+      }
 #pragma unroll
       for (int pg = 0; pg < 2; ++pg) {
 #pragma unroll
@@ -613,8 +651,12 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
       }
     }
 
-    // running softmax; the maxima are looked at across the tokens only when one rises
-    bool rises = false;
+    // running softmax; the maxima (and those of the value scales) are looked at across the tokens only when one rises
+    __half2 seen = __habs2(u32_as_h2(look[0]));
+    if constexpr (D == 128) seen = __hmax2(seen, __habs2(u32_as_h2(look[kLook - 1])));
+    const uint32_t my_cap = D == 128 && (lane & 1) ? v_cap[G4 / 2 - 1] : v_cap[0];
+    const bool grows = !__hble2(seen, u32_as_h2(my_cap));
+    bool rises = grows;
     float2 top[kH];
 #pragma unroll
     for (int hh = 0; hh < kH; ++hh) {
@@ -623,6 +665,36 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
       rises |= top[hh].x > m[hh].x || top[hh].y > m[hh].y;
     }
     if (__any_sync(0xffffffffu, rises)) {
+      if (__any_sync(0xffffffffu, grows)) {
+        uint32_t cap = h2_as_u32(seen);
+        // (a group with a scale that is not finite gives NaN, whatever its factor)
+        if ((cap & 0x7c00u) == 0x7c00u) cap &= 0xffff0000u;
+        if ((cap & 0x7c000000u) == 0x7c000000u) cap &= 0x0000ffffu;
+        cap = __vmaxu2(cap, my_cap);
+#pragma unroll
+        for (int d = D == 128 ? 2 : 1; d < 32; d <<= 1) cap = __vmaxu2(cap, __shfl_xor_sync(0xffffffffu, cap, d));
+        cap |= 0x03ff03ffu;
+        uint32_t next[G4 / 2];
+        bool now = false;
+#pragma unroll
+        for (int i = 0; i < G4 / 2; ++i) {
+          next[i] = __shfl_sync(0xffffffffu, cap, i);
+          now |= next[i] != kPlainCap;
+        }
+#pragma unroll
+        for (int k = 0; k < G4; ++k) {  // the groups' sums, by their new factors over their present ones
+          const float smaller = __uint_as_float(
+              (127u + factor_of(next[k >> 1], k & 1, now) - factor_of(v_cap[k >> 1], k & 1, scaled)) << 23);
+#pragma unroll
+          for (int hh = 0; hh < kH; ++hh) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[hh][2 * k + (e >> 2)][e & 3] *= smaller;
+          }
+          if (k & 1) v_cap[k >> 1] = next[k >> 1];
+        }
+        scaled = now;
+      }
+      const float exponent = scaled ? kScaledExponent : kWeightExponent;
 #pragma unroll
       for (int hh = 0; hh < kH; ++hh) {
         float2 to = top[hh];
@@ -631,10 +703,14 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
           to.x = fmaxf(to.x, __shfl_xor_sync(0xffffffffu, to.x, d));
           to.y = fmaxf(to.y, __shfl_xor_sync(0xffffffffu, to.y, d));
         }
-        to = make_float2(fmaxf(to.x, m[hh].x), fmaxf(to.y, m[hh].y));
-        minus_base[hh] = make_float2(to.x == -INFINITY ? 0.0f : -to.x, to.y == -INFINITY ? 0.0f : -to.y);
-        const float2 f = make_float2(ex2(m[hh].x + minus_base[hh].x), ex2(m[hh].y + minus_base[hh].y));
+        // rounded up to a whole number, so that the exponents' base is exact (or, from 2^24 on, no further down than m)
+        to = make_float2(fmaxf(ceilf(to.x), m[hh].x), fmaxf(ceilf(to.y), m[hh].y));
+        const float2 base = make_float2(to.x == -INFINITY ? 0.0f : __fadd_rd(exponent, -to.x),
+                                        to.y == -INFINITY ? 0.0f : __fadd_rd(exponent, -to.y));
+        const float2 f = make_float2(m[hh].x == -INFINITY ? 0.0f : ex2(base.x - minus_base[hh].x),
+                                     m[hh].y == -INFINITY ? 0.0f : ex2(base.y - minus_base[hh].y));
         m[hh] = to;
+        minus_base[hh] = base;
         l[hh] = __fmul2_rn(l[hh], f);
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
@@ -656,6 +732,18 @@ __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) :
           const float2 y = __fadd2_rn(x[hh][pg][n], minus_base[hh]);
           x[hh][pg][n] = make_float2(ex2(y.x), ex2(y.y));
           l[hh] = __fadd2_rn(l[hh], x[hh][pg][n]);
+        }
+      }
+    }
+
+    if (scaled) {
+#pragma unroll
+      for (int pg = 0; pg < 2; ++pg) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+          for (int k = 0; k < G4; ++k)
+            vs[pg][n][k] = h2_as_u32(__hmul2(u32_as_h2(vs[pg][n][k]), factors_of(v_cap[k % (G4 / 2)])));
         }
       }
     }

@@ -559,3 +559,36 @@ def test_queries_near_the_ends_of_bf16(exponent):
     got = out.double().cpu().numpy()
     assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -14 * 7 * float(c["cache"][3].max())).all()
     assert (np.abs(lse.double().cpu().numpy() - want_lse) <= 2.0 ** -14 + 2.0 ** -18 * np.abs(want_lse)).all()
+
+
+SIZES = {
+    "one small group": lambda t, k, n: 5e-4 if k == 1 else 0.28,
+    "all small": lambda t, k, n: 5e-4,
+    "the smallest": lambda t, k, n: 2.0 ** -14,
+    "smallest beside largest": lambda t, k, n: 9000.0 if k == 0 else 2.0 ** -14,
+    "rising": lambda t, k, n: 2.0 ** (-14 + 24 * t / n),
+    "falling": lambda t, k, n: 2.0 ** (10 - 24 * t / n),
+    "small first token": lambda t, k, n: np.where(t == 0, 2.0 ** -12, 2.0 ** -2),
+}
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hq,hkv,dim", [(2, 2, 64), (4, 1, 128), (8, 1, 128), (16, 1, 64), (12, 1, 128)])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_small_values_are_as_exact_as_large_ones(sizes, hq, hkv, dim, dtype):
+    """One token holds a quarter of the weight or more, 2047 others about 2^-11 of
+    its weight each; the values' group scales are small in all groups, in some,
+    or change along the sequence."""
+    n = 2048
+    c = _case(21, hq, hkv, dim, [n], n // 16, dtype)
+    query = R.f32(c["query"]).reshape(1, hkv, hq // hkv, dim)
+    query[:] = query[:, :, :1] * (1 + np.arange(hq // hkv)[:, None] / 64)  # one direction a KV head
+    c["query"] = R.to_type(query.reshape(1, hq, dim), dtype)
+    kd, _, ks, vs = c["cache"]
+    at = c["bt"][0, 0]
+    kd[at, 0] = R.pack((3 * np.sign(query[0, :, 0])).astype(np.int8))
+    ks[at, 0] = 0.28 * (1.0 if dim == 128 else 2.0 ** 0.5)
+    for page, col in zip(c["bt"][0], range(n // 16)):
+        for k in range(dim // 32):
+            vs[page, :, :, k] = np.broadcast_to(SIZES[sizes](16 * col + np.arange(16), k, n), 16).astype(np.float16)[:, None]
+    _close(c)
