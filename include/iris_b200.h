@@ -202,7 +202,9 @@ IRIS_API size_t iris_b200_mrope_append_workspace_bytes(int64_t num_tokens, int64
  *              has its count)
  *   cos_cache, sin_cache [max_position, rotary_dim / 2] of `dtype`
  *   query_out  [num_tokens, num_q_heads, head_dim], key_out [num_tokens,
- *              num_kv_heads, head_dim] or NULL: contiguous, of `dtype`
+ *              num_kv_heads, head_dim] or NULL: contiguous, of `dtype`, in
+ *              memory of their own: apart from each other, from every input
+ *              and from the cache
  * Dims i and i + rotary_dim / 2 turn together, dims from rotary_dim on pass
  * through.  Rotation in fp32, not rounded before the quantisation; scale =
  * fp16(min(max(amax / 7, 2^-14), 65504)), q = clamp(rint(y / scale), -7, 7);

@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <initializer_list>
 #include <string>
 
 #include "iris_b200.h"
@@ -195,16 +196,25 @@ Rows token_rows(const char* name, const Tensor& t, at::IntArrayRef shape, at::Sc
   return {ptr(t), shape[0] > 1 ? t.stride(0) : 0};
 }
 
-// A kernel that reads vectors of `in` after it has written others of `out`
-// cannot have both in one place.
-void check_apart(const char* name, const Tensor& out, const char* of, const Tensor& in) {
-  if (out.numel() == 0 || in.numel() == 0) return;
-  int64_t last = 0;
-  for (int64_t d = 0; d < in.dim(); ++d) last += (in.size(d) - 1) * in.stride(d);
+// A given output, contiguous, must not share memory with what the kernel reads
+// after it has begun to write, or with what else it writes.
+struct Named {
+  const char* name;
+  const Tensor* tensor;  // NULL: not given
+};
+void check_apart(const char* name, const Tensor& out, std::initializer_list<Named> others) {
+  if (out.numel() == 0) return;
   const char* a = static_cast<const char*>(out.const_data_ptr());
-  const char* b = static_cast<const char*>(in.const_data_ptr());
-  if (a < b + (last + 1) * in.element_size() && b < a + out.numel() * out.element_size())
-    refuse(PyExc_ValueError, std::string(name) + " must not overlap " + of);
+  const char* end = a + out.numel() * out.element_size();
+  for (const Named& other : others) {
+    if (other.tensor == nullptr || other.tensor->numel() == 0) continue;
+    const Tensor& in = *other.tensor;
+    int64_t last = 0;
+    for (int64_t d = 0; d < in.dim(); ++d) last += (in.size(d) - 1) * in.stride(d);
+    const char* b = static_cast<const char*>(in.const_data_ptr());
+    if (a < b + (last + 1) * in.element_size() && b < end)
+      refuse(PyExc_ValueError, std::string(name) + " must not overlap " + other.name);
+  }
 }
 
 // (key, value, positions, slot_mapping, cos, sin, k_data, v_data, k_scale, v_scale, query, sections, rotary_dim,
@@ -277,9 +287,10 @@ PyObject* mrope_append(PyObject* const* a) {
       rotated = empty(shape, type, device);
     } else {
       check("query_out", *query_out, shape, type, device);
-      check_apart("query_out", *query_out, "query", *query);
-      check_apart("query_out", *query_out, "key", key);
-      check_apart("query_out", *query_out, "value", value);
+      check_apart("query_out", *query_out,
+                  {{"query", query}, {"key", &key}, {"value", &value}, {"positions", &positions},
+                   {"slot_mapping", &slots}, {"cos_cache", &cos}, {"sin_cache", &sin}, {"k_data", &kd}, {"v_data", &vd},
+                   {"k_scale", &ks}, {"v_scale", &vs}});
       rotated = *query_out;
     }
   } else {
@@ -287,9 +298,10 @@ PyObject* mrope_append(PyObject* const* a) {
   }
   if (key_out != nullptr) {
     check("key_out", *key_out, key.sizes(), type, device);
-    check_apart("key_out", *key_out, "key", key);
-    check_apart("key_out", *key_out, "value", value);
-    if (query != nullptr) check_apart("key_out", *key_out, "query", *query);
+    check_apart("key_out", *key_out,
+                {{"query_out", query_out}, {"query", query}, {"key", &key}, {"value", &value}, {"positions", &positions},
+                 {"slot_mapping", &slots}, {"cos_cache", &cos}, {"sin_cache", &sin}, {"k_data", &kd}, {"v_data", &vd},
+                 {"k_scale", &ks}, {"v_scale", &vs}});
   }
   require(heads <= INT32_MAX && q_heads <= INT32_MAX, PyExc_ValueError, "too many heads");
   if (tokens > 0) {
@@ -378,12 +390,16 @@ PyObject* gather(PyObject* const* a) {
     k = empty(shape, type, device);
   } else {
     check("key", *key, shape, type, device);
+    check_apart("key", *key, {{"value", value}, {"k_data", &kd}, {"v_data", &vd}, {"k_scale", &ks}, {"v_scale", &vs},
+                              {"block_table", &bt}, {"cu_seqlens", &cu}, {"first_token", first}});
     k = *key;
   }
   if (value == nullptr) {
     v = empty(shape, type, device);
   } else {
     check("value", *value, shape, type, device);
+    check_apart("value", *value, {{"k_data", &kd}, {"v_data", &vd}, {"k_scale", &ks}, {"v_scale", &vs},
+                                  {"block_table", &bt}, {"cu_seqlens", &cu}, {"first_token", first}});
     v = *value;
   }
   if (tokens > 0) {
@@ -481,12 +497,16 @@ PyObject* page_select(PyObject* const* a) {
     l = empty(shape, at::kInt, device);
   } else {
     check("page_list", *list, shape, at::kInt, device);
+    check_apart("page_list", *list, {{"page_count", count}, {"query", &query}, {"bounds", &bounds}, {"bounds_step", &step},
+                                     {"block_table", &bt}, {"seq_lens", &lens}});
     l = *list;
   }
   if (count == nullptr) {
     n = empty({batch, heads}, at::kInt, device);
   } else {
     check("page_count", *count, {batch, heads}, at::kInt, device);
+    check_apart("page_count", *count, {{"query", &query}, {"bounds", &bounds}, {"bounds_step", &step},
+                                       {"block_table", &bt}, {"seq_lens", &lens}});
     n = *count;
   }
   if (batch > 0) {
@@ -537,6 +557,11 @@ PyObject* sparse_decode(PyObject* const* a) {
     o = empty(query.sizes(), query.scalar_type(), device);
   } else {
     check("output", *output, query.sizes(), query.scalar_type(), device);
+    // (in the query's own place it is: a row is read before it is written)
+    const bool in_place = output->const_data_ptr() == query.const_data_ptr();
+    check_apart("output", *output, {{"query", in_place ? nullptr : &query}, {"k_data", &kd}, {"v_data", &vd},
+                                    {"k_scale", &ks}, {"v_scale", &vs}, {"block_table", &bt}, {"seq_lens", &lens},
+                                    {"page_list", &list}, {"page_count", &count}});
     o = *output;
   }
   const int with_lse = PyObject_IsTrue(a[13]);

@@ -342,9 +342,9 @@ def fused_mrope_int4_paged_append(
     ``key_out [T, Hkv, D]`` receives the rotated keys, as a prefill's own
     attention needs them.  ``key``, ``value`` and ``query`` may be slices of a
     fused projection: tokens apart, heads and dims contiguous; the outputs must
-    not overlap them.  Tokens with
-    ``slot_mapping < 0`` are padding: not stored, their rotated rows zero.  A
-    batch with a bad slot or position writes nothing."""
+    overlap neither them, nor another input or the cache, nor each other.
+    Tokens with ``slot_mapping < 0`` are padding: not stored, their rotated rows
+    zero.  A batch with a bad slot or position writes nothing."""
     rotated = _ops.mrope_append(key, value, positions, slot_mapping, cos_cache, sin_cache, k_data, v_data, k_scale,
                                 v_scale, query, sections, rotary_dim, interleaved, group_size, page_size, query_out,
                                 key_out)

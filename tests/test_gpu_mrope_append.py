@@ -279,6 +279,47 @@ def test_refusals():
         _run(c, query=False, query_out=torch.empty_like(c["query"]))
 
 
+@pytest.mark.parametrize("what", ["the same", "half over", "key", "k_data", "v_scale", "cos"])
+def test_outputs_that_overlap_are_refused(what):
+    """Rotated keys in the rotated queries' place, or in memory that the call
+    reads or stores to: nothing is written."""
+    from iris_kernel.fused_kv import fused_mrope_int4_paged_append
+
+    c = _case(34, hq=2, hkv=2)
+    n = c["query"].numel()
+
+    def call(query_out, key_out):
+        fused_mrope_int4_paged_append(c["key"], c["value"], c["positions"], c["slots"], c["cos"], c["sin"], *c["cache"],
+                                      c["query"], sections=c["sections"], rotary_dim=c["rotary"], page_size=c["page"],
+                                      query_out=query_out, key_out=key_out)
+        torch.cuda.synchronize()
+
+    room = torch.full((2 * n,), 3.0, dtype=torch.float16, device="cuda")
+    query_out = room[:n].view(c["query"].shape)
+    places = {"the same": query_out, "half over": room[n // 2:n // 2 + n].view(c["query"].shape), "key": c["key"]}
+    if what in places:
+        key_out = places[what]
+    else:  # the output in the other tensor's memory
+        big = torch.zeros(40960, dtype=torch.float16, device="cuda")
+        key_out = big[:n].view(c["query"].shape)
+        if what == "cos":
+            c["cos"] = big[:c["cos"].numel()].view(c["cos"].shape).copy_(c["cos"])
+        else:
+            i = ["k_data", "v_data", "k_scale", "v_scale"].index(what)
+            x = c["cache"][i]
+            c["cache"][i] = big.view(x.dtype)[:x.numel()].view(x.shape).copy_(x)
+    before = [x.clone() for x in c["cache"]]
+    for outputs in ((query_out, key_out), (key_out, query_out)):
+        with pytest.raises(ValueError, match="overlap"):
+            call(*outputs)
+    torch.cuda.synchronize()
+    assert bool((room == 3).all())
+    for x, y in zip(before, c["cache"]):
+        assert torch.equal(x, y)
+    call(query_out, room[n:].view(c["query"].shape))  # one right after the other
+    assert not bool((room == 3).any())
+
+
 # ------------------------------------------------------------------ read back
 def _table(rng, lens, page, width=None):
     counts = [-(-n // page) for n in lens]
@@ -431,3 +472,24 @@ def test_offsets_past_32_bits():
     k, v = fused_int4_paged_gather(*big, bt, torch.tensor([0, 32], dtype=torch.int32, device="cuda"), num_tokens=32)
     ref = np.concatenate([R.dequant(want[0][8], want[2][8]), R.dequant(want[0][0], want[2][0])])
     _same_bits(k, R.to_type(ref, torch.float16))
+
+
+def test_gather_outputs_that_overlap_are_refused():
+    from iris_kernel.fused_kv import fused_int4_paged_gather
+
+    rng = np.random.default_rng(8)
+    cache = [torch.from_numpy(x).cuda() for x in R.random_cache(rng, 4, 2, 64)]
+    bt, cu = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([[0, 3]], [0, 20]))
+    room = torch.zeros(3 * 20 * 128, dtype=torch.float16, device="cuda")
+    at = [room[i * 1280:i * 1280 + 2560].view(20, 2, 64) for i in range(3)]
+    for key, value in ((at[0], at[0]), (at[0], at[1]), (at[1], at[0])):
+        with pytest.raises(ValueError, match="overlap"):
+            fused_int4_paged_gather(*cache, bt, cu, key, value, num_tokens=20)
+    inside = cache[0].view(-1).view(torch.float16)[:1280].view(10, 2, 64)  # the cache's own bytes
+    with pytest.raises(ValueError, match="overlap"):
+        fused_int4_paged_gather(*cache, bt, cu, inside, num_tokens=10)
+    with pytest.raises(ValueError, match="overlap"):
+        fused_int4_paged_gather(*cache, bt, cu, None, inside, num_tokens=10)
+    key, value = fused_int4_paged_gather(*cache, bt, cu, at[0], at[2], num_tokens=20)
+    for got, want in zip((key, value), fused_int4_paged_gather(*cache, bt, cu, num_tokens=20)):
+        assert torch.equal(got, want)

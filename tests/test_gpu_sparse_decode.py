@@ -592,3 +592,28 @@ def test_small_values_are_as_exact_as_large_ones(sizes, hq, hkv, dim, dtype):
         for k in range(dim // 32):
             vs[page, :, :, k] = np.broadcast_to(SIZES[sizes](16 * col + np.arange(16), k, n), 16).astype(np.float16)[:, None]
     _close(c)
+
+
+def test_outputs_that_overlap_are_refused():
+    """An output over part of the query or in the cache's memory, a list in the
+    counts' place; the output in the query's own place is the output."""
+    from iris_kernel.sparse_attention import fused_page_select
+
+    c = _case(25, 8, 2, 128, [100, 333], 9)
+    args, out, lse = _check_attend(c)
+    room = torch.zeros(3 * out.numel(), dtype=out.dtype, device="cuda")
+    args[0] = room[:out.numel()].view(out.shape).copy_(args[0])
+    for at in (out.numel() // 2, 8):
+        with pytest.raises(ValueError, match="overlap"):
+            _attend(args, output=room[at:at + out.numel()].view(out.shape))
+    with pytest.raises(ValueError, match="overlap"):
+        _attend(args, output=args[3].view(-1)[:out.numel()].view(out.shape))
+    own, lse2 = _attend(args, output=args[0])
+    assert own is args[0] and torch.equal(own, out) and torch.equal(lse, lse2)
+
+    ints = torch.zeros(64, dtype=I32, device="cuda")
+    index = _dev(np.zeros((c["bt"].max() + 1, 2, 2, 128), np.int8), np.ones((c["bt"].max() + 1, 2), np.float32))
+    for lists, counts in ((ints[:16], ints[:4]), (ints[:16], ints[12:16])):
+        with pytest.raises(ValueError, match="overlap"):
+            fused_page_select(out, *index, args[5], args[6], lists.view(2, 2, 4), counts.view(2, 2), max_pages=4)
+    fused_page_select(out, *index, args[5], args[6], ints[:16].view(2, 2, 4), ints[16:20].view(2, 2), max_pages=4)
