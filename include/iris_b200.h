@@ -235,9 +235,10 @@ IRIS_API int iris_b200_mrope_int4_paged_append(
  * The cache read back: sequence b's tokens from first_token[b] (NULL: 0) on,
  * cu_seqlens[b + 1] - cu_seqlens[b] of them, dequantised (nibble * scale, one
  * rounding to `dtype`) into rows cu_seqlens[b] .. of key / value [num_tokens,
- * num_kv_heads, head_dim].  cu_seqlens [batch + 1] int32 rises from 0; rows
- * from cu_seqlens[batch] on are zeros.  A token without a page (table too
- * narrow, bad page id) gives zeros and its bit.  Any page_size; head_dim a
+ * num_kv_heads, head_dim].  cu_seqlens [batch + 1] int32 rises from 0 (its bit
+ * if it does not); rows from cu_seqlens[batch] on are zeros, rows from
+ * num_tokens on are not there.  A token without a page (table too narrow, bad
+ * page id) gives zeros and its bit.  Any page_size; head_dim a
  * multiple of 32 up to 512; key / value 16-byte aligned.  No counterpart in
  * the reference.
  */

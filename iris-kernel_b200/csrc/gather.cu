@@ -68,7 +68,7 @@ IRIS_DEV int64_t row_of(const GatherParams& p, int64_t n, int seq) {
     end = __ldg(p.cu_seqlens + ++seq + 1);
   }
   const int64_t from = p.first_token != nullptr ? __ldg(p.first_token + seq) : 0;
-  if (n < start || n >= end || end > total || from < 0) {  // offsets that do not rise from 0
+  if (start < 0 || n < start || n >= end || end > total || from < 0) {
     set_error(p.err, IRIS_ERR_SEQ_LEN);
     return -1;
   }
@@ -130,6 +130,11 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const GatherParams p) 
   if (threadIdx.x < 32) {
     const int seq = sequence_of(p, n0);
     if (threadIdx.x < rows) s_row[threadIdx.x] = row_of(p, n0 + threadIdx.x, seq);
+  } else if (blockIdx.x == 0) {  // the other warps of one CTA meanwhile: the offsets rise from 0
+    for (int i = static_cast<int>(threadIdx.x) - 32; i < p.batch; i += kThreads - 32) {
+      const int from = __ldg(p.cu_seqlens + i), to = __ldg(p.cu_seqlens + i + 1);
+      if (to < from || (i == 0 && from != 0)) set_error(p.err, IRIS_ERR_SEQ_LEN);
+    }
   }
   constexpr int kVecs = kWide ? 2 : 1;
   const int units = p.vecs / kVecs;

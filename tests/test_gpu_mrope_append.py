@@ -493,3 +493,17 @@ def test_gather_outputs_that_overlap_are_refused():
     key, value = fused_int4_paged_gather(*cache, bt, cu, at[0], at[2], num_tokens=20)
     for got, want in zip((key, value), fused_int4_paged_gather(*cache, bt, cu, num_tokens=20)):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("cu", [[-5, 10], [-5, 0, 10], [-8, -5, 10], [1, 1, 10], [0, 8, 3, 10], [0, 3, -2, 10],
+                                [0] * 400 + [9, 8, 10]])
+def test_gather_offsets_that_do_not_rise_from_0(cu):
+    from iris_kernel.fused_kv import fused_int4_paged_gather
+
+    rng = np.random.default_rng(9)
+    cache = [torch.from_numpy(x).cuda() for x in R.random_cache(rng, 4, 2, 64)]
+    bt = torch.tensor([[0, 3]], dtype=torch.int32, device="cuda").expand(len(cu) - 1, 2)
+    with pytest.raises(ValueError):
+        fused_int4_paged_gather(*cache, bt, torch.tensor(cu, dtype=torch.int32, device="cuda"), num_tokens=10)
+    cu = [0] + sorted(abs(x) for x in cu[1:])
+    fused_int4_paged_gather(*cache, bt, torch.tensor(cu, dtype=torch.int32, device="cuda"), num_tokens=10)
