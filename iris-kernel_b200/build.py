@@ -7,10 +7,12 @@ Plain nvcc: the library exposes only the C ABI declared in
 ``include/iris_b200.h``.  The bindings are one C++ file over that ABI and
 torch's headers, which calls what ctypes would, without a Python layer's time.  IEEE
 division / square root stay on (no ``--use_fast_math``): the write path must
-be bit-exact.
+be bit-exact.  The library knows nothing of torch; the bindings are built anew
+where torch or Python is another one than they were built for.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -35,6 +37,13 @@ NVCC_FLAGS = [
 ]
 
 
+def _stamp():
+    spec = importlib.util.spec_from_file_location("iris_ops_stamp", os.path.join(HERE, "iris_kernel", "_stamp.py"))
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
 def _nvcc() -> str:
     for cand in (os.environ.get("NVCC"), shutil.which("nvcc"), "/usr/local/cuda/bin/nvcc"):
         if cand and os.path.exists(cand):
@@ -43,11 +52,16 @@ def _nvcc() -> str:
 
 
 def _stale() -> bool:
-    if not os.path.exists(OUT) or not os.path.exists(BINDINGS):
+    if not os.path.exists(OUT) or _bindings_stale():
         return True
     t = min(os.path.getmtime(OUT), os.path.getmtime(BINDINGS))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(INCLUDE, "iris_b200.h"), __file__]
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _bindings_stale() -> bool:
+    stamp = _stamp()
+    return not os.path.exists(BINDINGS) or stamp.built() != stamp.present()
 
 
 def _run(cmd: list, verbose: bool) -> None:
@@ -81,7 +95,12 @@ def build(force: bool = False, verbose: bool = False) -> str:
     _run(cmd, verbose)
     os.replace(OUT + ".tmp", OUT)
     _run(_bindings_command(), verbose)
+    stamp = _stamp()
+    if os.path.exists(stamp.PATH):
+        os.remove(stamp.PATH)
     os.replace(BINDINGS + ".tmp", BINDINGS)
+    with open(stamp.PATH, "w") as f:
+        f.write(stamp.present() + "\n")
     return OUT
 
 

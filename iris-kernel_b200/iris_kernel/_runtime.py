@@ -25,7 +25,7 @@ import threading
 
 import torch
 
-from . import _lib, _ops
+from . import _lib
 
 _MODES = ("sync", "deferred")
 _state = threading.local()
@@ -125,7 +125,25 @@ def _prepare(index: int) -> int:
     return error_word(device).data_ptr()
 
 
-_ops.set_up(_prepare)
+_ops_module = None
+
+
+def ops():
+    """The bindings, loaded at the first call that needs them: unlike the library
+    they depend on the torch and the Python that they were built for."""
+    global _ops_module
+    if _ops_module is None:
+        from . import _stamp
+
+        built, present = _stamp.built(), _stamp.present()
+        if built is not None and built != present:
+            raise ImportError(f"iris_kernel: the bindings _ops.so were built for {built}, this is {present}; build them "
+                              "with `python iris-kernel_b200/build.py`")
+        from . import _ops
+
+        _ops.set_up(_prepare)
+        _ops_module = _ops
+    return _ops_module
 
 
 def finish(t: torch.Tensor) -> None:

@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib, _ops, _runtime
+from . import _lib, _runtime
 
 
 def _check_append_args(key, value, positions, slot_mapping, cos_cache, sin_cache, k_data, v_data, k_scale, v_scale,
@@ -345,9 +345,9 @@ def fused_mrope_int4_paged_append(
     overlap neither them, nor another input or the cache, nor each other.
     Tokens with ``slot_mapping < 0`` are padding: not stored, their rotated rows
     zero.  A batch with a bad slot or position writes nothing."""
-    rotated = _ops.mrope_append(key, value, positions, slot_mapping, cos_cache, sin_cache, k_data, v_data, k_scale,
-                                v_scale, query, sections, rotary_dim, interleaved, group_size, page_size, query_out,
-                                key_out)
+    rotated = _runtime.ops().mrope_append(key, value, positions, slot_mapping, cos_cache, sin_cache, k_data, v_data,
+                                          k_scale, v_scale, query, sections, rotary_dim, interleaved, group_size,
+                                          page_size, query_out, key_out)
     _runtime.finish(key)
     return rotated
 
@@ -377,7 +377,7 @@ def fused_int4_paged_gather(
     of rows, ``cu_seqlens[-1]``; rows past that are zeros.  For another chunk
     of prefill over a cached context, or to move a cache to another format."""
     bf16 = True if dtype is torch.bfloat16 else False if dtype is torch.float16 else None
-    out = _ops.gather(k_data, v_data, k_scale, v_scale, block_table, cu_seqlens, key, value, num_tokens, first_token,
-                      bf16, page_size, group_size)
+    out = _runtime.ops().gather(k_data, v_data, k_scale, v_scale, block_table, cu_seqlens, key, value, num_tokens,
+                                first_token, bf16, page_size, group_size)
     _runtime.finish(k_data)
     return out

@@ -20,7 +20,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _ops, _runtime
+from . import _runtime
 
 
 def fused_int4_page_bounds(
@@ -44,8 +44,8 @@ def fused_int4_page_bounds(
     every page.  ``values [pages, Hkv, 2, D]`` fp16, if given, receives what
     the codes of those pages stand for (rounded to FP16), for a score of the
     caller's own."""
-    _ops.page_bounds(k_data, k_scale, block_table, seq_lens, bounds, bounds_step, first_token, values, page_size,
-                     group_size)
+    _runtime.ops().page_bounds(k_data, k_scale, block_table, seq_lens, bounds, bounds_step, first_token, values,
+                               page_size, group_size)
     _runtime.finish(k_data)
 
 
@@ -74,8 +74,8 @@ def fused_page_select(
     count among the ``max_pages``; ties go to the lowest page.  The last page's
     bounds need not be up to date while ``recent_pages >= 1``.  An empty
     sequence keeps no page."""
-    out = _ops.page_select(query, bounds, bounds_step, block_table, seq_lens, page_list, page_count, max_pages,
-                           sink_pages, recent_pages, page_size)
+    out = _runtime.ops().page_select(query, bounds, bounds_step, block_table, seq_lens, page_list, page_count,
+                                     max_pages, sink_pages, recent_pages, page_size)
     _runtime.finish(query)
     return out
 
@@ -108,7 +108,7 @@ def fused_int4_sparse_paged_decode_attention(
     ``return_lse``: fp32 ``[B, Hq]``, log2-sum-exp2 of the scaled logits (-inf
     without a token), to merge with attention over other tokens.
     ``softmax_scale`` None (or 0.0) means ``D ** -0.5``."""
-    out = _ops.sparse_decode(query, k_data, v_data, k_scale, v_scale, block_table, seq_lens, page_list, page_count,
-                             output, page_size, group_size, softmax_scale, return_lse)
+    out = _runtime.ops().sparse_decode(query, k_data, v_data, k_scale, v_scale, block_table, seq_lens, page_list,
+                                       page_count, output, page_size, group_size, softmax_scale, return_lse)
     _runtime.finish(query)
     return out
