@@ -51,10 +51,12 @@ extern "C" {
 #define IRIS_ERR_POS_NEGATIVE 0x2      /* position < 0                       (IndexError) */
 #define IRIS_ERR_POS_RANGE 0x4         /* position >= max_position           (IndexError) */
 #define IRIS_ERR_DUP_SLOT 0x8          /* two tokens target one slot         (ValueError) */
-#define IRIS_ERR_SEQ_LEN 0x10          /* seq_len <= 0                       (ValueError) */
+#define IRIS_ERR_SEQ_LEN 0x10          /* seq_len <= 0, where it must be > 0 (ValueError) */
 #define IRIS_ERR_BLOCK_TABLE 0x20      /* block_table row shorter than needed (ValueError) */
 #define IRIS_ERR_PAGE_ID 0x40          /* page id outside [0, num_pages)     (IndexError) */
 #define IRIS_ERR_PIPELINE_TIMEOUT 0x80 /* a bounded wait gave up             (RuntimeError) */
+#define IRIS_ERR_SEQ_NEGATIVE 0x100    /* seq_len < 0, where it may be 0     (ValueError) */
+#define IRIS_ERR_OFFSETS 0x200         /* offsets or first token of a gather (ValueError) */
 
 /* ---- 16-bit element types of the entry points that take either ---------- */
 #define IRIS_DTYPE_FP16 0

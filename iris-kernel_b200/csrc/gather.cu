@@ -69,7 +69,7 @@ IRIS_DEV int64_t row_of(const GatherParams& p, int64_t n, int seq) {
   }
   const int64_t from = p.first_token != nullptr ? __ldg(p.first_token + seq) : 0;
   if (start < 0 || n < start || n >= end || end > total || from < 0) {
-    set_error(p.err, IRIS_ERR_SEQ_LEN);
+    set_error(p.err, IRIS_ERR_OFFSETS);
     return -1;
   }
   const int64_t at = from + n - start, col = at / p.page_size;
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const GatherParams p) 
   } else if (blockIdx.x == 0) {  // the other warps of one CTA meanwhile: the offsets rise from 0
     for (int i = static_cast<int>(threadIdx.x) - 32; i < p.batch; i += kThreads - 32) {
       const int from = __ldg(p.cu_seqlens + i), to = __ldg(p.cu_seqlens + i + 1);
-      if (to < from || (i == 0 && from != 0)) set_error(p.err, IRIS_ERR_SEQ_LEN);
+      if (to < from || (i == 0 && from != 0)) set_error(p.err, IRIS_ERR_OFFSETS);
     }
   }
   constexpr int kVecs = kWide ? 2 : 1;

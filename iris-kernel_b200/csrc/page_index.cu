@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(256, 2) bounds_kernel(const BoundsParams p) {
   const int len = __ldg(p.seq_lens + b);
   const int from = p.first_token != nullptr ? max(0, __ldg(p.first_token + b)) / kPage : 0;
   if (len <= 0) {
-    if (len < 0 && blockIdx.x == 0 && threadIdx.x == 0) set_error(p.err, IRIS_ERR_SEQ_LEN);
+    if (len < 0 && blockIdx.x == 0 && threadIdx.x == 0) set_error(p.err, IRIS_ERR_SEQ_NEGATIVE);
     return;
   }
   int last = (len - 1) / kPage;
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps, 3) score_kernel(const ScoreP
   };
   load_queries(warp);
   const bool first = blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0;
-  if (len < 0 && first) set_error(p.err, IRIS_ERR_SEQ_LEN);
+  if (len < 0 && first) set_error(p.err, IRIS_ERR_SEQ_NEGATIVE);
   const int64_t all = len > 0 ? (static_cast<int64_t>(len) + kPage - 1) / kPage : 0;
   if (all > p.max_pages && first) set_error(p.err, IRIS_ERR_BLOCK_TABLE);
   const int n = static_cast<int>(all < p.max_pages ? all : p.max_pages);

@@ -830,7 +830,7 @@ __global__ void __launch_bounds__(128) sparse_join_kernel(SparseParams p) {
     start = __reduce_add_sync(0xffffffffu, before);
     length = run_length(p, __reduce_add_sync(0xffffffffu, all), p.warps);
   }
-  if (head == 0 && lane == 0 && __ldg(p.seq_lens + row / p.kv_heads) < 0) set_error(p.err, IRIS_ERR_SEQ_LEN);
+  if (head == 0 && lane == 0 && __ldg(p.seq_lens + row / p.kv_heads) < 0) set_error(p.err, IRIS_ERR_SEQ_NEGATIVE);
   grid_dependency_wait();
   if (head >= p.group) return;
   const int64_t out = static_cast<int64_t>(row) * p.group + head;

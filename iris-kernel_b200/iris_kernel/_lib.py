@@ -23,6 +23,8 @@ ERR_SEQ_LEN = 0x10
 ERR_BLOCK_TABLE = 0x20
 ERR_PAGE_ID = 0x40
 ERR_PIPELINE_TIMEOUT = 0x80
+ERR_SEQ_NEGATIVE = 0x100
+ERR_OFFSETS = 0x200
 
 DECODE_OUT_FP16 = 0
 DECODE_OUT_LSE = 1

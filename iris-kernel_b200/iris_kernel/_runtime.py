@@ -74,6 +74,8 @@ _APPEND_ERRORS = (
 )
 _DECODE_ERRORS = (
     (_lib.ERR_SEQ_LEN, ValueError, "all sequence lengths must be positive"),
+    (_lib.ERR_SEQ_NEGATIVE, ValueError, "sequence lengths must not be negative"),
+    (_lib.ERR_OFFSETS, ValueError, "cu_seqlens must rise from 0 and first_token must not be negative"),
     (_lib.ERR_BLOCK_TABLE, ValueError, "block_table does not contain enough pages"),
     (_lib.ERR_PAGE_ID, IndexError, "block_table contains an invalid physical page id"),
 )

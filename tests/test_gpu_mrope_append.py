@@ -507,3 +507,15 @@ def test_gather_offsets_that_do_not_rise_from_0(cu):
         fused_int4_paged_gather(*cache, bt, torch.tensor(cu, dtype=torch.int32, device="cuda"), num_tokens=10)
     cu = [0] + sorted(abs(x) for x in cu[1:])
     fused_int4_paged_gather(*cache, bt, torch.tensor(cu, dtype=torch.int32, device="cuda"), num_tokens=10)
+
+
+def test_gather_names_its_own_arguments():
+    from iris_kernel.fused_kv import fused_int4_paged_gather
+
+    rng = np.random.default_rng(10)
+    cache = [torch.from_numpy(x).cuda() for x in R.random_cache(rng, 4, 2, 64)]
+    bt, cu, first = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([[0, 3]], [0, 10], [-1]))
+    with pytest.raises(ValueError, match="first_token"):
+        fused_int4_paged_gather(*cache, bt, cu, num_tokens=10, first_token=first)
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        fused_int4_paged_gather(*cache, bt, cu + 2, num_tokens=12)

@@ -617,3 +617,20 @@ def test_outputs_that_overlap_are_refused():
         with pytest.raises(ValueError, match="overlap"):
             fused_page_select(out, *index, args[5], args[6], lists.view(2, 2, 4), counts.view(2, 2), max_pages=4)
     fused_page_select(out, *index, args[5], args[6], ints[:16].view(2, 2, 4), ints[16:20].view(2, 2), max_pages=4)
+
+
+def test_a_negative_length_says_so():
+    """These operators take a length of 0: the message is not the dense decode's."""
+    from iris_kernel.sparse_attention import fused_page_select
+
+    c = _case(26, 4, 2, 64, [100], 5)
+    args = [c["query"].cuda(), *_dev(*c["cache"], c["bt"], c["lens"], c["lists"], c["counts"])]
+    pages = args[1].shape[0]
+    index = _dev(np.zeros((pages, 2, 2, 64), np.int8), np.zeros((pages, 2), np.float32))
+    lens = torch.tensor([-1], dtype=I32, device="cuda")
+    with pytest.raises(ValueError, match="negative"):
+        _bounds(args[1], args[3], args[5], lens, *index)
+    with pytest.raises(ValueError, match="negative"):
+        fused_page_select(args[0], *index, args[5], lens, max_pages=4)
+    with pytest.raises(ValueError, match="negative"):
+        _attend([*args[:6], lens, *args[7:]])
