@@ -201,7 +201,7 @@ IRIS_API size_t iris_b200_mrope_append_workspace_bytes(int64_t num_tokens, int64
  *   sections   host array of num_axes counts that add up to rotary_dim / 2:
  *              the frequencies each axis turns, in runs, or dealt out in turn
  *              with `interleaved` (axis 0, 1, .., passing over an axis that
- *              has its count)
+ *              has its count); no other order can be given
  *   cos_cache, sin_cache [max_position, rotary_dim / 2] of `dtype`
  *   query_out  [num_tokens, num_q_heads, head_dim], key_out [num_tokens,
  *              num_kv_heads, head_dim] or NULL: contiguous, of `dtype`, in
@@ -439,8 +439,12 @@ IRIS_API size_t iris_b200_sparse_decode_workspace_bytes(int32_t batch, int32_t n
  * reference.
  *   query, output [batch, num_q_heads, head_dim] of `dtype`; out_lse [batch,
  *   num_q_heads] fp32 or NULL: log2-sum-exp2 of the scaled logits, as in
- *   IRIS_DECODE_OUT_LSE.  Limits as iris_b200_int4_paged_decode; seq_lens may
- *   be 0; batch * num_kv_heads * max_pages below 2^31.  query, k_data, v_data
+ *   IRIS_DECODE_OUT_LSE.  output may be the query itself.  softmax_scale > 0.
+ *   Logits are fp32: one that overflows to +inf makes its head's outputs NaN.  A
+ *   listed token's key scale that is not finite makes all outputs of its heads
+ *   NaN, a value scale those of its 32 dims.  Limits as
+ *   iris_b200_int4_paged_decode; seq_lens may be 0; batch * num_kv_heads *
+ *   max_pages below 2^31.  query, k_data, v_data
  *   and workspace 16-byte aligned, the scales and output 8-byte.  The
  *   workspace's contents do not matter and belong to one call at a time.
  */

@@ -19,11 +19,16 @@
 // lowest page; written in rising order.
 //
 // Measured (B200, 8 KV heads of 128 dims).  Bounds of 16 sequences of up to
-// 8191 tokens: 36.3 us, 3.1 TB/s, the integer and minimum pipe at two thirds;
-// of one new page in each of 64 sequences 3.1 us.  Scores and selection over
+// 8191 tokens: 36.5 us, 3.1 TB/s, the integer and minimum pipe at two thirds:
+// 7.7 instructions a key and dim, of which the product, the minimum and the
+// maximum are 2 and the unpacking 2; the others are the codes' quotients, the
+// finiteness of the scales and the next page's words moved to their place.
+// Of one new page in each of 64 sequences 3.1 us.  Scores and selection over
 // 64 sequences of up to 16384 tokens: 32.9 us, 3.7 TB/s; the scores take 26 of
 // them, 23 at 5.4 TB/s behind a start of 3.5.  One sequence of 131072 tokens
-// 10.8 us, two launches and their chains of dependent loads.
+// 11.1 us, two launches and their chains of dependent loads; of 524288 tokens
+// 20.9, and of one page more 132: past 32768 pages a row is one CTA's, which reads
+// its keys again in every round.
 #include <mutex>
 #include <set>
 #include <utility>

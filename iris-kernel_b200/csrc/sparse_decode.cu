@@ -53,12 +53,13 @@
 // kernel joins them in the order of the list.
 //
 // Measured (B200): 64 sequences x 128 pages of 8192 tokens, 32 + 8 heads of 128
-// dims: 56.2 us, 2.7 TB/s of the bytes it needs (DRAM moves 1.5 times those:
-// other heads' scales share a sector).  Bound by instructions, about 400 a page
-// and warp at half an instruction a cycle, three CTAs of 158 registers an SM.
-// 96 x 45 pages, 16 heads of 64 dims: 51.4 us; DRAM moves 200 MB, 2.5 times what
-// is needed.  One sequence, 128 pages: 11.6 us, a chain of launches and
-// dependent loads.
+// dims: 57.4 us, 2.6 TB/s of the bytes it needs.  DRAM moves 226 MB, 1.5 times
+// those (other heads' scales share a sector), which would take 35; the rest is
+// 364 instructions a page and warp at half an instruction a cycle, with three
+// CTAs of 164 registers an SM.  64 and 128 query heads: 61.4 and 78.2 us.  96 x 45
+// pages, 16 heads of 64 dims: 51.8 us; DRAM moves 200 MB, 2.5 times what is
+// needed, which would take 31, and a page has 283 instructions.  One sequence,
+// 128 pages: 11.5 us, a chain of launches and dependent loads.
 #include <map>
 #include <mutex>
 #include <type_traits>
@@ -281,10 +282,10 @@ struct SlotInfo {
 
 // kHeads: 4, 8 or 16, what the group fits in.  With up to four query heads
 // the columns 4 to 7 are theirs again, and the second terms of the scaled
-// weights take the place of a second product (64 x 128 pages: 62.3 -> 59.0 us).
-// CTAs an SM, by registers: 16 heads of 128 dims 2 (82.7 us; 3 spill: 107), of
-// 64 dims 3 (54.7; 2 or 4: 56.1); fewer heads of 128 dims 3 (4 spill), of 64
-// dims 5 (96 x 45 pages 51.4; 4: 52.1, 6: 53.9).
+// weights take the place of a second product (64 x 128 pages: 3 us less).
+// CTAs an SM, by registers: 16 heads of 128 dims 2 (78.2 us; 3 spill: 24 more), of
+// 64 dims 3 (53.0; 2 or 4: 1.4 more); fewer heads of 128 dims 3 (4 spill), of 64
+// dims 5 (96 x 45 pages 51.8; 4: 0.7 more, 6: 2.5 more).
 template <typename E, int D, int kHeads>
 __global__ void __launch_bounds__(32 * kWarps, D == 128 ? (kHeads > 8 ? 2 : 3) : (kHeads > 8 ? 3 : 5)) sparse_decode_kernel(SparseParams p) {
   using C = SparseCfg<D>;

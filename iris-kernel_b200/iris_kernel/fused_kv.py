@@ -332,7 +332,7 @@ def fused_mrope_int4_paged_append(
     many of the ``rotary_dim // 2`` frequencies each axis turns: the first
     ``sections[0]`` frequencies by axis 0, and so on, or with ``interleaved``
     dealt out in turn (axis 0, 1, .., 0, 1, .., an axis that has its count
-    being passed over).  ``cos_cache / sin_cache [max_position, rotary_dim //
+    being passed over); other orders cannot be given.  ``cos_cache / sin_cache [max_position, rotary_dim //
     2]`` have the keys' type.  Dims ``i`` and ``i + rotary_dim // 2`` turn
     together; dims from ``rotary_dim`` on pass through.  Unlike
     :func:`fused_rope_int4_paged_append`, which rounds to FP16 after every
@@ -374,7 +374,7 @@ def fused_int4_paged_gather(
     Sequence ``b`` fills rows ``cu_seqlens[b] .. cu_seqlens[b + 1]`` (int32
     ``[B + 1]``, rising from 0) with its tokens from ``first_token[b]`` on
     (int32 ``[B]``; None: from its first).  ``num_tokens`` is the host's count
-    of rows, ``cu_seqlens[-1]``; rows past that are zeros.  For another chunk
+    of rows, ``cu_seqlens[-1]``; if it is more, rows past that are zeros.  For another chunk
     of prefill over a cached context, or to move a cache to another format."""
     bf16 = True if dtype is torch.bfloat16 else False if dtype is torch.float16 else None
     out = _runtime.ops().gather(k_data, v_data, k_scale, v_scale, block_table, cu_seqlens, key, value, num_tokens,

@@ -107,7 +107,8 @@ def fused_int4_sparse_paged_decode_attention(
     Returns the output in the query's type, or ``(output, lse)`` with
     ``return_lse``: fp32 ``[B, Hq]``, log2-sum-exp2 of the scaled logits (-inf
     without a token), to merge with attention over other tokens.
-    ``softmax_scale`` None (or 0.0) means ``D ** -0.5``."""
+    ``softmax_scale`` None (or 0.0) means ``D ** -0.5``; a negative one is
+    refused with a RuntimeError.  ``output`` may be the query itself."""
     out = _runtime.ops().sparse_decode(query, k_data, v_data, k_scale, v_scale, block_table, seq_lens, page_list,
                                        page_count, output, page_size, group_size, softmax_scale, return_lse)
     _runtime.finish(query)
