@@ -634,3 +634,29 @@ def test_a_negative_length_says_so():
         fused_page_select(args[0], *index, args[5], lens, max_pages=4)
     with pytest.raises(ValueError, match="negative"):
         _attend([*args[:6], lens, *args[7:]])
+
+
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+@pytest.mark.parametrize("hq,dim", [(2, 64), (8, 128), (16, 128), (32, 64)])
+def test_a_value_group_that_is_not_finite_shows_in_its_dims(hq, dim, bad):
+    """NaN in the 32 dims of that head's outputs, and nowhere else; the other
+    dims, of ordinary scales and of scales of 2 and more, are what they are
+    without it."""
+    for large in (1.0, 40.0):
+        c = _case(27, hq, 2, dim, [300, 90], 19)
+        c["cache"][3] = (c["cache"][3].astype(np.float32) * large).astype(np.float16)
+        for b in range(2):
+            total = -(-int(c["lens"][b]) // 16)
+            c["lists"][b] = -1
+            c["lists"][b, :, :total] = np.arange(total)
+            c["counts"][b] = total
+        args, out, lse = _check_attend(c)
+        page, k = c["bt"][0, 4], dim // 32 - 1
+        vd, vs = args[2].clone(), args[4].clone()
+        vd[page, 9, 1, 16 * k:16 * k + 16] = 0
+        vs[page, 9, 1, k] = float(bad)
+        got, lse2 = _attend([*args[:2], vd, args[3], vs, *args[5:]])
+        nan = torch.zeros_like(out, dtype=torch.bool)
+        nan[0, hq // 2:, 32 * k:32 * k + 32] = True
+        assert torch.equal(torch.isnan(got), nan) and torch.equal(lse2, lse)
+        assert torch.equal(got[~nan], out[~nan])
