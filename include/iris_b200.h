@@ -57,6 +57,7 @@ extern "C" {
 #define IRIS_ERR_PIPELINE_TIMEOUT 0x80 /* a bounded wait gave up             (RuntimeError) */
 #define IRIS_ERR_SEQ_NEGATIVE 0x100    /* seq_len < 0, where it may be 0     (ValueError) */
 #define IRIS_ERR_OFFSETS 0x200         /* offsets or first token of a gather (ValueError) */
+#define IRIS_ERR_QUERY_LEN 0x400       /* more new tokens than cached ones   (ValueError) */
 
 /* ---- 16-bit element types of the entry points that take either ---------- */
 #define IRIS_DTYPE_FP16 0
@@ -399,6 +400,41 @@ IRIS_API int iris_b200_int4_page_bounds(const void* k_data, const void* k_scale,
                                         int32_t batch, int32_t num_kv_heads, int32_t head_dim, int64_t num_pages,
                                         int32_t page_size, int32_t max_pages_per_seq, int32_t* error_word,
                                         void* stream);
+
+/* Bytes of device workspace iris_b200_int4_paged_varlen_attention needs (0: none). */
+IRIS_API size_t iris_b200_varlen_attention_workspace_bytes(int64_t tokens, int32_t batch, int32_t num_q_heads,
+                                                           int32_t num_kv_heads, int32_t head_dim,
+                                                           int32_t max_pages_per_seq, int32_t window, int32_t has_prefix,
+                                                           int32_t has_offsets, int32_t device);
+
+/*
+ * Attention of new tokens over the INT4 paged cache that holds them already.
+ * Sequence b has the query rows cu_seqlens[b] .. cu_seqlens[b + 1] (int32
+ * [batch + 1], rising from 0; NULL: one row each, tokens == batch); they are
+ * the last of its seq_lens[b] cached tokens, row i at place pos =
+ * seq_lens[b] - rows + i.  No counterpart in the reference.
+ *   logit = softmax_scale * q.k;  logit_cap > 0: logit_cap * tanh(logit / logit_cap)
+ *   slopes [num_q_heads] fp32 or NULL: - slopes[h] * |pos - j|
+ * Token j is visible iff j < seq_lens[b] and j >= first_visible[row] (int32
+ * [tokens]; NULL: 0) and (j < prefix_lens[b] (int32 [batch]; NULL: 0) or (j <=
+ * pos and (window == 0 or j > pos - window))).
+ *   query [tokens, num_q_heads, head_dim] of `dtype`, tokens query_stride
+ *   elements apart (a multiple of 8); output dense, may be a dense query itself;
+ *   out_lse [tokens, num_q_heads] fp32 or NULL: log2-sum-exp2 of the logits.
+ * A row that sees nothing: output 0, lse -inf.  Rows behind cu_seqlens[batch]:
+ * the same.  A visible key scale that is not finite, or a query row that is
+ * not, makes the row's outputs and lse NaN; a visible value scale the outputs of its 32 dims.
+ * page_size 16, head_dim 64 or 128.  query, k_data, v_data, output and
+ * workspace 16-byte aligned, the scales 8-byte.  The workspace's contents do
+ * not matter and belong to one call at a time.
+ */
+IRIS_API int iris_b200_int4_paged_varlen_attention(
+    const void* query, int64_t query_stride, const void* k_data, const void* v_data, const void* k_scale,
+    const void* v_scale, const int32_t* block_table, int64_t block_table_stride, const int32_t* seq_lens,
+    const int32_t* cu_seqlens, const float* slopes, const int32_t* prefix_lens, const int32_t* first_visible, void* output,
+    float* out_lse, int64_t tokens, int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int64_t num_pages, int32_t page_size, int32_t max_pages_per_seq, int32_t window, float logit_cap, float softmax_scale,
+    int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* error_word, void* stream);
 
 /* Bytes of device workspace iris_b200_page_select needs. */
 IRIS_API size_t iris_b200_page_select_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t max_pages_per_seq);

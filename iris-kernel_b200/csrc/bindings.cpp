@@ -590,6 +590,123 @@ PyObject* sparse_decode(PyObject* const* a) {
   return pair(first_out, THPVariable_Wrap(std::move(lse)));
 }
 
+// ------------------------------------------------- attention of new tokens
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw Raised{};
+  return v;
+}
+
+// What attention of new tokens and its weights share: the query's rows, the sequences, what a row sees.
+struct NewTokens {
+  Rows query;
+  Table table;
+  int64_t tokens, hq, batch;
+  int32_t code, window;
+  float scale, cap;
+  const Tensor *cu, *slopes, *prefix, *first;
+};
+NewTokens new_tokens(const Tensor& query, const Cache& c, const Tensor& bt, const Tensor& lens, PyObject* cu_arg,
+                     PyObject* page_arg, PyObject* group_arg, PyObject* scale_arg, PyObject* cap_arg,
+                     PyObject* slopes_arg, PyObject* window_arg, PyObject* prefix_arg, PyObject* first_arg,
+                     c10::Device device) {
+  NewTokens n;
+  require(integer(group_arg) == 32, PyExc_NotImplementedError, "varlen attention currently supports group_size=32");
+  require(integer(page_arg) == 16, PyExc_NotImplementedError, "varlen attention currently supports page_size=16");
+  require(c.dim == 64 || c.dim == 128, PyExc_NotImplementedError,
+          "varlen attention currently supports head_dim in {64, 128}");
+  require(query.dim() == 3, PyExc_ValueError, "query must have shape [T, Hq, D]");
+  n.code = dtype_code("query", query.scalar_type());
+  n.tokens = query.size(0);
+  n.hq = query.size(1);
+  require(c.page_size == 16 && query.size(2) == c.dim, PyExc_ValueError,
+          "packed cache shape does not match query/page_size");
+  require(c.heads > 0 && n.hq > 0 && n.hq % c.heads == 0, PyExc_ValueError,
+          "num_query_heads must be divisible by num_kv_heads");
+  n.query = token_rows("query", query, query.sizes(), query.scalar_type(), device);
+  if (n.tokens == 1) n.query.stride = n.hq * c.dim;
+  require(bt.dim() == 2, PyExc_ValueError, "block_table must have shape [B, max_pages_per_sequence]");
+  n.batch = bt.size(0);
+  n.table = block_table(bt, n.batch, device);
+  check("seq_lens", lens, {n.batch}, at::kInt, device);
+  n.cu = optional_tensor(cu_arg, "cu_seqlens");
+  if (n.cu != nullptr)
+    check("cu_seqlens", *n.cu, {n.batch + 1}, at::kInt, device);
+  else
+    require(n.tokens == n.batch, PyExc_ValueError, "query needs one row a sequence, or cu_seqlens");
+  n.slopes = optional_tensor(slopes_arg, "slopes");
+  if (n.slopes != nullptr) check("slopes", *n.slopes, {n.hq}, at::kFloat, device);
+  n.prefix = optional_tensor(prefix_arg, "prefix_lens");
+  if (n.prefix != nullptr) check("prefix_lens", *n.prefix, {n.batch}, at::kInt, device);
+  n.first = optional_tensor(first_arg, "first_visible");
+  if (n.first != nullptr) check("first_visible", *n.first, {n.tokens}, at::kInt, device);
+  n.window = integer32(window_arg, "window");
+  require(n.window >= 0, PyExc_ValueError, "window must not be negative");
+  double scale = scale_arg == Py_None ? 0.0 : number(scale_arg);
+  if (scale == 0.0) scale = c.dim == 64 ? 0.125 : 0.08838834764831845;  // dim ** -0.5
+  n.scale = static_cast<float>(scale);
+  require(n.scale > 0.0f && n.scale <= 3.0e38f, PyExc_ValueError, "softmax_scale must be positive and finite");
+  n.cap = static_cast<float>(number(cap_arg));
+  require(n.cap >= 0.0f && n.cap <= 3.0e38f, PyExc_ValueError, "logit_cap must be finite and not negative");
+  require(n.tokens <= INT32_MAX && n.hq <= INT32_MAX && n.batch <= INT32_MAX && c.heads <= INT32_MAX, PyExc_ValueError,
+          "too many tokens, heads or sequences");
+  if (n.tokens > 0) {
+    require(n.batch > 0, PyExc_ValueError, "query must be empty without sequences");
+    require(c.num_pages > 0, PyExc_IndexError, "block_table contains an invalid physical page id");
+  }
+  return n;
+}
+const float* floats(const Tensor* t) { return t == nullptr ? nullptr : static_cast<const float*>(t->const_data_ptr()); }
+
+// (query, k_data, v_data, k_scale, v_scale, block_table, seq_lens, cu_seqlens, output, page_size, group_size,
+//  softmax_scale, logit_cap, slopes, window, prefix_lens, first_visible, return_lse) -> output or (output, lse)
+PyObject* varlen_attention(PyObject* const* a) {
+  const Tensor &query = tensor(a[0], "query"), &kd = tensor(a[1], "k_data"), &vd = tensor(a[2], "v_data"),
+               &ks = tensor(a[3], "k_scale"), &vs = tensor(a[4], "v_scale"), &bt = tensor(a[5], "block_table"),
+               &lens = tensor(a[6], "seq_lens");
+  const Tensor* output = optional_tensor(a[8], "output");
+  const c10::Device device = device_of("query", query);
+  const Cache c = cache_shape(kd);
+  const NewTokens n = new_tokens(query, c, bt, lens, a[7], a[9], a[10], a[11], a[12], a[13], a[14], a[15], a[16], device);
+  check_cache(c, kd, vd, ks, vs, device);
+  Tensor o, lse;
+  if (output == nullptr) {
+    o = empty(query.sizes(), query.scalar_type(), device);
+  } else {
+    check("output", *output, query.sizes(), query.scalar_type(), device);
+    // (in a dense query's own place it is: a row is read before it is written)
+    const bool in_place = output->const_data_ptr() == query.const_data_ptr() && query.is_contiguous();
+    check_apart("output", *output,
+                {{"query", in_place ? nullptr : &query}, {"k_data", &kd}, {"v_data", &vd}, {"k_scale", &ks},
+                 {"v_scale", &vs}, {"block_table", &bt}, {"seq_lens", &lens}, {"cu_seqlens", n.cu}, {"slopes", n.slopes},
+                 {"prefix_lens", n.prefix}, {"first_visible", n.first}});
+    require(reinterpret_cast<uintptr_t>(ptr(*output)) % 16 == 0, PyExc_ValueError,
+            "output must start on a 16-byte boundary");
+    o = *output;
+  }
+  const int with_lse = PyObject_IsTrue(a[17]);
+  if (with_lse < 0) throw Raised{};
+  if (with_lse) lse = empty({n.tokens, n.hq}, at::kFloat, device);
+  if (n.tokens > 0) {
+    const size_t bytes = iris_b200_varlen_attention_workspace_bytes(
+        n.tokens, static_cast<int32_t>(n.batch), static_cast<int32_t>(n.hq), static_cast<int32_t>(c.heads),
+        static_cast<int32_t>(c.dim), n.table.width, n.window, n.prefix != nullptr, n.cu != nullptr, device.index());
+    Tensor ws;
+    if (bytes > 0) ws = workspace(bytes, device);
+    launch("iris_b200_int4_paged_varlen_attention", device, [&](int32_t* word, void* stream) {
+      return iris_b200_int4_paged_varlen_attention(
+          n.query.data, n.query.stride, ptr(kd), ptr(vd), ptr(ks), ptr(vs), n.table.data, n.table.stride, ints(lens),
+          ints(n.cu), floats(n.slopes), ints(n.prefix), ints(n.first), out(o),
+          with_lse ? static_cast<float*>(out(lse)) : nullptr, n.tokens, static_cast<int32_t>(n.batch),
+          static_cast<int32_t>(n.hq), static_cast<int32_t>(c.heads), static_cast<int32_t>(c.dim), c.num_pages, 16,
+          n.table.width, n.window, n.cap, n.scale, n.code, ws.defined() ? out(ws) : nullptr, bytes, word, stream);
+    });
+  }
+  PyObject* first_out = given_or(a[8], o);
+  if (!with_lse) return first_out;
+  return pair(first_out, THPVariable_Wrap(std::move(lse)));
+}
+
 // ------------------------------------------------------------------- module
 template <PyObject* (*kFn)(PyObject* const*), int kArgs>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -628,6 +745,7 @@ PyMethodDef g_methods[] = {
     method<page_bounds, 10>("page_bounds"),
     method<page_select, 11>("page_select"),
     method<sparse_decode, 14>("sparse_decode"),
+    method<varlen_attention, 18>("varlen_attention"),
     {nullptr, nullptr, 0, nullptr},
 };
 

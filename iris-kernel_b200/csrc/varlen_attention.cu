@@ -1,0 +1,756 @@
+// Attention of new tokens over the INT4 paged cache (prompts, chunks of
+// prompts, drafts, single tokens): the public form is
+// iris_b200_int4_paged_varlen_attention.
+//
+// A block owns up to 128 * kTiles rows (new token x query head) of one KV head
+// and walks the tiles of 128 cached tokens that any of them sees.  Its warps:
+//   * softmax warps, a row a thread, four warps a row tile: scores from tensor
+//     memory, mask, cap and bias, running maximum and sum in registers,
+//     probabilities back to tensor memory as the next product's operand;
+//   * unpacking warps, a cached token a thread: packed rows and scales arrive in
+//     a ring of the thread's own (cp.async), and leave as swizzled fp16 tiles;
+//   * one warp that issues the products: S = Q K^T (both operands in shared
+//     memory, K-major) and O += P V (P in tensor memory, V as it lies, MN-major).
+// Two row tiles take turns: one's softmax runs while the other's products do.
+//
+// Roundings.  Stored values are nibble * scale, 15 bits: fp16 keeps 11.  Each
+// run of 32 tokens is first scaled by a power of two that brings its largest
+// scale into [2^12, 2^13), so that neither large scales overflow nor small
+// ones lose bits; the power goes into the logit's factor (keys) and the
+// probability's exponent (values).  Probabilities are fp16 with the row's
+// reference at 2^8.  Logits, statistics and sums are fp32.
+#include "varlen_common.cuh"
+
+namespace iris {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr float kRise = 7.0f;    // log2 that a row's logits may pass its reference by
+constexpr float kHead = 8.0f;    // log2 of the reference's own probability
+#define kMinusInf (-__int_as_float(0x7f800000))
+
+struct AttendParams {
+  VarlenBatch s;
+  const uint16_t* query;
+  const uint8_t *k_data, *v_data;
+  const uint8_t *k_scale, *v_scale;
+  void* out;
+  float* out_lse;   // or NULL
+  float* part_o;    // [splits][tokens][hq][D], splits > 1
+  float* part_lse;  // [splits][tokens][hq]
+  int64_t q_stride; // elements between tokens of the query
+  int32_t splits;
+  int32_t bf16;
+};
+
+template <int D, int kTiles>
+struct Cfg {
+  static constexpr int kUnpackGroups = kTiles == 1 ? 2 : 1;        // warpgroups that unpack
+  static constexpr int kRing = 3;                                  // raw units a ring
+  static constexpr int kOperand = kTile * D * 2;                   // one fp16 tile
+  static constexpr int kUnit = kTile * (D / 2 + D / 16);           // one packed tile with its scales
+  static constexpr int kSmem = 1024 + (kTiles + 4) * kOperand + kUnpackGroups * kRing * kUnit;
+  static constexpr int kColumns = kTiles == 2 ? 512 : 256;
+  static constexpr int kOutColumn = kTiles * kTile;                // first column of O
+  static constexpr int kSoftWarps = 4 * kTiles;
+  static constexpr int kMmaWarp = kSoftWarps + 4 * kUnpackGroups;
+};
+
+struct Shared {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_full[2], o_full[2], drain;
+  uint32_t tmem;
+  int32_t k_exp[4][4], v_exp[4][4];  // [tile & 3][run of 32 tokens]
+  uint32_t v_any[2][4];              // a run has values that are not finite
+  uint8_t v_bad[2][kTile];           // which groups of a token's
+  // the block's work
+  int32_t b, index, start, count, len, first_lo;
+  int32_t live;
+};
+
+IRIS_DEV bool wait_all(uint64_t* bar, uint32_t parity, int32_t* err) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, err));
+}
+
+// ------------------------------------------------------------------ unpacking
+// kKind: 0 keys, 1 values, 2 both in turn.
+template <int D, int kTiles, int kKind>
+IRIS_DEV void unpack_tiles(const AttendParams& p, Shared& sh, const Tiles& tiles, int k0, int n, int b, int len, int h,
+                           uint32_t ring, uint32_t k_tiles, uint32_t v_tiles, int tid) {
+  using C = Cfg<D, kTiles>;
+  constexpr int kChunks = D / 32;
+  const int warp = tid >> 5, lane = tid & 31;
+  const int units = kKind == 2 ? 2 * n : n;
+  const int64_t row_bytes = static_cast<int64_t>(p.s.hkv) * (D / 2);
+  int32_t next_page = page_of(p.s, b, tiles.at(k0) * kTile + tid, len), page = 0;
+  int loaded = -1;  // tile that `page` belongs to
+  auto load = [&](int u) {
+    if (u < units) {
+      const int k = kKind == 2 ? u >> 1 : u;
+      const bool keys = kKind == 0 || (kKind == 2 && (u & 1) == 0);
+      const int32_t j = tiles.at(k0 + k) * kTile + tid;
+      if (k != loaded) {
+        page = next_page;
+        loaded = k;
+        if (k + 1 < n) next_page = page_of(p.s, b, tiles.at(k0 + k + 1) * kTile + tid, len);
+      }
+      const bool there = j < len;
+      const int64_t row = static_cast<int64_t>(page) * kTokPage + j % kTokPage;
+      const uint8_t* data = (keys ? p.k_data : p.v_data) + row * row_bytes + h * (D / 2);
+      const uint8_t* scale = (keys ? p.k_scale : p.v_scale) + (row * p.s.hkv + h) * (D / 16);
+      const uint32_t slot = ring + (u % C::kRing) * C::kUnit;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) copy_async<16>(slot + c * 2048 + tid * 16, data + c * 16, there);
+      copy_async<D / 16>(slot + kChunks * 2048 + tid * (D / 16), scale, there);
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int u = 0; u < C::kRing - 1; ++u) load(u);
+  for (int u = 0; u < units; ++u) {
+    load(u + C::kRing - 1);
+    copies_wait<C::kRing - 1>();
+    const int k = kKind == 2 ? u >> 1 : u;
+    const bool keys = kKind == 0 || (kKind == 2 && (u & 1) == 0);
+    const uint32_t slot = ring + (u % C::kRing) * C::kUnit;
+    // scales: what the run of 32 tokens is scaled by, and what is not finite
+    uint32_t sc[kChunks / 2];
+    if constexpr (D == 128) {
+      const uint2 v = lds64(slot + kChunks * 2048 + tid * 8);
+      sc[0] = v.x;
+      sc[1] = v.y;
+    } else {
+      sc[0] = lds32(slot + kChunks * 2048 + tid * 4);
+    }
+    const bool there = tiles.at(k0 + k) * kTile + tid < len;
+    uint32_t most = 0, bad = 0;
+    float f[kChunks];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const uint32_t bits = there ? (sc[c / 2] >> (16 * (c & 1))) & 0xffffu : 0u;
+      const uint32_t mag = bits & 0x7fffu;
+      if (mag >= 0x7c00u) bad |= 1u << c; else most = max(most, mag);
+      f[c] = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+    }
+    const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 10);
+    const float up = pow2i(27 - e);
+    uint32_t s2[kChunks];  // the scale twice, as fp16
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const float v = f[c] * up;
+      s2[c] = (bad >> c) & 1u ? (keys ? 0x7fff7fffu : 0u) : Fp16Elem::pack(v, v);
+    }
+    const int st = k & 1;
+    if (!wait_all(keys ? &sh.k_empty[st] : &sh.v_empty[st], ((k >> 1) & 1) ^ 1, p.s.err)) break;
+    if (keys) {
+      if (lane == 0) sh.k_exp[k & 3][warp] = e - 27;
+    } else {
+      const bool any = __any_sync(0xffffffffu, bad != 0);
+      if (lane == 0) {
+        sh.v_exp[k & 3][warp] = e - 27;
+        sh.v_any[st][warp] = any;
+      }
+      if (any) sh.v_bad[st][tid] = static_cast<uint8_t>(bad);
+    }
+    const uint32_t dst = (keys ? k_tiles : v_tiles) + st * C::kOperand;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const uint4 w4 = lds128(slot + c * 2048 + tid * 16);
+      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+      const __half2 s = u32_as_h2(s2[c]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = w[i], hi = w[i] >> 8;
+        sts128(dst + operand_at(tid, 4 * c + i), h2_as_u32(__hmul2(u32_as_h2(int4_lo_exact(lo)), s)),
+               h2_as_u32(__hmul2(u32_as_h2(int4_hi_exact(lo)), s)), h2_as_u32(__hmul2(u32_as_h2(int4_lo_exact(hi)), s)),
+               h2_as_u32(__hmul2(u32_as_h2(int4_hi_exact(hi)), s)));
+      }
+    }
+    fence_proxy_async_shared();
+    mbar_arrive(keys ? &sh.k_full[st] : &sh.v_full[st]);
+  }
+  copies_wait<0>();
+}
+
+// ------------------------------------------------------------------- products
+template <int D, int kTiles>
+IRIS_DEV void issue_products(const AttendParams& p, Shared& sh, int n, int active, uint32_t q_tiles, uint32_t k_tiles,
+                             uint32_t v_tiles, uint32_t tmem, int lane) {
+  using C = Cfg<D, kTiles>;
+  constexpr uint32_t kScores = umma_idesc(kTile, kTile, false), kOut = umma_idesc(kTile, D, true);
+  auto scores = [&](int i, int k) {
+    if (lane == 0) {
+      const uint32_t q = q_tiles + i * C::kOperand, kk = k_tiles + (k & 1) * C::kOperand;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) {
+        const uint32_t at = (s >> 2) * (kTile * 128) + (s & 3) * 32;
+        umma_ss(tmem + i * kTile, umma_desc(q + at, 16, 1024), umma_desc(kk + at, 16, 1024), kScores, s > 0);
+      }
+      umma_commit(smem_u32(&sh.s_full[i]));
+      if (i == active - 1) umma_commit(smem_u32(&sh.k_empty[k & 1]));
+    }
+    __syncwarp();
+  };
+  bool ok = wait_all(&sh.k_full[0], 0, p.s.err);
+  if (ok) {
+    umma_fence_after();
+    for (int i = 0; i < active; ++i) scores(i, 0);
+  }
+  for (int k = 0; ok && k < n; ++k) {
+    ok = wait_all(&sh.v_full[k & 1], (k >> 1) & 1, p.s.err);
+    for (int i = 0; ok && i < active; ++i) {
+      ok = wait_all(&sh.p_full[i], k & 1, p.s.err);
+      if (!ok) break;
+      umma_fence_after();
+      if (lane == 0) {
+        const uint32_t v = v_tiles + (k & 1) * C::kOperand;
+#pragma unroll
+        for (int s = 0; s < kTile / 16; ++s)
+          umma_ts(tmem + C::kOutColumn + i * D, tmem + i * kTile + 8 * s, umma_desc(v + s * 2048, kTile * 128, 1024), kOut,
+                  k > 0 || s > 0);
+        umma_commit(smem_u32(&sh.o_full[i]));
+        if (i == active - 1) umma_commit(smem_u32(&sh.v_empty[k & 1]));
+      }
+      __syncwarp();
+      if (k + 1 < n) {
+        if (i == 0) ok = wait_all(&sh.k_full[(k + 1) & 1], ((k + 1) >> 1) & 1, p.s.err);
+        if (!ok) break;
+        umma_fence_after();
+        scores(i, k + 1);
+      }
+    }
+  }
+  // everything issued is done before the block lets go of its memory
+  if (lane == 0) umma_commit(smem_u32(&sh.drain));
+  __syncwarp();
+  wait_all(&sh.drain, 0, p.s.err);
+}
+
+// -------------------------------------------------------------------- softmax
+template <int D, int kTiles, bool kCap, bool kBias>
+IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles, int k0, int n, int rows, int h, int tile,
+                           uint32_t q_tiles, uint32_t tmem, int split, int warp, int lane) {
+  using C = Cfg<D, kTiles>;
+  constexpr bool kMod = kCap || kBias;
+  const int local = warp * 32 + lane;  // row of the row tile
+  const int r = sh.index * (kTile * kTiles) + tile * kTile + local;
+  const bool valid = r < rows;
+  const int i = valid ? r / p.s.group : 0, g = valid ? r % p.s.group : 0;
+  const int token = sh.start + i, head = h * p.s.group + g;
+  const int32_t pos = sh.len - sh.count + i;
+  Sight sight = {0, 0, 0, 0};
+  float back = 1.0f;  // undoes the query row's power of two
+  if (valid) {
+    const int32_t prefix = p.s.prefix_lens != nullptr ? __ldg(p.s.prefix_lens + sh.b) : 0;
+    const int32_t first = p.s.first_visible != nullptr ? __ldg(p.s.first_visible + token) : 0;
+    sight = row_sight(pos, first, prefix, p.s.window, sh.len);
+    if (n > 0) {
+      const uint4* src = reinterpret_cast<const uint4*>(p.query + token * p.q_stride + static_cast<int64_t>(head) * D);
+      uint32_t w[D / 2];
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 v = src[c];
+        w[4 * c] = v.x;
+        w[4 * c + 1] = v.y;
+        w[4 * c + 2] = v.z;
+        w[4 * c + 3] = v.w;
+      }
+      back = scale_row<D>(w, p.bf16 != 0);
+      const uint32_t dst = q_tiles + tile * C::kOperand;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 v = order8(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+        sts128(dst + operand_at(local, c), v.x, v.y, v.z, v.w);
+      }
+    }
+  }
+  fence_proxy_async_shared();
+  asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftWarps * 32 + 32) : "memory");  // with the warp of the products
+
+  const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+  const uint32_t s_at = lanes + tile * kTile, o_at = lanes + C::kOutColumn + tile * D;
+  const bool busy = __any_sync(0xffffffffu, valid);
+  const float unit = kCap ? p.s.scale * back / p.s.cap : p.s.scale * kLog2e * back;
+  const float cap2 = p.s.cap * kLog2e;
+  const float slope2 = kBias ? -__ldg(p.s.slopes + head) * kLog2e : 0.0f;
+  float m = kMinusInf, l = 0.0f;
+  int ref = -127;
+  uint32_t spoilt = 0;  // groups of dims with a visible value that is not finite
+  bool ok = true;
+  for (int k = 0; k < n; ++k) {
+    if (!(ok = wait_all(&sh.s_full[tile], k & 1, p.s.err))) break;
+    if (!(ok = wait_all(&sh.v_full[k & 1], (k >> 1) & 1, p.s.err))) break;
+    umma_fence_after();
+    if (busy) {
+      float s[kTile];
+      uint32_t* sw = reinterpret_cast<uint32_t*>(s);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) umma_ld32(s_at + 32 * c, sw + 32 * c);
+      umma_wait_ld();
+#pragma unroll
+      for (int j = 0; j < kTile; ++j) asm volatile("" : "+f"(s[j]));
+      const int32_t base = tiles.at(k0 + k) * kTile;
+      float f[4];
+      int ve[4], top_e = ref;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        f[c] = fmaxf(unit * pow2i(sh.k_exp[k & 3][c]), 1.17549435e-38f);
+        ve[c] = sh.v_exp[k & 3][c];
+        top_e = max(top_e, ve[c]);
+      }
+      if (kMod) {
+        const float d0 = static_cast<float>(pos - base);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int j = 32 * c; j < 32 * c + 32; ++j) {
+            float y = s[j] * f[c];
+            if (kCap) y = cap2 * tanh_f(y);
+            if (kBias) y = fmaf(slope2, fabsf(d0 - j), y);
+            s[j] = y;
+          }
+      }
+      const bool full = !valid || (sight.b0 <= base && base + kTile <= sight.b1) ||
+                        (sight.a0 <= base && base + kTile <= sight.a1);
+      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+      if (!__all_sync(0xffffffffu, full)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          bits[c] = sight_bits(sight, base + 32 * c);
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (!((bits[c] >> j) & 1u)) s[32 * c + j] = kMinusInf;
+        }
+      }
+      float top = kMinusInf;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float t = s[32 * c];
+#pragma unroll
+        for (int j = 1; j < 32; ++j) t = fmaxf(t, s[32 * c + j]);
+        top = fmaxf(top, kMod ? t : t * f[c]);
+      }
+      // raise the row's reference where its logits pass it by too much, and the values' power where one is larger
+      const bool rise = top > m + kRise;  // (also from -inf)
+      if (__any_sync(0xffffffffu, rise) || top_e > ref) {
+        const float to = rise ? top : m;
+        if (k > 0) {
+          const float by = (rise ? ex2(m - to) : 1.0f) * pow2i(max(ref - top_e, -126));
+          if (!(ok = wait_all(&sh.o_full[tile], (k - 1) & 1, p.s.err))) break;
+          umma_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            umma_ld32(o_at + 32 * c, o);
+            umma_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              asm volatile("" : "+r"(o[j]));
+              o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
+            }
+            umma_st32(o_at + 32 * c, o);
+          }
+          if (rise) l *= ex2(m - to);
+        }
+        m = to;
+        ref = top_e;
+      }
+      const float zero = m == kMinusInf ? 0.0f : -m;  // (a row that sees nothing yet)
+      // a product that is not rounded as the reference was may pass it by half a step, which is 2^7 from 2^31 on:
+      // so far out products are rounded first
+      if (!kMod && __any_sync(0xffffffffu, fabsf(m) > 16777216.0f && m != kMinusInf)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+          for (int j = 32 * c; j < 32 * c + 32; ++j) s[j] *= f[c];
+          f[c] = 1.0f;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float add = zero + (kHead + static_cast<float>(ve[c] - ref));
+        float2 sum = make_float2(0.0f, 0.0f);
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float2 y = make_float2(s[32 * c + 2 * j], s[32 * c + 2 * j + 1]);
+          y = kMod ? __fadd2_rn(y, make_float2(add, add)) : __ffma2_rn(y, make_float2(f[c], f[c]), make_float2(add, add));
+          y.x = ex2(y.x);
+          y.y = ex2(y.y);
+          sum = __fadd2_rn(sum, y);
+          w[j] = Fp16Elem::pack(y.x, y.y);
+        }
+        l = fmaf(sum.x + sum.y, pow2i(min(ref - ve[c], 126)) * (1.0f / 256.0f), l);
+        umma_st16(s_at + 16 * c, w);
+      }
+      if (sh.v_any[k & 1][0] | sh.v_any[k & 1][1] | sh.v_any[k & 1][2] | sh.v_any[k & 1][3]) {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          if (!sh.v_any[k & 1][c]) continue;
+          for (uint32_t left = valid ? sight_bits(sight, base + 32 * c) : 0u; left != 0; left &= left - 1)
+            spoilt |= sh.v_bad[k & 1][32 * c + __ffs(left) - 1];
+        }
+      }
+      umma_wait_st();
+    }
+    umma_fence_before();
+    mbar_arrive(&sh.p_full[tile]);
+  }
+  // the row's output
+  if (ok && n > 0) {
+    ok = wait_all(&sh.o_full[tile], (n - 1) & 1, p.s.err);
+    umma_fence_after();
+  }
+  if (!busy || !ok) return;
+  const bool whole = p.splits == 1;
+  const int64_t row = static_cast<int64_t>(token) * p.s.hq + head;
+  const float norm = l == 0.0f ? 0.0f : pow2i(max(ref, -126)) * (1.0f / 256.0f) / l;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    if (n > 0) {
+      umma_ld32(o_at + 32 * c, o);
+      umma_wait_ld();
+    }
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      if (n > 0) asm volatile("" : "+r"(o[j]));
+      v[j] = n > 0 && l != 0.0f ? __uint_as_float(o[j]) * norm : 0.0f;
+      if ((spoilt >> c) & 1u) v[j] = __int_as_float(0x7fffffff);
+    }
+    if (!valid) continue;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {  // 8 dims, back in their order
+      const float* x = v + 8 * q;
+      if (whole) {
+        uint4 w;
+        if (p.bf16)
+          w = make_uint4(Bf16Elem::pack(x[0], x[2]), Bf16Elem::pack(x[4], x[6]), Bf16Elem::pack(x[1], x[3]),
+                         Bf16Elem::pack(x[5], x[7]));
+        else
+          w = make_uint4(Fp16Elem::pack(x[0], x[2]), Fp16Elem::pack(x[4], x[6]), Fp16Elem::pack(x[1], x[3]),
+                         Fp16Elem::pack(x[5], x[7]));
+        reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * D)[4 * c + q] = w;
+      } else {
+        float4* dst = reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(split) * p.s.tokens * p.s.hq + row) * D);
+        dst[2 * (4 * c + q)] = make_float4(x[0], x[2], x[4], x[6]);
+        dst[2 * (4 * c + q) + 1] = make_float4(x[1], x[3], x[5], x[7]);
+      }
+    }
+  }
+  if (!valid) return;
+  const float lse = l == 0.0f ? kMinusInf : (m == kMinusInf ? 0.0f : m) + lg2(l);
+  if (!whole)
+    p.part_lse[static_cast<int64_t>(split) * p.s.tokens * p.s.hq + row] = lse;
+  else if (p.out_lse != nullptr)
+    p.out_lse[row] = lse;
+}
+
+template <int D, int kTiles, bool kCap, bool kBias>
+__global__ void __launch_bounds__(kThreads, 1) varlen_attention_kernel(const AttendParams p) {
+  using C = Cfg<D, kTiles>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Shared sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int unit = blockIdx.x / (p.s.hkv * p.splits);
+  const int h = blockIdx.x / p.splits % p.s.hkv, split = blockIdx.x % p.splits;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.k_full[i], 128);
+      mbar_init(&sh.v_full[i], 128);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 128);
+      mbar_init(&sh.o_full[i], 1);
+    }
+    mbar_init(&sh.drain, 1);
+    fence_barrier_init();
+  }
+  grid_dependency_wait();
+  grid_dependents_launch();
+  if (warp == 0) {
+    if (blockIdx.x == 0) check_offsets(p.s, lane);
+    Block blk = {0, 0};
+    const bool live = find_block(p.s, unit, kTile * kTiles, lane, &blk);
+    int first = 0;
+    Span sp = {0, 0};
+    int32_t len = 0;
+    if (live) {
+      sp = new_tokens(p.s, blk.b);
+      len = cached_tokens(p.s, blk.b, sp.count, lane == 0 && h == 0 && split == 0 && blk.index == 0);
+      if (p.s.first_visible != nullptr) {
+        const int64_t r0 = static_cast<int64_t>(blk.index) * (kTile * kTiles);
+        const int i0 = static_cast<int>(r0 / p.s.group);
+        const int i1 = static_cast<int>(min((r0 + kTile * kTiles - 1) / p.s.group, static_cast<int64_t>(sp.count - 1)));
+        first = INT32_MAX;
+        for (int i = i0 + lane; i <= i1; i += 32) first = min(first, __ldg(p.s.first_visible + sp.start + i));
+        first = __reduce_min_sync(0xffffffffu, first);
+      }
+    }
+    if (lane == 0) {
+      sh.live = live;
+      sh.b = blk.b;
+      sh.index = blk.index;
+      sh.start = sp.start;
+      sh.count = sp.count;
+      sh.len = len;
+      sh.first_lo = first;
+    }
+  }
+  // rows that the offsets leave over: zeros
+  for (int64_t row = static_cast<int64_t>(used_rows(p.s)) * p.s.hq + blockIdx.x; row < static_cast<int64_t>(p.s.tokens) * p.s.hq;
+       row += gridDim.x) {
+    if (threadIdx.x < D / 2) reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + row * D)[threadIdx.x] = 0u;
+    if (threadIdx.x == 0 && p.out_lse != nullptr) p.out_lse[row] = kMinusInf;
+  }
+  __syncthreads();
+  if (!sh.live) return;
+  if (warp == C::kMmaWarp) umma_alloc(&sh.tmem, C::kColumns);
+  umma_fence_before();
+  __syncthreads();
+  umma_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  const int rows = sh.count * p.s.group;
+  const int r0 = sh.index * (kTile * kTiles), r1 = min(r0 + kTile * kTiles, rows);
+  const int active = r1 - r0 > kTile ? 2 : 1;
+  const int32_t off = sh.len - sh.count;
+  const int32_t prefix = p.s.prefix_lens != nullptr ? __ldg(p.s.prefix_lens + sh.b) : 0;
+  const Tiles tiles =
+      tiles_seen(off + r0 / p.s.group, off + (r1 - 1) / p.s.group, sh.first_lo, prefix, p.s.window, sh.len);
+  const int64_t all = tiles.count();
+  const int k0 = static_cast<int>(all * split / p.splits), n = static_cast<int>(all * (split + 1) / p.splits) - k0;
+
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t q_tiles = base, k_tiles = base + kTiles * C::kOperand, v_tiles = k_tiles + 2 * C::kOperand;
+  const uint32_t ring = v_tiles + 2 * C::kOperand;
+  // Registers: 512 threads come with 128 each.  kTiles 2: 256 x 176 + 256 x 80
+  // = 65,536; kTiles 1: 128 x 176 + 256 x 120 + 128 x 80 = 63,488.
+  if (warp < C::kSoftWarps) {
+    regs_take<176>();
+    const int tile = warp >> 2;
+    if (tile < active) {
+      softmax_rows<D, kTiles, kCap, kBias>(p, sh, tiles, k0, n, rows, h, tile, q_tiles, tmem, split, warp & 3, lane);
+    } else {
+      asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftWarps * 32 + 32) : "memory");
+    }
+  } else if (warp < C::kMmaWarp) {
+    const int tid = (threadIdx.x - C::kSoftWarps * 32) & 127;
+    if constexpr (kTiles == 2) {
+      regs_give<80>();
+      if (n > 0)
+        unpack_tiles<D, kTiles, 2>(p, sh, tiles, k0, n, sh.b, sh.len, h, ring, k_tiles, v_tiles, tid);
+    } else {
+      regs_give<120>();
+      if (n > 0) {
+        if (warp < C::kSoftWarps + 4)
+          unpack_tiles<D, kTiles, 0>(p, sh, tiles, k0, n, sh.b, sh.len, h, ring, k_tiles, v_tiles, tid);
+        else
+          unpack_tiles<D, kTiles, 1>(p, sh, tiles, k0, n, sh.b, sh.len, h, ring + C::kRing * C::kUnit, k_tiles, v_tiles,
+                                     tid);
+      }
+    }
+  } else {
+    regs_give<80>();
+    if (warp == C::kMmaWarp) {
+      asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftWarps * 32 + 32) : "memory");
+      if (n > 0) issue_products<D, kTiles>(p, sh, n, active, q_tiles, k_tiles, v_tiles, tmem, lane);
+    }
+  }
+  umma_fence_before();
+  __syncthreads();
+  umma_fence_after();
+  if (warp == C::kMmaWarp) umma_free(tmem, C::kColumns);
+}
+
+// Joins the parts of rows whose tiles several blocks shared: a warp a row.
+template <int D>
+__global__ void __launch_bounds__(256) varlen_join_kernel(const AttendParams p) {
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = static_cast<int64_t>(used_rows(p.s)) * p.s.hq, stride = static_cast<int64_t>(p.s.tokens) * p.s.hq;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  float top = kMinusInf;
+  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, __ldcg(p.part_lse + s * stride + row));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float zero = top == kMinusInf ? 0.0f : top;
+  float acc[D / 32] = {}, total = 0.0f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float part = __ldcg(p.part_lse + s * stride + row);
+    if (part == kMinusInf) continue;  // it saw nothing
+    const float w = ex2(part - zero);
+    total += w;
+    const float* o = p.part_o + (s * stride + row) * D + lane * (D / 32);
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) acc[j] = fmaf(w, __ldcg(o + j), acc[j]);
+  }
+  const float norm = total == 0.0f ? 0.0f : 1.0f / total;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + row * D) + lane * (D / 64);
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j) {
+    const float a = acc[2 * j] * norm, b = acc[2 * j + 1] * norm;
+    dst[j] = p.bf16 ? Bf16Elem::pack(a, b) : Fp16Elem::pack(a, b);
+  }
+  if (lane == 0 && p.out_lse != nullptr) p.out_lse[row] = total == 0.0f ? kMinusInf : zero + lg2(total);
+}
+
+// ----------------------------------------------------------------------- host
+// Two row tiles a block where sequences have more than 128 rows on average.
+int row_tiles(int64_t tokens, int32_t batch, int32_t group, bool offsets) {
+  return offsets && tokens * group > 128 * static_cast<int64_t>(batch) ? 2 : 1;
+}
+
+int64_t blocks_of(int64_t tokens, int32_t batch, int32_t group, bool offsets, int tiles) {
+  const int64_t rows = 128 * tiles;
+  if (!offsets) return batch * ((group + rows - 1) / rows);
+  return tokens * group / rows + (batch < tokens ? batch : tokens);  // every sequence's last block may be a short one
+}
+
+// Blocks that share a row's tiles: as many as bring a block to every SM, each with four tiles or more.
+int32_t splits_of(int64_t blocks, int32_t hkv, int32_t max_pages, int32_t window, bool prefix, int sms) {
+  int64_t tiles = (static_cast<int64_t>(max_pages) * kTokPage + kTile - 1) / kTile;
+  if (window > 0 && !prefix) tiles = tiles < window / kTile + 4 ? tiles : window / kTile + 4;
+  const int64_t want = sms / (blocks * hkv), most = tiles / 4;
+  const int64_t n = want < most ? want : most;
+  return static_cast<int32_t>(n < 1 ? 1 : n);
+}
+
+int sm_count(int device) {
+  static int known[64] = {};
+  if (device < 0 || device >= 64) return 148;
+  if (known[device] == 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) n = 148;
+    known[device] = n;
+  }
+  return known[device];
+}
+
+template <int D, int kTiles, bool kCap, bool kBias>
+cudaError_t launch_attend(const AttendParams& p, int64_t grid, cudaStream_t stream) {
+  auto fn = varlen_attention_kernel<D, kTiles, kCap, kBias>;
+  static thread_local uint64_t ready = 0;  // GPUs that know the kernel's shared memory
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (device >= 64 || !((ready >> device) & 1)) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D, kTiles>::kSmem);
+    if (e != cudaSuccess) return e;
+    if (device < 64) ready |= 1ull << device;
+  }
+  return launch_early(fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Cfg<D, kTiles>::kSmem, stream, p);
+}
+
+template <int D, int kTiles>
+cudaError_t launch_attend(const AttendParams& p, int64_t grid, cudaStream_t stream) {
+  const bool cap = p.s.cap > 0.0f, bias = p.s.slopes != nullptr;
+  if (cap && bias) return launch_attend<D, kTiles, true, true>(p, grid, stream);
+  if (cap) return launch_attend<D, kTiles, true, false>(p, grid, stream);
+  if (bias) return launch_attend<D, kTiles, false, true>(p, grid, stream);
+  return launch_attend<D, kTiles, false, false>(p, grid, stream);
+}
+
+}  // namespace
+}  // namespace iris
+
+using namespace iris;
+
+extern "C" size_t iris_b200_varlen_attention_workspace_bytes(int64_t tokens, int32_t batch, int32_t num_q_heads,
+                                                             int32_t num_kv_heads, int32_t head_dim,
+                                                             int32_t max_pages_per_seq, int32_t window, int32_t has_prefix,
+                                                             int32_t has_offsets, int32_t device) {
+  if (tokens <= 0 || batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0) return 0;
+  const int32_t group = num_q_heads / num_kv_heads;
+  const bool offsets = has_offsets != 0;
+  const int tiles = row_tiles(tokens, batch, group, offsets);
+  const int32_t splits = splits_of(blocks_of(tokens, batch, group, offsets, tiles), num_kv_heads, max_pages_per_seq, window,
+                                   has_prefix != 0, sm_count(device));
+  return splits > 1 ? static_cast<size_t>(splits) * tokens * num_q_heads * (head_dim + 1) * 4 : 0;
+}
+
+extern "C" int iris_b200_int4_paged_varlen_attention(
+    const void* query, int64_t query_stride, const void* k_data, const void* v_data, const void* k_scale,
+    const void* v_scale, const int32_t* block_table, int64_t block_table_stride, const int32_t* seq_lens,
+    const int32_t* cu_seqlens, const float* slopes, const int32_t* prefix_lens, const int32_t* first_visible, void* output,
+    float* out_lse, int64_t tokens, int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int64_t num_pages, int32_t page_size, int32_t max_pages_per_seq, int32_t window, float logit_cap, float softmax_scale,
+    int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* error_word, void* stream) {
+  if (tokens < 0 || batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || window < 0 ||
+      !(logit_cap >= 0.0f) || !(softmax_scale > 0.0f) || (dtype != IRIS_DTYPE_FP16 && dtype != IRIS_DTYPE_BF16))
+    return IRIS_EINVAL;
+  if (page_size != kTokPage || (head_dim != 64 && head_dim != 128)) return IRIS_EUNSUPPORTED;
+  if (cu_seqlens == nullptr && tokens != batch) return IRIS_EINVAL;
+  if (tokens == 0) return IRIS_OK;
+  if (batch == 0 || num_pages <= 0 || max_pages_per_seq <= 0) return IRIS_EINVAL;
+  if (query == nullptr || k_data == nullptr || v_data == nullptr || k_scale == nullptr || v_scale == nullptr ||
+      block_table == nullptr || seq_lens == nullptr || output == nullptr)
+    return IRIS_EINVAL;
+  const int32_t group = num_q_heads / num_kv_heads;
+  // rows, places and page offsets are 32-bit numbers in the kernel
+  if (tokens * group > INT32_MAX / 2 || num_pages > INT32_MAX || max_pages_per_seq > INT32_MAX / 2 / kTokPage)
+    return IRIS_EUNSUPPORTED;
+  if (!aligned_to(query, 16) || query_stride % 8 != 0 || !aligned_to(k_data, 16) || !aligned_to(v_data, 16) ||
+      !aligned_to(k_scale, 8) || !aligned_to(v_scale, 8) || !aligned_to(output, 16))
+    return IRIS_EALIGN;
+  const bool offsets = cu_seqlens != nullptr;
+  int device = 0;
+  clear_stale_cuda_error();
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return record_cuda_error(e, "cudaGetDevice"), IRIS_ECUDA;
+  const int tiles = row_tiles(tokens, batch, group, offsets);
+  const int64_t blocks = blocks_of(tokens, batch, group, offsets, tiles);
+  const int32_t splits = splits_of(blocks, num_kv_heads, max_pages_per_seq, window, prefix_lens != nullptr, sm_count(device));
+  const int64_t grid = blocks * num_kv_heads * splits;
+  if (grid > INT32_MAX) return IRIS_EUNSUPPORTED;
+  const size_t part = static_cast<size_t>(splits) * tokens * num_q_heads;
+  if (splits > 1 && (workspace == nullptr || workspace_bytes < part * (head_dim + 1) * 4)) return IRIS_EWORKSPACE;
+  if (splits > 1 && !aligned_to(workspace, 16)) return IRIS_EALIGN;
+  AttendParams p = {};
+  p.s.block_table = block_table;
+  p.s.bt_stride = block_table_stride;
+  p.s.seq_lens = seq_lens;
+  p.s.cu = cu_seqlens;
+  p.s.prefix_lens = prefix_lens;
+  p.s.first_visible = first_visible;
+  p.s.slopes = slopes;
+  p.s.err = error_word;
+  p.s.num_pages = num_pages;
+  p.s.tokens = static_cast<int32_t>(tokens);
+  p.s.batch = batch;
+  p.s.hq = num_q_heads;
+  p.s.hkv = num_kv_heads;
+  p.s.group = group;
+  p.s.max_pages = max_pages_per_seq;
+  p.s.window = window < (1 << 30) ? window : 0;
+  p.s.scale = softmax_scale;
+  p.s.cap = logit_cap;
+  p.query = static_cast<const uint16_t*>(query);
+  p.k_data = static_cast<const uint8_t*>(k_data);
+  p.v_data = static_cast<const uint8_t*>(v_data);
+  p.k_scale = static_cast<const uint8_t*>(k_scale);
+  p.v_scale = static_cast<const uint8_t*>(v_scale);
+  p.out = output;
+  p.out_lse = out_lse;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_lse = splits > 1 ? p.part_o + part * head_dim : nullptr;
+  p.q_stride = query_stride;
+  p.splits = splits;
+  p.bf16 = dtype == IRIS_DTYPE_BF16;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (head_dim == 128)
+    e = tiles == 2 ? launch_attend<128, 2>(p, grid, st) : launch_attend<128, 1>(p, grid, st);
+  else
+    e = tiles == 2 ? launch_attend<64, 2>(p, grid, st) : launch_attend<64, 1>(p, grid, st);
+  if (e != cudaSuccess) return record_cuda_error(e, "varlen_attention"), IRIS_ECUDA;
+  if (splits > 1) {
+    const dim3 join(static_cast<unsigned>((tokens * num_q_heads + 7) / 8));
+    e = head_dim == 128 ? launch_early(varlen_join_kernel<128>, join, dim3(256), 0, st, p)
+                        : launch_early(varlen_join_kernel<64>, join, dim3(256), 0, st, p);
+    if (e != cudaSuccess) return record_cuda_error(e, "varlen_join"), IRIS_ECUDA;
+  }
+  return IRIS_OK;
+}

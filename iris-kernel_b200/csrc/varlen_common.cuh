@@ -1,0 +1,242 @@
+// What attention over new tokens and its weights share: which rows a block
+// has, which cached tokens they see, and what becomes of a logit.
+//
+// Sequence b has n_b new tokens, the last n_b of its seq_lens[b] cached ones;
+// new token i is at place seq_lens[b] - n_b + i.  Row r of a (sequence, KV
+// head) is its new token r / group with query head r % group of the KV head.
+// A row at place `pos` sees token j iff
+//   j < seq_lens[b]  and  j >= first_visible  and
+//   (j < prefix_lens[b]  or  (j <= pos and (window == 0 or j > pos - window)))
+// which is two runs of tokens.
+#pragma once
+
+#include "elem.cuh"
+#include "umma.cuh"
+
+namespace iris {
+
+constexpr int kTile = 128;        // cached tokens of a tile
+constexpr int kTokPage = 16;      // tokens of a page
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct VarlenBatch {
+  const int32_t* block_table;
+  int64_t bt_stride;
+  const int32_t* seq_lens;
+  const int32_t* cu;             // [batch + 1], or NULL: one new token a sequence
+  const int32_t* prefix_lens;    // [batch] or NULL
+  const int32_t* first_visible;  // [tokens] or NULL
+  const float* slopes;           // [hq] or NULL
+  int32_t* err;
+  int64_t num_pages;
+  int32_t tokens;                // rows of the query
+  int32_t batch, hq, hkv, group, max_pages;
+  int32_t window;                // 0: none
+  float scale;                   // softmax scale
+  float cap;                     // 0: none
+};
+
+// New tokens [start, start + count) of sequence b; offsets outside the query are cut off.
+struct Span {
+  int32_t start, count;
+};
+IRIS_DEV Span new_tokens(const VarlenBatch& p, int b) {
+  if (p.cu == nullptr) return {b, 1};
+  const int32_t s = min(max(__ldg(p.cu + b), 0), p.tokens);
+  const int32_t e = min(max(__ldg(p.cu + b + 1), s), p.tokens);
+  return {s, e - s};
+}
+
+// Offsets have to rise from 0 and end inside the query (one warp looks).
+IRIS_DEV void check_offsets(const VarlenBatch& p, int lane) {
+  if (p.cu == nullptr) return;
+  bool bad = lane == 0 && __ldg(p.cu) != 0;
+  for (int b = lane; b < p.batch; b += 32) {
+    const int32_t s = __ldg(p.cu + b), e = __ldg(p.cu + b + 1);
+    bad |= s < 0 || e < s || e > p.tokens;
+  }
+  if (bad) set_error(p.err, IRIS_ERR_OFFSETS);
+}
+
+// Rows that the offsets leave over start here.
+IRIS_DEV int32_t used_rows(const VarlenBatch& p) {
+  return p.cu == nullptr ? min(p.batch, p.tokens) : min(max(__ldg(p.cu + p.batch), 0), p.tokens);
+}
+
+// Length of sequence b in the cache, as far as its pages go; `say` reports what is wrong with it.
+IRIS_DEV int32_t cached_tokens(const VarlenBatch& p, int b, int32_t count, bool say) {
+  int32_t n = __ldg(p.seq_lens + b);
+  if (n < 0) {
+    if (say) set_error(p.err, IRIS_ERR_SEQ_NEGATIVE);
+    return 0;
+  }
+  if ((static_cast<int64_t>(n) + kTokPage - 1) / kTokPage > p.max_pages) {
+    if (say) set_error(p.err, IRIS_ERR_BLOCK_TABLE);
+    n = p.max_pages * kTokPage;
+  }
+  if (n > 0 && n < count && say) set_error(p.err, IRIS_ERR_QUERY_LEN);
+  return n;
+}
+
+IRIS_DEV int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
+
+// Block u of all sequences' blocks of `rows` rows, heaviest first: the last
+// block of every sequence, then the one before it, and so on (a block's work
+// grows with its tokens' places).  One warp; false: there is no block u.
+struct Block {
+  int32_t b, index;
+};
+IRIS_DEV bool find_block(const VarlenBatch& p, int u, int rows, int lane, Block* out) {
+  if (p.cu == nullptr) {
+    const int per = (p.group + rows - 1) / rows;
+    out->b = u / per;
+    out->index = u % per;
+    return out->b < p.batch;
+  }
+  auto blocks = [&](int b) {
+    return static_cast<int32_t>((static_cast<int64_t>(new_tokens(p, b).count) * p.group + rows - 1) / rows);
+  };
+  int most = 0;
+  for (int b = lane; b < p.batch; b += 32) most = max(most, blocks(b));
+  most = __reduce_max_sync(0xffffffffu, most);
+  auto upto = [&](int depth) {  // blocks among the last `depth` of every sequence
+    int n = 0;
+    for (int b = lane; b < p.batch; b += 32) n += min(depth, blocks(b));
+    return warp_sum(n);
+  };
+  if (u >= upto(most)) return false;
+  int lo = 0, hi = most;  // upto(lo) <= u < upto(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (upto(mid) <= u) lo = mid; else hi = mid;
+  }
+  int left = u - upto(lo);
+  for (int base = 0; base < p.batch; base += 32) {
+    const int b = base + lane;
+    const int n = b < p.batch ? blocks(b) : 0;
+    const unsigned has = __ballot_sync(0xffffffffu, n > lo);
+    const int c = __popc(has);
+    if (left < c) {
+      const int src = __fns(has, 0, left + 1);
+      out->b = base + src;
+      out->index = __shfl_sync(0xffffffffu, n, src) - 1 - lo;
+      return true;
+    }
+    left -= c;
+  }
+  return false;
+}
+
+// What one row sees, as two runs [a0, a1) and [b0, b1) of tokens (a: prefix).
+struct Sight {
+  int32_t a0, a1, b0, b1;
+};
+IRIS_DEV Sight row_sight(int32_t pos, int32_t first, int32_t prefix, int32_t window, int32_t len) {
+  Sight s;
+  s.a0 = max(first, 0);
+  s.a1 = min(prefix, len);
+  s.b0 = window > 0 ? max(s.a0, pos - window + 1) : s.a0;
+  s.b1 = min(pos + 1, len);
+  return s;
+}
+
+// Bits [lo, hi) of 32, bounds anywhere.
+IRIS_DEV uint32_t bits_between(int lo, int hi) {
+  lo = max(lo, 0);
+  hi = min(hi, 32);
+  if (hi <= lo) return 0u;
+  return (0xffffffffu >> (32 - (hi - lo))) << lo;
+}
+IRIS_DEV uint32_t sight_bits(const Sight& s, int32_t base) {
+  return bits_between(s.a0 - base, s.a1 - base) | bits_between(s.b0 - base, s.b1 - base);
+}
+
+// Tiles that a block's rows may see: `head` tiles from `head0` (the prefix) and `body` from `body0`.
+struct Tiles {
+  int32_t head0, head, body0, body;
+  IRIS_DEV int32_t count() const { return head + body; }
+  IRIS_DEV int32_t at(int32_t k) const { return k < head ? head0 + k : body0 + (k - head); }
+};
+IRIS_DEV Tiles tiles_seen(int32_t pos_lo, int32_t pos_hi, int32_t first, int32_t prefix, int32_t window, int32_t len) {
+  Tiles t;
+  const int32_t a0 = max(first, 0), a1 = min(prefix, len);
+  const int32_t b0 = window > 0 ? max(a0, pos_lo - window + 1) : a0, b1 = min(pos_hi + 1, len);
+  t.head0 = a0 / kTile;
+  t.head = a1 > a0 ? (a1 + kTile - 1) / kTile - t.head0 : 0;
+  t.body0 = b0 / kTile;
+  t.body = b1 > b0 ? (b1 + kTile - 1) / kTile - t.body0 : 0;
+  if (t.head > 0 && t.body > 0 && t.body0 < t.head0 + t.head) {  // tiles of both count once
+    const int32_t end = max(t.body0 + t.body, t.head0 + t.head);
+    t.body0 = t.head0 + t.head;
+    t.body = end - t.body0;
+  }
+  return t;
+}
+
+// tanh, within a few units in the last place of 1 anywhere and relatively near
+// 0: from e^-2|x| where that is well below 1, by its series (to x^9; the next
+// term is 6e-8 of the sum at 0.3) where 1 - e^-2|x| would cancel.
+IRIS_DEV float tanh_f(float x) {
+  const float a = fabsf(x);
+  const float t = ex2(-2.0f * kLog2e * a);
+  const float big = __fdividef(1.0f - t, 1.0f + t);
+  const float q = x * x;
+  const float small =
+      fmaf(a * q, fmaf(q, fmaf(q, fmaf(q, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), a);
+  return copysignf(a < 0.3f ? small : big, x);
+}
+
+// Two's power as fp32, |e| < 127.
+IRIS_DEV float pow2i(int e) { return __int_as_float((e + 127) << 23); }
+
+// ---------------------------------------------------------- query rows in fp16
+// A query row goes to the tensor cores as fp16 times a power of two that
+// brings its largest value into [2^15, 2^16): exact for fp16 and bf16 values
+// down to 2^-29 of the largest.  Within a group of 8 dims the order is 0 4 1 5
+// 2 6 3 7, as the nibbles of a word come apart (stored keys have it too, so
+// products do not change).  A row with a value that is not finite becomes NaN.
+//
+// `words`: D / 2 pairs as loaded.  Returns the factor that undoes the power.
+template <int D>
+IRIS_DEV float scale_row(uint32_t (&words)[D / 2], bool bf16) {
+  uint32_t most = 0;  // the largest magnitude's bits, of either type
+#pragma unroll
+  for (int i = 0; i < D / 2; ++i) {
+    const uint32_t w = words[i] & 0x7fff7fffu;
+    most = max(most, max(w & 0xffffu, w >> 16));
+  }
+  const bool finite = most < (bf16 ? 0x7f80u : 0x7c00u);
+  const float top = bf16 ? __uint_as_float(most << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(most)));
+  int e = 15;
+  if (finite && top > 0.0f) e = max(static_cast<int>((__float_as_uint(top) >> 23) & 255) - 127, -110);
+  const float up = pow2i(15 - e);
+#pragma unroll
+  for (int i = 0; i < D / 2; ++i) {
+    const float2 v = bf16 ? Bf16Elem::unpack(words[i]) : Fp16Elem::unpack(words[i]);
+    words[i] = finite ? Fp16Elem::pack(v.x * up, v.y * up) : 0x7fff7fffu;
+  }
+  return pow2i(e - 15);
+}
+
+// Eight dims (four pairs as loaded) in the order above.
+IRIS_DEV uint4 order8(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+  return make_uint4(prmt(w0, w2, 0x5410), prmt(w0, w2, 0x7632), prmt(w1, w3, 0x5410), prmt(w1, w3, 0x7632));
+}
+
+// Byte offset of 16-byte chunk c (of D / 8) of row r in an operand tile of 128 rows.
+IRIS_DEV uint32_t operand_at(int row, int chunk) {
+  return (chunk >> 3) * (kTile * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+
+// Page of token j, 0 (and an error) for an id outside the cache.
+IRIS_DEV int32_t page_of(const VarlenBatch& p, int b, int32_t j, int32_t len) {
+  if (j >= len) return 0;
+  const int32_t id = __ldg(p.block_table + b * p.bt_stride + j / kTokPage);
+  if (id < 0 || id >= p.num_pages) {
+    set_error(p.err, IRIS_ERR_PAGE_ID);
+    return 0;
+  }
+  return id;
+}
+
+}  // namespace iris

@@ -25,6 +25,7 @@ ERR_PAGE_ID = 0x40
 ERR_PIPELINE_TIMEOUT = 0x80
 ERR_SEQ_NEGATIVE = 0x100
 ERR_OFFSETS = 0x200
+ERR_QUERY_LEN = 0x400
 
 DECODE_OUT_FP16 = 0
 DECODE_OUT_LSE = 1
@@ -96,6 +97,12 @@ SIGNATURES = {
         [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i32,
          _c_i64, _c_i32, _c_i32, _c_i32, _c_f, _c_i32, _c_p, _c_sz, _c_p, _c_p]),
     "iris_b200_sparse_decode_workspace_bytes": (_c_sz, [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
+    "iris_b200_varlen_attention_workspace_bytes": (
+        _c_sz, [_c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32]),
+    "iris_b200_int4_paged_varlen_attention": (
+        ctypes.c_int,
+        [_c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32,
+         _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_f, _c_f, _c_i32, _c_p, _c_sz, _c_p, _c_p]),
     "iris_b200_xchg_buffer_bytes": (_c_sz, [_c_i64, _c_i32]),
     "iris_b200_xchg_alloc": (ctypes.c_int, [_c_sz, ctypes.POINTER(_c_p)]),
     "iris_b200_xchg_free": (ctypes.c_int, [_c_p]),

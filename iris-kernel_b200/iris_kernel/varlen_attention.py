@@ -1,0 +1,67 @@
+"""Attention of new tokens over the INT4 paged cache: whole prompts, chunks of
+prompts, drafts of a few tokens, single tokens (none of it has a counterpart in
+the reference).
+
+The new tokens' keys and values are in the cache already
+(:func:`iris_kernel.fused_kv.fused_mrope_int4_paged_append` or
+:func:`iris_kernel.fused_kv.fused_rope_int4_paged_append`): sequence ``b``
+counts ``seq_lens[b]`` cached tokens, of which its rows of the query are the
+last.  Row ``i`` of ``n`` is at place ``pos = seq_lens[b] - n + i``.  The kernel
+is csrc/varlen_attention.cu; argument checks, outputs and calls are in
+csrc/bindings.cpp, data-dependent errors go through the device error word (see
+``_runtime``).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _runtime
+
+
+def fused_int4_paged_varlen_attention(
+    query: torch.Tensor,
+    k_data: torch.Tensor,
+    v_data: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    cu_seqlens: torch.Tensor | None = None,
+    output: torch.Tensor | None = None,
+    *,
+    page_size: int = 16,
+    group_size: int = 32,
+    softmax_scale: float | None = None,
+    logit_cap: float = 0.0,
+    slopes: torch.Tensor | None = None,
+    window: int = 0,
+    prefix_lens: torch.Tensor | None = None,
+    first_visible: torch.Tensor | None = None,
+    return_lse: bool = False,
+):
+    """Causal attention of ``query [T, Hq, D]`` (FP16 or BF16) over the cache.
+
+    Sequence ``b`` has the rows ``cu_seqlens[b] .. cu_seqlens[b + 1]`` (int32
+    ``[B + 1]``, rising from 0); None means one row a sequence, a decode step.
+    Rows behind ``cu_seqlens[B]`` belong to none: output 0, lse -inf.
+
+    The logit of a row at place ``pos`` and cached token ``j`` is
+    ``softmax_scale * q.k``, capped to ``logit_cap * tanh(logit / logit_cap)``
+    if ``logit_cap`` is not 0, less ``slopes[head] * |pos - j|`` (fp32 ``[Hq]``)
+    if given.  A row sees token ``j`` of its sequence if ``j >=
+    first_visible[row]`` (int32 ``[T]``: its document's first token, say) and
+    either ``j < prefix_lens[b]`` (int32 ``[B]``: tokens that all rows see, also
+    earlier ones and those that the window has left behind) or ``j <= pos`` and,
+    with a ``window``, ``j > pos - window``.  A row that sees nothing has output
+    0 and lse -inf; so has a sequence of length 0 (an idle row of the batch).
+
+    Returns the output in the query's type, or ``(output, lse)`` with
+    ``return_lse``: fp32 ``[T, Hq]``, log2-sum-exp2 of the logits, as
+    :func:`fused_int4_paged_attention_mass` wants it.  ``softmax_scale`` None
+    (or 0.0) means ``D ** -0.5``.  ``query`` may be a slice of a fused
+    projection; ``output`` may be the query itself where that is dense."""
+    out = _runtime.ops().varlen_attention(query, k_data, v_data, k_scale, v_scale, block_table, seq_lens, cu_seqlens,
+                                          output, page_size, group_size, softmax_scale, logit_cap, slopes, window,
+                                          prefix_lens, first_visible, return_lse)
+    _runtime.finish(query)
+    return out
