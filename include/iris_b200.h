@@ -436,6 +436,54 @@ IRIS_API int iris_b200_int4_paged_varlen_attention(
     int64_t num_pages, int32_t page_size, int32_t max_pages_per_seq, int32_t window, float logit_cap, float softmax_scale,
     int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* error_word, void* stream);
 
+/*
+ * The attention weight that each cached token got from the query rows, added
+ * up: for the tokens j of sequence b and each KV head,
+ *   mass[page, head, slot] = (j >= first_token[b] ? 0 : decay * mass) +
+ *     sum over rows and the KV head's query heads of min(1, 2^(logit - lse))
+ * over the rows that see j, with logits and visibility as in
+ * iris_b200_int4_paged_varlen_attention (keys unrounded) and that call's lse
+ * [tokens, num_q_heads] fp32; a row whose lse is -inf gives nothing.  A token
+ * with a key scale that is not finite and a visible row: NaN.
+ *   mass [num_pages, num_kv_heads, 16] fp32; first_token [batch] int32 or NULL: 0.
+ * No two sequences may share a page.  Sums do not depend on timing.  Limits and
+ * alignments as iris_b200_int4_paged_varlen_attention.
+ */
+IRIS_API int iris_b200_int4_paged_attention_mass(
+    const void* query, int64_t query_stride, const float* lse, const void* k_data, const void* k_scale,
+    const int32_t* block_table, int64_t block_table_stride, const int32_t* seq_lens, const int32_t* cu_seqlens,
+    const float* slopes, const int32_t* prefix_lens, const int32_t* first_visible, const int32_t* first_token, float* mass,
+    int64_t tokens, int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int64_t num_pages,
+    int32_t page_size, int32_t max_pages_per_seq, int32_t window, float logit_cap, float softmax_scale, float decay,
+    int32_t dtype, int32_t* error_word, void* stream);
+
+/* Bytes of device workspace iris_b200_int4_paged_evict needs. */
+IRIS_API size_t iris_b200_evict_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t budget,
+                                                int32_t recent_tokens);
+
+/*
+ * Cuts every sequence of more than `budget` cached tokens to `budget`, each KV
+ * head by its own weights: the first sink_tokens, the last recent_tokens and
+ * the heaviest of the others stay (ties: the lowest index; NaN counts as +inf).
+ * With heavy = budget - recent_tokens, kept tokens in front of `heavy` stay
+ * where they are, the other kept ones (rising) move to the places that are free
+ * there (rising), the last recent_tokens move to places heavy .. budget in
+ * order; rows and weights move together.  No counterpart in the reference.
+ *   new_lens [batch]: min(seq_lens, budget); kept [batch, num_kv_heads, budget]
+ *   or NULL: the index that each place's token had, -1 behind the last.
+ * A sequence with a bad length or page id stays as it is.  No two sequences may
+ * share a page.  page_size 16, head_dim 64 or 128.  k_data and v_data 16-byte
+ * aligned, the scales 8-byte, mass and workspace 4-byte; the workspace's
+ * contents do not matter and belong to one call at a time.
+ */
+IRIS_API int iris_b200_int4_paged_evict(void* k_data, void* v_data, void* k_scale, void* v_scale, float* mass,
+                                        const int32_t* block_table, int64_t block_table_stride, const int32_t* seq_lens,
+                                        int32_t* new_lens, int32_t* kept, int32_t batch, int32_t num_kv_heads,
+                                        int32_t head_dim, int64_t num_pages, int32_t page_size,
+                                        int32_t max_pages_per_seq, int32_t budget, int32_t sink_tokens,
+                                        int32_t recent_tokens, void* workspace, size_t workspace_bytes,
+                                        int32_t* error_word, void* stream);
+
 /* Bytes of device workspace iris_b200_page_select needs. */
 IRIS_API size_t iris_b200_page_select_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t max_pages_per_seq);
 

@@ -26,7 +26,7 @@ INCLUDE = os.path.join(ROOT, "include")
 OUT = os.path.join(HERE, "iris_kernel", "libiris_b200.so")
 BINDINGS = os.path.join(HERE, "iris_kernel", "_ops.so")
 SOURCES = ["append.cu", "mrope_append.cu", "gather.cu", "decode.cu", "decode_noalloc.cu", "page_index.cu",
-           "sparse_decode.cu", "varlen_attention.cu", "exchange.cu"]
+           "sparse_decode.cu", "varlen_attention.cu", "attention_mass.cu", "evict.cu", "exchange.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,0 +1,375 @@
+// The attention weight that each cached token received, added up beside the
+// cache: iris_b200_int4_paged_attention_mass.
+//
+// mass[page, head, slot] of a KV head is decay * its old value (0 from
+// first_token on) plus the sum over the sequence's query rows and the KV head's
+// query heads of 2^(logit - lse).  Products are turned around against the
+// attention's: cached tokens are the rows (a thread a token), query rows the
+// columns, so a token's sum stays in one thread and no order of additions
+// depends on timing.  Stored nibbles go to the tensor cores as whole numbers,
+// one accumulator a group of 32 dims, and a token's fp32 scales join them
+// afterwards: nothing is rounded but the fp32 sums.
+//
+// A block is 128 threads that take turns at unpacking a tile of 128 tokens and
+// at its columns; several blocks an SM overlap each other.
+#include "varlen_common.cuh"
+
+namespace iris {
+namespace {
+
+constexpr int kCols = 32;       // query rows of a product
+constexpr int kResident = 128;  // query rows that stay in shared memory
+
+struct MassParams {
+  VarlenBatch s;
+  const uint16_t* query;
+  const float* lse;  // [tokens, hq]
+  const uint8_t* k_data;
+  const uint8_t* k_scale;
+  float* mass;       // [pages, hkv, 16]
+  const int32_t* first_token;  // [batch] or NULL: 0
+  int64_t q_stride;
+  float decay;
+  int32_t bf16;
+  int32_t per;       // tiles of a block
+  int32_t chunks;    // blocks of a (sequence, KV head)
+  int32_t slots;     // column tiles in shared memory
+};
+
+template <int D>
+struct MassCfg {
+  static constexpr int kKeys = kTile * D * 2;
+  static constexpr int kQuery = kCols * D * 2;
+  static constexpr int kUnit = kTile * (D / 2 + D / 16);
+  static constexpr int kMeta = kCols * 32;  // a row: factor, lse, place, slope; what it sees
+  static constexpr int kColumns = D;        // tensor memory: D / 32 groups x 32 columns
+  static int smem(int slots) { return 1024 + kKeys + slots * (kQuery + kMeta) + 2 * kUnit; }
+};
+
+struct MassShared {
+  uint64_t done;
+  uint32_t tmem;
+  int32_t all_lo[4], all_hi[4];  // tokens that every row of a column tile sees (without the prefix), a slot each
+  int32_t any_lo[4], any_hi[4];  // between them lies all that any row sees
+};
+
+IRIS_DEV float min_nan(float a, float b) {  // NaN stays NaN
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Query rows r0 .. r0 + 32 into a slot: four threads a row.
+template <int D, bool kCap, bool kBias>
+IRIS_DEV void load_columns(const MassParams& p, MassShared& sh, const Span& sp, int b, int len, int h, int r0, int rows,
+                           uint32_t q_tile, float4* row_f, int4* row_s, int slot, int tid) {
+  constexpr int kWords = D / 8;  // a thread's pairs
+  __syncthreads();  // what the slot held is read
+  if (tid == 0) {
+    sh.all_lo[slot] = 0;
+    sh.all_hi[slot] = INT32_MAX;
+    sh.any_lo[slot] = INT32_MAX;
+    sh.any_hi[slot] = 0;
+  }
+  __syncthreads();
+  const int row = tid >> 2, part = tid & 3, r = r0 + row;
+  const bool valid = r < rows;
+  const int i = valid ? r / p.s.group : 0, g = valid ? r % p.s.group : 0;
+  const int64_t token = sp.start + i;
+  const int head = h * p.s.group + g;
+  uint32_t w[kWords];
+#pragma unroll
+  for (int c = 0; c < kWords / 4; ++c) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (valid)
+      v = *reinterpret_cast<const uint4*>(p.query + token * p.q_stride + static_cast<int64_t>(head) * D + part * (D / 4) +
+                                          8 * c);
+    w[4 * c] = v.x;
+    w[4 * c + 1] = v.y;
+    w[4 * c + 2] = v.z;
+    w[4 * c + 3] = v.w;
+  }
+  const float back = scale_row_part<kWords>(w, p.bf16 != 0, [](uint32_t m) {
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  });
+#pragma unroll
+  for (int c = 0; c < kWords / 4; ++c) {
+    const uint4 v = order8(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+    const int chunk = part * (D / 32) + c;
+    sts128(q_tile + (chunk >> 3) * (kCols * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), v.x, v.y, v.z, v.w);
+  }
+  if (part == 0) {
+    Sight see = {0, 0, 0, 0};
+    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (valid) {
+      const int32_t pos = len - sp.count + i;
+      const float lse = __ldg(p.lse + token * p.s.hq + head);
+      f.x = kCap ? p.s.scale * back / p.s.cap : p.s.scale * kLog2e * back;
+      f.y = lse;
+      f.z = __int_as_float(pos);
+      f.w = kBias ? -__ldg(p.s.slopes + head) * kLog2e : 0.0f;
+      if (lse != -__int_as_float(0x7f800000))  // (a row that saw nothing gives nothing)
+        see = row_sight(pos, p.s.first_visible != nullptr ? __ldg(p.s.first_visible + token) : 0,
+                        p.s.prefix_lens != nullptr ? __ldg(p.s.prefix_lens + b) : 0, p.s.window, len);
+    }
+    row_f[row] = f;
+    row_s[row] = make_int4(see.a0, see.a1, see.b0, see.b1);
+    atomicMax(&sh.all_lo[slot], see.b0);
+    atomicMin(&sh.all_hi[slot], see.b1);
+    if (see.a1 > see.a0) {
+      atomicMin(&sh.any_lo[slot], see.a0);
+      atomicMax(&sh.any_hi[slot], see.a1);
+    }
+    if (see.b1 > see.b0) {
+      atomicMin(&sh.any_lo[slot], see.b0);
+      atomicMax(&sh.any_hi[slot], see.b1);
+    }
+  }
+  fence_proxy_async_shared();
+  __syncthreads();
+}
+
+template <int D, bool kCap, bool kBias>
+__global__ void __launch_bounds__(128) attention_mass_kernel(const MassParams p) {
+  using C = MassCfg<D>;
+  constexpr int kGroups = D / 32;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ MassShared sh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int chunk = blockIdx.x % p.chunks, h = blockIdx.x / p.chunks % p.s.hkv, b = blockIdx.x / p.chunks / p.s.hkv;
+  if (tid == 0) {
+    mbar_init(&sh.done, 1);
+    fence_barrier_init();
+  }
+  grid_dependency_wait();
+  grid_dependents_launch();
+  if (blockIdx.x == 0 && warp == 0) check_offsets(p.s, lane);
+  const Span sp = new_tokens(p.s, b);
+  const int len = cached_tokens(p.s, b, sp.count, tid == 0 && h == 0 && chunk == 0);
+  const int tiles = (len + kTile - 1) / kTile;
+  const int k0 = chunk * p.per, n = min(p.per, tiles - k0);
+  if (n <= 0) return;
+
+  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+  uint8_t* base = smem_raw + pad;
+  const uint32_t k_tile = smem_u32(base), q_tiles = k_tile + C::kKeys, ring = q_tiles + p.slots * C::kQuery;
+  float4* row_f = reinterpret_cast<float4*>(base + C::kKeys + p.slots * C::kQuery + 2 * C::kUnit);
+  int4* row_s = reinterpret_cast<int4*>(row_f + p.slots * kCols);
+
+  const int64_t row_bytes = static_cast<int64_t>(p.s.hkv) * (D / 2);
+  int32_t pages[2];  // of this thread's token in the tile that is unpacked, and in the next
+  auto load = [&](int k, int32_t& page) {
+    if (k < n) {
+      const int32_t j = (k0 + k) * kTile + tid;
+      page = page_of(p.s, b, j, len);
+      const int64_t row = static_cast<int64_t>(page) * kTokPage + j % kTokPage;
+      const uint32_t slot = ring + (k & 1) * C::kUnit;
+      const uint8_t* data = p.k_data + row * row_bytes + h * (D / 2);
+#pragma unroll
+      for (int c = 0; c < kGroups; ++c) copy_async<16>(slot + c * 2048 + tid * 16, data + c * 16, j < len);
+      copy_async<D / 16>(slot + kGroups * 2048 + tid * (D / 16), p.k_scale + (row * p.s.hkv + h) * (D / 16), j < len);
+    }
+    copies_commit();
+  };
+  load(0, pages[0]);
+  if (warp == 0) umma_alloc(&sh.tmem, C::kColumns);
+  umma_fence_before();
+  __syncthreads();
+  umma_fence_after();
+  const uint32_t tmem = sh.tmem, lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+  const int rows = sp.count * p.s.group, col_tiles = (rows + kCols - 1) / kCols;
+  const bool resident = col_tiles <= p.slots;
+  if (resident)
+    for (int q = 0; q < col_tiles; ++q)
+      load_columns<D, kCap, kBias>(p, sh, sp, b, len, h, q * kCols, rows, q_tiles + q * C::kQuery, row_f + q * kCols,
+                                   row_s + q * kCols, q, tid);
+  const int32_t fresh = p.first_token != nullptr ? __ldg(p.first_token + b) : 0;
+  const float cap2 = p.s.cap * kLog2e;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int k = 0; ok && k < n; ++k) {
+    load(k + 1, pages[1]);
+    const int32_t base_j = (k0 + k) * kTile, j = base_j + tid;
+    float* slot_mass = p.mass + (static_cast<int64_t>(pages[0]) * p.s.hkv + h) * kTokPage + j % kTokPage;
+    const float old = j < len && j < fresh ? *slot_mass : 0.0f;
+    copies_wait<1>();
+    const uint32_t raw = ring + (k & 1) * C::kUnit;
+    float sc[kGroups];
+    if constexpr (D == 128) {
+      const uint2 v = lds64(raw + kGroups * 2048 + tid * 8);
+      const float2 a = __half22float2(u32_as_h2(v.x)), c = __half22float2(u32_as_h2(v.y));
+      sc[0] = a.x; sc[1] = a.y; sc[2] = c.x; sc[3] = c.y;
+    } else {
+      const float2 a = __half22float2(u32_as_h2(lds32(raw + kGroups * 2048 + tid * 4)));
+      sc[0] = a.x; sc[1] = a.y;
+    }
+    bool odd = false;  // a scale that is not finite makes the token's logits NaN
+#pragma unroll
+    for (int c = 0; c < kGroups; ++c) odd |= !(fabsf(sc[c]) <= 65504.0f);
+    if (odd) sc[0] = __int_as_float(0x7fffffff);
+#pragma unroll
+    for (int c = 0; c < kGroups; ++c) {
+      const uint4 w4 = lds128(raw + c * 2048 + tid * 16);
+      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sts128(k_tile + operand_at(tid, 4 * c + i), int4_lo_exact(w[i]), int4_hi_exact(w[i]), int4_lo_exact(w[i] >> 8),
+               int4_hi_exact(w[i] >> 8));
+    }
+    fence_proxy_async_shared();
+    __syncthreads();
+    float sum = 0.0f;
+    for (int q = 0; q < col_tiles; ++q) {
+      const int slot = resident ? q : 0;
+      if (!resident)
+        load_columns<D, kCap, kBias>(p, sh, sp, b, len, h, q * kCols, rows, q_tiles, row_f, row_s, 0, tid);
+      if (sh.any_hi[slot] <= base_j || sh.any_lo[slot] >= base_j + kTile) continue;  // no row sees the tile
+      const int cols = min(kCols, rows - q * kCols);
+      if (tid == 0) {
+        umma_fence_after();
+        const uint32_t idesc = umma_idesc(kTile, cols <= 16 ? 16 : 32, false);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+          umma_ss(tmem + (s >> 1) * kCols,
+                  umma_desc(k_tile + (s >> 2) * (kTile * 128) + (s & 3) * 32, 16, 1024),
+                  umma_desc(q_tiles + slot * C::kQuery + (s >> 2) * (kCols * 128) + (s & 3) * 32, 16, 1024), idesc, s & 1);
+        umma_commit(smem_u32(&sh.done));
+      }
+      ok = mbar_wait_bounded(&sh.done, phase, p.s.err);
+      phase ^= 1;
+      if (!(ok = __syncthreads_and(ok))) break;
+      umma_fence_after();
+      const bool full = sh.all_lo[slot] <= base_j && base_j + kTile <= sh.all_hi[slot];
+      const float4* fs = row_f + slot * kCols;
+      const int4* ss = row_s + slot * kCols;
+#pragma unroll 1
+      for (int c0 = 0; c0 < cols; c0 += 8) {
+        uint32_t v[kGroups][8];
+#pragma unroll
+        for (int c = 0; c < kGroups; ++c) umma_ld8(lanes + c * kCols + c0, v[c]);
+        umma_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float s = 0.0f;
+#pragma unroll
+          for (int c = 0; c < kGroups; ++c) {
+            asm volatile("" : "+r"(v[c][i]));
+            s = fmaf(__uint_as_float(v[c][i]), sc[c], s);
+          }
+          const float4 f = fs[c0 + i];
+          float y = s * f.x;
+          if (kCap) y = cap2 * tanh_f(y);
+          if (kBias) y = fmaf(f.w, fabsf(static_cast<float>(__float_as_int(f.z) - j)), y);
+          const float e = ex2(min_nan(y - f.y, 0.0f));  // (a weight is at most 1)
+          if (full) {
+            sum += e;
+          } else {
+            const int4 z = ss[c0 + i];
+            sum += (j >= z.x && j < z.y) || (j >= z.z && j < z.w) ? e : 0.0f;
+          }
+        }
+      }
+      umma_fence_before();
+      __syncthreads();  // the columns are read: the next product may overwrite them
+    }
+    if (ok && j < len) *slot_mass = fmaf(old, p.decay, sum);
+    pages[0] = pages[1];
+  }
+  copies_wait<0>();
+  umma_fence_before();
+  __syncthreads();
+  umma_fence_after();
+  if (warp == 0) umma_free(tmem, C::kColumns);
+}
+
+template <int D, bool kCap, bool kBias>
+cudaError_t launch_mass(const MassParams& p, int64_t grid, cudaStream_t stream) {
+  auto fn = attention_mass_kernel<D, kCap, kBias>;
+  const int smem = MassCfg<D>::smem(p.slots);
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, MassCfg<D>::smem(4));
+  if (e != cudaSuccess) return e;
+  return launch_early(fn, dim3(static_cast<unsigned>(grid)), dim3(128), smem, stream, p);
+}
+template <int D>
+cudaError_t launch_mass(const MassParams& p, int64_t grid, cudaStream_t stream) {
+  const bool cap = p.s.cap > 0.0f, bias = p.s.slopes != nullptr;
+  if (cap && bias) return launch_mass<D, true, true>(p, grid, stream);
+  if (cap) return launch_mass<D, true, false>(p, grid, stream);
+  if (bias) return launch_mass<D, false, true>(p, grid, stream);
+  return launch_mass<D, false, false>(p, grid, stream);
+}
+
+}  // namespace
+}  // namespace iris
+
+using namespace iris;
+
+extern "C" int iris_b200_int4_paged_attention_mass(
+    const void* query, int64_t query_stride, const float* lse, const void* k_data, const void* k_scale,
+    const int32_t* block_table, int64_t block_table_stride, const int32_t* seq_lens, const int32_t* cu_seqlens,
+    const float* slopes, const int32_t* prefix_lens, const int32_t* first_visible, const int32_t* first_token, float* mass,
+    int64_t tokens, int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int64_t num_pages,
+    int32_t page_size, int32_t max_pages_per_seq, int32_t window, float logit_cap, float softmax_scale, float decay,
+    int32_t dtype, int32_t* error_word, void* stream) {
+  if (tokens < 0 || batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || window < 0 ||
+      !(logit_cap >= 0.0f) || !(softmax_scale > 0.0f) || (dtype != IRIS_DTYPE_FP16 && dtype != IRIS_DTYPE_BF16))
+    return IRIS_EINVAL;
+  if (page_size != kTokPage || (head_dim != 64 && head_dim != 128)) return IRIS_EUNSUPPORTED;
+  if (cu_seqlens == nullptr && tokens != batch) return IRIS_EINVAL;
+  if (batch == 0) return tokens == 0 ? IRIS_OK : IRIS_EINVAL;
+  if (num_pages <= 0 || max_pages_per_seq <= 0) return IRIS_EINVAL;
+  if (k_data == nullptr || k_scale == nullptr || block_table == nullptr || seq_lens == nullptr || mass == nullptr ||
+      (tokens > 0 && (query == nullptr || lse == nullptr)))
+    return IRIS_EINVAL;
+  const int32_t group = num_q_heads / num_kv_heads;
+  if (tokens * group > INT32_MAX / 2 || num_pages > INT32_MAX || max_pages_per_seq > INT32_MAX / 2 / kTokPage)
+    return IRIS_EUNSUPPORTED;
+  if (!aligned_to(query, 16) || query_stride % 8 != 0 || !aligned_to(k_data, 16) || !aligned_to(k_scale, 8) ||
+      !aligned_to(mass, 4))
+    return IRIS_EALIGN;
+  MassParams p = {};
+  p.s.block_table = block_table;
+  p.s.bt_stride = block_table_stride;
+  p.s.seq_lens = seq_lens;
+  p.s.cu = cu_seqlens;
+  p.s.prefix_lens = prefix_lens;
+  p.s.first_visible = first_visible;
+  p.s.slopes = slopes;
+  p.s.err = error_word;
+  p.s.num_pages = num_pages;
+  p.s.tokens = static_cast<int32_t>(tokens);
+  p.s.batch = batch;
+  p.s.hq = num_q_heads;
+  p.s.hkv = num_kv_heads;
+  p.s.group = group;
+  p.s.max_pages = max_pages_per_seq;
+  p.s.window = window < (1 << 30) ? window : 0;
+  p.s.scale = softmax_scale;
+  p.s.cap = logit_cap;
+  p.query = static_cast<const uint16_t*>(query);
+  p.lse = lse;
+  p.k_data = static_cast<const uint8_t*>(k_data);
+  p.k_scale = static_cast<const uint8_t*>(k_scale);
+  p.mass = mass;
+  p.first_token = first_token;
+  p.q_stride = query_stride;
+  p.decay = decay;
+  p.bf16 = dtype == IRIS_DTYPE_BF16;
+  const int64_t tiles = (static_cast<int64_t>(max_pages_per_seq) * kTokPage + kTile - 1) / kTile;
+  const int64_t units = static_cast<int64_t>(batch) * num_kv_heads;
+  int64_t per = units * tiles / (148 * 16);  // 16 blocks an SM and more, of up to eight tiles
+  per = per < 1 ? 1 : per > 8 ? 8 : per;
+  p.per = static_cast<int32_t>(per);
+  p.chunks = static_cast<int32_t>((tiles + per - 1) / per);
+  const int64_t most = cu_seqlens == nullptr ? group : static_cast<int64_t>(tokens) * group;
+  p.slots = most >= kResident ? kResident / kCols : static_cast<int32_t>((most + kCols - 1) / kCols);
+  if (p.slots < 1) p.slots = 1;
+  const int64_t grid = units * p.chunks;
+  if (grid > INT32_MAX) return IRIS_EUNSUPPORTED;
+  clear_stale_cuda_error();
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = head_dim == 128 ? launch_mass<128>(p, grid, st) : launch_mass<64>(p, grid, st);
+  if (e != cudaSuccess) return record_cuda_error(e, "attention_mass"), IRIS_ECUDA;
+  return IRIS_OK;
+}

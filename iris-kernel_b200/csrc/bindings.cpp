@@ -707,6 +707,108 @@ PyObject* varlen_attention(PyObject* const* a) {
   return pair(first_out, THPVariable_Wrap(std::move(lse)));
 }
 
+// (query, lse, k_data, k_scale, block_table, seq_lens, mass, cu_seqlens, first_token, decay, page_size, group_size,
+//  softmax_scale, logit_cap, slopes, window, prefix_lens, first_visible) -> None
+PyObject* attention_mass(PyObject* const* a) {
+  const Tensor &query = tensor(a[0], "query"), &lse = tensor(a[1], "lse"), &kd = tensor(a[2], "k_data"),
+               &ks = tensor(a[3], "k_scale"), &bt = tensor(a[4], "block_table"), &lens = tensor(a[5], "seq_lens"),
+               &mass = tensor(a[6], "mass");
+  const Tensor* first_token = optional_tensor(a[8], "first_token");
+  const c10::Device device = device_of("query", query);
+  const Cache c = cache_shape(kd);
+  const NewTokens n =
+      new_tokens(query, c, bt, lens, a[7], a[10], a[11], a[12], a[13], a[14], a[15], a[16], a[17], device);
+  check("k_data", kd, {c.num_pages, 16, c.heads, c.dim / 2}, at::kByte, device);
+  check("k_scale", ks, {c.num_pages, 16, c.heads, c.dim / 32}, at::kHalf, device);
+  check("lse", lse, {n.tokens, n.hq}, at::kFloat, device);
+  check("mass", mass, {c.num_pages, c.heads, 16}, at::kFloat, device);
+  if (first_token != nullptr) check("first_token", *first_token, {n.batch}, at::kInt, device);
+  check_apart("mass", mass, {{"query", &query}, {"lse", &lse}, {"k_data", &kd}, {"k_scale", &ks}, {"block_table", &bt},
+                             {"seq_lens", &lens}, {"cu_seqlens", n.cu}, {"first_token", first_token},
+                             {"slopes", n.slopes}, {"prefix_lens", n.prefix}, {"first_visible", n.first}});
+  const double decay = number(a[9]);
+  require(decay >= 0.0 && decay <= 1.0, PyExc_ValueError, "decay must lie in [0, 1]");
+  if (n.batch > 0) {
+    require(c.num_pages > 0, PyExc_IndexError, "block_table contains an invalid physical page id");
+    launch("iris_b200_int4_paged_attention_mass", device, [&](int32_t* word, void* stream) {
+      return iris_b200_int4_paged_attention_mass(
+          n.query.data, n.query.stride, floats(&lse), ptr(kd), ptr(ks), n.table.data, n.table.stride, ints(lens),
+          ints(n.cu), floats(n.slopes), ints(n.prefix), ints(n.first), ints(first_token), static_cast<float*>(out(mass)),
+          n.tokens, static_cast<int32_t>(n.batch), static_cast<int32_t>(n.hq), static_cast<int32_t>(c.heads),
+          static_cast<int32_t>(c.dim), c.num_pages, 16, n.table.width, n.window, n.cap, n.scale,
+          static_cast<float>(decay), n.code, word, stream);
+    });
+  }
+  Py_RETURN_NONE;
+}
+
+// (k_data, v_data, k_scale, v_scale, mass, block_table, seq_lens, new_lens, kept, budget, sink_tokens, recent_tokens,
+//  page_size, group_size, return_kept) -> new_lens or (new_lens, kept)
+PyObject* evict(PyObject* const* a) {
+  const Tensor &kd = tensor(a[0], "k_data"), &vd = tensor(a[1], "v_data"), &ks = tensor(a[2], "k_scale"),
+               &vs = tensor(a[3], "v_scale"), &mass = tensor(a[4], "mass"), &bt = tensor(a[5], "block_table"),
+               &lens = tensor(a[6], "seq_lens");
+  const Tensor *new_lens = optional_tensor(a[7], "new_lens"), *kept = optional_tensor(a[8], "kept");
+  const c10::Device device = device_of("k_data", kd);
+  require(integer(a[13]) == 32, PyExc_NotImplementedError, "eviction currently supports group_size=32");
+  require(integer(a[12]) == 16, PyExc_NotImplementedError, "eviction currently supports page_size=16");
+  const Cache c = cache_shape(kd);
+  require(c.dim == 64 || c.dim == 128, PyExc_NotImplementedError, "eviction currently supports head_dim in {64, 128}");
+  require(c.page_size == 16 && c.heads > 0 && c.heads <= INT32_MAX, PyExc_ValueError,
+          "packed cache shape does not match page_size");
+  check_cache(c, kd, vd, ks, vs, device);
+  check("mass", mass, {c.num_pages, c.heads, 16}, at::kFloat, device);
+  require(bt.dim() == 2, PyExc_ValueError, "block_table must have shape [B, max_pages_per_sequence]");
+  const int64_t batch = bt.size(0);
+  const Table table = block_table(bt, batch, device);
+  check("seq_lens", lens, {batch}, at::kInt, device);
+  const int32_t budget = integer32(a[9], "budget"), sink = integer32(a[10], "sink_tokens"),
+                recent = integer32(a[11], "recent_tokens");
+  require(budget > 0 && sink >= 0 && recent >= 0 && sink <= budget && recent <= budget - sink, PyExc_ValueError,
+          "budget must be positive and hold sink_tokens and recent_tokens");
+  const int with_kept = PyObject_IsTrue(a[14]);
+  if (with_kept < 0) throw Raised{};
+  const std::initializer_list<Named> data = {{"k_data", &kd}, {"v_data", &vd}, {"k_scale", &ks}, {"v_scale", &vs},
+                                             {"block_table", &bt}, {"seq_lens", &lens}};
+  check_apart("mass", mass, data);
+  Tensor l, k;
+  if (new_lens == nullptr) {
+    l = empty({batch}, at::kInt, device);
+  } else {
+    check("new_lens", *new_lens, {batch}, at::kInt, device);
+    check_apart("new_lens", *new_lens, data);
+    check_apart("new_lens", *new_lens, {{"mass", &mass}, {"kept", kept}});
+    l = *new_lens;
+  }
+  if (kept != nullptr) {
+    check("kept", *kept, {batch, c.heads, budget}, at::kInt, device);
+    check_apart("kept", *kept, data);
+    check_apart("kept", *kept, {{"mass", &mass}});
+    k = *kept;
+  } else if (with_kept) {
+    k = empty({batch, c.heads, budget}, at::kInt, device);
+  }
+  if (batch > 0) {
+    require(c.num_pages > 0, PyExc_IndexError, "block_table contains an invalid physical page id");
+    require(batch <= INT32_MAX, PyExc_ValueError, "too many sequences");
+    const size_t bytes = iris_b200_evict_workspace_bytes(static_cast<int32_t>(batch), static_cast<int32_t>(c.heads),
+                                                         budget, recent);
+    Tensor ws;
+    if (bytes > 0) ws = workspace(bytes, device);
+    launch("iris_b200_int4_paged_evict", device, [&](int32_t* word, void* stream) {
+      return iris_b200_int4_paged_evict(out(kd), out(vd), out(ks), out(vs), static_cast<float*>(out(mass)), table.data,
+                                        table.stride, ints(lens), static_cast<int32_t*>(out(l)),
+                                        k.defined() ? static_cast<int32_t*>(out(k)) : nullptr,
+                                        static_cast<int32_t>(batch), static_cast<int32_t>(c.heads),
+                                        static_cast<int32_t>(c.dim), c.num_pages, 16, table.width, budget, sink, recent,
+                                        ws.defined() ? out(ws) : nullptr, bytes, word, stream);
+    });
+  }
+  PyObject* first_out = given_or(a[7], l);
+  if (!k.defined()) return first_out;
+  return pair(first_out, given_or(a[8], k));
+}
+
 // ------------------------------------------------------------------- module
 template <PyObject* (*kFn)(PyObject* const*), int kArgs>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -746,6 +848,8 @@ PyMethodDef g_methods[] = {
     method<page_select, 11>("page_select"),
     method<sparse_decode, 14>("sparse_decode"),
     method<varlen_attention, 18>("varlen_attention"),
+    method<attention_mass, 18>("attention_mass"),
+    method<evict, 15>("evict"),
     {nullptr, nullptr, 0, nullptr},
 };
 

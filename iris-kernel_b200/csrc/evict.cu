@@ -1,0 +1,418 @@
+// The cache kept to a budget: iris_b200_int4_paged_evict.
+//
+// A (sequence, KV head) with more than `budget` tokens keeps its first
+// `sink`, its last `recent` and, of those between, the heaviest (ties to the
+// lowest index; NaN counts as +inf).  Order matters to nothing in attention but
+// recency, so few rows move: kept tokens in front of heavy = budget - recent
+// stay, the kept ones behind fill the holes there, both in rising order, and
+// the last `recent` follow in order.
+//
+// One thread-block cluster a (sequence, KV head), each block a run of its
+// tokens: weights are read once into shared memory as keys whose order is that
+// of unsigned numbers; three histograms over the cluster (11, 11 and 10 bits)
+// find the lightest key that stays; ranks by block scans and the cluster's
+// counts; rows are copied by the whole cluster between its barriers.
+#include <cooperative_groups.h>
+
+#include "varlen_common.cuh"
+
+namespace iris {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kEvictThreads = 512;
+constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kMostKeys = 40960;  // keys of a block that stay in shared memory
+
+struct EvictParams {
+  uint8_t *k_data, *v_data, *k_scale, *v_scale;
+  float* mass;
+  const int32_t* block_table;
+  int64_t bt_stride;
+  const int32_t* seq_lens;
+  int32_t* new_lens;
+  int32_t* kept;     // [batch, hkv, budget] or NULL
+  int32_t* late;     // workspace [batch * hkv][2][budget - recent]: tokens that move, places they move to
+  int32_t* err;
+  int64_t num_pages;
+  int32_t batch, hkv, max_pages, budget, sink, recent;
+  int32_t keys;      // keys of a block in shared memory
+};
+
+// The order of weights as that of unsigned numbers; -0 is 0, NaN is +inf.
+IRIS_DEV uint32_t weight_key(float w) {
+  if (w != w) w = __int_as_float(0x7f800000);
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+struct EvictShared {
+  uint32_t bins[3][kBins];
+  int32_t warp_sums[kEvictWarps];
+  int32_t equal, moving, holes;  // of this block's run
+  int32_t bad;                   // a page id outside the cache
+  uint32_t pick[2];              // this round's bin, and how many keys above it stay in question
+};
+
+// Exclusive sum over the block and its total.
+IRIS_DEV int block_scan(int v, int32_t* sums, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // sums of the call before are read
+  if (lane == 31) sums[warp] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kEvictWarps; ++i) {
+    const int s = sums[i];
+    before += i < warp ? s : 0;
+    all += s;
+  }
+  *total = all;
+  return before + x - v;
+}
+
+template <int D>
+struct EvictRow {
+  static constexpr int kVectors = D / 32;  // 16-byte vectors of packed keys (or values)
+  static constexpr int kLanes = 2 * kVectors;  // threads that carry a row
+};
+
+// This thread's part of a row: a vector of the packed data, a scale pair or the weight.
+struct Part {
+  uint4 data;
+  uint2 scale;
+  float mass;
+};
+template <int D>
+IRIS_DEV Part read_part(const EvictParams& p, int64_t row, int h, int sub) {
+  constexpr int kV = EvictRow<D>::kVectors;
+  const int64_t r = row * p.hkv + h;
+  const bool value = sub >= kV;
+  Part x;
+  x.data = *reinterpret_cast<const uint4*>((value ? p.v_data : p.k_data) + r * (D / 2) + (sub % kV) * 16);
+  x.scale = make_uint2(0, 0);
+  if (sub % kV == 0) {
+    const uint8_t* s = (value ? p.v_scale : p.k_scale) + r * (D / 16);
+    if constexpr (D == 128)
+      x.scale = *reinterpret_cast<const uint2*>(s);
+    else
+      x.scale.x = *reinterpret_cast<const uint32_t*>(s);
+  }
+  x.mass = sub == 1 ? p.mass[(row / kTokPage * p.hkv + h) * kTokPage + row % kTokPage] : 0.0f;
+  return x;
+}
+template <int D>
+IRIS_DEV void write_part(const EvictParams& p, int64_t row, int h, int sub, const Part& x) {
+  constexpr int kV = EvictRow<D>::kVectors;
+  const int64_t r = row * p.hkv + h;
+  const bool value = sub >= kV;
+  *reinterpret_cast<uint4*>((value ? p.v_data : p.k_data) + r * (D / 2) + (sub % kV) * 16) = x.data;
+  if (sub % kV == 0) {
+    uint8_t* s = (value ? p.v_scale : p.k_scale) + r * (D / 16);
+    if constexpr (D == 128)
+      *reinterpret_cast<uint2*>(s) = x.scale;
+    else
+      *reinterpret_cast<uint32_t*>(s) = x.scale.x;
+  }
+  if (sub == 1) p.mass[(row / kTokPage * p.hkv + h) * kTokPage + row % kTokPage] = x.mass;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kEvictThreads, 1) evict_kernel(const EvictParams p) {
+  extern __shared__ uint32_t keys[];
+  __shared__ EvictShared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank()), size = static_cast<int>(cluster.num_blocks());
+  const int pair = blockIdx.x / size, b = pair / p.hkv, h = pair % p.hkv;
+  const int tid = threadIdx.x;
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const int32_t raw = __ldg(p.seq_lens + b);
+  const bool wrong = raw < 0 || (static_cast<int64_t>(raw) + kTokPage - 1) / kTokPage > p.max_pages;
+  if (tid == 0 && rank == 0 && h == 0) {
+    if (raw < 0) set_error(p.err, IRIS_ERR_SEQ_NEGATIVE);
+    else if (wrong) set_error(p.err, IRIS_ERR_BLOCK_TABLE);
+  }
+  const int len = wrong ? 0 : raw, budget = p.budget;
+  int32_t* kept = p.kept != nullptr ? p.kept + static_cast<int64_t>(pair) * budget : nullptr;
+  const int32_t* table = p.block_table + b * p.bt_stride;
+  auto row_of = [&](int j) { return static_cast<int64_t>(__ldg(table + j / kTokPage)) * kTokPage + j % kTokPage; };
+
+  // a block's run of tokens: whole pages
+  const int pages = (len + kTokPage - 1) / kTokPage;
+  const int j0 = static_cast<int>(static_cast<int64_t>(pages) * rank / size) * kTokPage;
+  const int j1 = min(len, static_cast<int>(static_cast<int64_t>(pages) * (rank + 1) / size) * kTokPage);
+  if (tid == 0) sh.bad = 0;
+  __syncthreads();
+  for (int c = j0 / kTokPage + tid; c * kTokPage < j1; c += kEvictThreads) {
+    const int32_t id = __ldg(table + c);
+    if (id < 0 || id >= p.num_pages) {
+      set_error(p.err, IRIS_ERR_PAGE_ID);
+      sh.bad = 1;
+    }
+  }
+  for (int i = tid; i < 3 * kBins; i += kEvictThreads) (&sh.bins[0][0])[i] = 0;
+  cluster.sync();
+  bool stay = len <= budget;  // nothing to do, or nothing that may be touched
+  bool bad = false;
+  for (int r = 0; r < size; ++r) bad |= *cluster.map_shared_rank(&sh.bad, r) != 0;
+  if (stay || bad) {
+    if (kept != nullptr)
+      for (int i = rank * kEvictThreads + tid; i < budget; i += size * kEvictThreads) kept[i] = i < len ? i : -1;
+    if (tid == 0 && rank == 0 && h == 0) p.new_lens[b] = wrong || bad ? raw : min(len, budget);
+    cluster.sync();
+    return;
+  }
+  if (tid == 0 && rank == 0 && h == 0) p.new_lens[b] = budget;
+
+  const int sink = p.sink, recent = p.recent, heavy = budget - recent, last = len - recent;
+  const int want = heavy - sink;  // tokens of [sink, last) that stay
+  const bool cached = j1 - j0 <= p.keys;
+  auto key_at = [&](int j) {
+    return cached ? keys[j - j0]
+                  : weight_key(p.mass[(static_cast<int64_t>(__ldg(table + j / kTokPage)) * p.hkv + h) * kTokPage + j % kTokPage]);
+  };
+  const int c0 = max(j0, sink), c1 = min(j1, last);  // this block's tokens in question
+  // the lightest key that stays: `low`, of which the first `ties` in the cluster's order stay
+  uint32_t low = 0;
+  int ties = 0;
+  if (want > 0) {
+    int left = want;  // keys at or above the prefix found so far that still have to be picked
+#pragma unroll 1
+    for (int round = 0; round < 3; ++round) {
+      const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, width = round == 2 ? 10 : 11;
+      uint32_t* bins = sh.bins[round];
+      for (int j = c0 + tid; j < c1; j += kEvictThreads) {
+        uint32_t key;
+        if (round == 0) {
+          key = weight_key(
+              p.mass[(static_cast<int64_t>(__ldg(table + j / kTokPage)) * p.hkv + h) * kTokPage + j % kTokPage]);
+          if (cached) keys[j - j0] = key;
+        } else {
+          key = key_at(j);
+          if ((key >> (shift + width)) != (low >> (shift + width))) continue;
+        }
+        atomicAdd(&bins[(key >> shift) & ((1u << width) - 1)], 1u);
+      }
+      cluster.sync();
+      // from the top bin down: four bins a thread, summed over the cluster
+      constexpr int kEach = kBins / kEvictThreads;
+      int n[kEach], mine = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int bin = kBins - 1 - (tid * kEach + i);
+        n[i] = 0;
+        for (int r = 0; r < size; ++r) n[i] += static_cast<int>(cluster.map_shared_rank(bins, r)[bin]);
+        mine += n[i];
+      }
+      int total, above = block_scan(mine, sh.warp_sums, &total);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (above < left && left <= above + n[i]) {
+          sh.pick[0] = kBins - 1 - (tid * kEach + i);
+          sh.pick[1] = left - above;
+        }
+        above += n[i];
+      }
+      __syncthreads();
+      low |= sh.pick[0] << shift;
+      left = static_cast<int>(sh.pick[1]);
+      __syncthreads();
+    }
+    ties = left;
+  }
+  // how many of a block's tokens have that key: ties go to the lowest index
+  int count = 0, total;
+  for (int j = c0 + tid; want > 0 && j < c1; j += kEvictThreads) count += key_at(j) == low;
+  block_scan(count, sh.warp_sums, &total);
+  if (tid == 0) sh.equal = total;
+  cluster.sync();
+  int equal_before = 0;
+  for (int r = 0; r < rank; ++r) equal_before += *cluster.map_shared_rank(&sh.equal, r);
+  // ranks: a thread takes `each` tokens in a row, in whole sweeps of the block
+  constexpr int kEach = 8;
+  auto chosen = [&](uint32_t key, int equal_rank) { return want > 0 && (key > low || (key == low && equal_rank < ties)); };
+  int32_t* moving = p.late + static_cast<int64_t>(pair) * 2 * heavy;
+  int32_t* holes = moving + heavy;
+  // twice over the run: the counts first, then the lists at the places the counts of the blocks before give
+  int move_at = 0, hole_at = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    int equal_at = equal_before, moves = 0, gaps = 0;
+    for (int s = c0; s < c1; s += kEvictThreads * kEach) {
+      const int a = s + tid * kEach, e = min(a + kEach, c1);
+      uint32_t key[kEach];
+      int equals = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        key[i] = a + i < e && want > 0 ? key_at(a + i) : 0u;
+        equals += a + i < e && key[i] == low && want > 0;
+      }
+      int all_equal, all_moves, all_gaps;
+      int eq = equal_at + block_scan(equals, sh.warp_sums, &all_equal);
+      equal_at += all_equal;
+      int mv = 0, gp = 0;
+      uint32_t in = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (a + i >= e) continue;
+        const bool yes = chosen(key[i], eq);
+        eq += key[i] == low && want > 0;
+        in |= static_cast<uint32_t>(yes) << i;
+        mv += yes && a + i >= heavy;
+        gp += !yes && a + i < heavy;
+      }
+      int m = moves + block_scan(mv, sh.warp_sums, &all_moves), g = gaps + block_scan(gp, sh.warp_sums, &all_gaps);
+      moves += all_moves;
+      gaps += all_gaps;
+      if (pass == 1) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          if (a + i >= e) continue;
+          const bool yes = (in >> i) & 1u;
+          if (yes && a + i >= heavy) moving[move_at + m++] = a + i;
+          if (!yes && a + i < heavy) holes[hole_at + g++] = a + i;
+          if (yes && a + i < heavy && kept != nullptr) kept[a + i] = a + i;
+        }
+      }
+    }
+    if (pass == 0) {
+      if (tid == 0) {
+        sh.moving = moves;
+        sh.holes = gaps;
+      }
+      cluster.sync();
+      for (int r = 0; r < rank; ++r) {
+        move_at += *cluster.map_shared_rank(&sh.moving, r);
+        hole_at += *cluster.map_shared_rank(&sh.holes, r);
+      }
+    }
+  }
+  int n = 0;
+  for (int r = 0; r < size; ++r) n += *cluster.map_shared_rank(&sh.moving, r);
+  if (kept != nullptr) {
+    for (int i = rank * kEvictThreads + tid; i < sink; i += size * kEvictThreads) kept[i] = i;
+    for (int i = rank * kEvictThreads + tid; i < recent; i += size * kEvictThreads) kept[heavy + i] = last + i;
+  }
+  __threadfence();
+  cluster.sync();
+
+  // kept tokens from behind into the holes: sources and targets do not meet
+  constexpr int kLanes = EvictRow<D>::kLanes, kRows = kEvictThreads / kLanes;
+  const int sub = tid % kLanes, unit = rank * kRows + tid / kLanes;
+  for (int i = unit; i < n; i += size * kRows) {
+    const int src = __ldcg(moving + i), dst = __ldcg(holes + i);
+    write_part<D>(p, row_of(dst), h, sub, read_part<D>(p, row_of(src), h, sub));
+    if (sub == 0 && kept != nullptr) kept[dst] = src;
+  }
+  // then the recent ones, in steps: all of a step's rows are read before any is written, and a step's targets lie at
+  // or before its own sources, so no later step reads what it wrote
+  constexpr int kDeep = 4;
+#pragma unroll 1
+  for (int i0 = 0; i0 < recent; i0 += size * kRows * kDeep) {
+    cluster.sync();  // what this step overwrites has been read
+    Part x[kDeep];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      const int i = i0 + d * size * kRows + unit;
+      if (i < recent) x[d] = read_part<D>(p, row_of(last + i), h, sub);
+    }
+    __threadfence();
+    cluster.sync();
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      const int i = i0 + d * size * kRows + unit;
+      if (i < recent) write_part<D>(p, row_of(heavy + i), h, sub, x[d]);
+    }
+  }
+  cluster.sync();  // (no block leaves while another reads its shared memory)
+}
+
+// Blocks of a cluster: enough for two an SM, each with 1024 tokens or more.
+int cluster_of(int64_t pairs, int64_t most_tokens) {
+  int size = 1;
+  while (size < 8 && pairs * size * 2 <= 296 && most_tokens / (size * 2) >= 1024) size *= 2;
+  return size;
+}
+
+template <int D>
+cudaError_t launch_evict(EvictParams p, cudaStream_t stream) {
+  const int64_t pairs = static_cast<int64_t>(p.batch) * p.hkv, tokens = static_cast<int64_t>(p.max_pages) * kTokPage;
+  const int size = cluster_of(pairs, tokens);
+  const int64_t run = ((p.max_pages + size - 1) / size) * static_cast<int64_t>(kTokPage);
+  p.keys = static_cast<int32_t>(run < kMostKeys ? run : kMostKeys);
+  const size_t smem = static_cast<size_t>(p.keys) * 4;
+  const cudaError_t e = cudaFuncSetAttribute(evict_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostKeys * 4);
+  if (e != cudaSuccess) return e;
+  return launch_early_clusters(evict_kernel<D>, dim3(static_cast<unsigned>(pairs * size)), dim3(kEvictThreads),
+                               static_cast<unsigned>(size), smem, stream, p);
+}
+
+}  // namespace
+}  // namespace iris
+
+using namespace iris;
+
+extern "C" size_t iris_b200_evict_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t budget, int32_t recent_tokens) {
+  if (batch <= 0 || num_kv_heads <= 0 || budget <= recent_tokens) return 0;
+  return static_cast<size_t>(batch) * num_kv_heads * 2 * (budget - recent_tokens) * 4;
+}
+
+extern "C" int iris_b200_int4_paged_evict(void* k_data, void* v_data, void* k_scale, void* v_scale, float* mass,
+                                          const int32_t* block_table, int64_t block_table_stride, const int32_t* seq_lens,
+                                          int32_t* new_lens, int32_t* kept, int32_t batch, int32_t num_kv_heads,
+                                          int32_t head_dim, int64_t num_pages, int32_t page_size, int32_t max_pages_per_seq,
+                                          int32_t budget, int32_t sink_tokens, int32_t recent_tokens, void* workspace,
+                                          size_t workspace_bytes, int32_t* error_word, void* stream) {
+  if (batch < 0 || num_kv_heads <= 0 || budget <= 0 || sink_tokens < 0 || recent_tokens < 0 || sink_tokens > budget ||
+      recent_tokens > budget - sink_tokens)
+    return IRIS_EINVAL;
+  if (page_size != kTokPage || (head_dim != 64 && head_dim != 128)) return IRIS_EUNSUPPORTED;
+  if (batch == 0) return IRIS_OK;
+  if (num_pages <= 0 || max_pages_per_seq <= 0) return IRIS_EINVAL;
+  if (k_data == nullptr || v_data == nullptr || k_scale == nullptr || v_scale == nullptr || mass == nullptr ||
+      block_table == nullptr || seq_lens == nullptr || new_lens == nullptr)
+    return IRIS_EINVAL;
+  if (num_pages > INT32_MAX || max_pages_per_seq > INT32_MAX / 2 / kTokPage ||
+      static_cast<int64_t>(batch) * num_kv_heads > INT32_MAX / 8)
+    return IRIS_EUNSUPPORTED;
+  if (!aligned_to(k_data, 16) || !aligned_to(v_data, 16) || !aligned_to(k_scale, 8) || !aligned_to(v_scale, 8) ||
+      !aligned_to(mass, 4))
+    return IRIS_EALIGN;
+  const size_t need = iris_b200_evict_workspace_bytes(batch, num_kv_heads, budget, recent_tokens);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return IRIS_EWORKSPACE;
+  if (!aligned_to(workspace, 4)) return IRIS_EALIGN;
+  EvictParams p = {};
+  p.k_data = static_cast<uint8_t*>(k_data);
+  p.v_data = static_cast<uint8_t*>(v_data);
+  p.k_scale = static_cast<uint8_t*>(k_scale);
+  p.v_scale = static_cast<uint8_t*>(v_scale);
+  p.mass = mass;
+  p.block_table = block_table;
+  p.bt_stride = block_table_stride;
+  p.seq_lens = seq_lens;
+  p.new_lens = new_lens;
+  p.kept = kept;
+  p.late = static_cast<int32_t*>(workspace);
+  p.err = error_word;
+  p.num_pages = num_pages;
+  p.batch = batch;
+  p.hkv = num_kv_heads;
+  p.max_pages = max_pages_per_seq;
+  p.budget = budget;
+  p.sink = sink_tokens;
+  p.recent = recent_tokens;
+  clear_stale_cuda_error();
+  const cudaError_t e = head_dim == 128 ? launch_evict<128>(p, static_cast<cudaStream_t>(stream))
+                                        : launch_evict<64>(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return record_cuda_error(e, "evict"), IRIS_ECUDA;
+  return IRIS_OK;
+}

@@ -255,7 +255,7 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
         w[4 * c + 2] = v.z;
         w[4 * c + 3] = v.w;
       }
-      back = scale_row<D>(w, p.bf16 != 0);
+      back = scale_row(w, p.bf16 != 0);
       const uint32_t dst = q_tiles + tile * C::kOperand;
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) {

@@ -196,26 +196,32 @@ IRIS_DEV float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 // 2 6 3 7, as the nibbles of a word come apart (stored keys have it too, so
 // products do not change).  A row with a value that is not finite becomes NaN.
 //
-// `words`: D / 2 pairs as loaded.  Returns the factor that undoes the power.
-template <int D>
-IRIS_DEV float scale_row(uint32_t (&words)[D / 2], bool bf16) {
-  uint32_t most = 0;  // the largest magnitude's bits, of either type
+// `words`: a thread's pairs as loaded; `widest` takes the largest magnitude's
+// bits over the threads that share the row.  Returns the factor that undoes the power.
+template <int kWords, typename F>
+IRIS_DEV float scale_row_part(uint32_t (&words)[kWords], bool bf16, F&& widest) {
+  uint32_t most = 0;  // of either type
 #pragma unroll
-  for (int i = 0; i < D / 2; ++i) {
+  for (int i = 0; i < kWords; ++i) {
     const uint32_t w = words[i] & 0x7fff7fffu;
     most = max(most, max(w & 0xffffu, w >> 16));
   }
+  most = widest(most);
   const bool finite = most < (bf16 ? 0x7f80u : 0x7c00u);
   const float top = bf16 ? __uint_as_float(most << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(most)));
   int e = 15;
   if (finite && top > 0.0f) e = max(static_cast<int>((__float_as_uint(top) >> 23) & 255) - 127, -110);
   const float up = pow2i(15 - e);
 #pragma unroll
-  for (int i = 0; i < D / 2; ++i) {
+  for (int i = 0; i < kWords; ++i) {
     const float2 v = bf16 ? Bf16Elem::unpack(words[i]) : Fp16Elem::unpack(words[i]);
     words[i] = finite ? Fp16Elem::pack(v.x * up, v.y * up) : 0x7fff7fffu;
   }
   return pow2i(e - 15);
+}
+template <int kWords>
+IRIS_DEV float scale_row(uint32_t (&words)[kWords], bool bf16) {
+  return scale_row_part(words, bf16, [](uint32_t m) { return m; });
 }
 
 // Eight dims (four pairs as loaded) in the order above.

@@ -381,3 +381,46 @@ def fused_int4_paged_gather(
                                 first_token, bf16, page_size, group_size)
     _runtime.finish(k_data)
     return out
+
+
+def fused_int4_paged_evict(
+    k_data: torch.Tensor,
+    v_data: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    mass: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    new_lens: torch.Tensor | None = None,
+    kept: torch.Tensor | None = None,
+    *,
+    budget: int,
+    sink_tokens: int = 4,
+    recent_tokens: int = 64,
+    page_size: int = 16,
+    group_size: int = 32,
+    return_kept: bool = False,
+):
+    """Cuts every sequence of more than ``budget`` cached tokens to ``budget``,
+    in place, each KV head by its own weights ``mass [pages, Hkv, 16]`` (fp32,
+    :func:`iris_kernel.varlen_attention.fused_int4_paged_attention_mass`).
+
+    The first ``sink_tokens``, the last ``recent_tokens`` and the heaviest of the
+    others stay (ties: the lowest index; NaN counts as +inf).  Kept tokens in
+    front of ``budget - recent_tokens`` stay where they are, the other kept ones
+    fill the places that are free there, and the recent ones follow in order, so
+    the first and the last tokens are still that and the others have no order:
+    attention does not ask for one, but a window, a prefix or a bias by distance
+    then goes by places, not by the positions that tokens once had (keys carry
+    their rotation).  Rows and weights move together; bounds of pages
+    (``fused_int4_page_bounds``) have to be computed anew.
+
+    Returns the new lengths (``new_lens``, int32 ``[B]``), ``min(seq_lens,
+    budget)``; with ``return_kept`` (or ``kept`` given) also ``kept [B, Hkv,
+    budget]`` int32: the index that each place's token had, -1 behind the last.
+    A page must belong to one sequence only.  A sequence with a bad length or
+    page id stays as it is."""
+    out = _runtime.ops().evict(k_data, v_data, k_scale, v_scale, mass, block_table, seq_lens, new_lens, kept, budget,
+                               sink_tokens, recent_tokens, page_size, group_size, return_kept)
+    _runtime.finish(k_data)
+    return out

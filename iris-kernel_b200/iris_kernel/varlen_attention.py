@@ -65,3 +65,46 @@ def fused_int4_paged_varlen_attention(
                                           prefix_lens, first_visible, return_lse)
     _runtime.finish(query)
     return out
+
+
+def fused_int4_paged_attention_mass(
+    query: torch.Tensor,
+    lse: torch.Tensor,
+    k_data: torch.Tensor,
+    k_scale: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    mass: torch.Tensor,
+    cu_seqlens: torch.Tensor | None = None,
+    *,
+    first_token: torch.Tensor | None = None,
+    decay: float = 1.0,
+    page_size: int = 16,
+    group_size: int = 32,
+    softmax_scale: float | None = None,
+    logit_cap: float = 0.0,
+    slopes: torch.Tensor | None = None,
+    window: int = 0,
+    prefix_lens: torch.Tensor | None = None,
+    first_visible: torch.Tensor | None = None,
+) -> None:
+    """Adds to ``mass [pages, Hkv, 16]`` (fp32, in place) the attention weight
+    that each cached token got from the query rows, summed over a KV head's
+    query heads: what :func:`iris_kernel.fused_kv.fused_int4_paged_evict` goes
+    by.
+
+    ``query`` may hold all rows of an attention call or, with offsets to match,
+    the last ones of every sequence (a prompt's last 32 tokens, say); ``lse
+    [T, Hq]`` is what :func:`fused_int4_paged_varlen_attention` returned for
+    them, and the other arguments are that call's.  Old weights are first
+    multiplied by ``decay`` (0 to 1); tokens from ``first_token[b]`` on (int32
+    ``[B]``; None: all) start from 0, as they must where their slots held other
+    tokens before: None after a prompt, ``seq_lens - 1`` after a decode step.
+
+    A weight is at most 1; a row whose lse is -inf gives nothing.  A page must
+    belong to one sequence only.  Keys are exact here and rounded to FP16 in the
+    attention, whose weights are those to about 1e-3."""
+    _runtime.ops().attention_mass(query, lse, k_data, k_scale, block_table, seq_lens, mass, cu_seqlens, first_token, decay,
+                                  page_size, group_size, softmax_scale, logit_cap, slopes, window, prefix_lens,
+                                  first_visible)
+    _runtime.finish(query)

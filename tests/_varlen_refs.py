@@ -14,7 +14,9 @@ Half a step of a rounding: fp16 2^-11, bf16 2^-8 of the value (`half_step`).
 * lse: delta / ln 2, and 2^-20 of its size for fp32.
 * Weights (mass): keys are exact there; a logit is off by 2^-20 of sum |q k| *
   scale and of its own size and the lse's; each weight by e to that, sums of
-  fp32 by 2^-20 of the sum.
+  fp32 by 2^-20 of the sum.  Each of a token's weights below 2^-126 may count as
+  0 (the exponential flushes what fp32 holds with fewer bits), one a row and
+  query head of the group.
 """
 from __future__ import annotations
 
@@ -142,10 +144,10 @@ def mass_ref(query, lse, cache, bt, lens, cu, mass, first_token, decay, **kw):
             x, size, seen = _sequence(query, cache, bt, lens, cu, b, h, **kw)
             y = lse[r0:r1, h * group:(h + 1) * group].astype(np.float64).T[..., None] * math.log(2.0)
             with np.errstate(all="ignore"):
-                w = np.where(seen, np.exp(x - y), 0.0)
+                w = np.where(seen, np.exp(np.minimum(x - y, 0.0)), 0.0)  # a weight is at most 1
                 e = np.where(seen, np.expm1(2.0 ** -20 * (1 + size + np.abs(x) + np.abs(y))), 0.0)
                 out[pages, h, j % PAGE] = before + w.sum((0, 1))
-                far[pages, h, j % PAGE] = (w * e).sum((0, 1)) + 2.0 ** -20 * np.abs(out[pages, h, j % PAGE]) + 2.0 ** -126
+                far[pages, h, j % PAGE] = (w * e).sum((0, 1)) + 2.0 ** -20 * np.abs(out[pages, h, j % PAGE]) + w.shape[0] * w.shape[1] * 2.0 ** -126
     return out, far
 
 
