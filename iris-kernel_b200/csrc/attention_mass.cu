@@ -226,14 +226,16 @@ __global__ void __launch_bounds__(128) attention_mass_kernel(const MassParams p)
         load_columns<D, kCap, kBias>(p, sh, sp, b, len, h, q * kCols, rows, q_tiles, row_f, row_s, 0, tid);
       if (sh.any_hi[slot] <= base_j || sh.any_lo[slot] >= base_j + kTile) continue;  // no row sees the tile
       const int cols = min(kCols, rows - q * kCols);
-      if (tid == 0) {
+      if (warp == 0 && elect_one()) {
         umma_fence_after();
-        const uint32_t idesc = umma_idesc(kTile, cols <= 16 ? 16 : 32, false);
+        const uint32_t idesc = umma_idesc(kTile, cols <= 16 ? 16 : 32, false, false);
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-          umma_ss(tmem + (s >> 1) * kCols,
-                  umma_desc(k_tile + (s >> 2) * (kTile * 128) + (s & 3) * 32, 16, 1024),
-                  umma_desc(q_tiles + slot * C::kQuery + (s >> 2) * (kCols * 128) + (s & 3) * 32, 16, 1024), idesc, s & 1);
+        for (int x = 0; x < D / 16; ++x) {  // the groups in turn, twice: a product does not wait for the one before it
+          const int g = x % kGroups, s = 2 * g + x / kGroups;
+          umma_ss(tmem + g * kCols, umma_desc(k_tile + (s >> 2) * (kTile * 128) + (s & 3) * 32, 16, 1024),
+                  umma_desc(q_tiles + slot * C::kQuery + (s >> 2) * (kCols * 128) + (s & 3) * 32, 16, 1024), idesc,
+                  x >= kGroups);
+        }
         umma_commit(smem_u32(&sh.done));
       }
       ok = mbar_wait_bounded(&sh.done, phase, p.s.err);

@@ -12,6 +12,15 @@
 
 namespace iris {
 
+// True in one thread of a converged warp.  The compiler knows that form: what
+// only one thread runs needs no loop over the threads whose operands might
+// differ (a product or copy under `lane == 0` took 150 cycles to issue).
+IRIS_DEV bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
+}
+
 // One warp; the columns (a power of two, 32 to 512) stay allocated until umma_free.
 IRIS_DEV void umma_alloc(uint32_t* slot, uint32_t columns) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(columns)
@@ -33,8 +42,8 @@ IRIS_DEV void umma_commit(uint32_t bar) {
 }
 
 // Instruction descriptor of kind::f16 with fp16 operands and fp32 accumulators.
-__host__ __device__ constexpr uint32_t umma_idesc(int m, int n, bool b_mn_major) {
-  return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n / 8) << 17) |
+__host__ __device__ constexpr uint32_t umma_idesc(int m, int n, bool a_mn_major, bool b_mn_major) {
+  return (1u << 4) | (a_mn_major ? 1u << 15 : 0u) | (b_mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n / 8) << 17) |
          (static_cast<uint32_t>(m / 16) << 24);
 }
 
@@ -85,6 +94,15 @@ IRIS_DEV void umma_ld8(uint32_t addr, uint32_t* r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(addr));
+}
+template <int kColumns>
+IRIS_DEV void umma_ld(uint32_t addr, uint32_t* r) {
+  if constexpr (kColumns == 8)
+    umma_ld8(addr, r);
+  else
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
 }
 IRIS_DEV void umma_ld16(uint32_t addr, uint32_t* r) {
   asm volatile(

@@ -19,30 +19,12 @@
 // ones lose bits; the power goes into the logit's factor (keys) and the
 // probability's exponent (values).  Probabilities are fp16 with the row's
 // reference at 2^8.  Logits, statistics and sums are fp32.
-#include "varlen_common.cuh"
+#include "varlen_few.cuh"
 
 namespace iris {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr float kRise = 7.0f;    // log2 that a row's logits may pass its reference by
-constexpr float kHead = 8.0f;    // log2 of the reference's own probability
-#define kMinusInf (-__int_as_float(0x7f800000))
-
-struct AttendParams {
-  VarlenBatch s;
-  const uint16_t* query;
-  const uint8_t *k_data, *v_data;
-  const uint8_t *k_scale, *v_scale;
-  void* out;
-  float* out_lse;   // or NULL
-  float* part_o;    // [splits][tokens][hq][D], splits > 1
-  float* part_lse;  // [splits][tokens][hq]
-  int64_t q_stride; // elements between tokens of the query
-  int32_t splits;
-  int32_t bf16;
-};
-
 template <int D, int kTiles>
 struct Cfg {
   static constexpr int kUnpackGroups = kTiles == 1 ? 2 : 1;        // warpgroups that unpack
@@ -67,10 +49,6 @@ struct Shared {
   int32_t b, index, start, count, len, first_lo;
   int32_t live;
 };
-
-IRIS_DEV bool wait_all(uint64_t* bar, uint32_t parity, int32_t* err) {
-  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, err));
-}
 
 // ------------------------------------------------------------------ unpacking
 // kKind: 0 keys, 1 values, 2 both in turn.
@@ -175,11 +153,11 @@ IRIS_DEV void unpack_tiles(const AttendParams& p, Shared& sh, const Tiles& tiles
 // ------------------------------------------------------------------- products
 template <int D, int kTiles>
 IRIS_DEV void issue_products(const AttendParams& p, Shared& sh, int n, int active, uint32_t q_tiles, uint32_t k_tiles,
-                             uint32_t v_tiles, uint32_t tmem, int lane) {
+                             uint32_t v_tiles, uint32_t tmem) {
   using C = Cfg<D, kTiles>;
-  constexpr uint32_t kScores = umma_idesc(kTile, kTile, false), kOut = umma_idesc(kTile, D, true);
+  constexpr uint32_t kScores = umma_idesc(kTile, kTile, false, false), kOut = umma_idesc(kTile, D, false, true);
   auto scores = [&](int i, int k) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t q = q_tiles + i * C::kOperand, kk = k_tiles + (k & 1) * C::kOperand;
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
@@ -202,7 +180,7 @@ IRIS_DEV void issue_products(const AttendParams& p, Shared& sh, int n, int activ
       ok = wait_all(&sh.p_full[i], k & 1, p.s.err);
       if (!ok) break;
       umma_fence_after();
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t v = v_tiles + (k & 1) * C::kOperand;
 #pragma unroll
         for (int s = 0; s < kTile / 16; ++s)
@@ -221,7 +199,7 @@ IRIS_DEV void issue_products(const AttendParams& p, Shared& sh, int n, int activ
     }
   }
   // everything issued is done before the block lets go of its memory
-  if (lane == 0) umma_commit(smem_u32(&sh.drain));
+  if (elect_one()) umma_commit(smem_u32(&sh.drain));
   __syncwarp();
   wait_all(&sh.drain, 0, p.s.err);
 }
@@ -333,7 +311,7 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
       // raise the row's reference where its logits pass it by too much, and the values' power where one is larger
       const bool rise = top > m + kRise;  // (also from -inf)
       if (__any_sync(0xffffffffu, rise) || top_e > ref) {
-        const float to = rise ? top : m;
+        const float to = rise ? rintf(top) : m;  // (whole: what is taken off and added below is then exact)
         if (k > 0) {
           const float by = (rise ? ex2(m - to) : 1.0f) * pow2i(max(ref - top_e, -126));
           if (!(ok = wait_all(&sh.o_full[tile], (k - 1) & 1, p.s.err))) break;
@@ -356,19 +334,20 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
         ref = top_e;
       }
       const float zero = m == kMinusInf ? 0.0f : -m;  // (a row that sees nothing yet)
-      // a product that is not rounded as the reference was may pass it by half a step, which is 2^7 from 2^31 on:
-      // so far out products are rounded first
-      if (!kMod && __any_sync(0xffffffffu, fabsf(m) > 16777216.0f && m != kMinusInf)) {
+      // From 2^24 on a product that is not rounded may pass the reference by more than fp16 holds, and the addend has no
+      // room for the power beside it: there the reference comes off first, from rounded products.
+      const bool far = __any_sync(0xffffffffu, fabsf(zero) > 8388608.0f);
+      if (far) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
 #pragma unroll
-          for (int j = 32 * c; j < 32 * c + 32; ++j) s[j] *= f[c];
+          for (int j = 32 * c; j < 32 * c + 32; ++j) s[j] = (kMod ? s[j] : __fmul_rn(s[j], f[c])) + zero;
           f[c] = 1.0f;
         }
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const float add = zero + (kHead + static_cast<float>(ve[c] - ref));
+        const float add = (far ? 0.0f : zero) + (kHead + static_cast<float>(ve[c] - ref));
         float2 sum = make_float2(0.0f, 0.0f);
         uint32_t w[16];
 #pragma unroll
@@ -473,21 +452,14 @@ __global__ void __launch_bounds__(kThreads, 1) varlen_attention_kernel(const Att
   if (warp == 0) {
     if (blockIdx.x == 0) check_offsets(p.s, lane);
     Block blk = {0, 0};
-    const bool live = find_block(p.s, unit, kTile * kTiles, lane, &blk);
+    const bool live = find_block(p.s, unit, kTile * kTiles, p.few ? kFewRows : 0, INT64_MAX, lane, &blk);
     int first = 0;
     Span sp = {0, 0};
     int32_t len = 0;
     if (live) {
       sp = new_tokens(p.s, blk.b);
       len = cached_tokens(p.s, blk.b, sp.count, lane == 0 && h == 0 && split == 0 && blk.index == 0);
-      if (p.s.first_visible != nullptr) {
-        const int64_t r0 = static_cast<int64_t>(blk.index) * (kTile * kTiles);
-        const int i0 = static_cast<int>(r0 / p.s.group);
-        const int i1 = static_cast<int>(min((r0 + kTile * kTiles - 1) / p.s.group, static_cast<int64_t>(sp.count - 1)));
-        first = INT32_MAX;
-        for (int i = i0 + lane; i <= i1; i += 32) first = min(first, __ldg(p.s.first_visible + sp.start + i));
-        first = __reduce_min_sync(0xffffffffu, first);
-      }
+      first = first_of_block(p.s, sp, blk.index, kTile * kTiles, lane);
     }
     if (lane == 0) {
       sh.live = live;
@@ -499,12 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) varlen_attention_kernel(const Att
       sh.first_lo = first;
     }
   }
-  // rows that the offsets leave over: zeros
-  for (int64_t row = static_cast<int64_t>(used_rows(p.s)) * p.s.hq + blockIdx.x; row < static_cast<int64_t>(p.s.tokens) * p.s.hq;
-       row += gridDim.x) {
-    if (threadIdx.x < D / 2) reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + row * D)[threadIdx.x] = 0u;
-    if (threadIdx.x == 0 && p.out_lse != nullptr) p.out_lse[row] = kMinusInf;
-  }
+  clear_unused<D>(p);
   __syncthreads();
   if (!sh.live) return;
   if (warp == C::kMmaWarp) umma_alloc(&sh.tmem, C::kColumns);
@@ -556,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) varlen_attention_kernel(const Att
     regs_give<80>();
     if (warp == C::kMmaWarp) {
       asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftWarps * 32 + 32) : "memory");
-      if (n > 0) issue_products<D, kTiles>(p, sh, n, active, q_tiles, k_tiles, v_tiles, tmem, lane);
+      if (n > 0) issue_products<D, kTiles>(p, sh, n, active, q_tiles, k_tiles, v_tiles, tmem);
     }
   }
   umma_fence_before();
@@ -569,55 +536,26 @@ __global__ void __launch_bounds__(kThreads, 1) varlen_attention_kernel(const Att
 template <int D>
 __global__ void __launch_bounds__(256) varlen_join_kernel(const AttendParams p) {
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = static_cast<int64_t>(used_rows(p.s)) * p.s.hq, stride = static_cast<int64_t>(p.s.tokens) * p.s.hq;
+  grid_dependents_launch();
+  const int64_t rows = static_cast<int64_t>(used_rows(p.s)) * p.s.hq;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
-  float top = kMinusInf;
-  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, __ldcg(p.part_lse + s * stride + row));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float zero = top == kMinusInf ? 0.0f : top;
-  float acc[D / 32] = {}, total = 0.0f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float part = __ldcg(p.part_lse + s * stride + row);
-    if (part == kMinusInf) continue;  // it saw nothing
-    const float w = ex2(part - zero);
-    total += w;
-    const float* o = p.part_o + (s * stride + row) * D + lane * (D / 32);
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) acc[j] = fmaf(w, __ldcg(o + j), acc[j]);
+  if (p.few) {  // the other kernel's rows are not here; the row's sequence is the last that starts at or before it
+    const int32_t token = static_cast<int32_t>(row / p.s.hq);
+    int lo = 0, hi = p.s.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(p.s.cu + mid) <= token) lo = mid; else hi = mid;
+    }
+    if (static_cast<int64_t>(new_tokens(p.s, lo).count) * p.s.group <= kFewRows) return;
   }
-  const float norm = total == 0.0f ? 0.0f : 1.0f / total;
-  uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + row * D) + lane * (D / 64);
-#pragma unroll
-  for (int j = 0; j < D / 64; ++j) {
-    const float a = acc[2 * j] * norm, b = acc[2 * j + 1] * norm;
-    dst[j] = p.bf16 ? Bf16Elem::pack(a, b) : Fp16Elem::pack(a, b);
-  }
-  if (lane == 0 && p.out_lse != nullptr) p.out_lse[row] = total == 0.0f ? kMinusInf : zero + lg2(total);
+  join_row<D>(p, p.part_o + row * D, p.part_lse + row, p.splits, static_cast<int64_t>(p.s.tokens) * p.s.hq, row,
+              threadIdx.x & 31);
 }
 
 // ----------------------------------------------------------------------- host
-// Two row tiles a block where sequences have more than 128 rows on average.
-int row_tiles(int64_t tokens, int32_t batch, int32_t group, bool offsets) {
-  return offsets && tokens * group > 128 * static_cast<int64_t>(batch) ? 2 : 1;
-}
-
-int64_t blocks_of(int64_t tokens, int32_t batch, int32_t group, bool offsets, int tiles) {
-  const int64_t rows = 128 * tiles;
-  if (!offsets) return batch * ((group + rows - 1) / rows);
-  return tokens * group / rows + (batch < tokens ? batch : tokens);  // every sequence's last block may be a short one
-}
-
-// Blocks that share a row's tiles: as many as bring a block to every SM, each with four tiles or more.
-int32_t splits_of(int64_t blocks, int32_t hkv, int32_t max_pages, int32_t window, bool prefix, int sms) {
-  int64_t tiles = (static_cast<int64_t>(max_pages) * kTokPage + kTile - 1) / kTile;
-  if (window > 0 && !prefix) tiles = tiles < window / kTile + 4 ? tiles : window / kTile + 4;
-  const int64_t want = sms / (blocks * hkv), most = tiles / 4;
-  const int64_t n = want < most ? want : most;
-  return static_cast<int32_t>(n < 1 ? 1 : n);
-}
+constexpr int kFewWaves = 2;  // blocks of few rows: so many waves
+constexpr int kFewTiles = 2;  // ... each of so many tiles or more
 
 int sm_count(int device) {
   static int known[64] = {};
@@ -628,6 +566,63 @@ int sm_count(int device) {
     known[device] = n;
   }
   return known[device];
+}
+
+// Which kernels run, and how the work is cut.
+//
+// Sequences of at most kFewRows rows go to varlen_few_kernel, the others to
+// varlen_attention_kernel.  With one new token a sequence the host knows which;
+// with offsets both are launched unless all rows together are few (an empty
+// launch costs about 2 us beside the other; one kernel for both would give single
+// tokens 128-row products, 837 us where the other takes a tenth of it at 64 x 4096).
+struct Plan {
+  bool few, many;
+  int tiles;               // row tiles of a block (many)
+  int64_t many_blocks, few_blocks;
+  int32_t splits, chunks, per;
+  int cols;                // columns of a block (few)
+  int64_t many_parts, few_parts;  // rows of parts in the workspace
+};
+Plan plan(int64_t tokens, int32_t batch, int32_t group, bool offsets, int32_t hkv, int32_t max_pages, int32_t window,
+          bool prefix, int sms) {
+  Plan r = {};
+  const int64_t rows = tokens * group;
+  r.few = offsets || group <= kFewRows;
+  r.many = offsets ? rows > kFewRows : group > kFewRows;
+  int64_t tiles = (static_cast<int64_t>(max_pages) * kTokPage + kTile - 1) / kTile;  // that a block may see
+  const int64_t all_tiles = tiles;
+  if (window > 0 && !prefix) tiles = tiles < window / kTile + 4 ? tiles : window / kTile + 4;
+  r.splits = r.chunks = 1;
+  const int64_t some = batch < tokens ? batch : tokens;
+  if (r.many) {
+    // two row tiles a block where sequences have more than 128 rows on average
+    r.tiles = offsets && rows > 128 * static_cast<int64_t>(batch) ? 2 : 1;
+    const int64_t each = 128 * r.tiles;
+    r.many_blocks = offsets ? rows / each + some : batch * ((group + each - 1) / each);
+    // blocks that share a row's tiles: as many as bring a block to every SM, each with four tiles or more
+    const int64_t want = sms / (r.many_blocks * hkv), most = tiles / 4;
+    const int64_t n = want < most ? want : most;
+    r.splits = static_cast<int32_t>(n < 1 ? 1 : n);
+  }
+  if (r.few) {
+    const int64_t most_rows = offsets ? (rows < kFewRows ? rows : kFewRows) : group;
+    r.cols = most_rows <= 4 ? 4 : most_rows <= 8 ? 8 : most_rows <= 16 ? 16 : 32;
+    r.few_blocks = offsets ? some : batch;  // (kFewRows rows are one block)
+    if (offsets && r.cols < kFewRows) r.few_blocks = some;
+    // chunks of equal size, for blocks of about kFewWaves waves over the GPU
+    const int64_t slots = static_cast<int64_t>(sms) * (r.cols <= 8 ? 3 : 2);
+    int64_t n = (slots * kFewWaves + r.few_blocks * hkv - 1) / (r.few_blocks * hkv);
+    const int64_t most = (tiles + kFewTiles - 1) / kFewTiles;
+    if (n > most) n = most;
+    if (n < 1) n = 1;
+    r.per = static_cast<int32_t>((all_tiles < tiles ? all_tiles : tiles) + n - 1) / static_cast<int32_t>(n);
+    // a window's tiles are an estimate from above; a prefix may add to it, so chunks cover all tiles there
+    const int64_t cover = window > 0 && !prefix ? tiles : all_tiles;
+    r.chunks = static_cast<int32_t>((cover + r.per - 1) / r.per);
+  }
+  r.many_parts = r.many && r.splits > 1 ? r.splits * rows * hkv : 0;
+  r.few_parts = r.few && r.chunks > 1 ? static_cast<int64_t>(r.chunks) * batch * hkv * r.cols : 0;
+  return r;
 }
 
 template <int D, int kTiles, bool kCap, bool kBias>
@@ -643,6 +638,41 @@ cudaError_t launch_attend(const AttendParams& p, int64_t grid, cudaStream_t stre
     if (device < 64) ready |= 1ull << device;
   }
   return launch_early(fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Cfg<D, kTiles>::kSmem, stream, p);
+}
+
+template <int D, int kCols, bool kCap, bool kBias>
+cudaError_t launch_few(const AttendParams& p, int64_t grid, cudaStream_t stream) {
+  auto fn = varlen_few_kernel<D, kCols, kCap, kBias>;
+  static thread_local uint64_t ready = 0;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (device >= 64 || !((ready >> device) & 1)) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, FewCfg<D, kCols>::kSmem);
+    if (e != cudaSuccess) return e;
+    if (device < 64) ready |= 1ull << device;
+  }
+  CUtensorMap k, v;
+  const int64_t pages = p.s.num_pages;
+  if (!packed_map(&k, p.k_data, D, p.s.hkv, pages) || !packed_map(&v, p.v_data, D, p.s.hkv, pages))
+    return cudaErrorInvalidValue;
+  return launch_early(fn, dim3(static_cast<unsigned>(grid)), dim3(288), FewCfg<D, kCols>::kSmem, stream, k, v, p);
+}
+template <int D, int kCols>
+cudaError_t launch_few(const AttendParams& p, int64_t grid, cudaStream_t stream) {
+  const bool cap = p.s.cap > 0.0f, bias = p.s.slopes != nullptr;
+  if (cap && bias) return launch_few<D, kCols, true, true>(p, grid, stream);
+  if (cap) return launch_few<D, kCols, true, false>(p, grid, stream);
+  if (bias) return launch_few<D, kCols, false, true>(p, grid, stream);
+  return launch_few<D, kCols, false, false>(p, grid, stream);
+}
+
+template <int D>
+cudaError_t launch_few(const AttendParams& p, int cols, int64_t grid, cudaStream_t stream) {
+  if (cols == 4) return launch_few<D, 4>(p, grid, stream);
+  if (cols == 8) return launch_few<D, 8>(p, grid, stream);
+  if (cols == 16) return launch_few<D, 16>(p, grid, stream);
+  return launch_few<D, 32>(p, grid, stream);
 }
 
 template <int D, int kTiles>
@@ -664,12 +694,9 @@ extern "C" size_t iris_b200_varlen_attention_workspace_bytes(int64_t tokens, int
                                                              int32_t max_pages_per_seq, int32_t window, int32_t has_prefix,
                                                              int32_t has_offsets, int32_t device) {
   if (tokens <= 0 || batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0) return 0;
-  const int32_t group = num_q_heads / num_kv_heads;
-  const bool offsets = has_offsets != 0;
-  const int tiles = row_tiles(tokens, batch, group, offsets);
-  const int32_t splits = splits_of(blocks_of(tokens, batch, group, offsets, tiles), num_kv_heads, max_pages_per_seq, window,
-                                   has_prefix != 0, sm_count(device));
-  return splits > 1 ? static_cast<size_t>(splits) * tokens * num_q_heads * (head_dim + 1) * 4 : 0;
+  const Plan r = plan(tokens, batch, num_q_heads / num_kv_heads, has_offsets != 0, num_kv_heads, max_pages_per_seq, window,
+                      has_prefix != 0, sm_count(device));
+  return static_cast<size_t>(r.many_parts + r.few_parts) * (head_dim + 1) * 4;
 }
 
 extern "C" int iris_b200_int4_paged_varlen_attention(
@@ -701,14 +728,14 @@ extern "C" int iris_b200_int4_paged_varlen_attention(
   clear_stale_cuda_error();
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return record_cuda_error(e, "cudaGetDevice"), IRIS_ECUDA;
-  const int tiles = row_tiles(tokens, batch, group, offsets);
-  const int64_t blocks = blocks_of(tokens, batch, group, offsets, tiles);
-  const int32_t splits = splits_of(blocks, num_kv_heads, max_pages_per_seq, window, prefix_lens != nullptr, sm_count(device));
-  const int64_t grid = blocks * num_kv_heads * splits;
-  if (grid > INT32_MAX) return IRIS_EUNSUPPORTED;
-  const size_t part = static_cast<size_t>(splits) * tokens * num_q_heads;
-  if (splits > 1 && (workspace == nullptr || workspace_bytes < part * (head_dim + 1) * 4)) return IRIS_EWORKSPACE;
-  if (splits > 1 && !aligned_to(workspace, 16)) return IRIS_EALIGN;
+  const Plan r = plan(tokens, batch, group, offsets, num_kv_heads, max_pages_per_seq, window, prefix_lens != nullptr,
+                      sm_count(device));
+  const int64_t many_grid = r.many_blocks * num_kv_heads * r.splits, few_grid = r.few_blocks * num_kv_heads * r.chunks;
+  if (many_grid > INT32_MAX || few_grid > INT32_MAX) return IRIS_EUNSUPPORTED;
+  const int64_t parts = r.many_parts + r.few_parts;
+  if (parts > 0 && (workspace == nullptr || workspace_bytes < static_cast<size_t>(parts) * (head_dim + 1) * 4))
+    return IRIS_EWORKSPACE;
+  if (parts > 0 && !aligned_to(workspace, 16)) return IRIS_EALIGN;
   AttendParams p = {};
   p.s.block_table = block_table;
   p.s.bt_stride = block_table_stride;
@@ -736,20 +763,38 @@ extern "C" int iris_b200_int4_paged_varlen_attention(
   p.out = output;
   p.out_lse = out_lse;
   p.part_o = static_cast<float*>(workspace);
-  p.part_lse = splits > 1 ? p.part_o + part * head_dim : nullptr;
+  p.few_o = p.part_o + r.many_parts * head_dim;
+  p.part_lse = p.part_o + parts * head_dim;
+  p.few_lse = p.part_lse + r.many_parts;
   p.q_stride = query_stride;
-  p.splits = splits;
+  p.splits = r.splits;
+  p.chunks = r.chunks;
+  p.per = r.per;
+  p.few = r.few;
+  p.many = r.many;
   p.bf16 = dtype == IRIS_DTYPE_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128)
-    e = tiles == 2 ? launch_attend<128, 2>(p, grid, st) : launch_attend<128, 1>(p, grid, st);
-  else
-    e = tiles == 2 ? launch_attend<64, 2>(p, grid, st) : launch_attend<64, 1>(p, grid, st);
-  if (e != cudaSuccess) return record_cuda_error(e, "varlen_attention"), IRIS_ECUDA;
-  if (splits > 1) {
-    const dim3 join(static_cast<unsigned>((tokens * num_q_heads + 7) / 8));
-    e = head_dim == 128 ? launch_early(varlen_join_kernel<128>, join, dim3(256), 0, st, p)
-                        : launch_early(varlen_join_kernel<64>, join, dim3(256), 0, st, p);
+  if (r.many) {
+    if (head_dim == 128)
+      e = r.tiles == 2 ? launch_attend<128, 2>(p, many_grid, st) : launch_attend<128, 1>(p, many_grid, st);
+    else
+      e = r.tiles == 2 ? launch_attend<64, 2>(p, many_grid, st) : launch_attend<64, 1>(p, many_grid, st);
+    if (e != cudaSuccess) return record_cuda_error(e, "varlen_attention"), IRIS_ECUDA;
+  }
+  if (r.few) {
+    e = head_dim == 128 ? launch_few<128>(p, r.cols, few_grid, st) : launch_few<64>(p, r.cols, few_grid, st);
+    if (e != cudaSuccess) return record_cuda_error(e, "varlen_few"), IRIS_ECUDA;
+  }
+  if (r.few_parts > 0) {
+    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(batch) * num_kv_heads));
+    e = head_dim == 128 ? launch_early(varlen_few_join_kernel<128>, grid, dim3(128), 0, st, p, r.cols)
+                        : launch_early(varlen_few_join_kernel<64>, grid, dim3(128), 0, st, p, r.cols);
+    if (e != cudaSuccess) return record_cuda_error(e, "varlen_few_join"), IRIS_ECUDA;
+  }
+  if (r.many_parts > 0) {
+    const dim3 grid(static_cast<unsigned>((tokens * num_q_heads + 7) / 8));
+    e = head_dim == 128 ? launch_early(varlen_join_kernel<128>, grid, dim3(256), 0, st, p)
+                        : launch_early(varlen_join_kernel<64>, grid, dim3(256), 0, st, p);
     if (e != cudaSuccess) return record_cuda_error(e, "varlen_join"), IRIS_ECUDA;
   }
   return IRIS_OK;

@@ -19,6 +19,12 @@ constexpr int kTile = 128;        // cached tokens of a tile
 constexpr int kTokPage = 16;      // tokens of a page
 constexpr float kLog2e = 1.4426950408889634f;
 
+IRIS_DEV float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct VarlenBatch {
   const int32_t* block_table;
   int64_t bt_stride;
@@ -35,6 +41,18 @@ struct VarlenBatch {
   float scale;                   // softmax scale
   float cap;                     // 0: none
 };
+
+// Waits of a whole warp: false (and an error) if the phase does not complete
+// within the limit.  The clock is only read once a first round of polls, each of
+// which the hardware may let sleep, has failed.
+IRIS_DEV bool wait_all(uint64_t* bar, uint32_t parity, int32_t* err) {
+  const uint32_t at = smem_u32(bar);
+  bool there = false;
+#pragma unroll 1
+  for (int i = 0; i < 64 && !there; ++i) there = mbar_try_wait(at, parity);
+  if (__all_sync(0xffffffffu, there)) return true;
+  return __all_sync(0xffffffffu, mbar_wait_bounded(at, parity, err));
+}
 
 // New tokens [start, start + count) of sequence b; offsets outside the query are cut off.
 struct Span {
@@ -80,13 +98,15 @@ IRIS_DEV int32_t cached_tokens(const VarlenBatch& p, int b, int32_t count, bool 
 
 IRIS_DEV int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
 
-// Block u of all sequences' blocks of `rows` rows, heaviest first: the last
-// block of every sequence, then the one before it, and so on (a block's work
-// grows with its tokens' places).  One warp; false: there is no block u.
+// Block u of the blocks of `rows` rows of all sequences with more than `over`
+// and at most `most_rows` rows, heaviest first: the last block of every
+// sequence, then the one before it, and so on (a block's work grows with its
+// tokens' places).  One warp; false: there is no block u.  (With one new token
+// a sequence the rows are the host's to choose a kernel by, and all are taken.)
 struct Block {
   int32_t b, index;
 };
-IRIS_DEV bool find_block(const VarlenBatch& p, int u, int rows, int lane, Block* out) {
+IRIS_DEV bool find_block(const VarlenBatch& p, int u, int rows, int64_t over, int64_t most_rows, int lane, Block* out) {
   if (p.cu == nullptr) {
     const int per = (p.group + rows - 1) / rows;
     out->b = u / per;
@@ -94,7 +114,8 @@ IRIS_DEV bool find_block(const VarlenBatch& p, int u, int rows, int lane, Block*
     return out->b < p.batch;
   }
   auto blocks = [&](int b) {
-    return static_cast<int32_t>((static_cast<int64_t>(new_tokens(p, b).count) * p.group + rows - 1) / rows);
+    const int64_t n = static_cast<int64_t>(new_tokens(p, b).count) * p.group;
+    return n > over && n <= most_rows ? static_cast<int32_t>((n + rows - 1) / rows) : 0;
   };
   int most = 0;
   for (int b = lane; b < p.batch; b += 32) most = max(most, blocks(b));
@@ -125,6 +146,17 @@ IRIS_DEV bool find_block(const VarlenBatch& p, int u, int rows, int lane, Block*
     left -= c;
   }
   return false;
+}
+
+// The smallest first visible token of a block's rows (one warp).
+IRIS_DEV int32_t first_of_block(const VarlenBatch& p, const Span& sp, int index, int rows, int lane) {
+  if (p.first_visible == nullptr) return 0;
+  const int64_t r0 = static_cast<int64_t>(index) * rows;
+  const int i0 = static_cast<int>(r0 / p.group);
+  const int i1 = static_cast<int>(min((r0 + rows - 1) / p.group, static_cast<int64_t>(sp.count - 1)));
+  int32_t first = INT32_MAX;
+  for (int i = i0 + lane; i <= i1; i += 32) first = min(first, __ldg(p.first_visible + sp.start + i));
+  return __reduce_min_sync(0xffffffffu, first);
 }
 
 // What one row sees, as two runs [a0, a1) and [b0, b1) of tokens (a: prefix).
@@ -174,16 +206,14 @@ IRIS_DEV Tiles tiles_seen(int32_t pos_lo, int32_t pos_hi, int32_t first, int32_t
 }
 
 // tanh, within a few units in the last place of 1 anywhere and relatively near
-// 0: from e^-2|x| where that is well below 1, by its series (to x^9; the next
-// term is 6e-8 of the sum at 0.3) where 1 - e^-2|x| would cancel.
+// 0: 1 - 2 / (1 + e^2x) (right at both infinities), or its series (to x^9; the
+// next term is 6e-8 of the sum at 0.3) where that would cancel.
 IRIS_DEV float tanh_f(float x) {
-  const float a = fabsf(x);
-  const float t = ex2(-2.0f * kLog2e * a);
-  const float big = __fdividef(1.0f - t, 1.0f + t);
+  const float t = ex2(2.0f * kLog2e * x);
+  const float big = fmaf(-2.0f, rcp(1.0f + t), 1.0f);
   const float q = x * x;
-  const float small =
-      fmaf(a * q, fmaf(q, fmaf(q, fmaf(q, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), a);
-  return copysignf(a < 0.3f ? small : big, x);
+  const float r = fmaf(q, fmaf(q, fmaf(q, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f);
+  return fabsf(x) < 0.3f ? fmaf(x * q, r, x) : big;
 }
 
 // Two's power as fp32, |e| < 127.
@@ -234,15 +264,66 @@ IRIS_DEV uint32_t operand_at(int row, int chunk) {
   return (chunk >> 3) * (kTile * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
 }
 
-// Page of token j, 0 (and an error) for an id outside the cache.
+// Page of token j as the table has it (to be checked where it is used, so that
+// nothing waits for the load before), 0 past the sequence's end.
+IRIS_DEV int32_t raw_page(const VarlenBatch& p, int b, int32_t j, int32_t len) {
+  return j < len ? __ldg(p.block_table + b * p.bt_stride + j / kTokPage) : 0;
+}
+// 0 (and an error) for an id outside the cache.
+IRIS_DEV int32_t checked_page(const VarlenBatch& p, int32_t id) {
+  if (static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_pages)) return id;  // (num_pages fits 31 bits)
+  set_error(p.err, IRIS_ERR_PAGE_ID);
+  return 0;
+}
 IRIS_DEV int32_t page_of(const VarlenBatch& p, int b, int32_t j, int32_t len) {
-  if (j >= len) return 0;
-  const int32_t id = __ldg(p.block_table + b * p.bt_stride + j / kTokPage);
-  if (id < 0 || id >= p.num_pages) {
-    set_error(p.err, IRIS_ERR_PAGE_ID);
-    return 0;
-  }
-  return id;
+  return checked_page(p, raw_page(p, b, j, len));
+}
+
+// ------------------------------------------------------- packed tiles by TMA
+// A tile's packed rows of one head land as [128 tokens][D / 2 bytes], a page
+// (16 rows) a copy, 16-byte chunk c of row r at c ^ ((r >> 1) & 3) (D = 128: the
+// 64-byte swizzle) or c ^ ((r >> 2) & 1) (D = 64: the 32-byte one), so that a
+// warp whose threads each read a row of their own meets no bank twice.  (Loads
+// straight from memory, a row a thread, kept L1 57 % busy with their 32 lines
+// each.)  Pages past the sequence's end are left out: what the rows held before
+// has finite nibbles and counts for nothing.
+template <int D>
+IRIS_DEV uint32_t packed_at(int row, int chunk) {
+  return row * (D / 2) + (D == 128 ? (chunk ^ ((row >> 1) & 3)) << 4 : (chunk ^ ((row >> 2) & 1)) << 4);
+}
+// One warp: the copies of a tile whose first token is j0; lane i < 8 has page i's
+// id and issues its copy (a loop over the lanes after all, but half as long as
+// one that hands the ids round).
+template <int D>
+IRIS_DEV void load_packed(uint8_t* dst, const CUtensorMap* map, int32_t page, int32_t j0, int32_t len, int h,
+                          uint64_t* bar, int lane) {
+  const int pages = min(kTile / kTokPage, (len - j0 + kTokPage - 1) / kTokPage);
+  if (elect_one()) mbar_arrive_expect_tx(bar, pages * kTokPage * (D / 2));
+  __syncwarp();
+  if (lane < pages) tma_load_4d(dst + lane * kTokPage * (D / 2), map, 0, 0, h, page, bar);
+  __syncwarp();
+}
+
+// Host: the cache [pages, 16, Hkv, D / 2] as (row bytes, 16 tokens, heads, pages), a box of one page of one head.
+inline bool packed_map(CUtensorMap* map, const void* base, int dim, int hkv, int64_t num_pages) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<Encode>(f) : nullptr;
+  }();
+  if (encode == nullptr) return false;
+  const cuuint64_t row = static_cast<cuuint64_t>(dim) / 2;
+  const cuuint64_t dims[4] = {row, kTokPage, static_cast<cuuint64_t>(hkv), static_cast<cuuint64_t>(num_pages)};
+  const cuuint64_t strides[3] = {row * hkv, row, row * hkv * kTokPage};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(row), kTokPage, 1u, 1u}, step[4] = {1u, 1u, 1u, 1u};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, step,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, dim == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace iris

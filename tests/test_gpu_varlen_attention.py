@@ -327,3 +327,22 @@ def test_another_stream_and_a_graph():
             assert torch.equal(g, f(*a))
     finally:
         set_validation_mode("sync")
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+def test_few_and_many_rows_together(dim, dtype):
+    """Decode steps, drafts and prompts in one batch, short and long contexts."""
+    new, lens = [1, 300, 4, 0, 8, 9, 1, 33], [9000, 300, 700, 50, 8, 2000, 1, 40]
+    Case(new, lens, 8, 2, dim, dtype, seed=31).spoil_tails().check()
+    Case(new, lens, 8, 2, dim, dtype, seed=32, window=150, prefix_lens=np.array([40, 290, 0, 9, 8, 777, 1, 0], np.int32),
+         logit_cap=30.0).spoil_tails().check()
+    Case(new, lens, 3, 1, dim, dtype, seed=33, slopes=np.array([0.5, 0.01, 0.0], np.float32),
+         first_visible=np.repeat([100, 7, 0, 3, 1990, 0, 5], [1, 300, 4, 8, 9, 1, 33]).astype(np.int32)).spoil_tails().check()
+
+
+@pytest.mark.parametrize("hq", [3, 9, 17, 32])
+@pytest.mark.parametrize("lens", [[5], [130, 5000]])
+def test_single_tokens_of_wide_groups(hq, lens):
+    for how in ({}, dict(logit_cap=5.0), dict(slopes=(0.1 * np.arange(hq)).astype(np.float32)), dict(window=77)):
+        Case([1] * len(lens), lens, hq, 1, 64 if hq % 2 else 128, seed=hq, offsets=False, **how).spoil_tails().check()
+        Case([1] * len(lens), lens, hq, 1, 128 if hq % 2 else 64, seed=hq, offsets=True, **how).spoil_tails().check()
