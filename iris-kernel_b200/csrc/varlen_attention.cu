@@ -7,11 +7,16 @@
 //   * softmax warps, a row a thread, four warps a row tile: scores from tensor
 //     memory, mask, cap and bias, running maximum and sum in registers,
 //     probabilities back to tensor memory as the next product's operand;
-//   * unpacking warps, a cached token a thread: packed rows and scales arrive in
-//     a ring of the thread's own (cp.async), and leave as swizzled fp16 tiles;
+//   * eight unpacking warps, a cached token a thread, four for keys and four for
+//     values: packed rows (TMA) and scales become swizzled fp16 tiles;
 //   * one warp that issues the products: S = Q K^T (both operands in shared
-//     memory, K-major) and O += P V (P in tensor memory, V as it lies, MN-major).
+//     memory, K-major) and O += P V (P in tensor memory, V as it lies, MN-major);
+//   * one warp that issues the copies.
 // Two row tiles take turns: one's softmax runs while the other's products do.
+// A row's scores are read twice, 32 columns at a time (maximum, then
+// probabilities): all 128 at once would not fit the registers of 18 warps, and
+// what is spilled here misses the few kilobytes of L1 that are left (740 us
+// for two prompts of 4096 tokens).
 //
 // Roundings.  Stored values are nibble * scale, 15 bits: fp16 keeps 11.  Each
 // run of 32 tokens is first scaled by a power of two that brings its largest
@@ -24,25 +29,24 @@
 namespace iris {
 namespace {
 
-constexpr int kThreads = 512;
 template <int D, int kTiles>
 struct Cfg {
-  static constexpr int kUnpackGroups = kTiles == 1 ? 2 : 1;        // warpgroups that unpack
-  static constexpr int kRing = 3;                                  // raw units a ring
-  static constexpr int kOperand = kTile * D * 2;                   // one fp16 tile
-  static constexpr int kUnit = kTile * (D / 2 + D / 16);           // one packed tile with its scales
-  static constexpr int kSmem = 1024 + (kTiles + 4) * kOperand + kUnpackGroups * kRing * kUnit;
+  static constexpr int kOperand = kTile * D * 2;       // one fp16 tile
+  static constexpr int kPacked = kTile * D / 2;        // one packed tile
+  static constexpr int kSmem = 1024 + (kTiles + 4) * kOperand + 4 * kPacked;
   static constexpr int kColumns = kTiles == 2 ? 512 : 256;
-  static constexpr int kOutColumn = kTiles * kTile;                // first column of O
+  static constexpr int kOutColumn = kTiles * kTile;    // first column of O
   static constexpr int kSoftWarps = 4 * kTiles;
-  static constexpr int kMmaWarp = kSoftWarps + 4 * kUnpackGroups;
+  static constexpr int kMmaWarp = kSoftWarps + 8, kCopyWarp = kMmaWarp + 1;
+  static constexpr int kThreads = 32 * (kCopyWarp + 1);
 };
 
 struct Shared {
+  uint64_t raw_full[2][2], raw_empty[2][2];  // [keys, values][slot]: packed tiles
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2], p_full[2], o_full[2], drain;
   uint32_t tmem;
-  int32_t k_exp[4][4], v_exp[4][4];  // [tile & 3][run of 32 tokens]
+  alignas(16) int32_t k_exp[4][4], v_exp[4][4];  // [tile & 3][run of 32 tokens]
   uint32_t v_any[2][4];              // a run has values that are not finite
   uint8_t v_bad[2][kTile];           // which groups of a token's
   // the block's work
@@ -51,76 +55,52 @@ struct Shared {
 };
 
 // ------------------------------------------------------------------ unpacking
-// kKind: 0 keys, 1 values, 2 both in turn.
-template <int D, int kTiles, int kKind>
+template <int D, bool kKeys>
 IRIS_DEV void unpack_tiles(const AttendParams& p, Shared& sh, const Tiles& tiles, int k0, int n, int b, int len, int h,
-                           uint32_t ring, uint32_t k_tiles, uint32_t v_tiles, int tid) {
-  using C = Cfg<D, kTiles>;
-  constexpr int kChunks = D / 32;
+                           uint32_t packed, uint32_t operands, int tid) {
+  using C = Cfg<D, 1>;
+  constexpr int kGroups = D / 32;
   const int warp = tid >> 5, lane = tid & 31;
-  const int units = kKind == 2 ? 2 * n : n;
-  const int64_t row_bytes = static_cast<int64_t>(p.s.hkv) * (D / 2);
-  int32_t next_page = page_of(p.s, b, tiles.at(k0) * kTile + tid, len), page = 0;
-  int loaded = -1;  // tile that `page` belongs to
-  auto load = [&](int u) {
-    if (u < units) {
-      const int k = kKind == 2 ? u >> 1 : u;
-      const bool keys = kKind == 0 || (kKind == 2 && (u & 1) == 0);
-      const int32_t j = tiles.at(k0 + k) * kTile + tid;
-      if (k != loaded) {
-        page = next_page;
-        loaded = k;
-        if (k + 1 < n) next_page = page_of(p.s, b, tiles.at(k0 + k + 1) * kTile + tid, len);
-      }
-      const bool there = j < len;
-      const int64_t row = static_cast<int64_t>(page) * kTokPage + j % kTokPage;
-      const uint8_t* data = (keys ? p.k_data : p.v_data) + row * row_bytes + h * (D / 2);
-      const uint8_t* scale = (keys ? p.k_scale : p.v_scale) + (row * p.s.hkv + h) * (D / 16);
-      const uint32_t slot = ring + (u % C::kRing) * C::kUnit;
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) copy_async<16>(slot + c * 2048 + tid * 16, data + c * 16, there);
-      copy_async<D / 16>(slot + kChunks * 2048 + tid * (D / 16), scale, there);
-    }
-    copies_commit();
-  };
-#pragma unroll
-  for (int u = 0; u < C::kRing - 1; ++u) load(u);
-  for (int u = 0; u < units; ++u) {
-    load(u + C::kRing - 1);
-    copies_wait<C::kRing - 1>();
-    const int k = kKind == 2 ? u >> 1 : u;
-    const bool keys = kKind == 0 || (kKind == 2 && (u & 1) == 0);
-    const uint32_t slot = ring + (u % C::kRing) * C::kUnit;
-    // scales: what the run of 32 tokens is scaled by, and what is not finite
-    uint32_t sc[kChunks / 2];
+  const uint8_t* scales = kKeys ? p.k_scale : p.v_scale;
+  auto token = [&](int k) { return tiles.at(k0 + k) * kTile + tid; };
+  uint32_t sc2[kGroups / 2];  // the scales of the tile that is next
+  auto fetch = [&](int32_t page, int32_t j) {
+    const uint8_t* x = scales + ((static_cast<int64_t>(page) * kTokPage + (j & (kTokPage - 1))) * p.s.hkv + h) * (D / 16);
     if constexpr (D == 128) {
-      const uint2 v = lds64(slot + kChunks * 2048 + tid * 8);
-      sc[0] = v.x;
-      sc[1] = v.y;
+      const uint2 v = j < len ? __ldg(reinterpret_cast<const uint2*>(x)) : make_uint2(0, 0);
+      sc2[0] = v.x;
+      sc2[1] = v.y;
     } else {
-      sc[0] = lds32(slot + kChunks * 2048 + tid * 4);
+      sc2[0] = j < len ? __ldg(reinterpret_cast<const uint32_t*>(x)) : 0u;
     }
-    const bool there = tiles.at(k0 + k) * kTile + tid < len;
-    uint32_t most = 0, bad = 0;
-    float f[kChunks];
+  };
+  fetch(page_of(p.s, b, token(0), len), token(0));
+  int32_t page = n > 1 ? raw_page(p.s, b, token(1), len) : 0;
+#pragma unroll 1
+  for (int k = 0; k < n; ++k) {
+    const int st = k & 1;
+    // what the run of 32 tokens is scaled by, and what is not finite
+    uint32_t most = 0, bad = 0, s2[kGroups];
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const uint32_t bits = there ? (sc[c / 2] >> (16 * (c & 1))) & 0xffffu : 0u;
-      const uint32_t mag = bits & 0x7fffu;
+    for (int c = 0; c < kGroups; ++c) {
+      s2[c] = (sc2[c / 2] >> (16 * (c & 1))) & 0xffffu;
+      const uint32_t mag = s2[c] & 0x7fffu;
       if (mag >= 0x7c00u) bad |= 1u << c; else most = max(most, mag);
-      f[c] = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
     }
     const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 10);
     const float up = pow2i(27 - e);
-    uint32_t s2[kChunks];  // the scale twice, as fp16
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const float v = f[c] * up;
-      s2[c] = (bad >> c) & 1u ? (keys ? 0x7fff7fffu : 0u) : Fp16Elem::pack(v, v);
+    for (int c = 0; c < kGroups; ++c) {  // the scale twice, as fp16
+      const float v = __half2float(__ushort_as_half(static_cast<unsigned short>(s2[c]))) * up;
+      s2[c] = (bad >> c) & 1u ? (kKeys ? 0x7fff7fffu : 0u) : Fp16Elem::pack(v, v);
     }
-    const int st = k & 1;
-    if (!wait_all(keys ? &sh.k_empty[st] : &sh.v_empty[st], ((k >> 1) & 1) ^ 1, p.s.err)) break;
-    if (keys) {
+    if (k + 1 < n) {
+      fetch(checked_page(p.s, page), token(k + 1));
+      if (k + 2 < n) page = raw_page(p.s, b, token(k + 2), len);
+    }
+    if (!wait_all(&sh.raw_full[kKeys ? 0 : 1][st], (k >> 1) & 1, p.s.err)) break;
+    if (!wait_all(kKeys ? &sh.k_empty[st] : &sh.v_empty[st], ((k >> 1) & 1) ^ 1, p.s.err)) break;
+    if (kKeys) {
       if (lane == 0) sh.k_exp[k & 3][warp] = e - 27;
     } else {
       const bool any = __any_sync(0xffffffffu, bad != 0);
@@ -130,10 +110,10 @@ IRIS_DEV void unpack_tiles(const AttendParams& p, Shared& sh, const Tiles& tiles
       }
       if (any) sh.v_bad[st][tid] = static_cast<uint8_t>(bad);
     }
-    const uint32_t dst = (keys ? k_tiles : v_tiles) + st * C::kOperand;
+    const uint32_t src = packed + st * C::kPacked, dst = operands + st * C::kOperand;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const uint4 w4 = lds128(slot + c * 2048 + tid * 16);
+    for (int c = 0; c < kGroups; ++c) {
+      const uint4 w4 = lds128(src + packed_at<D>(tid, c));
       const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
       const __half2 s = u32_as_h2(s2[c]);
 #pragma unroll
@@ -145,9 +125,32 @@ IRIS_DEV void unpack_tiles(const AttendParams& p, Shared& sh, const Tiles& tiles
       }
     }
     fence_proxy_async_shared();
-    mbar_arrive(keys ? &sh.k_full[st] : &sh.v_full[st]);
+    mbar_arrive(kKeys ? &sh.k_full[st] : &sh.v_full[st]);
+    mbar_arrive(&sh.raw_empty[kKeys ? 0 : 1][st]);
   }
-  copies_wait<0>();
+}
+
+// --------------------------------------------------------------------- copies
+template <int D>
+IRIS_DEV void issue_copies(const AttendParams& p, const CUtensorMap* k_map, const CUtensorMap* v_map, Shared& sh,
+                           const Tiles& tiles, int k0, int n, int b, int len, int h, uint8_t* packed, int lane) {
+  constexpr int kPacked = kTile * D / 2;
+  auto first = [&](int k) { return tiles.at(k0 + k) * kTile; };
+  auto page_at = [&](int k) { return lane < 8 ? raw_page(p.s, b, first(k) + lane * kTokPage, len) : 0; };
+  int32_t later = page_at(0);
+  int k = 0;
+#pragma unroll 1
+  for (; k < n; ++k) {
+    const int32_t page = checked_page(p.s, later);
+    if (k + 1 < n) later = page_at(k + 1);
+    const int st = k & 1;
+    if (!wait_all(&sh.raw_empty[0][st], ((k >> 1) & 1) ^ 1, p.s.err)) break;
+    load_packed<D>(packed + st * kPacked, k_map, page, first(k), len, h, &sh.raw_full[0][st], lane);
+    if (!wait_all(&sh.raw_empty[1][st], ((k >> 1) & 1) ^ 1, p.s.err)) break;
+    load_packed<D>(packed + (2 + st) * kPacked, v_map, page, first(k), len, h, &sh.raw_full[1][st], lane);
+  }
+  if (k < n)  // a wait gave up: copies that are under way land before the block ends
+    for (int i = 0; i < 8; ++i) mbar_wait_bounded(&sh.raw_full[i & 1][(i >> 1) & 1], i >> 2, p.s.err);
 }
 
 // ------------------------------------------------------------------- products
@@ -205,6 +208,14 @@ IRIS_DEV void issue_products(const AttendParams& p, Shared& sh, int n, int activ
 }
 
 // -------------------------------------------------------------------- softmax
+// 32 columns of this thread's lane.
+IRIS_DEV void load_scores(uint32_t at, float (&s)[32]) {
+  umma_ld32(at, reinterpret_cast<uint32_t*>(s));
+  umma_wait_ld();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) asm volatile("" : "+f"(s[j]));
+}
+
 template <int D, int kTiles, bool kCap, bool kBias>
 IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles, int k0, int n, int rows, int h, int tile,
                            uint32_t q_tiles, uint32_t tmem, int split, int warp, int lane) {
@@ -260,54 +271,52 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
     if (!(ok = wait_all(&sh.v_full[k & 1], (k >> 1) & 1, p.s.err))) break;
     umma_fence_after();
     if (busy) {
-      float s[kTile];
-      uint32_t* sw = reinterpret_cast<uint32_t*>(s);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) umma_ld32(s_at + 32 * c, sw + 32 * c);
-      umma_wait_ld();
-#pragma unroll
-      for (int j = 0; j < kTile; ++j) asm volatile("" : "+f"(s[j]));
       const int32_t base = tiles.at(k0 + k) * kTile;
+      const int4 ke = *reinterpret_cast<const int4*>(sh.k_exp[k & 3]), ve = *reinterpret_cast<const int4*>(sh.v_exp[k & 3]);
+      const int kes[4] = {ke.x, ke.y, ke.z, ke.w}, ves[4] = {ve.x, ve.y, ve.z, ve.w};
       float f[4];
-      int ve[4], top_e = ref;
+      int top_e = ref;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        f[c] = fmaxf(unit * pow2i(sh.k_exp[k & 3][c]), 1.17549435e-38f);
-        ve[c] = sh.v_exp[k & 3][c];
-        top_e = max(top_e, ve[c]);
+        f[c] = fmaxf(unit * pow2i(kes[c]), 1.17549435e-38f);
+        top_e = max(top_e, ves[c]);
       }
-      if (kMod) {
-        const float d0 = static_cast<float>(pos - base);
+      const bool full = !valid || (sight.b0 <= base && base + kTile <= sight.b1) ||
+                        (sight.a0 <= base && base + kTile <= sight.a1);
+      const bool masked = !__all_sync(0xffffffffu, full);
+      // ---- the largest logit; with a mask, a cap or a bias the logits go back as they now are
+      float top = kMinusInf;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 4; ++c) {
+        float s[32];
+        load_scores(s_at + 32 * c, s);
+        if (kMod) {
+          const float d0 = static_cast<float>(pos - base - 32 * c);
 #pragma unroll
-          for (int j = 32 * c; j < 32 * c + 32; ++j) {
+          for (int j = 0; j < 32; ++j) {
             float y = s[j] * f[c];
             if (kCap) y = cap2 * tanh_f(y);
             if (kBias) y = fmaf(slope2, fabsf(d0 - j), y);
             s[j] = y;
           }
-      }
-      const bool full = !valid || (sight.b0 <= base && base + kTile <= sight.b1) ||
-                        (sight.a0 <= base && base + kTile <= sight.a1);
-      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
-      if (!__all_sync(0xffffffffu, full)) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          bits[c] = sight_bits(sight, base + 32 * c);
+        }
+        if (masked) {
+          const uint32_t bits = valid ? sight_bits(sight, base + 32 * c) : ~0u;
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (!((bits[c] >> j) & 1u)) s[32 * c + j] = kMinusInf;
+            if (!((bits >> j) & 1u)) s[j] = kMinusInf;
         }
-      }
-      float top = kMinusInf;
+        if (kMod || masked) umma_st32(s_at + 32 * c, reinterpret_cast<const uint32_t*>(s));
+        float t0 = s[0], t1 = s[1];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float t = s[32 * c];
-#pragma unroll
-        for (int j = 1; j < 32; ++j) t = fmaxf(t, s[32 * c + j]);
-        top = fmaxf(top, kMod ? t : t * f[c]);
+        for (int j = 2; j < 32; j += 2) {
+          t0 = fmaxf(t0, s[j]);
+          t1 = fmaxf(t1, s[j + 1]);
+        }
+        t0 = fmaxf(t0, t1);
+        top = fmaxf(top, kMod ? t0 : t0 * f[c]);
       }
+      if (kMod || masked) umma_wait_st();
       // raise the row's reference where its logits pass it by too much, and the values' power where one is larger
       const bool rise = top > m + kRise;  // (also from -inf)
       if (__any_sync(0xffffffffu, rise) || top_e > ref) {
@@ -316,17 +325,13 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
           const float by = (rise ? ex2(m - to) : 1.0f) * pow2i(max(ref - top_e, -126));
           if (!(ok = wait_all(&sh.o_full[tile], (k - 1) & 1, p.s.err))) break;
           umma_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            umma_ld32(o_at + 32 * c, o);
-            umma_wait_ld();
+            float o[32];
+            load_scores(o_at + 32 * c, o);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              asm volatile("" : "+r"(o[j]));
-              o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
-            }
-            umma_st32(o_at + 32 * c, o);
+            for (int j = 0; j < 32; ++j) o[j] *= by;
+            umma_st32(o_at + 32 * c, reinterpret_cast<const uint32_t*>(o));
           }
           if (rise) l *= ex2(m - to);
         }
@@ -337,29 +342,31 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
       // From 2^24 on a product that is not rounded may pass the reference by more than fp16 holds, and the addend has no
       // room for the power beside it: there the reference comes off first, from rounded products.
       const bool far = __any_sync(0xffffffffu, fabsf(zero) > 8388608.0f);
-      if (far) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-#pragma unroll
-          for (int j = 32 * c; j < 32 * c + 32; ++j) s[j] = (kMod ? s[j] : __fmul_rn(s[j], f[c])) + zero;
-          f[c] = 1.0f;
-        }
-      }
+      // ---- probabilities and their sum
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const float add = (far ? 0.0f : zero) + (kHead + static_cast<float>(ve[c] - ref));
+        float s[32];
+        load_scores(s_at + 32 * c, s);
+        float add = kHead + static_cast<float>(ves[c] - ref), by = f[c];
+        if (far) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) s[j] = (kMod ? s[j] : __fmul_rn(s[j], by)) + zero;
+          by = 1.0f;
+        } else {
+          add += zero;
+        }
         float2 sum = make_float2(0.0f, 0.0f);
         uint32_t w[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          float2 y = make_float2(s[32 * c + 2 * j], s[32 * c + 2 * j + 1]);
-          y = kMod ? __fadd2_rn(y, make_float2(add, add)) : __ffma2_rn(y, make_float2(f[c], f[c]), make_float2(add, add));
+          float2 y = make_float2(s[2 * j], s[2 * j + 1]);
+          y = kMod ? __fadd2_rn(y, make_float2(add, add)) : __ffma2_rn(y, make_float2(by, by), make_float2(add, add));
           y.x = ex2(y.x);
           y.y = ex2(y.y);
           sum = __fadd2_rn(sum, y);
           w[j] = Fp16Elem::pack(y.x, y.y);
         }
-        l = fmaf(sum.x + sum.y, pow2i(min(ref - ve[c], 126)) * (1.0f / 256.0f), l);
+        l = fmaf(sum.x + sum.y, pow2i(min(ref - ves[c], 126)) * (1.0f / 256.0f), l);
         umma_st16(s_at + 16 * c, w);
       }
       if (sh.v_any[k & 1][0] | sh.v_any[k & 1][1] | sh.v_any[k & 1][2] | sh.v_any[k & 1][3]) {
@@ -384,18 +391,13 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
   const bool whole = p.splits == 1;
   const int64_t row = static_cast<int64_t>(token) * p.s.hq + head;
   const float norm = l == 0.0f ? 0.0f : pow2i(max(ref, -126)) * (1.0f / 256.0f) / l;
-#pragma unroll
+#pragma unroll 1
   for (int c = 0; c < D / 32; ++c) {
-    uint32_t o[32];
-    if (n > 0) {
-      umma_ld32(o_at + 32 * c, o);
-      umma_wait_ld();
-    }
     float v[32];
+    if (n > 0) load_scores(o_at + 32 * c, v);
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
-      if (n > 0) asm volatile("" : "+r"(o[j]));
-      v[j] = n > 0 && l != 0.0f ? __uint_as_float(o[j]) * norm : 0.0f;
+      v[j] = n > 0 && l != 0.0f ? v[j] * norm : 0.0f;
       if ((spoilt >> c) & 1u) v[j] = __int_as_float(0x7fffffff);
     }
     if (!valid) continue;
@@ -427,7 +429,9 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
 }
 
 template <int D, int kTiles, bool kCap, bool kBias>
-__global__ void __launch_bounds__(kThreads, 1) varlen_attention_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(Cfg<D, kTiles>::kThreads, 1)
+    varlen_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                            const AttendParams p) {
   using C = Cfg<D, kTiles>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared sh;
@@ -443,6 +447,10 @@ __global__ void __launch_bounds__(kThreads, 1) varlen_attention_kernel(const Att
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i], 128);
       mbar_init(&sh.o_full[i], 1);
+      for (int kind = 0; kind < 2; ++kind) {
+        mbar_init(&sh.raw_full[kind][i], 1);
+        mbar_init(&sh.raw_empty[kind][i], 128);
+      }
     }
     mbar_init(&sh.drain, 1);
     fence_barrier_init();
@@ -490,13 +498,10 @@ __global__ void __launch_bounds__(kThreads, 1) varlen_attention_kernel(const Att
   const int64_t all = tiles.count();
   const int k0 = static_cast<int>(all * split / p.splits), n = static_cast<int>(all * (split + 1) / p.splits) - k0;
 
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t q_tiles = base, k_tiles = base + kTiles * C::kOperand, v_tiles = k_tiles + 2 * C::kOperand;
-  const uint32_t ring = v_tiles + 2 * C::kOperand;
-  // Registers: 512 threads come with 128 each.  kTiles 2: 256 x 176 + 256 x 80
-  // = 65,536; kTiles 1: 128 x 176 + 256 x 120 + 128 x 80 = 63,488.
+  uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t q_tiles = smem_u32(base), k_tiles = q_tiles + kTiles * C::kOperand, v_tiles = k_tiles + 2 * C::kOperand;
+  uint8_t* packed = base + (kTiles + 4) * C::kOperand;  // two slots of keys, two of values
   if (warp < C::kSoftWarps) {
-    regs_take<176>();
     const int tile = warp >> 2;
     if (tile < active) {
       softmax_rows<D, kTiles, kCap, kBias>(p, sh, tiles, k0, n, rows, h, tile, q_tiles, tmem, split, warp & 3, lane);
@@ -505,26 +510,17 @@ __global__ void __launch_bounds__(kThreads, 1) varlen_attention_kernel(const Att
     }
   } else if (warp < C::kMmaWarp) {
     const int tid = (threadIdx.x - C::kSoftWarps * 32) & 127;
-    if constexpr (kTiles == 2) {
-      regs_give<80>();
-      if (n > 0)
-        unpack_tiles<D, kTiles, 2>(p, sh, tiles, k0, n, sh.b, sh.len, h, ring, k_tiles, v_tiles, tid);
-    } else {
-      regs_give<120>();
-      if (n > 0) {
-        if (warp < C::kSoftWarps + 4)
-          unpack_tiles<D, kTiles, 0>(p, sh, tiles, k0, n, sh.b, sh.len, h, ring, k_tiles, v_tiles, tid);
-        else
-          unpack_tiles<D, kTiles, 1>(p, sh, tiles, k0, n, sh.b, sh.len, h, ring + C::kRing * C::kUnit, k_tiles, v_tiles,
-                                     tid);
-      }
+    if (n > 0) {
+      if (warp < C::kSoftWarps + 4)
+        unpack_tiles<D, true>(p, sh, tiles, k0, n, sh.b, sh.len, h, smem_u32(packed), k_tiles, tid);
+      else
+        unpack_tiles<D, false>(p, sh, tiles, k0, n, sh.b, sh.len, h, smem_u32(packed) + 2 * C::kPacked, v_tiles, tid);
     }
-  } else {
-    regs_give<80>();
-    if (warp == C::kMmaWarp) {
-      asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftWarps * 32 + 32) : "memory");
-      if (n > 0) issue_products<D, kTiles>(p, sh, n, active, q_tiles, k_tiles, v_tiles, tmem);
-    }
+  } else if (warp == C::kMmaWarp) {
+    asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftWarps * 32 + 32) : "memory");
+    if (n > 0) issue_products<D, kTiles>(p, sh, n, active, q_tiles, k_tiles, v_tiles, tmem);
+  } else if (n > 0) {
+    issue_copies<D>(p, &k_map, &v_map, sh, tiles, k0, n, sh.b, sh.len, h, packed, lane);
   }
   umma_fence_before();
   __syncthreads();
@@ -637,7 +633,11 @@ cudaError_t launch_attend(const AttendParams& p, int64_t grid, cudaStream_t stre
     if (e != cudaSuccess) return e;
     if (device < 64) ready |= 1ull << device;
   }
-  return launch_early(fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Cfg<D, kTiles>::kSmem, stream, p);
+  CUtensorMap k, v;
+  if (!packed_map(&k, p.k_data, D, p.s.hkv, p.s.num_pages) || !packed_map(&v, p.v_data, D, p.s.hkv, p.s.num_pages))
+    return cudaErrorInvalidValue;
+  return launch_early(fn, dim3(static_cast<unsigned>(grid)), dim3(Cfg<D, kTiles>::kThreads), Cfg<D, kTiles>::kSmem, stream,
+                      k, v, p);
 }
 
 template <int D, int kCols, bool kCap, bool kBias>
