@@ -4,9 +4,9 @@
 //
 // A block owns up to 128 * kTiles rows (new token x query head) of one KV head
 // and walks the tiles of 128 cached tokens that any of them sees.  Its warps:
-//   * softmax warps, a row a thread, four warps a row tile: scores from tensor
-//     memory, mask, cap and bias, running maximum and sum in registers,
-//     probabilities back to tensor memory as the next product's operand;
+//   * softmax warps, two threads a row (64 columns each), eight warps a row tile:
+//     scores from tensor memory, mask, cap and bias, running maximum and sum in
+//     registers, probabilities back to tensor memory as the next product's operand;
 //   * eight unpacking warps, a cached token a thread, four for keys and four for
 //     values: packed rows (TMA) and scales become swizzled fp16 tiles;
 //   * one warp that issues the products: S = Q K^T (both operands in shared
@@ -14,9 +14,9 @@
 //   * one warp that issues the copies.
 // Two row tiles take turns: one's softmax runs while the other's products do.
 // A row's scores are read twice, 32 columns at a time (maximum, then
-// probabilities): all 128 at once would not fit the registers of 18 warps, and
-// what is spilled here misses the few kilobytes of L1 that are left (740 us
-// for two prompts of 4096 tokens).
+// probabilities): all at once would not fit the registers, and what is spilled
+// here misses the few kilobytes of L1 that are left (740 us for two prompts of
+// 4096 tokens; 506 without).
 //
 // Roundings.  Stored values are nibble * scale, 15 bits: fp16 keeps 11.  Each
 // run of 32 tokens is first scaled by a power of two that brings its largest
@@ -33,22 +33,25 @@ template <int D, int kTiles>
 struct Cfg {
   static constexpr int kOperand = kTile * D * 2;       // one fp16 tile
   static constexpr int kPacked = kTile * D / 2;        // one packed tile
-  static constexpr int kSmem = 1024 + (kTiles + 4) * kOperand + 4 * kPacked;
+  static constexpr int kSmem = 1024 + (kTiles + 4) * kOperand + 3 * kPacked;  // two packed slots of keys, one of values
   static constexpr int kColumns = kTiles == 2 ? 512 : 256;
   static constexpr int kOutColumn = kTiles * kTile;    // first column of O
-  static constexpr int kSoftWarps = 4 * kTiles;
+  static constexpr int kSoftWarps = 8 * kTiles;
   static constexpr int kMmaWarp = kSoftWarps + 8, kCopyWarp = kMmaWarp + 1;
   static constexpr int kThreads = 32 * (kCopyWarp + 1);
 };
 
 struct Shared {
-  uint64_t raw_full[2][2], raw_empty[2][2];  // [keys, values][slot]: packed tiles
+  uint64_t raw_full[3], raw_empty[3];  // packed tiles: two slots of keys, one of values
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2], p_full[2], o_full[2], drain;
   uint32_t tmem;
   alignas(16) int32_t k_exp[4][4], v_exp[4][4];  // [tile & 3][run of 32 tokens]
   uint32_t v_any[2][4];              // a run has values that are not finite
   uint8_t v_bad[2][kTile];           // which groups of a token's
+  float top[2][2][2][kTile];         // [tile & 1][row tile][half]: a row's largest logit; at the end its sum
+  float back[2][kTile];              // undoes the query row's power of two
+  uint32_t spoilt[2][kTile];         // groups of dims with a visible value that is not finite
   // the block's work
   int32_t b, index, start, count, len, first_lo;
   int32_t live;
@@ -98,7 +101,8 @@ IRIS_DEV void unpack_tiles(const AttendParams& p, Shared& sh, const Tiles& tiles
       fetch(checked_page(p.s, page), token(k + 1));
       if (k + 2 < n) page = raw_page(p.s, b, token(k + 2), len);
     }
-    if (!wait_all(&sh.raw_full[kKeys ? 0 : 1][st], (k >> 1) & 1, p.s.err)) break;
+    const int slot = kKeys ? st : 2;
+    if (!wait_all(&sh.raw_full[slot], kKeys ? (k >> 1) & 1 : k & 1, p.s.err)) break;
     if (!wait_all(kKeys ? &sh.k_empty[st] : &sh.v_empty[st], ((k >> 1) & 1) ^ 1, p.s.err)) break;
     if (kKeys) {
       if (lane == 0) sh.k_exp[k & 3][warp] = e - 27;
@@ -110,7 +114,7 @@ IRIS_DEV void unpack_tiles(const AttendParams& p, Shared& sh, const Tiles& tiles
       }
       if (any) sh.v_bad[st][tid] = static_cast<uint8_t>(bad);
     }
-    const uint32_t src = packed + st * C::kPacked, dst = operands + st * C::kOperand;
+    const uint32_t src = packed + slot * C::kPacked, dst = operands + st * C::kOperand;
 #pragma unroll
     for (int c = 0; c < kGroups; ++c) {
       const uint4 w4 = lds128(src + packed_at<D>(tid, c));
@@ -126,7 +130,7 @@ IRIS_DEV void unpack_tiles(const AttendParams& p, Shared& sh, const Tiles& tiles
     }
     fence_proxy_async_shared();
     mbar_arrive(kKeys ? &sh.k_full[st] : &sh.v_full[st]);
-    mbar_arrive(&sh.raw_empty[kKeys ? 0 : 1][st]);
+    mbar_arrive(&sh.raw_empty[slot]);
   }
 }
 
@@ -144,13 +148,13 @@ IRIS_DEV void issue_copies(const AttendParams& p, const CUtensorMap* k_map, cons
     const int32_t page = checked_page(p.s, later);
     if (k + 1 < n) later = page_at(k + 1);
     const int st = k & 1;
-    if (!wait_all(&sh.raw_empty[0][st], ((k >> 1) & 1) ^ 1, p.s.err)) break;
-    load_packed<D>(packed + st * kPacked, k_map, page, first(k), len, h, &sh.raw_full[0][st], lane);
-    if (!wait_all(&sh.raw_empty[1][st], ((k >> 1) & 1) ^ 1, p.s.err)) break;
-    load_packed<D>(packed + (2 + st) * kPacked, v_map, page, first(k), len, h, &sh.raw_full[1][st], lane);
+    if (!wait_all(&sh.raw_empty[st], ((k >> 1) & 1) ^ 1, p.s.err)) break;
+    load_packed<D>(packed + st * kPacked, k_map, page, first(k), len, h, &sh.raw_full[st], lane);
+    if (!wait_all(&sh.raw_empty[2], (k & 1) ^ 1, p.s.err)) break;
+    load_packed<D>(packed + 2 * kPacked, v_map, page, first(k), len, h, &sh.raw_full[2], lane);
   }
   if (k < n)  // a wait gave up: copies that are under way land before the block ends
-    for (int i = 0; i < 8; ++i) mbar_wait_bounded(&sh.raw_full[i & 1][(i >> 1) & 1], i >> 2, p.s.err);
+    for (int i = 0; i < 6; ++i) mbar_wait_bounded(&sh.raw_full[i % 3], i / 3, p.s.err);
 }
 
 // ------------------------------------------------------------------- products
@@ -187,7 +191,7 @@ IRIS_DEV void issue_products(const AttendParams& p, Shared& sh, int n, int activ
         const uint32_t v = v_tiles + (k & 1) * C::kOperand;
 #pragma unroll
         for (int s = 0; s < kTile / 16; ++s)
-          umma_ts(tmem + C::kOutColumn + i * D, tmem + i * kTile + 8 * s, umma_desc(v + s * 2048, kTile * 128, 1024), kOut,
+          umma_ts(tmem + C::kOutColumn + i * D, tmem + i * kTile + 8 * s + (s < 4 ? 0 : 32), umma_desc(v + s * 2048, kTile * 128, 1024), kOut,
                   k > 0 || s > 0);
         umma_commit(smem_u32(&sh.o_full[i]));
         if (i == active - 1) umma_commit(smem_u32(&sh.v_empty[k & 1]));
@@ -221,73 +225,71 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
                            uint32_t q_tiles, uint32_t tmem, int split, int warp, int lane) {
   using C = Cfg<D, kTiles>;
   constexpr bool kMod = kCap || kBias;
-  const int local = warp * 32 + lane;  // row of the row tile
+  const int half = warp >> 2, quarter = warp & 3;
+  const int local = quarter * 32 + lane;  // row of the row tile
   const int r = sh.index * (kTile * kTiles) + tile * kTile + local;
   const bool valid = r < rows;
   const int i = valid ? r / p.s.group : 0, g = valid ? r % p.s.group : 0;
   const int token = sh.start + i, head = h * p.s.group + g;
   const int32_t pos = sh.len - sh.count + i;
   Sight sight = {0, 0, 0, 0};
-  float back = 1.0f;  // undoes the query row's power of two
   if (valid) {
     const int32_t prefix = p.s.prefix_lens != nullptr ? __ldg(p.s.prefix_lens + sh.b) : 0;
     const int32_t first = p.s.first_visible != nullptr ? __ldg(p.s.first_visible + token) : 0;
     sight = row_sight(pos, first, prefix, p.s.window, sh.len);
-    if (n > 0) {
+    if (n > 0 && half == 0) {
       const uint4* src = reinterpret_cast<const uint4*>(p.query + token * p.q_stride + static_cast<int64_t>(head) * D);
-      uint32_t w[D / 2];
-#pragma unroll
+      uint32_t most = 0;
+#pragma unroll 4
       for (int c = 0; c < D / 8; ++c) {
         const uint4 v = src[c];
-        w[4 * c] = v.x;
-        w[4 * c + 1] = v.y;
-        w[4 * c + 2] = v.z;
-        w[4 * c + 3] = v.w;
+        most = max(max(most, pair_size(v.x)), max(max(pair_size(v.y), pair_size(v.z)), pair_size(v.w)));
       }
-      back = scale_row(w, p.bf16 != 0);
+      float up;
+      sh.back[tile][local] = row_power(most, p.bf16 != 0, &up);
       const uint32_t dst = q_tiles + tile * C::kOperand;
-#pragma unroll
+#pragma unroll 4
       for (int c = 0; c < D / 8; ++c) {
-        const uint4 v = order8(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+        uint4 v = src[c];
+        v = order8(scale_pair(v.x, p.bf16 != 0, up), scale_pair(v.y, p.bf16 != 0, up), scale_pair(v.z, p.bf16 != 0, up),
+                   scale_pair(v.w, p.bf16 != 0, up));
         sts128(dst + operand_at(local, c), v.x, v.y, v.z, v.w);
       }
     }
   }
+  if (half == 0) sh.spoilt[tile][local] = 0;
   fence_proxy_async_shared();
   asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftWarps * 32 + 32) : "memory");  // with the warp of the products
 
-  const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-  const uint32_t s_at = lanes + tile * kTile, o_at = lanes + C::kOutColumn + tile * D;
+  const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  const uint32_t s_at = lanes + tile * kTile + half * 64, o_at = lanes + C::kOutColumn + tile * D + half * (D / 2);
   const bool busy = __any_sync(0xffffffffu, valid);
+  const float back = n > 0 ? sh.back[tile][local] : 1.0f;
   const float unit = kCap ? p.s.scale * back / p.s.cap : p.s.scale * kLog2e * back;
   const float cap2 = p.s.cap * kLog2e;
   const float slope2 = kBias ? -__ldg(p.s.slopes + head) * kLog2e : 0.0f;
+  auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + tile * 4 + quarter) : "memory"); };  // the rows' two warps
   float m = kMinusInf, l = 0.0f;
   int ref = -127;
-  uint32_t spoilt = 0;  // groups of dims with a visible value that is not finite
   bool ok = true;
+#pragma unroll 1
   for (int k = 0; k < n; ++k) {
     if (!(ok = wait_all(&sh.s_full[tile], k & 1, p.s.err))) break;
     if (!(ok = wait_all(&sh.v_full[k & 1], (k >> 1) & 1, p.s.err))) break;
     umma_fence_after();
     if (busy) {
-      const int32_t base = tiles.at(k0 + k) * kTile;
-      const int4 ke = *reinterpret_cast<const int4*>(sh.k_exp[k & 3]), ve = *reinterpret_cast<const int4*>(sh.v_exp[k & 3]);
-      const int kes[4] = {ke.x, ke.y, ke.z, ke.w}, ves[4] = {ve.x, ve.y, ve.z, ve.w};
-      float f[4];
-      int top_e = ref;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        f[c] = fmaxf(unit * pow2i(kes[c]), 1.17549435e-38f);
-        top_e = max(top_e, ves[c]);
-      }
-      const bool full = !valid || (sight.b0 <= base && base + kTile <= sight.b1) ||
-                        (sight.a0 <= base && base + kTile <= sight.a1);
+      const int32_t base = tiles.at(k0 + k) * kTile + half * 64;
+      const int4 ve = *reinterpret_cast<const int4*>(sh.v_exp[k & 3]);
+      const int2 ke = *reinterpret_cast<const int2*>(sh.k_exp[k & 3] + 2 * half);
+      const int top_e = max(max(ref, max(ve.x, ve.y)), max(ve.z, ve.w));
+      const float f[2] = {fmaxf(unit * pow2i(ke.x), 1.17549435e-38f), fmaxf(unit * pow2i(ke.y), 1.17549435e-38f)};
+      const int ves[2] = {half ? ve.z : ve.x, half ? ve.w : ve.y};
+      const bool full = !valid || (sight.b0 <= base && base + 64 <= sight.b1) || (sight.a0 <= base && base + 64 <= sight.a1);
       const bool masked = !__all_sync(0xffffffffu, full);
       // ---- the largest logit; with a mask, a cap or a bias the logits go back as they now are
       float top = kMinusInf;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         float s[32];
         load_scores(s_at + 32 * c, s);
         if (kMod) {
@@ -316,7 +318,10 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
         t0 = fmaxf(t0, t1);
         top = fmaxf(top, kMod ? t0 : t0 * f[c]);
       }
+      sh.top[k & 1][tile][half][local] = top;
       if (kMod || masked) umma_wait_st();
+      meet();
+      top = fmaxf(top, sh.top[k & 1][tile][half ^ 1][local]);
       // raise the row's reference where its logits pass it by too much, and the values' power where one is larger
       const bool rise = top > m + kRise;  // (also from -inf)
       if (__any_sync(0xffffffffu, rise) || top_e > ref) {
@@ -326,7 +331,7 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
           if (!(ok = wait_all(&sh.o_full[tile], (k - 1) & 1, p.s.err))) break;
           umma_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
+          for (int c = 0; c < D / 64; ++c) {
             float o[32];
             load_scores(o_at + 32 * c, o);
 #pragma unroll
@@ -344,7 +349,7 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
       const bool far = __any_sync(0xffffffffu, fabsf(zero) > 8388608.0f);
       // ---- probabilities and their sum
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         float s[32];
         load_scores(s_at + 32 * c, s);
         float add = kHead + static_cast<float>(ves[c] - ref), by = f[c];
@@ -367,14 +372,16 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
           w[j] = Fp16Elem::pack(y.x, y.y);
         }
         l = fmaf(sum.x + sum.y, pow2i(min(ref - ves[c], 126)) * (1.0f / 256.0f), l);
-        umma_st16(s_at + 16 * c, w);
+        umma_st16(s_at + 16 * c, w);  // over this thread's own scores, which are read
       }
-      if (sh.v_any[k & 1][0] | sh.v_any[k & 1][1] | sh.v_any[k & 1][2] | sh.v_any[k & 1][3]) {
+      if (sh.v_any[k & 1][2 * half] | sh.v_any[k & 1][2 * half + 1]) {
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          if (!sh.v_any[k & 1][c]) continue;
+        for (int c = 0; c < 2; ++c) {
+          if (!sh.v_any[k & 1][2 * half + c]) continue;
+          uint32_t hit = 0;
           for (uint32_t left = valid ? sight_bits(sight, base + 32 * c) : 0u; left != 0; left &= left - 1)
-            spoilt |= sh.v_bad[k & 1][32 * c + __ffs(left) - 1];
+            hit |= sh.v_bad[k & 1][64 * half + 32 * c + __ffs(left) - 1];
+          if (hit != 0) atomicOr(&sh.spoilt[tile][local], hit);
         }
       }
       umma_wait_st();
@@ -382,23 +389,28 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
     umma_fence_before();
     mbar_arrive(&sh.p_full[tile]);
   }
-  // the row's output
+  // the row's output: half the dims each
   if (ok && n > 0) {
     ok = wait_all(&sh.o_full[tile], (n - 1) & 1, p.s.err);
     umma_fence_after();
   }
+  sh.top[n & 1][tile][half][local] = l;
   if (!busy || !ok) return;
+  meet();
+  l += sh.top[n & 1][tile][half ^ 1][local];
+  const uint32_t spoilt = sh.spoilt[tile][local];
   const bool whole = p.splits == 1;
   const int64_t row = static_cast<int64_t>(token) * p.s.hq + head;
   const float norm = l == 0.0f ? 0.0f : pow2i(max(ref, -126)) * (1.0f / 256.0f) / l;
 #pragma unroll 1
-  for (int c = 0; c < D / 32; ++c) {
+  for (int c = 0; c < D / 64; ++c) {
+    const int group = half * (D / 64) + c;  // of 32 dims
     float v[32];
     if (n > 0) load_scores(o_at + 32 * c, v);
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
       v[j] = n > 0 && l != 0.0f ? v[j] * norm : 0.0f;
-      if ((spoilt >> c) & 1u) v[j] = __int_as_float(0x7fffffff);
+      if ((spoilt >> group) & 1u) v[j] = __int_as_float(0x7fffffff);
     }
     if (!valid) continue;
 #pragma unroll
@@ -412,21 +424,23 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
         else
           w = make_uint4(Fp16Elem::pack(x[0], x[2]), Fp16Elem::pack(x[4], x[6]), Fp16Elem::pack(x[1], x[3]),
                          Fp16Elem::pack(x[5], x[7]));
-        reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * D)[4 * c + q] = w;
+        reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * D)[4 * group + q] = w;
       } else {
         float4* dst = reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(split) * p.s.tokens * p.s.hq + row) * D);
-        dst[2 * (4 * c + q)] = make_float4(x[0], x[2], x[4], x[6]);
-        dst[2 * (4 * c + q) + 1] = make_float4(x[1], x[3], x[5], x[7]);
+        dst[2 * (4 * group + q)] = make_float4(x[0], x[2], x[4], x[6]);
+        dst[2 * (4 * group + q) + 1] = make_float4(x[1], x[3], x[5], x[7]);
       }
     }
   }
-  if (!valid) return;
+  if (!valid || half != 0) return;
   const float lse = l == 0.0f ? kMinusInf : (m == kMinusInf ? 0.0f : m) + lg2(l);
   if (!whole)
     p.part_lse[static_cast<int64_t>(split) * p.s.tokens * p.s.hq + row] = lse;
   else if (p.out_lse != nullptr)
     p.out_lse[row] = lse;
 }
+
+static_assert(Cfg<128, 2>::kSmem + sizeof(Shared) <= 227 * 1024, "a block's shared memory");
 
 template <int D, int kTiles, bool kCap, bool kBias>
 __global__ void __launch_bounds__(Cfg<D, kTiles>::kThreads, 1)
@@ -445,12 +459,12 @@ __global__ void __launch_bounds__(Cfg<D, kTiles>::kThreads, 1)
       mbar_init(&sh.k_empty[i], 1);
       mbar_init(&sh.v_empty[i], 1);
       mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 128);
+      mbar_init(&sh.p_full[i], 256);
       mbar_init(&sh.o_full[i], 1);
-      for (int kind = 0; kind < 2; ++kind) {
-        mbar_init(&sh.raw_full[kind][i], 1);
-        mbar_init(&sh.raw_empty[kind][i], 128);
-      }
+    }
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&sh.raw_full[i], 1);
+      mbar_init(&sh.raw_empty[i], 128);
     }
     mbar_init(&sh.drain, 1);
     fence_barrier_init();
@@ -500,11 +514,11 @@ __global__ void __launch_bounds__(Cfg<D, kTiles>::kThreads, 1)
 
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t q_tiles = smem_u32(base), k_tiles = q_tiles + kTiles * C::kOperand, v_tiles = k_tiles + 2 * C::kOperand;
-  uint8_t* packed = base + (kTiles + 4) * C::kOperand;  // two slots of keys, two of values
+  uint8_t* packed = base + (kTiles + 4) * C::kOperand;
   if (warp < C::kSoftWarps) {
-    const int tile = warp >> 2;
+    const int tile = warp >> 3;
     if (tile < active) {
-      softmax_rows<D, kTiles, kCap, kBias>(p, sh, tiles, k0, n, rows, h, tile, q_tiles, tmem, split, warp & 3, lane);
+      softmax_rows<D, kTiles, kCap, kBias>(p, sh, tiles, k0, n, rows, h, tile, q_tiles, tmem, split, warp & 7, lane);
     } else {
       asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftWarps * 32 + 32) : "memory");
     }
@@ -514,7 +528,7 @@ __global__ void __launch_bounds__(Cfg<D, kTiles>::kThreads, 1)
       if (warp < C::kSoftWarps + 4)
         unpack_tiles<D, true>(p, sh, tiles, k0, n, sh.b, sh.len, h, smem_u32(packed), k_tiles, tid);
       else
-        unpack_tiles<D, false>(p, sh, tiles, k0, n, sh.b, sh.len, h, smem_u32(packed) + 2 * C::kPacked, v_tiles, tid);
+        unpack_tiles<D, false>(p, sh, tiles, k0, n, sh.b, sh.len, h, smem_u32(packed), v_tiles, tid);
     }
   } else if (warp == C::kMmaWarp) {
     asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftWarps * 32 + 32) : "memory");

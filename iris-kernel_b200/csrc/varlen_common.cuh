@@ -226,32 +226,33 @@ IRIS_DEV float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 // 2 6 3 7, as the nibbles of a word come apart (stored keys have it too, so
 // products do not change).  A row with a value that is not finite becomes NaN.
 //
-// `words`: a thread's pairs as loaded; `widest` takes the largest magnitude's
-// bits over the threads that share the row.  Returns the factor that undoes the power.
-template <int kWords, typename F>
-IRIS_DEV float scale_row_part(uint32_t (&words)[kWords], bool bf16, F&& widest) {
-  uint32_t most = 0;  // of either type
-#pragma unroll
-  for (int i = 0; i < kWords; ++i) {
-    const uint32_t w = words[i] & 0x7fff7fffu;
-    most = max(most, max(w & 0xffffu, w >> 16));
-  }
-  most = widest(most);
+// The larger magnitude's bits of a pair, of either type.
+IRIS_DEV uint32_t pair_size(uint32_t w) { return max(w & 0x7fffu, (w >> 16) & 0x7fffu); }
+// From a row's largest magnitude's bits: the power to scale by (NaN: not finite), and what undoes it.
+IRIS_DEV float row_power(uint32_t most, bool bf16, float* up) {
   const bool finite = most < (bf16 ? 0x7f80u : 0x7c00u);
   const float top = bf16 ? __uint_as_float(most << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(most)));
   int e = 15;
   if (finite && top > 0.0f) e = max(static_cast<int>((__float_as_uint(top) >> 23) & 255) - 127, -110);
-  const float up = pow2i(15 - e);
-#pragma unroll
-  for (int i = 0; i < kWords; ++i) {
-    const float2 v = bf16 ? Bf16Elem::unpack(words[i]) : Fp16Elem::unpack(words[i]);
-    words[i] = finite ? Fp16Elem::pack(v.x * up, v.y * up) : 0x7fff7fffu;
-  }
+  *up = finite ? pow2i(15 - e) : __int_as_float(0x7fffffff);
   return pow2i(e - 15);
 }
-template <int kWords>
-IRIS_DEV float scale_row(uint32_t (&words)[kWords], bool bf16) {
-  return scale_row_part(words, bf16, [](uint32_t m) { return m; });
+IRIS_DEV uint32_t scale_pair(uint32_t w, bool bf16, float up) {
+  const float2 v = bf16 ? Bf16Elem::unpack(w) : Fp16Elem::unpack(w);
+  return Fp16Elem::pack(v.x * up, v.y * up);
+}
+// `words`: a thread's pairs as loaded; `widest` takes the largest magnitude's
+// bits over the threads that share the row.  Returns the factor that undoes the power.
+template <int kWords, typename F>
+IRIS_DEV float scale_row_part(uint32_t (&words)[kWords], bool bf16, F&& widest) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) most = max(most, pair_size(words[i]));
+  float up;
+  const float back = row_power(widest(most), bf16, &up);
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) words[i] = scale_pair(words[i], bf16, up);
+  return back;
 }
 
 // Eight dims (four pairs as loaded) in the order above.
