@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(128) attention_mass_kernel(const MassParams p)
   grid_dependents_launch();
   if (blockIdx.x == 0 && warp == 0) check_offsets(p.s, lane);
   const Span sp = new_tokens(p.s, b);
-  const int len = cached_tokens(p.s, b, sp.count, tid == 0 && h == 0 && chunk == 0);
+  const int len = cached_tokens(p.s, __ldg(p.s.seq_lens + b), sp.count, tid == 0 && h == 0 && chunk == 0);
   const int tiles = (len + kTile - 1) / kTile;
   const int k0 = chunk * p.per, n = min(p.per, tiles - k0);
   if (n <= 0) return;

@@ -237,23 +237,34 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
     const int32_t prefix = p.s.prefix_lens != nullptr ? __ldg(p.s.prefix_lens + sh.b) : 0;
     const int32_t first = p.s.first_visible != nullptr ? __ldg(p.s.first_visible + token) : 0;
     sight = row_sight(pos, first, prefix, p.s.window, sh.len);
-    if (n > 0 && half == 0) {
-      const uint4* src = reinterpret_cast<const uint4*>(p.query + token * p.q_stride + static_cast<int64_t>(head) * D);
-      uint32_t most = 0;
-#pragma unroll 4
-      for (int c = 0; c < D / 8; ++c) {
+  }
+  if (n > 0) {  // the tile's query rows: four threads a row, 64 rows at a time
+    constexpr int kWords = D / 8;
+#pragma unroll
+    for (int r0 = 0; r0 < kTile; r0 += 64) {
+      const int row = r0 + (warp * 32 + lane) / 4, part = lane & 3;
+      const int rr = min(sh.index * (kTile * kTiles) + tile * kTile + row, rows - 1);
+      const int64_t at = (sh.start + rr / p.s.group) * p.q_stride + static_cast<int64_t>(h * p.s.group + rr % p.s.group) * D;
+      const uint4* src = reinterpret_cast<const uint4*>(p.query + at + part * (D / 4));
+      uint32_t w[kWords];
+#pragma unroll
+      for (int c = 0; c < kWords / 4; ++c) {
         const uint4 v = src[c];
-        most = max(max(most, pair_size(v.x)), max(max(pair_size(v.y), pair_size(v.z)), pair_size(v.w)));
+        w[4 * c] = v.x;
+        w[4 * c + 1] = v.y;
+        w[4 * c + 2] = v.z;
+        w[4 * c + 3] = v.w;
       }
-      float up;
-      sh.back[tile][local] = row_power(most, p.bf16 != 0, &up);
+      const float undo = scale_row_part<kWords>(w, p.bf16 != 0, [](uint32_t m) {
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      });
+      if (part == 0) sh.back[tile][row] = undo;
       const uint32_t dst = q_tiles + tile * C::kOperand;
-#pragma unroll 4
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 v = src[c];
-        v = order8(scale_pair(v.x, p.bf16 != 0, up), scale_pair(v.y, p.bf16 != 0, up), scale_pair(v.z, p.bf16 != 0, up),
-                   scale_pair(v.w, p.bf16 != 0, up));
-        sts128(dst + operand_at(local, c), v.x, v.y, v.z, v.w);
+#pragma unroll
+      for (int c = 0; c < kWords / 4; ++c) {
+        const uint4 v = order8(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+        sts128(dst + operand_at(row, part * (D / 32) + c), v.x, v.y, v.z, v.w);
       }
     }
   }
@@ -293,13 +304,16 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
         float s[32];
         load_scores(s_at + 32 * c, s);
         if (kMod) {
-          const float d0 = static_cast<float>(pos - base - 32 * c);
+          if (kCap) {
+            cap_logits(s, f[c], cap2);
+          } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            float y = s[j] * f[c];
-            if (kCap) y = cap2 * tanh_f(y);
-            if (kBias) y = fmaf(slope2, fabsf(d0 - j), y);
-            s[j] = y;
+            for (int j = 0; j < 32; ++j) s[j] *= f[c];
+          }
+          if (kBias) {
+            const float d0 = static_cast<float>(pos - base - 32 * c);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s[j] = fmaf(slope2, fabsf(d0 - j), s[j]);
           }
         }
         if (masked) {
@@ -473,14 +487,14 @@ __global__ void __launch_bounds__(Cfg<D, kTiles>::kThreads, 1)
   grid_dependents_launch();
   if (warp == 0) {
     if (blockIdx.x == 0) check_offsets(p.s, lane);
-    Block blk = {0, 0};
+    Block blk = {0, 0, {0, 0}, 0};
     const bool live = find_block(p.s, unit, kTile * kTiles, p.few ? kFewRows : 0, INT64_MAX, lane, &blk);
     int first = 0;
     Span sp = {0, 0};
     int32_t len = 0;
     if (live) {
-      sp = new_tokens(p.s, blk.b);
-      len = cached_tokens(p.s, blk.b, sp.count, lane == 0 && h == 0 && split == 0 && blk.index == 0);
+      sp = blk.span;
+      len = cached_tokens(p.s, blk.len, sp.count, lane == 0 && h == 0 && split == 0 && blk.index == 0);
       first = first_of_block(p.s, sp, blk.index, kTile * kTiles, lane);
     }
     if (lane == 0) {

@@ -81,9 +81,8 @@ IRIS_DEV int32_t used_rows(const VarlenBatch& p) {
   return p.cu == nullptr ? min(p.batch, p.tokens) : min(max(__ldg(p.cu + p.batch), 0), p.tokens);
 }
 
-// Length of sequence b in the cache, as far as its pages go; `say` reports what is wrong with it.
-IRIS_DEV int32_t cached_tokens(const VarlenBatch& p, int b, int32_t count, bool say) {
-  int32_t n = __ldg(p.seq_lens + b);
+// A sequence's length n in the cache, as far as its pages go; `say` reports what is wrong with it.
+IRIS_DEV int32_t cached_tokens(const VarlenBatch& p, int32_t n, int32_t count, bool say) {
   if (n < 0) {
     if (say) set_error(p.err, IRIS_ERR_SEQ_NEGATIVE);
     return 0;
@@ -105,14 +104,75 @@ IRIS_DEV int warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
 // a sequence the rows are the host's to choose a kernel by, and all are taken.)
 struct Block {
   int32_t b, index;
+  Span span;
+  int32_t len;  // as the sequence's length stands, not checked
 };
+
+// Up to 32 * kHeld sequences: a lane has kHeld of them in registers (one trip to
+// memory; the search that asked memory again at each step took 7000 cycles).
+constexpr int kHeld = 4;
+IRIS_DEV bool find_held_block(const VarlenBatch& p, int u, int rows, int64_t over, int64_t most_rows, int lane, Block* out) {
+  int32_t start[kHeld], count[kHeld], len[kHeld], n[kHeld];
+  int most = 0;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int b = lane + 32 * i;
+    start[i] = count[i] = len[i] = 0;
+    if (b < p.batch) {
+      const Span s = new_tokens(p, b);
+      start[i] = s.start;
+      count[i] = s.count;
+      len[i] = __ldg(p.seq_lens + b);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int64_t r = static_cast<int64_t>(count[i]) * p.group;
+    n[i] = r > over && r <= most_rows ? static_cast<int32_t>((r + rows - 1) / rows) : 0;
+    most = max(most, n[i]);
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  auto upto = [&](int depth) {  // blocks among the last `depth` of every sequence
+    int x = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) x += min(depth, n[i]);
+    return warp_sum(x);
+  };
+  if (u >= upto(most)) return false;
+  int lo = 0, hi = most, before = 0;  // upto(lo) = before <= u < upto(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1, x = upto(mid);
+    if (x <= u) lo = mid, before = x; else hi = mid;
+  }
+  int left = u - before;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const unsigned has = __ballot_sync(0xffffffffu, n[i] > lo);
+    const int c = __popc(has);
+    if (left >= 0 && left < c) {
+      const int src = __fns(has, 0, left + 1);
+      out->b = src + 32 * i;
+      out->index = __shfl_sync(0xffffffffu, n[i], src) - 1 - lo;
+      out->span = {__shfl_sync(0xffffffffu, start[i], src), __shfl_sync(0xffffffffu, count[i], src)};
+      out->len = __shfl_sync(0xffffffffu, len[i], src);
+      return true;
+    }
+    left -= c;
+  }
+  return false;
+}
+
 IRIS_DEV bool find_block(const VarlenBatch& p, int u, int rows, int64_t over, int64_t most_rows, int lane, Block* out) {
   if (p.cu == nullptr) {
     const int per = (p.group + rows - 1) / rows;
     out->b = u / per;
     out->index = u % per;
-    return out->b < p.batch;
+    if (out->b >= p.batch) return false;
+    out->span = {out->b, 1};
+    out->len = __ldg(p.seq_lens + out->b);
+    return true;
   }
+  if (p.batch <= 32 * kHeld) return find_held_block(p, u, rows, over, most_rows, lane, out);
   auto blocks = [&](int b) {
     const int64_t n = static_cast<int64_t>(new_tokens(p, b).count) * p.group;
     return n > over && n <= most_rows ? static_cast<int32_t>((n + rows - 1) / rows) : 0;
@@ -120,7 +180,7 @@ IRIS_DEV bool find_block(const VarlenBatch& p, int u, int rows, int64_t over, in
   int most = 0;
   for (int b = lane; b < p.batch; b += 32) most = max(most, blocks(b));
   most = __reduce_max_sync(0xffffffffu, most);
-  auto upto = [&](int depth) {  // blocks among the last `depth` of every sequence
+  auto upto = [&](int depth) {
     int n = 0;
     for (int b = lane; b < p.batch; b += 32) n += min(depth, blocks(b));
     return warp_sum(n);
@@ -141,6 +201,8 @@ IRIS_DEV bool find_block(const VarlenBatch& p, int u, int rows, int64_t over, in
       const int src = __fns(has, 0, left + 1);
       out->b = base + src;
       out->index = __shfl_sync(0xffffffffu, n, src) - 1 - lo;
+      out->span = new_tokens(p, out->b);
+      out->len = __ldg(p.seq_lens + out->b);
       return true;
     }
     left -= c;
@@ -206,14 +268,48 @@ IRIS_DEV Tiles tiles_seen(int32_t pos_lo, int32_t pos_hi, int32_t first, int32_t
 }
 
 // tanh, within a few units in the last place of 1 anywhere and relatively near
-// 0: 1 - 2 / (1 + e^2x) (right at both infinities), or its series (to x^9; the
-// next term is 6e-8 of the sum at 0.3) where that would cancel.
+// 0: 1 - 2 / (1 + e^2x) (right at both infinities), or, where that would cancel, x
+// times a polynomial in x^2 (Chebyshev's of degree 5 over |x| <= 0.6: 3e-9).
+constexpr float kTanhNear = 0.6f;
+IRIS_DEV float2 tanh_near(float2 x) {
+  const float2 q = __fmul2_rn(x, x);
+  float2 r = make_float2(-0.00585643f, -0.00585643f);
+  r = __ffma2_rn(r, q, make_float2(0.02075748f, 0.02075748f));
+  r = __ffma2_rn(r, q, make_float2(-0.05376992f, -0.05376992f));
+  r = __ffma2_rn(r, q, make_float2(0.13331705f, 0.13331705f));
+  r = __ffma2_rn(r, q, make_float2(-0.33333284f, -0.33333284f));
+  r = __ffma2_rn(r, q, make_float2(1.0f, 1.0f));
+  return __fmul2_rn(x, r);
+}
 IRIS_DEV float tanh_f(float x) {
   const float t = ex2(2.0f * kLog2e * x);
-  const float big = fmaf(-2.0f, rcp(1.0f + t), 1.0f);
-  const float q = x * x;
-  const float r = fmaf(q, fmaf(q, fmaf(q, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f);
-  return fabsf(x) < 0.3f ? fmaf(x * q, r, x) : big;
+  const float far = fmaf(-2.0f, rcp(1.0f + t), 1.0f);
+  return fabsf(x) < kTanhNear ? tanh_near(make_float2(x, x)).x : far;
+}
+// s = cap2 * tanh(s * f), by a whole warp.  Logits mostly lie well inside a cap,
+// and then the polynomial alone does: no exponential and no reciprocal, whose
+// unit (16 a cycle and SM) would bound the kernel.
+template <int N>
+IRIS_DEV void cap_logits(float (&s)[N], float f, float cap2) {
+  float most = 0.0f;
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    const float2 x = __fmul2_rn(make_float2(s[j], s[j + 1]), make_float2(f, f));
+    s[j] = x.x;
+    s[j + 1] = x.y;
+    most = fmaxf(most, fmaxf(fabsf(x.x), fabsf(x.y)));
+  }
+  if (__any_sync(0xffffffffu, most >= kTanhNear)) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) s[j] = cap2 * tanh_f(s[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const float2 y = __fmul2_rn(tanh_near(make_float2(s[j], s[j + 1])), make_float2(cap2, cap2));
+      s[j] = y.x;
+      s[j + 1] = y.y;
+    }
+  }
 }
 
 // Two's power as fp32, |e| < 127.

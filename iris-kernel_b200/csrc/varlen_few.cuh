@@ -144,14 +144,14 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
   grid_dependents_launch();
   if (threadIdx.x < 32) {
     if (blockIdx.x == 0) check_offsets(p.s, lane);
-    Block blk = {0, 0};
+    Block blk = {0, 0, {0, 0}, 0};
     const bool live = find_block(p.s, unit, kCols, 0, kFewRows, lane, &blk);
     int first = 0;
     Span sp = {0, 0};
     int32_t len = 0;
     if (live) {
-      sp = new_tokens(p.s, blk.b);
-      len = cached_tokens(p.s, blk.b, sp.count, lane == 0 && h == 0 && chunk == 0 && blk.index == 0);
+      sp = blk.span;
+      len = cached_tokens(p.s, blk.len, sp.count, lane == 0 && h == 0 && chunk == 0 && blk.index == 0);
       first = first_of_block(p.s, sp, blk.index, kCols, lane);
     }
     if (lane == 0) {
@@ -380,25 +380,28 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
 #pragma unroll
         for (int g = 0; g < C::kSums; ++g) umma_ld<kStep>(lanes + s_at + g * kN + c0, v[g]);
         umma_wait_ld();
+        float x[kStep];
 #pragma unroll
         for (int i = 0; i < kStep; ++i) {
-          const int c = c0 + i;
-          float x = 0.0f;
+          x[i] = 0.0f;
 #pragma unroll
           for (int g = 0; g < C::kSums; ++g) {
             asm volatile("" : "+r"(v[g][i]));
-            x = fmaf(__uint_as_float(v[g][i]), sc[g], x);
+            x[i] = fmaf(__uint_as_float(v[g][i]), sc[g], x[i]);
           }
-          const float4 f = sh.row[c];
-          x *= f.x;
-          if (kCap) x = cap2 * tanh_f(x);
-          if (kBias) x = fmaf(sh.more[c].y, fabsf(static_cast<float>(__float_as_int(sh.more[c].x) - j)), x);
+          x[i] *= sh.row[c0 + i].x;
+        }
+        if (kCap) cap_logits(x, 1.0f, cap2);
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) {
+          const int c = c0 + i;
+          if (kBias) x[i] = fmaf(sh.more[c].y, fabsf(static_cast<float>(__float_as_int(sh.more[c].x) - j)), x[i]);
           if (!full) {
             const int4 z = sh.sight[c];
-            if (!((j >= z.x && j < z.y) || (j >= z.z && j < z.w))) x = kMinusInf;
+            if (!((j >= z.x && j < z.y) || (j >= z.z && j < z.w))) x[i] = kMinusInf;
           }
-          y[c] = x;
-          rise |= x > f.z;
+          y[c] = x[i];
+          rise |= x[i] > sh.row[c].z;
         }
       }
       if (group_or<1>(rise || !ok)) {
