@@ -7,8 +7,8 @@
 //   * softmax warps, two threads a row (64 columns each), eight warps a row tile:
 //     scores from tensor memory, mask, cap and bias, running maximum and sum in
 //     registers, probabilities back to tensor memory as the next product's operand;
-//   * eight unpacking warps, a cached token a thread, four for keys and four for
-//     values: packed rows (TMA) and scales become swizzled fp16 tiles;
+//   * four or eight unpacking warps, a cached token a thread: packed rows (TMA)
+//     and scales become swizzled fp16 tiles;
 //   * one warp that issues the products: S = Q K^T (both operands in shared
 //     memory, K-major) and O += P V (P in tensor memory, V as it lies, MN-major);
 //   * one warp that issues the copies.
@@ -37,8 +37,11 @@ struct Cfg {
   static constexpr int kColumns = kTiles == 2 ? 512 : 256;
   static constexpr int kOutColumn = kTiles * kTile;    // first column of O
   static constexpr int kSoftWarps = 8 * kTiles;
-  static constexpr int kMmaWarp = kSoftWarps + 8, kCopyWarp = kMmaWarp + 1;
-  static constexpr int kThreads = 32 * (kCopyWarp + 1);
+  static constexpr int kMmaWarp = kSoftWarps + (kTiles == 2 ? 4 : 8), kCopyWarp = kMmaWarp + 1;
+  static constexpr int kThreads = 32 * (kMmaWarp + 4);  // (two warps idle: registers move by warpgroups)
+  // Registers a thread: launched with 80 (kTiles 2: 768 x 80 = 61,440) or 96 (640 x 96 = 61,440), then shared out as
+  // 512 x 96 + 128 x 64 + 128 x 32 = 61,440 or 256 x 136 + 256 x 72 + 128 x 56 = 60,416.
+  static constexpr int kSoftRegs = kTiles == 2 ? 96 : 136, kUnpackRegs = kTiles == 2 ? 64 : 72, kIssueRegs = kTiles == 2 ? 32 : 56;
 };
 
 struct Shared {
@@ -58,79 +61,95 @@ struct Shared {
 };
 
 // ------------------------------------------------------------------ unpacking
-template <int D, bool kKeys>
-IRIS_DEV void unpack_tiles(const AttendParams& p, Shared& sh, const Tiles& tiles, int k0, int n, int b, int len, int h,
-                           uint32_t packed, uint32_t operands, int tid) {
+// One tile of keys or values, with its scales.  False: a wait gave up.
+template <int D, bool keys>
+IRIS_DEV bool unpack_tile(const AttendParams& p, Shared& sh, int k, const uint32_t (&sc)[D / 64], uint32_t packed,
+                        uint32_t operands, int tid) {
   using C = Cfg<D, 1>;
   constexpr int kGroups = D / 32;
   const int warp = tid >> 5, lane = tid & 31;
-  const uint8_t* scales = kKeys ? p.k_scale : p.v_scale;
+  const int st = k & 1, slot = keys ? st : 2;
+  // what the run of 32 tokens is scaled by, and what is not finite
+  uint32_t most = 0, bad = 0, s2[kGroups];
+#pragma unroll
+  for (int c = 0; c < kGroups; ++c) {
+    s2[c] = (sc[c / 2] >> (16 * (c & 1))) & 0xffffu;
+    const uint32_t mag = s2[c] & 0x7fffu;
+    if (mag >= 0x7c00u) bad |= 1u << c; else most = max(most, mag);
+  }
+  const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 10);
+  const float up = pow2i(27 - e);
+#pragma unroll
+  for (int c = 0; c < kGroups; ++c) {  // the scale twice, as fp16
+    const float v = __half2float(__ushort_as_half(static_cast<unsigned short>(s2[c]))) * up;
+    s2[c] = (bad >> c) & 1u ? (keys ? 0x7fff7fffu : 0u) : Fp16Elem::pack(v, v);
+  }
+  if (!wait_all(&sh.raw_full[slot], keys ? (k >> 1) & 1 : k & 1, p.s.err)) return false;
+  if (!wait_all(keys ? &sh.k_empty[st] : &sh.v_empty[st], ((k >> 1) & 1) ^ 1, p.s.err)) return false;
+  if (keys) {
+    if (lane == 0) sh.k_exp[k & 3][warp] = e - 27;
+  } else {
+    const bool any = __any_sync(0xffffffffu, bad != 0);
+    if (lane == 0) {
+      sh.v_exp[k & 3][warp] = e - 27;
+      sh.v_any[st][warp] = any;
+    }
+    if (any) sh.v_bad[st][tid] = static_cast<uint8_t>(bad);
+  }
+  const uint32_t src = packed + slot * C::kPacked, dst = operands + st * C::kOperand;
+#pragma unroll
+  for (int c = 0; c < kGroups; ++c) {
+    const uint4 w4 = lds128(src + packed_at<D>(tid, c));
+    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+    const __half2 s = u32_as_h2(s2[c]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = w[i], hi = w[i] >> 8;
+      sts128(dst + operand_at(tid, 4 * c + i), h2_as_u32(__hmul2(u32_as_h2(int4_lo_exact(lo)), s)),
+             h2_as_u32(__hmul2(u32_as_h2(int4_hi_exact(lo)), s)), h2_as_u32(__hmul2(u32_as_h2(int4_lo_exact(hi)), s)),
+             h2_as_u32(__hmul2(u32_as_h2(int4_hi_exact(hi)), s)));
+    }
+  }
+  fence_proxy_async_shared();
+  mbar_arrive(keys ? &sh.k_full[st] : &sh.v_full[st]);
+  mbar_arrive(&sh.raw_empty[slot]);
+  return true;
+  }
+
+// kKeys, kValues: what this warpgroup unpacks (both: in turn).
+template <int D, bool kKeys, bool kValues>
+IRIS_DEV void unpack_tiles(const AttendParams& p, Shared& sh, const Tiles& tiles, int k0, int n, int b, int len, int h,
+                           uint32_t packed, uint32_t k_tiles, uint32_t v_tiles, int tid) {
+  constexpr int kGroups = D / 32;
   auto token = [&](int k) { return tiles.at(k0 + k) * kTile + tid; };
-  uint32_t sc2[kGroups / 2];  // the scales of the tile that is next
-  auto fetch = [&](int32_t page, int32_t j) {
+  uint32_t sc2[2][kGroups / 2];  // the scales of the tile that is next
+  auto fetch = [&](const uint8_t* scales, int32_t page, int32_t j, uint32_t (&s)[kGroups / 2]) {
     const uint8_t* x = scales + ((static_cast<int64_t>(page) * kTokPage + (j & (kTokPage - 1))) * p.s.hkv + h) * (D / 16);
     if constexpr (D == 128) {
       const uint2 v = j < len ? __ldg(reinterpret_cast<const uint2*>(x)) : make_uint2(0, 0);
-      sc2[0] = v.x;
-      sc2[1] = v.y;
+      s[0] = v.x;
+      s[1] = v.y;
     } else {
-      sc2[0] = j < len ? __ldg(reinterpret_cast<const uint32_t*>(x)) : 0u;
+      s[0] = j < len ? __ldg(reinterpret_cast<const uint32_t*>(x)) : 0u;
     }
   };
-  fetch(page_of(p.s, b, token(0), len), token(0));
-  int32_t page = n > 1 ? raw_page(p.s, b, token(1), len) : 0;
+  int32_t page = page_of(p.s, b, token(0), len);
+  if (kKeys) fetch(p.k_scale, page, token(0), sc2[0]);
+  if (kValues) fetch(p.v_scale, page, token(0), sc2[1]);
+  page = n > 1 ? raw_page(p.s, b, token(1), len) : 0;
 #pragma unroll 1
   for (int k = 0; k < n; ++k) {
-    const int st = k & 1;
-    // what the run of 32 tokens is scaled by, and what is not finite
-    uint32_t most = 0, bad = 0, s2[kGroups];
+    uint32_t now[2][kGroups / 2];
 #pragma unroll
-    for (int c = 0; c < kGroups; ++c) {
-      s2[c] = (sc2[c / 2] >> (16 * (c & 1))) & 0xffffu;
-      const uint32_t mag = s2[c] & 0x7fffu;
-      if (mag >= 0x7c00u) bad |= 1u << c; else most = max(most, mag);
-    }
-    const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 10);
-    const float up = pow2i(27 - e);
-#pragma unroll
-    for (int c = 0; c < kGroups; ++c) {  // the scale twice, as fp16
-      const float v = __half2float(__ushort_as_half(static_cast<unsigned short>(s2[c]))) * up;
-      s2[c] = (bad >> c) & 1u ? (kKeys ? 0x7fff7fffu : 0u) : Fp16Elem::pack(v, v);
-    }
+    for (int i = 0; i < kGroups / 2; ++i) now[0][i] = sc2[0][i], now[1][i] = sc2[1][i];
     if (k + 1 < n) {
-      fetch(checked_page(p.s, page), token(k + 1));
+      const int32_t id = checked_page(p.s, page);
+      if (kKeys) fetch(p.k_scale, id, token(k + 1), sc2[0]);
+      if (kValues) fetch(p.v_scale, id, token(k + 1), sc2[1]);
       if (k + 2 < n) page = raw_page(p.s, b, token(k + 2), len);
     }
-    const int slot = kKeys ? st : 2;
-    if (!wait_all(&sh.raw_full[slot], kKeys ? (k >> 1) & 1 : k & 1, p.s.err)) break;
-    if (!wait_all(kKeys ? &sh.k_empty[st] : &sh.v_empty[st], ((k >> 1) & 1) ^ 1, p.s.err)) break;
-    if (kKeys) {
-      if (lane == 0) sh.k_exp[k & 3][warp] = e - 27;
-    } else {
-      const bool any = __any_sync(0xffffffffu, bad != 0);
-      if (lane == 0) {
-        sh.v_exp[k & 3][warp] = e - 27;
-        sh.v_any[st][warp] = any;
-      }
-      if (any) sh.v_bad[st][tid] = static_cast<uint8_t>(bad);
-    }
-    const uint32_t src = packed + slot * C::kPacked, dst = operands + st * C::kOperand;
-#pragma unroll
-    for (int c = 0; c < kGroups; ++c) {
-      const uint4 w4 = lds128(src + packed_at<D>(tid, c));
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-      const __half2 s = u32_as_h2(s2[c]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = w[i], hi = w[i] >> 8;
-        sts128(dst + operand_at(tid, 4 * c + i), h2_as_u32(__hmul2(u32_as_h2(int4_lo_exact(lo)), s)),
-               h2_as_u32(__hmul2(u32_as_h2(int4_hi_exact(lo)), s)), h2_as_u32(__hmul2(u32_as_h2(int4_lo_exact(hi)), s)),
-               h2_as_u32(__hmul2(u32_as_h2(int4_hi_exact(hi)), s)));
-      }
-    }
-    fence_proxy_async_shared();
-    mbar_arrive(kKeys ? &sh.k_full[st] : &sh.v_full[st]);
-    mbar_arrive(&sh.raw_empty[slot]);
+    if (kKeys && !unpack_tile<D, true>(p, sh, k, now[0], packed, k_tiles, tid)) break;
+    if (kValues && !unpack_tile<D, false>(p, sh, k, now[1], packed, v_tiles, tid)) break;
   }
 }
 
@@ -304,11 +323,23 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
         float s[32];
         load_scores(s_at + 32 * c, s);
         if (kMod) {
-          if (kCap) {
-            cap_logits(s, f[c], cap2);
-          } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) s[j] *= f[c];
+          for (int j = 0; j < 32; ++j) s[j] *= f[c];
+          if (kCap && !cap_near(s, cap2)) {  // 16 at a time, through tensor memory: there are no registers for more
+#pragma unroll 1
+            for (int q = 0; q < 32; q += 16) {
+              float x[16];
+              umma_ld16(s_at + 32 * c + q, reinterpret_cast<uint32_t*>(x));
+              umma_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                asm volatile("" : "+f"(x[j]));
+                x[j] = cap2 * tanh_f(x[j] * f[c]);
+              }
+              umma_st16(s_at + 32 * c + q, reinterpret_cast<const uint32_t*>(x));
+            }
+            umma_wait_st();
+            load_scores(s_at + 32 * c, s);
           }
           if (kBias) {
             const float d0 = static_cast<float>(pos - base - 32 * c);
@@ -530,6 +561,7 @@ __global__ void __launch_bounds__(Cfg<D, kTiles>::kThreads, 1)
   const uint32_t q_tiles = smem_u32(base), k_tiles = q_tiles + kTiles * C::kOperand, v_tiles = k_tiles + 2 * C::kOperand;
   uint8_t* packed = base + (kTiles + 4) * C::kOperand;
   if (warp < C::kSoftWarps) {
+    regs_take<C::kSoftRegs>();
     const int tile = warp >> 3;
     if (tile < active) {
       softmax_rows<D, kTiles, kCap, kBias>(p, sh, tiles, k0, n, rows, h, tile, q_tiles, tmem, split, warp & 7, lane);
@@ -537,18 +569,25 @@ __global__ void __launch_bounds__(Cfg<D, kTiles>::kThreads, 1)
       asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftWarps * 32 + 32) : "memory");
     }
   } else if (warp < C::kMmaWarp) {
+    regs_give<C::kUnpackRegs>();
     const int tid = (threadIdx.x - C::kSoftWarps * 32) & 127;
     if (n > 0) {
-      if (warp < C::kSoftWarps + 4)
-        unpack_tiles<D, true>(p, sh, tiles, k0, n, sh.b, sh.len, h, smem_u32(packed), k_tiles, tid);
+      const uint32_t raw = smem_u32(packed);
+      if (kTiles == 2)
+        unpack_tiles<D, true, true>(p, sh, tiles, k0, n, sh.b, sh.len, h, raw, k_tiles, v_tiles, tid);
+      else if (warp < C::kSoftWarps + 4)
+        unpack_tiles<D, true, false>(p, sh, tiles, k0, n, sh.b, sh.len, h, raw, k_tiles, v_tiles, tid);
       else
-        unpack_tiles<D, false>(p, sh, tiles, k0, n, sh.b, sh.len, h, smem_u32(packed), v_tiles, tid);
+        unpack_tiles<D, false, true>(p, sh, tiles, k0, n, sh.b, sh.len, h, raw, k_tiles, v_tiles, tid);
     }
-  } else if (warp == C::kMmaWarp) {
-    asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftWarps * 32 + 32) : "memory");
-    if (n > 0) issue_products<D, kTiles>(p, sh, n, active, q_tiles, k_tiles, v_tiles, tmem);
-  } else if (n > 0) {
-    issue_copies<D>(p, &k_map, &v_map, sh, tiles, k0, n, sh.b, sh.len, h, packed, lane);
+  } else {
+    regs_give<C::kIssueRegs>();
+    if (warp == C::kMmaWarp) {
+      asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftWarps * 32 + 32) : "memory");
+      if (n > 0) issue_products<D, kTiles>(p, sh, n, active, q_tiles, k_tiles, v_tiles, tmem);
+    } else if (warp == C::kCopyWarp && n > 0) {
+      issue_copies<D>(p, &k_map, &v_map, sh, tiles, k0, n, sh.b, sh.len, h, packed, lane);
+    }
   }
   umma_fence_before();
   __syncthreads();

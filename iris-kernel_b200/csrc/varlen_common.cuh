@@ -286,30 +286,23 @@ IRIS_DEV float tanh_f(float x) {
   const float far = fmaf(-2.0f, rcp(1.0f + t), 1.0f);
   return fabsf(x) < kTanhNear ? tanh_near(make_float2(x, x)).x : far;
 }
-// s = cap2 * tanh(s * f), by a whole warp.  Logits mostly lie well inside a cap,
-// and then the polynomial alone does: no exponential and no reciprocal, whose
-// unit (16 a cycle and SM) would bound the kernel.
+// s = cap2 * tanh(s), by a whole warp; false: some lie too far out for the
+// polynomial, and s is as it was.  Logits mostly lie well inside a cap, and then
+// no exponential and no reciprocal is needed, whose unit (16 a cycle and SM) would
+// bound the kernel.
 template <int N>
-IRIS_DEV void cap_logits(float (&s)[N], float f, float cap2) {
+IRIS_DEV bool cap_near(float (&s)[N], float cap2) {
   float most = 0.0f;
 #pragma unroll
+  for (int j = 0; j < N; ++j) most = fmaxf(most, fabsf(s[j]));
+  if (__any_sync(0xffffffffu, most >= kTanhNear)) return false;
+#pragma unroll
   for (int j = 0; j < N; j += 2) {
-    const float2 x = __fmul2_rn(make_float2(s[j], s[j + 1]), make_float2(f, f));
-    s[j] = x.x;
-    s[j + 1] = x.y;
-    most = fmaxf(most, fmaxf(fabsf(x.x), fabsf(x.y)));
+    const float2 y = __fmul2_rn(tanh_near(make_float2(s[j], s[j + 1])), make_float2(cap2, cap2));
+    s[j] = y.x;
+    s[j + 1] = y.y;
   }
-  if (__any_sync(0xffffffffu, most >= kTanhNear)) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) s[j] = cap2 * tanh_f(s[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; j += 2) {
-      const float2 y = __fmul2_rn(tanh_near(make_float2(s[j], s[j + 1])), make_float2(cap2, cap2));
-      s[j] = y.x;
-      s[j + 1] = y.y;
-    }
-  }
+  return true;
 }
 
 // Two's power as fp32, |e| < 127.

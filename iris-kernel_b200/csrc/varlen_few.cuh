@@ -391,7 +391,10 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
           }
           x[i] *= sh.row[c0 + i].x;
         }
-        if (kCap) cap_logits(x, 1.0f, cap2);
+        if (kCap && !cap_near(x, cap2)) {
+#pragma unroll
+          for (int i = 0; i < kStep; ++i) x[i] = cap2 * tanh_f(x[i]);
+        }
 #pragma unroll
         for (int i = 0; i < kStep; ++i) {
           const int c = c0 + i;
