@@ -758,6 +758,7 @@ PyObject* evict(PyObject* const* a) {
           "packed cache shape does not match page_size");
   check_cache(c, kd, vd, ks, vs, device);
   check("mass", mass, {c.num_pages, c.heads, 16}, at::kFloat, device);
+  require(reinterpret_cast<uintptr_t>(ptr(mass)) % 16 == 0, PyExc_ValueError, "mass must start on a 16-byte boundary");
   require(bt.dim() == 2, PyExc_ValueError, "block_table must have shape [B, max_pages_per_sequence]");
   const int64_t batch = bt.size(0);
   const Table table = block_table(bt, batch, device);

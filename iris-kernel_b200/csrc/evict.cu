@@ -49,7 +49,7 @@ IRIS_DEV uint32_t weight_key(float w) {
 }
 
 struct EvictShared {
-  uint32_t bins[3][kBins];
+  alignas(16) uint32_t bins[3][kBins];
   int32_t warp_sums[kEvictWarps];
   int32_t equal, moving, holes;  // of this block's run
   int32_t bad;                   // a page id outside the cache
@@ -126,7 +126,7 @@ IRIS_DEV void write_part(const EvictParams& p, int64_t row, int h, int sub, cons
 }
 
 template <int D>
-__global__ void __launch_bounds__(kEvictThreads, 1) evict_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const EvictParams p) {
   extern __shared__ uint32_t keys[];
   __shared__ EvictShared sh;
   cg::cluster_group cluster = cg::this_cluster();
@@ -190,29 +190,39 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_kernel(const EvictPara
     for (int round = 0; round < 3; ++round) {
       const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, width = round == 2 ? 10 : 11;
       uint32_t* bins = sh.bins[round];
-      for (int j = c0 + tid; j < c1; j += kEvictThreads) {
-        uint32_t key;
-        if (round == 0) {
-          key = weight_key(
-              p.mass[(static_cast<int64_t>(__ldg(table + j / kTokPage)) * p.hkv + h) * kTokPage + j % kTokPage]);
-          if (cached) keys[j - j0] = key;
-        } else {
-          key = key_at(j);
-          if ((key >> (shift + width)) != (low >> (shift + width))) continue;
+      if (round == 0 || !cached) {  // from memory, four tokens a load
+#pragma unroll 4
+        for (int j = j0 + 4 * tid; j < j1; j += 4 * kEvictThreads) {
+          const float4 w = *reinterpret_cast<const float4*>(
+              p.mass + (static_cast<int64_t>(__ldg(table + j / kTokPage)) * p.hkv + h) * kTokPage + j % kTokPage);
+          const uint32_t k4[4] = {weight_key(w.x), weight_key(w.y), weight_key(w.z), weight_key(w.w)};
+          if (cached) *reinterpret_cast<uint4*>(keys + (j - j0)) = make_uint4(k4[0], k4[1], k4[2], k4[3]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (j + i >= c0 && j + i < c1 && (round == 0 || (k4[i] >> (shift + width)) == (low >> (shift + width))))
+              atomicAdd(&bins[(k4[i] >> shift) & ((1u << width) - 1)], 1u);
         }
-        atomicAdd(&bins[(key >> shift) & ((1u << width) - 1)], 1u);
+      } else {
+        for (int j = c0 + tid; j < c1; j += kEvictThreads) {
+          const uint32_t key = keys[j - j0];
+          if ((key >> (shift + width)) == (low >> (shift + width)))
+            atomicAdd(&bins[(key >> shift) & ((1u << width) - 1)], 1u);
+        }
       }
       cluster.sync();
       // from the top bin down: four bins a thread, summed over the cluster
       constexpr int kEach = kBins / kEvictThreads;
-      int n[kEach], mine = 0;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int bin = kBins - 1 - (tid * kEach + i);
-        n[i] = 0;
-        for (int r = 0; r < size; ++r) n[i] += static_cast<int>(cluster.map_shared_rank(bins, r)[bin]);
-        mine += n[i];
+      static_assert(kEach == 4, "a thread's bins are one load");
+      int n[kEach] = {}, mine = 0;
+      for (int r = 0; r < size; ++r) {
+        const uint4 v = reinterpret_cast<const uint4*>(cluster.map_shared_rank(bins, r))[kBins / kEach - 1 - tid];
+        n[0] += static_cast<int>(v.w);
+        n[1] += static_cast<int>(v.z);
+        n[2] += static_cast<int>(v.y);
+        n[3] += static_cast<int>(v.x);
       }
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) mine += n[i];
       int total, above = block_scan(mine, sh.warp_sums, &total);
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
@@ -242,44 +252,51 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_kernel(const EvictPara
   auto chosen = [&](uint32_t key, int equal_rank) { return want > 0 && (key > low || (key == low && equal_rank < ties)); };
   int32_t* moving = p.late + static_cast<int64_t>(pair) * 2 * heavy;
   int32_t* holes = moving + heavy;
-  // twice over the run: the counts first, then the lists at the places the counts of the blocks before give
-  int move_at = 0, hole_at = 0;
+  // twice over the run: the counts first, then the lists at the places the counts of the blocks before give (once where
+  // one sweep is the whole run: what the first time found is still there)
+  const bool once = c1 - c0 <= kEvictThreads * kEach;
+  int move_at = 0, hole_at = 0, both = 0;  // (counts of a sweep: moves below, holes above 16 bits)
+  uint32_t in = 0;
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
-    int equal_at = equal_before, moves = 0, gaps = 0;
+    int equal_at = equal_before, moves = 0, gaps = 0, before_m = 0, before_g = 0;
     for (int s = c0; s < c1; s += kEvictThreads * kEach) {
       const int a = s + tid * kEach, e = min(a + kEach, c1);
-      uint32_t key[kEach];
-      int equals = 0;
+      if (pass == 0 || !once) {
+        uint32_t key[kEach];
+        int equals = 0;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        key[i] = a + i < e && want > 0 ? key_at(a + i) : 0u;
-        equals += a + i < e && key[i] == low && want > 0;
-      }
-      int all_equal, all_moves, all_gaps;
-      int eq = equal_at + block_scan(equals, sh.warp_sums, &all_equal);
-      equal_at += all_equal;
-      int mv = 0, gp = 0;
-      uint32_t in = 0;
+        for (int i = 0; i < kEach; ++i) {
+          key[i] = a + i < e && want > 0 ? key_at(a + i) : 0u;
+          equals += a + i < e && key[i] == low && want > 0;
+        }
+        int all;
+        int eq = equal_at + block_scan(equals, sh.warp_sums, &all);
+        equal_at += all;
+        int mine = 0;
+        in = 0;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        if (a + i >= e) continue;
-        const bool yes = chosen(key[i], eq);
-        eq += key[i] == low && want > 0;
-        in |= static_cast<uint32_t>(yes) << i;
-        mv += yes && a + i >= heavy;
-        gp += !yes && a + i < heavy;
+        for (int i = 0; i < kEach; ++i) {
+          if (a + i >= e) continue;
+          const bool yes = chosen(key[i], eq);
+          eq += key[i] == low && want > 0;
+          in |= static_cast<uint32_t>(yes) << i;
+          mine += (yes && a + i >= heavy) + ((!yes && a + i < heavy) << 16);
+        }
+        both = block_scan(mine, sh.warp_sums, &all);
+        before_m = moves;
+        before_g = gaps;
+        moves += all & 0xffff;
+        gaps += all >> 16;
       }
-      int m = moves + block_scan(mv, sh.warp_sums, &all_moves), g = gaps + block_scan(gp, sh.warp_sums, &all_gaps);
-      moves += all_moves;
-      gaps += all_gaps;
       if (pass == 1) {
+        int m = move_at + before_m + (both & 0xffff), g = hole_at + before_g + (both >> 16);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
           if (a + i >= e) continue;
           const bool yes = (in >> i) & 1u;
-          if (yes && a + i >= heavy) moving[move_at + m++] = a + i;
-          if (!yes && a + i < heavy) holes[hole_at + g++] = a + i;
+          if (yes && a + i >= heavy) moving[m++] = a + i;
+          if (!yes && a + i < heavy) holes[g++] = a + i;
           if (yes && a + i < heavy && kept != nullptr) kept[a + i] = a + i;
         }
       }
@@ -308,14 +325,29 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_kernel(const EvictPara
   // kept tokens from behind into the holes: sources and targets do not meet
   constexpr int kLanes = EvictRow<D>::kLanes, kRows = kEvictThreads / kLanes;
   const int sub = tid % kLanes, unit = rank * kRows + tid / kLanes;
-  for (int i = unit; i < n; i += size * kRows) {
-    const int src = __ldcg(moving + i), dst = __ldcg(holes + i);
-    write_part<D>(p, row_of(dst), h, sub, read_part<D>(p, row_of(src), h, sub));
-    if (sub == 0 && kept != nullptr) kept[dst] = src;
+  constexpr int kDeep = 4;
+#pragma unroll 1
+  for (int i0 = unit; i0 < n; i0 += kDeep * size * kRows) {
+    int src[kDeep], dst[kDeep];
+    Part x[kDeep];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      const int i = i0 + d * size * kRows;
+      src[d] = i < n ? __ldcg(moving + i) : -1;
+      dst[d] = i < n ? __ldcg(holes + i) : 0;
+    }
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d)
+      if (src[d] >= 0) x[d] = read_part<D>(p, row_of(src[d]), h, sub);
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      if (src[d] < 0) continue;
+      write_part<D>(p, row_of(dst[d]), h, sub, x[d]);
+      if (sub == 0 && kept != nullptr) kept[dst[d]] = src[d];
+    }
   }
   // then the recent ones, in steps: all of a step's rows are read before any is written, and a step's targets lie at
   // or before its own sources, so no later step reads what it wrote
-  constexpr int kDeep = 4;
 #pragma unroll 1
   for (int i0 = 0; i0 < recent; i0 += size * kRows * kDeep) {
     cluster.sync();  // what this step overwrites has been read
@@ -385,7 +417,7 @@ extern "C" int iris_b200_int4_paged_evict(void* k_data, void* v_data, void* k_sc
       static_cast<int64_t>(batch) * num_kv_heads > INT32_MAX / 8)
     return IRIS_EUNSUPPORTED;
   if (!aligned_to(k_data, 16) || !aligned_to(v_data, 16) || !aligned_to(k_scale, 8) || !aligned_to(v_scale, 8) ||
-      !aligned_to(mass, 4))
+      !aligned_to(mass, 16))
     return IRIS_EALIGN;
   const size_t need = iris_b200_evict_workspace_bytes(batch, num_kv_heads, budget, recent_tokens);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return IRIS_EWORKSPACE;
