@@ -10,15 +10,18 @@
 // one accumulator a group of 32 dims, and a token's fp32 scales join them
 // afterwards: nothing is rounded but the fp32 sums.
 //
-// A block is 128 threads that take turns at unpacking a tile of 128 tokens and
-// at its columns; several blocks an SM overlap each other.
+// A block is 128 threads that unpack a tile of 128 tokens into tensor memory
+// (thread = token = lane) and then take its columns, 16 query rows a product; the
+// packed rows of the next tile are on their way meanwhile (TMA).  Four blocks an SM
+// (their keys and sums fill its tensor memory) overlap each other.
 #include "varlen_common.cuh"
 
 namespace iris {
 namespace {
 
-constexpr int kCols = 32;       // query rows of a product
+constexpr int kCols = 16;       // query rows of a product
 constexpr int kResident = 128;  // query rows that stay in shared memory
+constexpr int kSlots = kResident / kCols;
 
 struct MassParams {
   VarlenBatch s;
@@ -38,19 +41,19 @@ struct MassParams {
 
 template <int D>
 struct MassCfg {
-  static constexpr int kKeys = kTile * D * 2;
   static constexpr int kQuery = kCols * D * 2;
-  static constexpr int kUnit = kTile * (D / 2 + D / 16);
-  static constexpr int kMeta = kCols * 32;  // a row: factor, lse, place, slope; what it sees
-  static constexpr int kColumns = D;        // tensor memory: D / 32 groups x 32 columns
-  static int smem(int slots) { return 1024 + kKeys + slots * (kQuery + kMeta) + 2 * kUnit; }
+  static constexpr int kPacked = kTile * D / 2;
+  static constexpr int kMeta = kCols * (8 + 8 + 16);  // a row: factor and lse (two rows a vector), place and slope, sight
+  static constexpr int kSumColumn = D / 2;            // tensor memory: keys, then D / 32 groups x 16 columns of sums
+  static constexpr int kColumns = D;
+  static int smem(int slots) { return 1024 + slots * (kQuery + kMeta) + kPacked; }
 };
 
 struct MassShared {
-  uint64_t done;
+  uint64_t here, done;
   uint32_t tmem;
-  int32_t all_lo[4], all_hi[4];  // tokens that every row of a column tile sees (without the prefix), a slot each
-  int32_t any_lo[4], any_hi[4];  // between them lies all that any row sees
+  int32_t all_lo[kSlots], all_hi[kSlots];  // tokens that every row of a slot sees (without the prefix)
+  int32_t any_lo[kSlots], any_hi[kSlots];  // between them lies all that any row sees
 };
 
 IRIS_DEV float min_nan(float a, float b) {  // NaN stays NaN
@@ -59,12 +62,19 @@ IRIS_DEV float min_nan(float a, float b) {  // NaN stays NaN
   return r;
 }
 
-// Query rows r0 .. r0 + 32 into a slot: four threads a row.
+// A slot's rows in shared memory.
+struct MassRows {
+  float4* f;     // [8] factors of two rows, minus their lse
+  float2* more;  // [16] place, slope
+  int4* sight;   // [16]
+};
+
+// Query rows r0 .. r0 + 16 into a slot: eight threads a row.
 template <int D, bool kCap, bool kBias>
 IRIS_DEV void load_columns(const MassParams& p, MassShared& sh, const Span& sp, int b, int len, int h, int r0, int rows,
-                           uint32_t q_tile, float4* row_f, int4* row_s, int slot, int tid) {
-  constexpr int kWords = D / 8;  // a thread's pairs
-  __syncthreads();  // what the slot held is read
+                           uint32_t q_tile, const MassRows& to, int slot, int tid) {
+  constexpr int kWords = D / 16;  // a thread's pairs
+  __syncthreads();                // what the slot held is read
   if (tid == 0) {
     sh.all_lo[slot] = 0;
     sh.all_hi[slot] = INT32_MAX;
@@ -72,49 +82,53 @@ IRIS_DEV void load_columns(const MassParams& p, MassShared& sh, const Span& sp, 
     sh.any_hi[slot] = 0;
   }
   __syncthreads();
-  const int row = tid >> 2, part = tid & 3, r = r0 + row;
+  const int row = tid >> 3, part = tid & 7, r = r0 + row;
   const bool valid = r < rows;
   const int i = valid ? r / p.s.group : 0, g = valid ? r % p.s.group : 0;
   const int64_t token = sp.start + i;
   const int head = h * p.s.group + g;
-  uint32_t w[kWords];
+  uint32_t w[kWords] = {};
+  if (valid) {
+    const uint4* src = reinterpret_cast<const uint4*>(p.query + token * p.q_stride + static_cast<int64_t>(head) * D +
+                                                      part * (D / 8));
 #pragma unroll
-  for (int c = 0; c < kWords / 4; ++c) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (valid)
-      v = *reinterpret_cast<const uint4*>(p.query + token * p.q_stride + static_cast<int64_t>(head) * D + part * (D / 4) +
-                                          8 * c);
-    w[4 * c] = v.x;
-    w[4 * c + 1] = v.y;
-    w[4 * c + 2] = v.z;
-    w[4 * c + 3] = v.w;
+    for (int c = 0; c < kWords / 4; ++c) {
+      const uint4 v = src[c];
+      w[4 * c] = v.x;
+      w[4 * c + 1] = v.y;
+      w[4 * c + 2] = v.z;
+      w[4 * c + 3] = v.w;
+    }
   }
   const float back = scale_row_part<kWords>(w, p.bf16 != 0, [](uint32_t m) {
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    return max(m, __shfl_xor_sync(0xffffffffu, m, 4));
   });
 #pragma unroll
   for (int c = 0; c < kWords / 4; ++c) {
     const uint4 v = order8(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-    const int chunk = part * (D / 32) + c;
+    const int chunk = part * (D / 64) + c;
     sts128(q_tile + (chunk >> 3) * (kCols * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), v.x, v.y, v.z, v.w);
   }
   if (part == 0) {
     Sight see = {0, 0, 0, 0};
-    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float factor = 0.0f, lse = 0.0f, slope = 0.0f;
+    int32_t pos = 0;
     if (valid) {
-      const int32_t pos = len - sp.count + i;
-      const float lse = __ldg(p.lse + token * p.s.hq + head);
-      f.x = kCap ? p.s.scale * back / p.s.cap : p.s.scale * kLog2e * back;
-      f.y = lse;
-      f.z = __int_as_float(pos);
-      f.w = kBias ? -__ldg(p.s.slopes + head) * kLog2e : 0.0f;
+      pos = len - sp.count + i;
+      lse = __ldg(p.lse + token * p.s.hq + head);
+      factor = kCap ? p.s.scale * back / p.s.cap : p.s.scale * kLog2e * back;
+      slope = kBias ? -__ldg(p.s.slopes + head) * kLog2e : 0.0f;
       if (lse != -__int_as_float(0x7f800000))  // (a row that saw nothing gives nothing)
         see = row_sight(pos, p.s.first_visible != nullptr ? __ldg(p.s.first_visible + token) : 0,
                         p.s.prefix_lens != nullptr ? __ldg(p.s.prefix_lens + b) : 0, p.s.window, len);
     }
-    row_f[row] = f;
-    row_s[row] = make_int4(see.a0, see.a1, see.b0, see.b1);
+    float* f = reinterpret_cast<float*>(to.f + row / 2);
+    f[row & 1] = factor;
+    f[2 + (row & 1)] = -lse;
+    to.more[row] = make_float2(__int_as_float(pos), slope);
+    to.sight[row] = make_int4(see.a0, see.a1, see.b0, see.b1);
     atomicMax(&sh.all_lo[slot], see.b0);
     atomicMin(&sh.all_hi[slot], see.b1);
     if (see.a1 > see.a0) {
@@ -131,7 +145,7 @@ IRIS_DEV void load_columns(const MassParams& p, MassShared& sh, const Span& sp, 
 }
 
 template <int D, bool kCap, bool kBias>
-__global__ void __launch_bounds__(128) attention_mass_kernel(const MassParams p) {
+__global__ void __launch_bounds__(128, 4) attention_mass_kernel(const __grid_constant__ CUtensorMap k_map, const MassParams p) {
   using C = MassCfg<D>;
   constexpr int kGroups = D / 32;
   extern __shared__ uint8_t smem_raw[];
@@ -139,6 +153,7 @@ __global__ void __launch_bounds__(128) attention_mass_kernel(const MassParams p)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int chunk = blockIdx.x % p.chunks, h = blockIdx.x / p.chunks % p.s.hkv, b = blockIdx.x / p.chunks / p.s.hkv;
   if (tid == 0) {
+    mbar_init(&sh.here, 1);
     mbar_init(&sh.done, 1);
     fence_barrier_init();
   }
@@ -150,29 +165,40 @@ __global__ void __launch_bounds__(128) attention_mass_kernel(const MassParams p)
   const int tiles = (len + kTile - 1) / kTile;
   const int k0 = chunk * p.per, n = min(p.per, tiles - k0);
   if (n <= 0) return;
+  __syncthreads();  // (the barriers are ready)
 
-  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
-  uint8_t* base = smem_raw + pad;
-  const uint32_t k_tile = smem_u32(base), q_tiles = k_tile + C::kKeys, ring = q_tiles + p.slots * C::kQuery;
-  float4* row_f = reinterpret_cast<float4*>(base + C::kKeys + p.slots * C::kQuery + 2 * C::kUnit);
-  int4* row_s = reinterpret_cast<int4*>(row_f + p.slots * kCols);
-
-  const int64_t row_bytes = static_cast<int64_t>(p.s.hkv) * (D / 2);
-  int32_t pages[2];  // of this thread's token in the tile that is unpacked, and in the next
-  auto load = [&](int k, int32_t& page) {
-    if (k < n) {
-      const int32_t j = (k0 + k) * kTile + tid;
-      page = page_of(p.s, b, j, len);
-      const int64_t row = static_cast<int64_t>(page) * kTokPage + j % kTokPage;
-      const uint32_t slot = ring + (k & 1) * C::kUnit;
-      const uint8_t* data = p.k_data + row * row_bytes + h * (D / 2);
-#pragma unroll
-      for (int c = 0; c < kGroups; ++c) copy_async<16>(slot + c * 2048 + tid * 16, data + c * 16, j < len);
-      copy_async<D / 16>(slot + kGroups * 2048 + tid * (D / 16), p.k_scale + (row * p.s.hkv + h) * (D / 16), j < len);
-    }
-    copies_commit();
+  uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t q_tiles = smem_u32(base);
+  uint8_t* packed = base + p.slots * C::kQuery;
+  const uint32_t raw = smem_u32(packed);
+  float4* row_f = reinterpret_cast<float4*>(packed + C::kPacked);
+  float2* row_more = reinterpret_cast<float2*>(row_f + p.slots * kCols / 2);
+  int4* row_sight_ = reinterpret_cast<int4*>(row_more + p.slots * kCols);
+  auto rows_of = [&](int slot) {
+    return MassRows{row_f + slot * kCols / 2, row_more + slot * kCols, row_sight_ + slot * kCols};
   };
-  load(0, pages[0]);
+
+  auto first = [&](int k) { return (k0 + k) * kTile; };
+  auto page_at = [&](int k) { return lane < 8 ? raw_page(p.s, b, first(k) + lane * kTokPage, len) : 0; };
+  uint32_t sc2[kGroups / 2];  // scales of the tile that is next
+  auto fetch = [&](int32_t page, int32_t j) {
+    const uint8_t* x = p.k_scale + ((static_cast<int64_t>(page) * kTokPage + (j & (kTokPage - 1))) * p.s.hkv + h) * (D / 16);
+    if constexpr (D == 128) {
+      const uint2 v = j < len ? __ldg(reinterpret_cast<const uint2*>(x)) : make_uint2(0, 0);
+      sc2[0] = v.x;
+      sc2[1] = v.y;
+    } else {
+      sc2[0] = j < len ? __ldg(reinterpret_cast<const uint32_t*>(x)) : 0u;
+    }
+  };
+  int32_t copy_page = 0;  // (warp 0) of the tile whose copies are next, not checked yet
+  if (warp == 0) {
+    load_packed<D>(packed, &k_map, checked_page(p.s, page_at(0)), first(0), len, h, &sh.here, lane);
+    if (n > 1) copy_page = page_at(1);
+  }
+  int32_t page = page_of(p.s, b, first(0) + tid, len);  // of this thread's token
+  fetch(page, first(0) + tid);
+  int32_t later = n > 1 ? raw_page(p.s, b, first(1) + tid, len) : 0;
   if (warp == 0) umma_alloc(&sh.tmem, C::kColumns);
   umma_fence_before();
   __syncthreads();
@@ -182,103 +208,133 @@ __global__ void __launch_bounds__(128) attention_mass_kernel(const MassParams p)
   const bool resident = col_tiles <= p.slots;
   if (resident)
     for (int q = 0; q < col_tiles; ++q)
-      load_columns<D, kCap, kBias>(p, sh, sp, b, len, h, q * kCols, rows, q_tiles + q * C::kQuery, row_f + q * kCols,
-                                   row_s + q * kCols, q, tid);
+      load_columns<D, kCap, kBias>(p, sh, sp, b, len, h, q * kCols, rows, q_tiles + q * C::kQuery, rows_of(q), q, tid);
   const int32_t fresh = p.first_token != nullptr ? __ldg(p.first_token + b) : 0;
   const float cap2 = p.s.cap * kLog2e;
   uint32_t phase = 0;
   bool ok = true;
+#pragma unroll 1
   for (int k = 0; ok && k < n; ++k) {
-    load(k + 1, pages[1]);
-    const int32_t base_j = (k0 + k) * kTile, j = base_j + tid;
-    float* slot_mass = p.mass + (static_cast<int64_t>(pages[0]) * p.s.hkv + h) * kTokPage + j % kTokPage;
+    const int32_t base_j = first(k), j = base_j + tid;
+    float* slot_mass = p.mass + (static_cast<int64_t>(page) * p.s.hkv + h) * kTokPage + j % kTokPage;
     const float old = j < len && j < fresh ? *slot_mass : 0.0f;
-    copies_wait<1>();
-    const uint32_t raw = ring + (k & 1) * C::kUnit;
     float sc[kGroups];
-    if constexpr (D == 128) {
-      const uint2 v = lds64(raw + kGroups * 2048 + tid * 8);
-      const float2 a = __half22float2(u32_as_h2(v.x)), c = __half22float2(u32_as_h2(v.y));
-      sc[0] = a.x; sc[1] = a.y; sc[2] = c.x; sc[3] = c.y;
-    } else {
-      const float2 a = __half22float2(u32_as_h2(lds32(raw + kGroups * 2048 + tid * 4)));
-      sc[0] = a.x; sc[1] = a.y;
-    }
-    bool odd = false;  // a scale that is not finite makes the token's logits NaN
+    {
+      bool odd = false;  // a scale that is not finite makes the token's logits NaN
 #pragma unroll
-    for (int c = 0; c < kGroups; ++c) odd |= !(fabsf(sc[c]) <= 65504.0f);
-    if (odd) sc[0] = __int_as_float(0x7fffffff);
+      for (int c = 0; c < kGroups; ++c) {
+        const uint32_t bits = (sc2[c / 2] >> (16 * (c & 1))) & 0xffffu;
+        odd |= (bits & 0x7fffu) >= 0x7c00u;
+        sc[c] = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+      }
+      if (odd) sc[0] = __int_as_float(0x7fffffff);
+    }
+    if (k + 1 < n) {
+      page = checked_page(p.s, later);
+      fetch(page, first(k + 1) + tid);
+      if (k + 2 < n) later = raw_page(p.s, b, first(k + 2) + tid, len);
+    }
+    ok = wait_all(&sh.here, k & 1, p.s.err);
 #pragma unroll
     for (int c = 0; c < kGroups; ++c) {
-      const uint4 w4 = lds128(raw + c * 2048 + tid * 16);
+      const uint4 w4 = lds128(raw + packed_at<D>(tid, c));
       const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+      uint32_t x[16];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sts128(k_tile + operand_at(tid, 4 * c + i), int4_lo_exact(w[i]), int4_hi_exact(w[i]), int4_lo_exact(w[i] >> 8),
-               int4_hi_exact(w[i] >> 8));
+      for (int i = 0; i < 4; ++i) {
+        x[4 * i] = int4_lo_exact(w[i]);
+        x[4 * i + 1] = int4_hi_exact(w[i]);
+        x[4 * i + 2] = int4_lo_exact(w[i] >> 8);
+        x[4 * i + 3] = int4_hi_exact(w[i] >> 8);
+      }
+      umma_st16(lanes + 16 * c, x);
     }
-    fence_proxy_async_shared();
-    __syncthreads();
-    float sum = 0.0f;
+    umma_wait_st();
+    umma_fence_before();
+    if (!(ok = __syncthreads_and(ok))) break;
+    float2 sum = make_float2(0.0f, 0.0f);
+    bool loaded = k + 1 >= n;  // the next tile's copies are under way
+#pragma unroll 1
     for (int q = 0; q < col_tiles; ++q) {
       const int slot = resident ? q : 0;
       if (!resident)
-        load_columns<D, kCap, kBias>(p, sh, sp, b, len, h, q * kCols, rows, q_tiles, row_f, row_s, 0, tid);
+        load_columns<D, kCap, kBias>(p, sh, sp, b, len, h, q * kCols, rows, q_tiles, rows_of(0), 0, tid);
       if (sh.any_hi[slot] <= base_j || sh.any_lo[slot] >= base_j + kTile) continue;  // no row sees the tile
-      const int cols = min(kCols, rows - q * kCols);
-      if (warp == 0 && elect_one()) {
-        umma_fence_after();
-        const uint32_t idesc = umma_idesc(kTile, cols <= 16 ? 16 : 32, false, false);
+      if (warp == 0) {
+        if (elect_one()) {
+          umma_fence_after();
 #pragma unroll
-        for (int x = 0; x < D / 16; ++x) {  // the groups in turn, twice: a product does not wait for the one before it
-          const int g = x % kGroups, s = 2 * g + x / kGroups;
-          umma_ss(tmem + g * kCols, umma_desc(k_tile + (s >> 2) * (kTile * 128) + (s & 3) * 32, 16, 1024),
-                  umma_desc(q_tiles + slot * C::kQuery + (s >> 2) * (kCols * 128) + (s & 3) * 32, 16, 1024), idesc,
-                  x >= kGroups);
+          for (int x = 0; x < D / 16; ++x) {  // the groups in turn, twice: a product does not wait for the one before it
+            const int g = x % kGroups, s = 2 * g + x / kGroups;
+            umma_ts(tmem + C::kSumColumn + g * kCols, tmem + 8 * s,
+                    umma_desc(q_tiles + slot * C::kQuery + (s >> 2) * (kCols * 128) + (s & 3) * 32, 16, 1024),
+                    umma_idesc(kTile, kCols, false, false), x >= kGroups);
+          }
+          umma_commit(smem_u32(&sh.done));
         }
-        umma_commit(smem_u32(&sh.done));
+        __syncwarp();
+        if (!loaded) {
+          load_packed<D>(packed, &k_map, checked_page(p.s, copy_page), first(k + 1), len, h, &sh.here, lane);
+          if (k + 2 < n) copy_page = page_at(k + 2);
+        }
       }
-      ok = mbar_wait_bounded(&sh.done, phase, p.s.err);
+      loaded = true;
+      ok = wait_all(&sh.done, phase, p.s.err);
       phase ^= 1;
-      if (!(ok = __syncthreads_and(ok))) break;
       umma_fence_after();
       const bool full = sh.all_lo[slot] <= base_j && base_j + kTile <= sh.all_hi[slot];
-      const float4* fs = row_f + slot * kCols;
-      const int4* ss = row_s + slot * kCols;
-#pragma unroll 1
-      for (int c0 = 0; c0 < cols; c0 += 8) {
+      const MassRows at = rows_of(slot);
+      const int cols = min(kCols, rows - q * kCols);
+#pragma unroll
+      for (int c0 = 0; c0 < kCols; c0 += 8) {
+        if (c0 >= cols) break;
         uint32_t v[kGroups][8];
 #pragma unroll
-        for (int c = 0; c < kGroups; ++c) umma_ld8(lanes + c * kCols + c0, v[c]);
+        for (int c = 0; c < kGroups; ++c) umma_ld8(lanes + C::kSumColumn + c * kCols + c0, v[c]);
         umma_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float s = 0.0f;
+        for (int i = 0; i < 8; i += 2) {
+          float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
           for (int c = 0; c < kGroups; ++c) {
-            asm volatile("" : "+r"(v[c][i]));
-            s = fmaf(__uint_as_float(v[c][i]), sc[c], s);
+            asm volatile("" : "+r"(v[c][i]), "+r"(v[c][i + 1]));
+            s = __ffma2_rn(make_float2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), make_float2(sc[c], sc[c]), s);
           }
-          const float4 f = fs[c0 + i];
-          float y = s * f.x;
-          if (kCap) y = cap2 * tanh_f(y);
-          if (kBias) y = fmaf(f.w, fabsf(static_cast<float>(__float_as_int(f.z) - j)), y);
-          const float e = ex2(min_nan(y - f.y, 0.0f));  // (a weight is at most 1)
-          if (full) {
-            sum += e;
+          const float4 f = at.f[(c0 + i) / 2];
+          float2 y;
+          if (kCap || kBias) {
+            y = __fmul2_rn(s, make_float2(f.x, f.y));
+            if (kCap) y = make_float2(cap2 * tanh_f(y.x), cap2 * tanh_f(y.y));
+            if (kBias) {
+              const float2 a = at.more[c0 + i], d = at.more[c0 + i + 1];
+              y.x = fmaf(a.y, fabsf(static_cast<float>(__float_as_int(a.x) - j)), y.x);
+              y.y = fmaf(d.y, fabsf(static_cast<float>(__float_as_int(d.x) - j)), y.y);
+            }
+            y = __fadd2_rn(y, make_float2(f.z, f.w));
           } else {
-            const int4 z = ss[c0 + i];
-            sum += (j >= z.x && j < z.y) || (j >= z.z && j < z.w) ? e : 0.0f;
+            y = __ffma2_rn(s, make_float2(f.x, f.y), make_float2(f.z, f.w));
           }
+          float2 e = make_float2(ex2(min_nan(y.x, 0.0f)), ex2(min_nan(y.y, 0.0f)));  // (a weight is at most 1)
+          if (!full) {
+            const int4 a = at.sight[c0 + i], d = at.sight[c0 + i + 1];
+            if (!((j >= a.x && j < a.y) || (j >= a.z && j < a.w))) e.x = 0.0f;
+            if (!((j >= d.x && j < d.y) || (j >= d.z && j < d.w))) e.y = 0.0f;
+          }
+          sum = __fadd2_rn(sum, e);
         }
       }
       umma_fence_before();
-      __syncthreads();  // the columns are read: the next product may overwrite them
+      if (!(ok = __syncthreads_and(ok))) break;  // the sums are read: the next product may overwrite them
     }
-    if (ok && j < len) *slot_mass = fmaf(old, p.decay, sum);
-    pages[0] = pages[1];
+    if (!loaded && warp == 0) {
+      load_packed<D>(packed, &k_map, checked_page(p.s, copy_page), first(k + 1), len, h, &sh.here, lane);
+      if (k + 2 < n) copy_page = page_at(k + 2);
+    }
+    if (ok && j < len) *slot_mass = fmaf(old, p.decay, sum.x + sum.y);
   }
-  copies_wait<0>();
+  if (!ok) {  // a wait gave up: copies that are under way land before the block ends
+    for (uint32_t parity = 0; parity < 2; ++parity) mbar_wait_bounded(&sh.here, parity, p.s.err);
+  }
   umma_fence_before();
   __syncthreads();
   umma_fence_after();
@@ -288,10 +344,11 @@ __global__ void __launch_bounds__(128) attention_mass_kernel(const MassParams p)
 template <int D, bool kCap, bool kBias>
 cudaError_t launch_mass(const MassParams& p, int64_t grid, cudaStream_t stream) {
   auto fn = attention_mass_kernel<D, kCap, kBias>;
+  CUtensorMap k;
+  if (!packed_map(&k, p.k_data, D, p.s.hkv, p.s.num_pages)) return cudaErrorInvalidValue;
   const int smem = MassCfg<D>::smem(p.slots);
-  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, MassCfg<D>::smem(4));
-  if (e != cudaSuccess) return e;
-  return launch_early(fn, dim3(static_cast<unsigned>(grid)), dim3(128), smem, stream, p);
+  static_assert(kSlots == 8, "48 KB hold every slot: no attribute is needed");
+  return launch_early(fn, dim3(static_cast<unsigned>(grid)), dim3(128), smem, stream, k, p);
 }
 template <int D>
 cudaError_t launch_mass(const MassParams& p, int64_t grid, cudaStream_t stream) {
@@ -365,7 +422,7 @@ extern "C" int iris_b200_int4_paged_attention_mass(
   p.per = static_cast<int32_t>(per);
   p.chunks = static_cast<int32_t>((tiles + per - 1) / per);
   const int64_t most = cu_seqlens == nullptr ? group : static_cast<int64_t>(tokens) * group;
-  p.slots = most >= kResident ? kResident / kCols : static_cast<int32_t>((most + kCols - 1) / kCols);
+  p.slots = most >= kResident ? kSlots : static_cast<int32_t>((most + kCols - 1) / kCols);
   if (p.slots < 1) p.slots = 1;
   const int64_t grid = units * p.chunks;
   if (grid > INT32_MAX) return IRIS_EUNSUPPORTED;

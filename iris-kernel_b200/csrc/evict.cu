@@ -150,29 +150,25 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const EvictPara
   const int pages = (len + kTokPage - 1) / kTokPage;
   const int j0 = static_cast<int>(static_cast<int64_t>(pages) * rank / size) * kTokPage;
   const int j1 = min(len, static_cast<int>(static_cast<int64_t>(pages) * (rank + 1) / size) * kTokPage);
-  if (tid == 0) sh.bad = 0;
-  __syncthreads();
-  for (int c = j0 / kTokPage + tid; c * kTokPage < j1; c += kEvictThreads) {
-    const int32_t id = __ldg(table + c);
-    if (id < 0 || id >= p.num_pages) {
-      set_error(p.err, IRIS_ERR_PAGE_ID);
-      sh.bad = 1;
-    }
-  }
-  for (int i = tid; i < 3 * kBins; i += kEvictThreads) (&sh.bins[0][0])[i] = 0;
-  cluster.sync();
-  bool stay = len <= budget;  // nothing to do, or nothing that may be touched
-  bool bad = false;
-  for (int r = 0; r < size; ++r) bad |= *cluster.map_shared_rank(&sh.bad, r) != 0;
-  if (stay || bad) {
+  auto meet = [&] {  // of the cluster's blocks
+    if (size == 1) __syncthreads(); else cluster.sync();
+  };
+  auto stay = [&](bool bad) {  // nothing to do, or nothing that may be touched
     if (kept != nullptr)
       for (int i = rank * kEvictThreads + tid; i < budget; i += size * kEvictThreads) kept[i] = i < len ? i : -1;
-    if (tid == 0 && rank == 0 && h == 0) p.new_lens[b] = wrong || bad ? raw : min(len, budget);
-    cluster.sync();
+    if (tid == 0 && rank == 0 && h == 0) p.new_lens[b] = wrong || bad ? raw : len;
+  };
+  auto id_ok = [&](int32_t id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_pages); };
+  if (len <= budget) {
+    bool bad = false;  // (page ids are looked at all the same)
+    for (int c = j0 / kTokPage + tid; c * kTokPage < j1; c += kEvictThreads) bad |= !id_ok(__ldg(table + c));
+    if (bad) set_error(p.err, IRIS_ERR_PAGE_ID);
+    stay(false);
     return;
   }
-  if (tid == 0 && rank == 0 && h == 0) p.new_lens[b] = budget;
-
+  if (tid == 0) sh.bad = 0;
+  for (int i = tid; i < 3 * kBins; i += kEvictThreads) (&sh.bins[0][0])[i] = 0;
+  __syncthreads();
   const int sink = p.sink, recent = p.recent, heavy = budget - recent, last = len - recent;
   const int want = heavy - sink;  // tokens of [sink, last) that stay
   const bool cached = j1 - j0 <= p.keys;
@@ -181,6 +177,32 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const EvictPara
                   : weight_key(p.mass[(static_cast<int64_t>(__ldg(table + j / kTokPage)) * p.hkv + h) * kTokPage + j % kTokPage]);
   };
   const int c0 = max(j0, sink), c1 = min(j1, last);  // this block's tokens in question
+  // the weights' keys, their first histogram, and a look at every page id
+#pragma unroll 4
+  for (int j = j0 + 4 * tid; j < j1; j += 4 * kEvictThreads) {
+    const int32_t id = __ldg(table + j / kTokPage);
+    if (!id_ok(id)) {
+      set_error(p.err, IRIS_ERR_PAGE_ID);
+      sh.bad = 1;
+      continue;
+    }
+    const float4 w =
+        *reinterpret_cast<const float4*>(p.mass + (static_cast<int64_t>(id) * p.hkv + h) * kTokPage + j % kTokPage);
+    const uint32_t k4[4] = {weight_key(w.x), weight_key(w.y), weight_key(w.z), weight_key(w.w)};
+    if (cached) *reinterpret_cast<uint4*>(keys + (j - j0)) = make_uint4(k4[0], k4[1], k4[2], k4[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (j + i >= c0 && j + i < c1) atomicAdd(&sh.bins[0][k4[i] >> 21], 1u);
+  }
+  meet();
+  bool bad = false;
+  for (int r = 0; r < size; ++r) bad |= *cluster.map_shared_rank(&sh.bad, r) != 0;
+  if (bad) {  // the sequence stays as it is (its other heads see the same pages)
+    stay(true);
+    meet();
+    return;
+  }
+  if (tid == 0 && rank == 0 && h == 0) p.new_lens[b] = budget;
   // the lightest key that stays: `low`, of which the first `ties` in the cluster's order stay
   uint32_t low = 0;
   int ties = 0;
@@ -190,26 +212,14 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const EvictPara
     for (int round = 0; round < 3; ++round) {
       const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, width = round == 2 ? 10 : 11;
       uint32_t* bins = sh.bins[round];
-      if (round == 0 || !cached) {  // from memory, four tokens a load
-#pragma unroll 4
-        for (int j = j0 + 4 * tid; j < j1; j += 4 * kEvictThreads) {
-          const float4 w = *reinterpret_cast<const float4*>(
-              p.mass + (static_cast<int64_t>(__ldg(table + j / kTokPage)) * p.hkv + h) * kTokPage + j % kTokPage);
-          const uint32_t k4[4] = {weight_key(w.x), weight_key(w.y), weight_key(w.z), weight_key(w.w)};
-          if (cached) *reinterpret_cast<uint4*>(keys + (j - j0)) = make_uint4(k4[0], k4[1], k4[2], k4[3]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (j + i >= c0 && j + i < c1 && (round == 0 || (k4[i] >> (shift + width)) == (low >> (shift + width))))
-              atomicAdd(&bins[(k4[i] >> shift) & ((1u << width) - 1)], 1u);
-        }
-      } else {
+      if (round > 0) {
         for (int j = c0 + tid; j < c1; j += kEvictThreads) {
-          const uint32_t key = keys[j - j0];
+          const uint32_t key = key_at(j);
           if ((key >> (shift + width)) == (low >> (shift + width)))
             atomicAdd(&bins[(key >> shift) & ((1u << width) - 1)], 1u);
         }
+        meet();
       }
-      cluster.sync();
       // from the top bin down: four bins a thread, summed over the cluster
       constexpr int kEach = kBins / kEvictThreads;
       static_assert(kEach == 4, "a thread's bins are one load");
@@ -244,7 +254,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const EvictPara
   for (int j = c0 + tid; want > 0 && j < c1; j += kEvictThreads) count += key_at(j) == low;
   block_scan(count, sh.warp_sums, &total);
   if (tid == 0) sh.equal = total;
-  cluster.sync();
+  meet();
   int equal_before = 0;
   for (int r = 0; r < rank; ++r) equal_before += *cluster.map_shared_rank(&sh.equal, r);
   // ranks: a thread takes `each` tokens in a row, in whole sweeps of the block
@@ -306,7 +316,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const EvictPara
         sh.moving = moves;
         sh.holes = gaps;
       }
-      cluster.sync();
+      meet();
       for (int r = 0; r < rank; ++r) {
         move_at += *cluster.map_shared_rank(&sh.moving, r);
         hole_at += *cluster.map_shared_rank(&sh.holes, r);
@@ -319,8 +329,8 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const EvictPara
     for (int i = rank * kEvictThreads + tid; i < sink; i += size * kEvictThreads) kept[i] = i;
     for (int i = rank * kEvictThreads + tid; i < recent; i += size * kEvictThreads) kept[heavy + i] = last + i;
   }
-  __threadfence();
-  cluster.sync();
+  if (size > 1) __threadfence();
+  meet();
 
   // kept tokens from behind into the holes: sources and targets do not meet
   constexpr int kLanes = EvictRow<D>::kLanes, kRows = kEvictThreads / kLanes;
@@ -350,22 +360,21 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_kernel(const EvictPara
   // or before its own sources, so no later step reads what it wrote
 #pragma unroll 1
   for (int i0 = 0; i0 < recent; i0 += size * kRows * kDeep) {
-    cluster.sync();  // what this step overwrites has been read
+    meet();  // what this step overwrites has been read
     Part x[kDeep];
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
       const int i = i0 + d * size * kRows + unit;
       if (i < recent) x[d] = read_part<D>(p, row_of(last + i), h, sub);
     }
-    __threadfence();
-    cluster.sync();
+    meet();
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
       const int i = i0 + d * size * kRows + unit;
       if (i < recent) write_part<D>(p, row_of(heavy + i), h, sub, x[d]);
     }
   }
-  cluster.sync();  // (no block leaves while another reads its shared memory)
+  meet();  // (no block leaves while another reads its shared memory)
 }
 
 // Blocks of a cluster: enough for two an SM, each with 1024 tokens or more.
