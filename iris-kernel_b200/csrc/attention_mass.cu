@@ -74,14 +74,6 @@ template <int D, bool kCap, bool kBias>
 IRIS_DEV void load_columns(const MassParams& p, MassShared& sh, const Span& sp, int b, int len, int h, int r0, int rows,
                            uint32_t q_tile, const MassRows& to, int slot, int tid) {
   constexpr int kWords = D / 16;  // a thread's pairs
-  __syncthreads();                // what the slot held is read
-  if (tid == 0) {
-    sh.all_lo[slot] = 0;
-    sh.all_hi[slot] = INT32_MAX;
-    sh.any_lo[slot] = INT32_MAX;
-    sh.any_hi[slot] = 0;
-  }
-  __syncthreads();
   const int row = tid >> 3, part = tid & 7, r = r0 + row;
   const bool valid = r < rows;
   const int i = valid ? r / p.s.group : 0, g = valid ? r % p.s.group : 0;
@@ -140,6 +132,18 @@ IRIS_DEV void load_columns(const MassParams& p, MassShared& sh, const Span& sp, 
       atomicMax(&sh.any_hi[slot], see.b1);
     }
   }
+}
+IRIS_DEV void clear_slots(MassShared& sh, int slots, int tid) {
+  __syncthreads();  // what they held is read
+  if (tid < slots) {
+    sh.all_lo[tid] = 0;
+    sh.all_hi[tid] = INT32_MAX;
+    sh.any_lo[tid] = INT32_MAX;
+    sh.any_hi[tid] = 0;
+  }
+  __syncthreads();
+}
+IRIS_DEV void slots_done() {
   fence_proxy_async_shared();
   __syncthreads();
 }
@@ -206,9 +210,13 @@ __global__ void __launch_bounds__(128, 4) attention_mass_kernel(const __grid_con
   const uint32_t tmem = sh.tmem, lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
   const int rows = sp.count * p.s.group, col_tiles = (rows + kCols - 1) / kCols;
   const bool resident = col_tiles <= p.slots;
-  if (resident)
+  if (resident) {
+    clear_slots(sh, col_tiles, tid);
+#pragma unroll 2
     for (int q = 0; q < col_tiles; ++q)
       load_columns<D, kCap, kBias>(p, sh, sp, b, len, h, q * kCols, rows, q_tiles + q * C::kQuery, rows_of(q), q, tid);
+    slots_done();
+  }
   const int32_t fresh = p.first_token != nullptr ? __ldg(p.first_token + b) : 0;
   const float cap2 = p.s.cap * kLog2e;
   uint32_t phase = 0;
@@ -257,8 +265,11 @@ __global__ void __launch_bounds__(128, 4) attention_mass_kernel(const __grid_con
 #pragma unroll 1
     for (int q = 0; q < col_tiles; ++q) {
       const int slot = resident ? q : 0;
-      if (!resident)
+      if (!resident) {
+        clear_slots(sh, 1, tid);
         load_columns<D, kCap, kBias>(p, sh, sp, b, len, h, q * kCols, rows, q_tiles, rows_of(0), 0, tid);
+        slots_done();
+      }
       if (sh.any_hi[slot] <= base_j || sh.any_lo[slot] >= base_j + kTile) continue;  // no row sees the tile
       if (warp == 0) {
         if (elect_one()) {
@@ -417,10 +428,11 @@ extern "C" int iris_b200_int4_paged_attention_mass(
   p.bf16 = dtype == IRIS_DTYPE_BF16;
   const int64_t tiles = (static_cast<int64_t>(max_pages_per_seq) * kTokPage + kTile - 1) / kTile;
   const int64_t units = static_cast<int64_t>(batch) * num_kv_heads;
-  int64_t per = units * tiles / (148 * 16);  // 16 blocks an SM and more, of up to eight tiles
-  per = per < 1 ? 1 : per > 8 ? 8 : per;
-  p.per = static_cast<int32_t>(per);
-  p.chunks = static_cast<int32_t>((tiles + per - 1) / per);
+  // about two waves of four blocks an SM: more would load the query rows more often
+  int64_t chunks = (148 * 4 * 2 + units - 1) / units;
+  if (chunks > tiles) chunks = tiles;
+  p.per = static_cast<int32_t>((tiles + chunks - 1) / chunks);
+  p.chunks = static_cast<int32_t>((tiles + p.per - 1) / p.per);
   const int64_t most = cu_seqlens == nullptr ? group : static_cast<int64_t>(tokens) * group;
   p.slots = most >= kResident ? kSlots : static_cast<int32_t>((most + kCols - 1) / kCols);
   if (p.slots < 1) p.slots = 1;
