@@ -18,11 +18,15 @@
 // here misses the few kilobytes of L1 that are left (740 us for two prompts of
 // 4096 tokens; 506 without).
 //
-// Roundings.  Stored values are nibble * scale, 15 bits: fp16 keeps 11.  Each
-// run of 32 tokens is first scaled by a power of two that brings its largest
-// scale into [2^12, 2^13), so that neither large scales overflow nor small
-// ones lose bits; the power goes into the logit's factor (keys) and the
-// probability's exponent (values).  Probabilities are fp16 with the row's
+// Roundings.  A stored key or value is nibble * scale: 15 bits, where fp16 has 11.
+// Values are rounded.  Keys are not, as the log-sum-exp of a row with few tokens
+// would show it (1e-4 of a logit): their scale is split into its upper 8 bits and
+// the rest, and two exact fp16 tiles follow each other in the product.  (That
+// costs 256 of its cycles and a second tile's store, and with 128 dims the second
+// key buffer.)  Each run of 32 tokens is first scaled by a power of two that
+// brings its largest scale into [2^12, 2^13), so that neither large scales
+// overflow nor small ones lose bits; the power goes into the logit's factor (keys)
+// and the probability's exponent (values).  Probabilities are fp16 with the row's
 // reference at 2^8.  Logits, statistics and sums are fp32.
 #include "varlen_few.cuh"
 
@@ -33,7 +37,9 @@ template <int D, int kTiles>
 struct Cfg {
   static constexpr int kOperand = kTile * D * 2;       // one fp16 tile
   static constexpr int kPacked = kTile * D / 2;        // one packed tile
-  static constexpr int kSmem = 1024 + (kTiles + 4) * kOperand + 3 * kPacked;  // two packed slots of keys, one of values
+  static constexpr int kKeySlots = D == 128 ? 1 : 2;   // of two tiles
+  static constexpr int kOperands = kTiles + 2 * kKeySlots + 2;
+  static constexpr int kSmem = 1024 + kOperands * kOperand + 3 * kPacked;  // two packed slots of keys, one of values
   static constexpr int kColumns = kTiles == 2 ? 512 : 256;
   static constexpr int kOutColumn = kTiles * kTile;    // first column of O
   static constexpr int kSoftWarps = 8 * kTiles;
@@ -68,24 +74,19 @@ IRIS_DEV bool unpack_tile(const AttendParams& p, Shared& sh, int k, const uint32
   using C = Cfg<D, 1>;
   constexpr int kGroups = D / 32;
   const int warp = tid >> 5, lane = tid & 31;
-  const int st = k & 1, slot = keys ? st : 2;
+  const int st = keys ? k % C::kKeySlots : k & 1, slot = keys ? k & 1 : 2;
+  const uint32_t round = keys ? k / C::kKeySlots & 1 : (k >> 1) & 1;
   // what the run of 32 tokens is scaled by, and what is not finite
-  uint32_t most = 0, bad = 0, s2[kGroups];
+  uint32_t most = 0, bad = 0;
 #pragma unroll
   for (int c = 0; c < kGroups; ++c) {
-    s2[c] = (sc[c / 2] >> (16 * (c & 1))) & 0xffffu;
-    const uint32_t mag = s2[c] & 0x7fffu;
+    const uint32_t mag = (sc[c / 2] >> (16 * (c & 1))) & 0x7fffu;
     if (mag >= 0x7c00u) bad |= 1u << c; else most = max(most, mag);
   }
   const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 10);
   const float up = pow2i(27 - e);
-#pragma unroll
-  for (int c = 0; c < kGroups; ++c) {  // the scale twice, as fp16
-    const float v = __half2float(__ushort_as_half(static_cast<unsigned short>(s2[c]))) * up;
-    s2[c] = (bad >> c) & 1u ? (keys ? 0x7fff7fffu : 0u) : Fp16Elem::pack(v, v);
-  }
   if (!wait_all(&sh.raw_full[slot], keys ? (k >> 1) & 1 : k & 1, p.s.err)) return false;
-  if (!wait_all(keys ? &sh.k_empty[st] : &sh.v_empty[st], ((k >> 1) & 1) ^ 1, p.s.err)) return false;
+  if (!wait_all(keys ? &sh.k_empty[st] : &sh.v_empty[st], round ^ 1, p.s.err)) return false;
   if (keys) {
     if (lane == 0) sh.k_exp[k & 3][warp] = e - 27;
   } else {
@@ -96,18 +97,30 @@ IRIS_DEV bool unpack_tile(const AttendParams& p, Shared& sh, int k, const uint32
     }
     if (any) sh.v_bad[st][tid] = static_cast<uint8_t>(bad);
   }
-  const uint32_t src = packed + slot * C::kPacked, dst = operands + st * C::kOperand;
-#pragma unroll
+  const uint32_t src = packed + slot * C::kPacked, dst = operands + st * (keys ? 2 : 1) * C::kOperand;
+#pragma unroll 1
   for (int c = 0; c < kGroups; ++c) {
     const uint4 w4 = lds128(src + packed_at<D>(tid, c));
     const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-    const __half2 s = u32_as_h2(s2[c]);
+    const uint32_t bits = (D == 128 && c >= 2 ? sc[kGroups / 2 - 1] : sc[0]) >> (16 * (c & 1));
+    const float v = __half2float(__ushort_as_half(static_cast<unsigned short>(bits))) * up;
+    float top = v;
+    if (keys) {  // its upper 8 bits (Veltkamp's split), and what is left
+      const float t = __fmul_rn(v, 65537.0f);
+      top = __fsub_rn(t, __fsub_rn(t, v));
+    }
+    const bool odd = (bad >> c) & 1u;
+    const __half2 s = u32_as_h2(odd ? (keys ? 0x7fff7fffu : 0u) : Fp16Elem::pack(top, top)),
+                  r = u32_as_h2(odd ? 0u : Fp16Elem::pack(v - top, v - top));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = w[i], hi = w[i] >> 8;
-      sts128(dst + operand_at(tid, 4 * c + i), h2_as_u32(__hmul2(u32_as_h2(int4_lo_exact(lo)), s)),
-             h2_as_u32(__hmul2(u32_as_h2(int4_hi_exact(lo)), s)), h2_as_u32(__hmul2(u32_as_h2(int4_lo_exact(hi)), s)),
-             h2_as_u32(__hmul2(u32_as_h2(int4_hi_exact(hi)), s)));
+      const __half2 n0 = u32_as_h2(int4_lo_exact(w[i])), n1 = u32_as_h2(int4_hi_exact(w[i])),
+                    n2 = u32_as_h2(int4_lo_exact(w[i] >> 8)), n3 = u32_as_h2(int4_hi_exact(w[i] >> 8));
+      const uint32_t at = dst + operand_at(tid, 4 * c + i);
+      sts128(at, h2_as_u32(__hmul2(n0, s)), h2_as_u32(__hmul2(n1, s)), h2_as_u32(__hmul2(n2, s)), h2_as_u32(__hmul2(n3, s)));
+      if (keys)
+        sts128(at + C::kOperand, h2_as_u32(__hmul2(n0, r)), h2_as_u32(__hmul2(n1, r)), h2_as_u32(__hmul2(n2, r)),
+               h2_as_u32(__hmul2(n3, r)));
     }
   }
   fence_proxy_async_shared();
@@ -184,14 +197,16 @@ IRIS_DEV void issue_products(const AttendParams& p, Shared& sh, int n, int activ
   constexpr uint32_t kScores = umma_idesc(kTile, kTile, false, false), kOut = umma_idesc(kTile, D, false, true);
   auto scores = [&](int i, int k) {
     if (elect_one()) {
-      const uint32_t q = q_tiles + i * C::kOperand, kk = k_tiles + (k & 1) * C::kOperand;
+      const uint32_t q = q_tiles + i * C::kOperand, kk = k_tiles + k % C::kKeySlots * 2 * C::kOperand;
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
+      for (int x = 0; x < 2 * D / 16; ++x) {
+        const int s = x % (D / 16);
         const uint32_t at = (s >> 2) * (kTile * 128) + (s & 3) * 32;
-        umma_ss(tmem + i * kTile, umma_desc(q + at, 16, 1024), umma_desc(kk + at, 16, 1024), kScores, s > 0);
+        umma_ss(tmem + i * kTile, umma_desc(q + at, 16, 1024), umma_desc(kk + at + (x < D / 16 ? 0 : C::kOperand), 16, 1024),
+                kScores, x > 0);
       }
       umma_commit(smem_u32(&sh.s_full[i]));
-      if (i == active - 1) umma_commit(smem_u32(&sh.k_empty[k & 1]));
+      if (i == active - 1) umma_commit(smem_u32(&sh.k_empty[k % C::kKeySlots]));
     }
     __syncwarp();
   };
@@ -217,7 +232,7 @@ IRIS_DEV void issue_products(const AttendParams& p, Shared& sh, int n, int activ
       }
       __syncwarp();
       if (k + 1 < n) {
-        if (i == 0) ok = wait_all(&sh.k_full[(k + 1) & 1], ((k + 1) >> 1) & 1, p.s.err);
+        if (i == 0) ok = wait_all(&sh.k_full[(k + 1) % C::kKeySlots], (k + 1) / C::kKeySlots & 1, p.s.err);
         if (!ok) break;
         umma_fence_after();
         scores(i, k + 1);
@@ -558,8 +573,8 @@ __global__ void __launch_bounds__(Cfg<D, kTiles>::kThreads, 1)
   const int k0 = static_cast<int>(all * split / p.splits), n = static_cast<int>(all * (split + 1) / p.splits) - k0;
 
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const uint32_t q_tiles = smem_u32(base), k_tiles = q_tiles + kTiles * C::kOperand, v_tiles = k_tiles + 2 * C::kOperand;
-  uint8_t* packed = base + (kTiles + 4) * C::kOperand;
+  const uint32_t q_tiles = smem_u32(base), k_tiles = q_tiles + kTiles * C::kOperand, v_tiles = k_tiles + 2 * C::kKeySlots * C::kOperand;
+  uint8_t* packed = base + C::kOperands * C::kOperand;
   if (warp < C::kSoftWarps) {
     regs_take<C::kSoftRegs>();
     const int tile = warp >> 3;
