@@ -54,6 +54,18 @@ IRIS_DEV uint64_t umma_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
          (static_cast<uint64_t>(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// The same with its low word given (umma_desc_low, plus 16-byte units): a row of
+// products that differ in an immediate each.  umma_fresh keeps the compiler from
+// holding all of a loop's descriptors in registers.
+IRIS_DEV uint32_t umma_desc_low(uint32_t addr, uint32_t leading) { return ((addr & 0x3ffffu) >> 4) | (leading >> 4 << 16); }
+IRIS_DEV uint64_t umma_desc_from(uint32_t low, uint32_t stride) {
+  return (static_cast<uint64_t>((stride >> 4) | (1u << 14) | (2u << 29)) << 32) | low;
+}
+IRIS_DEV uint32_t umma_fresh(uint32_t low) {
+  asm volatile("" : "+r"(low));
+  return low;
+}
+
 // D[tmem] (+)= A[smem] B[smem], by one thread.
 IRIS_DEV void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(

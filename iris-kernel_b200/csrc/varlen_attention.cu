@@ -46,8 +46,8 @@ struct Cfg {
   static constexpr int kMmaWarp = kSoftWarps + (kTiles == 2 ? 4 : 8), kCopyWarp = kMmaWarp + 1;
   static constexpr int kThreads = 32 * (kMmaWarp + 4);  // (two warps idle: registers move by warpgroups)
   // Registers a thread: launched with 80 (kTiles 2: 768 x 80 = 61,440) or 96 (640 x 96 = 61,440), then shared out as
-  // 512 x 96 + 128 x 64 + 128 x 32 = 61,440 or 256 x 136 + 256 x 72 + 128 x 56 = 60,416.
-  static constexpr int kSoftRegs = kTiles == 2 ? 96 : 136, kUnpackRegs = kTiles == 2 ? 64 : 72, kIssueRegs = kTiles == 2 ? 32 : 56;
+  // 512 x 88 + 128 x 72 + 128 x 56 = 61,440 or 256 x 136 + 256 x 72 + 128 x 56 = 60,416.
+  static constexpr int kSoftRegs = kTiles == 2 ? 88 : 136, kUnpackRegs = 72, kIssueRegs = 56;
 };
 
 struct Shared {
@@ -197,13 +197,14 @@ IRIS_DEV void issue_products(const AttendParams& p, Shared& sh, int n, int activ
   constexpr uint32_t kScores = umma_idesc(kTile, kTile, false, false), kOut = umma_idesc(kTile, D, false, true);
   auto scores = [&](int i, int k) {
     if (elect_one()) {
-      const uint32_t q = q_tiles + i * C::kOperand, kk = k_tiles + k % C::kKeySlots * 2 * C::kOperand;
+      const uint32_t q = umma_fresh(umma_desc_low(q_tiles + i * C::kOperand, 16)),
+                     kk = umma_fresh(umma_desc_low(k_tiles + k % C::kKeySlots * 2 * C::kOperand, 16));
 #pragma unroll
       for (int x = 0; x < 2 * D / 16; ++x) {
         const int s = x % (D / 16);
-        const uint32_t at = (s >> 2) * (kTile * 128) + (s & 3) * 32;
-        umma_ss(tmem + i * kTile, umma_desc(q + at, 16, 1024), umma_desc(kk + at + (x < D / 16 ? 0 : C::kOperand), 16, 1024),
-                kScores, x > 0);
+        const uint32_t at = ((s >> 2) * (kTile * 128) + (s & 3) * 32) >> 4;
+        umma_ss(tmem + i * kTile, umma_desc_from(q + at, 1024),
+                umma_desc_from(kk + at + (x < D / 16 ? 0 : C::kOperand >> 4), 1024), kScores, x > 0);
       }
       umma_commit(smem_u32(&sh.s_full[i]));
       if (i == active - 1) umma_commit(smem_u32(&sh.k_empty[k % C::kKeySlots]));
@@ -222,10 +223,10 @@ IRIS_DEV void issue_products(const AttendParams& p, Shared& sh, int n, int activ
       if (!ok) break;
       umma_fence_after();
       if (elect_one()) {
-        const uint32_t v = v_tiles + (k & 1) * C::kOperand;
+        const uint32_t v = umma_fresh(umma_desc_low(v_tiles + (k & 1) * C::kOperand, kTile * 128));
 #pragma unroll
         for (int s = 0; s < kTile / 16; ++s)
-          umma_ts(tmem + C::kOutColumn + i * D, tmem + i * kTile + 8 * s + (s < 4 ? 0 : 32), umma_desc(v + s * 2048, kTile * 128, 1024), kOut,
+          umma_ts(tmem + C::kOutColumn + i * D, tmem + i * kTile + 8 * s + (s < 4 ? 0 : 32), umma_desc_from(v + (s * 2048 >> 4), 1024), kOut,
                   k > 0 || s > 0);
         umma_commit(smem_u32(&sh.o_full[i]));
         if (i == active - 1) umma_commit(smem_u32(&sh.v_empty[k & 1]));
