@@ -442,7 +442,7 @@ IRIS_API int iris_b200_int4_paged_varlen_attention(
  *   mass[page, head, slot] = (j >= first_token[b] ? 0 : decay * mass) +
  *     sum over rows and the KV head's query heads of min(1, 2^(logit - lse))
  * over the rows that see j, with logits and visibility as in
- * iris_b200_int4_paged_varlen_attention (keys unrounded) and that call's lse
+ * iris_b200_int4_paged_varlen_attention and that call's lse
  * [tokens, num_q_heads] fp32; a row whose lse is -inf gives nothing.  A token
  * with a key scale that is not finite and a visible row: NaN.
  *   mass [num_pages, num_kv_heads, 16] fp32; first_token [batch] int32 or NULL: 0.

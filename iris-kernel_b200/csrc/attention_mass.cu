@@ -428,9 +428,8 @@ extern "C" int iris_b200_int4_paged_attention_mass(
   p.bf16 = dtype == IRIS_DTYPE_BF16;
   const int64_t tiles = (static_cast<int64_t>(max_pages_per_seq) * kTokPage + kTile - 1) / kTile;
   const int64_t units = static_cast<int64_t>(batch) * num_kv_heads;
-  // about two waves of four blocks an SM: more would load the query rows more often
-  int64_t chunks = (148 * 4 * 2 + units - 1) / units;
-  if (chunks > tiles) chunks = tiles;
+  // a block's start is about three tiles long, and as much again where it has many query rows to load
+  const int64_t chunks = best_chunks(units, tiles, 148 * 4, cu_seqlens == nullptr && group <= kCols ? 3 : 6, tiles);
   p.per = static_cast<int32_t>((tiles + chunks - 1) / chunks);
   p.chunks = static_cast<int32_t>((tiles + p.per - 1) / p.per);
   const int64_t most = cu_seqlens == nullptr ? group : static_cast<int64_t>(tokens) * group;

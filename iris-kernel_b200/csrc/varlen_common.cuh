@@ -394,6 +394,24 @@ IRIS_DEV void load_packed(uint8_t* dst, const CUtensorMap* map, int32_t page, in
   __syncwarp();
 }
 
+// Host: into how many chunks to cut each of `units` rows of `tiles` tiles, for a
+// GPU that runs `slots` blocks at once: the one whose rounds of blocks take the
+// least, a block costing `start` tiles before its first.
+inline int64_t best_chunks(int64_t units, int64_t tiles, int64_t slots, int64_t start, int64_t most) {
+  if (most > 1024) most = 1024;
+  if (most < 1) most = 1;
+  int64_t best = 1, least = INT64_MAX;
+  for (int64_t n = 1; n <= most; ++n) {
+    const int64_t cost = (units * n + slots - 1) / slots * ((tiles + n - 1) / n + start);
+    if (cost < least) {
+      least = cost;
+      best = n;
+    }
+    if (units * n > 4 * slots) break;  // finer cuts only add starts
+  }
+  return best;
+}
+
 // Host: the cache [pages, 16, Hkv, D / 2] as (row bytes, 16 tokens, heads, pages), a box of one page of one head.
 inline bool packed_map(CUtensorMap* map, const void* base, int dim, int hkv, int64_t num_pages) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,

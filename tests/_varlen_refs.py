@@ -4,14 +4,15 @@ be from them.
 
 Half a step of a rounding: fp16 2^-11, bf16 2^-8 of the value (`half_step`).
 
-* Attention.  A stored key or value, nibble * scale, is rounded to fp16: 2^-11
-  of it.  So a logit is off by at most delta_j = scale * sum_d |q_d k_jd| *
-  2^-11 (the cap and the bias do not make it more), and by what fp32 sums of 128
-  products lose, 2^-20 of the same sum; the largest over the visible tokens is
-  delta.  Weights move by a factor of e^(2 delta) at most, each is rounded to
-  fp16 once more (2^-11 of it, or 2^-25 of 1/256 of the largest where it is
-  tiny), and so is the value.  The output is then rounded to its type.
-* lse: delta / ln 2, and 2^-20 of its size for fp32.
+* Attention.  Keys enter the products exactly, as do queries; a logit is off by
+  what fp32 sums lose: at most 32 steps of the tensor cores, each with 2^-23 of the
+  running sum, so 2^-18 of sum_d |q_d k_jd| * scale (the cap and the bias do not
+  make it more, and round with 2^-22 of their own size, which that covers or the
+  2^-18 below); the largest over the visible tokens is delta.  Weights move by a
+  factor of e^(2 delta) at most, each is rounded to fp16 (2^-11 of it, or 2^-25 of
+  1/256 of the largest where it is tiny), and so is the value, nibble * scale.  The
+  output is then rounded to its type.
+* lse: delta / ln 2, and 2^-18 of its size and of 1 for fp32.
 * Weights (mass): keys are exact there; a logit is off by 2^-20 of sum |q k| *
   scale and of its own size and the lse's; each weight by e to that, sums of
   fp32 by 2^-20 of the sum.  Each of a token's weights below 2^-126 may count as
@@ -113,7 +114,7 @@ def attend_ref(query, cache, bt, lens, cu, dtype, **kw):
                 o = w @ np.where(bad, 0.0, value)
                 hit = (seen.astype(float) @ bad.astype(float)) > 0  # [rows, dims]
                 o = np.where(hit[None], np.nan, o)
-                delta = (size.max(-1, keepdims=True) * (half + 2.0 ** -20))
+                delta = size.max(-1, keepdims=True) * 2.0 ** -18
                 most = np.abs(w) @ np.abs(np.where(bad, 0.0, value))
                 big = np.abs(np.where(bad, 0.0, value)).max()
                 f = most * (np.expm1(2 * delta) + 2 * half + 2.0 ** -18) + n * 2.0 ** -33 * big / np.maximum(total, 1.0)
@@ -122,7 +123,7 @@ def attend_ref(query, cache, bt, lens, cu, dtype, **kw):
                 rows = slice(h * group, (h + 1) * group)
                 out[r0:r1, rows], far[r0:r1, rows] = o.transpose(1, 0, 2), f.transpose(1, 0, 2)
                 lse[r0:r1, rows] = s.T
-                lse_far[r0:r1, rows] = (delta[..., 0] / math.log(2.0) + 2.0 ** -20 * (1 + np.abs(s))).T
+                lse_far[r0:r1, rows] = (delta[..., 0] / math.log(2.0) + 2.0 ** -18 * (1 + np.abs(s))).T
     return out, lse, far, lse_far
 
 
