@@ -413,7 +413,7 @@ IRIS_API size_t iris_b200_varlen_attention_workspace_bytes(int64_t tokens, int32
  * [batch + 1], rising from 0; NULL: one row each, tokens == batch); they are
  * the last of its seq_lens[b] cached tokens, row i at place pos =
  * seq_lens[b] - rows + i.  No counterpart in the reference.
- *   logit = softmax_scale * q.k;  logit_cap > 0: logit_cap * tanh(logit / logit_cap)
+ *   logit = softmax_scale * q.k;  logit_cap > 0 (at most 1e20): logit_cap * tanh(logit / logit_cap)
  *   slopes [num_q_heads] fp32 or NULL: - slopes[h] * |pos - j|
  * Token j is visible iff j < seq_lens[b] and j >= first_visible[row] (int32
  * [tokens]; NULL: 0) and (j < prefix_lens[b] (int32 [batch]; NULL: 0) or (j <=
@@ -457,7 +457,7 @@ IRIS_API int iris_b200_int4_paged_attention_mass(
     int32_t page_size, int32_t max_pages_per_seq, int32_t window, float logit_cap, float softmax_scale, float decay,
     int32_t dtype, int32_t* error_word, void* stream);
 
-/* Bytes of device workspace iris_b200_int4_paged_evict needs. */
+/* Bytes of device workspace iris_b200_int4_paged_evict needs; none where budget >= 16 * max_pages_per_seq. */
 IRIS_API size_t iris_b200_evict_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t budget,
                                                 int32_t recent_tokens);
 

@@ -110,7 +110,7 @@ IRIS_DEV void load_columns(const MassParams& p, MassShared& sh, const Span& sp, 
     if (valid) {
       pos = len - sp.count + i;
       lse = __ldg(p.lse + token * p.s.hq + head);
-      factor = kCap ? p.s.scale * back / p.s.cap : p.s.scale * kLog2e * back;
+      factor = fminf(kCap ? p.s.scale * back / p.s.cap : p.s.scale * kLog2e * back, 1e38f);
       slope = kBias ? -__ldg(p.s.slopes + head) * kLog2e : 0.0f;
       if (lse != -__int_as_float(0x7f800000))  // (a row that saw nothing gives nothing)
         see = row_sight(pos, p.s.first_visible != nullptr ? __ldg(p.s.first_visible + token) : 0,
@@ -383,7 +383,7 @@ extern "C" int iris_b200_int4_paged_attention_mass(
     int32_t page_size, int32_t max_pages_per_seq, int32_t window, float logit_cap, float softmax_scale, float decay,
     int32_t dtype, int32_t* error_word, void* stream) {
   if (tokens < 0 || batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || window < 0 ||
-      !(logit_cap >= 0.0f) || !(softmax_scale > 0.0f) || (dtype != IRIS_DTYPE_FP16 && dtype != IRIS_DTYPE_BF16))
+      !(logit_cap >= 0.0f && logit_cap <= 1e20f) || !(softmax_scale > 0.0f) || (dtype != IRIS_DTYPE_FP16 && dtype != IRIS_DTYPE_BF16))
     return IRIS_EINVAL;
   if (page_size != kTokPage || (head_dim != 64 && head_dim != 128)) return IRIS_EUNSUPPORTED;
   if (cu_seqlens == nullptr && tokens != batch) return IRIS_EINVAL;

@@ -647,7 +647,7 @@ NewTokens new_tokens(const Tensor& query, const Cache& c, const Tensor& bt, cons
   n.scale = static_cast<float>(scale);
   require(n.scale > 0.0f && n.scale <= 3.0e38f, PyExc_ValueError, "softmax_scale must be positive and finite");
   n.cap = static_cast<float>(number(cap_arg));
-  require(n.cap >= 0.0f && n.cap <= 3.0e38f, PyExc_ValueError, "logit_cap must be finite and not negative");
+  require(n.cap >= 0.0f && n.cap <= 1.0e20f, PyExc_ValueError, "logit_cap must lie in [0, 1e20]");
   require(n.tokens <= INT32_MAX && n.hq <= INT32_MAX && n.batch <= INT32_MAX && c.heads <= INT32_MAX, PyExc_ValueError,
           "too many tokens, heads or sequences");
   if (n.tokens > 0) {
@@ -792,8 +792,10 @@ PyObject* evict(PyObject* const* a) {
   if (batch > 0) {
     require(c.num_pages > 0, PyExc_IndexError, "block_table contains an invalid physical page id");
     require(batch <= INT32_MAX, PyExc_ValueError, "too many sequences");
-    const size_t bytes = iris_b200_evict_workspace_bytes(static_cast<int32_t>(batch), static_cast<int32_t>(c.heads),
-                                                         budget, recent);
+    const size_t bytes = budget >= static_cast<int64_t>(table.width) * 16
+                             ? 0
+                             : iris_b200_evict_workspace_bytes(static_cast<int32_t>(batch), static_cast<int32_t>(c.heads),
+                                                               budget, recent);
     Tensor ws;
     if (bytes > 0) ws = workspace(bytes, device);
     launch("iris_b200_int4_paged_evict", device, [&](int32_t* word, void* stream) {

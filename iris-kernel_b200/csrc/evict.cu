@@ -428,7 +428,9 @@ extern "C" int iris_b200_int4_paged_evict(void* k_data, void* v_data, void* k_sc
   if (!aligned_to(k_data, 16) || !aligned_to(v_data, 16) || !aligned_to(k_scale, 8) || !aligned_to(v_scale, 8) ||
       !aligned_to(mass, 16))
     return IRIS_EALIGN;
-  const size_t need = iris_b200_evict_workspace_bytes(batch, num_kv_heads, budget, recent_tokens);
+  // (a table that holds no more than the budget has nothing to move)
+  const size_t need = budget >= max_pages_per_seq * kTokPage
+                          ? 0 : iris_b200_evict_workspace_bytes(batch, num_kv_heads, budget, recent_tokens);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return IRIS_EWORKSPACE;
   if (!aligned_to(workspace, 4)) return IRIS_EALIGN;
   EvictParams p = {};

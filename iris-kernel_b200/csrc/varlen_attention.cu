@@ -311,7 +311,7 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
   const uint32_t s_at = lanes + tile * kTile + half * 64, o_at = lanes + C::kOutColumn + tile * D + half * (D / 2);
   const bool busy = __any_sync(0xffffffffu, valid);
   const float back = n > 0 ? sh.back[tile][local] : 1.0f;
-  const float unit = kCap ? p.s.scale * back / p.s.cap : p.s.scale * kLog2e * back;
+  const float unit = fminf(kCap ? p.s.scale * back / p.s.cap : p.s.scale * kLog2e * back, 1e38f);  // (0 times it is 0)
   const float cap2 = p.s.cap * kLog2e;
   const float slope2 = kBias ? -__ldg(p.s.slopes + head) * kLog2e : 0.0f;
   auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + tile * 4 + quarter) : "memory"); };  // the rows' two warps
@@ -320,8 +320,9 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
   bool ok = true;
 #pragma unroll 1
   for (int k = 0; k < n; ++k) {
-    if (!(ok = wait_all(&sh.s_full[tile], k & 1, p.s.err))) break;
-    if (!(ok = wait_all(&sh.v_full[k & 1], (k >> 1) & 1, p.s.err))) break;
+    // (once a wait has given up no other is made, but the two warps go on meeting)
+    ok = ok && wait_all(&sh.s_full[tile], k & 1, p.s.err);
+    ok = ok && wait_all(&sh.v_full[k & 1], (k >> 1) & 1, p.s.err);
     umma_fence_after();
     if (busy) {
       const int32_t base = tiles.at(k0 + k) * kTile + half * 64;
@@ -389,7 +390,7 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
         const float to = rise ? rintf(top) : m;  // (whole: what is taken off and added below is then exact)
         if (k > 0) {
           const float by = (rise ? ex2(m - to) : 1.0f) * pow2i(max(ref - top_e, -126));
-          if (!(ok = wait_all(&sh.o_full[tile], (k - 1) & 1, p.s.err))) break;
+          ok = ok && wait_all(&sh.o_full[tile], (k - 1) & 1, p.s.err);
           umma_fence_after();
 #pragma unroll 1
           for (int c = 0; c < D / 64; ++c) {
@@ -456,8 +457,9 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
     umma_fence_after();
   }
   sh.top[n & 1][tile][half][local] = l;
-  if (!busy || !ok) return;
+  if (!busy) return;
   meet();
+  if (!ok) return;
   l += sh.top[n & 1][tile][half ^ 1][local];
   const uint32_t spoilt = sh.spoilt[tile][local];
   const bool whole = p.splits == 1;
@@ -787,7 +789,7 @@ extern "C" int iris_b200_int4_paged_varlen_attention(
     int64_t num_pages, int32_t page_size, int32_t max_pages_per_seq, int32_t window, float logit_cap, float softmax_scale,
     int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* error_word, void* stream) {
   if (tokens < 0 || batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || window < 0 ||
-      !(logit_cap >= 0.0f) || !(softmax_scale > 0.0f) || (dtype != IRIS_DTYPE_FP16 && dtype != IRIS_DTYPE_BF16))
+      !(logit_cap >= 0.0f && logit_cap <= 1e20f) || !(softmax_scale > 0.0f) || (dtype != IRIS_DTYPE_FP16 && dtype != IRIS_DTYPE_BF16))
     return IRIS_EINVAL;
   if (page_size != kTokPage || (head_dim != 64 && head_dim != 128)) return IRIS_EUNSUPPORTED;
   if (cu_seqlens == nullptr && tokens != batch) return IRIS_EINVAL;

@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
       const int32_t pos = off + i;
       const Sight see = row_sight(pos, p.s.first_visible != nullptr ? __ldg(p.s.first_visible + token) : 0, prefix,
                                   p.s.window, len);
-      sh.row[c] = make_float4(kCap ? p.s.scale * back / p.s.cap : p.s.scale * kLog2e * back, kHead, kMinusInf, kMinusInf);
+      sh.row[c] = make_float4(fminf(kCap ? p.s.scale * back / p.s.cap : p.s.scale * kLog2e * back, 1e38f), kHead, kMinusInf, kMinusInf);
       sh.more[c] = make_float2(__int_as_float(pos), kBias ? -__ldg(p.s.slopes + head) * kLog2e : 0.0f);
       sh.sight[c] = make_int4(see.a0, see.a1, see.b0, see.b1);
       atomicMax(&sh.all_lo, see.b0);

@@ -204,8 +204,10 @@ class BudgetDecodeStep:
         # the warm-up sees no tokens: it changes neither the cache nor its weights
         lens = seq_lens.clone()
         seq_lens.zero_()
-        _capture(self.graph, dev, self._calls)
-        seq_lens.copy_(lens)
+        try:
+            _capture(self.graph, dev, self._calls)
+        finally:
+            seq_lens.copy_(lens)
 
     def _calls(self):
         fused_mrope_int4_paged_append(self.key, self.value, self.positions, self.slots, self.cos, self.sin,

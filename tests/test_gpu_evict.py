@@ -135,3 +135,11 @@ def test_errors_leave_the_sequence_alone():
     with pytest.raises(ValueError, match="overlap"):
         fused_int4_paged_evict(*args, args[6], budget=100)
     _runtime.check_errors()
+
+
+def test_a_budget_that_no_sequence_can_pass():
+    bt, cache, mass = _batch([200, 40], 2, 64, 4)
+    dev, new = _evict(bt, cache, mass, [200, 40], budget=2 ** 31 - 1)
+    assert new.tolist() == [200, 40]
+    for x, w in zip(dev, (*cache, mass)):
+        assert x.cpu().numpy().tobytes() == w.tobytes()

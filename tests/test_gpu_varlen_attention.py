@@ -283,7 +283,8 @@ def test_errors():
         f(*a, slopes=torch.ones(2, device="cuda"))
     with pytest.raises(TypeError):
         f(*a, first_visible=torch.zeros(14, device="cuda"))
-    for kw in (dict(window=-1), dict(logit_cap=-1.0), dict(logit_cap=float("nan")), dict(softmax_scale=-0.5)):
+    for kw in (dict(window=-1), dict(logit_cap=-1.0), dict(logit_cap=float("nan")), dict(logit_cap=3e38),
+               dict(softmax_scale=-0.5)):
         with pytest.raises(ValueError):
             f(*a, **kw)
     with pytest.raises(NotImplementedError):
@@ -346,3 +347,19 @@ def test_single_tokens_of_wide_groups(hq, lens):
     for how in ({}, dict(logit_cap=5.0), dict(slopes=(0.1 * np.arange(hq)).astype(np.float32)), dict(window=77)):
         Case([1] * len(lens), lens, hq, 1, 64 if hq % 2 else 128, seed=hq, offsets=False, **how).spoil_tails().check()
         Case([1] * len(lens), lens, hq, 1, 128 if hq % 2 else 64, seed=hq, offsets=True, **how).spoil_tails().check()
+
+
+@pytest.mark.parametrize("how", [dict(logit_cap=1e-30), dict(logit_cap=1e20), dict(softmax_scale=1e-38), dict(logit_cap=1e-3, softmax_scale=1e30)])
+def test_extreme_caps_and_scales(how):
+    """A cap far below the logits, one far above them, logits that vanish: finite, and as the definition has it."""
+    for new, lens in (([40], [300]), ([1, 3], [200, 33])):
+        Case(new, lens, 4, 2, 64, seed=34, **how).check()
+
+
+def test_keys_are_exact():
+    """The log-sum-exp of a row that sees one token is its logit: fp32's, not fp16's."""
+    for new, lens in (([200], [200]), ([1, 1], [300, 40])):
+        c = Case(new, lens, 4, 2, 128, seed=35, window=1)
+        out, lse = c.run()
+        want = c.want()[1]
+        assert np.abs(lse.double().cpu().numpy() - want).max() < 2.0 ** -19 * max(1.0, np.abs(want).max())

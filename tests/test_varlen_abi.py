@@ -25,7 +25,7 @@ def _attend(**kw):
 
 SHARED = [
     (dict(tokens=-1), EINVAL), (dict(batch=-1), EINVAL), (dict(hq=7), EINVAL), (dict(hkv=0), EINVAL), (dict(window=-1), EINVAL),
-    (dict(cap=-1.0), EINVAL), (dict(cap=math.nan), EINVAL), (dict(scale=0.0), EINVAL), (dict(scale=math.nan), EINVAL),
+    (dict(cap=-1.0), EINVAL), (dict(cap=math.nan), EINVAL), (dict(cap=2e20), EINVAL), (dict(scale=0.0), EINVAL), (dict(scale=math.nan), EINVAL),
     (dict(dtype=2), EINVAL), (dict(cu=None), EINVAL), (dict(batch=0), EINVAL), (dict(num_pages=0), EINVAL),
     (dict(max_pages=0), EINVAL), (dict(query=None), EINVAL), (dict(k_scale=None), EINVAL), (dict(seq_lens=None), EINVAL),
     (dict(page_size=32), EUNSUPPORTED), (dict(head_dim=96), EUNSUPPORTED), (dict(head_dim=256), EUNSUPPORTED),
@@ -101,6 +101,7 @@ def test_evict_workspace():
     assert need(2, 2, 32, 8) == 2 * 2 * 2 * 24 * 4
     assert need(0, 2, 32, 8) == 0 and need(2, 2, 32, 32) == 0
     assert _evict(batch=0) == 0
+    assert _evict(budget=2 ** 31 - 1, mass=P + 4, workspace=None, workspace_bytes=0) == EALIGN  # not EWORKSPACE
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="checks the no-CUDA error path")
