@@ -446,8 +446,9 @@ IRIS_API int iris_b200_int4_paged_varlen_attention(
  * [tokens, num_q_heads] fp32; a row whose lse is -inf gives nothing.  A token
  * with a key scale that is not finite and a visible row: NaN.
  *   mass [num_pages, num_kv_heads, 16] fp32; first_token [batch] int32 or NULL: 0.
- * No two sequences may share a page.  Sums do not depend on timing.  Limits and
- * alignments as iris_b200_int4_paged_varlen_attention.
+ * No two sequences may share a page; tokens behind a page id outside the cache
+ * get no weight written.  Sums do not depend on timing.  Limits and alignments
+ * as iris_b200_int4_paged_varlen_attention.
  */
 IRIS_API int iris_b200_int4_paged_attention_mass(
     const void* query, int64_t query_stride, const float* lse, const void* k_data, const void* k_scale,

@@ -200,7 +200,11 @@ __global__ void __launch_bounds__(128, 4) attention_mass_kernel(const __grid_con
     load_packed<D>(packed, &k_map, checked_page(p.s, page_at(0)), first(0), len, h, &sh.here, lane);
     if (n > 1) copy_page = page_at(1);
   }
-  int32_t page = page_of(p.s, b, first(0) + tid, len);  // of this thread's token
+  // This thread's token's page.  An id outside the cache is read as page 0, whose weights are others': none is written.
+  auto in_cache = [&](int32_t id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(p.s.num_pages); };
+  int32_t page = raw_page(p.s, b, first(0) + tid, len);
+  bool good = in_cache(page);
+  page = checked_page(p.s, page);
   fetch(page, first(0) + tid);
   int32_t later = n > 1 ? raw_page(p.s, b, first(1) + tid, len) : 0;
   if (warp == 0) umma_alloc(&sh.tmem, C::kColumns);
@@ -225,7 +229,8 @@ __global__ void __launch_bounds__(128, 4) attention_mass_kernel(const __grid_con
   for (int k = 0; ok && k < n; ++k) {
     const int32_t base_j = first(k), j = base_j + tid;
     float* slot_mass = p.mass + (static_cast<int64_t>(page) * p.s.hkv + h) * kTokPage + j % kTokPage;
-    const float old = j < len && j < fresh ? *slot_mass : 0.0f;
+    const bool writes = j < len && good;
+    const float old = writes && j < fresh ? *slot_mass : 0.0f;
     float sc[kGroups];
     {
       bool odd = false;  // a scale that is not finite makes the token's logits NaN
@@ -238,6 +243,7 @@ __global__ void __launch_bounds__(128, 4) attention_mass_kernel(const __grid_con
       if (odd) sc[0] = __int_as_float(0x7fffffff);
     }
     if (k + 1 < n) {
+      good = in_cache(later);
       page = checked_page(p.s, later);
       fetch(page, first(k + 1) + tid);
       if (k + 2 < n) later = raw_page(p.s, b, first(k + 2) + tid, len);
@@ -341,7 +347,7 @@ __global__ void __launch_bounds__(128, 4) attention_mass_kernel(const __grid_con
       load_packed<D>(packed, &k_map, checked_page(p.s, copy_page), first(k + 1), len, h, &sh.here, lane);
       if (k + 2 < n) copy_page = page_at(k + 2);
     }
-    if (ok && j < len) *slot_mass = fmaf(old, p.decay, sum.x + sum.y);
+    if (ok && writes) *slot_mass = fmaf(old, p.decay, sum.x + sum.y);
   }
   if (!ok) {  // a wait gave up: copies that are under way land before the block ends
     for (uint32_t parity = 0; parity < 2; ++parity) mbar_wait_bounded(&sh.here, parity, p.s.err);

@@ -102,7 +102,8 @@ def fused_int4_paged_attention_mass(
     tokens before: None after a prompt, ``seq_lens - 1`` after a decode step.
 
     A weight is at most 1; a row whose lse is -inf gives nothing.  A page must
-    belong to one sequence only."""
+    belong to one sequence only; tokens behind a bad page id get no weight
+    written."""
     _runtime.ops().attention_mass(query, lse, k_data, k_scale, block_table, seq_lens, mass, cu_seqlens, first_token, decay,
                                   page_size, group_size, softmax_scale, logit_cap, slopes, window, prefix_lens,
                                   first_visible)

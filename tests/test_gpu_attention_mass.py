@@ -135,3 +135,24 @@ def test_errors():
         with pytest.raises(error):
             f(*good[:at], torch.tensor(x, dtype=torch.int32, device="cuda"), *good[at + 1:])
     _check(c)
+
+
+@pytest.mark.parametrize("place", [1, 18])
+@pytest.mark.parametrize("bad", [-1, 2 ** 31 - 1])
+def test_a_bad_page_id_writes_to_no_page(place, bad):
+    from iris_kernel.varlen_attention import fused_int4_paged_attention_mass as f
+
+    c = Case([3], [300], 4, 2, 64, seed=27)
+    a = c.args()
+    lse, mass = c.run()[1], _mass(c)
+    table = c.bt.copy()
+    table[table == 0] = table[0, place]  # page 0 is nobody's
+    table[0, place] = bad
+    got = _dev(mass)
+    with pytest.raises(IndexError):
+        f(a[0], lse, a[1], a[3], _dev(table), a[6], got, a[7])
+    torch.cuda.synchronize()
+    others = np.setdiff1d(np.arange(mass.shape[0]), table[0, :19])
+    assert 0 in others and np.array_equal(got.cpu().numpy()[others], mass[others])
+    mine = table[0, :18 if place == 18 else 19][np.arange(18 if place == 18 else 19) != place]
+    assert (got.cpu().numpy()[mine] != mass[mine]).any(axis=(1, 2)).all()
