@@ -228,7 +228,7 @@ struct Sight {
 IRIS_DEV Sight row_sight(int32_t pos, int32_t first, int32_t prefix, int32_t window, int32_t len) {
   Sight s;
   s.a0 = max(first, 0);
-  s.a1 = min(prefix, len);
+  s.a1 = max(min(prefix, len), 0);  // (differences of places must fit 32 bits)
   s.b0 = window > 0 ? max(s.a0, pos - window + 1) : s.a0;
   s.b1 = min(pos + 1, len);
   return s;
