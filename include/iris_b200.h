@@ -401,7 +401,7 @@ IRIS_API int iris_b200_int4_page_bounds(const void* k_data, const void* k_scale,
                                         int32_t page_size, int32_t max_pages_per_seq, int32_t* error_word,
                                         void* stream);
 
-/* Bytes of device workspace iris_b200_int4_paged_varlen_attention needs (0: none). */
+/* Bytes of device workspace iris_b200_int4_paged_varlen_attention needs (0: none, or sizes that it refuses). */
 IRIS_API size_t iris_b200_varlen_attention_workspace_bytes(int64_t tokens, int32_t batch, int32_t num_q_heads,
                                                            int32_t num_kv_heads, int32_t head_dim,
                                                            int32_t max_pages_per_seq, int32_t window, int32_t has_prefix,

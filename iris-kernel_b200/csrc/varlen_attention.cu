@@ -649,6 +649,11 @@ int sm_count(int device) {
   return known[device];
 }
 
+// Rows, places and page offsets are 32-bit numbers in the kernels.
+bool too_long(int64_t tokens, int32_t group, int32_t max_pages) {
+  return tokens > INT32_MAX / 2 / group || max_pages > INT32_MAX / 2 / kTokPage;
+}
+
 // Which kernels run, and how the work is cut.
 //
 // Sequences of at most kFewRows rows go to varlen_few_kernel, the others to
@@ -775,7 +780,11 @@ extern "C" size_t iris_b200_varlen_attention_workspace_bytes(int64_t tokens, int
                                                              int32_t num_kv_heads, int32_t head_dim,
                                                              int32_t max_pages_per_seq, int32_t window, int32_t has_prefix,
                                                              int32_t has_offsets, int32_t device) {
-  if (tokens <= 0 || batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0) return 0;
+  // (what the operator refuses, or is done with at once, needs none; the plan is only right for the rest)
+  if (tokens <= 0 || batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 ||
+      (head_dim != 64 && head_dim != 128) || max_pages_per_seq <= 0 || window < 0 ||
+      too_long(tokens, num_q_heads / num_kv_heads, max_pages_per_seq) || (has_offsets == 0 && tokens != batch))
+    return 0;
   const Plan r = plan(tokens, batch, num_q_heads / num_kv_heads, has_offsets != 0, num_kv_heads, max_pages_per_seq, window,
                       has_prefix != 0, sm_count(device));
   return static_cast<size_t>(r.many_parts + r.few_parts) * (head_dim + 1) * 4;
@@ -799,9 +808,7 @@ extern "C" int iris_b200_int4_paged_varlen_attention(
       block_table == nullptr || seq_lens == nullptr || output == nullptr)
     return IRIS_EINVAL;
   const int32_t group = num_q_heads / num_kv_heads;
-  // rows, places and page offsets are 32-bit numbers in the kernel
-  if (tokens * group > INT32_MAX / 2 || num_pages > INT32_MAX || max_pages_per_seq > INT32_MAX / 2 / kTokPage)
-    return IRIS_EUNSUPPORTED;
+  if (too_long(tokens, group, max_pages_per_seq) || num_pages > INT32_MAX) return IRIS_EUNSUPPORTED;
   if (!aligned_to(query, 16) || query_stride % 8 != 0 || !aligned_to(k_data, 16) || !aligned_to(v_data, 16) ||
       !aligned_to(k_scale, 8) || !aligned_to(v_scale, 8) || !aligned_to(output, 16))
     return IRIS_EALIGN;

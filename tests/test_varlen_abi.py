@@ -57,6 +57,19 @@ def test_attention_workspace():
     assert need(8192, 2, 32, 8, 128, 256, 0, 0, 1, 0) < 16 << 20
 
 
+@pytest.mark.parametrize("change", [
+    dict(max_pages=0), dict(max_pages=-5), dict(max_pages=-(2 ** 31)), dict(max_pages=1 << 27), dict(max_pages=2 ** 31 - 1),
+    dict(head_dim=0), dict(head_dim=-64), dict(head_dim=96), dict(window=-3), dict(tokens=1 << 29), dict(tokens=2 ** 63 - 1),
+    dict(batch=-1), dict(hq=7), dict(hkv=0), dict(hq=0), dict(offsets=0)])
+def test_attention_workspace_of_what_is_refused(change):
+    """A size is asked for before the call that refuses the sizes: no workspace, and the process goes on."""
+    a = dict(tokens=8, batch=2, hq=8, hkv=2, head_dim=64, max_pages=5000, window=0, prefix=0, offsets=1, device=0)
+    need = lib.iris_b200_varlen_attention_workspace_bytes
+    assert need(*a.values()) > 0
+    a.update(change)
+    assert need(*a.values()) == 0
+
+
 def _mass(**kw):
     a = dict(query=P, query_stride=512, lse=P, k_data=P, k_scale=P, block_table=P, stride=4, seq_lens=P, cu=P, slopes=None,
              prefix=None, first=None, first_token=None, mass=P, tokens=8, batch=2, hq=8, hkv=2, head_dim=64, num_pages=4,
