@@ -473,7 +473,9 @@ IRIS_API size_t iris_b200_evict_workspace_bytes(int32_t batch, int32_t num_kv_he
  *   new_lens [batch]: min(seq_lens, budget); kept [batch, num_kv_heads, budget]
  *   or NULL: the index that each place's token had, -1 behind the last.
  * A sequence with a bad length or page id stays as it is.  No two sequences may
- * share a page.  page_size 16, head_dim 64 or 128.  k_data, v_data and mass
+ * share a page.  Neither output may overlap the other, seq_lens (no update in
+ * place: other heads still read it), block_table, the weights, the cache or the
+ * workspace (IRIS_EINVAL).  page_size 16, head_dim 64 or 128.  k_data, v_data and mass
  * 16-byte aligned, the scales 8-byte, the workspace 4-byte; the workspace's
  * contents do not matter and belong to one call at a time.
  */

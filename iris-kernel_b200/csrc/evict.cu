@@ -397,6 +397,16 @@ cudaError_t launch_evict(EvictParams p, cudaStream_t stream) {
                                static_cast<unsigned>(size), smem, stream, p);
 }
 
+// Bytes that an argument covers.
+struct Range {
+  const void* at;
+  uint64_t bytes;
+  bool meets(const Range& o) const {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(at), b = reinterpret_cast<uintptr_t>(o.at);
+    return bytes > 0 && o.bytes > 0 && (a < b ? b - a < bytes : a - b < o.bytes);
+  }
+};
+
 }  // namespace
 }  // namespace iris
 
@@ -433,6 +443,17 @@ extern "C" int iris_b200_int4_paged_evict(void* k_data, void* v_data, void* k_sc
                           ? 0 : iris_b200_evict_workspace_bytes(batch, num_kv_heads, budget, recent_tokens);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return IRIS_EWORKSPACE;
   if (!aligned_to(workspace, 4)) return IRIS_EALIGN;
+  // Clusters of other heads read lengths and tables after the first has written: neither output may lie in what is read,
+  // or in the other one.
+  const uint64_t heads = num_kv_heads, rows = static_cast<uint64_t>(num_pages) * kTokPage * heads, sequences = batch;
+  const uint64_t table = (sequences - 1) * static_cast<uint64_t>(block_table_stride > 0 ? block_table_stride : 0) + max_pages_per_seq;
+  const Range read[] = {{seq_lens, sequences * 4}, {block_table, table * 4}, {mass, rows * 4},
+                        {k_data, rows * (head_dim / 2)}, {v_data, rows * (head_dim / 2)}, {k_scale, rows * (head_dim / 16)},
+                        {v_scale, rows * (head_dim / 16)}, {workspace, need}};
+  const Range lens_out = {new_lens, sequences * 4}, kept_out = {kept, kept != nullptr ? sequences * heads * budget * 4 : 0};
+  if (lens_out.meets(kept_out)) return IRIS_EINVAL;
+  for (const Range& r : read)
+    if (lens_out.meets(r) || kept_out.meets(r)) return IRIS_EINVAL;
   EvictParams p = {};
   p.k_data = static_cast<uint8_t*>(k_data);
   p.v_data = static_cast<uint8_t*>(v_data);

@@ -109,6 +109,25 @@ def test_evict_status(kw, status):
     assert _evict(**kw) == status
 
 
+APART = {k: (i + 1) << 20 for i, k in enumerate(
+    ("k_data", "v_data", "k_scale", "v_scale", "mass", "block_table", "seq_lens", "new_lens", "kept", "workspace"))}
+
+
+@pytest.mark.parametrize("out,size", [("new_lens", 2 * 4), ("kept", 2 * 2 * 32 * 4)])
+@pytest.mark.parametrize("other,other_size", [("seq_lens", 2 * 4), ("block_table", (4 + 4) * 4), ("mass", 4 * 2 * 16 * 4),
+                                              ("k_data", 4 * 16 * 2 * 32), ("v_scale", 4 * 16 * 2 * 4), ("workspace", 768), (None, 0)])
+def test_evict_outputs_apart(out, size, other, other_size):
+    """An output in what the kernel's other clusters still read, or in the other output, is refused: the first byte and the last."""
+    other = other or {"new_lens": "kept", "kept": "new_lens"}[out]
+    other_size = other_size or {"new_lens": 2 * 4, "kept": 2 * 2 * 32 * 4}[other]
+    at = APART[other]
+    for where in (at, at + other_size - 4, at - size + 4):
+        assert _evict(**dict(APART, **{out: where}), workspace_bytes=768) == EINVAL
+    if out == "new_lens" and other == "seq_lens" and not torch.cuda.is_available():  # (no GPU here: what is accepted ends at the launch)
+        for where in (at + other_size, at - size):
+            assert _evict(**dict(APART, **{out: where}), workspace_bytes=768) not in (0, EINVAL)
+
+
 def test_evict_workspace():
     need = lib.iris_b200_evict_workspace_bytes
     assert need(2, 2, 32, 8) == 2 * 2 * 2 * 24 * 4
