@@ -385,7 +385,7 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
       meet();
       top = fmaxf(top, sh.top[k & 1][tile][half ^ 1][local]);
       // raise the row's reference where its logits pass it by too much, and the values' power where one is larger
-      const bool rise = top > m + kRise;  // (also from -inf)
+      const bool rise = top - m > kRise;  // (also from -inf; the difference, as the sum may round)
       if (__any_sync(0xffffffffu, rise) || top_e > ref) {
         const float to = rise ? rintf(top) : m;  // (whole: what is taken off and added below is then exact)
         if (k > 0) {

@@ -87,7 +87,7 @@ struct FewShared {
   int32_t live, b, index, start, count, len, first_lo;
   alignas(16) int32_t v_exp[4][4];     // [tile & 3][run of 32 tokens]
   int32_t risen[2];                    // whether references rose in a tile
-  float4 row[kFewRows];                // factor, addend (8 - reference), threshold, reference
+  float4 row[kFewRows];                // factor, what comes off a logit (the reference, 0 before there is one), reference
   float2 more[kFewRows];               // place, slope
   int4 sight[kFewRows];
   float warp_top[4][kFewRows];
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
   }
   if (threadIdx.x < kFewRows) {  // columns that no row has: computed along, and never written
     sh.spoilt[threadIdx.x] = 0;
-    sh.row[threadIdx.x] = make_float4(0.0f, 0.0f, -kMinusInf, kMinusInf);
+    sh.row[threadIdx.x] = make_float4(0.0f, 0.0f, -kMinusInf, 0.0f);
     sh.more[threadIdx.x] = make_float2(0.0f, 0.0f);
     sh.sight[threadIdx.x] = make_int4(0, 0, 0, 0);
   }
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
       const int32_t pos = off + i;
       const Sight see = row_sight(pos, p.s.first_visible != nullptr ? __ldg(p.s.first_visible + token) : 0, prefix,
                                   p.s.window, len);
-      sh.row[c] = make_float4(fminf(kCap ? p.s.scale * back / p.s.cap : p.s.scale * kLog2e * back, 1e38f), kHead, kMinusInf, kMinusInf);
+      sh.row[c] = make_float4(fminf(kCap ? p.s.scale * back / p.s.cap : p.s.scale * kLog2e * back, 1e38f), 0.0f, kMinusInf, 0.0f);
       sh.more[c] = make_float2(__int_as_float(pos), kBias ? -__ldg(p.s.slopes + head) * kLog2e : 0.0f);
       sh.sight[c] = make_int4(see.a0, see.a1, see.b0, see.b1);
       atomicMax(&sh.all_lo, see.b0);
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
             if (!((j >= z.x && j < z.y) || (j >= z.z && j < z.w))) x[i] = kMinusInf;
           }
           y[c] = x[i];
-          rise |= x[i] > sh.row[c].z;
+          rise |= x[i] - sh.row[c].z > kRise;  // (the difference: the sum may round)
         }
       }
       if (group_or<1>(rise || !ok)) {
@@ -426,9 +426,9 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
           const float4 f = sh.row[tid];
           const float t =
               fmaxf(fmaxf(sh.warp_top[0][tid], sh.warp_top[1][tid]), fmaxf(sh.warp_top[2][tid], sh.warp_top[3][tid]));
-          const float m = t > f.z ? rintf(t) : f.w;  // (whole, so that 8 - m is exact)
-          sh.fall[k & 1][tid] = m == f.w ? 1.0f : ex2(f.w - m);
-          sh.row[tid] = make_float4(f.x, kHead - (m == kMinusInf ? 0.0f : m), m == kMinusInf ? kMinusInf : m + kRise, m);
+          const float m = t - f.z > kRise ? rintf(t) : f.z;
+          sh.fall[k & 1][tid] = m == f.z ? 1.0f : ex2(f.z - m);
+          sh.row[tid] = make_float4(f.x, m == kMinusInf ? 0.0f : m, m, 0.0f);
         }
         if (tid == 0) sh.risen[k & 1] = 1;
         group_sync<1>();
@@ -445,12 +445,13 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
       ok = wait_all(&sh.v_ready, k & 1, p.s.err) && ok;                  // (for the values' powers)
       const int4 ves = *reinterpret_cast<const int4*>(sh.v_exp[k & 3]);
       const int top_e = max(max(ves.x, ves.y), max(ves.z, ves.w)), own_e = sh.v_exp[k & 3][warp];
-      const float lift = static_cast<float>(own_e - top_e), unlift = pow2i(top_e - own_e - 8);
+      // (8 is added to the power, not to the reference: 8 - reference need not be an fp32 number)
+      const float lift = kHead + static_cast<float>(own_e - top_e), unlift = pow2i(top_e - own_e - 8);
       const uint32_t p_at = p_tile + (tid >> 6) * (kN * 128) + (tid & 7) * 2, p_chunk = (tid & 63) >> 3;
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
         if (c % kStep == 0 && c >= cols) break;
-        const float e = ex2(y[c] + sh.row[c].y + lift);
+        const float e = ex2((y[c] - sh.row[c].y) + lift);
         l[c] = fmaf(e, unlift, l[c]);
         asm volatile("st.shared.u16 [%0], %1;" ::"r"(p_at + c * 128 + ((p_chunk ^ (c & 7)) << 4)),
                      "h"(__half_as_ushort(__float2half_rn(e)))
@@ -561,7 +562,7 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
     for (int c = 0; c < kCols; ++c) {
       if (c >= cols) break;
       const float sum = (sh.total[0][c] + sh.total[1][c]) + (sh.total[2][c] + sh.total[3][c]);
-      const float m = sh.row[c].w;
+      const float m = sh.row[c].z;
       const float lse = sum == 0.0f ? kMinusInf : (m == kMinusInf ? 0.0f : m) + lg2(sum);
       float v = sum == 0.0f ? 0.0f : o[c] / sum;
       if ((sh.spoilt[c] >> (dim / 32)) & 1u) v = __int_as_float(0x7fffffff);
