@@ -25,9 +25,15 @@
 // costs 256 of its cycles and a second tile's store, and with 128 dims the second
 // key buffer.)  Each run of 32 tokens is first scaled by a power of two that
 // brings its largest scale into [2^12, 2^13), so that neither large scales
-// overflow nor small ones lose bits; the power goes into the logit's factor (keys)
-// and the probability's exponent (values).  Probabilities are fp16 with the row's
-// reference at 2^8.  Logits, statistics and sums are fp32.
+// overflow nor small ones lose bits (keys stay exact down to 2^-26 of the run's
+// largest scale); the power goes into the logit's factor (keys) and the
+// probability's exponent (values).  Runs whose tokens' values lie further apart
+// than 2^8 give each token a power of its own.  Probabilities are fp16 relative to
+// the largest that a token adds to the row, its probability times its values'
+// power, at 2^8: values that the row does not see, or that weigh nothing, cost the
+// others no bits (relative to the largest probability and the largest value they
+// did, all of them from 2^25 on; 2x4096 prompt 422 us then, 431 now).  Logits,
+// statistics and sums are fp32.
 #include "varlen_few.cuh"
 
 namespace iris {
@@ -56,8 +62,9 @@ struct Shared {
   uint64_t s_full[2], p_full[2], o_full[2], drain;
   uint32_t tmem;
   alignas(16) int32_t k_exp[4][4], v_exp[4][4];  // [tile & 3][run of 32 tokens]
-  uint32_t v_any[2][4];              // a run has values that are not finite
+  alignas(8) uint32_t v_any[2][4];   // 1: a run has values that are not finite; 2: its tokens have powers of their own
   uint8_t v_bad[2][kTile];           // which groups of a token's
+  float v_own[2][kTile];             // a token's own power
   float top[2][2][2][kTile];         // [tile & 1][row tile][half]: a row's largest logit; at the end its sum
   float back[2][kTile];              // undoes the query row's power of two
   uint32_t spoilt[2][kTile];         // groups of dims with a visible value that is not finite
@@ -65,6 +72,9 @@ struct Shared {
   int32_t b, index, start, count, len, first_lo;
   int32_t live;
 };
+
+// Tokens of a run share a power where their largest scales lie this many powers of two apart or less.
+constexpr int kSpread = 8;
 
 // ------------------------------------------------------------------ unpacking
 // One tile of keys or values, with its scales.  False: a wait gave up.
@@ -83,7 +93,14 @@ IRIS_DEV bool unpack_tile(const AttendParams& p, Shared& sh, int k, const uint32
     const uint32_t mag = (sc[c / 2] >> (16 * (c & 1))) & 0x7fffu;
     if (mag >= 0x7c00u) bad |= 1u << c; else most = max(most, mag);
   }
-  const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 10);
+  int e = static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 10);
+  const int run_e = e;
+  bool wide = false;
+  if (!keys) {
+    const int own = static_cast<int>(most >> 10);
+    wide = run_e - static_cast<int>(__reduce_min_sync(0xffffffffu, most != 0 ? own : 31)) > kSpread;
+    if (wide) e = own;
+  }
   const float up = pow2i(27 - e);
   if (!wait_all(&sh.raw_full[slot], keys ? (k >> 1) & 1 : k & 1, p.s.err)) return false;
   if (!wait_all(keys ? &sh.k_empty[st] : &sh.v_empty[st], round ^ 1, p.s.err)) return false;
@@ -92,9 +109,10 @@ IRIS_DEV bool unpack_tile(const AttendParams& p, Shared& sh, int k, const uint32
   } else {
     const bool any = __any_sync(0xffffffffu, bad != 0);
     if (lane == 0) {
-      sh.v_exp[k & 3][warp] = e - 27;
-      sh.v_any[st][warp] = any;
+      sh.v_exp[k & 3][warp] = run_e - 27;
+      sh.v_any[st][warp] = static_cast<uint32_t>(any) | (wide ? 2u : 0u);
     }
+    if (wide) sh.v_own[st][tid] = static_cast<float>(e - 27);
     if (any) sh.v_bad[st][tid] = static_cast<uint8_t>(bad);
   }
   const uint32_t src = packed + slot * C::kPacked, dst = operands + st * (keys ? 2 : 1) * C::kOperand;
@@ -315,8 +333,9 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
   const float cap2 = p.s.cap * kLog2e;
   const float slope2 = kBias ? -__ldg(p.s.slopes + head) * kLog2e : 0.0f;
   auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + tile * 4 + quarter) : "memory"); };  // the rows' two warps
-  float m = kMinusInf, l = 0.0f;
-  int ref = -127;
+  // Probabilities stand relative to 2^(m + ref): what a token adds to the row, 2^(logit + its values' power), is near or
+  // below that.  m is 0 unless the logits lie far out, where whole numbers as small as ref have no room beside them.
+  float m = 0.0f, ref = kMinusInf, l = 0.0f;
   bool ok = true;
 #pragma unroll 1
   for (int k = 0; k < n; ++k) {
@@ -328,12 +347,23 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
       const int32_t base = tiles.at(k0 + k) * kTile + half * 64;
       const int4 ve = *reinterpret_cast<const int4*>(sh.v_exp[k & 3]);
       const int2 ke = *reinterpret_cast<const int2*>(sh.k_exp[k & 3] + 2 * half);
-      const int top_e = max(max(ref, max(ve.x, ve.y)), max(ve.z, ve.w));
       const float f[2] = {fmaxf(unit * pow2i(ke.x), 1.17549435e-38f), fmaxf(unit * pow2i(ke.y), 1.17549435e-38f)};
       const int ves[2] = {half ? ve.z : ve.x, half ? ve.w : ve.y};
+      const uint2 any2 = *reinterpret_cast<const uint2*>(&sh.v_any[k & 1][2 * half]);
+      const uint32_t any[2] = {any2.x, any2.y};
       const bool full = !valid || (sight.b0 <= base && base + 64 <= sight.b1) || (sight.a0 <= base && base + 64 <= sight.a1);
       const bool masked = !__all_sync(0xffffffffu, full);
-      // ---- the largest logit; with a mask, a cap or a bias the logits go back as they now are
+      // the largest that a token of run c adds, from the logits in tensor memory as they now are
+      auto largest = [&](int c) {
+        float s[32], t = kMinusInf;
+        load_scores(s_at + 32 * c, s);
+        const float* own = sh.v_own[k & 1] + 64 * half + 32 * c;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          t = fmaxf(t, ((kMod ? s[j] : __fmul_rn(s[j], f[c])) - m) + (any[c] & 2 ? own[j] : static_cast<float>(ves[c])));
+        return t;
+      };
+      // ---- the largest that a token adds; with a mask, a cap or a bias the logits go back as they now are
       float top = kMinusInf;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -378,18 +408,38 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
           t1 = fmaxf(t1, s[j + 1]);
         }
         t0 = fmaxf(t0, t1);
-        top = fmaxf(top, kMod ? t0 : t0 * f[c]);
+        if (!(any[c] & 2)) top = fmaxf(top, ((kMod ? t0 : __fmul_rn(t0, f[c])) - m) + static_cast<float>(ves[c]));
       }
-      sh.top[k & 1][tile][half][local] = top;
       if (kMod || masked) umma_wait_st();
-      meet();
-      top = fmaxf(top, sh.top[k & 1][tile][half ^ 1][local]);
-      // raise the row's reference where its logits pass it by too much, and the values' power where one is larger
-      const bool rise = top - m > kRise;  // (also from -inf; the difference, as the sum may round)
-      if (__any_sync(0xffffffffu, rise) || top_e > ref) {
-        const float to = rise ? rintf(top) : m;  // (whole: what is taken off and added below is then exact)
+      if ((any[0] | any[1]) & 2) {
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c)
+          if (any[c] & 2) top = fmaxf(top, largest(c));
+      }
+      auto share = [&] {  // the larger of the two halves' (uniform over a row's two warps from there on)
+        sh.top[k & 1][tile][half][local] = top;
+        meet();
+        top = fmaxf(top, sh.top[k & 1][tile][half ^ 1][local]);
+      };
+      share();
+      // raise the row's reference where something passes it by too much
+      const bool rise = top > ref + kRise;  // (also from -inf)
+      if (__any_sync(0xffffffffu, rise)) {
+        const float m_old = m, ref_old = ref;
+        bool out = rise && fabsf(top) >= kFarOut;
+#pragma unroll 1
+        for (int look = 0; look < 3 && __any_sync(0xffffffffu, out); ++look) {  // m about there, and a look at the rest
+          if (out) m += rintf(top);
+          const float before = top;
+          top = fmaxf(largest(0), largest(1));
+          meet();  // what was shared is read
+          share();
+          if (!out) top = before;
+          out = out && fabsf(top) >= kFarOut;
+        }
+        if (rise) ref = rintf(top);
+        const float by = rise ? ex2((m_old - m) + (ref_old - ref)) : 1.0f;
         if (k > 0) {
-          const float by = (rise ? ex2(m - to) : 1.0f) * pow2i(max(ref - top_e, -126));
           ok = ok && wait_all(&sh.o_full[tile], (k - 1) & 1, p.s.err);
           umma_fence_after();
 #pragma unroll 1
@@ -400,27 +450,31 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
             for (int j = 0; j < 32; ++j) o[j] *= by;
             umma_st32(o_at + 32 * c, reinterpret_cast<const uint32_t*>(o));
           }
-          if (rise) l *= ex2(m - to);
+          l *= by;
         }
-        m = to;
-        ref = top_e;
       }
-      const float zero = m == kMinusInf ? 0.0f : -m;  // (a row that sees nothing yet)
-      // From 2^24 on a product that is not rounded may pass the reference by more than fp16 holds, and the addend has no
-      // room for the power beside it: there the reference comes off first, from rounded products.
-      const bool far = __any_sync(0xffffffffu, fabsf(zero) > 8388608.0f);
+      const float off = ref == kMinusInf ? 0.0f : ref;  // (a row that sees nothing yet)
+      const bool far = __any_sync(0xffffffffu, m != 0.0f);
       // ---- probabilities and their sum
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float s[32];
         load_scores(s_at + 32 * c, s);
-        float add = kHead + static_cast<float>(ves[c] - ref), by = f[c];
-        if (far) {
+        float add = kHead + static_cast<float>(ves[c]) - off, by = f[c], unlift = pow2i(-ves[c] - 8);
+        if (far || (any[c] & 2)) {  // (m comes off rounded products: one that is not rounded would be another logit)
 #pragma unroll
-          for (int j = 0; j < 32; ++j) s[j] = (kMod ? s[j] : __fmul_rn(s[j], by)) + zero;
+          for (int j = 0; j < 32; ++j) s[j] = (kMod ? s[j] : __fmul_rn(s[j], by)) - m;
           by = 1.0f;
-        } else {
-          add += zero;
+        }
+        if (any[c] & 2) {  // tokens with powers of their own
+          const float* own = sh.v_own[k & 1] + 64 * half + 32 * c;
+          add = kHead - off;
+          unlift = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            l += ex2(s[j] - off);
+            s[j] += own[j];
+          }
         }
         float2 sum = make_float2(0.0f, 0.0f);
         uint32_t w[16];
@@ -433,13 +487,13 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
           sum = __fadd2_rn(sum, y);
           w[j] = Fp16Elem::pack(y.x, y.y);
         }
-        l = fmaf(sum.x + sum.y, pow2i(min(ref - ves[c], 126)) * (1.0f / 256.0f), l);
+        l = fmaf(sum.x + sum.y, unlift, l);
         umma_st16(s_at + 16 * c, w);  // over this thread's own scores, which are read
       }
-      if (sh.v_any[k & 1][2 * half] | sh.v_any[k & 1][2 * half + 1]) {
+      if ((any[0] | any[1]) & 1) {
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
-          if (!sh.v_any[k & 1][2 * half + c]) continue;
+          if (!(any[c] & 1)) continue;
           uint32_t hit = 0;
           for (uint32_t left = valid ? sight_bits(sight, base + 32 * c) : 0u; left != 0; left &= left - 1)
             hit |= sh.v_bad[k & 1][64 * half + 32 * c + __ffs(left) - 1];
@@ -464,7 +518,7 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
   const uint32_t spoilt = sh.spoilt[tile][local];
   const bool whole = p.splits == 1;
   const int64_t row = static_cast<int64_t>(token) * p.s.hq + head;
-  const float norm = l == 0.0f ? 0.0f : pow2i(max(ref, -126)) * (1.0f / 256.0f) / l;
+  const float norm = l == 0.0f ? 0.0f : (1.0f / 256.0f) / l;
 #pragma unroll 1
   for (int c = 0; c < D / 64; ++c) {
     const int group = half * (D / 64) + c;  // of 32 dims
@@ -496,7 +550,7 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
     }
   }
   if (!valid || half != 0) return;
-  const float lse = l == 0.0f ? kMinusInf : (m == kMinusInf ? 0.0f : m) + lg2(l);
+  const float lse = l == 0.0f ? kMinusInf : m + (ref + lg2(l));
   if (!whole)
     p.part_lse[static_cast<int64_t>(split) * p.s.tokens * p.s.hq + row] = lse;
   else if (p.out_lse != nullptr)

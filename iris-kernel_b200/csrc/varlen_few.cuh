@@ -9,7 +9,10 @@
 // A thread has a token's logits in registers, then a dim's outputs; sums over
 // tokens of the probabilities stay in the thread until the end.  Keys go in as
 // whole numbers with an accumulator a group of 32 dims, and a token's fp32 scales
-// join the sums: no product by the scale, and nothing is rounded.  A product of so
+// join the sums: no product by the scale, and nothing is rounded.  Values are fp16,
+// each token's scaled by a power of two of its own; probabilities are fp16 too,
+// relative to the largest probability times power of the row, so values that it
+// does not see, or that weigh nothing, cost the others no bits.  A product of so
 // few columns takes its latency, about 140 cycles, when it adds to the one before
 // it; dealt out over several accumulators (the groups; four for the outputs, that
 // are added up as they are read) they follow each other without it.
@@ -50,6 +53,7 @@ struct AttendParams {
 
 constexpr float kRise = 7.0f;  // log2 that a row's logits may pass its reference by
 constexpr float kHead = 8.0f;  // log2 of the reference's own probability
+constexpr float kFarOut = 4194304.0f;  // 2^22: from there on a reference is two numbers
 #define kMinusInf (-__int_as_float(0x7f800000))
 
 // Rows that the offsets leave over: zeros.
@@ -83,15 +87,17 @@ struct FewShared {
   uint64_t s_done, o_done;             // products are done
   uint64_t k_ready, p_ready, v_ready;  // operands are in their places
   uint64_t o_free;                     // outputs are read
+  uint64_t e_ready;                    // the values' powers are in their place
   uint32_t tmem;
   int32_t live, b, index, start, count, len, first_lo;
-  alignas(16) int32_t v_exp[4][4];     // [tile & 3][run of 32 tokens]
+  int32_t v_exp[kTile];                // what a token's values were scaled down by, log2
   int32_t risen[2];                    // whether references rose in a tile
-  float4 row[kFewRows];                // factor, what comes off a logit (the reference, 0 before there is one), reference
+  float4 row[kFewRows];                // factor, m, the limit r + 15 (-inf before there is a reference), r
   float2 more[kFewRows];               // place, slope
   int4 sight[kFewRows];
   float warp_top[4][kFewRows];
   float fall[2][kFewRows];             // what a rise of the reference multiplies sums by
+  float by[kFewRows];                  // ... and takes off logits that m was taken off
   float total[4][kFewRows];
   uint32_t spoilt[kFewRows];
   int32_t all_lo, all_hi;
@@ -128,6 +134,7 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
     mbar_init(&sh.p_ready, 128);
     mbar_init(&sh.v_ready, 128);
     mbar_init(&sh.o_free, 128);
+    mbar_init(&sh.e_ready, 128);
     fence_barrier_init();
     sh.all_lo = 0;
     sh.all_hi = INT32_MAX;
@@ -368,11 +375,10 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
       }
       const bool full = all_lo <= base_j && base_j + kTile <= all_hi;
 
-      // ---- logits in log2 units, -inf where a token is not seen
+      // ---- logits in log2 units less m, -inf where a token is not seen
       ok = wait_all(&sh.s_done, k & 1, p.s.err) && ok;
       umma_fence_after();
       float y[kCols];
-      bool rise = false;
 #pragma unroll
       for (int c0 = 0; c0 < kCols; c0 += kStep) {
         if (c0 >= cols) break;
@@ -403,55 +409,79 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
             const int4 z = sh.sight[c];
             if (!((j >= z.x && j < z.y) || (j >= z.z && j < z.w))) x[i] = kMinusInf;
           }
-          y[c] = x[i];
-          rise |= x[i] - sh.row[c].z > kRise;  // (the difference: the sum may round)
+          y[c] = x[i] - sh.row[c].y;
         }
       }
+      // ---- what a token adds to a row has the size 2^(y + ve)
+      ok = wait_all(&sh.e_ready, k & 1, p.s.err) && ok;
+      const int ve = sh.v_exp[tid];
+      const float lift = kHead + static_cast<float>(ve), unlift = pow2i(-ve - 8);
+      bool rise = false;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        if (c % kStep == 0 && c >= cols) break;
+        rise |= y[c] + lift > sh.row[c].z;
+      }
+      bool risen = false;
       if (group_or<1>(rise || !ok)) {
-        if (group_or<1>(!ok)) {
-          ok = false;
-          break;
-        }
-        // a logit passes its row's reference by too much: the largest one of the tile is the new reference
+        // something passes its row's reference by too much: the largest of the tile is the new one.  Where it is far out,
+        // m becomes about that, and the rest is looked at again (twice at most, as 2^(y + ve) is then near 1).
+        bool again = false;
+        float m_old = 0.0f, r_old = 0.0f;
+        risen = true;
+#pragma unroll 1
+        for (int look = 0; ; ++look) {
+          if (group_or<1>(!ok)) {
+            ok = false;
+            break;
+          }
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          if (c >= cols) break;
-          float t = y[c];
+          for (int c = 0; c < kCols; ++c) {
+            if (c >= cols) break;
+            float t = y[c] + static_cast<float>(ve);
 #pragma unroll
-          for (int x = 16; x > 0; x >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
-          if (lane == 0) sh.warp_top[warp][c] = t;
+            for (int x = 16; x > 0; x >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+            if (lane == 0) sh.warp_top[warp][c] = t;
+          }
+          group_sync<1>();
+          if (tid < cols) {
+            const float4 f = sh.row[tid];
+            const float t =
+                fmaxf(fmaxf(sh.warp_top[0][tid], sh.warp_top[1][tid]), fmaxf(sh.warp_top[2][tid], sh.warp_top[3][tid]));
+            if (look == 0) {
+              m_old = f.y;
+              r_old = f.z == kMinusInf ? kMinusInf : f.w;
+            }
+            const bool go = look == 0 ? t + kHead > f.z : again;
+            again = go && fabsf(t) >= kFarOut && look < 3;
+            const float by = again ? rintf(t) : 0.0f, r = go && !again ? rintf(t) : f.w, m = f.y + by;
+            sh.by[tid] = by;
+            sh.fall[k & 1][tid] = go ? ex2((m_old - m) + (r_old - r)) : look == 0 ? 1.0f : sh.fall[k & 1][tid];
+            sh.row[tid] = make_float4(f.x, m, go && !again ? r + (kHead + kRise) : f.z, r);
+          }
+          group_sync<1>();
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) {
+            if (c >= cols) break;
+            y[c] -= sh.by[c];
+          }
+          if (!group_or<1>(again)) break;
         }
-        group_sync<1>();
-        if (tid < cols) {
-          const float4 f = sh.row[tid];
-          const float t =
-              fmaxf(fmaxf(sh.warp_top[0][tid], sh.warp_top[1][tid]), fmaxf(sh.warp_top[2][tid], sh.warp_top[3][tid]));
-          const float m = t - f.z > kRise ? rintf(t) : f.z;
-          sh.fall[k & 1][tid] = m == f.z ? 1.0f : ex2(f.z - m);
-          sh.row[tid] = make_float4(f.x, m == kMinusInf ? 0.0f : m, m, 0.0f);
-        }
-        if (tid == 0) sh.risen[k & 1] = 1;
-        group_sync<1>();
+        if (!ok) break;
 #pragma unroll
         for (int c = 0; c < kCols; ++c) {
           if (c >= cols) break;
           l[c] *= sh.fall[k & 1][c];
         }
-      } else if (tid == 0) {
-        sh.risen[k & 1] = 0;
       }
+      if (tid == 0) sh.risen[k & 1] = risen;
       // ---- probabilities: fp16, K-major [row][token], and their sums
       if (k > 0) ok = wait_all(&sh.o_done, (k - 1) & 1, p.s.err) && ok;  // the product before has read its own
-      ok = wait_all(&sh.v_ready, k & 1, p.s.err) && ok;                  // (for the values' powers)
-      const int4 ves = *reinterpret_cast<const int4*>(sh.v_exp[k & 3]);
-      const int top_e = max(max(ves.x, ves.y), max(ves.z, ves.w)), own_e = sh.v_exp[k & 3][warp];
-      // (8 is added to the power, not to the reference: 8 - reference need not be an fp32 number)
-      const float lift = kHead + static_cast<float>(own_e - top_e), unlift = pow2i(top_e - own_e - 8);
       const uint32_t p_at = p_tile + (tid >> 6) * (kN * 128) + (tid & 7) * 2, p_chunk = (tid & 63) >> 3;
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
         if (c % kStep == 0 && c >= cols) break;
-        const float e = ex2((y[c] - sh.row[c].y) + lift);
+        const float e = ex2(y[c] + (lift - sh.row[c].w));
         l[c] = fmaf(e, unlift, l[c]);
         asm volatile("st.shared.u16 [%0], %1;" ::"r"(p_at + c * 128 + ((p_chunk ^ (c & 7)) << 4)),
                      "h"(__half_as_ushort(__float2half_rn(e)))
@@ -491,8 +521,6 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
             o[c] *= sh.fall[(k - 1) & 1][c];
           }
         }
-        const int4 ves = *reinterpret_cast<const int4*>(sh.v_exp[(k - 1) & 3]);
-        const float down = pow2i(max(max(ves.x, ves.y), max(ves.z, ves.w)) - 8);
 #pragma unroll
         for (int c0 = 0; c0 < kCols; c0 += kStep) {
           if (c0 >= cols) break;
@@ -508,23 +536,24 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
               asm volatile("" : "+r"(v[g][i]));
               t += __uint_as_float(v[g][i]);
             }
-            o[c0 + i] = fmaf(t, down, o[c0 + i]);
+            o[c0 + i] += t;
           }
         }
         umma_fence_before();
         mbar_arrive(&sh.o_free);
         if (k == n) break;
       }
-      // a power of two for each run of 32 tokens
+      // a power of two for each token (the powers before have been read: the product that they went into is done)
       uint32_t bad = 0, most = 0;
 #pragma unroll
       for (int c = 0; c < kGroups; ++c) {
         const uint32_t mag = scale_bits(c) & 0x7fffu;
         if (mag >= 0x7c00u) bad |= 1u << c; else most = max(most, mag);
       }
-      const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 10);
+      const int e = static_cast<int>(most >> 10);
       const float up = pow2i(27 - e);
-      if (lane == 0) sh.v_exp[k & 3][warp] = e - 27;
+      sh.v_exp[tid] = e - 27;
+      mbar_arrive(&sh.e_ready);
       if (bad != 0) {
         const int32_t j = first_token(k) + tid;
         for (int c = 0; c < cols; ++c) {
@@ -562,9 +591,8 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
     for (int c = 0; c < kCols; ++c) {
       if (c >= cols) break;
       const float sum = (sh.total[0][c] + sh.total[1][c]) + (sh.total[2][c] + sh.total[3][c]);
-      const float m = sh.row[c].z;
-      const float lse = sum == 0.0f ? kMinusInf : (m == kMinusInf ? 0.0f : m) + lg2(sum);
-      float v = sum == 0.0f ? 0.0f : o[c] / sum;
+      const float lse = sum == 0.0f ? kMinusInf : sh.row[c].y + (sh.row[c].w + lg2(sum));
+      float v = sum == 0.0f ? 0.0f : o[c] * (1.0f / 256.0f) / sum;
       if ((sh.spoilt[c] >> (dim / 32)) & 1u) v = __int_as_float(0x7fffffff);
       const int64_t row = row_at(c);
       if (whole) {

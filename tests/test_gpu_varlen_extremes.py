@@ -66,3 +66,84 @@ def test_logits_that_tower(new, lens, hq, offsets, exponent, extra):
     close(out, want, np.broadcast_to(far, want.shape))
     want_lse = base + max(extra, 0) + np.log2(1 + 2.0 ** -abs(extra))
     close(lse, want_lse, np.abs(want_lse) * 2.0 ** -22)
+
+
+# ---- values of very different sizes
+def _alike(c, got, rows, quiet):
+    """`rows` have what they would have if the tokens `quiet` had no value: those are not seen, or weigh nothing."""
+    out, lse = got
+    for b, j in quiet:
+        c.cache[3][c.bt[b, j // 16], j % 16] = 0
+    want, want_lse, far, far_lse = c.want()
+    close(out[rows], want[rows], far[rows])
+    close(lse[rows], want_lse[rows], far_lse[rows])
+
+
+def _sized(c, b, tokens, lo, hi):
+    """Values of a few sizes in [lo, hi]."""
+    for j in tokens:
+        c.cache[3][c.bt[b, j // 16], j % 16] = np.exp(c.rng.uniform(np.log(lo), np.log(hi), c.cache[3].shape[2:])).astype(np.float16)
+
+
+@pytest.mark.parametrize("small", [2.0 ** -9, 2.0 ** -19])
+@pytest.mark.parametrize("new,hq,dim,dtype", [([60], 8, 64, BF16), ([200], 4, 128, F16), ([3], 8, 128, BF16), ([1], 4, 64, F16)])
+def test_unseen_values_do_not_matter(new, hq, dim, dtype, small):
+    """Large values that a window has left behind, in the same page as what is seen and before it."""
+    n = 260
+    c = Case(new, [n], hq, 2, dim, dtype, seed=41, window=50)
+    edge = n - new[0] - 49  # the first token that any row sees
+    _sized(c, 0, range(edge), 9000.0, 60000.0)
+    _sized(c, 0, range(edge, n), small / 8, small)
+    _alike(c, c.run(), slice(None), [(0, j) for j in range(edge)])
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (128, BF16)])
+def test_documents_with_values_of_different_sizes(dim, dtype):
+    """Two documents that share tiles and runs, one with values 2^30 times the other's: each has its own bits."""
+    n, cut = 300, 150
+    first = np.where(np.arange(n) < cut, 0, cut).astype(np.int32)
+    for large in (range(cut), range(cut, n)):
+        c = Case([n], [n], 4, 2, dim, dtype, seed=42, first_visible=first)
+        rest = sorted(set(range(n)) - set(large))
+        _sized(c, 0, large, 9000.0, 60000.0)
+        _sized(c, 0, rest, 2.0 ** -20, 2.0 ** -16)
+        got = c.run()
+        _alike(c, [x.clone() for x in got], np.array(rest), [(0, j) for j in large])
+
+
+@pytest.mark.parametrize("new", [[100], [2], [1]])
+def test_large_values_that_weigh_nothing(new):
+    """A bias puts the large values' tokens 2^-60 and further down: what is left of them is below the small ones' last bit."""
+    n = 400
+    slopes = np.array([1.0, 2.0, 1.0, 0.7], np.float32)
+    c = Case(new, [n], 4, 2, 64, BF16, seed=43, slopes=slopes, sharp=0.1)
+    far = range(n - new[0] - 150)
+    _sized(c, 0, far, 9000.0, 60000.0)
+    _sized(c, 0, range(far.stop, n), 2.0 ** -19, 2.0 ** -17)
+    _alike(c, c.run(), slice(None), [(0, j) for j in far])
+
+
+@pytest.mark.parametrize("new,offsets", [([40], True), ([5], True), ([1], False)])
+def test_values_that_decide_by_their_size(new, offsets):
+    """Tokens of next to no weight with values so large that the output is theirs."""
+    n = 300
+    c = Case(new, [n], 4, 1, 64, F16, seed=44, offsets=offsets, softmax_scale=1.0)
+    query = np.zeros((new[0], 4, 64), np.float32)
+    query[..., 0] = 1.0
+    c.query = R.to_type(query, F16)
+    for j in range(n):
+        at = c.bt[0, j // 16], j % 16, 0
+        c.cache[0][at] = 0
+        light = j % 3 == 0 and j < 250
+        c.cache[0][at][0] = 0 if light else 7  # logits 0, or 17.5: 2^-25 of the weight
+        c.cache[2][at] = 2.5
+        c.cache[3][at] = np.float16(2.0 ** 14 if light else 2.0 ** -16)
+    out, lse = c.run()
+    want, want_lse, far, far_lse = c.want()
+    # (relative to the sum of what tokens contribute: probabilities and values in fp16)
+    x, _, seen = V._sequence(R.f32(c.query), c.cache, c.bt, c.lens, c.cu, 0, 0, **V._options(dict(scale=1.0)))
+    w = np.where(seen, np.exp(x - np.log(np.exp(x).sum(-1, keepdims=True))), 0.0)
+    pages = c.bt[0, np.arange(n) // 16], np.arange(n) % 16, 0
+    most = (w @ np.abs(R.dequant(c.cache[1][pages], c.cache[3][pages], np.float64))).transpose(1, 0, 2)
+    close(out, want, most * (2 * 2.0 ** -11 + 2.0 ** -15) + np.abs(want) * 2.0 ** -11 + 2.0 ** -25)
+    close(lse, want_lse, far_lse)
