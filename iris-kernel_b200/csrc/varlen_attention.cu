@@ -713,8 +713,8 @@ bool too_long(int64_t tokens, int32_t group, int32_t max_pages) {
 // Sequences of at most kFewRows rows go to varlen_few_kernel, the others to
 // varlen_attention_kernel.  With one new token a sequence the host knows which;
 // with offsets both are launched unless all rows together are few (an empty
-// launch costs about 2 us beside the other; one kernel for both would give single
-// tokens 128-row products, 837 us where the other takes a tenth of it at 64 x 4096).
+// launch costs 2 to 5 us; one kernel for both would give single tokens 128-row
+// products, 837 us where the other takes a sixth of it at 64 x 4096).
 struct Plan {
   bool few, many;
   int tiles;               // row tiles of a block (many)

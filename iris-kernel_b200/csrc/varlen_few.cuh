@@ -145,9 +145,7 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
     sh.more[threadIdx.x] = make_float2(0.0f, 0.0f);
     sh.sight[threadIdx.x] = make_int4(0, 0, 0, 0);
   }
-  // behind the kernel of the sequences with many rows nothing needs a wait: that kernel let this one come up after its
-  // own wait, and their rows are apart
-  if (!p.many) grid_dependency_wait();
+  grid_dependency_wait();
   grid_dependents_launch();
   if (threadIdx.x < 32) {
     if (blockIdx.x == 0) check_offsets(p.s, lane);
@@ -173,10 +171,7 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
   }
   if (!p.many) clear_unused<D>(p);
   __syncthreads();
-  if (!sh.live) {
-    if (p.many) grid_dependency_wait();  // what waits for this kernel waits for both
-    return;
-  }
+  if (!sh.live) return;
   const int b = sh.b, len = sh.len, group = p.s.group;
   const int rows_all = sh.count * group, r0 = sh.index * kCols, cols = min(kCols, rows_all - r0);
   const int32_t off = len - sh.count;
@@ -200,7 +195,6 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
         if (tid == 0 && p.out_lse != nullptr) p.out_lse[row_at(c)] = kMinusInf;
       }
     }
-    if (p.many) grid_dependency_wait();
     return;
   }
 
@@ -606,7 +600,6 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
       }
     }
   }
-  if (p.many) grid_dependency_wait();
 }
 
 // Joins the parts of a row: `parts` of them, `stride` rows apart.  One warp.
