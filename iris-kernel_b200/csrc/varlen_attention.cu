@@ -25,8 +25,9 @@
 // costs 256 of its cycles and a second tile's store, and with 128 dims the second
 // key buffer.)  Each run of 32 tokens is first scaled by a power of two that
 // brings its largest scale into [2^12, 2^13), so that neither large scales
-// overflow nor small ones lose bits (keys stay exact down to 2^-26 of the run's
-// largest scale); the power goes into the logit's factor (keys) and the
+// overflow nor small ones lose bits, a key's into [2^11, 2^12), as its upper 8 bits
+// may round up and -8 times 2^13 is past fp16 (keys stay exact down to 2^-25 of the
+// run's largest scale); the power goes into the logit's factor (keys) and the
 // probability's exponent (values).  Runs whose tokens' values lie further apart
 // than 2^8 give each token a power of its own.  Probabilities are fp16 relative to
 // the largest that a token adds to the row, its probability times its values'
@@ -101,18 +102,19 @@ IRIS_DEV bool unpack_tile(const AttendParams& p, Shared& sh, int k, const uint32
     wide = run_e - static_cast<int>(__reduce_min_sync(0xffffffffu, most != 0 ? own : 31)) > kSpread;
     if (wide) e = own;
   }
-  const float up = pow2i(27 - e);
+  constexpr int kUp = keys ? 26 : 27;
+  const float up = pow2i(kUp - e);
   if (!wait_all(&sh.raw_full[slot], keys ? (k >> 1) & 1 : k & 1, p.s.err)) return false;
   if (!wait_all(keys ? &sh.k_empty[st] : &sh.v_empty[st], round ^ 1, p.s.err)) return false;
   if (keys) {
-    if (lane == 0) sh.k_exp[k & 3][warp] = e - 27;
+    if (lane == 0) sh.k_exp[k & 3][warp] = e - kUp;
   } else {
     const bool any = __any_sync(0xffffffffu, bad != 0);
     if (lane == 0) {
-      sh.v_exp[k & 3][warp] = run_e - 27;
+      sh.v_exp[k & 3][warp] = run_e - kUp;
       sh.v_any[st][warp] = static_cast<uint32_t>(any) | (wide ? 2u : 0u);
     }
-    if (wide) sh.v_own[st][tid] = static_cast<float>(e - 27);
+    if (wide) sh.v_own[st][tid] = static_cast<float>(e - kUp);
     if (any) sh.v_bad[st][tid] = static_cast<uint8_t>(bad);
   }
   const uint32_t src = packed + slot * C::kPacked, dst = operands + st * (keys ? 2 : 1) * C::kOperand;

@@ -147,3 +147,15 @@ def test_values_that_decide_by_their_size(new, offsets):
     most = (w @ np.abs(R.dequant(c.cache[1][pages], c.cache[3][pages], np.float64))).transpose(1, 0, 2)
     close(out, want, most * (2 * 2.0 ** -11 + 2.0 ** -15) + np.abs(want) * 2.0 ** -11 + 2.0 ** -25)
     close(lse, want_lse, far_lse)
+
+
+@pytest.mark.parametrize("exponent", [-10, -4, 0, 12])
+@pytest.mark.parametrize("new,lens", [([70], [400]), ([5, 1], [300, 130])])
+def test_every_nibble_and_full_mantissas(new, lens, exponent):
+    """-8, which the append does not write but the format has, times scales just below a power of two."""
+    c = Case(new, lens, 4, 2, 64, BF16, seed=45, sharp=2.0 ** -max(exponent, 0))
+    for x in c.cache[:2]:
+        x[...] = c.rng.integers(0, 256, x.shape)
+    for x in c.cache[2:]:
+        x[...] = ((2.0 - c.rng.integers(1, 9, x.shape) * 2.0 ** -10) * 2.0 ** exponent).astype(np.float16)
+    c.check()
