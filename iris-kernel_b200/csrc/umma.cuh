@@ -139,20 +139,6 @@ IRIS_DEV void regs_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :
 template <int kRegs>
 IRIS_DEV void regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 
-// ------------------------------------------------------------- per-thread copies
-// 16, 8 or 4 bytes global -> shared, zeros where !there (then nothing is read).
-template <int kBytes>
-IRIS_DEV void copy_async(uint32_t dst, const void* src, bool there) {
-  const int n = there ? kBytes : 0;
-  if constexpr (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kBytes), "r"(n) : "memory");
-}
-IRIS_DEV void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kPending>
-IRIS_DEV void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
-
 IRIS_DEV uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
