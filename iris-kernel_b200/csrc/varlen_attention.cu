@@ -428,10 +428,10 @@ IRIS_DEV void softmax_rows(const AttendParams& p, Shared& sh, const Tiles& tiles
       const bool rise = top > ref + kRise;  // (also from -inf)
       if (__any_sync(0xffffffffu, rise)) {
         const float m_old = m, ref_old = ref;
-        bool out = rise && fabsf(top) >= kFarOut;
+        bool out = rise && (m != 0.0f || fabsf(top) >= kFarOut);
 #pragma unroll 1
-        for (int look = 0; look < 3 && __any_sync(0xffffffffu, out); ++look) {  // m about there, and a look at the rest
-          if (out) m += rintf(top);
+        for (int look = 0; look < 3 && __any_sync(0xffffffffu, out); ++look) {  // m about there, or 0, and a look at the rest
+          if (out) m = fabsf(m + top) >= kFarOut ? rintf(m + top) : 0.0f;
           const float before = top;
           top = fmaxf(largest(0), largest(1));
           meet();  // what was shared is read

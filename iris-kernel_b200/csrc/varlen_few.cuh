@@ -97,7 +97,6 @@ struct FewShared {
   int4 sight[kFewRows];
   float warp_top[4][kFewRows];
   float fall[2][kFewRows];             // what a rise of the reference multiplies sums by
-  float by[kFewRows];                  // ... and takes off logits that m was taken off
   float total[4][kFewRows];
   uint32_t spoilt[kFewRows];
   int32_t all_lo, all_hi;
@@ -369,7 +368,7 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
       }
       const bool full = all_lo <= base_j && base_j + kTile <= all_hi;
 
-      // ---- logits in log2 units less m, -inf where a token is not seen
+      // ---- logits in log2 units, -inf where a token is not seen
       ok = wait_all(&sh.s_done, k & 1, p.s.err) && ok;
       umma_fence_after();
       float y[kCols];
@@ -403,7 +402,7 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
             const int4 z = sh.sight[c];
             if (!((j >= z.x && j < z.y) || (j >= z.z && j < z.w))) x[i] = kMinusInf;
           }
-          y[c] = x[i] - sh.row[c].y;
+          y[c] = x[i];
         }
       }
       // ---- what a token adds to a row has the size 2^(y + ve)
@@ -414,12 +413,12 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
         if (c % kStep == 0 && c >= cols) break;
-        rise |= y[c] + lift > sh.row[c].z;
+        rise |= (y[c] - sh.row[c].y) + lift > sh.row[c].z;
       }
       bool risen = false;
       if (group_or<1>(rise || !ok)) {
-        // something passes its row's reference by too much: the largest of the tile is the new one.  Where it is far out,
-        // m becomes about that, and the rest is looked at again (twice at most, as 2^(y + ve) is then near 1).
+        // something passes its row's reference by too much: the largest of the tile is the new one.  Where that or m is far
+        // out, m becomes about the largest (0, if that is not), and what lies above it is looked at again.
         bool again = false;
         float m_old = 0.0f, r_old = 0.0f;
         risen = true;
@@ -432,7 +431,7 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
 #pragma unroll
           for (int c = 0; c < kCols; ++c) {
             if (c >= cols) break;
-            float t = y[c] + static_cast<float>(ve);
+            float t = (y[c] - sh.row[c].y) + static_cast<float>(ve);
 #pragma unroll
             for (int x = 16; x > 0; x >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
             if (lane == 0) sh.warp_top[warp][c] = t;
@@ -447,18 +446,12 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
               r_old = f.z == kMinusInf ? kMinusInf : f.w;
             }
             const bool go = look == 0 ? t + kHead > f.z : again;
-            again = go && fabsf(t) >= kFarOut && look < 3;
-            const float by = again ? rintf(t) : 0.0f, r = go && !again ? rintf(t) : f.w, m = f.y + by;
-            sh.by[tid] = by;
+            again = go && look < 3 && (fabsf(t) >= kFarOut || (look == 0 && f.y != 0.0f));
+            const float m = again ? (fabsf(f.y + t) >= kFarOut ? rintf(f.y + t) : 0.0f) : f.y, r = go && !again ? rintf(t) : f.w;
             sh.fall[k & 1][tid] = go ? ex2((m_old - m) + (r_old - r)) : look == 0 ? 1.0f : sh.fall[k & 1][tid];
             sh.row[tid] = make_float4(f.x, m, go && !again ? r + (kHead + kRise) : f.z, r);
           }
           group_sync<1>();
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) {
-            if (c >= cols) break;
-            y[c] -= sh.by[c];
-          }
           if (!group_or<1>(again)) break;
         }
         if (!ok) break;
@@ -475,7 +468,7 @@ __global__ void __launch_bounds__(288, FewCfg<D, kCols>::kBlocks) varlen_few_ker
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
         if (c % kStep == 0 && c >= cols) break;
-        const float e = ex2(y[c] + (lift - sh.row[c].w));
+        const float e = ex2((y[c] - sh.row[c].y) + (lift - sh.row[c].w));
         l[c] = fmaf(e, unlift, l[c]);
         asm volatile("st.shared.u16 [%0], %1;" ::"r"(p_at + c * 128 + ((p_chunk ^ (c & 7)) << 4)),
                      "h"(__half_as_ushort(__float2half_rn(e)))

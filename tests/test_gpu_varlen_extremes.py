@@ -159,3 +159,29 @@ def test_every_nibble_and_full_mantissas(new, lens, exponent):
     for x in c.cache[2:]:
         x[...] = ((2.0 - c.rng.integers(1, 9, x.shape) * 2.0 ** -10) * 2.0 ** exponent).astype(np.float16)
     c.check()
+
+
+@pytest.mark.parametrize("new,lens,offsets", [([1, 1], [400, 300], False), ([5, 2], [300, 500], True), ([40], [300], True)])
+@pytest.mark.parametrize("q0", [64.0, -128.0])
+def test_logits_far_below_those_that_count(new, lens, offsets, q0):
+    """A row whose first tile lies at -2^22 to -2^24, and the rest where logits usually are: nothing is lost on the way."""
+    c = Case(new, lens, 8, 2, 64, BF16, seed=46, offsets=offsets)
+    c.query[..., 0] = -abs(q0)
+    for b in range(len(lens)):
+        at = c.bt[b, np.arange(lens[b]) // 16], np.arange(lens[b]) % 16
+        c.cache[0][at[0], at[1], :, 0] &= 0xf0  # dim 0: nothing ...
+        for j in range(128):                   # ... but in the first tile
+            c.cache[0][c.bt[b, j // 16], j % 16, :, 0] |= 7
+            c.cache[2][c.bt[b, j // 16], j % 16, :, 0] = 62000.0 if q0 < 0 else 65504.0
+    out, lse = c.run()
+    c.how["first_visible"] = np.full(c.query.shape[0], 128, np.int32)
+    want, want_lse, far, far_lse = c.want()
+    close(out, want, far)
+    close(lse, want_lse, far_lse)
+
+
+def test_a_bias_that_falls_to_far_below():
+    """The nearest token decides, and its logit is the log-sum-exp to the last bits."""
+    for new, lens, offsets in (([1], [400], False), ([3], [300], True), ([60], [300], True)):
+        slopes = np.array([2e4, 5e4, 1e5, 3e4], np.float32)
+        Case(new, lens, 4, 2, 64, BF16, seed=47, offsets=offsets, slopes=slopes).check()
