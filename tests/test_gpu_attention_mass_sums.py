@@ -1,10 +1,11 @@
 """Attention and its accumulated weights beside each other."""
 import numpy as np
 import pytest
+import torch
 
 import _varlen_refs as V
 from test_gpu_attention_mass import _run
-from test_gpu_varlen_attention import BF16, F16, Case
+from test_gpu_varlen_attention import BF16, F16, Case, close
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +27,13 @@ def test_weights_of_rows_add_up_to_one_as_far_as_exact_keys_allow(new, lens, hq,
             rows = (hq // hkv) * new[b]
             total = got[pages, h, np.arange(n) % 16].sum()
             assert off < 2.0 ** -11 and abs(total / rows - 1) <= off, f"{abs(total / rows - 1):.2e} of {off:.2e}"
+
+
+@pytest.mark.parametrize("rows,hq,dim", [(190, 64, 64), (700, 64, 128), (3, 33, 64), (1000, 1, 64)])
+def test_sums_over_many_rows(rows, hq, dim):
+    """Thousands of weights of one size: what each addition to a sum of fp32 loses must not add up.  A weight is off by
+    2^-22 (the exponential), 8 of them added by 2^-21, and sums of those by 2^-22 however many they are."""
+    c = Case([rows], [rows], hq, 1, dim, F16, seed=5, sharp=0.0, prefix_lens=np.array([rows], np.int32))
+    lse = torch.full((rows, hq), float(np.log2(rows)), device="cuda")
+    got, want, _ = _run(c, np.zeros((c.cache[0].shape[0], 1, 16), np.float32), lse=lse)
+    close(got, want, want * 2.0 ** -20)
