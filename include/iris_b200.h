@@ -422,8 +422,12 @@ IRIS_API size_t iris_b200_varlen_attention_workspace_bytes(int64_t tokens, int32
  *   elements apart (a multiple of 8); output dense, may be a dense query itself;
  *   out_lse [tokens, num_q_heads] fp32 or NULL: log2-sum-exp2 of the logits.
  * A row that sees nothing: output 0, lse -inf.  Rows behind cu_seqlens[batch]:
- * the same.  A visible key scale that is not finite, or a query row that is
- * not, makes the row's outputs and lse NaN; a visible value scale the outputs of its 32 dims.
+ * the same.  Lengths of sequences without rows are not looked at, nor pages that
+ * no row sees.  Logits are fp32; one past its range makes NaN.  Keys enter the
+ * products exactly, values as fp16 of nibble * scale, probabilities as fp16
+ * relative to the largest that a token adds to the row.  A visible key scale that
+ * is not finite, or a query row that is not, makes the row's outputs and lse NaN;
+ * a visible value scale the outputs of its 32 dims.
  * page_size 16, head_dim 64 or 128.  query, k_data, v_data, output and
  * workspace 16-byte aligned, the scales 8-byte.  The workspace's contents do
  * not matter and belong to one call at a time.

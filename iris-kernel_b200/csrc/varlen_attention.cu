@@ -15,26 +15,30 @@
 // Two row tiles take turns: one's softmax runs while the other's products do.
 // A row's scores are read twice, 32 columns at a time (maximum, then
 // probabilities): all at once would not fit the registers, and what is spilled
-// here misses the few kilobytes of L1 that are left (740 us for two prompts of
-// 4096 tokens; 506 without).
+// here misses the few kilobytes of L1 that are left (740 us against 506 for two
+// prompts of 4096 tokens when that was tried).  Some spills remain, 40 to 230 bytes
+// read a thread, most of them with a cap or a bias.
 //
 // Roundings.  A stored key or value is nibble * scale: 15 bits, where fp16 has 11.
 // Values are rounded.  Keys are not, as the log-sum-exp of a row with few tokens
 // would show it (1e-4 of a logit): their scale is split into its upper 8 bits and
-// the rest, and two exact fp16 tiles follow each other in the product.  (That
-// costs 256 of its cycles and a second tile's store, and with 128 dims the second
-// key buffer.)  Each run of 32 tokens is first scaled by a power of two that
-// brings its largest scale into [2^12, 2^13), so that neither large scales
-// overflow nor small ones lose bits, a key's into [2^11, 2^12), as its upper 8 bits
-// may round up and -8 times 2^13 is past fp16 (keys stay exact down to 2^-25 of the
-// run's largest scale); the power goes into the logit's factor (keys) and the
-// probability's exponent (values).  Runs whose tokens' values lie further apart
-// than 2^8 give each token a power of its own.  Probabilities are fp16 relative to
-// the largest that a token adds to the row, its probability times its values'
-// power, at 2^8: values that the row does not see, or that weigh nothing, cost the
-// others no bits (relative to the largest probability and the largest value they
-// did, all of them from 2^25 on; 2x4096 prompt 422 us then, 431 now).  Logits,
-// statistics and sums are fp32.
+// the rest, and two exact fp16 tiles follow each other in the product.  (The
+// second one's products take 50 of the 432 us of two prompts of 4096 tokens; there
+// is a second tile's store as well, and with 128 dims no second key buffer.)
+//
+// Each run of 32 tokens is first scaled by a power of two that brings its largest
+// scale into [2^12, 2^13), so that neither large scales overflow nor small ones
+// lose bits; a key's into [2^11, 2^12), as its upper 8 bits may round up and -8
+// times 2^13 is past fp16 (keys stay exact down to 2^-25 of the run's largest
+// scale).  Runs whose tokens' values lie further apart than 2^8 give each token a
+// power of its own.  The power goes into the logit's factor (keys) and the
+// probability's exponent (values).
+//
+// Probabilities are fp16, at 2^8 for the largest that a token adds to the row, its
+// probability times its values' power.  So values that the row does not see, or
+// that weigh nothing, cost the others no bits; relative to the largest probability
+// and to all tokens' largest value they cost them all from a factor of 2^25 on (two
+// prompts of 4096 tokens took 422 us then).  Logits, statistics and sums are fp32.
 #include "varlen_few.cuh"
 
 namespace iris {
@@ -751,7 +755,7 @@ Plan plan(int64_t tokens, int32_t batch, int32_t group, bool offsets, int32_t hk
     r.cols = most_rows <= 4 ? 4 : most_rows <= 8 ? 8 : most_rows <= 16 ? 16 : 32;
     r.few_blocks = offsets ? some : batch;  // (kFewRows rows are one block)
     if (offsets && r.cols < kFewRows) r.few_blocks = some;
-    // (64 x 4096 tokens: two chunks 137 us, four 154; 16 x 5 drafts over 4096: two chunks 98 us, five 122)
+    // (when they were chosen, 64 x 4096 tokens: two chunks 137 us, four 154; 16 x 5 drafts over 4096: two 98 us, five 122)
     const int64_t slots = static_cast<int64_t>(sms) * (r.cols <= 8 ? 3 : 2);
     const int64_t n = best_chunks(r.few_blocks * hkv, tiles, slots, kFewStart, (tiles + kFewTiles - 1) / kFewTiles);
     r.per = static_cast<int32_t>((all_tiles < tiles ? all_tiles : tiles) + n - 1) / static_cast<int32_t>(n);

@@ -101,6 +101,11 @@ def fused_int4_paged_attention_mass(
     ``[B]``; None: all) start from 0, as they must where their slots held other
     tokens before: None after a prompt, ``seq_lens - 1`` after a decode step.
 
+    The fast use is the last rows: up to 128 of them a KV head (32 new tokens
+    with four query heads each) are loaded once, more again for every tile of
+    128 cached tokens (all rows of a prompt of 4096 tokens take five times as
+    long as its attention).
+
     A weight is at most 1; a row whose lse is -inf gives nothing.  A page must
     belong to one sequence only; tokens behind a bad page id get no weight
     written."""
